@@ -61,6 +61,9 @@ typedef enum {
   MI355Q_QTYPE_MXFP4_OCP = 4   /* e2m1 with e8m0 group scales, OCP rule (MSE searches only) */
 } mi355q_qtype;
 
+/* Scales of block-scaled fp8 activations: fp32, or e8m0 bytes 2^(b - 127). */
+typedef enum { MI355Q_SCALE_F32 = 0, MI355Q_SCALE_E8M0 = 1 } mi355q_scale_type;
+
 /* MXFP4 shared-exponent rule (see mi355q_mxfp4_quantize_pack). */
 typedef enum { MI355Q_MX_RULE_CT = 0, MI355Q_MX_RULE_OCP = 1 } mi355q_mx_rule;
 
@@ -515,6 +518,82 @@ int mi355q_quantize_fp8(const void* x_dev, mi355q_dtype dtype, int64_t rows, int
  * / scale)), -128, 127).  scale_out is bf16 bits [rows]. */
 int mi355q_quantize_int8_per_token(const void* x_dev, int64_t rows, int64_t cols, int64_t ldx,
                                    int8_t* codes_dev, uint16_t* scale_out_dev, void* stream);
+
+/* ------------------------------------------------------------------ block-scaled fp8
+ * An fp8 matrix is e4m3fn codes with one scale per row and 128 columns
+ * (activations) or per 128 x 128 block (weights); the last group or block
+ * of a row or column may be narrower.  value = code * scale.
+ *
+ * mi355q_fp8_quantize_groups: per row and 128 columns, a = max |x|; scale =
+ * a / 448 (fp32, correctly rounded; 2^-23 where a is 0) or the least power of
+ * two not below it as an e8m0 byte (1 where a is 0, 2^-126 at the least);
+ * codes = e4m3fn(x / scale), round to nearest even.  A group holding an
+ * infinity or a NaN becomes NaN as a whole (scale NaN / byte 255, NaN codes).
+ * codes [rows, cols] (ld_codes), scales [rows, ceil(cols / 128)] (ld_scales,
+ * in scales).  rows may be 0.  fp32 scales are those of the FP8_BLOCK
+ * scheme's dynamic group-128 activations; with e8m0 scales code * scale is
+ * exact in bf16, which the weight gradient relies on. */
+int mi355q_fp8_quantize_groups(const void* x_dev, mi355q_dtype dtype, int64_t rows, int64_t cols,
+                               int64_t ldx, uint8_t* codes_dev, int64_t ld_codes, void* scales_dev,
+                               mi355q_scale_type scale_type, int64_t ld_scales, void* stream);
+
+/* The same over 128 x 128 blocks of a weight, fp32 scales
+ * [ceil(rows / 128), ceil(cols / 128)]. */
+int mi355q_fp8_quantize_blocks(const void* w_dev, mi355q_dtype dtype, int64_t rows, int64_t cols,
+                               int64_t ldw, uint8_t* codes_dev, int64_t ld_codes, float* scales_dev,
+                               int64_t ld_scales, void* stream);
+
+/* y[m][n] = bias[n] + sum over 128-column groups kb of
+ *   x_scales[m][kb] * w_scales[n / 128][kb] * sum_{k in kb} x[m][k] w[n][k]
+ * x codes [rows, cols], w codes [out, cols], y [rows, out] in y_dtype, rounded
+ * once from fp32; bias_dev may be NULL (bias_dtype then unused).  Code
+ * products are exact in fp32.  rows may be 0.  Workspace: the queried size, or
+ * NULL / 0: the sum over the columns is then not split over workgroups. */
+size_t mi355q_fp8_block_matmul_workspace_size(int64_t rows, int64_t out, int64_t cols);
+int mi355q_fp8_block_matmul(const uint8_t* x_dev, int64_t ldx, const void* x_scales_dev,
+                            mi355q_scale_type x_scale_type, int64_t ld_x_scales, const uint8_t* w_dev,
+                            int64_t ldw, const float* w_scales_dev, int64_t ld_w_scales,
+                            const void* bias_dev, mi355q_dtype bias_dtype, void* y_dev,
+                            mi355q_dtype y_dtype, int64_t ldy, int64_t rows, int64_t out, int64_t cols,
+                            void* workspace_dev, size_t workspace_bytes, void* stream);
+
+/* dx[m][k] = sum over 128-row blocks nb of w_scales[nb][k / 128] *
+ *   sum_{n in nb} dy[m][n] w[n][k]: the input gradient of the product above.
+ * dy [rows, out] and dx [rows, cols] are bf16, w the same codes and scales as
+ * in the forward product.  Workspace as above. */
+size_t mi355q_fp8_block_grad_input_workspace_size(int64_t rows, int64_t out, int64_t cols);
+int mi355q_fp8_block_grad_input(const uint16_t* dy_dev, int64_t lddy, const uint8_t* w_dev, int64_t ldw,
+                                const float* w_scales_dev, int64_t ld_w_scales, uint16_t* dx_dev,
+                                int64_t lddx, int64_t rows, int64_t out, int64_t cols, void* workspace_dev,
+                                size_t workspace_bytes, void* stream);
+
+/* dw[n][k] = sum_m dy[m][n] * x[m][k] * 2^(x_scales[m][k / 128] - 127): the
+ * weight gradient of the product from the 8-bit checkpoint of its input
+ * (mi355q_fp8_quantize_groups with e8m0 scales).  dy [rows, out] bf16, dw [out, cols] in
+ * dw_dtype, zeros for rows == 0.  Workspace as above. */
+size_t mi355q_fp8_block_grad_weight_workspace_size(int64_t rows, int64_t out, int64_t cols);
+int mi355q_fp8_block_grad_weight(const uint16_t* dy_dev, int64_t lddy, const uint8_t* x_dev, int64_t ldx,
+                                 const uint8_t* x_scales_dev, int64_t ld_x_scales, void* dw_dev,
+                                 mi355q_dtype dw_dtype, int64_t lddw, int64_t rows, int64_t out,
+                                 int64_t cols, void* workspace_dev, size_t workspace_bytes, void* stream);
+
+/* h = silu(gate) * up of x [rows, 2 cols] (gate in the first cols columns),
+ * quantized as mi355q_fp8_quantize_groups does with e8m0 scales from its fp32
+ * values: h codes [rows, cols], h scales [rows, G], G = ceil(cols / 128).
+ * kept codes [rows, 2 cols] and kept scales [rows, 2 G] (both NULL: not kept)
+ * receive gate and up quantized the same way, grouped apart: group j of gate at
+ * scale j, of up at G + j.  Scales are contiguous. */
+int mi355q_fp8_silu_mul(const void* x_dev, mi355q_dtype dtype, int64_t rows, int64_t cols, int64_t ldx,
+                        uint8_t* h_codes_dev, int64_t ld_h, uint8_t* h_scales_dev, uint8_t* kept_codes_dev,
+                        int64_t ld_kept, uint8_t* kept_scales_dev, void* stream);
+
+/* Its backward pass from what was kept: dx [rows, 2 cols] in dtype,
+ *   d gate = dh up s (1 + gate (1 - s)), d up = dh gate s, s = sigmoid(gate),
+ * dh [rows, cols] in dtype, gate and up as kept. */
+int mi355q_fp8_silu_mul_backward(const void* dh_dev, mi355q_dtype dtype, int64_t rows, int64_t cols,
+                                 int64_t ld_dh, const uint8_t* kept_codes_dev, int64_t ld_kept,
+                                 const uint8_t* kept_scales_dev, int64_t ld_scales, void* dx_dev,
+                                 int64_t ld_dx, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,59 @@
+// Shared pieces of the block-scaled fp8 kernels (fp8_quant.hip, fp8_matmul.hip).
+//
+// An fp8 matrix is e4m3 codes with one scale per row and kGroup columns
+// (activations, gradients' checkpoints) or per kGroup x kGroup block (weights):
+// value = code * scale.  Scales are fp32, or for activations e8m0 bytes
+// (2^(byte - 127), 255 = NaN).
+#pragma once
+
+#include "common.h"
+
+namespace mi355q {
+
+constexpr int kGroup = 128;
+
+inline int64_t group_count(int64_t n) { return (n + kGroup - 1) / kGroup; }
+
+// fp32 value of an e8m0 byte (0 is 2^-127, a subnormal)
+__device__ __forceinline__ float e8m0_to_f32(uint32_t b) {
+  const uint32_t u = b == 0 ? 0x00400000u : b == 255 ? 0x7fc00000u : b << 23;
+  return __uint_as_float(u);
+}
+
+__device__ __forceinline__ float load_scale(const void* s, int type, int64_t i) {
+  return type == MI355Q_SCALE_E8M0 ? e8m0_to_f32(static_cast<const uint8_t*>(s)[i]) : static_cast<const float*>(s)[i];
+}
+
+// 16-bit and fp32 element types of the activations, outputs and biases
+struct Bf16 {
+  typedef uint16_t raw;
+  static constexpr mi355q_dtype code = MI355Q_BF16;
+  static __device__ __forceinline__ float load(uint16_t v) { return bf16_bits_to_f32(v); }
+  static __device__ __forceinline__ uint16_t store(float f) { return f32_to_bf16_bits(f); }
+};
+struct F16 {
+  typedef uint16_t raw;
+  static constexpr mi355q_dtype code = MI355Q_F16;
+  static __device__ __forceinline__ float load(uint16_t v) { return (float)__builtin_bit_cast(_Float16, v); }
+  static __device__ __forceinline__ uint16_t store(float f) { return __builtin_bit_cast(uint16_t, (_Float16)f); }
+};
+struct F32 {
+  typedef float raw;
+  static constexpr mi355q_dtype code = MI355Q_F32;
+  static __device__ __forceinline__ float load(float v) { return v; }
+  static __device__ __forceinline__ float store(float f) { return f; }
+};
+
+// calls f(Bf16{} / F16{} / F32{}) for a dtype that the caller has checked
+template <class Fn>
+inline void with_dtype(mi355q_dtype dt, Fn&& f) {
+  if (dt == MI355Q_BF16) f(Bf16{});
+  else if (dt == MI355Q_F16) f(F16{});
+  else f(F32{});
+}
+
+inline bool known_dtype(int dt) { return dt == MI355Q_BF16 || dt == MI355Q_F16 || dt == MI355Q_F32; }
+inline int dtype_size(int dt) { return dt == MI355Q_F32 ? 4 : 2; }
+inline bool aligned_to(const void* p, unsigned n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+}  // namespace mi355q

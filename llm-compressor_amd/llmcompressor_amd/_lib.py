@@ -16,6 +16,7 @@ OK, INVALID_ARGUMENT, UNSUPPORTED, NOT_POSITIVE_DEFINITE, HIP_ERROR, TIMEOUT = 0
 BF16, F32, F16 = 0, 1, 2
 TENSOR, CHANNEL, GROUP, BLOCK, TOKEN = 0, 1, 2, 3, 4
 MX_RULE_CT, MX_RULE_OCP = 0, 1
+SCALE_F32, SCALE_E8M0 = 0, 1
 QTYPE_INT, QTYPE_FP8_E4M3, QTYPE_FP4_E2M1, QTYPE_MXFP4_CT, QTYPE_MXFP4_OCP = 0, 1, 2, 3, 4
 
 _vp, _i64, _i32, _f32, _f64, _sz = C.c_void_p, C.c_int64, C.c_int, C.c_float, C.c_double, C.c_size_t
@@ -86,6 +87,19 @@ SIGNATURES = {
     "mi355q_quantize_fp8": (_i32, [_vp, _i32, _i64, _i64, _i64, _vp, _i64, _i32, _i64, _i32, _vp, _vp]),
     "mi355q_fp4_quantize_pack": (_i32, [_vp, _i32, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp]),
     "mi355q_quantize_int8_per_token": (_i32, [_vp, _i64, _i64, _i64, _vp, _vp, _vp]),
+    "mi355q_fp8_quantize_groups": (_i32, [_vp, _i32, _i64, _i64, _i64, _vp, _i64, _vp, _i32, _i64, _vp]),
+    "mi355q_fp8_quantize_blocks": (_i32, [_vp, _i32, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp]),
+    "mi355q_fp8_block_matmul_workspace_size": (_sz, [_i64, _i64, _i64]),
+    "mi355q_fp8_block_matmul": (_i32, [_vp, _i64, _vp, _i32, _i64, _vp, _i64, _vp, _i64, _vp, _i32, _vp, _i32, _i64,
+                                       _i64, _i64, _i64, _vp, _sz, _vp]),
+    "mi355q_fp8_block_grad_input_workspace_size": (_sz, [_i64, _i64, _i64]),
+    "mi355q_fp8_block_grad_input": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _vp, _sz,
+                                           _vp]),
+    "mi355q_fp8_block_grad_weight_workspace_size": (_sz, [_i64, _i64, _i64]),
+    "mi355q_fp8_block_grad_weight": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i32, _i64, _i64, _i64, _i64, _vp,
+                                            _sz, _vp]),
+    "mi355q_fp8_silu_mul": (_i32, [_vp, _i32, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _vp]),
+    "mi355q_fp8_silu_mul_backward": (_i32, [_vp, _i32, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp]),
 }
 
 _lock = threading.Lock()

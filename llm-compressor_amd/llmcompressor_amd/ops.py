@@ -651,6 +651,220 @@ def quantize_int8_per_token(x: torch.Tensor):
     return codes, scale
 
 
+# ---------------------------------------------------------------- block-scaled fp8
+FP8_GROUP = 128     # columns per activation scale, rows and columns per weight scale
+_FP8_DT = {torch.bfloat16: L.BF16, torch.float16: L.F16, torch.float32: L.F32}
+_FP8_SCALES = {torch.float32: L.SCALE_F32, torch.float8_e8m0fnu: L.SCALE_E8M0}
+
+
+def _fp8_groups(n: int) -> int:
+    return -(-n // FP8_GROUP)
+
+
+def _fp8_source(x: torch.Tensor, what: str) -> torch.Tensor:
+    """x as a 2-D matrix with contiguous rows of bf16, fp16 or fp32."""
+    L.require_gpu(x)
+    if x.dtype not in _FP8_DT:
+        raise TypeError(f"{what} must be bf16, fp16 or fp32, got {x.dtype}")
+    if x.dim() != 2 or x.shape[1] == 0:
+        raise ValueError(f"{what} must be a 2-D matrix with columns, got {tuple(x.shape)}")
+    return x if x.stride(1) == 1 and x.stride(0) >= x.shape[1] else x.contiguous()
+
+
+def _fp8_matrix(codes: torch.Tensor, scales: torch.Tensor, what: str, blocks: bool, scale_dtypes):
+    """A checked fp8 matrix: e4m3 codes [rows, cols] and its scales."""
+    L.require_gpu(codes, scales)
+    if codes.dtype != torch.float8_e4m3fn or codes.dim() != 2 or codes.shape[1] == 0:
+        raise TypeError(f"{what} must be a 2-D float8_e4m3fn matrix with columns, got {tuple(codes.shape)} "
+                        f"{codes.dtype}")
+    rows = _fp8_groups(codes.shape[0]) if blocks else codes.shape[0]
+    want = (rows, _fp8_groups(codes.shape[1]))
+    if scales.dtype not in scale_dtypes:
+        raise TypeError(f"{what} scales must be {' or '.join(str(d) for d in scale_dtypes)}, got {scales.dtype}")
+    if tuple(scales.shape) != want:
+        raise ValueError(f"{what} of {tuple(codes.shape)} takes scales of {want}, got {tuple(scales.shape)}")
+    if codes.stride(1) != 1 or codes.stride(0) < codes.shape[1]:
+        codes = codes.contiguous()
+    if scales.stride(1) != 1 or scales.stride(0) < scales.shape[1]:
+        scales = scales.contiguous()
+    return codes, scales
+
+
+def _fp8_gradient(dy: torch.Tensor, cols: int) -> torch.Tensor:
+    L.require_gpu(dy)
+    if dy.dtype != torch.bfloat16:
+        raise TypeError(f"the output gradient must be bf16, got {dy.dtype}")
+    if dy.dim() != 2 or dy.shape[1] != cols:
+        raise ValueError(f"the output gradient must be [rows, {cols}], got {tuple(dy.shape)}")
+    return dy if dy.stride(1) == 1 and dy.stride(0) >= cols else dy.contiguous()
+
+
+def _one_device(*tensors) -> None:
+    if len({t.device for t in tensors if t is not None}) > 1:
+        raise ValueError(f"operands on several devices: {[str(t.device) for t in tensors if t is not None]}")
+
+
+def fp8_quantize_groups(x: torch.Tensor, scale_dtype: torch.dtype = torch.float32):
+    """x [rows, cols] as float8_e4m3fn codes and one scale per row and 128
+    columns: (codes [rows, cols], scales [rows, ceil(cols / 128)]).
+
+    ``scale_dtype`` float32: max |x| / 448; float8_e8m0fnu: the least power
+    of two not below it, with which the codes are also the 8-bit checkpoint
+    that ``fp8_block_grad_weight`` reads.  A group holding an infinity or a
+    NaN becomes NaN as a whole."""
+    x = _fp8_source(x, "x")
+    if scale_dtype not in _FP8_SCALES:
+        raise TypeError(f"scale_dtype must be float32 or float8_e8m0fnu, got {scale_dtype}")
+    rows, cols = x.shape
+    codes = torch.empty((rows, cols), dtype=torch.float8_e4m3fn, device=x.device)
+    scales = torch.empty((rows, _fp8_groups(cols)), dtype=scale_dtype, device=x.device)
+    L.call("mi355q_fp8_quantize_groups", x.data_ptr(), _FP8_DT[x.dtype], rows, cols, x.stride(0), codes.data_ptr(),
+           cols, scales.data_ptr(), _FP8_SCALES[scale_dtype], scales.shape[1], L.stream_of(x))
+    return codes, scales
+
+
+def fp8_quantize_blocks(w: torch.Tensor):
+    """w [rows, cols] as float8_e4m3fn codes and one fp32 scale (max |w| /
+    448) per 128 x 128 block: (codes [rows, cols], scales [ceil(rows / 128),
+    ceil(cols / 128)]).  A block holding an infinity or a NaN becomes NaN as a
+    whole."""
+    w = _fp8_source(w, "w")
+    rows, cols = w.shape
+    codes = torch.empty((rows, cols), dtype=torch.float8_e4m3fn, device=w.device)
+    scales = torch.empty((_fp8_groups(rows), _fp8_groups(cols)), dtype=torch.float32, device=w.device)
+    L.call("mi355q_fp8_quantize_blocks", w.data_ptr(), _FP8_DT[w.dtype], rows, cols, w.stride(0), codes.data_ptr(),
+           cols, scales.data_ptr(), scales.shape[1], L.stream_of(w))
+    return codes, scales
+
+
+def fp8_block_matmul(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor,
+                     bias: torch.Tensor | None = None, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """y = X W^T (+ bias) [rows, out] of two fp8 matrices: x [rows, cols] with
+    scales per row and 128 columns (float32 or float8_e8m0fnu,
+    ``fp8_quantize_groups``), w [out, cols] with float32 scales per 128 x 128
+    block (``fp8_quantize_blocks``, or an FP8_BLOCK checkpoint's
+    ``weight_scale`` in fp32).  Sums in fp32, rounded once to ``out_dtype``
+    (bf16, fp16 or fp32).  ``bias`` [out] is bf16, fp16 or fp32."""
+    x, x_scales = _fp8_matrix(x, x_scales, "x", False, tuple(_FP8_SCALES))
+    w, w_scales = _fp8_matrix(w, w_scales, "w", True, (torch.float32,))
+    rows, cols = x.shape
+    out = w.shape[0]
+    if w.shape[1] != cols or out == 0:
+        raise ValueError(f"x [{rows}, {cols}] does not multiply w {tuple(w.shape)}")
+    if out_dtype not in _FP8_DT:
+        raise TypeError(f"out_dtype must be bf16, fp16 or fp32, got {out_dtype}")
+    if bias is not None:
+        L.require_gpu(bias)
+        if bias.dtype not in _FP8_DT:
+            raise TypeError(f"bias must be bf16, fp16 or fp32, got {bias.dtype}")
+        if bias.shape != (out,):
+            raise ValueError(f"bias must be [{out}], got {tuple(bias.shape)}")
+        bias = bias.contiguous()
+    _one_device(x, x_scales, w, w_scales, bias)
+    y = torch.empty((rows, out), dtype=out_dtype, device=x.device)
+    lib = L.lib()
+    ws = _ws(lib.mi355q_fp8_block_matmul_workspace_size(rows, out, cols), x.device)
+    L.check(lib.mi355q_fp8_block_matmul(
+        x.data_ptr(), x.stride(0), x_scales.data_ptr(), _FP8_SCALES[x_scales.dtype], x_scales.stride(0), w.data_ptr(),
+        w.stride(0), w_scales.data_ptr(), w_scales.stride(0), L.ptr(bias), _FP8_DT[bias.dtype] if bias is not None else 0,
+        y.data_ptr(), _FP8_DT[out_dtype], out, rows, out, cols, L.ptr(ws), 0 if ws is None else ws.numel(),
+        L.stream_of(x)))
+    return y
+
+
+def fp8_block_grad_input(dy: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor) -> torch.Tensor:
+    """dX = dY W [rows, cols] in bf16: the input gradient of
+    ``fp8_block_matmul`` (dy bf16 [rows, out], w as in the forward product;
+    the weight's values enter exactly, sums in fp32)."""
+    w, w_scales = _fp8_matrix(w, w_scales, "w", True, (torch.float32,))
+    out, cols = w.shape
+    dy = _fp8_gradient(dy, out)
+    if out == 0:
+        raise ValueError("w has no rows")
+    _one_device(dy, w, w_scales)
+    rows = dy.shape[0]
+    dx = torch.empty((rows, cols), dtype=torch.bfloat16, device=dy.device)
+    lib = L.lib()
+    ws = _ws(lib.mi355q_fp8_block_grad_input_workspace_size(rows, out, cols), dy.device)
+    L.check(lib.mi355q_fp8_block_grad_input(dy.data_ptr(), dy.stride(0), w.data_ptr(), w.stride(0),
+                                            w_scales.data_ptr(), w_scales.stride(0), dx.data_ptr(), cols, rows, out,
+                                            cols, L.ptr(ws), 0 if ws is None else ws.numel(), L.stream_of(dy)))
+    return dx
+
+
+def fp8_block_grad_weight(dy: torch.Tensor, x: torch.Tensor, x_scales: torch.Tensor,
+                          out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """dW = dY^T X [out, cols]: the weight gradient of ``fp8_block_matmul``
+    from the 8-bit checkpoint of its input (``fp8_quantize_groups`` with
+    ``scale_dtype=torch.float8_e8m0fnu``; the checkpoint's values enter
+    exactly).  dy bf16 [rows, out]; sums in fp32, rounded once to
+    ``out_dtype`` (bf16, fp16 or fp32).  Zeros when there are no rows."""
+    x, x_scales = _fp8_matrix(x, x_scales, "x", False, (torch.float8_e8m0fnu,))
+    rows, cols = x.shape
+    if dy.dim() != 2 or dy.shape[0] != rows or dy.shape[1] == 0:
+        raise ValueError(f"the output gradient must be [{rows}, out], got {tuple(dy.shape)}")
+    out = dy.shape[1]
+    dy = _fp8_gradient(dy, out)
+    if out_dtype not in _FP8_DT:
+        raise TypeError(f"out_dtype must be bf16, fp16 or fp32, got {out_dtype}")
+    _one_device(dy, x, x_scales)
+    dw = torch.empty((out, cols), dtype=out_dtype, device=dy.device)
+    lib = L.lib()
+    ws = _ws(lib.mi355q_fp8_block_grad_weight_workspace_size(rows, out, cols), dy.device)
+    L.check(lib.mi355q_fp8_block_grad_weight(dy.data_ptr(), dy.stride(0), x.data_ptr(), x.stride(0),
+                                             x_scales.data_ptr(), x_scales.stride(0), dw.data_ptr(),
+                                             _FP8_DT[out_dtype], cols, rows, out, cols, L.ptr(ws),
+                                             0 if ws is None else ws.numel(), L.stream_of(dy)))
+    return dw
+
+
+def fp8_silu_mul(gate_up: torch.Tensor, save: bool = True):
+    """h = silu(gate) * up of gate_up [rows, 2 n] (gate in the first n
+    columns) as an fp8 matrix with e8m0 scales: (h codes [rows, n], h scales
+    [rows, ceil(n / 128)]).  With ``save`` also gate and up in 8 bits for the
+    backward pass: (..., saved codes [rows, 2 n], saved scales [rows, 2
+    ceil(n / 128)]), gate's groups before up's."""
+    x = _fp8_source(gate_up, "gate_up")
+    rows, cols = x.shape[0], x.shape[1] // 2
+    if x.shape[1] % 2:
+        raise ValueError(f"gate_up must hold gate and up side by side, got {x.shape[1]} columns")
+    groups = _fp8_groups(cols)
+
+    def new(width, dtype):
+        return torch.empty((rows, width), dtype=dtype, device=x.device)
+
+    h, hs = new(cols, torch.float8_e4m3fn), new(groups, torch.float8_e8m0fnu)
+    kept = new(2 * cols, torch.float8_e4m3fn) if save else None
+    ks = new(2 * groups, torch.float8_e8m0fnu) if save else None
+    L.call("mi355q_fp8_silu_mul", x.data_ptr(), _FP8_DT[x.dtype], rows, cols, x.stride(0), h.data_ptr(), cols,
+           hs.data_ptr(), L.ptr(kept), 2 * cols, L.ptr(ks), L.stream_of(x))
+    return (h, hs, kept, ks) if save else (h, hs)
+
+
+def fp8_silu_mul_backward(dh: torch.Tensor, saved: torch.Tensor, saved_scales: torch.Tensor) -> torch.Tensor:
+    """The gradient [rows, 2 n] of ``fp8_silu_mul``'s input, in dh's type,
+    from dh [rows, n] (bf16, fp16 or fp32) and what the forward pass saved."""
+    dh = _fp8_source(dh, "dh")
+    L.require_gpu(saved, saved_scales)
+    rows, cols = dh.shape
+    if saved.dtype != torch.float8_e4m3fn or saved_scales.dtype != torch.float8_e8m0fnu:
+        raise TypeError(f"saved codes and scales must be float8_e4m3fn and float8_e8m0fnu, got {saved.dtype} and "
+                        f"{saved_scales.dtype}")
+    if tuple(saved.shape) != (rows, 2 * cols) or tuple(saved_scales.shape) != (rows, 2 * _fp8_groups(cols)):
+        raise ValueError(f"dh of {tuple(dh.shape)} takes saved codes of {(rows, 2 * cols)} and scales of "
+                         f"{(rows, 2 * _fp8_groups(cols))}, got {tuple(saved.shape)} and {tuple(saved_scales.shape)}")
+    _one_device(dh, saved, saved_scales)
+    if saved.stride(1) != 1 or saved.stride(0) < 2 * cols:
+        saved = saved.contiguous()
+    if saved_scales.stride(1) != 1 or saved_scales.stride(0) < saved_scales.shape[1]:
+        saved_scales = saved_scales.contiguous()
+    dx = torch.empty((rows, 2 * cols), dtype=dh.dtype, device=dh.device)
+    L.call("mi355q_fp8_silu_mul_backward", dh.data_ptr(), _FP8_DT[dh.dtype], rows, cols, dh.stride(0),
+           saved.data_ptr(), saved.stride(0), saved_scales.data_ptr(), saved_scales.stride(0), dx.data_ptr(),
+           2 * cols, L.stream_of(dh))
+    return dx
+
+
 # ---------------------------------------------------------------- SparseGPT
 def sparsegpt_base_mask(w_work: torch.Tensor):
     """(mask uint8 [rows, cols] = w_work == 0, count int32 [1] on the device)."""
