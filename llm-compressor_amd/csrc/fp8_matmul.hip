@@ -29,6 +29,7 @@ struct ProductArgs {
   const void* bias;      // forward, or null
   int bias_type;
   void* c;
+  int c_type;
   int64_t ldc;
   int64_t P, Q, R;
   uint32_t q_tiles;
@@ -143,6 +144,522 @@ __global__ __launch_bounds__(256) void product_any_kernel(ProductArgs g) {
   }
 }
 
+// ---------------------------------------------------------------- forward, tiles
+// Rows of 128 codes (one K step) go global -> LDS by the gfx950 LDS-DMA load
+// with their 16-byte chunks XOR-swizzled by row & 7, so that both the DMA's
+// writes and the operand reads (rows of one chunk) spread over all banks.
+//
+// The fp8 matrix instructions would take the codes as they are at twice the
+// rate, but they add with few bits: on heavy-tailed codes up to 2.6e-4 of the
+// terms' magnitudes (16x16x128 and 16x16x32 alike) where the bf16 instructions
+// are within 3.2e-7.  So the codes are converted to bf16 in registers (exact,
+// two an instruction) and the sums are fp32 sums of exact products.
+//
+// A step is, per 32 x 32 tile, eight 32x32x16 MFMAs from zero and
+// acc += tile * (token scale * block scale) in fp32: the features are the
+// MFMA's rows, so a lane holds one token per tile (its scale is one register)
+// and the block scale is wave-uniform.
+typedef __attribute__((address_space(3))) void lds_void_t;
+
+__device__ __forceinline__ uint32_t lds_u32(const void* p) {
+  return (uint32_t) reinterpret_cast<uintptr_t>((lds_void_t*)p);
+}
+// 64 lanes x 16 bytes to LDS at m0, from a scalar base and lane offsets.
+// Completion is waited for explicitly (vmcnt).
+__device__ __forceinline__ void dma_s(uint32_t off, const void* base, uint32_t m0) {
+  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(m0) : "memory", "m0");
+}
+
+// eight codes as bf16
+__device__ __forceinline__ bf16x8_t codes_bf16(uint32_t lo, uint32_t hi) {
+  typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+  const bf16x2_t a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.f, false);
+  const bf16x2_t b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.f, true);
+  const bf16x2_t c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, false);
+  const bf16x2_t d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, true);
+  return bf16x8_t{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+// Work item of a workgroup: the workgroups of one XCD (every eighth) take
+// neighbouring tiles, in groups of 8 row tiles, so that they share operands in
+// its L2; the splits of the sum are the outermost order.
+struct TileOrder {
+  uint32_t row_tiles, col_tiles, splits;
+};
+__device__ __forceinline__ void tile_of(const TileOrder& o, uint32_t id, uint32_t& tr, uint32_t& tc, uint32_t& split) {
+  const uint32_t tiles = o.row_tiles * o.col_tiles, total = tiles * o.splits;
+  const uint32_t q = total / 8, r = total % 8, x = id % 8;
+  const uint32_t lin = x * q + (x < r ? x : r) + id / 8;
+  split = lin / tiles;
+  const uint32_t t = lin - split * tiles, g = t / (8 * o.col_tiles), left = o.row_tiles - 8 * g;
+  const uint32_t rows = left < 8 ? left : 8, in = t - g * 8 * o.col_tiles;
+  tc = in / rows;
+  tr = 8 * g + in - tc * rows;
+}
+
+// T x A tiles of 32 tokens x 32 features per wave, WT x WF waves.
+template <int T, int A, int WT, int WF>
+struct FwdShape {
+  static constexpr int W = WT * WF, NTH = 64 * W;
+  static constexpr int TT = 32 * T * WT, FT = 32 * A * WF;   // tokens, features per workgroup
+  static constexpr int A_SLOT = FT * kGroup, B_SLOT = TT * kGroup;
+  // three slots of features, two of tokens: a step's token operands are in
+  // registers before the step begins
+  static constexpr int RING = 3 * A_SLOT + 2 * B_SLOT;
+  static constexpr int PITCH = A * 64 + 16;                  // bytes per token row of the staged output
+  static constexpr int BIAS = W * 32 * T * PITCH;            // fp32 biases behind it
+  static constexpr int LDS = RING > BIAS + FT * 4 ? RING : BIAS + FT * 4;
+};
+
+template <int T, int A, int WT, int WF, bool E8M0>
+__global__ __launch_bounds__(64 * WT * WF) __attribute__((amdgpu_waves_per_eu(2)))
+void fp8_forward_kernel(ProductArgs g, TileOrder order, int steps_per_split, float* part) {
+  using S = FwdShape<T, A, WT, WF>;
+  __shared__ __attribute__((aligned(16))) char ring[S::LDS];
+  char* const ringb = ring + 3 * S::A_SLOT;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wt = wave % WT, wf = wave / WT;
+  uint32_t tr, tc, split;
+  tile_of(order, blockIdx.x, tr, tc, split);
+  const int64_t t0 = (int64_t)tr * S::TT, f0 = (int64_t)tc * S::FT;
+  const int nkb = (int)((g.R + kGroup - 1) / kGroup);
+  const int s_begin = (int)split * steps_per_split;
+  const int s_end = s_begin + steps_per_split < nkb ? s_begin + steps_per_split : nkb;
+
+  // DMA: instruction j of wave w fills 8 rows; lane l the chunk position l & 7
+  // of row l / 8, with the row's chunk (l & 7) ^ (row & 7).  Rows past the end
+  // read the last row again (their results are not stored).
+  constexpr int NA = S::FT / 8 / S::W, NB = S::TT / 8 / S::W;
+  static_assert(NA * 8 * S::W == S::FT && NB * 8 * S::W == S::TT, "rows per wave");
+  const int chunk = (lane & 7) ^ (lane >> 3);
+  uint32_t oa[NA], ob[NB];
+#pragma unroll
+  for (int j = 0; j < NA; ++j) {
+    const int64_t r = f0 + (wave * NA + j) * 8 + (lane >> 3);
+    oa[j] = (uint32_t)((r < g.Q ? r : g.Q - 1) - f0) * (uint32_t)g.ldb + 16 * chunk;
+    asm volatile("" : "+v"(oa[j]));   // one register, not re-derived in the loop
+  }
+#pragma unroll
+  for (int j = 0; j < NB; ++j) {
+    const int64_t r = t0 + (wave * NB + j) * 8 + (lane >> 3);
+    ob[j] = (uint32_t)((r < g.P ? r : g.P - 1) - t0) * (uint32_t)g.lda + 16 * chunk;
+    asm volatile("" : "+v"(ob[j]));
+  }
+  const char* const wbase = reinterpret_cast<const char*>(g.b) + f0 * g.ldb;
+  const char* const xbase = static_cast<const char*>(g.a) + t0 * g.lda;
+  const uint32_t la0 = lds_u32(ring) + wave * NA * 1024, lb0 = lds_u32(ringb) + wave * NB * 1024;
+  // A last step of fewer than 128 columns: a chunk past the end is read as its
+  // row's first chunk of the step, and the token rows' such chunks are cleared
+  // in LDS, so that it adds nothing (a NaN in the first chunk is in the row's
+  // sum anyway).
+  const int tail = (int)(g.R % kGroup) / 16;                    // whole chunks of a short last step
+  const uint32_t dead = tail && chunk >= tail ? 16 * chunk : 0;
+  auto load_a = [&](int s, int slot, int j) __attribute__((always_inline)) {
+    dma_s(oa[j] - (s == nkb - 1 ? dead : 0u), wbase + (int64_t)s * kGroup,
+          la0 + (uint32_t)(slot % 3) * S::A_SLOT + 1024 * j);
+  };
+  auto load_b = [&](int s, int slot, int j) __attribute__((always_inline)) {
+    dma_s(ob[j] - (s == nkb - 1 ? dead : 0u), xbase + (int64_t)s * kGroup,
+          lb0 + (uint32_t)(slot & 1) * S::B_SLOT + 1024 * j);
+  };
+  auto clear_tail = [&](int s) __attribute__((always_inline)) {
+    if (!tail || s != nkb - 1) return;
+#pragma unroll
+    for (int i = 0; i < S::TT * 8 / S::NTH; ++i) {
+      const int at = i * S::NTH + (int)threadIdx.x, row = at >> 3;
+      if (((at & 7) ^ (row & 7)) >= tail)
+        *reinterpret_cast<u32x4_t*>(ringb + (s & 1) * S::B_SLOT + at * 16) = u32x4_t{0u, 0u, 0u, 0u};
+    }
+    __syncthreads();
+  };
+
+  // operand reads: lane l holds row l & 31, codes 64 (l / 32) and on: two
+  // slices of eight per 16-byte chunk (which codes a slice pairs is free, as
+  // long as both operands agree)
+  int p[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    p[i] = (lane & 31) * kGroup + 16 * ((4 * (lane >> 5) + i) ^ (lane & 7));
+    asm volatile("" : "+v"(p[i]));
+  }
+  auto read_a = [&](int s, int a, int i) __attribute__((always_inline)) {
+    return *reinterpret_cast<const u32x4_t*>(ring + (s % 3) * S::A_SLOT + (wf * A + a) * 32 * kGroup + p[i]);
+  };
+  auto read_b = [&](int s, int b, int i) __attribute__((always_inline)) {
+    return *reinterpret_cast<const u32x4_t*>(ringb + (s & 1) * S::B_SLOT + (wt * T + b) * 32 * kGroup + p[i]);
+  };
+
+  // scales: this lane's tokens, and the block scale of the wave's features
+  uint32_t xsi[T];   // from the tile's first token
+#pragma unroll
+  for (int b = 0; b < T; ++b) {
+    const int64_t t = t0 + (wt * T + b) * 32 + (lane & 31);
+    xsi[b] = (uint32_t)((t < g.P ? t : g.P - 1) - t0) * (uint32_t)g.ldas;
+    asm volatile("" : "+v"(xsi[b]));
+  }
+  const char* const xsc = static_cast<const char*>(g.as) + t0 * g.ldas * (E8M0 ? 1 : 4);
+  int64_t fb = (f0 + wf * A * 32) / kGroup;
+  if (fb > (g.Q - 1) / kGroup) fb = (g.Q - 1) / kGroup;
+  const float* const wsc = g.bs + fb * g.ldbs;
+  uint32_t sx_load[T];
+  float sw_load;
+  auto load_scales = [&](int s) __attribute__((always_inline)) {
+#pragma unroll
+    for (int b = 0; b < T; ++b) {
+      if constexpr (E8M0) sx_load[b] = reinterpret_cast<const uint8_t*>(xsc + s)[xsi[b]];
+      else sx_load[b] = reinterpret_cast<const uint32_t*>(xsc + 4 * (int64_t)s)[xsi[b]];
+    }
+    sw_load = wsc[s];
+  };
+  float sc[T], sc_next[T];
+  auto take_scales = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int b = 0; b < T; ++b) {
+      sc_next[b] = (E8M0 ? e8m0_to_f32(sx_load[b]) : __uint_as_float(sx_load[b])) * sw_load;
+      asm volatile("" : "+v"(sc_next[b]));
+    }
+  };
+
+  f32x16_t acc[A][T];
+#pragma unroll
+  for (int a = 0; a < A; ++a)
+#pragma unroll
+    for (int b = 0; b < T; ++b)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[a][b][e] = 0.f;
+  bf16x8_t xb[T][8];   // the step's token operands
+  u32x4_t ra;          // the next two slices of the features, as codes
+  auto convert_b = [&](const u32x4_t* raw, int i) __attribute__((always_inline)) {
+#pragma unroll
+    for (int b = 0; b < T; ++b) {
+      xb[b][2 * i] = codes_bf16(raw[b][0], raw[b][1]);
+      xb[b][2 * i + 1] = codes_bf16(raw[b][2], raw[b][3]);
+    }
+  };
+
+  // Step s.  Its token operands and first feature codes are in registers; the
+  // barrier before its last row of tiles publishes step s + 1 and frees the
+  // feature slot of step s - 1 and the token slot of step s for step s + 2,
+  // whose DMA then has a step's time.  In the last row of tiles each token
+  // operand is replaced by its successor's as soon as its last MFMA is issued.
+  auto step = [&](int s) __attribute__((always_inline)) {
+    // past the last step the loads repeat it, into slots that nothing reads:
+    // without a branch in the step the compiler keeps the sums between the MFMAs
+    const int s1 = s + 1 < s_end ? s + 1 : s, s2 = s + 2 < s_end ? s + 2 : s_end - 1;
+    u32x4_t rb[T];
+#pragma unroll
+    for (int b = 0; b < T; ++b) sc[b] = sc_next[b];
+#pragma unroll
+    for (int a = 0; a < A; ++a) {
+      constexpr int LAST = A - 1;
+      if (a == LAST) {
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+        if (s1 != s) clear_tail(s1);
+        // (the scales of step s + 1 were requested a step ago, with the DMA
+        // that the wait above is for: a use anywhere else would wait for the
+        // DMA issued since)
+        take_scales();
+        load_scales(s2);
+#pragma unroll
+        for (int b = 0; b < T; ++b) rb[b] = read_b(s + 1, b, 0);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      f32x16_t t[T];
+#pragma unroll
+      for (int b = 0; b < T; ++b)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) t[b][e] = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const bf16x8_t f0r = codes_bf16(ra[0], ra[1]), f1r = codes_bf16(ra[2], ra[3]);
+        ra = i < 3 ? read_a(s, a, i + 1) : a < LAST ? read_a(s, a + 1, 0) : read_a(s + 1, 0, 0);
+#pragma unroll
+        for (int b = 0; b < T; ++b) t[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f0r, xb[b][2 * i], t[b], 0, 0, 0);
+#pragma unroll
+        for (int b = 0; b < T; ++b)
+          t[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f1r, xb[b][2 * i + 1], t[b], 0, 0, 0);
+        if (a == LAST) {
+          convert_b(rb, i);
+          if (i < 3) {
+#pragma unroll
+            for (int b = 0; b < T; ++b) rb[b] = read_b(s + 1, b, i + 1);
+          }
+#pragma unroll
+          for (int j = 0; j < NA; ++j)
+            if (j * 4 / NA == i) load_a(s2, s + 2, j);
+#pragma unroll
+          for (int j = 0; j < NB; ++j)
+            if (j * 4 / NB == i) load_b(s2, s + 2, j);
+        }
+      }
+#pragma unroll
+      for (int b = 0; b < T; ++b) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[a][b][e] = fmaf(t[b][e], sc[b], acc[a][b][e]);
+        asm volatile("" : "+v"(acc[a][b]));
+      }
+    }
+  };
+
+  {   // every split has a step
+    const int s1 = s_begin + 1 < s_end ? s_begin + 1 : s_begin;
+#pragma unroll
+    for (int j = 0; j < NA; ++j) load_a(s_begin, s_begin, j);
+#pragma unroll
+    for (int j = 0; j < NB; ++j) load_b(s_begin, s_begin, j);
+    load_scales(s_begin);
+    asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+    clear_tail(s_begin);
+    take_scales();
+    load_scales(s1);
+#pragma unroll
+    for (int j = 0; j < NA; ++j) load_a(s1, s_begin + 1, j);
+#pragma unroll
+    for (int j = 0; j < NB; ++j) load_b(s1, s_begin + 1, j);
+    ra = read_a(s_begin, 0, 0);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      u32x4_t rb[T];
+#pragma unroll
+      for (int b = 0; b < T; ++b) rb[b] = read_b(s_begin, b, i);
+      convert_b(rb, i);
+    }
+    for (int s = s_begin; s < s_end; ++s) step(s);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // before the ring is used again
+  }
+
+  // lane l holds token l & 31 and, in registers 4 j .. 4 j + 3 of a tile,
+  // features 8 j + 4 (l / 32) and on
+  const int64_t tw = t0 + wt * T * 32, fw = f0 + wf * A * 32;   // the wave's first token and feature
+  __syncthreads();   // the ring is no longer read
+  float* const biases = reinterpret_cast<float*>(ring + S::BIAS);
+  for (int i = threadIdx.x; i < S::FT; i += S::NTH)
+    biases[i] = g.bias && !part && f0 + i < g.Q ? load_typed(g.bias, g.bias_type, f0 + i) : 0.f;
+  __syncthreads();
+  const float* const bw = biases + wf * A * 32 + 4 * (lane >> 5);
+  if (part || g.c_type == MI355Q_F32) {
+    float* const out = part ? part + (int64_t)split * g.P * g.Q : static_cast<float*>(g.c);
+    const int64_t ld = part ? g.Q : g.ldc;
+    const bool wide = ld % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+#pragma unroll
+    for (int a = 0; a < A; ++a)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int64_t f = fw + 32 * a + 8 * j + 4 * (lane >> 5);
+        const f32x4_t bias = *reinterpret_cast<const f32x4_t*>(bw + 32 * a + 8 * j);
+#pragma unroll
+        for (int b = 0; b < T; ++b) {
+          const int64_t t = tw + 32 * b + (lane & 31);
+          const f32x4_t v = f32x4_t{acc[a][b][4 * j], acc[a][b][4 * j + 1], acc[a][b][4 * j + 2],
+                                    acc[a][b][4 * j + 3]} + bias;
+          if (t < g.P) {
+            float* o = out + t * ld + f;
+            if (wide && f + 4 <= g.Q) {
+              *reinterpret_cast<f32x4_t*>(o) = v;
+            } else {
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (f + e < g.Q) o[e] = v[e];
+            }
+          }
+        }
+      }
+    return;
+  }
+  // 16-bit outputs through LDS, so that a token's features leave as 16-byte
+  // stores of whole lines (straight from the tiles they are 16-byte pieces)
+  char* const stage = ring + wave * 32 * T * S::PITCH;
+  const bool bf = g.c_type == MI355Q_BF16;
+#pragma unroll
+  for (int a = 0; a < A; ++a)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const f32x4_t bias = *reinterpret_cast<const f32x4_t*>(bw + 32 * a + 8 * j);
+#pragma unroll
+      for (int b = 0; b < T; ++b) {
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = acc[a][b][4 * j + e] + bias[e];
+        uint32_t lo, hi;
+        if (bf) {
+          lo = Bf16::store(v[0]) | (uint32_t)Bf16::store(v[1]) << 16;
+          hi = Bf16::store(v[2]) | (uint32_t)Bf16::store(v[3]) << 16;
+        } else {
+          lo = F16::store(v[0]) | (uint32_t)F16::store(v[1]) << 16;
+          hi = F16::store(v[2]) | (uint32_t)F16::store(v[3]) << 16;
+        }
+        uint32_t* o = reinterpret_cast<uint32_t*>(stage + (32 * b + (lane & 31)) * S::PITCH + 64 * a + 16 * j +
+                                                  8 * (lane >> 5));
+        o[0] = lo;
+        o[1] = hi;
+      }
+    }
+  __syncthreads();
+  constexpr int LPR = 4 * A, RPI = 64 / LPR;   // lanes per row, rows per pass
+  uint16_t* const out = static_cast<uint16_t*>(g.c);
+  const bool wide = g.ldc % 8 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+  const int64_t f = fw + 8 * (lane % LPR);
+#pragma unroll
+  for (int i = 0; i < 32 * T / RPI; ++i) {
+    const int r = i * RPI + lane / LPR;
+    const u32x4_t v = *reinterpret_cast<const u32x4_t*>(stage + r * S::PITCH + 16 * (lane % LPR));
+    if (tw + r < g.P) {
+      uint16_t* o = out + (tw + r) * g.ldc + f;
+      if (wide && f + 8 <= g.Q) {
+        *reinterpret_cast<u32x4_t*>(o) = v;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (f + e < g.Q) o[e] = (uint16_t)(v[e >> 1] >> (16 * (e & 1)));
+      }
+    }
+  }
+}
+
+// Sums the splits' partial products [splits][rows][cols] in order, adds the
+// bias and rounds once.
+__global__ __launch_bounds__(256) void sum_splits_kernel(const float* part, int splits, int64_t rows, int64_t cols,
+                                                         const void* bias, int bias_type, void* c, int c_type,
+                                                         int64_t ldc) {
+  const int64_t n = rows * cols;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / cols, q = i - r * cols;
+    float v = 0.f;
+    for (int s = 0; s < splits; ++s) v += part[s * n + i];
+    if (bias) v += load_typed(bias, bias_type, q);
+    if (c_type == MI355Q_F32) static_cast<float*>(c)[r * ldc + q] = v;
+    else static_cast<uint16_t*>(c)[r * ldc + q] = c_type == MI355Q_BF16 ? Bf16::store(v) : F16::store(v);
+  }
+}
+
+// ---------------------------------------------------------------- forward, few tokens
+// Up to 16 TF tokens: the weight is read once, straight into the MFMA's
+// registers (lane l: row l & 15, 32 bytes at 32 (l / 16) of the step's 128), the
+// tokens come from L2, and the W waves of a workgroup take every W-th step of 16 AF
+// features; their sums are joined in LDS.  Bound by the weight's bytes, so what
+// counts is loads in flight: U steps are requested before the first is used.
+typedef int i32x4_t __attribute__((ext_vector_type(4)));
+typedef int i32x8_t __attribute__((ext_vector_type(8)));
+
+template <int TF, int AF, int W, int U, bool E8M0>
+__global__ __launch_bounds__(64 * W) void fp8_few_kernel(ProductArgs g) {
+  __shared__ f32x4_t sums[W][AF][TF][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t f0 = (int64_t)blockIdx.x * 16 * AF;
+  const int nkb = (int)((g.R + kGroup - 1) / kGroup);
+  const int koff = 32 * (lane >> 4);
+  const uint8_t* wp[AF];
+  const uint8_t* xp[TF];
+  int64_t xsi[TF];
+#pragma unroll
+  for (int a = 0; a < AF; ++a) {
+    const int64_t f = f0 + 16 * a + (lane & 15);
+    wp[a] = g.b + (f < g.Q ? f : g.Q - 1) * g.ldb + koff;
+  }
+#pragma unroll
+  for (int b = 0; b < TF; ++b) {
+    const int64_t t = 16 * b + (lane & 15), tt = t < g.P ? t : g.P - 1;
+    xp[b] = static_cast<const uint8_t*>(g.a) + tt * g.lda + koff;
+    xsi[b] = tt * g.ldas;
+  }
+  const float* const wsc = g.bs + f0 / kGroup * g.ldbs;   // 16 AF divides 128
+  f32x4_t acc[AF][TF];
+#pragma unroll
+  for (int a = 0; a < AF; ++a)
+#pragma unroll
+    for (int b = 0; b < TF; ++b) acc[a][b] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+
+  auto load32 = [&](const uint8_t* p, int64_t k) __attribute__((always_inline)) {
+    // chunks past the last column are zeros (the columns are a multiple of 16)
+    const i32x4_t z = {0, 0, 0, 0};
+    const i32x4_t lo = k + koff < g.R ? *reinterpret_cast<const i32x4_t*>(p + k) : z;
+    const i32x4_t hi = k + koff + 16 < g.R ? *reinterpret_cast<const i32x4_t*>(p + k + 16) : z;
+    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+  };
+  for (int s0 = wave; s0 < nkb; s0 += W * U) {
+    i32x8_t wa[U][AF], xb[U][TF];
+    float sx[U][TF], sw[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int s = s0 + u * W, sc = s < nkb ? s : nkb - 1;
+      const int64_t k = (int64_t)s * kGroup;     // steps past the end load zeros
+#pragma unroll
+      for (int a = 0; a < AF; ++a) wa[u][a] = load32(wp[a], k);
+#pragma unroll
+      for (int b = 0; b < TF; ++b) {
+        xb[u][b] = load32(xp[b], k);
+        sx[u][b] = load_scale(g.as, E8M0 ? MI355Q_SCALE_E8M0 : MI355Q_SCALE_F32, xsi[b] + sc);
+      }
+      sw[u] = wsc[sc];
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (s0 + u * W >= nkb) break;
+#pragma unroll
+      for (int b = 0; b < TF; ++b) {
+        const float s = sx[u][b] * sw[u];
+#pragma unroll
+        for (int a = 0; a < AF; ++a) {
+          f32x4_t t = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            t = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                codes_bf16(wa[u][a][2 * i], wa[u][a][2 * i + 1]), codes_bf16(xb[u][b][2 * i], xb[u][b][2 * i + 1]), t,
+                0, 0, 0);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[a][b][e] = fmaf(t[e], s, acc[a][b][e]);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int a = 0; a < AF; ++a)
+#pragma unroll
+    for (int b = 0; b < TF; ++b) sums[wave][a][b][lane] = acc[a][b];
+  __syncthreads();
+  // wave w finishes tiles w, w + W, ...
+  for (int i = wave; i < AF * TF; i += W) {
+    const int a = i / TF, b = i % TF;
+    f32x4_t v = sums[0][a][b][lane];
+#pragma unroll
+    for (int w = 1; w < W; ++w) v += sums[w][a][b][lane];
+    const int64_t t = 16 * b + (lane & 15), f = f0 + 16 * a + 4 * (lane >> 4);
+    if (t < g.P) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (f + e >= g.Q) continue;
+        const float r = v[e] + (g.bias ? load_typed(g.bias, g.bias_type, f + e) : 0.f);
+        const int64_t o = t * g.ldc + f + e;
+        if (g.c_type == MI355Q_F32) static_cast<float*>(g.c)[o] = r;
+        else static_cast<uint16_t*>(g.c)[o] = g.c_type == MI355Q_BF16 ? Bf16::store(r) : F16::store(r);
+      }
+    }
+  }
+}
+
+// How a forward product runs.
+struct FwdPlan {
+  int shape;        // 0: 256 x 256, 1: 64 x 128
+  uint32_t splits;
+  int steps;        // per split
+};
+static FwdPlan plan_forward(int64_t rows, int64_t out, int64_t cols) {
+  const int nkb = (int)group_count(cols);
+  const int64_t big = ((rows + 255) / 256) * ((out + 255) / 256);
+  FwdPlan p{big >= 192 ? 0 : 1, 1, nkb};
+  if (p.shape == 1) {
+    const int64_t tiles = ((rows + 63) / 64) * ((out + 127) / 128);
+    int64_t s = 512 / tiles;
+    if (s > nkb / 8) s = nkb / 8;
+    if (s > 1) {
+      p.steps = (int)((nkb + s - 1) / s);
+      p.splits = (uint32_t)((nkb + p.steps - 1) / p.steps);
+    }
+  }
+  return p;
+}
+
 template <int KIND>
 static int launch_any(ProductArgs g, mi355q_dtype out, hipStream_t st, const char* who) {
   const int64_t tp = (g.P + GT - 1) / GT, tq = (g.Q + GT - 1) / GT;
@@ -157,11 +674,42 @@ static int launch_any(ProductArgs g, mi355q_dtype out, hipStream_t st, const cha
   return MI355Q_OK;
 }
 
+constexpr int64_t kFewTokens = 64;
+
+template <int TF, int AF, int W, int U>
+static void launch_few_shape(const ProductArgs& g, bool e8, hipStream_t st) {
+  const dim3 grid((unsigned)((g.Q + 16 * AF - 1) / (16 * AF)));
+  if (e8) hipLaunchKernelGGL((fp8_few_kernel<TF, AF, W, U, true>), grid, dim3(64 * W), 0, st, g);
+  else    hipLaunchKernelGGL((fp8_few_kernel<TF, AF, W, U, false>), grid, dim3(64 * W), 0, st, g);
+}
+static void launch_few(const ProductArgs& g, bool e8, hipStream_t st) {
+  if (g.P <= 16) launch_few_shape<1, 1, 4, 4>(g, e8, st);
+  else if (g.P <= 32) launch_few_shape<2, 1, 8, 2>(g, e8, st);
+  else launch_few_shape<4, 2, 8, 1>(g, e8, st);
+}
+
+template <int T, int A, int WT, int WF>
+static int launch_forward(const ProductArgs& g, bool e8, const FwdPlan& p, float* part, hipStream_t st) {
+  using S = FwdShape<T, A, WT, WF>;
+  const int64_t tr = (g.P + S::TT - 1) / S::TT, tc = (g.Q + S::FT - 1) / S::FT;
+  MQ_CHECK_ARG(tr * tc * p.splits < (int64_t(1) << 31), "fp8_block_matmul: output too large");
+  const TileOrder o{(uint32_t)tr, (uint32_t)tc, p.splits};
+  const dim3 grid((unsigned)(tr * tc * p.splits));
+  if (e8) hipLaunchKernelGGL((fp8_forward_kernel<T, A, WT, WF, true>), grid, dim3(S::NTH), 0, st, g, o, p.steps, part);
+  else    hipLaunchKernelGGL((fp8_forward_kernel<T, A, WT, WF, false>), grid, dim3(S::NTH), 0, st, g, o, p.steps, part);
+  MQ_LAUNCH_CHECK();
+  return MI355Q_OK;
+}
+
 }  // namespace mi355q
 
 using namespace mi355q;
 
-extern "C" size_t mi355q_fp8_block_matmul_workspace_size(int64_t, int64_t, int64_t) { return 0; }
+extern "C" size_t mi355q_fp8_block_matmul_workspace_size(int64_t rows, int64_t out, int64_t cols) {
+  if (rows <= kFewTokens || out <= 0 || cols <= 0) return 0;
+  const FwdPlan p = plan_forward(rows, out, cols);
+  return p.splits > 1 ? sizeof(float) * p.splits * rows * out : 0;
+}
 
 extern "C" int mi355q_fp8_block_matmul(const uint8_t* x_dev, int64_t ldx, const void* x_scales_dev,
                                        mi355q_scale_type x_scale_type, int64_t ld_x_scales, const uint8_t* w_dev,
@@ -191,11 +739,41 @@ extern "C" int mi355q_fp8_block_matmul(const uint8_t* x_dev, int64_t ldx, const 
   g.bias = bias_dev;
   g.bias_type = bias_dtype;
   g.c = y_dev;
+  g.c_type = y_dtype;
   g.ldc = ldy;
   g.P = rows;
   g.Q = out;
   g.R = cols;
-  return launch_any<kForward>(g, y_dtype, reinterpret_cast<hipStream_t>(stream), "fp8_block_matmul");
+  const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  // 16-byte loads of whole chunks, and row offsets within a tile in 32 bits
+  const bool aligned = cols % 16 == 0 && ldx % 16 == 0 && ldw % 16 == 0 && aligned16(x_dev) && aligned16(w_dev) &&
+                       ldx < (int64_t(1) << 23) && ldw < (int64_t(1) << 23);
+  if (!aligned) return launch_any<kForward>(g, y_dtype, st, "fp8_block_matmul");
+  const bool e8 = x_scale_type == MI355Q_SCALE_E8M0;
+  if (rows <= kFewTokens) {
+    launch_few(g, e8, st);
+    MQ_LAUNCH_CHECK();
+    return MI355Q_OK;
+  }
+  FwdPlan p = plan_forward(rows, out, cols);
+  float* part = nullptr;
+  if (p.splits > 1) {
+    if (workspace_dev && workspace_bytes >= sizeof(float) * p.splits * rows * out && aligned16(workspace_dev))
+      part = static_cast<float*>(workspace_dev);
+    else
+      p = FwdPlan{p.shape, 1, (int)group_count(cols)};
+  }
+  const int rc = p.shape == 0 ? launch_forward<2, 2, 2, 2>(g, e8, p, part, st)
+                              : launch_forward<1, 2, 2, 2>(g, e8, p, part, st);
+  if (rc != MI355Q_OK) return rc;
+  if (part) {
+    const int64_t n = rows * out;
+    const unsigned grid = (unsigned)((n + 255) / 256 < 4096 ? (n + 255) / 256 : 4096);
+    hipLaunchKernelGGL(sum_splits_kernel, dim3(grid), dim3(256), 0, st, part, (int)p.splits, rows, out, bias_dev,
+                       (int)bias_dtype, y_dev, (int)y_dtype, ldy);
+    MQ_LAUNCH_CHECK();
+  }
+  return MI355Q_OK;
 }
 
 extern "C" size_t mi355q_fp8_block_grad_input_workspace_size(int64_t, int64_t, int64_t) { return 0; }
