@@ -170,14 +170,33 @@ __device__ __forceinline__ void dma_s(uint32_t off, const void* base, uint32_t m
   asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(m0) : "memory", "m0");
 }
 
+// 64 lanes x 1 byte, each as a dword
+__device__ __forceinline__ void dma_bytes(uint32_t off, const void* base, uint32_t m0) {
+  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_ubyte %0, %1" ::"v"(off), "s"(base), "s"(m0) : "memory", "m0");
+}
+
+typedef int i32x2_t __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(3))) i32x2_t lds_i32x2_t;
+typedef short v4s16_t __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) v4s16_t lds_v4s16_t;
+
+// eight codes times a power of two (its exponent is what counts), as bf16
+__device__ __forceinline__ u32x4_t scaled_bf16(uint32_t lo, uint32_t hi, float e) {
+  return u32x4_t{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, e, false)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, e, true)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, e, false)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, e, true))};
+}
+// four tokens of one column each from rows r and r + 4 of PITCH bytes
+template <int PITCH>
+__device__ __forceinline__ bf16x8_t tr_pair(const char* p) {
+  const v4s16_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s16_t*)p);
+  const v4s16_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s16_t*)(p + 4 * PITCH));
+  return __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+}
 // eight codes as bf16
 __device__ __forceinline__ bf16x8_t codes_bf16(uint32_t lo, uint32_t hi) {
-  typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
-  const bf16x2_t a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.f, false);
-  const bf16x2_t b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.f, true);
-  const bf16x2_t c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, false);
-  const bf16x2_t d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, true);
-  return bf16x8_t{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+  return __builtin_bit_cast(bf16x8_t, scaled_bf16(lo, hi, 1.f));
 }
 
 // Work item of a workgroup: the workgroups of one XCD (every eighth) take
@@ -210,6 +229,98 @@ struct FwdShape {
   static constexpr int BIAS = W * 32 * T * PITCH;            // fp32 biases behind it
   static constexpr int LDS = RING > BIAS + FT * 4 ? RING : BIAS + FT * 4;
 };
+
+// Stores a workgroup's tiles acc[A][T] of C [P][Q] (P on the lanes): lane l
+// holds row l & 31 of tile b and, in registers 4 j .. 4 j + 3 of tile a, columns
+// 8 j + 4 (l / 32) and on.  Split sums go to `part` in fp32 without the bias.
+template <class S, int T, int A>
+__device__ __forceinline__ void store_tiles(const ProductArgs& g, f32x16_t (&acc)[A][T], char* ring, int64_t t0, int64_t f0,
+                                            int wt, int wf, int wave, int lane, uint32_t split, float* part) {
+  const int64_t tw = t0 + wt * T * 32, fw = f0 + wf * A * 32;   // the wave's first row and column
+  __syncthreads();   // the ring is no longer read
+  float* const biases = reinterpret_cast<float*>(ring + S::BIAS);
+  for (int i = threadIdx.x; i < S::FT; i += S::NTH)
+    biases[i] = g.bias && !part && f0 + i < g.Q ? load_typed(g.bias, g.bias_type, f0 + i) : 0.f;
+  __syncthreads();
+  const float* const bw = biases + wf * A * 32 + 4 * (lane >> 5);
+  if (part || g.c_type == MI355Q_F32) {
+    float* const out = part ? part + (int64_t)split * g.P * g.Q : static_cast<float*>(g.c);
+    const int64_t ld = part ? g.Q : g.ldc;
+    const bool wide = ld % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+#pragma unroll
+    for (int a = 0; a < A; ++a)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int64_t f = fw + 32 * a + 8 * j + 4 * (lane >> 5);
+        const f32x4_t bias = *reinterpret_cast<const f32x4_t*>(bw + 32 * a + 8 * j);
+#pragma unroll
+        for (int b = 0; b < T; ++b) {
+          const int64_t t = tw + 32 * b + (lane & 31);
+          const f32x4_t v = f32x4_t{acc[a][b][4 * j], acc[a][b][4 * j + 1], acc[a][b][4 * j + 2],
+                                    acc[a][b][4 * j + 3]} + bias;
+          if (t < g.P) {
+            float* o = out + t * ld + f;
+            if (wide && f + 4 <= g.Q) {
+              *reinterpret_cast<f32x4_t*>(o) = v;
+            } else {
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (f + e < g.Q) o[e] = v[e];
+            }
+          }
+        }
+      }
+    return;
+  }
+  // 16-bit outputs through LDS, so that a token's features leave as 16-byte
+  // stores of whole lines (straight from the tiles they are 16-byte pieces)
+  char* const stage = ring + wave * 32 * T * S::PITCH;
+  const bool bf = g.c_type == MI355Q_BF16;
+#pragma unroll
+  for (int a = 0; a < A; ++a)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const f32x4_t bias = *reinterpret_cast<const f32x4_t*>(bw + 32 * a + 8 * j);
+#pragma unroll
+      for (int b = 0; b < T; ++b) {
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = acc[a][b][4 * j + e] + bias[e];
+        uint32_t lo, hi;
+        if (bf) {
+          lo = Bf16::store(v[0]) | (uint32_t)Bf16::store(v[1]) << 16;
+          hi = Bf16::store(v[2]) | (uint32_t)Bf16::store(v[3]) << 16;
+        } else {
+          lo = F16::store(v[0]) | (uint32_t)F16::store(v[1]) << 16;
+          hi = F16::store(v[2]) | (uint32_t)F16::store(v[3]) << 16;
+        }
+        uint32_t* o = reinterpret_cast<uint32_t*>(stage + (32 * b + (lane & 31)) * S::PITCH + 64 * a + 16 * j +
+                                                  8 * (lane >> 5));
+        o[0] = lo;
+        o[1] = hi;
+      }
+    }
+  __syncthreads();
+  constexpr int LPR = 4 * A, RPI = 64 / LPR;   // lanes per row, rows per pass
+  uint16_t* const out = static_cast<uint16_t*>(g.c);
+  const bool wide = g.ldc % 8 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+  const int64_t f = fw + 8 * (lane % LPR);
+#pragma unroll
+  for (int i = 0; i < 32 * T / RPI; ++i) {
+    const int r = i * RPI + lane / LPR;
+    const u32x4_t v = *reinterpret_cast<const u32x4_t*>(stage + r * S::PITCH + 16 * (lane % LPR));
+    if (tw + r < g.P) {
+      uint16_t* o = out + (tw + r) * g.ldc + f;
+      if (wide && f + 8 <= g.Q) {
+        *reinterpret_cast<u32x4_t*>(o) = v;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (f + e < g.Q) o[e] = (uint16_t)(v[e >> 1] >> (16 * (e & 1)));
+      }
+    }
+  }
+}
 
 template <int T, int A, int WT, int WF, bool E8M0>
 __global__ __launch_bounds__(64 * WT * WF) __attribute__((amdgpu_waves_per_eu(2)))
@@ -429,91 +540,450 @@ void fp8_forward_kernel(ProductArgs g, TileOrder order, int steps_per_split, flo
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // before the ring is used again
   }
 
-  // lane l holds token l & 31 and, in registers 4 j .. 4 j + 3 of a tile,
-  // features 8 j + 4 (l / 32) and on
-  const int64_t tw = t0 + wt * T * 32, fw = f0 + wf * A * 32;   // the wave's first token and feature
-  __syncthreads();   // the ring is no longer read
-  float* const biases = reinterpret_cast<float*>(ring + S::BIAS);
-  for (int i = threadIdx.x; i < S::FT; i += S::NTH)
-    biases[i] = g.bias && !part && f0 + i < g.Q ? load_typed(g.bias, g.bias_type, f0 + i) : 0.f;
-  __syncthreads();
-  const float* const bw = biases + wf * A * 32 + 4 * (lane >> 5);
-  if (part || g.c_type == MI355Q_F32) {
-    float* const out = part ? part + (int64_t)split * g.P * g.Q : static_cast<float*>(g.c);
-    const int64_t ld = part ? g.Q : g.ldc;
-    const bool wide = ld % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+  store_tiles<S, T, A>(g, acc, ring, t0, f0, wt, wf, wave, lane, split, part);
+}
+
+// ---------------------------------------------------------------- input gradient
+// As the forward product, with dY's rows (bf16, n contiguous) as the tokens and
+// the weight's 32 x 16 operands taken from its rows as they lie: the transposing
+// LDS load ds_read_b64_tr_b8 gives lane l of a group of 16 column l of the eight
+// rows whose 16-byte pieces the lane pairs point to, that is eight n of one k,
+// which are converted to bf16 in registers.  A step is 64 n; the tiles' sums
+// run over the two steps of a 128 x 128 block before they take its scale.
+template <int T, int WT>
+struct GradInputShape {
+  static constexpr int A = 2, WF = 2;                        // 128 columns: one block scale per workgroup
+  static constexpr int W = WT * WF, NTH = 64 * W;
+  static constexpr int TT = 32 * T * WT, FT = 32 * A * WF, SN = 64;
+  static constexpr int A_SLOT = SN * FT, B_SLOT = TT * SN * 2, NAS = 4, NBS = 3;
+  static constexpr int RING = NAS * A_SLOT + NBS * B_SLOT;
+  static constexpr int PITCH = A * 64 + 16;
+  static constexpr int BIAS = W * 32 * T * PITCH;
+  static constexpr int LDS = RING > BIAS + FT * 4 ? RING : BIAS + FT * 4;
+};
+
+template <int T, int WT>
+__global__ __launch_bounds__(128 * WT) __attribute__((amdgpu_waves_per_eu(2)))
+void fp8_grad_input_kernel(ProductArgs g, TileOrder order, int blocks_per_split, float* part) {
+  using S = GradInputShape<T, WT>;
+  constexpr int A = S::A;
+  __shared__ __attribute__((aligned(16))) char ring[S::LDS];
+  char* const ringb = ring + S::NAS * S::A_SLOT;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wt = wave % WT, wf = wave / WT;
+  uint32_t tr, tc, split;
+  tile_of(order, blockIdx.x, tr, tc, split);
+  const int64_t t0 = (int64_t)tr * S::TT, f0 = (int64_t)tc * S::FT;
+  const int nst = (int)((g.R + S::SN - 1) / S::SN);
+  const int s_begin = (int)split * blocks_per_split * 2;
+  const int s_end = s_begin + 2 * blocks_per_split < nst ? s_begin + 2 * blocks_per_split : nst;
+
+  // DMA: 8 rows of 128 bytes an instruction (n rows of the weight, token rows of
+  // dY), chunk (l & 7) ^ (row & 7) at position l & 7.  Columns and tokens past the
+  // end repeat the last ones (not stored); n past the end repeat the last weight
+  // row and meet zeros of dY (cleared in LDS; codes hold no infinity, and a
+  // NaN of the last row is in the sum anyway).
+  constexpr int NA = S::SN / 8 / S::W, NB = S::TT / 8 / S::W;
+  static_assert(NA * 8 * S::W == S::SN && NB * 8 * S::W == S::TT, "rows per wave");
+  const int chunk = (lane & 7) ^ (lane >> 3);
+  const int last_rows = (int)(g.R - (int64_t)(nst - 1) * S::SN);
+  const int64_t wcol = f0 + 16 * chunk < g.Q ? f0 + 16 * chunk : g.Q - 16;
+  uint32_t oa[NA], da[NA], ob[NB];
 #pragma unroll
-    for (int a = 0; a < A; ++a)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int64_t f = fw + 32 * a + 8 * j + 4 * (lane >> 5);
-        const f32x4_t bias = *reinterpret_cast<const f32x4_t*>(bw + 32 * a + 8 * j);
-#pragma unroll
-        for (int b = 0; b < T; ++b) {
-          const int64_t t = tw + 32 * b + (lane & 31);
-          const f32x4_t v = f32x4_t{acc[a][b][4 * j], acc[a][b][4 * j + 1], acc[a][b][4 * j + 2],
-                                    acc[a][b][4 * j + 3]} + bias;
-          if (t < g.P) {
-            float* o = out + t * ld + f;
-            if (wide && f + 4 <= g.Q) {
-              *reinterpret_cast<f32x4_t*>(o) = v;
-            } else {
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if (f + e < g.Q) o[e] = v[e];
-            }
-          }
-        }
-      }
-    return;
+  for (int j = 0; j < NA; ++j) {
+    const int r = (wave * NA + j) * 8 + (lane >> 3);
+    oa[j] = (uint32_t)r * (uint32_t)g.ldb + (uint32_t)(wcol - f0);
+    da[j] = r >= last_rows ? (uint32_t)(r - (last_rows - 1)) * (uint32_t)g.ldb : 0u;
+    asm volatile("" : "+v"(oa[j]), "+v"(da[j]));
   }
-  // 16-bit outputs through LDS, so that a token's features leave as 16-byte
-  // stores of whole lines (straight from the tiles they are 16-byte pieces)
-  char* const stage = ring + wave * 32 * T * S::PITCH;
-  const bool bf = g.c_type == MI355Q_BF16;
+#pragma unroll
+  for (int j = 0; j < NB; ++j) {
+    const int64_t r = t0 + (wave * NB + j) * 8 + (lane >> 3);
+    ob[j] = (uint32_t)((r < g.P ? r : g.P - 1) - t0) * (uint32_t)(2 * g.lda) + 16 * chunk;
+    asm volatile("" : "+v"(ob[j]));
+  }
+  const char* const wbase = reinterpret_cast<const char*>(g.b) + f0;
+  const char* const ybase = static_cast<const char*>(g.a) + 2 * t0 * g.lda;
+  const uint32_t la0 = lds_u32(ring) + wave * NA * 1024, lb0 = lds_u32(ringb) + wave * NB * 1024;
+  const int tail = (int)(g.R % S::SN) / 8;
+  const uint32_t dead = tail && chunk >= tail ? 16 * chunk : 0;
+  auto load_a = [&](int s, int slot, int j) __attribute__((always_inline)) {
+    dma_s(oa[j] - (s == nst - 1 ? da[j] : 0u), wbase + (int64_t)s * S::SN * g.ldb,
+          la0 + (uint32_t)(slot % S::NAS) * S::A_SLOT + 1024 * j);
+  };
+  auto load_b = [&](int s, int slot, int j) __attribute__((always_inline)) {
+    dma_s(ob[j] - (s == nst - 1 ? dead : 0u), ybase + (int64_t)s * S::SN * 2,
+          lb0 + (uint32_t)(slot % S::NBS) * S::B_SLOT + 1024 * j);
+  };
+  auto load = [&](int s, int slot) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < NA; ++j) load_a(s, slot, j);
+#pragma unroll
+    for (int j = 0; j < NB; ++j) load_b(s, slot, j);
+  };
+  auto clear_tail = [&](int s) __attribute__((always_inline)) {
+    if (!tail || s != nst - 1) return;
+#pragma unroll
+    for (int i = 0; i < S::TT * 8 / S::NTH; ++i) {
+      const int at = i * S::NTH + (int)threadIdx.x, row = at >> 3;
+      if (((at & 7) ^ (row & 7)) >= tail)
+        *reinterpret_cast<u32x4_t*>(ringb + (s % S::NBS) * S::B_SLOT + at * 16) = u32x4_t{0u, 0u, 0u, 0u};
+    }
+    __syncthreads();
+  };
+
+  // operand reads: slice j of a step is n = 16 j .. 16 j + 15, eight per half wave
+  const int gq = lane >> 4, gi = lane & 15;
+  int pa[A], pb[4];
+#pragma unroll
+  for (int a = 0; a < A; ++a) {
+    pa[a] = (8 * (gq >> 1) + (gi >> 1)) * S::FT + 16 * ((wf * 4 + 2 * a + (gq & 1)) ^ (gi >> 1)) + 8 * (gi & 1);
+    asm volatile("" : "+v"(pa[a]));
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    pb[j] = (wt * T * 32 + (lane & 31)) * 2 * S::SN + 16 * ((2 * j + (lane >> 5)) ^ (lane & 7));
+    asm volatile("" : "+v"(pb[j]));
+  }
+  auto read_a = [&](int s, int a, int j) __attribute__((always_inline)) {
+    return __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+        (lds_i32x2_t*)(ring + (s % S::NAS) * S::A_SLOT + j * 16 * S::FT + pa[a]));
+  };
+  auto read_b = [&](int s, int b, int j) __attribute__((always_inline)) {
+    return *reinterpret_cast<const bf16x8_t*>(ringb + (s % S::NBS) * S::B_SLOT + b * 32 * 2 * S::SN + pb[j]);
+  };
+
+  // the block scales of this column of blocks, 64 at a time, one per lane
+  const float* const wsc = g.bs + f0 / kGroup;
+  const int nb = (int)((g.R + kGroup - 1) / kGroup);
+  float scales = 0.f;
+
+  f32x16_t acc[A][T], t[A][T];
 #pragma unroll
   for (int a = 0; a < A; ++a)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const f32x4_t bias = *reinterpret_cast<const f32x4_t*>(bw + 32 * a + 8 * j);
+    for (int b = 0; b < T; ++b)
 #pragma unroll
-      for (int b = 0; b < T; ++b) {
-        float v[4];
+      for (int e = 0; e < 16; ++e) acc[a][b][e] = 0.f;
+  bf16x8_t xb[T][4];
+  i32x2_t ra;
+
+  // Step s: as in the forward product, the barrier before the last row of tiles
+  // publishes step s + 1 (its DMA, two steps old, is waited for; the youngest
+  // step's stays in flight) and frees the slots that step s + 3 takes.
+  auto step = [&](int s, bool first, bool last, float sw) __attribute__((always_inline)) {
+    const int s1 = s + 1 < s_end ? s + 1 : s, s3 = s + 3 < s_end ? s + 3 : s_end - 1;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = acc[a][b][4 * j + e] + bias[e];
-        uint32_t lo, hi;
-        if (bf) {
-          lo = Bf16::store(v[0]) | (uint32_t)Bf16::store(v[1]) << 16;
-          hi = Bf16::store(v[2]) | (uint32_t)Bf16::store(v[3]) << 16;
-        } else {
-          lo = F16::store(v[0]) | (uint32_t)F16::store(v[1]) << 16;
-          hi = F16::store(v[2]) | (uint32_t)F16::store(v[3]) << 16;
-        }
-        uint32_t* o = reinterpret_cast<uint32_t*>(stage + (32 * b + (lane & 31)) * S::PITCH + 64 * a + 16 * j +
-                                                  8 * (lane >> 5));
-        o[0] = lo;
-        o[1] = hi;
+    for (int a = 0; a < A; ++a) {
+      if (a == A - 1) {
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(NA + NB) : "memory");
+        if (s1 != s) clear_tail(s1);
+        __builtin_amdgcn_sched_barrier(0);
       }
-    }
-  __syncthreads();
-  constexpr int LPR = 4 * A, RPI = 64 / LPR;   // lanes per row, rows per pass
-  uint16_t* const out = static_cast<uint16_t*>(g.c);
-  const bool wide = g.ldc % 8 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
-  const int64_t f = fw + 8 * (lane % LPR);
+      if (first)
 #pragma unroll
-  for (int i = 0; i < 32 * T / RPI; ++i) {
-    const int r = i * RPI + lane / LPR;
-    const u32x4_t v = *reinterpret_cast<const u32x4_t*>(stage + r * S::PITCH + 16 * (lane % LPR));
-    if (tw + r < g.P) {
-      uint16_t* o = out + (tw + r) * g.ldc + f;
-      if (wide && f + 8 <= g.Q) {
+        for (int b = 0; b < T; ++b)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) t[a][b][e] = 0.f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const bf16x8_t f = codes_bf16(ra[0], ra[1]);
+        ra = j < 3 ? read_a(s, a, j + 1) : a < A - 1 ? read_a(s, a + 1, 0) : read_a(s + 1, 0, 0);
+#pragma unroll
+        for (int b = 0; b < T; ++b) t[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f, xb[b][j], t[a][b], 0, 0, 0);
+        if (a == A - 1) {
+#pragma unroll
+          for (int b = 0; b < T; ++b) xb[b][j] = read_b(s + 1, b, j);
+#pragma unroll
+          for (int i = 0; i < NA; ++i)
+            if (i * 4 / NA == j) load_a(s3, s + 3, i);
+#pragma unroll
+          for (int i = 0; i < NB; ++i)
+            if (i * 4 / NB == j) load_b(s3, s + 3, i);
+        }
+      }
+      if (last)
+#pragma unroll
+        for (int b = 0; b < T; ++b) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) acc[a][b][e] = fmaf(t[a][b][e], sw, acc[a][b][e]);
+          asm volatile("" : "+v"(acc[a][b]));
+        }
+    }
+  };
+
+  const int s_last = s_end - 1;
+  load(s_begin, s_begin);
+  load(s_begin + 1 < s_end ? s_begin + 1 : s_last, s_begin + 1);
+  load(s_begin + 2 < s_end ? s_begin + 2 : s_last, s_begin + 2);
+  asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(2 * (NA + NB)) : "memory");
+  clear_tail(s_begin);
+  ra = read_a(s_begin, 0, 0);
+#pragma unroll
+  for (int b = 0; b < T; ++b)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) xb[b][j] = read_b(s_begin, b, j);
+  for (int s = s_begin; s < s_end; s += 2) {
+    const int blk = s >> 1, rel = blk - (s_begin >> 1);
+    if ((rel & 63) == 0) {
+      const int i = blk + lane < nb ? blk + lane : nb - 1;
+      scales = wsc[(int64_t)i * g.ldbs];
+    }
+    const float sw = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(scales), rel & 63));
+    if (s + 1 < s_end) {
+      step(s, true, false, sw);
+      step(s + 1, false, true, sw);
+    } else {
+      step(s, true, true, sw);
+    }
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // before the ring is used again
+  store_tiles<S, T, A>(g, acc, ring, t0, f0, wt, wf, wave, lane, split, part);
+}
+
+// ---------------------------------------------------------------- weight gradient
+// C[n][k] over tokens m: both operands are needed with m contiguous and lie with m
+// as the row, so both come from LDS through the transposing load
+// ds_read_b64_tr_b16: lane l = 16 g + 4 q + r receives element r of the 8-byte rows
+// that lanes 16 g + 4 e + q, e = 0..3 point to; two of them are eight tokens of
+// one column.  Rows are stored with their 16-byte chunks XORed by 4 (row & 3),
+// which keeps reads and writes free of bank conflicts.  dY goes to LDS as it is
+// (DMA); the checkpoint's scale changes with the token, along the sum, so it has
+// to be in the operand: each wave's DMA brings codes and scale bytes of its own
+// rows, and the wave writes them to LDS as bf16, scaled by the conversion (exact).
+// The MFMAs then add straight into the accumulators.
+template <int MB, int NB2, int WK, int WN>
+struct GradWeightShape {
+  static constexpr int W = WK * WN, NTH = 64 * W;
+  static constexpr int FK = 32 * MB * WK, FN = 32 * NB2 * WN, SM = 32;   // k, n per workgroup, tokens per stage
+  static constexpr int X_SLOT = SM * FK * 2, Y_SLOT = SM * FN * 2, NXS = 3, NYS = 4;
+  static constexpr int RAW = 1024 + 256, NRS = 4;             // a wave's codes and scale bytes (as dwords)
+  static constexpr int RING = NXS * X_SLOT + NYS * Y_SLOT + W * NRS * RAW;
+  static constexpr int PITCH = 32 * MB * 4 + 16;              // bytes per staged output row (fp32)
+  static constexpr int STAGED = W * 32 * PITCH;
+  static constexpr int LDS = RING > STAGED ? RING : STAGED;
+  static_assert(SM * FK == NTH * 16, "one 16-byte chunk of codes per thread and stage");
+};
+
+template <int MB, int NB2, int WK, int WN>
+__global__ __launch_bounds__(64 * WK * WN) __attribute__((amdgpu_waves_per_eu(2)))
+void fp8_grad_weight_kernel(ProductArgs g, TileOrder order, int stages_per_split, float* part) {
+  using S = GradWeightShape<MB, NB2, WK, WN>;
+  __shared__ __attribute__((aligned(16))) char ring[S::LDS];
+  char* const ringy = ring + S::NXS * S::X_SLOT;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  char* const raw = ringy + S::NYS * S::Y_SLOT + wave * S::NRS * S::RAW;
+  const int wn = wave % WN, wk = wave / WN;
+  uint32_t tn, tk, split;
+  tile_of(order, blockIdx.x, tn, tk, split);
+  const int64_t n0 = (int64_t)tn * S::FN, k0 = (int64_t)tk * S::FK;
+  const int nst = (int)((g.R + S::SM - 1) / S::SM);
+  const int s_begin = (int)split * stages_per_split;
+  const int s_end = s_begin + stages_per_split < nst ? s_begin + stages_per_split : nst;
+  const int last_rows = (int)(g.R - (int64_t)(nst - 1) * S::SM);   // tokens of the last stage
+
+  // DMA of dY: 1 KB an instruction, RPI rows; n past the end repeat the last ones
+  // (not stored), tokens past the end the last one (cleared in LDS, as are
+  // their checkpoint rows: an infinity there must not meet a zero).
+  constexpr int YC = S::FN / 8, RPI = 64 / YC, NY = S::SM / RPI / S::W;
+  uint32_t oy[NY], dy[NY];
+#pragma unroll
+  for (int j = 0; j < NY; ++j) {
+    const int row = (wave * NY + j) * RPI + lane / YC;
+    const int64_t col = n0 + 8 * ((lane % YC) ^ (4 * (row & 3))), c = col < g.P ? col : g.P - 8;
+    oy[j] = (uint32_t)row * (uint32_t)(2 * g.lda) + (uint32_t)(2 * (c - n0));
+    dy[j] = row >= last_rows ? (uint32_t)(row - (last_rows - 1)) * (uint32_t)(2 * g.lda) : 0u;
+    asm volatile("" : "+v"(oy[j]), "+v"(dy[j]));
+  }
+  // ... of the checkpoint: lane l takes 16 codes of row XR l / XC of the wave's
+  constexpr int XC = S::FK / 16, XR = 64 / XC;
+  const int xrow = wave * XR + lane / XC, xch = lane % XC;
+  const int64_t xcol = k0 + 16 * xch < g.Q ? k0 + 16 * xch : g.Q - 16;
+  uint32_t ox = (uint32_t)xrow * (uint32_t)g.ldb + (uint32_t)(xcol - k0);
+  uint32_t oe = (uint32_t)xrow * (uint32_t)g.ldbs + (uint32_t)(xcol / kGroup - k0 / kGroup);
+  const int xpast = xrow >= last_rows ? xrow - (last_rows - 1) : 0;
+  uint32_t dx = (uint32_t)xpast * (uint32_t)g.ldb, de = (uint32_t)xpast * (uint32_t)g.ldbs;
+  asm volatile("" : "+v"(ox), "+v"(oe), "+v"(dx), "+v"(de));
+  const char* const ybase = static_cast<const char*>(g.a) + 2 * n0;
+  const char* const xbase = reinterpret_cast<const char*>(g.b) + k0;
+  const char* const ebase = reinterpret_cast<const char*>(g.be) + k0 / kGroup;
+  const uint32_t ly0 = lds_u32(ringy) + wave * NY * 1024, lr0 = lds_u32(raw);
+  auto load_y = [&](int s, int slot, int j) __attribute__((always_inline)) {
+    dma_s(oy[j] - (s == nst - 1 ? dy[j] : 0u), ybase + (int64_t)s * S::SM * 2 * g.lda,
+          ly0 + (uint32_t)(slot % S::NYS) * S::Y_SLOT + 1024 * j);
+  };
+  auto load_x = [&](int s, int slot) __attribute__((always_inline)) {
+    const uint32_t m0 = lr0 + (uint32_t)(slot % S::NRS) * S::RAW;
+    dma_s(ox - (s == nst - 1 ? dx : 0u), xbase + (int64_t)s * S::SM * g.ldb, m0);
+    dma_bytes(oe - (s == nst - 1 ? de : 0u), ebase + (int64_t)s * S::SM * g.ldbs, m0 + 1024);
+  };
+  constexpr int NDMA = NY + 2;
+  // the wave's rows of stage s as bf16: (byte << 23) | 2^22 is the scale as
+  // the conversion reads it, by its exponent alone (0: the subnormal 2^-127, 255:
+  // NaN)
+  const int xw = xrow * S::FK * 2 + 16 * ((2 * xch) ^ (4 * (xrow & 3)));
+  auto convert = [&](int s) __attribute__((always_inline)) {
+    const char* r = raw + (s % S::NRS) * S::RAW;
+    const u32x4_t c = *reinterpret_cast<const u32x4_t*>(r + 16 * lane);
+    const uint32_t byte = *reinterpret_cast<const uint32_t*>(r + 1024 + 4 * lane);
+    const float e = __uint_as_float((byte << 23) | 0x00400000u);
+    const bool past = s == nst - 1 && xpast > 0;
+    u32x4_t lo = scaled_bf16(c[0], c[1], e), hi = scaled_bf16(c[2], c[3], e);
+    if (past || s >= nst) lo = hi = u32x4_t{0u, 0u, 0u, 0u};
+    char* w = ring + (s % S::NXS) * S::X_SLOT + xw;
+    *reinterpret_cast<u32x4_t*>(w) = lo;
+    *reinterpret_cast<u32x4_t*>(w + 16) = hi;
+  };
+  auto clear_tail = [&](int s) __attribute__((always_inline)) {
+    if (last_rows == S::SM || s != nst - 1) return;
+    char* y = ringy + (s % S::NYS) * S::Y_SLOT;
+    for (int i = last_rows * YC + (int)threadIdx.x; i < S::SM * YC; i += S::NTH)
+      *reinterpret_cast<u32x4_t*>(y + 16 * i) = u32x4_t{0u, 0u, 0u, 0u};
+    __syncthreads();
+  };
+
+  // operand reads: lane 16 g + 4 e + q points to row 8 (g / 2) + e (and + 4) of a
+  // 16-token slice, columns 16 (g & 1) + 4 q of the 32-column block
+  const int gg = lane >> 4, ee = (lane >> 2) & 3, qq = lane & 3;
+  int px[MB], py[NB2];
+#pragma unroll
+  for (int b = 0; b < MB; ++b) {
+    px[b] = (8 * (gg >> 1) + ee) * S::FK * 2 + 8 * (qq & 1) +
+            16 * ((4 * ((MB * wk + b) ^ ee)) + 2 * (gg & 1) + (qq >> 1));
+    asm volatile("" : "+v"(px[b]));
+  }
+#pragma unroll
+  for (int b = 0; b < NB2; ++b) {
+    py[b] = (8 * (gg >> 1) + ee) * S::FN * 2 + 8 * (qq & 1) +
+            16 * ((4 * ((NB2 * wn + b) ^ ee)) + 2 * (gg & 1) + (qq >> 1));
+    asm volatile("" : "+v"(py[b]));
+  }
+  auto read_x = [&](int s, int kk, int b) __attribute__((always_inline)) {
+    return tr_pair<S::FK * 2>(ring + (s % S::NXS) * S::X_SLOT + kk * 16 * S::FK * 2 + px[b]);
+  };
+  auto read_y = [&](int s, int kk, int b) __attribute__((always_inline)) {
+    return tr_pair<S::FN * 2>(ringy + (s % S::NYS) * S::Y_SLOT + kk * 16 * S::FN * 2 + py[b]);
+  };
+
+  f32x16_t acc[MB][NB2];
+#pragma unroll
+  for (int x = 0; x < MB; ++x)
+#pragma unroll
+    for (int y = 0; y < NB2; ++y)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[x][y][e] = 0.f;
+  bf16x8_t fx0[MB], fy0[NB2], fx1[MB], fy1[NB2];
+
+  // Stage s, in two slices of 16 tokens; while one is multiplied the other's
+  // operands are read.  The barrier between them publishes stage s + 1 (dY's DMA
+  // and the converted rows; the checkpoint rows of stage s + 2 have arrived as well)
+  // and frees the slots of stage s - 1.
+  auto stage = [&](int s) __attribute__((always_inline)) {
+    const int s1 = s + 1 < s_end ? s + 1 : s, s3 = s + 3 < s_end ? s + 3 : s_end - 1,
+              s4 = s + 4 < s_end ? s + 4 : s_end - 1;
+#pragma unroll
+    for (int i = 0; i < MB * NB2; ++i) {
+      const int x = i / NB2, y = i % NB2;
+      if (i < NB2) fy1[i] = read_y(s, 1, i);
+      else if (i < NB2 + MB) fx1[i - NB2] = read_x(s, 1, i - NB2);
+      acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fx0[x], fy0[y], acc[x][y], 0, 0, 0);
+    }
+    if constexpr (MB * NB2 < MB + NB2)
+#pragma unroll
+      for (int i = MB * NB2; i < MB + NB2; ++i) fx1[i - NB2] = read_x(s, 1, i - NB2);
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(NDMA) : "memory");
+    if (s1 != s) clear_tail(s1);
+    __builtin_amdgcn_sched_barrier(0);
+    load_x(s4, s + 4);
+    convert(s + 2);
+#pragma unroll
+    for (int i = 0; i < MB * NB2; ++i) {
+      const int x = i / NB2, y = i % NB2;
+      if (i < NB2) fy0[i] = read_y(s + 1, 0, i);
+      else if (i < NB2 + MB) fx0[i - NB2] = read_x(s + 1, 0, i - NB2);
+      acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fx1[x], fy1[y], acc[x][y], 0, 0, 0);
+      if (i < NY) load_y(s3, s + 3, i);
+    }
+    if constexpr (MB * NB2 < MB + NB2)
+#pragma unroll
+      for (int i = MB * NB2; i < MB + NB2; ++i) fx0[i - NB2] = read_x(s + 1, 0, i - NB2);
+  };
+
+  {   // every split has a stage
+    auto at = [&](int s) { return s < s_end ? s : s_end - 1; };
+    load_x(s_begin, s_begin);
+    load_x(at(s_begin + 1), s_begin + 1);
+#pragma unroll
+    for (int j = 0; j < NY; ++j) load_y(s_begin, s_begin, j);
+    load_x(at(s_begin + 2), s_begin + 2);
+#pragma unroll
+    for (int j = 0; j < NY; ++j) load_y(at(s_begin + 1), s_begin + 1, j);
+    load_x(at(s_begin + 3), s_begin + 3);
+#pragma unroll
+    for (int j = 0; j < NY; ++j) load_y(at(s_begin + 2), s_begin + 2, j);
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * NDMA) : "memory");
+    convert(s_begin);
+    convert(s_begin + 1);
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    clear_tail(s_begin);
+#pragma unroll
+    for (int b = 0; b < NB2; ++b) fy0[b] = read_y(s_begin, 0, b);
+#pragma unroll
+    for (int b = 0; b < MB; ++b) fx0[b] = read_x(s_begin, 0, b);
+    for (int s = s_begin; s < s_end; ++s) stage(s);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // before the ring is used again
+  }
+
+  // One row of tiles at a time through LDS: lane l holds column n l & 31 and four
+  // consecutive k a register quad; rows of 32 MB k leave as whole lines.
+  __syncthreads();
+  const bool f32 = part || g.c_type == MI355Q_F32;
+  char* const stage_out = ring + wave * 32 * S::PITCH;
+  const int64_t ld = part ? g.Q : g.ldc;
+  const int es = f32 ? 4 : 2;
+  char* const out = part ? reinterpret_cast<char*>(part + (int64_t)split * g.P * g.Q) : static_cast<char*>(g.c);
+  const bool wide = (ld * es) % 16 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+  const int64_t kw = k0 + wk * MB * 32;
+#pragma unroll
+  for (int y = 0; y < NB2; ++y) {
+#pragma unroll
+    for (int x = 0; x < MB; ++x)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const f32x4_t v = {acc[x][y][4 * j], acc[x][y][4 * j + 1], acc[x][y][4 * j + 2], acc[x][y][4 * j + 3]};
+        char* o = stage_out + (lane & 31) * S::PITCH + (32 * x + 8 * j + 4 * (lane >> 5)) * es;
+        if (f32) {
+          *reinterpret_cast<f32x4_t*>(o) = v;
+        } else if (g.c_type == MI355Q_BF16) {
+          reinterpret_cast<uint32_t*>(o)[0] = Bf16::store(v[0]) | (uint32_t)Bf16::store(v[1]) << 16;
+          reinterpret_cast<uint32_t*>(o)[1] = Bf16::store(v[2]) | (uint32_t)Bf16::store(v[3]) << 16;
+        } else {
+          reinterpret_cast<uint32_t*>(o)[0] = F16::store(v[0]) | (uint32_t)F16::store(v[1]) << 16;
+          reinterpret_cast<uint32_t*>(o)[1] = F16::store(v[2]) | (uint32_t)F16::store(v[3]) << 16;
+        }
+      }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the wave's own region
+    const int per = 16 / es, lpr = 32 * MB / per, rpi = 64 / lpr;   // elements per lane, lanes per row, rows per pass
+    const int64_t k = kw + per * (lane % lpr), nw = n0 + (wn * NB2 + y) * 32;
+    for (int r = lane / lpr; r < 32; r += rpi) {
+      const u32x4_t v = *reinterpret_cast<const u32x4_t*>(stage_out + r * S::PITCH + 16 * (lane % lpr));
+      if (nw + r >= g.P) break;
+      char* o = out + ((nw + r) * ld + k) * es;
+      if (wide && k + per <= g.Q) {
         *reinterpret_cast<u32x4_t*>(o) = v;
+      } else if (f32) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (k + e < g.Q) reinterpret_cast<uint32_t*>(o)[e] = v[e];
       } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-          if (f + e < g.Q) o[e] = (uint16_t)(v[e >> 1] >> (16 * (e & 1)));
+          if (k + e < g.Q) reinterpret_cast<uint16_t*>(o)[e] = (uint16_t)(v[e >> 1] >> (16 * (e & 1)));
       }
     }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   }
 }
 
@@ -638,26 +1108,49 @@ __global__ __launch_bounds__(64 * W) void fp8_few_kernel(ProductArgs g) {
   }
 }
 
-// How a forward product runs.
-struct FwdPlan {
-  int shape;        // 0: 256 x 256, 1: 64 x 128
+// How a product is cut: row and column tiles, and splits of the sum where the
+// tiles leave CUs idle.
+struct Plan {
+  int big;            // the larger tile
   uint32_t splits;
-  int steps;        // per split
+  int steps;          // steps of the sum per split
 };
-static FwdPlan plan_forward(int64_t rows, int64_t out, int64_t cols) {
-  const int nkb = (int)group_count(cols);
-  const int64_t big = ((rows + 255) / 256) * ((out + 255) / 256);
-  FwdPlan p{big >= 192 ? 0 : 1, 1, nkb};
-  if (p.shape == 1) {
-    const int64_t tiles = ((rows + 63) / 64) * ((out + 127) / 128);
-    int64_t s = 512 / tiles;
-    if (s > nkb / 8) s = nkb / 8;
-    if (s > 1) {
-      p.steps = (int)((nkb + s - 1) / s);
-      p.splits = (uint32_t)((nkb + p.steps - 1) / p.steps);
-    }
+// `small` tiles of the output and `steps` of the sum: splits of at least
+// `least` steps until the CUs have two workgroups each
+static Plan split_plan(int big, int64_t tiles, int64_t steps, int64_t least) {
+  Plan p{big, 1, (int)steps};
+  int64_t s = 512 / tiles;
+  if (s > steps / least) s = steps / least;
+  if (s > 1) {
+    p.steps = (int)((steps + s - 1) / s);
+    p.splits = (uint32_t)((steps + p.steps - 1) / p.steps);
   }
   return p;
+}
+static int64_t tiles_of(int64_t rows, int64_t cols, int64_t tr, int64_t tc) {
+  return ((rows + tr - 1) / tr) * ((cols + tc - 1) / tc);
+}
+// forward and input gradient: `rows` tokens by `cols` columns, `sum` terms
+static Plan plan_tokens(int64_t rows, int64_t cols, int64_t sum) {
+  const int64_t big = tiles_of(rows, cols, 128, 128);
+  if (big >= 384) return split_plan(1, big, group_count(sum), 8);
+  return split_plan(0, tiles_of(rows, cols, 64, 128), group_count(sum), 8);
+}
+static Plan plan_weight(int64_t rows, int64_t out, int64_t cols) {
+  const int64_t big = tiles_of(out, cols, 256, 256), stages = (rows + 31) / 32;
+  if (big >= 192) return split_plan(1, 2 * big, stages, 64);
+  return split_plan(0, tiles_of(out, cols, 128, 128), stages, 8);
+}
+static size_t plan_bytes(const Plan& p, int64_t rows, int64_t cols) {
+  return p.splits > 1 ? sizeof(float) * p.splits * rows * cols : 0;
+}
+// the splits' partial sums, or null and an unsplit plan without room for them
+static float* plan_workspace(Plan& p, int64_t rows, int64_t cols, int64_t steps, void* ws, size_t bytes) {
+  if (p.splits <= 1) return nullptr;
+  if (ws && bytes >= plan_bytes(p, rows, cols) && aligned16(ws)) return static_cast<float*>(ws);
+  p.splits = 1;
+  p.steps = (int)steps;
+  return nullptr;
 }
 
 template <int KIND>
@@ -688,18 +1181,49 @@ static void launch_few(const ProductArgs& g, bool e8, hipStream_t st) {
   else launch_few_shape<4, 2, 8, 1>(g, e8, st);
 }
 
-template <int T, int A, int WT, int WF>
-static int launch_forward(const ProductArgs& g, bool e8, const FwdPlan& p, float* part, hipStream_t st) {
-  using S = FwdShape<T, A, WT, WF>;
-  const int64_t tr = (g.P + S::TT - 1) / S::TT, tc = (g.Q + S::FT - 1) / S::FT;
-  MQ_CHECK_ARG(tr * tc * p.splits < (int64_t(1) << 31), "fp8_block_matmul: output too large");
-  const TileOrder o{(uint32_t)tr, (uint32_t)tc, p.splits};
-  const dim3 grid((unsigned)(tr * tc * p.splits));
-  if (e8) hipLaunchKernelGGL((fp8_forward_kernel<T, A, WT, WF, true>), grid, dim3(S::NTH), 0, st, g, o, p.steps, part);
-  else    hipLaunchKernelGGL((fp8_forward_kernel<T, A, WT, WF, false>), grid, dim3(S::NTH), 0, st, g, o, p.steps, part);
+// Cuts C [rows][cols] into TR x TC tiles, runs `kernel(grid, order)` and adds up the splits.
+template <class Kernel>
+static int launch_tiles(const ProductArgs& g, int64_t tile_rows, int64_t tile_cols, const Plan& p, float* part,
+                        hipStream_t st, const char* who, Kernel&& kernel) {
+  const int64_t tr = (g.P + tile_rows - 1) / tile_rows, tc = (g.Q + tile_cols - 1) / tile_cols;
+  MQ_CHECK_ARG(tr * tc * p.splits < (int64_t(1) << 31), "%s: output too large", who);
+  kernel(dim3((unsigned)(tr * tc * p.splits)), TileOrder{(uint32_t)tr, (uint32_t)tc, p.splits});
   MQ_LAUNCH_CHECK();
+  if (part) {
+    const int64_t n = g.P * g.Q;
+    const unsigned grid = (unsigned)((n + 255) / 256 < 4096 ? (n + 255) / 256 : 4096);
+    hipLaunchKernelGGL(sum_splits_kernel, dim3(grid), dim3(256), 0, st, part, (int)p.splits, g.P, g.Q, g.bias,
+                       g.bias_type, g.c, g.c_type, g.ldc);
+    MQ_LAUNCH_CHECK();
+  }
   return MI355Q_OK;
 }
+
+template <int T, int A, int WT, int WF>
+static int launch_forward(const ProductArgs& g, bool e8, const Plan& p, float* part, hipStream_t st) {
+  using S = FwdShape<T, A, WT, WF>;
+  return launch_tiles(g, S::TT, S::FT, p, part, st, "fp8_block_matmul", [&](dim3 grid, TileOrder o) {
+    if (e8) hipLaunchKernelGGL((fp8_forward_kernel<T, A, WT, WF, true>), grid, dim3(S::NTH), 0, st, g, o, p.steps, part);
+    else    hipLaunchKernelGGL((fp8_forward_kernel<T, A, WT, WF, false>), grid, dim3(S::NTH), 0, st, g, o, p.steps, part);
+  });
+}
+template <int T, int WT>
+static int launch_grad_input(const ProductArgs& g, const Plan& p, float* part, hipStream_t st) {
+  using S = GradInputShape<T, WT>;
+  return launch_tiles(g, S::TT, S::FT, p, part, st, "fp8_block_grad_input", [&](dim3 grid, TileOrder o) {
+    hipLaunchKernelGGL((fp8_grad_input_kernel<T, WT>), grid, dim3(S::NTH), 0, st, g, o, p.steps, part);
+  });
+}
+template <int MB, int NB2, int WK, int WN>
+static int launch_grad_weight(const ProductArgs& g, const Plan& p, float* part, hipStream_t st) {
+  using S = GradWeightShape<MB, NB2, WK, WN>;
+  return launch_tiles(g, S::FN, S::FK, p, part, st, "fp8_block_grad_weight", [&](dim3 grid, TileOrder o) {
+    hipLaunchKernelGGL((fp8_grad_weight_kernel<MB, NB2, WK, WN>), grid, dim3(S::NTH), 0, st, g, o, p.steps, part);
+  });
+}
+
+// row offsets within a tile and a stage in 32 bits
+static bool small_pitch(int64_t ld) { return ld < (int64_t(1) << 22); }
 
 }  // namespace mi355q
 
@@ -707,8 +1231,7 @@ using namespace mi355q;
 
 extern "C" size_t mi355q_fp8_block_matmul_workspace_size(int64_t rows, int64_t out, int64_t cols) {
   if (rows <= kFewTokens || out <= 0 || cols <= 0) return 0;
-  const FwdPlan p = plan_forward(rows, out, cols);
-  return p.splits > 1 ? sizeof(float) * p.splits * rows * out : 0;
+  return plan_bytes(plan_tokens(rows, out, cols), rows, out);
 }
 
 extern "C" int mi355q_fp8_block_matmul(const uint8_t* x_dev, int64_t ldx, const void* x_scales_dev,
@@ -747,7 +1270,7 @@ extern "C" int mi355q_fp8_block_matmul(const uint8_t* x_dev, int64_t ldx, const 
   const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   // 16-byte loads of whole chunks, and row offsets within a tile in 32 bits
   const bool aligned = cols % 16 == 0 && ldx % 16 == 0 && ldw % 16 == 0 && aligned16(x_dev) && aligned16(w_dev) &&
-                       ldx < (int64_t(1) << 23) && ldw < (int64_t(1) << 23);
+                       small_pitch(ldx) && small_pitch(ldw);
   if (!aligned) return launch_any<kForward>(g, y_dtype, st, "fp8_block_matmul");
   const bool e8 = x_scale_type == MI355Q_SCALE_E8M0;
   if (rows <= kFewTokens) {
@@ -755,28 +1278,15 @@ extern "C" int mi355q_fp8_block_matmul(const uint8_t* x_dev, int64_t ldx, const 
     MQ_LAUNCH_CHECK();
     return MI355Q_OK;
   }
-  FwdPlan p = plan_forward(rows, out, cols);
-  float* part = nullptr;
-  if (p.splits > 1) {
-    if (workspace_dev && workspace_bytes >= sizeof(float) * p.splits * rows * out && aligned16(workspace_dev))
-      part = static_cast<float*>(workspace_dev);
-    else
-      p = FwdPlan{p.shape, 1, (int)group_count(cols)};
-  }
-  const int rc = p.shape == 0 ? launch_forward<2, 2, 2, 2>(g, e8, p, part, st)
-                              : launch_forward<1, 2, 2, 2>(g, e8, p, part, st);
-  if (rc != MI355Q_OK) return rc;
-  if (part) {
-    const int64_t n = rows * out;
-    const unsigned grid = (unsigned)((n + 255) / 256 < 4096 ? (n + 255) / 256 : 4096);
-    hipLaunchKernelGGL(sum_splits_kernel, dim3(grid), dim3(256), 0, st, part, (int)p.splits, rows, out, bias_dev,
-                       (int)bias_dtype, y_dev, (int)y_dtype, ldy);
-    MQ_LAUNCH_CHECK();
-  }
-  return MI355Q_OK;
+  Plan p = plan_tokens(rows, out, cols);
+  float* const part = plan_workspace(p, rows, out, group_count(cols), workspace_dev, workspace_bytes);
+  return p.big ? launch_forward<2, 2, 2, 2>(g, e8, p, part, st) : launch_forward<1, 2, 2, 2>(g, e8, p, part, st);
 }
 
-extern "C" size_t mi355q_fp8_block_grad_input_workspace_size(int64_t, int64_t, int64_t) { return 0; }
+extern "C" size_t mi355q_fp8_block_grad_input_workspace_size(int64_t rows, int64_t out, int64_t cols) {
+  if (rows <= 0 || out <= 0 || cols <= 0) return 0;
+  return plan_bytes(plan_tokens(rows, cols, out), rows, cols);
+}
 
 extern "C" int mi355q_fp8_block_grad_input(const uint16_t* dy_dev, int64_t lddy, const uint8_t* w_dev, int64_t ldw,
                                            const float* w_scales_dev, int64_t ld_w_scales, uint16_t* dx_dev,
@@ -795,14 +1305,25 @@ extern "C" int mi355q_fp8_block_grad_input(const uint16_t* dy_dev, int64_t lddy,
   g.bs = w_scales_dev;
   g.ldbs = ld_w_scales;
   g.c = dx_dev;
+  g.c_type = MI355Q_BF16;
   g.ldc = lddx;
   g.P = rows;
   g.Q = cols;
   g.R = out;
-  return launch_any<kGradInput>(g, MI355Q_BF16, reinterpret_cast<hipStream_t>(stream), "fp8_block_grad_input");
+  const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  // 16-byte loads of whole chunks
+  const bool aligned = cols % 16 == 0 && ldw % 16 == 0 && out % 8 == 0 && lddy % 8 == 0 && aligned16(dy_dev) &&
+                       aligned16(w_dev) && small_pitch(lddy) && small_pitch(ldw);
+  if (!aligned) return launch_any<kGradInput>(g, MI355Q_BF16, st, "fp8_block_grad_input");
+  Plan p = plan_tokens(rows, cols, out);
+  float* const part = plan_workspace(p, rows, cols, group_count(out), workspace_dev, workspace_bytes);
+  return p.big ? launch_grad_input<2, 2>(g, p, part, st) : launch_grad_input<1, 2>(g, p, part, st);
 }
 
-extern "C" size_t mi355q_fp8_block_grad_weight_workspace_size(int64_t, int64_t, int64_t) { return 0; }
+extern "C" size_t mi355q_fp8_block_grad_weight_workspace_size(int64_t rows, int64_t out, int64_t cols) {
+  if (rows <= 0 || out <= 0 || cols <= 0) return 0;
+  return plan_bytes(plan_weight(rows, out, cols), out, cols);
+}
 
 extern "C" int mi355q_fp8_block_grad_weight(const uint16_t* dy_dev, int64_t lddy, const uint8_t* x_dev, int64_t ldx,
                                             const uint8_t* x_scales_dev, int64_t ld_x_scales, void* dw_dev,
@@ -821,9 +1342,17 @@ extern "C" int mi355q_fp8_block_grad_weight(const uint16_t* dy_dev, int64_t lddy
   g.be = x_scales_dev;
   g.ldbs = ld_x_scales;
   g.c = dw_dev;
+  g.c_type = dw_dtype;
   g.ldc = lddw;
   g.P = out;
   g.Q = cols;
   g.R = rows;
-  return launch_any<kGradWeight>(g, dw_dtype, reinterpret_cast<hipStream_t>(stream), "fp8_block_grad_weight");
+  const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  const bool aligned = rows > 0 && cols % 16 == 0 && ldx % 16 == 0 && out % 8 == 0 && lddy % 8 == 0 &&
+                       aligned16(dy_dev) && aligned16(x_dev) && small_pitch(lddy) && small_pitch(ldx) &&
+                       small_pitch(ld_x_scales);
+  if (!aligned) return launch_any<kGradWeight>(g, dw_dtype, st, "fp8_block_grad_weight");
+  Plan p = plan_weight(rows, out, cols);
+  float* const part = plan_workspace(p, out, cols, (rows + 31) / 32, workspace_dev, workspace_bytes);
+  return p.big ? launch_grad_weight<4, 2, 2, 4>(g, p, part, st) : launch_grad_weight<2, 2, 2, 2>(g, p, part, st);
 }

@@ -212,6 +212,46 @@ def test_block_grad_weight(dev, rows, out, cols):
                   dy.double().abs().T @ a.abs(), dtype)
 
 
+# sizes at which the larger tiles run, with ragged edges in every direction
+LARGE = [(2500, 2600, 144), (130, 6200, 4096), (1700, 3800, 272)]
+
+
+def values_gpu(codes, scales):
+    rows = 1 if scales.shape[0] == codes.shape[0] else G
+    n, k = codes.shape
+    return codes.double() * scales.double().repeat_interleave(rows, 0)[:n].repeat_interleave(G, 1)[:, :k]
+
+
+def check_sum_gpu(got, a, b, dtype):
+    """check_sum against a b^T, all on the GPU (64-bit products of torch)."""
+    want, tol = a @ b.T.contiguous(), 2.0 ** -18 * (a.abs() @ b.abs().T.contiguous())
+    assert got.dtype == dtype and got.shape == want.shape
+    assert bool(((got >= (want - tol).to(dtype)) & (got <= (want + tol).to(dtype))).all())
+
+
+@pytest.mark.parametrize("kind", [torch.float32, E8M0])
+@pytest.mark.parametrize("rows,out,cols", LARGE)
+def test_large_products(dev, rows, out, cols, kind):
+    o, g = ops(), torch.Generator(device=dev).manual_seed(rows)
+    x, xs = o.fp8_quantize_groups((torch.randn(rows, cols, generator=g, device=dev) * 3).to(torch.bfloat16), kind)
+    w, ws = o.fp8_quantize_blocks((torch.randn(out, cols, generator=g, device=dev) * 0.02).to(torch.bfloat16))
+    a, b = values_gpu(x, xs), values_gpu(w, ws)
+    for dtype in (torch.bfloat16, torch.float32):
+        check_sum_gpu(o.fp8_block_matmul(x, xs, w, ws, out_dtype=dtype), a, b, dtype)
+    dy = torch.randn(rows, out, generator=g, device=dev).to(torch.bfloat16)
+    check_sum_gpu(o.fp8_block_grad_input(dy, w, ws), dy.double(), b.T, torch.bfloat16)
+
+
+@pytest.mark.parametrize("rows,out,cols", [(77, 3800, 3616), (2100, 3080, 4112), (33, 4096, 4096)])
+def test_large_weight_gradients(dev, rows, out, cols):
+    o, g = ops(), torch.Generator(device=dev).manual_seed(rows)
+    x, xs = o.fp8_quantize_groups((torch.randn(rows, cols, generator=g, device=dev) * 3).to(torch.bfloat16), E8M0)
+    dy = (torch.randn(rows, out, generator=g, device=dev) * 1e-4).to(torch.bfloat16)
+    for dtype in (torch.float32, torch.bfloat16):
+        check_sum_gpu(o.fp8_block_grad_weight(dy, x, xs, dtype), dy.double().T.contiguous(),
+                      values_gpu(x, xs).T.contiguous(), dtype)
+
+
 def test_products_of_strided_operands(dev):
     """Codes and gradients that are views of wider or transposed buffers."""
     o, g = ops(), gen(11)
