@@ -56,4 +56,15 @@ inline bool known_dtype(int dt) { return dt == MI355Q_BF16 || dt == MI355Q_F16 |
 inline int dtype_size(int dt) { return dt == MI355Q_F32 ? 4 : 2; }
 inline bool aligned_to(const void* p, unsigned n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
+// n / d for n < 2^31 without a division: (mulhi(n, mul) + n) >> shift
+struct FastDiv {
+  uint32_t d, mul, shift;
+};
+inline FastDiv fast_div(uint32_t d) {
+  uint32_t l = 0;
+  while ((uint64_t(1) << l) < d) ++l;
+  return {d, (uint32_t)((((uint64_t(1) << l) - d) << 32) / d + 1), l};
+}
+__device__ __forceinline__ uint32_t div(uint32_t n, const FastDiv& f) { return (__umulhi(n, f.mul) + n) >> f.shift; }
+
 }  // namespace mi355q

@@ -146,8 +146,9 @@ __global__ __launch_bounds__(256) void product_any_kernel(ProductArgs g) {
 
 // ---------------------------------------------------------------- forward, tiles
 // Rows of 128 codes (one K step) go global -> LDS by the gfx950 LDS-DMA load
-// with their 16-byte chunks XOR-swizzled by row & 7, so that both the DMA's
-// writes and the operand reads (rows of one chunk) spread over all banks.
+// with their 16-byte chunks XOR-swizzled by (row >> 1) & 7: 16 rows of one
+// chunk then lie in 16 different 16-byte columns of the banks (two rows a
+// 256-byte line of them), which is what a 16-byte read takes at a time.
 //
 // The fp8 matrix instructions would take the codes as they are at twice the
 // rate, but they add with few bits: on heavy-tailed codes up to 2.6e-4 of the
@@ -338,23 +339,23 @@ void fp8_forward_kernel(ProductArgs g, TileOrder order, int steps_per_split, flo
   const int s_end = s_begin + steps_per_split < nkb ? s_begin + steps_per_split : nkb;
 
   // DMA: instruction j of wave w fills 8 rows; lane l the chunk position l & 7
-  // of row l / 8, with the row's chunk (l & 7) ^ (row & 7).  Rows past the end
-  // read the last row again (their results are not stored).
+  // of row l / 8, with the row's chunk (l & 7) ^ ((row >> 1) & 7), the same for
+  // every second j.  Rows past the end read the last row again (their results
+  // are not stored).
   constexpr int NA = S::FT / 8 / S::W, NB = S::TT / 8 / S::W;
   static_assert(NA * 8 * S::W == S::FT && NB * 8 * S::W == S::TT, "rows per wave");
-  const int chunk = (lane & 7) ^ (lane >> 3);
+  static_assert(NA % 2 == 0 && NB % 2 == 0, "a wave's rows begin at a multiple of 16");
+  const int chunk[2] = {(lane & 7) ^ (lane >> 4), (lane & 7) ^ (4 + (lane >> 4))};
   uint32_t oa[NA], ob[NB];
 #pragma unroll
   for (int j = 0; j < NA; ++j) {
     const int64_t r = f0 + (wave * NA + j) * 8 + (lane >> 3);
-    oa[j] = (uint32_t)((r < g.Q ? r : g.Q - 1) - f0) * (uint32_t)g.ldb + 16 * chunk;
-    asm volatile("" : "+v"(oa[j]));   // one register, not re-derived in the loop
+    oa[j] = (uint32_t)((r < g.Q ? r : g.Q - 1) - f0) * (uint32_t)g.ldb + 16 * chunk[j & 1];
   }
 #pragma unroll
   for (int j = 0; j < NB; ++j) {
     const int64_t r = t0 + (wave * NB + j) * 8 + (lane >> 3);
-    ob[j] = (uint32_t)((r < g.P ? r : g.P - 1) - t0) * (uint32_t)g.lda + 16 * chunk;
-    asm volatile("" : "+v"(ob[j]));
+    ob[j] = (uint32_t)((r < g.P ? r : g.P - 1) - t0) * (uint32_t)g.lda + 16 * chunk[j & 1];
   }
   const char* const wbase = reinterpret_cast<const char*>(g.b) + f0 * g.ldb;
   const char* const xbase = static_cast<const char*>(g.a) + t0 * g.lda;
@@ -364,21 +365,26 @@ void fp8_forward_kernel(ProductArgs g, TileOrder order, int steps_per_split, flo
   // in LDS, so that it adds nothing (a NaN in the first chunk is in the row's
   // sum anyway).
   const int tail = (int)(g.R % kGroup) / 16;                    // whole chunks of a short last step
-  const uint32_t dead = tail && chunk >= tail ? 16 * chunk : 0;
+  auto turn_to_tail = [&](int s) __attribute__((always_inline)) {   // once, before the last step's DMA
+    if (tail && s == nkb - 1) {
+#pragma unroll
+      for (int j = 0; j < NA; ++j) oa[j] -= chunk[j & 1] >= tail ? 16 * chunk[j & 1] : 0;
+#pragma unroll
+      for (int j = 0; j < NB; ++j) ob[j] -= chunk[j & 1] >= tail ? 16 * chunk[j & 1] : 0;
+    }
+  };
   auto load_a = [&](int s, int slot, int j) __attribute__((always_inline)) {
-    dma_s(oa[j] - (s == nkb - 1 ? dead : 0u), wbase + (int64_t)s * kGroup,
-          la0 + (uint32_t)(slot % 3) * S::A_SLOT + 1024 * j);
+    dma_s(oa[j], wbase + (int64_t)s * kGroup, la0 + (uint32_t)(slot % 3) * S::A_SLOT + 1024 * j);
   };
   auto load_b = [&](int s, int slot, int j) __attribute__((always_inline)) {
-    dma_s(ob[j] - (s == nkb - 1 ? dead : 0u), xbase + (int64_t)s * kGroup,
-          lb0 + (uint32_t)(slot & 1) * S::B_SLOT + 1024 * j);
+    dma_s(ob[j], xbase + (int64_t)s * kGroup, lb0 + (uint32_t)(slot & 1) * S::B_SLOT + 1024 * j);
   };
   auto clear_tail = [&](int s) __attribute__((always_inline)) {
     if (!tail || s != nkb - 1) return;
 #pragma unroll
     for (int i = 0; i < S::TT * 8 / S::NTH; ++i) {
       const int at = i * S::NTH + (int)threadIdx.x, row = at >> 3;
-      if (((at & 7) ^ (row & 7)) >= tail)
+      if (((at & 7) ^ ((row >> 1) & 7)) >= tail)
         *reinterpret_cast<u32x4_t*>(ringb + (s & 1) * S::B_SLOT + at * 16) = u32x4_t{0u, 0u, 0u, 0u};
     }
     __syncthreads();
@@ -390,7 +396,7 @@ void fp8_forward_kernel(ProductArgs g, TileOrder order, int steps_per_split, flo
   int p[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    p[i] = (lane & 31) * kGroup + 16 * ((4 * (lane >> 5) + i) ^ (lane & 7));
+    p[i] = (lane & 31) * kGroup + 16 * ((4 * (lane >> 5) + i) ^ ((lane >> 1) & 7));
     asm volatile("" : "+v"(p[i]));
   }
   auto read_a = [&](int s, int a, int i) __attribute__((always_inline)) {
@@ -467,6 +473,7 @@ void fp8_forward_kernel(ProductArgs g, TileOrder order, int steps_per_split, flo
         __builtin_amdgcn_sched_barrier(0);
         asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
         if (s1 != s) clear_tail(s1);
+        if (s2 > s1) turn_to_tail(s2);
         // (the scales of step s + 1 were requested a step ago, with the DMA
         // that the wait above is for: a use anywhere else would wait for the
         // DMA issued since)
@@ -515,6 +522,7 @@ void fp8_forward_kernel(ProductArgs g, TileOrder order, int steps_per_split, flo
 
   {   // every split has a step
     const int s1 = s_begin + 1 < s_end ? s_begin + 1 : s_begin;
+    turn_to_tail(s_begin);
 #pragma unroll
     for (int j = 0; j < NA; ++j) load_a(s_begin, s_begin, j);
 #pragma unroll
@@ -524,6 +532,7 @@ void fp8_forward_kernel(ProductArgs g, TileOrder order, int steps_per_split, flo
     clear_tail(s_begin);
     take_scales();
     load_scales(s1);
+    if (s1 > s_begin) turn_to_tail(s1);
 #pragma unroll
     for (int j = 0; j < NA; ++j) load_a(s1, s_begin + 1, j);
 #pragma unroll
@@ -578,42 +587,47 @@ void fp8_grad_input_kernel(ProductArgs g, TileOrder order, int blocks_per_split,
   const int s_begin = (int)split * blocks_per_split * 2;
   const int s_end = s_begin + 2 * blocks_per_split < nst ? s_begin + 2 * blocks_per_split : nst;
 
-  // DMA: 8 rows of 128 bytes an instruction (n rows of the weight, token rows of
-  // dY), chunk (l & 7) ^ (row & 7) at position l & 7.  Columns and tokens past the
+  // DMA: 8 rows of 128 bytes an instruction; n rows of the weight with chunk
+  // (l & 7) ^ (row & 7) at position l & 7 (the eight rows of a transposed read), token
+  // rows of dY with (l & 7) ^ ((row >> 1) & 7), as in the forward product.  Columns and tokens past the
   // end repeat the last ones (not stored); n past the end repeat the last weight
   // row and meet zeros of dY (cleared in LDS; codes hold no infinity, and a
   // NaN of the last row is in the sum anyway).
   constexpr int NA = S::SN / 8 / S::W, NB = S::TT / 8 / S::W;
   static_assert(NA * 8 * S::W == S::SN && NB * 8 * S::W == S::TT, "rows per wave");
-  const int chunk = (lane & 7) ^ (lane >> 3);
+  static_assert(NB % 2 == 0, "a wave's token rows begin at a multiple of 16");
+  const int chunk = (lane & 7) ^ (lane >> 3), ychunk[2] = {(lane & 7) ^ (lane >> 4), (lane & 7) ^ (4 + (lane >> 4))};
   const int last_rows = (int)(g.R - (int64_t)(nst - 1) * S::SN);
   const int64_t wcol = f0 + 16 * chunk < g.Q ? f0 + 16 * chunk : g.Q - 16;
-  uint32_t oa[NA], da[NA], ob[NB];
+  uint32_t oa[NA], ob[NB];
 #pragma unroll
-  for (int j = 0; j < NA; ++j) {
-    const int r = (wave * NA + j) * 8 + (lane >> 3);
-    oa[j] = (uint32_t)r * (uint32_t)g.ldb + (uint32_t)(wcol - f0);
-    da[j] = r >= last_rows ? (uint32_t)(r - (last_rows - 1)) * (uint32_t)g.ldb : 0u;
-    asm volatile("" : "+v"(oa[j]), "+v"(da[j]));
-  }
+  for (int j = 0; j < NA; ++j)
+    oa[j] = (uint32_t)((wave * NA + j) * 8 + (lane >> 3)) * (uint32_t)g.ldb + (uint32_t)(wcol - f0);
 #pragma unroll
   for (int j = 0; j < NB; ++j) {
     const int64_t r = t0 + (wave * NB + j) * 8 + (lane >> 3);
-    ob[j] = (uint32_t)((r < g.P ? r : g.P - 1) - t0) * (uint32_t)(2 * g.lda) + 16 * chunk;
-    asm volatile("" : "+v"(ob[j]));
+    ob[j] = (uint32_t)((r < g.P ? r : g.P - 1) - t0) * (uint32_t)(2 * g.lda) + 16 * ychunk[j & 1];
   }
   const char* const wbase = reinterpret_cast<const char*>(g.b) + f0;
   const char* const ybase = static_cast<const char*>(g.a) + 2 * t0 * g.lda;
   const uint32_t la0 = lds_u32(ring) + wave * NA * 1024, lb0 = lds_u32(ringb) + wave * NB * 1024;
   const int tail = (int)(g.R % S::SN) / 8;
-  const uint32_t dead = tail && chunk >= tail ? 16 * chunk : 0;
+  auto turn_to_tail = [&](int s) __attribute__((always_inline)) {   // once, before the last step's DMA
+    if (tail && s == nst - 1) {
+#pragma unroll
+      for (int j = 0; j < NA; ++j) {
+        const int r = (wave * NA + j) * 8 + (lane >> 3);
+        oa[j] -= r >= last_rows ? (uint32_t)(r - (last_rows - 1)) * (uint32_t)g.ldb : 0u;
+      }
+#pragma unroll
+      for (int j = 0; j < NB; ++j) ob[j] -= ychunk[j & 1] >= tail ? 16 * ychunk[j & 1] : 0;
+    }
+  };
   auto load_a = [&](int s, int slot, int j) __attribute__((always_inline)) {
-    dma_s(oa[j] - (s == nst - 1 ? da[j] : 0u), wbase + (int64_t)s * S::SN * g.ldb,
-          la0 + (uint32_t)(slot % S::NAS) * S::A_SLOT + 1024 * j);
+    dma_s(oa[j], wbase + (int64_t)s * S::SN * g.ldb, la0 + (uint32_t)(slot % S::NAS) * S::A_SLOT + 1024 * j);
   };
   auto load_b = [&](int s, int slot, int j) __attribute__((always_inline)) {
-    dma_s(ob[j] - (s == nst - 1 ? dead : 0u), ybase + (int64_t)s * S::SN * 2,
-          lb0 + (uint32_t)(slot % S::NBS) * S::B_SLOT + 1024 * j);
+    dma_s(ob[j], ybase + (int64_t)s * S::SN * 2, lb0 + (uint32_t)(slot % S::NBS) * S::B_SLOT + 1024 * j);
   };
   auto load = [&](int s, int slot) __attribute__((always_inline)) {
 #pragma unroll
@@ -626,7 +640,7 @@ void fp8_grad_input_kernel(ProductArgs g, TileOrder order, int blocks_per_split,
 #pragma unroll
     for (int i = 0; i < S::TT * 8 / S::NTH; ++i) {
       const int at = i * S::NTH + (int)threadIdx.x, row = at >> 3;
-      if (((at & 7) ^ (row & 7)) >= tail)
+      if (((at & 7) ^ ((row >> 1) & 7)) >= tail)
         *reinterpret_cast<u32x4_t*>(ringb + (s % S::NBS) * S::B_SLOT + at * 16) = u32x4_t{0u, 0u, 0u, 0u};
     }
     __syncthreads();
@@ -642,7 +656,7 @@ void fp8_grad_input_kernel(ProductArgs g, TileOrder order, int blocks_per_split,
   }
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    pb[j] = (wt * T * 32 + (lane & 31)) * 2 * S::SN + 16 * ((2 * j + (lane >> 5)) ^ (lane & 7));
+    pb[j] = (wt * T * 32 + (lane & 31)) * 2 * S::SN + 16 * ((2 * j + (lane >> 5)) ^ ((lane >> 1) & 7));
     asm volatile("" : "+v"(pb[j]));
   }
   auto read_a = [&](int s, int a, int j) __attribute__((always_inline)) {
@@ -679,6 +693,7 @@ void fp8_grad_input_kernel(ProductArgs g, TileOrder order, int blocks_per_split,
         __builtin_amdgcn_sched_barrier(0);
         asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(NA + NB) : "memory");
         if (s1 != s) clear_tail(s1);
+        if (s + 3 < s_end) turn_to_tail(s + 3);
         __builtin_amdgcn_sched_barrier(0);
       }
       if (first)
@@ -714,9 +729,11 @@ void fp8_grad_input_kernel(ProductArgs g, TileOrder order, int blocks_per_split,
   };
 
   const int s_last = s_end - 1;
-  load(s_begin, s_begin);
-  load(s_begin + 1 < s_end ? s_begin + 1 : s_last, s_begin + 1);
-  load(s_begin + 2 < s_end ? s_begin + 2 : s_last, s_begin + 2);
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {
+    if (s_begin + i < s_end) turn_to_tail(s_begin + i);
+    load(s_begin + i < s_end ? s_begin + i : s_last, s_begin + i);
+  }
   asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(2 * (NA + NB)) : "memory");
   clear_tail(s_begin);
   ra = read_a(s_begin, 0, 0);
@@ -724,20 +741,21 @@ void fp8_grad_input_kernel(ProductArgs g, TileOrder order, int blocks_per_split,
   for (int b = 0; b < T; ++b)
 #pragma unroll
     for (int j = 0; j < 4; ++j) xb[b][j] = read_b(s_begin, b, j);
-  for (int s = s_begin; s < s_end; s += 2) {
-    const int blk = s >> 1, rel = blk - (s_begin >> 1);
+  auto scale_of = [&](int blk) __attribute__((always_inline)) {
+    const int rel = blk - (s_begin >> 1);
     if ((rel & 63) == 0) {
       const int i = blk + lane < nb ? blk + lane : nb - 1;
       scales = wsc[(int64_t)i * g.ldbs];
     }
-    const float sw = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(scales), rel & 63));
-    if (s + 1 < s_end) {
-      step(s, true, false, sw);
-      step(s + 1, false, true, sw);
-    } else {
-      step(s, true, true, sw);
-    }
+    return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(scales), rel & 63));
+  };
+  int s = s_begin;
+  for (; s + 1 < s_end; s += 2) {
+    const float sw = scale_of(s >> 1);
+    step(s, true, false, sw);
+    step(s + 1, false, true, sw);
   }
+  if (s < s_end) step(s, true, true, scale_of(s >> 1));   // a last block of 64 n or fewer
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // before the ring is used again
   store_tiles<S, T, A>(g, acc, ring, t0, f0, wt, wf, wave, lane, split, part);
 }
@@ -822,18 +840,24 @@ void fp8_grad_weight_kernel(ProductArgs g, TileOrder order, int stages_per_split
   // the wave's rows of stage s as bf16: (byte << 23) | 2^22 is the scale as
   // the conversion reads it, by its exponent alone (0: the subnormal 2^-127, 255:
   // NaN)
-  const int xw = xrow * S::FK * 2 + 16 * ((2 * xch) ^ (4 * (xrow & 3)));
-  auto convert = [&](int s) __attribute__((always_inline)) {
+  // (half of the lanes write the second half first, so that 8 or 16 neighbouring
+  // lanes write to as many different 16-byte columns of the banks)
+  const int xw = xrow * S::FK * 2 + 16 * ((2 * xch) ^ (4 * (xrow & 3))), xswap = ((lane >> 2) ^ (lane >> 3)) & 1;
+  u32x4_t raw_codes;
+  uint32_t raw_byte;
+  auto fetch = [&](int s) __attribute__((always_inline)) {
     const char* r = raw + (s % S::NRS) * S::RAW;
-    const u32x4_t c = *reinterpret_cast<const u32x4_t*>(r + 16 * lane);
-    const uint32_t byte = *reinterpret_cast<const uint32_t*>(r + 1024 + 4 * lane);
-    const float e = __uint_as_float((byte << 23) | 0x00400000u);
-    const bool past = s == nst - 1 && xpast > 0;
-    u32x4_t lo = scaled_bf16(c[0], c[1], e), hi = scaled_bf16(c[2], c[3], e);
-    if (past || s >= nst) lo = hi = u32x4_t{0u, 0u, 0u, 0u};
+    raw_codes = *reinterpret_cast<const u32x4_t*>(r + 16 * lane);
+    raw_byte = *reinterpret_cast<const uint32_t*>(r + 1024 + 4 * lane);
+  };
+  auto convert = [&](int s) __attribute__((always_inline)) {
+    const float e = __uint_as_float((raw_byte << 23) | 0x00400000u);
+    u32x4_t c = raw_codes;
+    if (s == nst - 1 && xpast > 0) c = u32x4_t{0u, 0u, 0u, 0u};
+    if (xswap) c = u32x4_t{c[2], c[3], c[0], c[1]};
     char* w = ring + (s % S::NXS) * S::X_SLOT + xw;
-    *reinterpret_cast<u32x4_t*>(w) = lo;
-    *reinterpret_cast<u32x4_t*>(w + 16) = hi;
+    *reinterpret_cast<u32x4_t*>(w + 16 * xswap) = scaled_bf16(c[0], c[1], e);
+    *reinterpret_cast<u32x4_t*>(w + 16 * (1 - xswap)) = scaled_bf16(c[2], c[3], e);
   };
   auto clear_tail = [&](int s) __attribute__((always_inline)) {
     if (last_rows == S::SM || s != nst - 1) return;
@@ -882,33 +906,30 @@ void fp8_grad_weight_kernel(ProductArgs g, TileOrder order, int stages_per_split
   auto stage = [&](int s) __attribute__((always_inline)) {
     const int s1 = s + 1 < s_end ? s + 1 : s, s3 = s + 3 < s_end ? s + 3 : s_end - 1,
               s4 = s + 4 < s_end ? s + 4 : s_end - 1;
+    static_assert(MB * NB2 >= MB + NB2, "an MFMA for each operand read");
 #pragma unroll
     for (int i = 0; i < MB * NB2; ++i) {
       const int x = i / NB2, y = i % NB2;
+      acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fx0[x], fy0[y], acc[x][y], 0, 0, 0);
       if (i < NB2) fy1[i] = read_y(s, 1, i);
       else if (i < NB2 + MB) fx1[i - NB2] = read_x(s, 1, i - NB2);
-      acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fx0[x], fy0[y], acc[x][y], 0, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
     }
-    if constexpr (MB * NB2 < MB + NB2)
-#pragma unroll
-      for (int i = MB * NB2; i < MB + NB2; ++i) fx1[i - NB2] = read_x(s, 1, i - NB2);
-    __builtin_amdgcn_sched_barrier(0);
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(NDMA) : "memory");
     if (s1 != s) clear_tail(s1);
     __builtin_amdgcn_sched_barrier(0);
-    load_x(s4, s + 4);
-    convert(s + 2);
+    fetch(s + 2);
 #pragma unroll
     for (int i = 0; i < MB * NB2; ++i) {
       const int x = i / NB2, y = i % NB2;
+      acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fx1[x], fy1[y], acc[x][y], 0, 0, 0);
       if (i < NB2) fy0[i] = read_y(s + 1, 0, i);
       else if (i < NB2 + MB) fx0[i - NB2] = read_x(s + 1, 0, i - NB2);
-      acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fx1[x], fy1[y], acc[x][y], 0, 0, 0);
-      if (i < NY) load_y(s3, s + 3, i);
+      if (i == 0) load_x(s4, s + 4);
+      else if (i <= NY) load_y(s3, s + 3, i - 1);
+      if (i == MB * NB2 - 2) convert(s + 2);
+      __builtin_amdgcn_sched_barrier(0);
     }
-    if constexpr (MB * NB2 < MB + NB2)
-#pragma unroll
-      for (int i = MB * NB2; i < MB + NB2; ++i) fx0[i - NB2] = read_x(s + 1, 0, i - NB2);
   };
 
   {   // every split has a stage
@@ -924,7 +945,9 @@ void fp8_grad_weight_kernel(ProductArgs g, TileOrder order, int stages_per_split
 #pragma unroll
     for (int j = 0; j < NY; ++j) load_y(at(s_begin + 2), s_begin + 2, j);
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * NDMA) : "memory");
+    fetch(s_begin);
     convert(s_begin);
+    fetch(s_begin + 1);
     convert(s_begin + 1);
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     clear_tail(s_begin);
@@ -987,19 +1010,61 @@ void fp8_grad_weight_kernel(ProductArgs g, TileOrder order, int stages_per_split
   }
 }
 
-// Sums the splits' partial products [splits][rows][cols] in order, adds the
-// bias and rounds once.
-__global__ __launch_bounds__(256) void sum_splits_kernel(const float* part, int splits, int64_t rows, int64_t cols,
+// Sums the splits' partial products [splits][rows][cols] in their order, adds
+// the bias and rounds once.  N consecutive columns a thread (4 where they divide
+// the row), four splits' loads in flight.
+template <int N>
+__global__ __launch_bounds__(256) void sum_splits_kernel(const float* part, int splits, int64_t n, FastDiv row,
                                                          const void* bias, int bias_type, void* c, int c_type,
-                                                         int64_t ldc) {
-  const int64_t n = rows * cols;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-    const int64_t r = i / cols, q = i - r * cols;
-    float v = 0.f;
-    for (int s = 0; s < splits; ++s) v += part[s * n + i];
-    if (bias) v += load_typed(bias, bias_type, q);
-    if (c_type == MI355Q_F32) static_cast<float*>(c)[r * ldc + q] = v;
-    else static_cast<uint16_t*>(c)[r * ldc + q] = c_type == MI355Q_BF16 ? Bf16::store(v) : F16::store(v);
+                                                         int64_t ldc, int wide) {
+  typedef float vec_t __attribute__((ext_vector_type(N)));
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;   // in vectors; below 2^31
+  if (i * N >= n) return;
+  const uint32_t r = div((uint32_t)i, row), q = ((uint32_t)i - r * row.d) * N;
+  const float* p = part + i * N;
+  float v[N];
+#pragma unroll
+  for (int e = 0; e < N; ++e) v[e] = 0.f;
+  int s = 0;
+  for (; s + 4 <= splits; s += 4) {
+    vec_t x[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) __builtin_memcpy(&x[u], p + (s + u) * n, 4 * N);
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int e = 0; e < N; ++e) v[e] += x[u][e];
+  }
+  for (; s < splits; ++s) {
+    vec_t x;
+    __builtin_memcpy(&x, p + s * n, 4 * N);
+#pragma unroll
+    for (int e = 0; e < N; ++e) v[e] += x[e];
+  }
+  if (bias)
+#pragma unroll
+    for (int e = 0; e < N; ++e) v[e] += load_typed(bias, bias_type, q + e);
+  const int64_t o = (int64_t)r * ldc + q;
+  if (c_type == MI355Q_F32) {
+    float* d = static_cast<float*>(c) + o;
+    if (N == 4 && wide) {
+      *reinterpret_cast<f32x4_t*>(d) = f32x4_t{v[0], v[N > 1], v[N > 2 ? 2 : 0], v[N > 3 ? 3 : 0]};
+    } else {
+#pragma unroll
+      for (int e = 0; e < N; ++e) d[e] = v[e];
+    }
+    return;
+  }
+  uint16_t h[N];
+#pragma unroll
+  for (int e = 0; e < N; ++e) h[e] = c_type == MI355Q_BF16 ? Bf16::store(v[e]) : F16::store(v[e]);
+  uint16_t* d = static_cast<uint16_t*>(c) + o;
+  if (N == 4 && wide) {
+    *reinterpret_cast<i32x2_t*>(d) = i32x2_t{(int)(h[0] | (uint32_t)h[N > 1] << 16),
+                                             (int)(h[N > 2 ? 2 : 0] | (uint32_t)h[N > 3 ? 3 : 0] << 16)};
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e) d[e] = h[e];
   }
 }
 
@@ -1190,10 +1255,16 @@ static int launch_tiles(const ProductArgs& g, int64_t tile_rows, int64_t tile_co
   kernel(dim3((unsigned)(tr * tc * p.splits)), TileOrder{(uint32_t)tr, (uint32_t)tc, p.splits});
   MQ_LAUNCH_CHECK();
   if (part) {
+    // (a split product has at most 511 tiles of 64 KB elements: fewer than 2^31 vectors)
     const int64_t n = g.P * g.Q;
-    const unsigned grid = (unsigned)((n + 255) / 256 < 4096 ? (n + 255) / 256 : 4096);
-    hipLaunchKernelGGL(sum_splits_kernel, dim3(grid), dim3(256), 0, st, part, (int)p.splits, g.P, g.Q, g.bias,
-                       g.bias_type, g.c, g.c_type, g.ldc);
+    const bool wide = (uintptr_t)g.c % 16 == 0 && g.ldc % 4 == 0;
+    if (g.Q % 4 == 0)
+      hipLaunchKernelGGL(sum_splits_kernel<4>, dim3((unsigned)((n / 4 + 255) / 256)), dim3(256), 0, st, part,
+                         (int)p.splits, n, fast_div((uint32_t)(g.Q / 4)), g.bias, g.bias_type, g.c, g.c_type, g.ldc,
+                         wide ? 1 : 0);
+    else
+      hipLaunchKernelGGL(sum_splits_kernel<1>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, part,
+                         (int)p.splits, n, fast_div((uint32_t)g.Q), g.bias, g.bias_type, g.c, g.c_type, g.ldc, 0);
     MQ_LAUNCH_CHECK();
   }
   return MI355Q_OK;

@@ -22,17 +22,6 @@ constexpr int kLanes = kGroup / kChunk;          // 16 lanes per group: one DPP 
 
 typedef unsigned u32x2_t __attribute__((ext_vector_type(2)));
 
-// n / d for n < 2^31 without a division: (mulhi(n, mul) + n) >> shift
-struct FastDiv {
-  uint32_t d, mul, shift;
-};
-static FastDiv fast_div(uint32_t d) {
-  uint32_t l = 0;
-  while ((uint64_t(1) << l) < d) ++l;
-  return {d, (uint32_t)((((uint64_t(1) << l) - d) << 32) / d + 1), l};
-}
-__device__ __forceinline__ uint32_t div(uint32_t n, const FastDiv& f) { return (__umulhi(n, f.mul) + n) >> f.shift; }
-
 // The largest magnitude is found on the bit patterns with the sign taken off,
 // which order as the magnitudes do and put infinities and NaN on top.
 template <class T> __device__ __forceinline__ uint32_t magnitude(typename T::raw v);
