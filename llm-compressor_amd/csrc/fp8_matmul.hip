@@ -200,21 +200,46 @@ __device__ __forceinline__ bf16x8_t codes_bf16(uint32_t lo, uint32_t hi) {
   return __builtin_bit_cast(bf16x8_t, scaled_bf16(lo, hi, 1.f));
 }
 
-// Work item of a workgroup: the workgroups of one XCD (every eighth) take
-// neighbouring tiles, in groups of 8 row tiles, so that they share operands in
-// its L2; the splits of the sum are the outermost order.
+// Work items: the first `full` tiles run whole, the others (what is left over
+// when every CU has had its whole tiles) in `splits` parts of the sum each, whose
+// fp32 tiles go to partial slots.  The workgroups of one XCD (every eighth) take
+// neighbouring tiles, in groups of 8 row tiles, so that they share operands in its L2.
 struct TileOrder {
-  uint32_t row_tiles, col_tiles, splits;
+  uint32_t row_tiles, col_tiles, full, splits;
 };
-__device__ __forceinline__ void tile_of(const TileOrder& o, uint32_t id, uint32_t& tr, uint32_t& tc, uint32_t& split) {
-  const uint32_t tiles = o.row_tiles * o.col_tiles, total = tiles * o.splits;
-  const uint32_t q = total / 8, r = total % 8, x = id % 8;
-  const uint32_t lin = x * q + (x < r ? x : r) + id / 8;
-  split = lin / tiles;
-  const uint32_t t = lin - split * tiles, g = t / (8 * o.col_tiles), left = o.row_tiles - 8 * g;
+struct TileItem {
+  uint32_t row, col;   // of the tile
+  uint32_t split;
+  int64_t slot;        // partial slot, or -1: the output itself
+};
+__device__ __forceinline__ uint32_t xcd_order(uint32_t id, uint32_t n) {
+  const uint32_t q = n / 8, r = n % 8, x = id % 8;
+  return x * q + (x < r ? x : r) + id / 8;
+}
+__device__ __forceinline__ TileItem tile_of(const TileOrder& o, uint32_t id) {
+  const uint32_t rest = o.row_tiles * o.col_tiles - o.full;
+  TileItem it;
+  uint32_t t;
+  if (id < o.full) {
+    t = xcd_order(id, o.full);
+    it.split = 0;
+    it.slot = -1;
+  } else {
+    const uint32_t lin = xcd_order(id - o.full, rest * o.splits);
+    it.split = lin / rest;
+    t = o.full + lin - it.split * rest;
+    it.slot = o.splits > 1 ? (int64_t)lin : -1;
+  }
+  const uint32_t g = t / (8 * o.col_tiles), left = o.row_tiles - 8 * g;
   const uint32_t rows = left < 8 ? left : 8, in = t - g * 8 * o.col_tiles;
-  tc = in / rows;
-  tr = 8 * g + in - tc * rows;
+  it.col = in / rows;
+  it.row = 8 * g + in - it.col * rows;
+  return it;
+}
+// the steps [begin, end) of an item: all, or one of `splits` ranges of `per`
+__device__ __forceinline__ void item_steps(const TileItem& it, int steps, int per, int& begin, int& end) {
+  begin = it.slot < 0 ? 0 : (int)it.split * per;
+  end = it.slot < 0 || begin + per > steps ? steps : begin + per;
 }
 
 // T x A tiles of 32 tokens x 32 features per wave, WT x WF waves.
@@ -233,20 +258,33 @@ struct FwdShape {
 
 // Stores a workgroup's tiles acc[A][T] of C [P][Q] (P on the lanes): lane l
 // holds row l & 31 of tile b and, in registers 4 j .. 4 j + 3 of tile a, columns
-// 8 j + 4 (l / 32) and on.  Split sums go to `part` in fp32 without the bias.
+// 8 j + 4 (l / 32) and on.  A split's sums go to its partial slot [TT][FT] in
+// fp32 without the bias.
 template <class S, int T, int A>
 __device__ __forceinline__ void store_tiles(const ProductArgs& g, f32x16_t (&acc)[A][T], char* ring, int64_t t0, int64_t f0,
-                                            int wt, int wf, int wave, int lane, uint32_t split, float* part) {
+                                            int wt, int wf, int wave, int lane, int64_t slot, float* parts) {
+  if (slot >= 0) {
+    float* const out = parts + slot * (S::TT * S::FT) + (wt * T * 32 + (lane & 31)) * S::FT + wf * A * 32 + 4 * (lane >> 5);
+#pragma unroll
+    for (int a = 0; a < A; ++a)
+#pragma unroll
+      for (int b = 0; b < T; ++b)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          *reinterpret_cast<f32x4_t*>(out + 32 * b * S::FT + 32 * a + 8 * j) =
+              f32x4_t{acc[a][b][4 * j], acc[a][b][4 * j + 1], acc[a][b][4 * j + 2], acc[a][b][4 * j + 3]};
+    return;
+  }
   const int64_t tw = t0 + wt * T * 32, fw = f0 + wf * A * 32;   // the wave's first row and column
   __syncthreads();   // the ring is no longer read
   float* const biases = reinterpret_cast<float*>(ring + S::BIAS);
   for (int i = threadIdx.x; i < S::FT; i += S::NTH)
-    biases[i] = g.bias && !part && f0 + i < g.Q ? load_typed(g.bias, g.bias_type, f0 + i) : 0.f;
+    biases[i] = g.bias && f0 + i < g.Q ? load_typed(g.bias, g.bias_type, f0 + i) : 0.f;
   __syncthreads();
   const float* const bw = biases + wf * A * 32 + 4 * (lane >> 5);
-  if (part || g.c_type == MI355Q_F32) {
-    float* const out = part ? part + (int64_t)split * g.P * g.Q : static_cast<float*>(g.c);
-    const int64_t ld = part ? g.Q : g.ldc;
+  if (g.c_type == MI355Q_F32) {
+    float* const out = static_cast<float*>(g.c);
+    const int64_t ld = g.ldc;
     const bool wide = ld % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
 #pragma unroll
     for (int a = 0; a < A; ++a)
@@ -325,18 +363,17 @@ __device__ __forceinline__ void store_tiles(const ProductArgs& g, f32x16_t (&acc
 
 template <int T, int A, int WT, int WF, bool E8M0>
 __global__ __launch_bounds__(64 * WT * WF) __attribute__((amdgpu_waves_per_eu(2)))
-void fp8_forward_kernel(ProductArgs g, TileOrder order, int steps_per_split, float* part) {
+void fp8_forward_kernel(ProductArgs g, TileOrder order, int steps_per_split, float* parts) {
   using S = FwdShape<T, A, WT, WF>;
   __shared__ __attribute__((aligned(16))) char ring[S::LDS];
   char* const ringb = ring + 3 * S::A_SLOT;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wt = wave % WT, wf = wave / WT;
-  uint32_t tr, tc, split;
-  tile_of(order, blockIdx.x, tr, tc, split);
-  const int64_t t0 = (int64_t)tr * S::TT, f0 = (int64_t)tc * S::FT;
+  const TileItem item = tile_of(order, blockIdx.x);
+  const int64_t t0 = (int64_t)item.row * S::TT, f0 = (int64_t)item.col * S::FT;
   const int nkb = (int)((g.R + kGroup - 1) / kGroup);
-  const int s_begin = (int)split * steps_per_split;
-  const int s_end = s_begin + steps_per_split < nkb ? s_begin + steps_per_split : nkb;
+  int s_begin, s_end;
+  item_steps(item, nkb, steps_per_split, s_begin, s_end);
 
   // DMA: instruction j of wave w fills 8 rows; lane l the chunk position l & 7
   // of row l / 8, with the row's chunk (l & 7) ^ ((row >> 1) & 7), the same for
@@ -549,7 +586,7 @@ void fp8_forward_kernel(ProductArgs g, TileOrder order, int steps_per_split, flo
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // before the ring is used again
   }
 
-  store_tiles<S, T, A>(g, acc, ring, t0, f0, wt, wf, wave, lane, split, part);
+  store_tiles<S, T, A>(g, acc, ring, t0, f0, wt, wf, wave, lane, item.slot, parts);
 }
 
 // ---------------------------------------------------------------- input gradient
@@ -573,19 +610,18 @@ struct GradInputShape {
 
 template <int T, int WT>
 __global__ __launch_bounds__(128 * WT) __attribute__((amdgpu_waves_per_eu(2)))
-void fp8_grad_input_kernel(ProductArgs g, TileOrder order, int blocks_per_split, float* part) {
+void fp8_grad_input_kernel(ProductArgs g, TileOrder order, int blocks_per_split, float* parts) {
   using S = GradInputShape<T, WT>;
   constexpr int A = S::A;
   __shared__ __attribute__((aligned(16))) char ring[S::LDS];
   char* const ringb = ring + S::NAS * S::A_SLOT;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wt = wave % WT, wf = wave / WT;
-  uint32_t tr, tc, split;
-  tile_of(order, blockIdx.x, tr, tc, split);
-  const int64_t t0 = (int64_t)tr * S::TT, f0 = (int64_t)tc * S::FT;
+  const TileItem item = tile_of(order, blockIdx.x);
+  const int64_t t0 = (int64_t)item.row * S::TT, f0 = (int64_t)item.col * S::FT;
   const int nst = (int)((g.R + S::SN - 1) / S::SN);
-  const int s_begin = (int)split * blocks_per_split * 2;
-  const int s_end = s_begin + 2 * blocks_per_split < nst ? s_begin + 2 * blocks_per_split : nst;
+  int s_begin, s_end;
+  item_steps(item, nst, 2 * blocks_per_split, s_begin, s_end);
 
   // DMA: 8 rows of 128 bytes an instruction; n rows of the weight with chunk
   // (l & 7) ^ (row & 7) at position l & 7 (the eight rows of a transposed read), token
@@ -757,7 +793,7 @@ void fp8_grad_input_kernel(ProductArgs g, TileOrder order, int blocks_per_split,
   }
   if (s < s_end) step(s, true, true, scale_of(s >> 1));   // a last block of 64 n or fewer
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // before the ring is used again
-  store_tiles<S, T, A>(g, acc, ring, t0, f0, wt, wf, wave, lane, split, part);
+  store_tiles<S, T, A>(g, acc, ring, t0, f0, wt, wf, wave, lane, item.slot, parts);
 }
 
 // ---------------------------------------------------------------- weight gradient
@@ -775,9 +811,10 @@ template <int MB, int NB2, int WK, int WN>
 struct GradWeightShape {
   static constexpr int W = WK * WN, NTH = 64 * W;
   static constexpr int FK = 32 * MB * WK, FN = 32 * NB2 * WN, SM = 32;   // k, n per workgroup, tokens per stage
-  static constexpr int X_SLOT = SM * FK * 2, Y_SLOT = SM * FN * 2, NXS = 3, NYS = 4;
-  static constexpr int RAW = 1024 + 256, NRS = 4;             // a wave's codes and scale bytes (as dwords)
-  static constexpr int RING = NXS * X_SLOT + NYS * Y_SLOT + W * NRS * RAW;
+  static constexpr int NS = 4, NRS = 2;                       // slots of bf16 rows, of a wave's raw rows
+  static constexpr int X_SLOT = SM * FK * 2, Y_SLOT = SM * FN * 2;
+  static constexpr int RAW = 1024 + 256;                      // a wave's codes and scale bytes (as dwords)
+  static constexpr int RING = NS * (X_SLOT + Y_SLOT) + W * NRS * RAW;
   static constexpr int PITCH = 32 * MB * 4 + 16;              // bytes per staged output row (fp32)
   static constexpr int STAGED = W * 32 * PITCH;
   static constexpr int LDS = RING > STAGED ? RING : STAGED;
@@ -786,33 +823,30 @@ struct GradWeightShape {
 
 template <int MB, int NB2, int WK, int WN>
 __global__ __launch_bounds__(64 * WK * WN) __attribute__((amdgpu_waves_per_eu(2)))
-void fp8_grad_weight_kernel(ProductArgs g, TileOrder order, int stages_per_split, float* part) {
+void fp8_grad_weight_kernel(ProductArgs g, TileOrder order, int stages_per_split, float* parts) {
   using S = GradWeightShape<MB, NB2, WK, WN>;
   __shared__ __attribute__((aligned(16))) char ring[S::LDS];
-  char* const ringy = ring + S::NXS * S::X_SLOT;
+  char* const ringy = ring + S::NS * S::X_SLOT;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  char* const raw = ringy + S::NYS * S::Y_SLOT + wave * S::NRS * S::RAW;
+  char* const raw = ringy + S::NS * S::Y_SLOT + wave * S::NRS * S::RAW;
   const int wn = wave % WN, wk = wave / WN;
-  uint32_t tn, tk, split;
-  tile_of(order, blockIdx.x, tn, tk, split);
-  const int64_t n0 = (int64_t)tn * S::FN, k0 = (int64_t)tk * S::FK;
+  const TileItem item = tile_of(order, blockIdx.x);
+  const int64_t n0 = (int64_t)item.row * S::FN, k0 = (int64_t)item.col * S::FK;
   const int nst = (int)((g.R + S::SM - 1) / S::SM);
-  const int s_begin = (int)split * stages_per_split;
-  const int s_end = s_begin + stages_per_split < nst ? s_begin + stages_per_split : nst;
+  int s_begin, s_end;
+  item_steps(item, nst, stages_per_split, s_begin, s_end);
   const int last_rows = (int)(g.R - (int64_t)(nst - 1) * S::SM);   // tokens of the last stage
 
   // DMA of dY: 1 KB an instruction, RPI rows; n past the end repeat the last ones
   // (not stored), tokens past the end the last one (cleared in LDS, as are
   // their checkpoint rows: an infinity there must not meet a zero).
   constexpr int YC = S::FN / 8, RPI = 64 / YC, NY = S::SM / RPI / S::W;
-  uint32_t oy[NY], dy[NY];
+  uint32_t oy[NY];
 #pragma unroll
   for (int j = 0; j < NY; ++j) {
     const int row = (wave * NY + j) * RPI + lane / YC;
     const int64_t col = n0 + 8 * ((lane % YC) ^ (4 * (row & 3))), c = col < g.P ? col : g.P - 8;
     oy[j] = (uint32_t)row * (uint32_t)(2 * g.lda) + (uint32_t)(2 * (c - n0));
-    dy[j] = row >= last_rows ? (uint32_t)(row - (last_rows - 1)) * (uint32_t)(2 * g.lda) : 0u;
-    asm volatile("" : "+v"(oy[j]), "+v"(dy[j]));
   }
   // ... of the checkpoint: lane l takes 16 codes of row XR l / XC of the wave's
   constexpr int XC = S::FK / 16, XR = 64 / XC;
@@ -820,50 +854,71 @@ void fp8_grad_weight_kernel(ProductArgs g, TileOrder order, int stages_per_split
   const int64_t xcol = k0 + 16 * xch < g.Q ? k0 + 16 * xch : g.Q - 16;
   uint32_t ox = (uint32_t)xrow * (uint32_t)g.ldb + (uint32_t)(xcol - k0);
   uint32_t oe = (uint32_t)xrow * (uint32_t)g.ldbs + (uint32_t)(xcol / kGroup - k0 / kGroup);
-  const int xpast = xrow >= last_rows ? xrow - (last_rows - 1) : 0;
-  uint32_t dx = (uint32_t)xpast * (uint32_t)g.ldb, de = (uint32_t)xpast * (uint32_t)g.ldbs;
-  asm volatile("" : "+v"(ox), "+v"(oe), "+v"(dx), "+v"(de));
-  const char* const ybase = static_cast<const char*>(g.a) + 2 * n0;
-  const char* const xbase = reinterpret_cast<const char*>(g.b) + k0;
-  const char* const ebase = reinterpret_cast<const char*>(g.be) + k0 / kGroup;
-  const uint32_t ly0 = lds_u32(ringy) + wave * NY * 1024, lr0 = lds_u32(raw);
-  auto load_y = [&](int s, int slot, int j) __attribute__((always_inline)) {
-    dma_s(oy[j] - (s == nst - 1 ? dy[j] : 0u), ybase + (int64_t)s * S::SM * 2 * g.lda,
-          ly0 + (uint32_t)(slot % S::NYS) * S::Y_SLOT + 1024 * j);
+  // before the last stage's DMA, once (dY's turn comes a stage after the checkpoint's)
+  auto turn_x = [&](int s) __attribute__((always_inline)) {
+    if (last_rows < S::SM && s == nst - 1 && xrow >= last_rows) {
+      ox -= (uint32_t)(xrow - (last_rows - 1)) * (uint32_t)g.ldb;
+      oe -= (uint32_t)(xrow - (last_rows - 1)) * (uint32_t)g.ldbs;
+    }
   };
-  auto load_x = [&](int s, int slot) __attribute__((always_inline)) {
+  auto turn_y = [&](int s) __attribute__((always_inline)) {
+    if (last_rows < S::SM && s == nst - 1)
+#pragma unroll
+      for (int j = 0; j < NY; ++j) {
+        const int row = (wave * NY + j) * RPI + lane / YC;
+        oy[j] -= row >= last_rows ? (uint32_t)(row - (last_rows - 1)) * (uint32_t)(2 * g.lda) : 0u;
+      }
+  };
+  // running stage bases; they stop at the item's last stage
+  const int64_t ystep = (int64_t)S::SM * 2 * g.lda, xstep = (int64_t)S::SM * g.ldb, estep = (int64_t)S::SM * g.ldbs;
+  const char* yp = static_cast<const char*>(g.a) + 2 * n0 + s_begin * ystep;
+  const char* xp = reinterpret_cast<const char*>(g.b) + k0 + s_begin * xstep;
+  const char* ep = reinterpret_cast<const char*>(g.be) + k0 / kGroup + s_begin * estep;
+  const uint32_t ly0 = lds_u32(ringy) + wave * NY * 1024, lr0 = lds_u32(raw);
+  auto load_y = [&](int slot, int j) __attribute__((always_inline)) {
+    dma_s(oy[j], yp, ly0 + (uint32_t)(slot % S::NS) * S::Y_SLOT + 1024 * j);
+  };
+  auto load_x = [&](int slot) __attribute__((always_inline)) {
     const uint32_t m0 = lr0 + (uint32_t)(slot % S::NRS) * S::RAW;
-    dma_s(ox - (s == nst - 1 ? dx : 0u), xbase + (int64_t)s * S::SM * g.ldb, m0);
-    dma_bytes(oe - (s == nst - 1 ? de : 0u), ebase + (int64_t)s * S::SM * g.ldbs, m0 + 1024);
+    dma_s(ox, xp, m0);
+    dma_bytes(oe, ep, m0 + 1024);
+  };
+  auto next_y = [&](int s) __attribute__((always_inline)) { yp += s < s_end ? ystep : 0; };   // to stage s
+  auto next_x = [&](int s) __attribute__((always_inline)) {
+    xp += s < s_end ? xstep : 0;
+    ep += s < s_end ? estep : 0;
   };
   constexpr int NDMA = NY + 2;
-  // the wave's rows of stage s as bf16: (byte << 23) | 2^22 is the scale as
-  // the conversion reads it, by its exponent alone (0: the subnormal 2^-127, 255:
-  // NaN)
-  // (half of the lanes write the second half first, so that 8 or 16 neighbouring
-  // lanes write to as many different 16-byte columns of the banks)
-  const int xw = xrow * S::FK * 2 + 16 * ((2 * xch) ^ (4 * (xrow & 3))), xswap = ((lane >> 2) ^ (lane >> 3)) & 1;
-  u32x4_t raw_codes;
+  // the wave's rows of a stage as bf16: (byte << 23) | 2^22 is the scale as the
+  // conversion reads it, by its exponent alone (0: the subnormal 2^-127, 255:
+  // NaN).  Half of the lanes take the second half of their 16 codes first, so that
+  // 8 or 16 neighbouring lanes write to as many different 16-byte columns of the
+  // banks.
+  const int xswap = ((lane >> 2) ^ (lane >> 3)) & 1;
+  const int xw = xrow * S::FK * 2 + 16 * ((2 * xch) ^ (4 * (xrow & 3))) + 16 * xswap, xw2 = xw + 16 - 32 * xswap;
+  const int rr = 16 * lane + 8 * xswap, rr2 = rr + 8 - 16 * xswap;
+  i32x2_t raw0, raw1;
   uint32_t raw_byte;
-  auto fetch = [&](int s) __attribute__((always_inline)) {
-    const char* r = raw + (s % S::NRS) * S::RAW;
-    raw_codes = *reinterpret_cast<const u32x4_t*>(r + 16 * lane);
+  auto fetch = [&](int slot) __attribute__((always_inline)) {
+    const char* r = raw + (slot % S::NRS) * S::RAW;
+    raw0 = *reinterpret_cast<const i32x2_t*>(r + rr);
+    raw1 = *reinterpret_cast<const i32x2_t*>(r + rr2);
     raw_byte = *reinterpret_cast<const uint32_t*>(r + 1024 + 4 * lane);
   };
-  auto convert = [&](int s) __attribute__((always_inline)) {
+  auto convert = [&](int slot) __attribute__((always_inline)) {
     const float e = __uint_as_float((raw_byte << 23) | 0x00400000u);
-    u32x4_t c = raw_codes;
-    if (s == nst - 1 && xpast > 0) c = u32x4_t{0u, 0u, 0u, 0u};
-    if (xswap) c = u32x4_t{c[2], c[3], c[0], c[1]};
-    char* w = ring + (s % S::NXS) * S::X_SLOT + xw;
-    *reinterpret_cast<u32x4_t*>(w + 16 * xswap) = scaled_bf16(c[0], c[1], e);
-    *reinterpret_cast<u32x4_t*>(w + 16 * (1 - xswap)) = scaled_bf16(c[2], c[3], e);
+    char* w = ring + (slot % S::NS) * S::X_SLOT;
+    *reinterpret_cast<u32x4_t*>(w + xw) = scaled_bf16((uint32_t)raw0[0], (uint32_t)raw0[1], e);
+    *reinterpret_cast<u32x4_t*>(w + xw2) = scaled_bf16((uint32_t)raw1[0], (uint32_t)raw1[1], e);
   };
-  auto clear_tail = [&](int s) __attribute__((always_inline)) {
+  auto clear_tail = [&](int s, int slot) __attribute__((always_inline)) {
     if (last_rows == S::SM || s != nst - 1) return;
-    char* y = ringy + (s % S::NYS) * S::Y_SLOT;
+    char* y = ringy + (slot % S::NS) * S::Y_SLOT;
     for (int i = last_rows * YC + (int)threadIdx.x; i < S::SM * YC; i += S::NTH)
       *reinterpret_cast<u32x4_t*>(y + 16 * i) = u32x4_t{0u, 0u, 0u, 0u};
+    char* x = ring + (slot % S::NS) * S::X_SLOT;
+    for (int i = last_rows * (S::FK / 8) + (int)threadIdx.x; i < S::SM * (S::FK / 8); i += S::NTH)
+      *reinterpret_cast<u32x4_t*>(x + 16 * i) = u32x4_t{0u, 0u, 0u, 0u};
     __syncthreads();
   };
 
@@ -872,22 +927,18 @@ void fp8_grad_weight_kernel(ProductArgs g, TileOrder order, int stages_per_split
   const int gg = lane >> 4, ee = (lane >> 2) & 3, qq = lane & 3;
   int px[MB], py[NB2];
 #pragma unroll
-  for (int b = 0; b < MB; ++b) {
+  for (int b = 0; b < MB; ++b)
     px[b] = (8 * (gg >> 1) + ee) * S::FK * 2 + 8 * (qq & 1) +
             16 * ((4 * ((MB * wk + b) ^ ee)) + 2 * (gg & 1) + (qq >> 1));
-    asm volatile("" : "+v"(px[b]));
-  }
 #pragma unroll
-  for (int b = 0; b < NB2; ++b) {
+  for (int b = 0; b < NB2; ++b)
     py[b] = (8 * (gg >> 1) + ee) * S::FN * 2 + 8 * (qq & 1) +
             16 * ((4 * ((NB2 * wn + b) ^ ee)) + 2 * (gg & 1) + (qq >> 1));
-    asm volatile("" : "+v"(py[b]));
-  }
-  auto read_x = [&](int s, int kk, int b) __attribute__((always_inline)) {
-    return tr_pair<S::FK * 2>(ring + (s % S::NXS) * S::X_SLOT + kk * 16 * S::FK * 2 + px[b]);
+  auto read_x = [&](int slot, int kk, int b) __attribute__((always_inline)) {
+    return tr_pair<S::FK * 2>(ring + (slot % S::NS) * S::X_SLOT + kk * 16 * S::FK * 2 + px[b]);
   };
-  auto read_y = [&](int s, int kk, int b) __attribute__((always_inline)) {
-    return tr_pair<S::FN * 2>(ringy + (s % S::NYS) * S::Y_SLOT + kk * 16 * S::FN * 2 + py[b]);
+  auto read_y = [&](int slot, int kk, int b) __attribute__((always_inline)) {
+    return tr_pair<S::FN * 2>(ringy + (slot % S::NS) * S::Y_SLOT + kk * 16 * S::FN * 2 + py[b]);
   };
 
   f32x16_t acc[MB][NB2];
@@ -902,73 +953,105 @@ void fp8_grad_weight_kernel(ProductArgs g, TileOrder order, int stages_per_split
   // Stage s, in two slices of 16 tokens; while one is multiplied the other's
   // operands are read.  The barrier between them publishes stage s + 1 (dY's DMA
   // and the converted rows; the checkpoint rows of stage s + 2 have arrived as well)
-  // and frees the slots of stage s - 1.
-  auto stage = [&](int s) __attribute__((always_inline)) {
-    const int s1 = s + 1 < s_end ? s + 1 : s, s3 = s + 3 < s_end ? s + 3 : s_end - 1,
-              s4 = s + 4 < s_end ? s + 4 : s_end - 1;
+  // and frees the slots of stage s - 1.  `c` is the stage's slot, a constant in
+  // the loop's four copies: slot numbers and addresses cost no instructions.
+  auto stage = [&](int s, int c) __attribute__((always_inline)) {
     static_assert(MB * NB2 >= MB + NB2, "an MFMA for each operand read");
 #pragma unroll
     for (int i = 0; i < MB * NB2; ++i) {
       const int x = i / NB2, y = i % NB2;
       acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fx0[x], fy0[y], acc[x][y], 0, 0, 0);
-      if (i < NB2) fy1[i] = read_y(s, 1, i);
-      else if (i < NB2 + MB) fx1[i - NB2] = read_x(s, 1, i - NB2);
+      if (i < NB2) fy1[i] = read_y(c, 1, i);
+      else if (i < NB2 + MB) fx1[i - NB2] = read_x(c, 1, i - NB2);
       __builtin_amdgcn_sched_barrier(0);
     }
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(NDMA) : "memory");
-    if (s1 != s) clear_tail(s1);
+    if (s + 1 < s_end) clear_tail(s + 1, c + 1);
+    next_y(s + 3);
+    next_x(s + 4);
+    if (s + 3 < s_end) turn_y(s + 3);
+    if (s + 4 < s_end) turn_x(s + 4);
     __builtin_amdgcn_sched_barrier(0);
-    fetch(s + 2);
+    fetch(c + 2);
 #pragma unroll
     for (int i = 0; i < MB * NB2; ++i) {
       const int x = i / NB2, y = i % NB2;
       acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fx1[x], fy1[y], acc[x][y], 0, 0, 0);
-      if (i < NB2) fy0[i] = read_y(s + 1, 0, i);
-      else if (i < NB2 + MB) fx0[i - NB2] = read_x(s + 1, 0, i - NB2);
-      if (i == 0) load_x(s4, s + 4);
-      else if (i <= NY) load_y(s3, s + 3, i - 1);
-      if (i == MB * NB2 - 2) convert(s + 2);
+      if (i < NB2) fy0[i] = read_y(c + 1, 0, i);
+      else if (i < NB2 + MB) fx0[i - NB2] = read_x(c + 1, 0, i - NB2);
+      if (i < NY) load_y(c + 3, i);
+      if (i == MB * NB2 - 2) convert(c + 2);
+      if (i == MB * NB2 - 1) load_x(c + 4);   // into the slot that `convert` has emptied
       __builtin_amdgcn_sched_barrier(0);
     }
   };
 
-  {   // every split has a stage
-    auto at = [&](int s) { return s < s_end ? s : s_end - 1; };
-    load_x(s_begin, s_begin);
-    load_x(at(s_begin + 1), s_begin + 1);
+  {   // every item has a stage; slots count from its first one
+    auto start_x = [&](int i) __attribute__((always_inline)) {
+      if (i > 0) next_x(s_begin + i);
+      if (s_begin + i < s_end) turn_x(s_begin + i);
+      load_x(i);
+    };
+    auto start_y = [&](int i) __attribute__((always_inline)) {
+      if (i > 0) next_y(s_begin + i);
+      if (s_begin + i < s_end) turn_y(s_begin + i);
 #pragma unroll
-    for (int j = 0; j < NY; ++j) load_y(s_begin, s_begin, j);
-    load_x(at(s_begin + 2), s_begin + 2);
+      for (int j = 0; j < NY; ++j) load_y(i, j);
+    };
+    start_x(0);
+    start_x(1);
+    start_y(0);
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NY) : "memory");
+    fetch(0);
+    convert(0);
+    fetch(1);
+    convert(1);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the raw slots are read
+    start_y(1);
+    start_x(2);
+    start_y(2);
+    start_x(3);
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * NDMA) : "memory");
+    clear_tail(s_begin, 0);
 #pragma unroll
-    for (int j = 0; j < NY; ++j) load_y(at(s_begin + 1), s_begin + 1, j);
-    load_x(at(s_begin + 3), s_begin + 3);
+    for (int b = 0; b < NB2; ++b) fy0[b] = read_y(0, 0, b);
 #pragma unroll
-    for (int j = 0; j < NY; ++j) load_y(at(s_begin + 2), s_begin + 2, j);
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * NDMA) : "memory");
-    fetch(s_begin);
-    convert(s_begin);
-    fetch(s_begin + 1);
-    convert(s_begin + 1);
-    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    clear_tail(s_begin);
-#pragma unroll
-    for (int b = 0; b < NB2; ++b) fy0[b] = read_y(s_begin, 0, b);
-#pragma unroll
-    for (int b = 0; b < MB; ++b) fx0[b] = read_x(s_begin, 0, b);
-    for (int s = s_begin; s < s_end; ++s) stage(s);
+    for (int b = 0; b < MB; ++b) fx0[b] = read_x(0, 0, b);
+    int s = s_begin;
+    for (; s + 4 <= s_end; s += 4) {
+      stage(s, 0);
+      stage(s + 1, 1);
+      stage(s + 2, 2);
+      stage(s + 3, 3);
+    }
+    if (s < s_end) stage(s, 0);
+    if (s + 1 < s_end) stage(s + 1, 1);
+    if (s + 2 < s_end) stage(s + 2, 2);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // before the ring is used again
   }
 
+  const int64_t kw = k0 + wk * MB * 32;
+  if (item.slot >= 0) {   // a split's sums: its partial slot [FN][FK]
+    float* const out = parts + item.slot * (S::FN * S::FK) + (wn * NB2 * 32 + (lane & 31)) * S::FK + wk * MB * 32 +
+                       4 * (lane >> 5);
+#pragma unroll
+    for (int y = 0; y < NB2; ++y)
+#pragma unroll
+      for (int x = 0; x < MB; ++x)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          *reinterpret_cast<f32x4_t*>(out + 32 * y * S::FK + 32 * x + 8 * j) =
+              f32x4_t{acc[x][y][4 * j], acc[x][y][4 * j + 1], acc[x][y][4 * j + 2], acc[x][y][4 * j + 3]};
+    return;
+  }
   // One row of tiles at a time through LDS: lane l holds column n l & 31 and four
   // consecutive k a register quad; rows of 32 MB k leave as whole lines.
   __syncthreads();
-  const bool f32 = part || g.c_type == MI355Q_F32;
+  const bool f32 = g.c_type == MI355Q_F32;
   char* const stage_out = ring + wave * 32 * S::PITCH;
-  const int64_t ld = part ? g.Q : g.ldc;
   const int es = f32 ? 4 : 2;
-  char* const out = part ? reinterpret_cast<char*>(part + (int64_t)split * g.P * g.Q) : static_cast<char*>(g.c);
-  const bool wide = (ld * es) % 16 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
-  const int64_t kw = k0 + wk * MB * 32;
+  char* const out = static_cast<char*>(g.c);
+  const bool wide = (g.ldc * es) % 16 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
 #pragma unroll
   for (int y = 0; y < NB2; ++y) {
 #pragma unroll
@@ -993,7 +1076,7 @@ void fp8_grad_weight_kernel(ProductArgs g, TileOrder order, int stages_per_split
     for (int r = lane / lpr; r < 32; r += rpi) {
       const u32x4_t v = *reinterpret_cast<const u32x4_t*>(stage_out + r * S::PITCH + 16 * (lane % lpr));
       if (nw + r >= g.P) break;
-      char* o = out + ((nw + r) * ld + k) * es;
+      char* o = out + ((nw + r) * g.ldc + k) * es;
       if (wide && k + per <= g.Q) {
         *reinterpret_cast<u32x4_t*>(o) = v;
       } else if (f32) {
@@ -1010,61 +1093,64 @@ void fp8_grad_weight_kernel(ProductArgs g, TileOrder order, int stages_per_split
   }
 }
 
-// Sums the splits' partial products [splits][rows][cols] in their order, adds
-// the bias and rounds once.  N consecutive columns a thread (4 where they divide
-// the row), four splits' loads in flight.
-template <int N>
-__global__ __launch_bounds__(256) void sum_splits_kernel(const float* part, int splits, int64_t n, FastDiv row,
-                                                         const void* bias, int bias_type, void* c, int c_type,
-                                                         int64_t ldc, int wide) {
-  typedef float vec_t __attribute__((ext_vector_type(N)));
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;   // in vectors; below 2^31
-  if (i * N >= n) return;
-  const uint32_t r = div((uint32_t)i, row), q = ((uint32_t)i - r * row.d) * N;
-  const float* p = part + i * N;
-  float v[N];
+// Sums the partial slots [splits][tiles][TR][TC] of the split tiles in their
+// order, adds the bias and rounds once.  Four columns a thread, four splits' loads
+// in flight.
+template <int TR, int TC>
+__global__ __launch_bounds__(256) void sum_splits_kernel(ProductArgs g, TileOrder o, const float* parts) {
+  constexpr uint32_t PER = TR * TC / 4 / 256;          // workgroups per tile
+  static_assert(PER * 256 * 4 == TR * TC, "whole workgroups");
+  const uint32_t rest = o.row_tiles * o.col_tiles - o.full, tile = blockIdx.x / PER;
+  const uint32_t at = (blockIdx.x - tile * PER) * 256 + threadIdx.x;
+  const uint32_t t = o.full + tile, gr = t / (8 * o.col_tiles), left = o.row_tiles - 8 * gr;
+  const uint32_t rows = left < 8 ? left : 8, in = t - gr * 8 * o.col_tiles, tc = in / rows;
+  const int64_t r = (int64_t)(8 * gr + in - tc * rows) * TR + at / (TC / 4), q = (int64_t)tc * TC + at % (TC / 4) * 4;
+  if (r >= g.P || q >= g.Q) return;
+  const float* p = parts + (int64_t)tile * (TR * TC) + 4 * at;
+  const int64_t step = (int64_t)rest * (TR * TC);
+  f32x4_t v = {0.f, 0.f, 0.f, 0.f};
+  uint32_t s = 0;
+  for (; s + 4 <= o.splits; s += 4) {
+    f32x4_t x[4];
 #pragma unroll
-  for (int e = 0; e < N; ++e) v[e] = 0.f;
-  int s = 0;
-  for (; s + 4 <= splits; s += 4) {
-    vec_t x[4];
-#pragma unroll
-    for (int u = 0; u < 4; ++u) __builtin_memcpy(&x[u], p + (s + u) * n, 4 * N);
+    for (int u = 0; u < 4; ++u) x[u] = *reinterpret_cast<const f32x4_t*>(p + (s + u) * step);
 #pragma unroll
     for (int u = 0; u < 4; ++u)
 #pragma unroll
-      for (int e = 0; e < N; ++e) v[e] += x[u][e];
+      for (int e = 0; e < 4; ++e) v[e] += x[u][e];
   }
-  for (; s < splits; ++s) {
-    vec_t x;
-    __builtin_memcpy(&x, p + s * n, 4 * N);
+  for (; s < o.splits; ++s) {
+    const f32x4_t x = *reinterpret_cast<const f32x4_t*>(p + s * step);
 #pragma unroll
-    for (int e = 0; e < N; ++e) v[e] += x[e];
+    for (int e = 0; e < 4; ++e) v[e] += x[e];
   }
-  if (bias)
+  const bool whole = q + 4 <= g.Q;
+  if (g.bias)
 #pragma unroll
-    for (int e = 0; e < N; ++e) v[e] += load_typed(bias, bias_type, q + e);
-  const int64_t o = (int64_t)r * ldc + q;
-  if (c_type == MI355Q_F32) {
-    float* d = static_cast<float*>(c) + o;
-    if (N == 4 && wide) {
-      *reinterpret_cast<f32x4_t*>(d) = f32x4_t{v[0], v[N > 1], v[N > 2 ? 2 : 0], v[N > 3 ? 3 : 0]};
+    for (int e = 0; e < 4; ++e)
+      if (q + e < g.Q) v[e] += load_typed(g.bias, g.bias_type, q + e);
+  const int64_t c = r * g.ldc + q;
+  if (g.c_type == MI355Q_F32) {
+    float* d = static_cast<float*>(g.c) + c;
+    if (whole && g.ldc % 4 == 0 && (reinterpret_cast<uintptr_t>(g.c) & 15) == 0) {
+      *reinterpret_cast<f32x4_t*>(d) = v;
     } else {
 #pragma unroll
-      for (int e = 0; e < N; ++e) d[e] = v[e];
+      for (int e = 0; e < 4; ++e)
+        if (q + e < g.Q) d[e] = v[e];
     }
     return;
   }
-  uint16_t h[N];
+  uint16_t h[4];
 #pragma unroll
-  for (int e = 0; e < N; ++e) h[e] = c_type == MI355Q_BF16 ? Bf16::store(v[e]) : F16::store(v[e]);
-  uint16_t* d = static_cast<uint16_t*>(c) + o;
-  if (N == 4 && wide) {
-    *reinterpret_cast<i32x2_t*>(d) = i32x2_t{(int)(h[0] | (uint32_t)h[N > 1] << 16),
-                                             (int)(h[N > 2 ? 2 : 0] | (uint32_t)h[N > 3 ? 3 : 0] << 16)};
+  for (int e = 0; e < 4; ++e) h[e] = g.c_type == MI355Q_BF16 ? Bf16::store(v[e]) : F16::store(v[e]);
+  uint16_t* d = static_cast<uint16_t*>(g.c) + c;
+  if (whole && g.ldc % 4 == 0 && (reinterpret_cast<uintptr_t>(g.c) & 7) == 0) {
+    *reinterpret_cast<i32x2_t*>(d) = i32x2_t{(int)(h[0] | (uint32_t)h[1] << 16), (int)(h[2] | (uint32_t)h[3] << 16)};
   } else {
 #pragma unroll
-    for (int e = 0; e < N; ++e) d[e] = h[e];
+    for (int e = 0; e < 4; ++e)
+      if (q + e < g.Q) d[e] = h[e];
   }
 }
 
@@ -1173,48 +1259,77 @@ __global__ __launch_bounds__(64 * W) void fp8_few_kernel(ProductArgs g) {
   }
 }
 
-// How a product is cut: row and column tiles, and splits of the sum where the
-// tiles leave CUs idle.
+// How a product is cut: a tile shape, the tiles that run whole, and parts of the
+// sum for the others.
 struct Plan {
-  int big;            // the larger tile
-  uint32_t splits;
-  int steps;          // steps of the sum per split
+  int shape;
+  uint32_t tile_rows, tile_cols;
+  uint32_t row_tiles, col_tiles, full, splits;
+  int steps;          // of the sum, per split
 };
-// `small` tiles of the output and `steps` of the sum: splits of at least
-// `least` steps until the CUs have two workgroups each
-static Plan split_plan(int big, int64_t tiles, int64_t steps, int64_t least) {
-  Plan p{big, 1, (int)steps};
-  int64_t s = 512 / tiles;
-  if (s > steps / least) s = steps / least;
-  if (s > 1) {
-    p.steps = (int)((steps + s - 1) / s);
-    p.splits = (uint32_t)((steps + p.steps - 1) / p.steps);
+// What a shape costs, in us: a step with one and with two workgroups on a CU
+// (one1, two; 0: only one fits), and what begins and ends a workgroup.
+struct ShapeCost {
+  int tile_rows, tile_cols;
+  double one, two, ends;
+};
+// The cheapest cut by these costs: every shape, whole tiles for as many rounds of
+// the 256 CUs as come out even or all, and 1 .. 16 parts for the rest, of at least
+// `least` steps.  Splits cost their partial sums' way through memory (written and read, at
+// 3.5 TB/s) and a second launch (4 us).
+static Plan make_plan(const ShapeCost* shapes, int n, int64_t rows, int64_t cols, int64_t steps, int64_t least) {
+  Plan best{};
+  double best_cost = 0;
+  for (int i = 0; i < n; ++i) {
+    const ShapeCost& c = shapes[i];
+    const int64_t tr = (rows + c.tile_rows - 1) / c.tile_rows, tc = (cols + c.tile_cols - 1) / c.tile_cols;
+    const int64_t tiles = tr * tc, even = tiles - tiles % 256;
+    const double pair = c.two > 0 ? c.two / 2 : c.one;   // a step of a workgroup that shares its CU
+    for (int f = 0; f < (even > 0 ? 2 : 1); ++f) {
+      const int64_t full = f ? even : 0, rest = tiles - full;
+      if (full == 0 && tiles > 1024) continue;           // (the partial sums of all tiles: never the cheapest)
+      for (int64_t want = 1; want <= 16; ++want) {
+        if (want > 1 && (rest == 0 || steps / want < least)) break;
+        const int64_t per = (steps + want - 1) / want, k = (steps + per - 1) / per;
+        const int64_t wgs = rest * k, rounds = (wgs + 255) / 256;
+        double t = (double)(full / 256) * (steps * pair + c.ends);
+        if (full == 0 && rounds == 1) t += per * c.one + c.ends;
+        else t += rounds * (per * pair + c.ends);
+        if (k > 1) t += 4 + (double)wgs * c.tile_rows * c.tile_cols * 8 / 3.5e6;
+        if (best.tile_rows == 0 || t < best_cost) {
+          best_cost = t;
+          best = Plan{i, (uint32_t)c.tile_rows, (uint32_t)c.tile_cols, (uint32_t)tr, (uint32_t)tc,
+                      (uint32_t)(k > 1 ? full : tiles), (uint32_t)(k > 1 ? k : 1), (int)per};
+        }
+      }
+    }
   }
-  return p;
+  return best;
 }
-static int64_t tiles_of(int64_t rows, int64_t cols, int64_t tr, int64_t tc) {
-  return ((rows + tr - 1) / tr) * ((cols + tc - 1) / tc);
+// forward and input gradient: `rows` tokens by `cols` columns, `sum` terms in
+// blocks of 128
+static Plan plan_forward(int64_t rows, int64_t cols, int64_t sum) {
+  static const ShapeCost shapes[] = {{64, 128, 0.72, 1.14, 3}, {128, 128, 1.10, 2.0, 4}};
+  return make_plan(shapes, 2, rows, cols, group_count(sum), 4);
 }
-// forward and input gradient: `rows` tokens by `cols` columns, `sum` terms
-static Plan plan_tokens(int64_t rows, int64_t cols, int64_t sum) {
-  const int64_t big = tiles_of(rows, cols, 128, 128);
-  if (big >= 384) return split_plan(1, big, group_count(sum), 8);
-  return split_plan(0, tiles_of(rows, cols, 64, 128), group_count(sum), 8);
+static Plan plan_grad_input(int64_t rows, int64_t cols, int64_t sum) {
+  static const ShapeCost shapes[] = {{64, 128, 0.95, 1.28, 3}, {128, 128, 1.25, 2.1, 4}};
+  return make_plan(shapes, 2, rows, cols, group_count(sum), 2);
 }
 static Plan plan_weight(int64_t rows, int64_t out, int64_t cols) {
-  const int64_t big = tiles_of(out, cols, 256, 256), stages = (rows + 31) / 32;
-  if (big >= 192) return split_plan(1, 2 * big, stages, 64);
-  return split_plan(0, tiles_of(out, cols, 128, 128), stages, 8);
+  static const ShapeCost shapes[] = {{128, 128, 0.46, 0.76, 3}, {256, 256, 1.0, 0, 8}};
+  return make_plan(shapes, 2, out, cols, (rows + 31) / 32, 4);
 }
-static size_t plan_bytes(const Plan& p, int64_t rows, int64_t cols) {
-  return p.splits > 1 ? sizeof(float) * p.splits * rows * cols : 0;
+static size_t plan_bytes(const Plan& p) {
+  if (p.splits <= 1) return 0;
+  return sizeof(float) * p.tile_rows * p.tile_cols * ((size_t)p.row_tiles * p.col_tiles - p.full) * p.splits;
 }
-// the splits' partial sums, or null and an unsplit plan without room for them
-static float* plan_workspace(Plan& p, int64_t rows, int64_t cols, int64_t steps, void* ws, size_t bytes) {
+// the splits' partial slots, or null and an unsplit plan without room for them
+static float* plan_workspace(Plan& p, void* ws, size_t bytes) {
   if (p.splits <= 1) return nullptr;
-  if (ws && bytes >= plan_bytes(p, rows, cols) && aligned16(ws)) return static_cast<float*>(ws);
+  if (ws && bytes >= plan_bytes(p) && aligned16(ws)) return static_cast<float*>(ws);
   p.splits = 1;
-  p.steps = (int)steps;
+  p.full = p.row_tiles * p.col_tiles;
   return nullptr;
 }
 
@@ -1246,50 +1361,43 @@ static void launch_few(const ProductArgs& g, bool e8, hipStream_t st) {
   else launch_few_shape<4, 2, 8, 1>(g, e8, st);
 }
 
-// Cuts C [rows][cols] into TR x TC tiles, runs `kernel(grid, order)` and adds up the splits.
-template <class Kernel>
-static int launch_tiles(const ProductArgs& g, int64_t tile_rows, int64_t tile_cols, const Plan& p, float* part,
-                        hipStream_t st, const char* who, Kernel&& kernel) {
-  const int64_t tr = (g.P + tile_rows - 1) / tile_rows, tc = (g.Q + tile_cols - 1) / tile_cols;
-  MQ_CHECK_ARG(tr * tc * p.splits < (int64_t(1) << 31), "%s: output too large", who);
-  kernel(dim3((unsigned)(tr * tc * p.splits)), TileOrder{(uint32_t)tr, (uint32_t)tc, p.splits});
+// Runs `kernel(grid, order)` over the plan's items and adds up its splits.
+template <int TR, int TC, class Kernel>
+static int launch_tiles(const ProductArgs& g, const Plan& p, float* parts, hipStream_t st, const char* who,
+                        Kernel&& kernel) {
+  const int64_t tiles = (int64_t)p.row_tiles * p.col_tiles, rest = tiles - p.full, items = p.full + rest * p.splits;
+  MQ_CHECK_ARG(tiles < (int64_t(1) << 28) && items < (int64_t(1) << 31), "%s: output too large", who);
+  const TileOrder o{p.row_tiles, p.col_tiles, p.full, p.splits};
+  kernel(dim3((unsigned)items), o);
   MQ_LAUNCH_CHECK();
-  if (part) {
-    // (a split product has at most 511 tiles of 64 KB elements: fewer than 2^31 vectors)
-    const int64_t n = g.P * g.Q;
-    const bool wide = (uintptr_t)g.c % 16 == 0 && g.ldc % 4 == 0;
-    if (g.Q % 4 == 0)
-      hipLaunchKernelGGL(sum_splits_kernel<4>, dim3((unsigned)((n / 4 + 255) / 256)), dim3(256), 0, st, part,
-                         (int)p.splits, n, fast_div((uint32_t)(g.Q / 4)), g.bias, g.bias_type, g.c, g.c_type, g.ldc,
-                         wide ? 1 : 0);
-    else
-      hipLaunchKernelGGL(sum_splits_kernel<1>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, part,
-                         (int)p.splits, n, fast_div((uint32_t)g.Q), g.bias, g.bias_type, g.c, g.c_type, g.ldc, 0);
+  if (parts) {
+    hipLaunchKernelGGL((sum_splits_kernel<TR, TC>), dim3((unsigned)(rest * (TR * TC / 1024))), dim3(256), 0, st, g, o,
+                       parts);
     MQ_LAUNCH_CHECK();
   }
   return MI355Q_OK;
 }
 
 template <int T, int A, int WT, int WF>
-static int launch_forward(const ProductArgs& g, bool e8, const Plan& p, float* part, hipStream_t st) {
+static int launch_forward(const ProductArgs& g, bool e8, const Plan& p, float* parts, hipStream_t st) {
   using S = FwdShape<T, A, WT, WF>;
-  return launch_tiles(g, S::TT, S::FT, p, part, st, "fp8_block_matmul", [&](dim3 grid, TileOrder o) {
-    if (e8) hipLaunchKernelGGL((fp8_forward_kernel<T, A, WT, WF, true>), grid, dim3(S::NTH), 0, st, g, o, p.steps, part);
-    else    hipLaunchKernelGGL((fp8_forward_kernel<T, A, WT, WF, false>), grid, dim3(S::NTH), 0, st, g, o, p.steps, part);
+  return launch_tiles<S::TT, S::FT>(g, p, parts, st, "fp8_block_matmul", [&](dim3 grid, TileOrder o) {
+    if (e8) hipLaunchKernelGGL((fp8_forward_kernel<T, A, WT, WF, true>), grid, dim3(S::NTH), 0, st, g, o, p.steps, parts);
+    else    hipLaunchKernelGGL((fp8_forward_kernel<T, A, WT, WF, false>), grid, dim3(S::NTH), 0, st, g, o, p.steps, parts);
   });
 }
 template <int T, int WT>
-static int launch_grad_input(const ProductArgs& g, const Plan& p, float* part, hipStream_t st) {
+static int launch_grad_input(const ProductArgs& g, const Plan& p, float* parts, hipStream_t st) {
   using S = GradInputShape<T, WT>;
-  return launch_tiles(g, S::TT, S::FT, p, part, st, "fp8_block_grad_input", [&](dim3 grid, TileOrder o) {
-    hipLaunchKernelGGL((fp8_grad_input_kernel<T, WT>), grid, dim3(S::NTH), 0, st, g, o, p.steps, part);
+  return launch_tiles<S::TT, S::FT>(g, p, parts, st, "fp8_block_grad_input", [&](dim3 grid, TileOrder o) {
+    hipLaunchKernelGGL((fp8_grad_input_kernel<T, WT>), grid, dim3(S::NTH), 0, st, g, o, p.steps, parts);
   });
 }
 template <int MB, int NB2, int WK, int WN>
-static int launch_grad_weight(const ProductArgs& g, const Plan& p, float* part, hipStream_t st) {
+static int launch_grad_weight(const ProductArgs& g, const Plan& p, float* parts, hipStream_t st) {
   using S = GradWeightShape<MB, NB2, WK, WN>;
-  return launch_tiles(g, S::FN, S::FK, p, part, st, "fp8_block_grad_weight", [&](dim3 grid, TileOrder o) {
-    hipLaunchKernelGGL((fp8_grad_weight_kernel<MB, NB2, WK, WN>), grid, dim3(S::NTH), 0, st, g, o, p.steps, part);
+  return launch_tiles<S::FN, S::FK>(g, p, parts, st, "fp8_block_grad_weight", [&](dim3 grid, TileOrder o) {
+    hipLaunchKernelGGL((fp8_grad_weight_kernel<MB, NB2, WK, WN>), grid, dim3(S::NTH), 0, st, g, o, p.steps, parts);
   });
 }
 
@@ -1302,7 +1410,7 @@ using namespace mi355q;
 
 extern "C" size_t mi355q_fp8_block_matmul_workspace_size(int64_t rows, int64_t out, int64_t cols) {
   if (rows <= kFewTokens || out <= 0 || cols <= 0) return 0;
-  return plan_bytes(plan_tokens(rows, out, cols), rows, out);
+  return plan_bytes(plan_forward(rows, out, cols));
 }
 
 extern "C" int mi355q_fp8_block_matmul(const uint8_t* x_dev, int64_t ldx, const void* x_scales_dev,
@@ -1349,14 +1457,14 @@ extern "C" int mi355q_fp8_block_matmul(const uint8_t* x_dev, int64_t ldx, const 
     MQ_LAUNCH_CHECK();
     return MI355Q_OK;
   }
-  Plan p = plan_tokens(rows, out, cols);
-  float* const part = plan_workspace(p, rows, out, group_count(cols), workspace_dev, workspace_bytes);
-  return p.big ? launch_forward<2, 2, 2, 2>(g, e8, p, part, st) : launch_forward<1, 2, 2, 2>(g, e8, p, part, st);
+  Plan p = plan_forward(rows, out, cols);
+  float* const parts = plan_workspace(p, workspace_dev, workspace_bytes);
+  return p.shape ? launch_forward<2, 2, 2, 2>(g, e8, p, parts, st) : launch_forward<1, 2, 2, 2>(g, e8, p, parts, st);
 }
 
 extern "C" size_t mi355q_fp8_block_grad_input_workspace_size(int64_t rows, int64_t out, int64_t cols) {
   if (rows <= 0 || out <= 0 || cols <= 0) return 0;
-  return plan_bytes(plan_tokens(rows, cols, out), rows, cols);
+  return plan_bytes(plan_grad_input(rows, cols, out));
 }
 
 extern "C" int mi355q_fp8_block_grad_input(const uint16_t* dy_dev, int64_t lddy, const uint8_t* w_dev, int64_t ldw,
@@ -1386,14 +1494,14 @@ extern "C" int mi355q_fp8_block_grad_input(const uint16_t* dy_dev, int64_t lddy,
   const bool aligned = cols % 16 == 0 && ldw % 16 == 0 && out % 8 == 0 && lddy % 8 == 0 && aligned16(dy_dev) &&
                        aligned16(w_dev) && small_pitch(lddy) && small_pitch(ldw);
   if (!aligned) return launch_any<kGradInput>(g, MI355Q_BF16, st, "fp8_block_grad_input");
-  Plan p = plan_tokens(rows, cols, out);
-  float* const part = plan_workspace(p, rows, cols, group_count(out), workspace_dev, workspace_bytes);
-  return p.big ? launch_grad_input<2, 2>(g, p, part, st) : launch_grad_input<1, 2>(g, p, part, st);
+  Plan p = plan_grad_input(rows, cols, out);
+  float* const parts = plan_workspace(p, workspace_dev, workspace_bytes);
+  return p.shape ? launch_grad_input<2, 2>(g, p, parts, st) : launch_grad_input<1, 2>(g, p, parts, st);
 }
 
 extern "C" size_t mi355q_fp8_block_grad_weight_workspace_size(int64_t rows, int64_t out, int64_t cols) {
   if (rows <= 0 || out <= 0 || cols <= 0) return 0;
-  return plan_bytes(plan_weight(rows, out, cols), out, cols);
+  return plan_bytes(plan_weight(rows, out, cols));
 }
 
 extern "C" int mi355q_fp8_block_grad_weight(const uint16_t* dy_dev, int64_t lddy, const uint8_t* x_dev, int64_t ldx,
@@ -1424,6 +1532,6 @@ extern "C" int mi355q_fp8_block_grad_weight(const uint16_t* dy_dev, int64_t lddy
                        small_pitch(ld_x_scales);
   if (!aligned) return launch_any<kGradWeight>(g, dw_dtype, st, "fp8_block_grad_weight");
   Plan p = plan_weight(rows, out, cols);
-  float* const part = plan_workspace(p, out, cols, (rows + 31) / 32, workspace_dev, workspace_bytes);
-  return p.big ? launch_grad_weight<4, 2, 2, 4>(g, p, part, st) : launch_grad_weight<2, 2, 2, 2>(g, p, part, st);
+  float* const parts = plan_workspace(p, workspace_dev, workspace_bytes);
+  return p.shape ? launch_grad_weight<4, 2, 2, 4>(g, p, parts, st) : launch_grad_weight<2, 2, 2, 2>(g, p, parts, st);
 }
