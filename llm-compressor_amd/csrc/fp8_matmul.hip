@@ -1267,16 +1267,17 @@ struct Plan {
   uint32_t row_tiles, col_tiles, full, splits;
   int steps;          // of the sum, per split
 };
-// What a shape costs, in us: a step with one and with two workgroups on a CU
-// (one1, two; 0: only one fits), and what begins and ends a workgroup.
+// What a shape costs, in us: a step of one workgroup that has its CU to itself,
+// a step of two that share one (0: only one fits), and what begins and ends a
+// workgroup.
 struct ShapeCost {
   int tile_rows, tile_cols;
   double one, two, ends;
 };
 // The cheapest cut by these costs: every shape, whole tiles for as many rounds of
-// the 256 CUs as come out even or all, and 1 .. 16 parts for the rest, of at least
-// `least` steps.  Splits cost their partial sums' way through memory (written and read, at
-// 3.5 TB/s) and a second launch (4 us).
+// the 256 CUs as come out even (or none, for fewer), and 1 .. 16 parts of at least
+// `least` steps for the rest.  Parts cost a second launch (4 us) and their partial
+// sums' way to it (written and read, mostly in the caches: 8 TB/s).
 static Plan make_plan(const ShapeCost* shapes, int n, int64_t rows, int64_t cols, int64_t steps, int64_t least) {
   Plan best{};
   double best_cost = 0;
@@ -1284,18 +1285,22 @@ static Plan make_plan(const ShapeCost* shapes, int n, int64_t rows, int64_t cols
     const ShapeCost& c = shapes[i];
     const int64_t tr = (rows + c.tile_rows - 1) / c.tile_rows, tc = (cols + c.tile_cols - 1) / c.tile_cols;
     const int64_t tiles = tr * tc, even = tiles - tiles % 256;
-    const double pair = c.two > 0 ? c.two / 2 : c.one;   // a step of a workgroup that shares its CU
     for (int f = 0; f < (even > 0 ? 2 : 1); ++f) {
       const int64_t full = f ? even : 0, rest = tiles - full;
-      if (full == 0 && tiles > 1024) continue;           // (the partial sums of all tiles: never the cheapest)
+      if (full == 0 && tiles > 1024) continue;           // (partial sums of all tiles: never the cheapest)
       for (int64_t want = 1; want <= 16; ++want) {
         if (want > 1 && (rest == 0 || steps / want < least)) break;
         const int64_t per = (steps + want - 1) / want, k = (steps + per - 1) / per;
-        const int64_t wgs = rest * k, rounds = (wgs + 255) / 256;
-        double t = (double)(full / 256) * (steps * pair + c.ends);
-        if (full == 0 && rounds == 1) t += per * c.one + c.ends;
-        else t += rounds * (per * pair + c.ends);
-        if (k > 1) t += 4 + (double)wgs * c.tile_rows * c.tile_cols * 8 / 3.5e6;
+        const int64_t wgs = rest * k, whole = full / 256, parts = (wgs + 255) / 256;
+        // rounds run in pairs where two workgroups fit a CU; an odd last one runs alone
+        double t;
+        if (c.two > 0) {
+          t = (whole * steps + parts * per) * c.two / 2 + ((whole + parts + 1) / 2) * c.ends;
+          if ((whole + parts) % 2) t += (parts ? per : steps) * (c.one - c.two / 2);
+        } else {
+          t = (whole * steps + parts * per) * c.one + (whole + parts) * c.ends;
+        }
+        if (k > 1) t += 4 + (double)wgs * c.tile_rows * c.tile_cols * 8 / 8e6;
         if (best.tile_rows == 0 || t < best_cost) {
           best_cost = t;
           best = Plan{i, (uint32_t)c.tile_rows, (uint32_t)c.tile_cols, (uint32_t)tr, (uint32_t)tc,
@@ -1306,18 +1311,26 @@ static Plan make_plan(const ShapeCost* shapes, int n, int64_t rows, int64_t cols
   }
   return best;
 }
-// forward and input gradient: `rows` tokens by `cols` columns, `sum` terms in
-// blocks of 128
+// Forward and input gradient: `rows` tokens by `cols` columns, `sum` terms in
+// blocks of 128.  Measured, forward: 1024 x 4096 x 4096 in 256 tiles of 128 x 128 40 us,
+// in 512 of 64 x 128 41; 100 x 4096 x 4096 in 32 tiles of 128 x 128 36 us, 64 of 64 x 128 28,
+// these in 2 / 4 / 8 parts 19 / 16 / 19; 333 x 4096 x 14336 in 96 tiles of 128 x 128 110 us,
+// in 2 / 5 / 8 parts 73 / 58 / 61, in 192 of 64 x 128 in 1 / 4 parts 92 / 64.
 static Plan plan_forward(int64_t rows, int64_t cols, int64_t sum) {
-  static const ShapeCost shapes[] = {{64, 128, 0.72, 1.14, 3}, {128, 128, 1.10, 2.0, 4}};
+  static const ShapeCost shapes[] = {{64, 128, 0.69, 1.0, 4}, {128, 128, 0.93, 1.75, 4}};
   return make_plan(shapes, 2, rows, cols, group_count(sum), 4);
 }
+// Input gradient: 1024 x 4096 x 4096 48 us in 256 tiles of 128 x 128, 46 in 512 of 64 x 128;
+// 16 x 4096 x 4096 44 us and 35, these in 2 / 4 / 8 / 16 parts 22 / 14 / 11 / 12.
 static Plan plan_grad_input(int64_t rows, int64_t cols, int64_t sum) {
-  static const ShapeCost shapes[] = {{64, 128, 0.95, 1.28, 3}, {128, 128, 1.25, 2.1, 4}};
+  static const ShapeCost shapes[] = {{64, 128, 0.95, 1.2, 4}, {128, 128, 1.2, 2.1, 4}};
   return make_plan(shapes, 2, rows, cols, group_count(sum), 2);
 }
+// Weight gradient, in stages of 32 tokens: 8192 x 1024 x 4096 in 256 tiles of 128 x 128 106 us, in
+// 64 of 256 x 256 in 1 / 2 / 4 / 8 parts 216 / 127 / 89 / 108; 517 x 768 x 2048 in 96 of 128 x 128
+// 12 us, in 24 of 256 x 256 22; 1024 x 4096 x 4096 in 256 of 256 x 256 39 us, 1024 of 128 x 128 60.
 static Plan plan_weight(int64_t rows, int64_t out, int64_t cols) {
-  static const ShapeCost shapes[] = {{128, 128, 0.46, 0.76, 3}, {256, 256, 1.0, 0, 8}};
+  static const ShapeCost shapes[] = {{128, 128, 0.39, 0.7, 4}, {256, 256, 0.9, 0, 8}};
   return make_plan(shapes, 2, out, cols, (rows + 31) / 32, 4);
 }
 static size_t plan_bytes(const Plan& p) {
