@@ -1156,7 +1156,8 @@ __global__ __launch_bounds__(256) void sum_splits_kernel(ProductArgs g, TileOrde
 
 // ---------------------------------------------------------------- forward, few tokens
 // Up to 16 TF tokens: the weight is read once, straight into the MFMA's
-// registers (lane l: row l & 15, 32 bytes at 32 (l / 16) of the step's 128), the
+// registers (lane l: row l & 15, 16 bytes each at 16 (l / 16) of
+// both halves of the step's 128, so that a load takes 64 bytes of 16 rows), the
 // tokens come from L2, and the W waves of a workgroup take every W-th step of 16 AF
 // features; their sums are joined in LDS.  Bound by the weight's bytes, so what
 // counts is loads in flight: U steps are requested before the first is used.
@@ -1169,7 +1170,7 @@ __global__ __launch_bounds__(64 * W) void fp8_few_kernel(ProductArgs g) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t f0 = (int64_t)blockIdx.x * 16 * AF;
   const int nkb = (int)((g.R + kGroup - 1) / kGroup);
-  const int koff = 32 * (lane >> 4);
+  const int koff = 16 * (lane >> 4);
   const uint8_t* wp[AF];
   const uint8_t* xp[TF];
   int64_t xsi[TF];
@@ -1195,7 +1196,7 @@ __global__ __launch_bounds__(64 * W) void fp8_few_kernel(ProductArgs g) {
     // chunks past the last column are zeros (the columns are a multiple of 16)
     const i32x4_t z = {0, 0, 0, 0};
     const i32x4_t lo = k + koff < g.R ? *reinterpret_cast<const i32x4_t*>(p + k) : z;
-    const i32x4_t hi = k + koff + 16 < g.R ? *reinterpret_cast<const i32x4_t*>(p + k + 16) : z;
+    const i32x4_t hi = k + koff + 64 < g.R ? *reinterpret_cast<const i32x4_t*>(p + k + 64) : z;
     return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
   };
   for (int s0 = wave; s0 < nkb; s0 += W * U) {
@@ -1360,7 +1361,9 @@ static int launch_any(ProductArgs g, mi355q_dtype out, hipStream_t st, const cha
   return MI355Q_OK;
 }
 
-constexpr int64_t kFewTokens = 64;
+// Up to here the weight's bytes decide (24 x 4096 x 4096 12 us against 18 in tiles, 24 x 14336 x 4096 23
+// against 25); beyond, 48 tokens took 15 .. 17 us against 18, but 35 .. 47 against 28.
+constexpr int64_t kFewTokens = 32;
 
 template <int TF, int AF, int W, int U>
 static void launch_few_shape(const ProductArgs& g, bool e8, hipStream_t st) {
@@ -1369,9 +1372,10 @@ static void launch_few_shape(const ProductArgs& g, bool e8, hipStream_t st) {
   else    hipLaunchKernelGGL((fp8_few_kernel<TF, AF, W, U, false>), grid, dim3(64 * W), 0, st, g);
 }
 static void launch_few(const ProductArgs& g, bool e8, hipStream_t st) {
-  if (g.P <= 16) launch_few_shape<1, 1, 4, 4>(g, e8, st);
-  else if (g.P <= 32) launch_few_shape<2, 1, 8, 2>(g, e8, st);
-  else launch_few_shape<4, 2, 8, 1>(g, e8, st);
+  // (one token: 4096 x 14336 16 us on eight waves, 18 on four; 14336 x 4096 18 on either)
+  if (g.P <= 16 && g.R > 8192) launch_few_shape<1, 1, 8, 4>(g, e8, st);
+  else if (g.P <= 16) launch_few_shape<1, 1, 4, 4>(g, e8, st);
+  else launch_few_shape<2, 2, 8, 1>(g, e8, st);
 }
 
 // Runs `kernel(grid, order)` over the plan's items and adds up its splits.

@@ -7,6 +7,7 @@ current stream.  All tensors must live on a ROCm GPU; there is no CPU path.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 
 import torch
 
@@ -661,47 +662,71 @@ def _fp8_groups(n: int) -> int:
     return -(-n // FP8_GROUP)
 
 
+# These calls take a few microseconds on the device at serving sizes, so the
+# checks are written to cost little: one pass over each operand's attributes, and
+# the workspace sizes, which depend on the shape alone, looked up.
+def _rows_2d(t: torch.Tensor) -> torch.Tensor:
+    """t with contiguous rows that do not overlap."""
+    pitch, step = t.stride()
+    return t if step == 1 and pitch >= t.shape[1] else t.contiguous()
+
+
 def _fp8_source(x: torch.Tensor, what: str) -> torch.Tensor:
     """x as a 2-D matrix with contiguous rows of bf16, fp16 or fp32."""
-    L.require_gpu(x)
+    if not x.is_cuda:
+        L.require_gpu(x)
     if x.dtype not in _FP8_DT:
         raise TypeError(f"{what} must be bf16, fp16 or fp32, got {x.dtype}")
     if x.dim() != 2 or x.shape[1] == 0:
         raise ValueError(f"{what} must be a 2-D matrix with columns, got {tuple(x.shape)}")
-    return x if x.stride(1) == 1 and x.stride(0) >= x.shape[1] else x.contiguous()
+    return _rows_2d(x)
 
 
 def _fp8_matrix(codes: torch.Tensor, scales: torch.Tensor, what: str, blocks: bool, scale_dtypes):
     """A checked fp8 matrix: e4m3 codes [rows, cols] and its scales."""
-    L.require_gpu(codes, scales)
+    if not (codes.is_cuda and scales.is_cuda):
+        L.require_gpu(codes, scales)
     if codes.dtype != torch.float8_e4m3fn or codes.dim() != 2 or codes.shape[1] == 0:
         raise TypeError(f"{what} must be a 2-D float8_e4m3fn matrix with columns, got {tuple(codes.shape)} "
                         f"{codes.dtype}")
-    rows = _fp8_groups(codes.shape[0]) if blocks else codes.shape[0]
-    want = (rows, _fp8_groups(codes.shape[1]))
+    rows, cols = codes.shape
+    want = (_fp8_groups(rows) if blocks else rows, _fp8_groups(cols))
     if scales.dtype not in scale_dtypes:
         raise TypeError(f"{what} scales must be {' or '.join(str(d) for d in scale_dtypes)}, got {scales.dtype}")
-    if tuple(scales.shape) != want:
-        raise ValueError(f"{what} of {tuple(codes.shape)} takes scales of {want}, got {tuple(scales.shape)}")
-    if codes.stride(1) != 1 or codes.stride(0) < codes.shape[1]:
-        codes = codes.contiguous()
-    if scales.stride(1) != 1 or scales.stride(0) < scales.shape[1]:
-        scales = scales.contiguous()
-    return codes, scales
+    if scales.shape != want:
+        raise ValueError(f"{what} of {(rows, cols)} takes scales of {want}, got {tuple(scales.shape)}")
+    return _rows_2d(codes), _rows_2d(scales)
 
 
 def _fp8_gradient(dy: torch.Tensor, cols: int) -> torch.Tensor:
-    L.require_gpu(dy)
+    if not dy.is_cuda:
+        L.require_gpu(dy)
     if dy.dtype != torch.bfloat16:
         raise TypeError(f"the output gradient must be bf16, got {dy.dtype}")
     if dy.dim() != 2 or dy.shape[1] != cols:
         raise ValueError(f"the output gradient must be [rows, {cols}], got {tuple(dy.shape)}")
-    return dy if dy.stride(1) == 1 and dy.stride(0) >= cols else dy.contiguous()
+    return _rows_2d(dy)
 
 
-def _one_device(*tensors) -> None:
-    if len({t.device for t in tensors if t is not None}) > 1:
-        raise ValueError(f"operands on several devices: {[str(t.device) for t in tensors if t is not None]}")
+def _one_device(first: torch.Tensor, *others) -> None:
+    here = first.get_device()
+    for t in others:
+        if t is not None and t.get_device() != here:
+            raise ValueError(f"operands on several devices: {first.device} and {t.device}")
+
+
+@functools.lru_cache(maxsize=4096)
+def _fp8_workspace(query: str, rows: int, out: int, cols: int) -> int:
+    return getattr(L.lib(), query)(rows, out, cols)
+
+
+def _fp8_scratch(query: str, rows: int, out: int, cols: int, like: torch.Tensor):
+    """(workspace or None to keep alive over the call, its address, its bytes)"""
+    n = _fp8_workspace(query, rows, out, cols)
+    if n == 0:
+        return None, None, 0
+    ws = torch.empty(n, dtype=torch.uint8, device=like.device)
+    return ws, ws.data_ptr(), n
 
 
 def fp8_quantize_groups(x: torch.Tensor, scale_dtype: torch.dtype = torch.float32):
@@ -716,10 +741,13 @@ def fp8_quantize_groups(x: torch.Tensor, scale_dtype: torch.dtype = torch.float3
     if scale_dtype not in _FP8_SCALES:
         raise TypeError(f"scale_dtype must be float32 or float8_e8m0fnu, got {scale_dtype}")
     rows, cols = x.shape
-    codes = torch.empty((rows, cols), dtype=torch.float8_e4m3fn, device=x.device)
-    scales = torch.empty((rows, _fp8_groups(cols)), dtype=scale_dtype, device=x.device)
-    L.call("mi355q_fp8_quantize_groups", x.data_ptr(), _FP8_DT[x.dtype], rows, cols, x.stride(0), codes.data_ptr(),
-           cols, scales.data_ptr(), _FP8_SCALES[scale_dtype], scales.shape[1], L.stream_of(x))
+    groups = _fp8_groups(cols)
+    codes = x.new_empty((rows, cols), dtype=torch.float8_e4m3fn)
+    scales = x.new_empty((rows, groups), dtype=scale_dtype)
+    rc = L.lib().mi355q_fp8_quantize_groups(x.data_ptr(), _FP8_DT[x.dtype], rows, cols, x.stride(0), codes.data_ptr(),
+                                            cols, scales.data_ptr(), _FP8_SCALES[scale_dtype], groups, L.stream_of(x))
+    if rc:
+        L.check(rc)
     return codes, scales
 
 
@@ -745,7 +773,7 @@ def fp8_block_matmul(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w
     block (``fp8_quantize_blocks``, or an FP8_BLOCK checkpoint's
     ``weight_scale`` in fp32).  Sums in fp32, rounded once to ``out_dtype``
     (bf16, fp16 or fp32).  ``bias`` [out] is bf16, fp16 or fp32."""
-    x, x_scales = _fp8_matrix(x, x_scales, "x", False, tuple(_FP8_SCALES))
+    x, x_scales = _fp8_matrix(x, x_scales, "x", False, _FP8_SCALES)
     w, w_scales = _fp8_matrix(w, w_scales, "w", True, (torch.float32,))
     rows, cols = x.shape
     out = w.shape[0]
@@ -754,21 +782,23 @@ def fp8_block_matmul(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w
     if out_dtype not in _FP8_DT:
         raise TypeError(f"out_dtype must be bf16, fp16 or fp32, got {out_dtype}")
     if bias is not None:
-        L.require_gpu(bias)
+        if not bias.is_cuda:
+            L.require_gpu(bias)
         if bias.dtype not in _FP8_DT:
             raise TypeError(f"bias must be bf16, fp16 or fp32, got {bias.dtype}")
         if bias.shape != (out,):
             raise ValueError(f"bias must be [{out}], got {tuple(bias.shape)}")
         bias = bias.contiguous()
     _one_device(x, x_scales, w, w_scales, bias)
-    y = torch.empty((rows, out), dtype=out_dtype, device=x.device)
-    lib = L.lib()
-    ws = _ws(lib.mi355q_fp8_block_matmul_workspace_size(rows, out, cols), x.device)
-    L.check(lib.mi355q_fp8_block_matmul(
+    y = x.new_empty((rows, out), dtype=out_dtype)
+    ws, ws_ptr, ws_bytes = _fp8_scratch("mi355q_fp8_block_matmul_workspace_size", rows, out, cols, x)
+    rc = L.lib().mi355q_fp8_block_matmul(
         x.data_ptr(), x.stride(0), x_scales.data_ptr(), _FP8_SCALES[x_scales.dtype], x_scales.stride(0), w.data_ptr(),
-        w.stride(0), w_scales.data_ptr(), w_scales.stride(0), L.ptr(bias), _FP8_DT[bias.dtype] if bias is not None else 0,
-        y.data_ptr(), _FP8_DT[out_dtype], out, rows, out, cols, L.ptr(ws), 0 if ws is None else ws.numel(),
-        L.stream_of(x)))
+        w.stride(0), w_scales.data_ptr(), w_scales.stride(0), None if bias is None else bias.data_ptr(),
+        0 if bias is None else _FP8_DT[bias.dtype], y.data_ptr(), _FP8_DT[out_dtype], out, rows, out, cols, ws_ptr,
+        ws_bytes, L.stream_of(x))
+    if rc:
+        L.check(rc)
     return y
 
 
@@ -783,12 +813,13 @@ def fp8_block_grad_input(dy: torch.Tensor, w: torch.Tensor, w_scales: torch.Tens
         raise ValueError("w has no rows")
     _one_device(dy, w, w_scales)
     rows = dy.shape[0]
-    dx = torch.empty((rows, cols), dtype=torch.bfloat16, device=dy.device)
-    lib = L.lib()
-    ws = _ws(lib.mi355q_fp8_block_grad_input_workspace_size(rows, out, cols), dy.device)
-    L.check(lib.mi355q_fp8_block_grad_input(dy.data_ptr(), dy.stride(0), w.data_ptr(), w.stride(0),
-                                            w_scales.data_ptr(), w_scales.stride(0), dx.data_ptr(), cols, rows, out,
-                                            cols, L.ptr(ws), 0 if ws is None else ws.numel(), L.stream_of(dy)))
+    dx = dy.new_empty((rows, cols))
+    ws, ws_ptr, ws_bytes = _fp8_scratch("mi355q_fp8_block_grad_input_workspace_size", rows, out, cols, dy)
+    rc = L.lib().mi355q_fp8_block_grad_input(dy.data_ptr(), dy.stride(0), w.data_ptr(), w.stride(0),
+                                             w_scales.data_ptr(), w_scales.stride(0), dx.data_ptr(), cols, rows, out,
+                                             cols, ws_ptr, ws_bytes, L.stream_of(dy))
+    if rc:
+        L.check(rc)
     return dx
 
 
@@ -808,13 +839,14 @@ def fp8_block_grad_weight(dy: torch.Tensor, x: torch.Tensor, x_scales: torch.Ten
     if out_dtype not in _FP8_DT:
         raise TypeError(f"out_dtype must be bf16, fp16 or fp32, got {out_dtype}")
     _one_device(dy, x, x_scales)
-    dw = torch.empty((out, cols), dtype=out_dtype, device=dy.device)
-    lib = L.lib()
-    ws = _ws(lib.mi355q_fp8_block_grad_weight_workspace_size(rows, out, cols), dy.device)
-    L.check(lib.mi355q_fp8_block_grad_weight(dy.data_ptr(), dy.stride(0), x.data_ptr(), x.stride(0),
-                                             x_scales.data_ptr(), x_scales.stride(0), dw.data_ptr(),
-                                             _FP8_DT[out_dtype], cols, rows, out, cols, L.ptr(ws),
-                                             0 if ws is None else ws.numel(), L.stream_of(dy)))
+    dw = dy.new_empty((out, cols), dtype=out_dtype)
+    ws, ws_ptr, ws_bytes = _fp8_scratch("mi355q_fp8_block_grad_weight_workspace_size", rows, out, cols, dy)
+    rc = L.lib().mi355q_fp8_block_grad_weight(dy.data_ptr(), dy.stride(0), x.data_ptr(), x.stride(0),
+                                              x_scales.data_ptr(), x_scales.stride(0), dw.data_ptr(),
+                                              _FP8_DT[out_dtype], cols, rows, out, cols, ws_ptr, ws_bytes,
+                                              L.stream_of(dy))
+    if rc:
+        L.check(rc)
     return dw
 
 
@@ -829,15 +861,15 @@ def fp8_silu_mul(gate_up: torch.Tensor, save: bool = True):
     if x.shape[1] % 2:
         raise ValueError(f"gate_up must hold gate and up side by side, got {x.shape[1]} columns")
     groups = _fp8_groups(cols)
-
-    def new(width, dtype):
-        return torch.empty((rows, width), dtype=dtype, device=x.device)
-
-    h, hs = new(cols, torch.float8_e4m3fn), new(groups, torch.float8_e8m0fnu)
-    kept = new(2 * cols, torch.float8_e4m3fn) if save else None
-    ks = new(2 * groups, torch.float8_e8m0fnu) if save else None
-    L.call("mi355q_fp8_silu_mul", x.data_ptr(), _FP8_DT[x.dtype], rows, cols, x.stride(0), h.data_ptr(), cols,
-           hs.data_ptr(), L.ptr(kept), 2 * cols, L.ptr(ks), L.stream_of(x))
+    h = x.new_empty((rows, cols), dtype=torch.float8_e4m3fn)
+    hs = x.new_empty((rows, groups), dtype=torch.float8_e8m0fnu)
+    kept = x.new_empty((rows, 2 * cols), dtype=torch.float8_e4m3fn) if save else None
+    ks = x.new_empty((rows, 2 * groups), dtype=torch.float8_e8m0fnu) if save else None
+    rc = L.lib().mi355q_fp8_silu_mul(x.data_ptr(), _FP8_DT[x.dtype], rows, cols, x.stride(0), h.data_ptr(), cols,
+                                     hs.data_ptr(), kept.data_ptr() if save else None, 2 * cols,
+                                     ks.data_ptr() if save else None, L.stream_of(x))
+    if rc:
+        L.check(rc)
     return (h, hs, kept, ks) if save else (h, hs)
 
 
@@ -845,23 +877,24 @@ def fp8_silu_mul_backward(dh: torch.Tensor, saved: torch.Tensor, saved_scales: t
     """The gradient [rows, 2 n] of ``fp8_silu_mul``'s input, in dh's type,
     from dh [rows, n] (bf16, fp16 or fp32) and what the forward pass saved."""
     dh = _fp8_source(dh, "dh")
-    L.require_gpu(saved, saved_scales)
+    if not (saved.is_cuda and saved_scales.is_cuda):
+        L.require_gpu(saved, saved_scales)
     rows, cols = dh.shape
+    groups = _fp8_groups(cols)
     if saved.dtype != torch.float8_e4m3fn or saved_scales.dtype != torch.float8_e8m0fnu:
         raise TypeError(f"saved codes and scales must be float8_e4m3fn and float8_e8m0fnu, got {saved.dtype} and "
                         f"{saved_scales.dtype}")
-    if tuple(saved.shape) != (rows, 2 * cols) or tuple(saved_scales.shape) != (rows, 2 * _fp8_groups(cols)):
-        raise ValueError(f"dh of {tuple(dh.shape)} takes saved codes of {(rows, 2 * cols)} and scales of "
-                         f"{(rows, 2 * _fp8_groups(cols))}, got {tuple(saved.shape)} and {tuple(saved_scales.shape)}")
+    if saved.shape != (rows, 2 * cols) or saved_scales.shape != (rows, 2 * groups):
+        raise ValueError(f"dh of {(rows, cols)} takes saved codes of {(rows, 2 * cols)} and scales of "
+                         f"{(rows, 2 * groups)}, got {tuple(saved.shape)} and {tuple(saved_scales.shape)}")
     _one_device(dh, saved, saved_scales)
-    if saved.stride(1) != 1 or saved.stride(0) < 2 * cols:
-        saved = saved.contiguous()
-    if saved_scales.stride(1) != 1 or saved_scales.stride(0) < saved_scales.shape[1]:
-        saved_scales = saved_scales.contiguous()
-    dx = torch.empty((rows, 2 * cols), dtype=dh.dtype, device=dh.device)
-    L.call("mi355q_fp8_silu_mul_backward", dh.data_ptr(), _FP8_DT[dh.dtype], rows, cols, dh.stride(0),
-           saved.data_ptr(), saved.stride(0), saved_scales.data_ptr(), saved_scales.stride(0), dx.data_ptr(),
-           2 * cols, L.stream_of(dh))
+    saved, saved_scales = _rows_2d(saved), _rows_2d(saved_scales)
+    dx = dh.new_empty((rows, 2 * cols))
+    rc = L.lib().mi355q_fp8_silu_mul_backward(dh.data_ptr(), _FP8_DT[dh.dtype], rows, cols, dh.stride(0),
+                                              saved.data_ptr(), saved.stride(0), saved_scales.data_ptr(),
+                                              saved_scales.stride(0), dx.data_ptr(), 2 * cols, L.stream_of(dh))
+    if rc:
+        L.check(rc)
     return dx
 
 
