@@ -547,8 +547,12 @@ int mi355q_fp8_quantize_blocks(const void* w_dev, mi355q_dtype dtype, int64_t ro
  *   x_scales[m][kb] * w_scales[n / 128][kb] * sum_{k in kb} x[m][k] w[n][k]
  * x codes [rows, cols], w codes [out, cols], y [rows, out] in y_dtype, rounded
  * once from fp32; bias_dev may be NULL (bias_dtype then unused).  Code
- * products are exact in fp32.  rows may be 0.  Workspace: the queried size, or
- * NULL / 0: the sum over the columns is then not split over workgroups. */
+ * products are exact in fp32.  rows may be 0.  Any leading dimension and
+ * alignment.  Workspace (16-byte aligned): the queried size; with less the sum is
+ * not split over workgroups, and operands that are not 16-byte aligned with rows
+ * of whole 16-byte chunks take a slow kernel instead of a padded copy (the query
+ * counts the copies where cols is no multiple of 16; operands that lie badly
+ * although it is are not copied). */
 size_t mi355q_fp8_block_matmul_workspace_size(int64_t rows, int64_t out, int64_t cols);
 int mi355q_fp8_block_matmul(const uint8_t* x_dev, int64_t ldx, const void* x_scales_dev,
                             mi355q_scale_type x_scale_type, int64_t ld_x_scales, const uint8_t* w_dev,

@@ -634,7 +634,8 @@ void fp8_grad_input_kernel(ProductArgs g, TileOrder order, int blocks_per_split,
   static_assert(NB % 2 == 0, "a wave's token rows begin at a multiple of 16");
   const int chunk = (lane & 7) ^ (lane >> 3), ychunk[2] = {(lane & 7) ^ (lane >> 4), (lane & 7) ^ (4 + (lane >> 4))};
   const int last_rows = (int)(g.R - (int64_t)(nst - 1) * S::SN);
-  const int64_t wcol = f0 + 16 * chunk < g.Q ? f0 + 16 * chunk : g.Q - 16;
+  const int64_t wide = (g.Q + 15) & ~int64_t(15);   // (a padded copy's width)
+  const int64_t wcol = f0 + 16 * chunk < wide ? f0 + 16 * chunk : wide - 16;
   uint32_t oa[NA], ob[NB];
 #pragma unroll
   for (int j = 0; j < NA; ++j)
@@ -647,16 +648,16 @@ void fp8_grad_input_kernel(ProductArgs g, TileOrder order, int blocks_per_split,
   const char* const wbase = reinterpret_cast<const char*>(g.b) + f0;
   const char* const ybase = static_cast<const char*>(g.a) + 2 * t0 * g.lda;
   const uint32_t la0 = lds_u32(ring) + wave * NA * 1024, lb0 = lds_u32(ringb) + wave * NB * 1024;
-  const int tail = (int)(g.R % S::SN) / 8;
+  const int tail = (int)((g.R + 7) / 8 % (S::SN / 8));   // whole chunks of dY (the last one may be padded)
   auto turn_to_tail = [&](int s) __attribute__((always_inline)) {   // once, before the last step's DMA
-    if (tail && s == nst - 1) {
+    if (last_rows < S::SN && s == nst - 1) {
 #pragma unroll
       for (int j = 0; j < NA; ++j) {
         const int r = (wave * NA + j) * 8 + (lane >> 3);
         oa[j] -= r >= last_rows ? (uint32_t)(r - (last_rows - 1)) * (uint32_t)g.ldb : 0u;
       }
 #pragma unroll
-      for (int j = 0; j < NB; ++j) ob[j] -= ychunk[j & 1] >= tail ? 16 * ychunk[j & 1] : 0;
+      for (int j = 0; j < NB; ++j) ob[j] -= tail && ychunk[j & 1] >= tail ? 16 * ychunk[j & 1] : 0;
     }
   };
   auto load_a = [&](int s, int slot, int j) __attribute__((always_inline)) {
@@ -841,17 +842,18 @@ void fp8_grad_weight_kernel(ProductArgs g, TileOrder order, int stages_per_split
   // (not stored), tokens past the end the last one (cleared in LDS, as are
   // their checkpoint rows: an infinity there must not meet a zero).
   constexpr int YC = S::FN / 8, RPI = 64 / YC, NY = S::SM / RPI / S::W;
+  const int64_t ywide = (g.P + 7) & ~int64_t(7), xwide = (g.Q + 15) & ~int64_t(15);   // (padded copies' widths)
   uint32_t oy[NY];
 #pragma unroll
   for (int j = 0; j < NY; ++j) {
     const int row = (wave * NY + j) * RPI + lane / YC;
-    const int64_t col = n0 + 8 * ((lane % YC) ^ (4 * (row & 3))), c = col < g.P ? col : g.P - 8;
+    const int64_t col = n0 + 8 * ((lane % YC) ^ (4 * (row & 3))), c = col < ywide ? col : ywide - 8;
     oy[j] = (uint32_t)row * (uint32_t)(2 * g.lda) + (uint32_t)(2 * (c - n0));
   }
   // ... of the checkpoint: lane l takes 16 codes of row XR l / XC of the wave's
   constexpr int XC = S::FK / 16, XR = 64 / XC;
   const int xrow = wave * XR + lane / XC, xch = lane % XC;
-  const int64_t xcol = k0 + 16 * xch < g.Q ? k0 + 16 * xch : g.Q - 16;
+  const int64_t xcol = k0 + 16 * xch < xwide ? k0 + 16 * xch : xwide - 16;
   uint32_t ox = (uint32_t)xrow * (uint32_t)g.ldb + (uint32_t)(xcol - k0);
   uint32_t oe = (uint32_t)xrow * (uint32_t)g.ldbs + (uint32_t)(xcol / kGroup - k0 / kGroup);
   // before the last stage's DMA, once (dY's turn comes a stage after the checkpoint's)
@@ -1164,7 +1166,7 @@ __global__ __launch_bounds__(256) void sum_splits_kernel(ProductArgs g, TileOrde
 typedef int i32x4_t __attribute__((ext_vector_type(4)));
 typedef int i32x8_t __attribute__((ext_vector_type(8)));
 
-template <int TF, int AF, int W, int U, bool E8M0>
+template <int TF, int AF, int W, int U, bool E8M0, bool ALIGNED>
 __global__ __launch_bounds__(64 * W) void fp8_few_kernel(ProductArgs g) {
   __shared__ f32x4_t sums[W][AF][TF][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -1192,12 +1194,25 @@ __global__ __launch_bounds__(64 * W) void fp8_few_kernel(ProductArgs g) {
 #pragma unroll
     for (int b = 0; b < TF; ++b) acc[a][b] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 
+  // 16 codes from column k, zeros past the last one: rows that are a multiple of 16
+  // wide and aligned have a chunk inside or outside as a whole
+  auto load16 = [&](const uint8_t* p, int64_t k) __attribute__((always_inline)) {
+    i32x4_t v = {0, 0, 0, 0};
+    const int64_t left = g.R - k - koff;
+    if constexpr (ALIGNED) {
+      if (left > 0) v = *reinterpret_cast<const i32x4_t*>(p + k);
+    } else if (left >= 16) {
+      __builtin_memcpy(&v, p + k, 16);
+    } else {
+      uint8_t b[16];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) b[e] = e < left ? p[k + e] : 0;
+      __builtin_memcpy(&v, b, 16);
+    }
+    return v;
+  };
   auto load32 = [&](const uint8_t* p, int64_t k) __attribute__((always_inline)) {
-    // chunks past the last column are zeros (the columns are a multiple of 16)
-    const i32x4_t z = {0, 0, 0, 0};
-    const i32x4_t lo = k + koff < g.R ? *reinterpret_cast<const i32x4_t*>(p + k) : z;
-    const i32x4_t hi = k + koff + 64 < g.R ? *reinterpret_cast<const i32x4_t*>(p + k + 64) : z;
-    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    return __builtin_shufflevector(load16(p, k), load16(p, k + 64), 0, 1, 2, 3, 4, 5, 6, 7);
   };
   for (int s0 = wave; s0 < nkb; s0 += W * U) {
     i32x8_t wa[U][AF], xb[U][TF];
@@ -1366,16 +1381,21 @@ static int launch_any(ProductArgs g, mi355q_dtype out, hipStream_t st, const cha
 constexpr int64_t kFewTokens = 32;
 
 template <int TF, int AF, int W, int U>
-static void launch_few_shape(const ProductArgs& g, bool e8, hipStream_t st) {
-  const dim3 grid((unsigned)((g.Q + 16 * AF - 1) / (16 * AF)));
-  if (e8) hipLaunchKernelGGL((fp8_few_kernel<TF, AF, W, U, true>), grid, dim3(64 * W), 0, st, g);
-  else    hipLaunchKernelGGL((fp8_few_kernel<TF, AF, W, U, false>), grid, dim3(64 * W), 0, st, g);
+static void launch_few_shape(const ProductArgs& g, bool e8, bool aligned, hipStream_t st) {
+  const dim3 grid((unsigned)((g.Q + 16 * AF - 1) / (16 * AF))), block(64 * W);
+  if (aligned) {
+    if (e8) hipLaunchKernelGGL((fp8_few_kernel<TF, AF, W, U, true, true>), grid, block, 0, st, g);
+    else    hipLaunchKernelGGL((fp8_few_kernel<TF, AF, W, U, false, true>), grid, block, 0, st, g);
+  } else {
+    if (e8) hipLaunchKernelGGL((fp8_few_kernel<TF, AF, W, U, true, false>), grid, block, 0, st, g);
+    else    hipLaunchKernelGGL((fp8_few_kernel<TF, AF, W, U, false, false>), grid, block, 0, st, g);
+  }
 }
-static void launch_few(const ProductArgs& g, bool e8, hipStream_t st) {
+static void launch_few(const ProductArgs& g, bool e8, bool aligned, hipStream_t st) {
   // (one token: 4096 x 14336 16 us on eight waves, 18 on four; 14336 x 4096 18 on either)
-  if (g.P <= 16 && g.R > 8192) launch_few_shape<1, 1, 8, 4>(g, e8, st);
-  else if (g.P <= 16) launch_few_shape<1, 1, 4, 4>(g, e8, st);
-  else launch_few_shape<2, 2, 8, 1>(g, e8, st);
+  if (g.P <= 16 && g.R > 8192) launch_few_shape<1, 1, 8, 4>(g, e8, aligned, st);
+  else if (g.P <= 16) launch_few_shape<1, 1, 4, 4>(g, e8, aligned, st);
+  else launch_few_shape<2, 2, 8, 1>(g, e8, aligned, st);
 }
 
 // Runs `kernel(grid, order)` over the plan's items and adds up its splits.
@@ -1418,6 +1438,41 @@ static int launch_grad_weight(const ProductArgs& g, const Plan& p, float* parts,
   });
 }
 
+// ---------------------------------------------------------------- rows of odd widths
+// The tile kernels take operands in 16-byte chunks.  Rows whose width is no whole
+// number of them are first copied to rows that are, ending in zeros.
+__global__ __launch_bounds__(256) void pad_rows_kernel(const uint8_t* src, int64_t pitch, int64_t row_bytes,
+                                                       uint8_t* dst, uint32_t chunks, FastDiv per_row) {
+  const uint32_t i = blockIdx.x * 256 + threadIdx.x;
+  if (i >= chunks) return;
+  const uint32_t r = div(i, per_row);
+  const int64_t at = (int64_t)(i - r * per_row.d) * 16, left = row_bytes - at;
+  const uint8_t* p = src + r * pitch + at;
+  u32x4_t v;
+  if (left >= 16) {
+    __builtin_memcpy(&v, p, 16);
+  } else {
+    uint8_t b[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) b[e] = e < left ? p[e] : 0;
+    __builtin_memcpy(&v, b, 16);
+  }
+  *reinterpret_cast<u32x4_t*>(dst + (int64_t)i * 16) = v;
+}
+static int64_t padded(int64_t row_bytes) { return (row_bytes + 15) / 16 * 16; }
+static size_t padded_bytes(int64_t rows, int64_t row_bytes) { return (size_t)rows * padded(row_bytes); }
+static int pad_rows(const void* src, int64_t pitch, int64_t rows, int64_t row_bytes, void* dst, hipStream_t st) {
+  const int64_t per = padded(row_bytes) / 16, most = ((int64_t(1) << 31) - 256) / per;
+  for (int64_t r = 0; r < rows; r += most) {
+    const int64_t n = rows - r < most ? rows - r : most;
+    hipLaunchKernelGGL(pad_rows_kernel, dim3((unsigned)((n * per + 255) / 256)), dim3(256), 0, st,
+                       static_cast<const uint8_t*>(src) + r * pitch, pitch, row_bytes,
+                       static_cast<uint8_t*>(dst) + r * per * 16, (uint32_t)(n * per), fast_div((uint32_t)per));
+    MQ_LAUNCH_CHECK();
+  }
+  return MI355Q_OK;
+}
+
 // row offsets within a tile and a stage in 32 bits
 static bool small_pitch(int64_t ld) { return ld < (int64_t(1) << 22); }
 
@@ -1427,7 +1482,8 @@ using namespace mi355q;
 
 extern "C" size_t mi355q_fp8_block_matmul_workspace_size(int64_t rows, int64_t out, int64_t cols) {
   if (rows <= kFewTokens || out <= 0 || cols <= 0) return 0;
-  return plan_bytes(plan_forward(rows, out, cols));
+  return plan_bytes(plan_forward(rows, out, cols)) +
+         (cols % 16 ? padded_bytes(rows, cols) + padded_bytes(out, cols) : 0);
 }
 
 extern "C" int mi355q_fp8_block_matmul(const uint8_t* x_dev, int64_t ldx, const void* x_scales_dev,
@@ -1464,24 +1520,34 @@ extern "C" int mi355q_fp8_block_matmul(const uint8_t* x_dev, int64_t ldx, const 
   g.Q = out;
   g.R = cols;
   const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  // 16-byte loads of whole chunks, and row offsets within a tile in 32 bits
-  const bool aligned = cols % 16 == 0 && ldx % 16 == 0 && ldw % 16 == 0 && aligned16(x_dev) && aligned16(w_dev) &&
-                       small_pitch(ldx) && small_pitch(ldw);
-  if (!aligned) return launch_any<kForward>(g, y_dtype, st, "fp8_block_matmul");
   const bool e8 = x_scale_type == MI355Q_SCALE_E8M0;
+  const bool aligned = cols % 16 == 0 && ldx % 16 == 0 && ldw % 16 == 0 && aligned16(x_dev) && aligned16(w_dev);
   if (rows <= kFewTokens) {
-    launch_few(g, e8, st);
+    launch_few(g, e8, aligned, st);
     MQ_LAUNCH_CHECK();
     return MI355Q_OK;
   }
   Plan p = plan_forward(rows, out, cols);
   float* const parts = plan_workspace(p, workspace_dev, workspace_bytes);
+  if (!aligned || !small_pitch(ldx) || !small_pitch(ldw)) {
+    const size_t base = plan_bytes(p), need = base + padded_bytes(rows, cols) + padded_bytes(out, cols);
+    if (!workspace_dev || !aligned16(workspace_dev) || workspace_bytes < need || !small_pitch(cols))
+      return launch_any<kForward>(g, y_dtype, st, "fp8_block_matmul");
+    char* const xc = static_cast<char*>(workspace_dev) + base;
+    char* const wc = xc + padded_bytes(rows, cols);
+    if (const int rc = pad_rows(x_dev, ldx, rows, cols, xc, st)) return rc;
+    if (const int rc = pad_rows(w_dev, ldw, out, cols, wc, st)) return rc;
+    g.a = xc;
+    g.b = reinterpret_cast<const uint8_t*>(wc);
+    g.lda = g.ldb = g.R = padded(cols);
+  }
   return p.shape ? launch_forward<2, 2, 2, 2>(g, e8, p, parts, st) : launch_forward<1, 2, 2, 2>(g, e8, p, parts, st);
 }
 
 extern "C" size_t mi355q_fp8_block_grad_input_workspace_size(int64_t rows, int64_t out, int64_t cols) {
   if (rows <= 0 || out <= 0 || cols <= 0) return 0;
-  return plan_bytes(plan_grad_input(rows, cols, out));
+  return plan_bytes(plan_grad_input(rows, cols, out)) + (out % 8 ? padded_bytes(rows, 2 * out) : 0) +
+         (cols % 16 ? padded_bytes(out, cols) : 0);
 }
 
 extern "C" int mi355q_fp8_block_grad_input(const uint16_t* dy_dev, int64_t lddy, const uint8_t* w_dev, int64_t ldw,
@@ -1507,18 +1573,34 @@ extern "C" int mi355q_fp8_block_grad_input(const uint16_t* dy_dev, int64_t lddy,
   g.Q = cols;
   g.R = out;
   const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  // 16-byte loads of whole chunks
-  const bool aligned = cols % 16 == 0 && ldw % 16 == 0 && out % 8 == 0 && lddy % 8 == 0 && aligned16(dy_dev) &&
-                       aligned16(w_dev) && small_pitch(lddy) && small_pitch(ldw);
-  if (!aligned) return launch_any<kGradInput>(g, MI355Q_BF16, st, "fp8_block_grad_input");
+  const bool y_ok = out % 8 == 0 && lddy % 8 == 0 && aligned16(dy_dev) && small_pitch(lddy);
+  const bool w_ok = cols % 16 == 0 && ldw % 16 == 0 && aligned16(w_dev) && small_pitch(ldw);
   Plan p = plan_grad_input(rows, cols, out);
   float* const parts = plan_workspace(p, workspace_dev, workspace_bytes);
+  if (!y_ok || !w_ok) {
+    const size_t base = plan_bytes(p), y_bytes = y_ok ? 0 : padded_bytes(rows, 2 * out);
+    const size_t need = base + y_bytes + (w_ok ? 0 : padded_bytes(out, cols));
+    if (!workspace_dev || !aligned16(workspace_dev) || workspace_bytes < need || !small_pitch(cols) || !small_pitch(out))
+      return launch_any<kGradInput>(g, MI355Q_BF16, st, "fp8_block_grad_input");
+    char* const yc = static_cast<char*>(workspace_dev) + base;
+    if (!y_ok) {
+      if (const int rc = pad_rows(dy_dev, 2 * lddy, rows, 2 * out, yc, st)) return rc;
+      g.a = yc;
+      g.lda = padded(2 * out) / 2;
+    }
+    if (!w_ok) {
+      if (const int rc = pad_rows(w_dev, ldw, out, cols, yc + y_bytes, st)) return rc;
+      g.b = reinterpret_cast<const uint8_t*>(yc + y_bytes);
+      g.ldb = padded(cols);
+    }
+  }
   return p.shape ? launch_grad_input<2, 2>(g, p, parts, st) : launch_grad_input<1, 2>(g, p, parts, st);
 }
 
 extern "C" size_t mi355q_fp8_block_grad_weight_workspace_size(int64_t rows, int64_t out, int64_t cols) {
   if (rows <= 0 || out <= 0 || cols <= 0) return 0;
-  return plan_bytes(plan_weight(rows, out, cols));
+  return plan_bytes(plan_weight(rows, out, cols)) + (out % 8 ? padded_bytes(rows, 2 * out) : 0) +
+         (cols % 16 ? padded_bytes(rows, cols) : 0);
 }
 
 extern "C" int mi355q_fp8_block_grad_weight(const uint16_t* dy_dev, int64_t lddy, const uint8_t* x_dev, int64_t ldx,
@@ -1544,11 +1626,28 @@ extern "C" int mi355q_fp8_block_grad_weight(const uint16_t* dy_dev, int64_t lddy
   g.Q = cols;
   g.R = rows;
   const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  const bool aligned = rows > 0 && cols % 16 == 0 && ldx % 16 == 0 && out % 8 == 0 && lddy % 8 == 0 &&
-                       aligned16(dy_dev) && aligned16(x_dev) && small_pitch(lddy) && small_pitch(ldx) &&
-                       small_pitch(ld_x_scales);
-  if (!aligned) return launch_any<kGradWeight>(g, dw_dtype, st, "fp8_block_grad_weight");
+  if (rows == 0) return launch_any<kGradWeight>(g, dw_dtype, st, "fp8_block_grad_weight");   // zeros
+  const bool y_ok = out % 8 == 0 && lddy % 8 == 0 && aligned16(dy_dev) && small_pitch(lddy);
+  const bool x_ok = cols % 16 == 0 && ldx % 16 == 0 && aligned16(x_dev) && small_pitch(ldx);
   Plan p = plan_weight(rows, out, cols);
   float* const parts = plan_workspace(p, workspace_dev, workspace_bytes);
+  if (!small_pitch(ld_x_scales)) return launch_any<kGradWeight>(g, dw_dtype, st, "fp8_block_grad_weight");
+  if (!y_ok || !x_ok) {
+    const size_t base = plan_bytes(p), y_bytes = y_ok ? 0 : padded_bytes(rows, 2 * out);
+    const size_t need = base + y_bytes + (x_ok ? 0 : padded_bytes(rows, cols));
+    if (!workspace_dev || !aligned16(workspace_dev) || workspace_bytes < need || !small_pitch(cols) || !small_pitch(out))
+      return launch_any<kGradWeight>(g, dw_dtype, st, "fp8_block_grad_weight");
+    char* const yc = static_cast<char*>(workspace_dev) + base;
+    if (!y_ok) {
+      if (const int rc = pad_rows(dy_dev, 2 * lddy, rows, 2 * out, yc, st)) return rc;
+      g.a = yc;
+      g.lda = padded(2 * out) / 2;
+    }
+    if (!x_ok) {
+      if (const int rc = pad_rows(x_dev, ldx, rows, cols, yc + y_bytes, st)) return rc;
+      g.b = reinterpret_cast<const uint8_t*>(yc + y_bytes);
+      g.ldb = padded(cols);
+    }
+  }
   return p.shape ? launch_grad_weight<4, 2, 2, 4>(g, p, parts, st) : launch_grad_weight<2, 2, 2, 2>(g, p, parts, st);
 }

@@ -671,6 +671,17 @@ def _rows_2d(t: torch.Tensor) -> torch.Tensor:
     return t if step == 1 and pitch >= t.shape[1] else t.contiguous()
 
 
+def _rows_16(t: torch.Tensor, width: int) -> torch.Tensor:
+    """``_rows_2d``, and copied if its rows are a multiple of ``width``
+    elements (16 bytes) but do not lie on 16-byte boundaries: the product
+    kernels load such rows in whole chunks."""
+    pitch, step = t.stride()
+    cols = t.shape[1]
+    if step == 1 and pitch >= cols and (cols % width or (pitch % width == 0 and t.data_ptr() % 16 == 0)):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
 def _fp8_source(x: torch.Tensor, what: str) -> torch.Tensor:
     """x as a 2-D matrix with contiguous rows of bf16, fp16 or fp32."""
     if not x.is_cuda:
@@ -695,7 +706,7 @@ def _fp8_matrix(codes: torch.Tensor, scales: torch.Tensor, what: str, blocks: bo
         raise TypeError(f"{what} scales must be {' or '.join(str(d) for d in scale_dtypes)}, got {scales.dtype}")
     if scales.shape != want:
         raise ValueError(f"{what} of {(rows, cols)} takes scales of {want}, got {tuple(scales.shape)}")
-    return _rows_2d(codes), _rows_2d(scales)
+    return _rows_16(codes, 16), _rows_2d(scales)
 
 
 def _fp8_gradient(dy: torch.Tensor, cols: int) -> torch.Tensor:
@@ -705,7 +716,7 @@ def _fp8_gradient(dy: torch.Tensor, cols: int) -> torch.Tensor:
         raise TypeError(f"the output gradient must be bf16, got {dy.dtype}")
     if dy.dim() != 2 or dy.shape[1] != cols:
         raise ValueError(f"the output gradient must be [rows, {cols}], got {tuple(dy.shape)}")
-    return _rows_2d(dy)
+    return _rows_16(dy, 8)
 
 
 def _one_device(first: torch.Tensor, *others) -> None:

@@ -252,6 +252,75 @@ def test_large_weight_gradients(dev, rows, out, cols):
                       values_gpu(x, xs).T.contiguous(), dtype)
 
 
+ODD = [(100, 131, 257), (70, 1003, 1001), (300, 777, 135), (1, 1001, 333), (20, 50, 4097), (33, 8, 127), (40, 9, 16),
+       (513, 260, 24)]
+
+
+def raw_products(o, x, xs, w, ws, dy, workspace):
+    """The three products through the C entry points, with the queried workspace or with none."""
+    from llmcompressor_amd import _lib as L
+    rows, cols, out, lib = x.shape[0], x.shape[1], w.shape[0], L.lib()
+    y, dx, dw = (torch.full(s, float("nan"), device=x.device, dtype=t) for s, t in (
+        ((rows, out), torch.float32), ((rows, cols), torch.bfloat16), ((out, cols), torch.float32)))
+
+    def room(query):
+        n = query(rows, out, cols) if workspace else 0
+        t = torch.empty(n, dtype=torch.uint8, device=x.device)
+        return t, t.data_ptr() if n else None, n
+    st = L.stream_of(x)
+    k, p, n = room(lib.mi355q_fp8_block_matmul_workspace_size)
+    L.check(lib.mi355q_fp8_block_matmul(x.data_ptr(), x.stride(0), xs.data_ptr(), L.SCALE_E8M0, xs.stride(0), w.data_ptr(),
+                                        w.stride(0), ws.data_ptr(), ws.stride(0), None, 0, y.data_ptr(), L.F32, out, rows,
+                                        out, cols, p, n, st))
+    k2, p, n = room(lib.mi355q_fp8_block_grad_input_workspace_size)
+    L.check(lib.mi355q_fp8_block_grad_input(dy.data_ptr(), dy.stride(0), w.data_ptr(), w.stride(0), ws.data_ptr(),
+                                            ws.stride(0), dx.data_ptr(), cols, rows, out, cols, p, n, st))
+    k3, p, n = room(lib.mi355q_fp8_block_grad_weight_workspace_size)
+    L.check(lib.mi355q_fp8_block_grad_weight(dy.data_ptr(), dy.stride(0), x.data_ptr(), x.stride(0), xs.data_ptr(),
+                                             xs.stride(0), dw.data_ptr(), L.F32, cols, rows, out, cols, p, n, st))
+    torch.cuda.synchronize()
+    return y, dx, dw
+
+
+def check_products(x, xs, w, ws, dy, y, dx, dw):
+    a, b, d = values(x, xs), values(w, ws), dy.cpu().double()
+    check_sum(y, a @ b.T, a.abs() @ b.abs().T, torch.float32)
+    check_sum(dx, d @ b, d.abs() @ b.abs(), torch.bfloat16)
+    check_sum(dw, d.T @ a, d.abs().T @ a.abs(), torch.float32)
+
+
+@pytest.mark.parametrize("rows,out,cols", ODD)
+def test_products_of_odd_widths(dev, rows, out, cols):
+    """Widths that are no whole number of 16-byte chunks: padded copies, element loads, few tokens."""
+    o, g = ops(), gen(rows, out, cols, 3)
+    x, xs, w, ws = fp8_pair(g, rows, out, cols, E8M0)
+    dy = heavy(g, rows, out).to(torch.bfloat16).to(dev)
+    check_products(x, xs, w, ws, dy, o.fp8_block_matmul(x, xs, w, ws, out_dtype=torch.float32),
+                   o.fp8_block_grad_input(dy, w, ws), o.fp8_block_grad_weight(dy, x, xs, torch.float32))
+
+
+@pytest.mark.parametrize("rows,out,cols", [(70, 1003, 1001), (300, 777, 135), (200, 384, 2048), (64, 512, 4096),
+                                           (700, 256, 512)])
+def test_products_without_a_workspace(dev, rows, out, cols):
+    """Without room for splits or padded copies the sums run whole and odd operands take element loads."""
+    o, g = ops(), gen(rows, out, cols, 4)
+    x, xs, w, ws = fp8_pair(g, rows, out, cols, E8M0)
+    dy = heavy(g, rows, out).to(torch.bfloat16).to(dev)
+    for workspace in (False, True):
+        check_products(x, xs, w, ws, dy, *raw_products(o, x, xs, w, ws, dy, workspace))
+
+
+def test_products_of_badly_placed_rows(dev):
+    """Rows of whole chunks that do not begin on 16 bytes, through the C entry points (no copies are queried)."""
+    o, g = ops(), gen(17)
+    x, xs, w, ws = fp8_pair(g, 50, 64, 256, E8M0)
+    dy = heavy(g, 50, 64).to(torch.bfloat16).to(dev)
+    bx, bw = (torch.zeros(t.shape[0], 275, device=dev).to(E4M3)[:, 3:259] for t in (x, w))
+    by = torch.zeros(50, 77, device=dev, dtype=torch.bfloat16)[:, 5:69]
+    bx.copy_(x), bw.copy_(w), by.copy_(dy)
+    check_products(x, xs, w, ws, dy, *raw_products(o, bx, xs, bw, ws, by, True))
+
+
 def test_products_of_strided_operands(dev):
     """Codes and gradients that are views of wider or transposed buffers."""
     o, g = ops(), gen(11)
