@@ -67,4 +67,11 @@ inline FastDiv fast_div(uint32_t d) {
 }
 __device__ __forceinline__ uint32_t div(uint32_t n, const FastDiv& f) { return (__umulhi(n, f.mul) + n) >> f.shift; }
 
+
+// Workgroup id of n, so that the workgroups of one XCD (every eighth) take
+// neighbouring items.
+__device__ __forceinline__ uint32_t xcd_order(uint32_t id, uint32_t n) {
+  const uint32_t q = n / 8, r = n % 8, x = id % 8;
+  return x * q + (x < r ? x : r) + id / 8;
+}
 }  // namespace mi355q

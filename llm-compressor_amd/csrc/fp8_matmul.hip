@@ -212,10 +212,6 @@ struct TileItem {
   uint32_t split;
   int64_t slot;        // partial slot, or -1: the output itself
 };
-__device__ __forceinline__ uint32_t xcd_order(uint32_t id, uint32_t n) {
-  const uint32_t q = n / 8, r = n % 8, x = id % 8;
-  return x * q + (x < r ? x : r) + id / 8;
-}
 __device__ __forceinline__ TileItem tile_of(const TileOrder& o, uint32_t id) {
   const uint32_t rest = o.row_tiles * o.col_tiles - o.full;
   TileItem it;
@@ -1473,6 +1469,12 @@ static int pad_rows(const void* src, int64_t pitch, int64_t rows, int64_t row_by
   return MI355Q_OK;
 }
 
+// Odd widths and a sum of one step: the element loads of one launch cost less than
+// copies of both operands (2102 x 80 x 69 9 us against 18; 100 rows into 300 x 301 13 against
+// 14; with three steps 300 x 513 x 515 44 against 17), unless the output is large.
+static bool short_sum(int64_t rows, int64_t cols, int64_t sum) {
+  return sum <= kGroup && ((rows + GT - 1) / GT) * ((cols + GT - 1) / GT) <= 1024;
+}
 // row offsets within a tile and a stage in 32 bits
 static bool small_pitch(int64_t ld) { return ld < (int64_t(1) << 22); }
 
@@ -1531,7 +1533,8 @@ extern "C" int mi355q_fp8_block_matmul(const uint8_t* x_dev, int64_t ldx, const 
   float* const parts = plan_workspace(p, workspace_dev, workspace_bytes);
   if (!aligned || !small_pitch(ldx) || !small_pitch(ldw)) {
     const size_t base = plan_bytes(p), need = base + padded_bytes(rows, cols) + padded_bytes(out, cols);
-    if (!workspace_dev || !aligned16(workspace_dev) || workspace_bytes < need || !small_pitch(cols))
+    if (!workspace_dev || !aligned16(workspace_dev) || workspace_bytes < need || !small_pitch(cols) ||
+        short_sum(rows, out, cols))
       return launch_any<kForward>(g, y_dtype, st, "fp8_block_matmul");
     char* const xc = static_cast<char*>(workspace_dev) + base;
     char* const wc = xc + padded_bytes(rows, cols);
@@ -1580,7 +1583,8 @@ extern "C" int mi355q_fp8_block_grad_input(const uint16_t* dy_dev, int64_t lddy,
   if (!y_ok || !w_ok) {
     const size_t base = plan_bytes(p), y_bytes = y_ok ? 0 : padded_bytes(rows, 2 * out);
     const size_t need = base + y_bytes + (w_ok ? 0 : padded_bytes(out, cols));
-    if (!workspace_dev || !aligned16(workspace_dev) || workspace_bytes < need || !small_pitch(cols) || !small_pitch(out))
+    if (!workspace_dev || !aligned16(workspace_dev) || workspace_bytes < need || !small_pitch(cols) ||
+        !small_pitch(out) || short_sum(rows, cols, out))
       return launch_any<kGradInput>(g, MI355Q_BF16, st, "fp8_block_grad_input");
     char* const yc = static_cast<char*>(workspace_dev) + base;
     if (!y_ok) {
@@ -1635,7 +1639,8 @@ extern "C" int mi355q_fp8_block_grad_weight(const uint16_t* dy_dev, int64_t lddy
   if (!y_ok || !x_ok) {
     const size_t base = plan_bytes(p), y_bytes = y_ok ? 0 : padded_bytes(rows, 2 * out);
     const size_t need = base + y_bytes + (x_ok ? 0 : padded_bytes(rows, cols));
-    if (!workspace_dev || !aligned16(workspace_dev) || workspace_bytes < need || !small_pitch(cols) || !small_pitch(out))
+    if (!workspace_dev || !aligned16(workspace_dev) || workspace_bytes < need || !small_pitch(cols) ||
+        !small_pitch(out) || short_sum(out, cols, rows))
       return launch_any<kGradWeight>(g, dw_dtype, st, "fp8_block_grad_weight");
     char* const yc = static_cast<char*>(workspace_dev) + base;
     if (!y_ok) {

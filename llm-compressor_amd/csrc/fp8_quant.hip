@@ -11,7 +11,15 @@
 // would hide the overflow.
 //
 // All kernels pass over the data once (a group never leaves the registers
-// between its maximum and its codes) and are bound by HBM.
+// between its maximum and its codes) and are bound by HBM.  What is read is read
+// once, so the loads are nontemporal; the stores are where a call moves more than the
+// last-level cache holds, and its results could not stay there for their reader
+// anyway.  Against plain accesses: gated activation of 8192 x 14336 142 -> 138 us with
+// the loads, 131 with the stores too (6.3 TB/s), its backward pass 164 -> 157 -> 149 us
+// (6.3 TB/s); 14336 x 4096 in blocks 37 -> 33 us (31 with the blocks ordered by XCD,
+// 5.6 TB/s); 16384 x 4096 in groups 37 -> 36 us (5.6 TB/s).
+#include <type_traits>
+
 #include "fp8.h"
 
 namespace mi355q {
@@ -52,7 +60,8 @@ __device__ __forceinline__ void load_chunk(Chunk<T>& c, const typename T::raw* p
     constexpr int W = kChunk * sizeof(typename T::raw) / 16;
     u32x4_t q[W];
 #pragma unroll
-    for (int i = 0; i < W; ++i) q[i] = left > 0 ? reinterpret_cast<const u32x4_t*>(p)[i] : u32x4_t{0u, 0u, 0u, 0u};
+    for (int i = 0; i < W; ++i)
+      q[i] = left > 0 ? __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(p) + i) : u32x4_t{0u, 0u, 0u, 0u};
     __builtin_memcpy(c.v, q, sizeof(c.v));
   } else {
 #pragma unroll
@@ -60,10 +69,15 @@ __device__ __forceinline__ void load_chunk(Chunk<T>& c, const typename T::raw* p
   }
 }
 
-template <bool VEC>
+template <bool STREAM, class V>
+__device__ __forceinline__ void put(V* p, V v) {
+  if constexpr (STREAM) __builtin_nontemporal_store(v, p);
+  else *p = v;
+}
+template <bool VEC, bool STREAM>
 __device__ __forceinline__ void store_codes(uint8_t* p, const uint32_t w[2], int64_t left) {
   if constexpr (VEC) {
-    if (left > 0) *reinterpret_cast<u32x2_t*>(p) = u32x2_t{w[0], w[1]};
+    if (left > 0) put<STREAM>(reinterpret_cast<u32x2_t*>(p), u32x2_t{w[0], w[1]});
   } else {
 #pragma unroll
     for (int i = 0; i < kChunk; ++i)
@@ -138,7 +152,7 @@ struct GroupsArgs {
 
 // One thread per chunk of 8 columns, 16 lanes per group; consecutive lanes
 // take consecutive chunks, so a wave moves 1 KB of 16-bit input per load.
-template <class T, bool E8M0, bool VEC>
+template <class T, bool E8M0, bool VEC, bool STREAM>
 __global__ __launch_bounds__(NT) void fp8_groups_kernel(GroupsArgs a) {
   const uint32_t i = blockIdx.x * NT + threadIdx.x;
   const uint32_t j = i < a.chunks ? i : a.chunks - 1;    // whole rows of lanes (chunks is a multiple of 16)
@@ -169,19 +183,20 @@ __global__ __launch_bounds__(NT) void fp8_groups_kernel(GroupsArgs a) {
     codes_f32(x, s, 1.f / s, w);
     if (first) static_cast<float*>(a.scales)[si] = s;
   }
-  if (i < a.chunks) store_codes<VEC>(a.codes + row * a.ldc + col, w, left);
+  if (i < a.chunks) store_codes<VEC, STREAM>(a.codes + row * a.ldc + col, w, left);
 }
 
 // ---------------------------------------------------------------- blocks
 // One workgroup per 128 x 128 block: 16 lanes per row, 16 rows a pass, eight
 // passes held in registers between the maximum and the codes.
-template <class T, bool VEC>
+template <class T, bool VEC, bool STREAM>
 __global__ __launch_bounds__(NT) void fp8_blocks_kernel(const void* w, int64_t rows, int64_t cols, int64_t ldw,
                                                         uint8_t* codes, int64_t ldc, float* scales, int64_t lds,
                                                         uint32_t col_blocks) {
   __shared__ uint32_t tops[NT / 64];
   constexpr int P = kGroup / (NT / kLanes);
-  const uint32_t br = blockIdx.x / col_blocks, bc = blockIdx.x - br * col_blocks;
+  // neighbouring blocks on one XCD
+  const uint32_t id = xcd_order(blockIdx.x, gridDim.x), br = id / col_blocks, bc = id - br * col_blocks;
   const int64_t r0 = (int64_t)br * kGroup + threadIdx.x / kLanes;
   const int64_t col = (int64_t)bc * kGroup + (threadIdx.x % kLanes) * kChunk;
   Chunk<T> c[P];
@@ -215,7 +230,7 @@ __global__ __launch_bounds__(NT) void fp8_blocks_kernel(const void* w, int64_t r
     for (int e = 0; e < kChunk; ++e) x[e] = T::load(c[p].v[e]);
     uint32_t o[2];
     codes_f32(x, s, rs, o);
-    store_codes<VEC>(codes + (left > 0 ? r * ldc + col : 0), o, left);
+    store_codes<VEC, STREAM>(codes + (left > 0 ? r * ldc + col : 0), o, left);
   }
 }
 
@@ -240,7 +255,7 @@ struct GluArgs {
   FastDiv per_row;
 };
 
-template <class T, bool KEEP, bool VEC>
+template <class T, bool KEEP, bool VEC, bool STREAM>
 __global__ __launch_bounds__(NT) void fp8_silu_mul_kernel(GluArgs a) {
   const uint32_t i = blockIdx.x * NT + threadIdx.x;
   const uint32_t j = i < a.chunks ? i : a.chunks - 1;
@@ -266,19 +281,19 @@ __global__ __launch_bounds__(NT) void fp8_silu_mul_kernel(GluArgs a) {
   }
   const uint32_t groups = a.per_row.d / kLanes, gi = ch / kLanes;
   const bool mine = i < a.chunks, first = mine && (ch & (kLanes - 1)) == 0;
-  auto put = [&](const float* v, uint32_t m, uint8_t* codes, uint8_t* scale) __attribute__((always_inline)) {
+  auto quantize = [&](const float* v, uint32_t m, uint8_t* codes, uint8_t* scale) __attribute__((always_inline)) {
     const uint32_t b = e8m0_of(max_row16(m));
     uint32_t w[2];
     codes_e8m0(v, b, w);
     if (first) *scale = (uint8_t)b;
-    if (mine) store_codes<VEC>(codes, w, left);
+    if (mine) store_codes<VEC, STREAM>(codes, w, left);
   };
-  put(h, mh, a.h + row * a.ldh + col, a.hs + (int64_t)row * groups + gi);
+  quantize(h, mh, a.h + row * a.ldh + col, a.hs + (int64_t)row * groups + gi);
   if constexpr (KEEP) {
     uint8_t* k = a.kept + row * a.ldk + col;
     uint8_t* s = a.ks + (int64_t)row * 2 * groups + gi;
-    put(g, mg, k, s);
-    put(u, mu, k + a.cols, s + groups);
+    quantize(g, mg, k, s);
+    quantize(u, mu, k + a.cols, s + groups);
   }
 }
 
@@ -320,7 +335,7 @@ __device__ __forceinline__ void load_codes(float v[kChunk], const uint8_t* p, fl
   }
 }
 
-template <class T, bool VEC>
+template <class T, bool VEC, bool STREAM>
 __device__ __forceinline__ void store_chunk(typename T::raw* p, const float v[kChunk], int64_t left) {
   Chunk<T> c;
 #pragma unroll
@@ -331,7 +346,7 @@ __device__ __forceinline__ void store_chunk(typename T::raw* p, const float v[kC
     __builtin_memcpy(q, c.v, sizeof(c.v));
     if (left > 0) {
 #pragma unroll
-      for (int i = 0; i < W; ++i) reinterpret_cast<u32x4_t*>(p)[i] = q[i];
+      for (int i = 0; i < W; ++i) put<STREAM>(reinterpret_cast<u32x4_t*>(p) + i, q[i]);
     }
   } else {
 #pragma unroll
@@ -341,7 +356,7 @@ __device__ __forceinline__ void store_chunk(typename T::raw* p, const float v[kC
 }
 
 // d gate = dh up s (1 + gate (1 - s)), d up = dh gate s, s = sigmoid(gate)
-template <class T, bool VEC>
+template <class T, bool VEC, bool STREAM>
 __global__ __launch_bounds__(NT) void fp8_silu_mul_backward_kernel(GluBackArgs a) {
   const uint32_t i = blockIdx.x * NT + threadIdx.x;
   if (i >= a.chunks) return;
@@ -363,8 +378,8 @@ __global__ __launch_bounds__(NT) void fp8_silu_mul_backward_kernel(GluBackArgs a
     du[e] = d * (g[e] * sg);
   }
   typename T::raw* o = static_cast<typename T::raw*>(a.dx) + row * a.lddx + col;
-  store_chunk<T, VEC>(o, dg, left);
-  store_chunk<T, VEC>(o + a.cols, du, left);
+  store_chunk<T, VEC, STREAM>(o, dg, left);
+  store_chunk<T, VEC, STREAM>(o + a.cols, du, left);
 }
 
 // Launches `f(first row, rows)` over row ranges whose chunks fit 31 bits.
@@ -372,6 +387,17 @@ template <class Fn>
 static void over_rows(int64_t rows, int64_t per_row, Fn&& f) {
   const int64_t most = ((int64_t(1) << 31) - NT) / per_row;
   for (int64_t r = 0; r < rows; r += most) f(r, rows - r < most ? rows - r : most);
+}
+
+// Calls f(VEC, STREAM) with the template arguments of a call: whole 16-byte
+// chunks, and nontemporal stores where its bytes outgrow the 256 MB last-level
+// cache.
+template <class Fn>
+static void with_access(bool vec, int64_t bytes, Fn&& f) {
+  const bool stream = bytes > (int64_t(256) << 20);
+  if (vec && stream) f(std::true_type{}, std::true_type{});
+  else if (vec) f(std::true_type{}, std::false_type{});
+  else f(std::false_type{}, std::false_type{});
 }
 
 static unsigned blocks_of(uint32_t chunks) { return (chunks + NT - 1) / NT; }
@@ -403,13 +429,13 @@ extern "C" int mi355q_fp8_quantize_groups(const void* x_dev, mi355q_dtype dtype,
     with_dtype(dtype, [&](auto t) {
       using T = decltype(t);
       const dim3 grid(blocks_of(a.chunks));
-      if (scale_type == MI355Q_SCALE_E8M0) {
-        if (vec) hipLaunchKernelGGL((fp8_groups_kernel<T, true, true>), grid, dim3(NT), 0, st, a);
-        else     hipLaunchKernelGGL((fp8_groups_kernel<T, true, false>), grid, dim3(NT), 0, st, a);
-      } else {
-        if (vec) hipLaunchKernelGGL((fp8_groups_kernel<T, false, true>), grid, dim3(NT), 0, st, a);
-        else     hipLaunchKernelGGL((fp8_groups_kernel<T, false, false>), grid, dim3(NT), 0, st, a);
-      }
+      with_access(vec, rows * cols * (es + 1), [&](auto v, auto nt) {
+        constexpr bool V = decltype(v)::value, S = decltype(nt)::value;
+        if (scale_type == MI355Q_SCALE_E8M0)
+          hipLaunchKernelGGL((fp8_groups_kernel<T, true, V, S>), grid, dim3(NT), 0, st, a);
+        else
+          hipLaunchKernelGGL((fp8_groups_kernel<T, false, V, S>), grid, dim3(NT), 0, st, a);
+      });
     });
   });
   MQ_LAUNCH_CHECK();
@@ -432,10 +458,10 @@ extern "C" int mi355q_fp8_quantize_blocks(const void* w_dev, mi355q_dtype dtype,
   with_dtype(dtype, [&](auto t) {
     using T = decltype(t);
     const dim3 grid((unsigned)n);
-    if (vec) hipLaunchKernelGGL((fp8_blocks_kernel<T, true>), grid, dim3(NT), 0, st, w_dev, rows, cols, ldw, codes_dev,
-                                ld_codes, scales_dev, ld_scales, (uint32_t)cb);
-    else     hipLaunchKernelGGL((fp8_blocks_kernel<T, false>), grid, dim3(NT), 0, st, w_dev, rows, cols, ldw, codes_dev,
-                                ld_codes, scales_dev, ld_scales, (uint32_t)cb);
+    with_access(vec, rows * cols * (dtype_size(dtype) + 1), [&](auto v, auto nt) {
+      hipLaunchKernelGGL((fp8_blocks_kernel<T, decltype(v)::value, decltype(nt)::value>), grid, dim3(NT), 0, st, w_dev,
+                         rows, cols, ldw, codes_dev, ld_codes, scales_dev, ld_scales, (uint32_t)cb);
+    });
   });
   MQ_LAUNCH_CHECK();
   return MI355Q_OK;
@@ -466,13 +492,11 @@ extern "C" int mi355q_fp8_silu_mul(const void* x_dev, mi355q_dtype dtype, int64_
     with_dtype(dtype, [&](auto t) {
       using T = decltype(t);
       const dim3 grid(blocks_of(a.chunks));
-      if (keep) {
-        if (vec) hipLaunchKernelGGL((fp8_silu_mul_kernel<T, true, true>), grid, dim3(NT), 0, st, a);
-        else     hipLaunchKernelGGL((fp8_silu_mul_kernel<T, true, false>), grid, dim3(NT), 0, st, a);
-      } else {
-        if (vec) hipLaunchKernelGGL((fp8_silu_mul_kernel<T, false, true>), grid, dim3(NT), 0, st, a);
-        else     hipLaunchKernelGGL((fp8_silu_mul_kernel<T, false, false>), grid, dim3(NT), 0, st, a);
-      }
+      with_access(vec, rows * cols * (2 * es + (keep ? 3 : 1)), [&](auto v, auto nt) {
+        constexpr bool V = decltype(v)::value, S = decltype(nt)::value;
+        if (keep) hipLaunchKernelGGL((fp8_silu_mul_kernel<T, true, V, S>), grid, dim3(NT), 0, st, a);
+        else      hipLaunchKernelGGL((fp8_silu_mul_kernel<T, false, V, S>), grid, dim3(NT), 0, st, a);
+      });
     });
   });
   MQ_LAUNCH_CHECK();
@@ -501,8 +525,10 @@ extern "C" int mi355q_fp8_silu_mul_backward(const void* dh_dev, mi355q_dtype dty
     with_dtype(dtype, [&](auto t) {
       using T = decltype(t);
       const dim3 grid(blocks_of(a.chunks));
-      if (vec) hipLaunchKernelGGL((fp8_silu_mul_backward_kernel<T, true>), grid, dim3(NT), 0, st, a);
-      else     hipLaunchKernelGGL((fp8_silu_mul_backward_kernel<T, false>), grid, dim3(NT), 0, st, a);
+      with_access(vec, rows * cols * (3 * es + 2), [&](auto v, auto nt) {
+        hipLaunchKernelGGL((fp8_silu_mul_backward_kernel<T, decltype(v)::value, decltype(nt)::value>), grid, dim3(NT), 0,
+                           st, a);
+      });
     });
   });
   MQ_LAUNCH_CHECK();
