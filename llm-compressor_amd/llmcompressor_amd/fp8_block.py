@@ -1,0 +1,200 @@
+"""Linear layers and gated MLPs in block-scaled fp8, for serving and for
+training with 8-bit activation checkpoints.
+
+A weight is e4m3 codes with one fp32 scale per 128 x 128 block, activations are
+e4m3 codes with one scale per row and 128 columns: the FP8_BLOCK format
+(compressed-tensors' preset of that name: float 8-bit weights of strategy
+block [128, 128], dynamic group-128 activations).  Without gradients activations take fp32 scales, as the scheme
+has them.  With gradients they take powers of two (e8m0), and the same codes
+that enter the product are all that is kept of the activation for the backward
+pass: one byte per element and one per 128, where the bf16 tensor takes two.
+
+Backward formulas, for y = x W^T + b with X, W the values that the codes stand
+for (quantization itself counts as the identity):
+
+    dX = dY W,  dW = dY^T X,  db = sum of dY's rows
+
+dY is read in bf16; gradients of other types are rounded to it first (2^-9
+relative, beside 2^-4 of the codes it is multiplied with).
+"""
+from __future__ import annotations
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import ops
+
+E8M0 = torch.float8_e8m0fnu
+_TYPES = (torch.bfloat16, torch.float16, torch.float32)
+
+
+def _rows(x: torch.Tensor, width: int, what: str) -> torch.Tensor:
+    """x [..., width] as a matrix."""
+    if x.dtype not in _TYPES:
+        raise TypeError(f"{what} must be bf16, fp16 or fp32, got {x.dtype}")
+    if x.dim() == 0 or x.shape[-1] != width:
+        raise ValueError(f"{what} must be [..., {width}], got {tuple(x.shape)}")
+    return x.reshape(-1, width)
+
+
+def _grad_rows(dy: torch.Tensor, width: int) -> torch.Tensor:
+    return dy.reshape(-1, width).to(torch.bfloat16)
+
+
+class _Linear(torch.autograd.Function):
+    """x [rows, in] times the fp8 weight; ``weight`` is the tensor that takes
+    the weight's gradient, or None."""
+
+    @staticmethod
+    def forward(ctx, x, weight, codes, scales, bias):
+        xc, xs = ops.fp8_quantize_groups(x, E8M0)
+        ctx.save_for_backward(xc, xs, codes, scales)
+        ctx.types = x.dtype, None if weight is None else weight.dtype, None if bias is None else bias.dtype
+        return ops.fp8_block_matmul(xc, xs, codes, scales, bias, x.dtype)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        xc, xs, codes, scales = ctx.saved_tensors
+        need, (x_type, w_type, b_type) = ctx.needs_input_grad, ctx.types
+        d = _grad_rows(dy, codes.shape[0])
+        dx = ops.fp8_block_grad_input(d, codes, scales).to(x_type) if need[0] else None
+        dw = ops.fp8_block_grad_weight(d, xc, xs, w_type) if need[1] else None
+        db = dy.sum(0, dtype=torch.float32).to(b_type) if need[4] else None
+        return dx, dw, None, None, db
+
+
+class _GatedMLP(torch.autograd.Function):
+    """down(silu(gate x) * (up x)); keeps the codes of x, of gate and up's
+    outputs and of their product, nothing wider."""
+
+    @staticmethod
+    def forward(ctx, x, gate_up_weight, down_weight, gu_codes, gu_scales, d_codes, d_scales):
+        xc, xs = ops.fp8_quantize_groups(x, E8M0)
+        gate_up = ops.fp8_block_matmul(xc, xs, gu_codes, gu_scales, None, x.dtype)
+        hc, hs, kept, ks = ops.fp8_silu_mul(gate_up)
+        ctx.save_for_backward(xc, xs, hc, hs, kept, ks, gu_codes, gu_scales, d_codes, d_scales)
+        ctx.types = x.dtype, *(None if w is None else w.dtype for w in (gate_up_weight, down_weight))
+        return ops.fp8_block_matmul(hc, hs, d_codes, d_scales, None, x.dtype)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        xc, xs, hc, hs, kept, ks, gu_codes, gu_scales, d_codes, d_scales = ctx.saved_tensors
+        need, (x_type, gu_type, d_type) = ctx.needs_input_grad, ctx.types
+        d = _grad_rows(dy, d_codes.shape[0])
+        d_down = ops.fp8_block_grad_weight(d, hc, hs, d_type) if need[2] else None
+        dx = d_gate_up = None
+        if need[0] or need[1]:
+            dgu = ops.fp8_silu_mul_backward(ops.fp8_block_grad_input(d, d_codes, d_scales), kept, ks)
+            if need[1]:
+                d_gate_up = ops.fp8_block_grad_weight(dgu, xc, xs, gu_type)
+            if need[0]:
+                dx = ops.fp8_block_grad_input(dgu, gu_codes, gu_scales).to(x_type)
+        return dx, d_gate_up, d_down, None, None, None, None
+
+
+class _Weight(torch.nn.Module):
+    """An fp8 weight: frozen codes and scales, or (``trainable``) a master
+    parameter that is quantized again for every forward pass."""
+
+    def __init__(self, weight: torch.Tensor, trainable: bool):
+        super().__init__()
+        if weight.dim() != 2 or weight.dtype not in _TYPES:
+            raise ValueError(f"a weight must be a bf16, fp16 or fp32 matrix, got {tuple(weight.shape)} {weight.dtype}")
+        self.shape = tuple(weight.shape)
+        if trainable:
+            self.master = torch.nn.Parameter(weight.detach().clone())
+        else:
+            self.register_parameter("master", None)
+            codes, scales = ops.fp8_quantize_blocks(weight.detach())
+            self.register_buffer("weight", codes)
+            self.register_buffer("weight_scale", scales)
+
+    def _apply(self, fn, *args, **kwargs):
+        # module.to(dtype) would turn codes into numbers of that type: the format
+        # keeps its types and moves only between devices
+        kept = dict(self._buffers)
+        super()._apply(fn, *args, **kwargs)
+        for name, t in kept.items():
+            if self._buffers[name].dtype != t.dtype:
+                self._buffers[name] = t.to(self._buffers[name].device)
+        return self
+
+    def codes(self):
+        if self.master is None:
+            return self.weight, self.weight_scale
+        return ops.fp8_quantize_blocks(self.master.detach())
+
+
+class Fp8BlockLinear(torch.nn.Module):
+    """``torch.nn.Linear`` with its weight in block-scaled fp8.
+
+    ``trainable``: the weight stays as a master parameter (``linear.master``,
+    in the type given) that receives gradients; otherwise only its codes and
+    scales are kept (``linear.weight``, ``linear.weight_scale``: the tensors of an
+    FP8_BLOCK checkpoint)."""
+
+    def __init__(self, weight: torch.Tensor, bias: torch.Tensor | None = None, trainable: bool = False):
+        super().__init__()
+        self.linear = _Weight(weight, trainable)
+        self.out_features, self.in_features = self.linear.shape
+        if bias is not None and tuple(bias.shape) != (self.out_features,):
+            raise ValueError(f"bias must be [{self.out_features}], got {tuple(bias.shape)}")
+        self.bias = None if bias is None else torch.nn.Parameter(bias.detach().clone(), requires_grad=trainable)
+
+    @classmethod
+    def from_linear(cls, linear: torch.nn.Linear, trainable: bool = False) -> "Fp8BlockLinear":
+        return cls(linear.weight, linear.bias, trainable)
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        rows = _rows(x, self.in_features, "input")
+        codes, scales = self.linear.codes()
+        master, bias = self.linear.master, self.bias
+        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, master, bias)):
+            y = _Linear.apply(rows, master, codes, scales, bias)
+        else:
+            y = ops.fp8_block_matmul(*ops.fp8_quantize_groups(rows), codes, scales, bias, x.dtype)
+        return y.reshape(*x.shape[:-1], self.out_features)
+
+
+class Fp8GatedMLP(torch.nn.Module):
+    """A gated MLP ``down(silu(gate x) * (up x))`` in block-scaled fp8, gate
+    and up stacked into one weight [2 intermediate, hidden].
+
+    The activation goes from the first product to the second in fp8 without a
+    pass of its own; with gradients, 8-bit codes are what the backward pass gets
+    (hidden + 3 intermediate bytes per token and their scales, where bf16
+    tensors of the same would be twice that)."""
+
+    def __init__(self, gate: torch.Tensor, up: torch.Tensor, down: torch.Tensor, trainable: bool = False):
+        super().__init__()
+        if gate.shape != up.shape or tuple(down.shape) != (gate.shape[1], gate.shape[0]):
+            raise ValueError(f"gate {tuple(gate.shape)}, up {tuple(up.shape)} and down {tuple(down.shape)} do not make "
+                             "a gated MLP")
+        self.intermediate_size, self.hidden_size = gate.shape
+        self.gate_up = _Weight(torch.cat([gate.detach(), up.detach()]), trainable)
+        self.down = _Weight(down, trainable)
+
+    @classmethod
+    def from_expert(cls, expert: torch.nn.Module, trainable: bool = False) -> "Fp8GatedMLP":
+        """From a module with ``gate_proj``, ``up_proj`` and ``down_proj``
+        linears without biases and SiLU between them (``moe.ExpertMLP``)."""
+        projs = expert.gate_proj, expert.up_proj, expert.down_proj
+        if any(p.bias is not None for p in projs):
+            raise NotImplementedError("gated MLPs with biases are not supported")
+        act = getattr(expert, "act", getattr(expert, "act_fn", torch.nn.functional.silu))
+        if act is not torch.nn.functional.silu and not isinstance(act, torch.nn.SiLU):
+            raise NotImplementedError(f"the activation must be SiLU, got {act}")
+        return cls(*(p.weight for p in projs), trainable=trainable)
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        rows = _rows(x, self.hidden_size, "input")
+        gu, d = self.gate_up.codes(), self.down.codes()
+        masters = self.gate_up.master, self.down.master
+        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, *masters)):
+            y = _GatedMLP.apply(rows, *masters, *gu, *d)
+        else:
+            h = ops.fp8_block_matmul(*ops.fp8_quantize_groups(rows), *gu, None, x.dtype)
+            y = ops.fp8_block_matmul(*ops.fp8_silu_mul(h, save=False), *d, None, x.dtype)
+        return y.reshape(x.shape)

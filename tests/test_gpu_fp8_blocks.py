@@ -550,3 +550,21 @@ def test_the_current_stream_is_used(dev):
              o.fp8_block_grad_input(dy, w, ws), *o.fp8_silu_mul(src))
     for a, b in zip((y, dw, dx, *h), again):
         assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+def test_calls_larger_than_the_cache_equal_their_rows(dev):
+    """Calls that move over 256 MB store past the caches; rows are independent, so each equals its own call."""
+    o = ops()
+    x = torch.randn(8192, 2 * 4992, generator=torch.Generator(device=dev).manual_seed(3), device=dev).to(torch.bfloat16)
+    pick = [0, 1, 4095, 8191]
+    for op in (lambda t: o.fp8_quantize_groups(t), lambda t: o.fp8_quantize_groups(t, E8M0), o.fp8_silu_mul):
+        for a, b in zip(op(x), op(x[pick])):
+            assert torch.equal(a[pick].view(torch.uint8), b.view(torch.uint8))
+    _, _, kept, ks = o.fp8_silu_mul(x)
+    dh = x[:, :4992].contiguous()
+    a, b = o.fp8_silu_mul_backward(dh, kept, ks), o.fp8_silu_mul_backward(dh[pick], kept[pick], ks[pick])
+    assert torch.equal(a[pick], b)
+    w = x.view(-1, 4992)
+    c, s = o.fp8_quantize_blocks(w)
+    c2, s2 = o.fp8_quantize_blocks(w[1280:1536])
+    assert torch.equal(c[1280:1536].view(torch.uint8), c2.view(torch.uint8)) and torch.equal(s[10:12], s2)

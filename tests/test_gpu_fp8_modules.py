@@ -1,0 +1,171 @@
+"""Fp8BlockLinear and Fp8GatedMLP: forward and backward are the entry points'
+results put together, and near the unquantized modules'.
+
+Nearness.  An e4m3 code is within 2^-4 of its value (relative, normal codes), the
+same for both factors of a product, so a product's relative error is below 2^-3 +
+2^-8; over many terms of random sign the errors average out.  The bound used is
+the worst case, 0.13 of the sum of the terms' magnitudes for one product.
+"""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+E8M0 = torch.float8_e8m0fnu
+
+
+def amd():
+    import llmcompressor_amd as m
+    return m
+
+
+def same(a, b):
+    assert a.dtype == b.dtype and a.shape == b.shape
+    assert torch.equal(a.contiguous().view(torch.uint8), b.contiguous().view(torch.uint8))
+
+
+def randn(dev, seed, *shape):
+    return torch.randn(*shape, generator=torch.Generator(device=dev).manual_seed(seed), device=dev)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("shape", [(1, 256), (7, 200), (2, 33, 384)])
+def test_linear(dev, shape, bias, dtype):
+    m, ops = amd(), amd().fp8_block.ops
+    out, cols = 144, shape[-1]
+    lin = torch.nn.Linear(cols, out, bias=bias).to(dev, dtype)
+    layer = m.Fp8BlockLinear.from_linear(lin, trainable=True)
+    x = randn(dev, 1, *shape).to(dtype)
+    with torch.no_grad():
+        y0 = layer(x)
+    xr = x.clone().requires_grad_()
+    y = layer(xr)
+    w, ws = ops.fp8_quantize_blocks(lin.weight.detach())
+    b = lin.bias.detach() if bias else None
+    rows = x.reshape(-1, cols)
+    same(y0.reshape(-1, out), ops.fp8_block_matmul(*ops.fp8_quantize_groups(rows), w, ws, b, dtype))
+    xc, xs = ops.fp8_quantize_groups(rows, E8M0)
+    same(y.detach().reshape(-1, out), ops.fp8_block_matmul(xc, xs, w, ws, b, dtype))
+    mags = rows.double().abs() @ lin.weight.detach().double().abs().T + (b.double().abs() if bias else 0)
+    full = rows.double() @ lin.weight.detach().double().T + (b.double() if bias else 0)
+    for got in (y0, y):
+        assert bool(((got.double().reshape(-1, out) - full).abs() <= 0.13 * mags + 1e-6).all())
+    dy = randn(dev, 2, *y.shape).to(dtype)
+    y.backward(dy)
+    d = dy.reshape(-1, out).to(torch.bfloat16)
+    same(xr.grad.reshape(-1, cols), ops.fp8_block_grad_input(d, w, ws).to(dtype))
+    same(layer.linear.master.grad, ops.fp8_block_grad_weight(d, xc, xs, dtype))
+    if bias:
+        same(layer.bias.grad, dy.reshape(-1, out).sum(0, dtype=torch.float32).to(dtype))
+
+
+def test_frozen_linear_and_partial_gradients(dev):
+    m = amd()
+    lin = torch.nn.Linear(256, 128).to(dev, torch.bfloat16)
+    x = randn(dev, 3, 9, 256).to(torch.bfloat16)
+    frozen = m.Fp8BlockLinear.from_linear(lin)
+    assert frozen.linear.weight.dtype == torch.float8_e4m3fn and frozen.linear.weight_scale.shape == (1, 2)
+    assert not [p for p in frozen.parameters() if p.requires_grad]
+    assert frozen(x).grad_fn is None
+    xr = x.clone().requires_grad_()
+    frozen(xr).sum().backward()
+    assert xr.grad is not None and frozen.bias.grad is None
+    live = m.Fp8BlockLinear.from_linear(lin, trainable=True)
+    live(x).sum().backward()                       # no gradient of x asked for
+    assert live.linear.master.grad is not None and live.bias.grad is not None
+    same(live(x[:, :256].reshape(3, 3, 256)).reshape(9, 128).detach(), live(x).detach())
+    assert live(x[:0]).shape == (0, 128)
+    for cast in (lambda t: t.to(torch.bfloat16), lambda t: t.float(), lambda t: t.half()):   # codes stay codes
+        same(cast(frozen).linear.weight, frozen.linear.codes()[0])
+        assert frozen.linear.weight.dtype == torch.float8_e4m3fn and frozen.linear.weight_scale.dtype == torch.float32
+    assert cast(live).linear.master.dtype == torch.float16
+    state = frozen.state_dict()
+    assert set(state) == {"bias", "linear.weight", "linear.weight_scale"}
+
+
+@pytest.mark.parametrize("trainable", [False, True])
+@pytest.mark.parametrize("rows,hidden,inter", [(1, 256, 128), (37, 384, 200), (300, 512, 768)])
+def test_gated_mlp(dev, rows, hidden, inter, trainable):
+    m, ops = amd(), amd().fp8_block.ops
+    from llmcompressor_amd.moe import ExpertMLP
+    expert = ExpertMLP(hidden, inter, dtype=torch.bfloat16, device=dev)
+    with torch.no_grad():
+        for i, p in enumerate(expert.parameters()):
+            p.copy_(randn(dev, 10 + i, *p.shape) * 0.05)
+    mlp = m.Fp8GatedMLP.from_expert(expert, trainable=trainable)
+    x = randn(dev, 5, rows, hidden).to(torch.bfloat16)
+    xr = x.clone().requires_grad_()
+    y = mlp(xr)
+    gu = ops.fp8_quantize_blocks(torch.cat([expert.gate_proj.weight, expert.up_proj.weight]).detach())
+    d = ops.fp8_quantize_blocks(expert.down_proj.weight.detach())
+    xq = ops.fp8_quantize_groups(x, E8M0)
+    hc, hs, kept, ks = ops.fp8_silu_mul(ops.fp8_block_matmul(*xq, *gu))
+    same(y.detach(), ops.fp8_block_matmul(hc, hs, *d))
+    dy = randn(dev, 6, rows, hidden).to(torch.bfloat16)
+    y.backward(dy)
+    dgu = ops.fp8_silu_mul_backward(ops.fp8_block_grad_input(dy, *d), kept, ks)
+    same(xr.grad, ops.fp8_block_grad_input(dgu, *gu))
+    if trainable:
+        same(mlp.down.master.grad, ops.fp8_block_grad_weight(dy, hc, hs))
+        same(mlp.gate_up.master.grad, ops.fp8_block_grad_weight(dgu, *xq))
+    # near the unquantized module: direction and size of output and gradients
+    ref = x.clone().requires_grad_()
+    want = expert(ref)
+    want.backward(dy)
+    pairs = [(y, want), (xr.grad, ref.grad)]
+    if trainable:
+        pairs += [(mlp.down.master.grad, expert.down_proj.weight.grad),
+                  (mlp.gate_up.master.grad, torch.cat([expert.gate_proj.weight.grad, expert.up_proj.weight.grad]))]
+    for got, full in pairs:
+        got, full = got.detach().double(), full.detach().double()
+        # three products one after the other, each below 0.13: their composition in the norm
+        assert float((got - full).norm() / full.norm()) < 0.13 * 3
+    with torch.no_grad():
+        assert float((mlp(x).double() - want.double()).norm() / want.double().norm()) < 0.13 * 2
+
+
+def test_what_the_backward_pass_keeps(dev):
+    """One byte per element and one scale byte per 128, of x, gate, up and h; no wider activation."""
+    m = amd()
+    rows, hidden, inter = 512, 1024, 768
+    mlp = m.Fp8GatedMLP(randn(dev, 1, inter, hidden), randn(dev, 2, inter, hidden), randn(dev, 3, hidden, inter),
+                        trainable=True)
+    kept = []
+    x = randn(dev, 4, rows, hidden).to(torch.bfloat16).requires_grad_()
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: (kept.append(t), t)[1], lambda t: t):
+        y = mlp(x)
+    activations = [t for t in kept if t.shape[0] == rows]
+    assert sum(t.numel() * t.element_size() for t in activations) == rows * (hidden + 3 * inter) * 129 // 128
+    y.sum().backward()
+
+
+def test_modules_refuse(dev):
+    m = amd()
+    from llmcompressor_amd.moe import ExpertMLP
+    lin = m.Fp8BlockLinear(randn(dev, 1, 128, 256))
+    with pytest.raises(ValueError, match=r"\[\.\.\., 256\]"):
+        lin(randn(dev, 2, 4, 128))
+    with pytest.raises(TypeError, match="bf16, fp16 or fp32"):
+        lin(randn(dev, 2, 4, 256).double())
+    with pytest.raises(ValueError, match="bias"):
+        m.Fp8BlockLinear(randn(dev, 1, 128, 256), torch.zeros(127, device=dev))
+    with pytest.raises(ValueError, match="gated MLP"):
+        m.Fp8GatedMLP(randn(dev, 1, 128, 256), randn(dev, 1, 128, 256), randn(dev, 1, 128, 256))
+    with pytest.raises(NotImplementedError, match="biases"):
+        m.Fp8GatedMLP.from_expert(ExpertMLP(256, 128, bias=True, dtype=torch.bfloat16, device=dev))
+    with pytest.raises(NotImplementedError, match="SiLU"):
+        m.Fp8GatedMLP.from_expert(ExpertMLP(256, 128, act=torch.nn.functional.gelu, dtype=torch.bfloat16, device=dev))
+
+
+def test_the_example_recovers(dev):
+    """The example's training lowers the pruned MLP's error: by a tenth at least in twelve steps of Adam at 1e-3,
+    each of which moves a weight by up to 1e-3 where the median weight is 0.013."""
+    import importlib.util
+    from pathlib import Path
+    path = Path(__file__).resolve().parents[1] / "examples" / "fp8_mlp_recovery.py"
+    spec = importlib.util.spec_from_file_location("fp8_mlp_recovery", path)
+    ex = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(ex)
+    errors = ex.recover(hidden=512, intermediate=256, tokens=512, steps=12)
+    assert errors[-1] < 0.9 * errors[0]
