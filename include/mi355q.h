@@ -531,8 +531,9 @@ int mi355q_quantize_int8_per_token(const void* x_dev, int64_t rows, int64_t cols
  * infinity or a NaN becomes NaN as a whole (scale NaN / byte 255, NaN codes).
  * codes [rows, cols] (ld_codes), scales [rows, ceil(cols / 128)] (ld_scales,
  * in scales).  rows may be 0.  fp32 scales are those of the FP8_BLOCK
- * scheme's dynamic group-128 activations; with e8m0 scales code * scale is
- * exact in bf16, which the weight gradient relies on. */
+ * scheme's dynamic group-128 activations; with e8m0 scales from 2^-117 up
+ * code * scale is exact in bf16, which the weight gradient relies on (values
+ * below bf16's normal range may lose bits). */
 int mi355q_fp8_quantize_groups(const void* x_dev, mi355q_dtype dtype, int64_t rows, int64_t cols,
                                int64_t ldx, uint8_t* codes_dev, int64_t ld_codes, void* scales_dev,
                                mi355q_scale_type scale_type, int64_t ld_scales, void* stream);

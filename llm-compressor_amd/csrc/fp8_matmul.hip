@@ -4,9 +4,10 @@
 //   grad input   dX[m][k] = sum_nb ws[nb][k / 128] sum_{n in nb} dY[m][n] w[n][k]
 //   grad weight  dW[n][k] = sum_m dY[m][n] x[m][k] 2^e[m][k / 128]
 //
-// x and w are e4m3 codes, dY is bf16.  Codes, and codes times a power of two,
-// are exact in bf16, and products of bf16 values are exact in fp32; so the only
-// roundings are those of the fp32 sums, the scales' products and the output.
+// x and w are e4m3 codes, dY is bf16.  Codes, and codes times a power of two from
+// 2^-117 up (below it a code's last bits fall out of bf16's range), are exact in
+// bf16, and products of bf16 values are exact in fp32; so the only roundings are
+// those of the fp32 sums, the scales' products and the output.
 #include "fp8.h"
 
 namespace mi355q {
@@ -44,7 +45,10 @@ __device__ __forceinline__ float load_typed(const void* p, int type, int64_t i) 
 // ---------------------------------------------------------------- any layout
 // 64 x 64 tiles over steps of 128, both operands as bf16 in LDS with r
 // contiguous, element loads with bounds: right for every size, stride and
-// alignment.
+// alignment.  It runs where the tile kernels cannot (operands off 16 bytes without
+// a workspace for their copies, pitches past 32-bit offsets), where odd widths
+// have a sum of one step, and for a weight gradient of no tokens.  Bound by its
+// element loads: input gradient of 8192 x 4096 x 14336 29 ms against the tiles' 0.97.
 constexpr int GT = 64, GPITCH = kGroup + 8;
 
 template <int KIND, class T>
@@ -160,6 +164,15 @@ __global__ __launch_bounds__(256) void product_any_kernel(ProductArgs g) {
 // acc += tile * (token scale * block scale) in fp32: the features are the
 // MFMA's rows, so a lane holds one token per tile (its scale is one register)
 // and the block scale is wave-uniform.
+//
+// Four waves with 2 x 2 tiles each, two workgroups on a CU: one's scaling and
+// conversions run beside the other's MFMAs (one workgroup of eight waves with
+// 256 x 128 tiles 2.06 ms against 1.77).  8192 x 28672 x 4096 1.77 ms, 1.09 PFLOP/s.  Per
+// MFMA it issues 7 vector instructions (4 conversions, 2 scaling FMAs); MFMAs and
+// vector instructions are busy 0.57 and 0.60 of the cycles at 1.75 GHz, down from
+// 2.4: what bounds it is power, which the conversions and the traffic from LDS
+// share with the MFMAs.  HBM reads are 2.8 GB of 150 MB (the operands once a row of
+// tiles and XCD), 1.6 TB/s.
 typedef __attribute__((address_space(3))) void lds_void_t;
 
 __device__ __forceinline__ uint32_t lds_u32(const void* p) {
@@ -592,6 +605,11 @@ void fp8_forward_kernel(ProductArgs g, TileOrder order, int steps_per_split, flo
 // rows whose 16-byte pieces the lane pairs point to, that is eight n of one k,
 // which are converted to bf16 in registers.  A step is 64 n; the tiles' sums
 // run over the two steps of a 128 x 128 block before they take its scale.
+//
+// 128 x 128 tiles on four waves, two workgroups on a CU (256 x 128 on eight waves
+// 1.03 .. 1.05 ms against 1.00 .. 1.02).  8192 x 4096 x 14336 0.97 ms, 0.99 PFLOP/s: MFMAs busy
+// 0.51 of the cycles, vector instructions 0.38, at 1.71 GHz: power again, and the
+// LDS, which carries dY in 16 bits.
 template <int T, int WT>
 struct GradInputShape {
   static constexpr int A = 2, WF = 2;                        // 128 columns: one block scale per workgroup
@@ -803,7 +821,11 @@ void fp8_grad_input_kernel(ProductArgs g, TileOrder order, int blocks_per_split,
 // (DMA); the checkpoint's scale changes with the token, along the sum, so it has
 // to be in the operand: each wave's DMA brings codes and scale bytes of its own
 // rows, and the wave writes them to LDS as bf16, scaled by the conversion (exact).
-// The MFMAs then add straight into the accumulators.
+// The MFMAs then add straight into the accumulators: vector instructions are few
+// (busy 0.18 of the cycles), so a large tile on eight waves, 256 x 256, saves
+// LDS reads (one wave's operands serve 4 x 2 tiles).  8192 x 4096 x 14336 0.865 ms,
+// 1.11 PFLOP/s, 16 us of it the sum of the split tiles; MFMAs busy 0.57 of the cycles
+// at 1.92 GHz.  Bound by the LDS, which a stage's rows pass twice, and by power.
 template <int MB, int NB2, int WK, int WN>
 struct GradWeightShape {
   static constexpr int W = WK * WN, NTH = 64 * W;
@@ -1093,7 +1115,7 @@ void fp8_grad_weight_kernel(ProductArgs g, TileOrder order, int stages_per_split
 
 // Sums the partial slots [splits][tiles][TR][TC] of the split tiles in their
 // order, adds the bias and rounds once.  Four columns a thread, four splits' loads
-// in flight.
+// in flight.  333 x 4096 in 5 parts 6.9 us.
 template <int TR, int TC>
 __global__ __launch_bounds__(256) void sum_splits_kernel(ProductArgs g, TileOrder o, const float* parts) {
   constexpr uint32_t PER = TR * TC / 4 / 256;          // workgroups per tile
@@ -1159,6 +1181,8 @@ __global__ __launch_bounds__(256) void sum_splits_kernel(ProductArgs g, TileOrde
 // tokens come from L2, and the W waves of a workgroup take every W-th step of 16 AF
 // features; their sums are joined in LDS.  Bound by the weight's bytes, so what
 // counts is loads in flight: U steps are requested before the first is used.
+// 1 x 14336 x 4096 16.3 us (58.7 MB, 3.6 TB/s: a launch this short ends before HBM is
+// at its full rate).
 typedef int i32x4_t __attribute__((ext_vector_type(4)));
 typedef int i32x8_t __attribute__((ext_vector_type(8)));
 
@@ -1436,7 +1460,8 @@ static int launch_grad_weight(const ProductArgs& g, const Plan& p, float* parts,
 
 // ---------------------------------------------------------------- rows of odd widths
 // The tile kernels take operands in 16-byte chunks.  Rows whose width is no whole
-// number of them are first copied to rows that are, ending in zeros.
+// number of them are first copied to rows that are, ending in zeros: a read and a
+// write of both operands, of which the product reads each many times.
 __global__ __launch_bounds__(256) void pad_rows_kernel(const uint8_t* src, int64_t pitch, int64_t row_bytes,
                                                        uint8_t* dst, uint32_t chunks, FastDiv per_row) {
   const uint32_t i = blockIdx.x * 256 + threadIdx.x;

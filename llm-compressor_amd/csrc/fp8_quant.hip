@@ -17,7 +17,7 @@
 // anyway.  Against plain accesses: gated activation of 8192 x 14336 142 -> 138 us with
 // the loads, 131 with the stores too (6.3 TB/s), its backward pass 164 -> 157 -> 149 us
 // (6.3 TB/s); 14336 x 4096 in blocks 37 -> 33 us (31 with the blocks ordered by XCD,
-// 5.6 TB/s); 16384 x 4096 in groups 37 -> 36 us (5.6 TB/s).
+// 5.7 TB/s); 16384 x 4096 in groups 37 -> 36 us (5.6 TB/s).
 #include <type_traits>
 
 #include "fp8.h"

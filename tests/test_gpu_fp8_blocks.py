@@ -568,3 +568,35 @@ def test_calls_larger_than_the_cache_equal_their_rows(dev):
     c, s = o.fp8_quantize_blocks(w)
     c2, s2 = o.fp8_quantize_blocks(w[1280:1536])
     assert torch.equal(c[1280:1536].view(torch.uint8), c2.view(torch.uint8)) and torch.equal(s[10:12], s2)
+
+
+@pytest.mark.parametrize("rows,out,cols", [(1, 256, 512), (100, 384, 1024), (300, 300, 301)])
+def test_replays_of_a_graph_follow_their_inputs(dev, rows, out, cols):
+    """A captured step (split sums and padded copies among it) gives the eager results for every input that is
+    put into its buffers, with eager work and synchronizations between the replays."""
+    o = ops()
+    g = gen(61, rows, out, cols)
+    x0 = torch.zeros(rows, cols, dtype=torch.bfloat16, device=dev)
+    dy0 = torch.zeros(rows, out, dtype=torch.bfloat16, device=dev)
+    w, ws = o.fp8_quantize_blocks(heavy(g, out, cols).to(torch.bfloat16).to(dev))
+
+    def step(x, dy):
+        c, s = o.fp8_quantize_groups(x, E8M0)
+        return (c, s, o.fp8_block_matmul(c, s, w, ws), o.fp8_block_grad_input(dy, w, ws),
+                o.fp8_block_grad_weight(dy, c, s, torch.float32))
+
+    step(x0, dy0)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step(x0, dy0)
+    for _ in range(4):
+        x = heavy(g, rows, cols).to(torch.bfloat16).to(dev)
+        dy = heavy(g, rows, out).to(torch.bfloat16).to(dev)
+        eager = step(x, dy)
+        x0.copy_(x)
+        dy0.copy_(dy)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(captured, eager):
+            assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
