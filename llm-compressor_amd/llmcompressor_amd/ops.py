@@ -666,9 +666,10 @@ def _fp8_groups(n: int) -> int:
 # checks are written to cost little: one pass over each operand's attributes, and
 # the workspace sizes, which depend on the shape alone, looked up.
 def _rows_2d(t: torch.Tensor) -> torch.Tensor:
-    """t with contiguous rows that do not overlap."""
+    """t with contiguous rows that do not overlap.  (``contiguous()`` would
+    return a single row as it is, whatever its pitch.)"""
     pitch, step = t.stride()
-    return t if step == 1 and pitch >= t.shape[1] else t.contiguous()
+    return t if step == 1 and pitch >= t.shape[1] else t.clone(memory_format=torch.contiguous_format)
 
 
 def _rows_16(t: torch.Tensor, width: int) -> torch.Tensor:

@@ -600,3 +600,33 @@ def test_replays_of_a_graph_follow_their_inputs(dev, rows, out, cols):
         torch.cuda.synchronize()
         for a, b in zip(captured, eager):
             assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+def test_single_rows_of_any_pitch(dev):
+    """A matrix of one row (or none) may carry any strides: a transposed column is as good as a row."""
+    o = ops()
+    g = gen(67)
+    w, ws = o.fp8_quantize_blocks(heavy(g, 256, 256).to(torch.bfloat16).to(dev))
+    x = heavy(g, 1, 256).to(torch.bfloat16).to(dev)
+    column = x.reshape(256, 1).clone().t()
+    assert column.stride() == (1, 1)
+    for kind in (torch.float32, E8M0):
+        c, s = o.fp8_quantize_groups(x, kind)
+        c2, s2 = o.fp8_quantize_groups(column, kind)
+        assert torch.equal(c.view(torch.uint8), c2.view(torch.uint8)) and torch.equal(s.float(), s2.float())
+        y = o.fp8_block_matmul(c, s, w, ws)
+        as_column = (t.reshape(-1, 1).clone().t() for t in (c, s))
+        assert torch.equal(y, o.fp8_block_matmul(*as_column, w, ws))
+    wc, wsc = o.fp8_quantize_blocks(column)
+    assert torch.equal(wc.float(), o.fp8_quantize_blocks(x)[0].float())
+    h, hs, kept, ks = o.fp8_silu_mul(column)
+    for a, b in zip(o.fp8_silu_mul(x), (h, hs, kept, ks)):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+    dh = heavy(g, 1, 128).to(torch.bfloat16).to(dev)
+    want = o.fp8_silu_mul_backward(dh, kept, ks)
+    got = o.fp8_silu_mul_backward(*(t.reshape(-1, 1).clone().t() for t in (dh, kept, ks)))
+    assert torch.equal(want, got)
+    none = torch.empty(256, 0, dtype=torch.bfloat16, device=dev).t()
+    c, s = o.fp8_quantize_groups(none)
+    assert c.shape == (0, 256) and s.shape == (0, 2)
+    assert o.fp8_block_grad_input(none, w, ws).shape == (0, 256)
