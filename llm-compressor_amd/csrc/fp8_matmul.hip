@@ -1556,6 +1556,7 @@ extern "C" int mi355q_fp8_block_matmul(const uint8_t* x_dev, int64_t ldx, const 
   }
   Plan p = plan_forward(rows, out, cols);
   float* const parts = plan_workspace(p, workspace_dev, workspace_bytes);
+  if (!small_pitch(ld_x_scales)) return launch_any<kForward>(g, y_dtype, st, "fp8_block_matmul");
   if (!aligned || !small_pitch(ldx) || !small_pitch(ldw)) {
     const size_t base = plan_bytes(p), need = base + padded_bytes(rows, cols) + padded_bytes(out, cols);
     if (!workspace_dev || !aligned16(workspace_dev) || workspace_bytes < need || !small_pitch(cols) ||

@@ -630,3 +630,21 @@ def test_single_rows_of_any_pitch(dev):
     c, s = o.fp8_quantize_groups(none)
     assert c.shape == (0, 256) and s.shape == (0, 2)
     assert o.fp8_block_grad_input(none, w, ws).shape == (0, 256)
+
+
+def test_scales_of_a_wide_pitch(dev):
+    """Offsets of a tile's scales that pass 32 bits: 130 rows of scales 2^25 + 2^21 apart, 4.6 GB of address range."""
+    o = ops()
+    g = gen(71)
+    rows, pitch = 130, 2 ** 25 + 2 ** 21
+    w, ws = o.fp8_quantize_blocks(heavy(g, 128, 256).to(torch.bfloat16).to(dev))
+    c, s = o.fp8_quantize_groups((heavy(g, rows, 256) * torch.exp2(torch.arange(rows) % 40.)[:, None]).to(dev), E8M0)
+    far = torch.empty(rows * pitch, dtype=torch.uint8, device=dev).view(E8M0).as_strided((rows, 2), (pitch, 1))
+    far.copy_(s)
+    assert torch.equal(o.fp8_block_matmul(c, s, w, ws, out_dtype=torch.float32).cpu().isnan(),
+                       torch.zeros(rows, 128, dtype=torch.bool))
+    check_sum(o.fp8_block_matmul(c, far, w, ws, out_dtype=torch.float32).cpu(), values(c, s) @ values(w, ws).T,
+              values(c, s).abs() @ values(w, ws).abs().T, torch.float32)
+    dy = heavy(g, rows, 128).to(torch.bfloat16).to(dev)
+    check_sum(o.fp8_block_grad_weight(dy, c, far, torch.float32).cpu(), dy.cpu().double().T @ values(c, s),
+              dy.cpu().double().abs().T @ values(c, s).abs(), torch.float32)
