@@ -43,12 +43,13 @@ def _grad_rows(dy: torch.Tensor, width: int) -> torch.Tensor:
 
 class _Linear(torch.autograd.Function):
     """x [rows, in] times the fp8 weight; ``weight`` is the tensor that takes
-    the weight's gradient, or None."""
+    the weight's gradient, or None.  Kept is what a gradient asked for reads."""
 
     @staticmethod
     def forward(ctx, x, weight, codes, scales, bias):
         xc, xs = ops.fp8_quantize_groups(x, E8M0)
-        ctx.save_for_backward(xc, xs, codes, scales)
+        need = ctx.needs_input_grad
+        ctx.save_for_backward(*((xc, xs) if need[1] else (None, None)), *((codes, scales) if need[0] else (None, None)))
         ctx.types = x.dtype, None if weight is None else weight.dtype, None if bias is None else bias.dtype
         return ops.fp8_block_matmul(xc, xs, codes, scales, bias, x.dtype)
 
@@ -57,7 +58,7 @@ class _Linear(torch.autograd.Function):
     def backward(ctx, dy):
         xc, xs, codes, scales = ctx.saved_tensors
         need, (x_type, w_type, b_type) = ctx.needs_input_grad, ctx.types
-        d = _grad_rows(dy, codes.shape[0])
+        d = _grad_rows(dy, dy.shape[-1])
         dx = ops.fp8_block_grad_input(d, codes, scales).to(x_type) if need[0] else None
         dw = ops.fp8_block_grad_weight(d, xc, xs, w_type) if need[1] else None
         db = dy.sum(0, dtype=torch.float32).to(b_type) if need[4] else None
@@ -66,14 +67,19 @@ class _Linear(torch.autograd.Function):
 
 class _GatedMLP(torch.autograd.Function):
     """down(silu(gate x) * (up x)); keeps the codes of x, of gate and up's
-    outputs and of their product, nothing wider."""
+    outputs and of their product, nothing wider, and of these what a gradient
+    asked for reads."""
 
     @staticmethod
     def forward(ctx, x, gate_up_weight, down_weight, gu_codes, gu_scales, d_codes, d_scales):
         xc, xs = ops.fp8_quantize_groups(x, E8M0)
         gate_up = ops.fp8_block_matmul(xc, xs, gu_codes, gu_scales, None, x.dtype)
-        hc, hs, kept, ks = ops.fp8_silu_mul(gate_up)
-        ctx.save_for_backward(xc, xs, hc, hs, kept, ks, gu_codes, gu_scales, d_codes, d_scales)
+        need, none = ctx.needs_input_grad, (None, None)
+        inner = need[0] or need[1]
+        hc, hs, *kept = ops.fp8_silu_mul(gate_up, save=inner)
+        ctx.save_for_backward(*((xc, xs) if need[1] else none), *((hc, hs) if need[2] else none), *(kept or none),
+                              *((gu_codes, gu_scales) if need[0] else none),
+                              *((d_codes, d_scales) if inner else none))
         ctx.types = x.dtype, *(None if w is None else w.dtype for w in (gate_up_weight, down_weight))
         return ops.fp8_block_matmul(hc, hs, d_codes, d_scales, None, x.dtype)
 
@@ -82,7 +88,7 @@ class _GatedMLP(torch.autograd.Function):
     def backward(ctx, dy):
         xc, xs, hc, hs, kept, ks, gu_codes, gu_scales, d_codes, d_scales = ctx.saved_tensors
         need, (x_type, gu_type, d_type) = ctx.needs_input_grad, ctx.types
-        d = _grad_rows(dy, d_codes.shape[0])
+        d = _grad_rows(dy, dy.shape[-1])
         d_down = ops.fp8_block_grad_weight(d, hc, hs, d_type) if need[2] else None
         dx = d_gate_up = None
         if need[0] or need[1]:

@@ -169,3 +169,39 @@ def test_the_example_recovers(dev):
     spec.loader.exec_module(ex)
     errors = ex.recover(hidden=512, intermediate=256, tokens=512, steps=12)
     assert errors[-1] < 0.9 * errors[0]
+
+
+@pytest.mark.parametrize("frozen", ["none", "input", "weights", "gate_up", "down"])
+def test_what_is_kept_follows_the_gradients_asked_for(dev, frozen):
+    """Gradients that are asked for do not depend on the others being asked for, and nothing is kept for the others."""
+    m = amd()
+    rows, hidden, inter = 48, 256, 384
+    weights = randn(dev, 1, inter, hidden), randn(dev, 2, inter, hidden), randn(dev, 3, hidden, inter)
+    x0, dy = randn(dev, 4, rows, hidden).to(torch.bfloat16), randn(dev, 5, rows, hidden).to(torch.bfloat16)
+
+    def run(frozen):
+        mlp = m.Fp8GatedMLP(*weights, trainable=True)
+        lin = m.Fp8BlockLinear(weights[0], trainable=True)
+        mlp.gate_up.master.requires_grad_(frozen not in ("weights", "gate_up"))
+        mlp.down.master.requires_grad_(frozen not in ("weights", "down"))
+        lin.linear.master.requires_grad_(frozen not in ("weights", "gate_up"))
+        x, x2 = x0.clone().requires_grad_(frozen != "input"), x0.clone().requires_grad_(frozen != "input")
+        sizes = []
+        for layer, inp, d in ((mlp, x, dy), (lin, x2, dy.repeat(1, 2)[:, :inter])):
+            kept = []
+            with torch.autograd.graph.saved_tensors_hooks(lambda t: (kept.append(t), t)[1], lambda t: t):
+                y = layer(inp)
+            sizes.append(sum(t.numel() * t.element_size() for t in kept if t.shape[0] == rows) * 128 // 129 // rows)
+            if y.requires_grad:
+                y.backward(d)
+        return sizes, (x.grad, mlp.gate_up.master.grad, mlp.down.master.grad, x2.grad, lin.linear.master.grad)
+
+    (_, full), (sizes, grads) = run("none"), run(frozen)
+    for a, b in zip(full, grads):
+        if b is not None:
+            same(a, b)
+    asked = dict(none="11111", input="01101", weights="10010", gate_up="10110", down="11011")[frozen]
+    assert "".join("01"[b is not None] for b in grads) == asked
+    want = dict(none=(hidden + 3 * inter, hidden), input=(hidden + 3 * inter, hidden), weights=(2 * inter, 0),
+                gate_up=(3 * inter, 0), down=(hidden + 2 * inter, hidden))[frozen]
+    assert tuple(sizes) == want
