@@ -973,9 +973,11 @@ void fp8_grad_weight_kernel(ProductArgs g, TileOrder order, int stages_per_split
   // Stage s, in two slices of 16 tokens; while one is multiplied the other's
   // operands are read.  The barrier between them publishes stage s + 1 (dY's DMA
   // and the converted rows; the checkpoint rows of stage s + 2 have arrived as well)
-  // and frees the slots of stage s - 1.  `c` is the stage's slot, a constant in
-  // the loop's four copies: slot numbers and addresses cost no instructions.
-  auto stage = [&](int s, int c) __attribute__((always_inline)) {
+  // and frees the slots of stage s - 1.  Scalar instructions are a third of what a
+  // wave issues, so stages that are far enough from the end (INNER) leave out its
+  // conditions, and their slot `c` is a constant in four copies of them.
+  auto stage = [&](int s, int c, auto inner) __attribute__((always_inline)) {
+    constexpr bool INNER = decltype(inner)::value;
     static_assert(MB * NB2 >= MB + NB2, "an MFMA for each operand read");
 #pragma unroll
     for (int i = 0; i < MB * NB2; ++i) {
@@ -986,11 +988,17 @@ void fp8_grad_weight_kernel(ProductArgs g, TileOrder order, int stages_per_split
       __builtin_amdgcn_sched_barrier(0);
     }
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(NDMA) : "memory");
-    if (s + 1 < s_end) clear_tail(s + 1, c + 1);
-    next_y(s + 3);
-    next_x(s + 4);
-    if (s + 3 < s_end) turn_y(s + 3);
-    if (s + 4 < s_end) turn_x(s + 4);
+    if constexpr (INNER) {
+      yp += ystep;
+      xp += xstep;
+      ep += estep;
+    } else {
+      if (s + 1 < s_end) clear_tail(s + 1, c + 1);
+      next_y(s + 3);
+      next_x(s + 4);
+      if (s + 3 < s_end) turn_y(s + 3);
+      if (s + 4 < s_end) turn_x(s + 4);
+    }
     __builtin_amdgcn_sched_barrier(0);
     fetch(c + 2);
 #pragma unroll
@@ -1038,15 +1046,13 @@ void fp8_grad_weight_kernel(ProductArgs g, TileOrder order, int stages_per_split
 #pragma unroll
     for (int b = 0; b < MB; ++b) fx0[b] = read_x(0, 0, b);
     int s = s_begin;
-    for (; s + 4 <= s_end; s += 4) {
-      stage(s, 0);
-      stage(s + 1, 1);
-      stage(s + 2, 2);
-      stage(s + 3, 3);
+    for (; s + 8 < s_end; s += 4) {   // s + 3 + 4, the last one loaded for, is before the item's last stage
+      stage(s, 0, std::true_type{});
+      stage(s + 1, 1, std::true_type{});
+      stage(s + 2, 2, std::true_type{});
+      stage(s + 3, 3, std::true_type{});
     }
-    if (s < s_end) stage(s, 0);
-    if (s + 1 < s_end) stage(s + 1, 1);
-    if (s + 2 < s_end) stage(s + 2, 2);
+    for (int c = 0; s < s_end; ++s, ++c) stage(s, c, std::false_type{});
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // before the ring is used again
   }
 
