@@ -425,13 +425,13 @@ void fp8_forward_kernel(ProductArgs g, TileOrder order, int steps_per_split, flo
   auto load_b = [&](int s, int slot, int j) __attribute__((always_inline)) {
     dma_s(ob[j], xbase + (int64_t)s * kGroup, lb0 + (uint32_t)(slot & 1) * S::B_SLOT + 1024 * j);
   };
-  auto clear_tail = [&](int s) __attribute__((always_inline)) {
+  auto clear_tail = [&](int s, int slot) __attribute__((always_inline)) {
     if (!tail || s != nkb - 1) return;
 #pragma unroll
     for (int i = 0; i < S::TT * 8 / S::NTH; ++i) {
       const int at = i * S::NTH + (int)threadIdx.x, row = at >> 3;
       if (((at & 7) ^ ((row >> 1) & 7)) >= tail)
-        *reinterpret_cast<u32x4_t*>(ringb + (s & 1) * S::B_SLOT + at * 16) = u32x4_t{0u, 0u, 0u, 0u};
+        *reinterpret_cast<u32x4_t*>(ringb + (slot & 1) * S::B_SLOT + at * 16) = u32x4_t{0u, 0u, 0u, 0u};
     }
     __syncthreads();
   };
@@ -445,11 +445,11 @@ void fp8_forward_kernel(ProductArgs g, TileOrder order, int steps_per_split, flo
     p[i] = (lane & 31) * kGroup + 16 * ((4 * (lane >> 5) + i) ^ ((lane >> 1) & 7));
     asm volatile("" : "+v"(p[i]));
   }
-  auto read_a = [&](int s, int a, int i) __attribute__((always_inline)) {
-    return *reinterpret_cast<const u32x4_t*>(ring + (s % 3) * S::A_SLOT + (wf * A + a) * 32 * kGroup + p[i]);
+  auto read_a = [&](int slot, int a, int i) __attribute__((always_inline)) {
+    return *reinterpret_cast<const u32x4_t*>(ring + (slot % 3) * S::A_SLOT + (wf * A + a) * 32 * kGroup + p[i]);
   };
-  auto read_b = [&](int s, int b, int i) __attribute__((always_inline)) {
-    return *reinterpret_cast<const u32x4_t*>(ringb + (s & 1) * S::B_SLOT + (wt * T + b) * 32 * kGroup + p[i]);
+  auto read_b = [&](int slot, int b, int i) __attribute__((always_inline)) {
+    return *reinterpret_cast<const u32x4_t*>(ringb + (slot & 1) * S::B_SLOT + (wt * T + b) * 32 * kGroup + p[i]);
   };
 
   // scales: this lane's tokens, and the block scale of the wave's features
@@ -505,10 +505,14 @@ void fp8_forward_kernel(ProductArgs g, TileOrder order, int steps_per_split, flo
   // feature slot of step s - 1 and the token slot of step s for step s + 2,
   // whose DMA then has a step's time.  In the last row of tiles each token
   // operand is replaced by its successor's as soon as its last MFMA is issued.
-  auto step = [&](int s) __attribute__((always_inline)) {
+  // Slots count from the item's first step.  Steps that are far enough from the
+  // end (INNER) leave out its conditions and have their slot numbers `c` as
+  // constants.
+  auto step = [&](int s, int c, auto inner) __attribute__((always_inline)) {
+    constexpr bool INNER = decltype(inner)::value;
     // past the last step the loads repeat it, into slots that nothing reads:
     // without a branch in the step the compiler keeps the sums between the MFMAs
-    const int s1 = s + 1 < s_end ? s + 1 : s, s2 = s + 2 < s_end ? s + 2 : s_end - 1;
+    const int s1 = INNER || s + 1 < s_end ? s + 1 : s, s2 = INNER || s + 2 < s_end ? s + 2 : s_end - 1;
     u32x4_t rb[T];
 #pragma unroll
     for (int b = 0; b < T; ++b) sc[b] = sc_next[b];
@@ -518,15 +522,17 @@ void fp8_forward_kernel(ProductArgs g, TileOrder order, int steps_per_split, flo
       if (a == LAST) {
         __builtin_amdgcn_sched_barrier(0);
         asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
-        if (s1 != s) clear_tail(s1);
-        if (s2 > s1) turn_to_tail(s2);
+        if constexpr (!INNER) {
+          if (s1 != s) clear_tail(s1, c + 1);
+          if (s2 > s1) turn_to_tail(s2);
+        }
         // (the scales of step s + 1 were requested a step ago, with the DMA
         // that the wait above is for: a use anywhere else would wait for the
         // DMA issued since)
         take_scales();
         load_scales(s2);
 #pragma unroll
-        for (int b = 0; b < T; ++b) rb[b] = read_b(s + 1, b, 0);
+        for (int b = 0; b < T; ++b) rb[b] = read_b(c + 1, b, 0);
         __builtin_amdgcn_sched_barrier(0);
       }
       f32x16_t t[T];
@@ -537,7 +543,7 @@ void fp8_forward_kernel(ProductArgs g, TileOrder order, int steps_per_split, flo
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const bf16x8_t f0r = codes_bf16(ra[0], ra[1]), f1r = codes_bf16(ra[2], ra[3]);
-        ra = i < 3 ? read_a(s, a, i + 1) : a < LAST ? read_a(s, a + 1, 0) : read_a(s + 1, 0, 0);
+        ra = i < 3 ? read_a(c, a, i + 1) : a < LAST ? read_a(c, a + 1, 0) : read_a(c + 1, 0, 0);
 #pragma unroll
         for (int b = 0; b < T; ++b) t[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f0r, xb[b][2 * i], t[b], 0, 0, 0);
 #pragma unroll
@@ -547,14 +553,14 @@ void fp8_forward_kernel(ProductArgs g, TileOrder order, int steps_per_split, flo
           convert_b(rb, i);
           if (i < 3) {
 #pragma unroll
-            for (int b = 0; b < T; ++b) rb[b] = read_b(s + 1, b, i + 1);
+            for (int b = 0; b < T; ++b) rb[b] = read_b(c + 1, b, i + 1);
           }
 #pragma unroll
           for (int j = 0; j < NA; ++j)
-            if (j * 4 / NA == i) load_a(s2, s + 2, j);
+            if (j * 4 / NA == i) load_a(s2, c + 2, j);
 #pragma unroll
           for (int j = 0; j < NB; ++j)
-            if (j * 4 / NB == i) load_b(s2, s + 2, j);
+            if (j * 4 / NB == i) load_b(s2, c + 2, j);
         }
       }
 #pragma unroll
@@ -570,28 +576,37 @@ void fp8_forward_kernel(ProductArgs g, TileOrder order, int steps_per_split, flo
     const int s1 = s_begin + 1 < s_end ? s_begin + 1 : s_begin;
     turn_to_tail(s_begin);
 #pragma unroll
-    for (int j = 0; j < NA; ++j) load_a(s_begin, s_begin, j);
+    for (int j = 0; j < NA; ++j) load_a(s_begin, 0, j);
 #pragma unroll
-    for (int j = 0; j < NB; ++j) load_b(s_begin, s_begin, j);
+    for (int j = 0; j < NB; ++j) load_b(s_begin, 0, j);
     load_scales(s_begin);
     asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
-    clear_tail(s_begin);
+    clear_tail(s_begin, 0);
     take_scales();
     load_scales(s1);
     if (s1 > s_begin) turn_to_tail(s1);
 #pragma unroll
-    for (int j = 0; j < NA; ++j) load_a(s1, s_begin + 1, j);
+    for (int j = 0; j < NA; ++j) load_a(s1, 1, j);
 #pragma unroll
-    for (int j = 0; j < NB; ++j) load_b(s1, s_begin + 1, j);
-    ra = read_a(s_begin, 0, 0);
+    for (int j = 0; j < NB; ++j) load_b(s1, 1, j);
+    ra = read_a(0, 0, 0);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       u32x4_t rb[T];
 #pragma unroll
-      for (int b = 0; b < T; ++b) rb[b] = read_b(s_begin, b, i);
+      for (int b = 0; b < T; ++b) rb[b] = read_b(0, b, i);
       convert_b(rb, i);
     }
-    for (int s = s_begin; s < s_end; ++s) step(s);
+    int s = s_begin;
+    for (; s + 8 < s_end; s += 6) {   // s + 5 + 2, the last one loaded for, is before the item's last step
+      step(s, 0, std::true_type{});
+      step(s + 1, 1, std::true_type{});
+      step(s + 2, 2, std::true_type{});
+      step(s + 3, 3, std::true_type{});
+      step(s + 4, 4, std::true_type{});
+      step(s + 5, 5, std::true_type{});
+    }
+    for (int c = 0; s < s_end; ++s, ++c) step(s, c, std::false_type{});
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // before the ring is used again
   }
 
@@ -686,13 +701,13 @@ void fp8_grad_input_kernel(ProductArgs g, TileOrder order, int blocks_per_split,
 #pragma unroll
     for (int j = 0; j < NB; ++j) load_b(s, slot, j);
   };
-  auto clear_tail = [&](int s) __attribute__((always_inline)) {
+  auto clear_tail = [&](int s, int slot) __attribute__((always_inline)) {
     if (!tail || s != nst - 1) return;
 #pragma unroll
     for (int i = 0; i < S::TT * 8 / S::NTH; ++i) {
       const int at = i * S::NTH + (int)threadIdx.x, row = at >> 3;
       if (((at & 7) ^ ((row >> 1) & 7)) >= tail)
-        *reinterpret_cast<u32x4_t*>(ringb + (s % S::NBS) * S::B_SLOT + at * 16) = u32x4_t{0u, 0u, 0u, 0u};
+        *reinterpret_cast<u32x4_t*>(ringb + (slot % S::NBS) * S::B_SLOT + at * 16) = u32x4_t{0u, 0u, 0u, 0u};
     }
     __syncthreads();
   };
@@ -710,12 +725,12 @@ void fp8_grad_input_kernel(ProductArgs g, TileOrder order, int blocks_per_split,
     pb[j] = (wt * T * 32 + (lane & 31)) * 2 * S::SN + 16 * ((2 * j + (lane >> 5)) ^ ((lane >> 1) & 7));
     asm volatile("" : "+v"(pb[j]));
   }
-  auto read_a = [&](int s, int a, int j) __attribute__((always_inline)) {
+  auto read_a = [&](int slot, int a, int j) __attribute__((always_inline)) {
     return __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-        (lds_i32x2_t*)(ring + (s % S::NAS) * S::A_SLOT + j * 16 * S::FT + pa[a]));
+        (lds_i32x2_t*)(ring + (slot % S::NAS) * S::A_SLOT + j * 16 * S::FT + pa[a]));
   };
-  auto read_b = [&](int s, int b, int j) __attribute__((always_inline)) {
-    return *reinterpret_cast<const bf16x8_t*>(ringb + (s % S::NBS) * S::B_SLOT + b * 32 * 2 * S::SN + pb[j]);
+  auto read_b = [&](int slot, int b, int j) __attribute__((always_inline)) {
+    return *reinterpret_cast<const bf16x8_t*>(ringb + (slot % S::NBS) * S::B_SLOT + b * 32 * 2 * S::SN + pb[j]);
   };
 
   // the block scales of this column of blocks, 64 at a time, one per lane
@@ -736,15 +751,18 @@ void fp8_grad_input_kernel(ProductArgs g, TileOrder order, int blocks_per_split,
   // Step s: as in the forward product, the barrier before the last row of tiles
   // publishes step s + 1 (its DMA, two steps old, is waited for; the youngest
   // step's stays in flight) and frees the slots that step s + 3 takes.
-  auto step = [&](int s, bool first, bool last, float sw) __attribute__((always_inline)) {
-    const int s1 = s + 1 < s_end ? s + 1 : s, s3 = s + 3 < s_end ? s + 3 : s_end - 1;
+  auto step = [&](int s, int c, bool first, bool last, float sw, auto inner) __attribute__((always_inline)) {
+    constexpr bool INNER = decltype(inner)::value;
+    const int s1 = INNER || s + 1 < s_end ? s + 1 : s, s3 = INNER || s + 3 < s_end ? s + 3 : s_end - 1;
 #pragma unroll
     for (int a = 0; a < A; ++a) {
       if (a == A - 1) {
         __builtin_amdgcn_sched_barrier(0);
         asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(NA + NB) : "memory");
-        if (s1 != s) clear_tail(s1);
-        if (s + 3 < s_end) turn_to_tail(s + 3);
+        if constexpr (!INNER) {
+          if (s1 != s) clear_tail(s1, c + 1);
+          if (s + 3 < s_end) turn_to_tail(s + 3);
+        }
         __builtin_amdgcn_sched_barrier(0);
       }
       if (first)
@@ -755,18 +773,18 @@ void fp8_grad_input_kernel(ProductArgs g, TileOrder order, int blocks_per_split,
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const bf16x8_t f = codes_bf16(ra[0], ra[1]);
-        ra = j < 3 ? read_a(s, a, j + 1) : a < A - 1 ? read_a(s, a + 1, 0) : read_a(s + 1, 0, 0);
+        ra = j < 3 ? read_a(c, a, j + 1) : a < A - 1 ? read_a(c, a + 1, 0) : read_a(c + 1, 0, 0);
 #pragma unroll
         for (int b = 0; b < T; ++b) t[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f, xb[b][j], t[a][b], 0, 0, 0);
         if (a == A - 1) {
 #pragma unroll
-          for (int b = 0; b < T; ++b) xb[b][j] = read_b(s + 1, b, j);
+          for (int b = 0; b < T; ++b) xb[b][j] = read_b(c + 1, b, j);
 #pragma unroll
           for (int i = 0; i < NA; ++i)
-            if (i * 4 / NA == j) load_a(s3, s + 3, i);
+            if (i * 4 / NA == j) load_a(s3, c + 3, i);
 #pragma unroll
           for (int i = 0; i < NB; ++i)
-            if (i * 4 / NB == j) load_b(s3, s + 3, i);
+            if (i * 4 / NB == j) load_b(s3, c + 3, i);
         }
       }
       if (last)
@@ -783,15 +801,15 @@ void fp8_grad_input_kernel(ProductArgs g, TileOrder order, int blocks_per_split,
 #pragma unroll
   for (int i = 0; i < 3; ++i) {
     if (s_begin + i < s_end) turn_to_tail(s_begin + i);
-    load(s_begin + i < s_end ? s_begin + i : s_last, s_begin + i);
+    load(s_begin + i < s_end ? s_begin + i : s_last, i);
   }
   asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(2 * (NA + NB)) : "memory");
-  clear_tail(s_begin);
-  ra = read_a(s_begin, 0, 0);
+  clear_tail(s_begin, 0);
+  ra = read_a(0, 0, 0);
 #pragma unroll
   for (int b = 0; b < T; ++b)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) xb[b][j] = read_b(s_begin, b, j);
+    for (int j = 0; j < 4; ++j) xb[b][j] = read_b(0, b, j);
   auto scale_of = [&](int blk) __attribute__((always_inline)) {
     const int rel = blk - (s_begin >> 1);
     if ((rel & 63) == 0) {
@@ -801,12 +819,21 @@ void fp8_grad_input_kernel(ProductArgs g, TileOrder order, int blocks_per_split,
     return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(scales), rel & 63));
   };
   int s = s_begin;
-  for (; s + 1 < s_end; s += 2) {
-    const float sw = scale_of(s >> 1);
-    step(s, true, false, sw);
-    step(s + 1, false, true, sw);
+  for (; s + 15 < s_end; s += 12) {   // s + 11 + 3, the last one loaded for, is before the item's last step
+#pragma unroll
+    for (int c = 0; c < 12; c += 2) {
+      const float sw = scale_of((s + c) >> 1);
+      step(s + c, c, true, false, sw, std::true_type{});
+      step(s + c + 1, c + 1, false, true, sw, std::true_type{});
+    }
   }
-  if (s < s_end) step(s, true, true, scale_of(s >> 1));   // a last block of 64 n or fewer
+  int c = 0;
+  for (; s + 1 < s_end; s += 2, c += 2) {
+    const float sw = scale_of(s >> 1);
+    step(s, c, true, false, sw, std::false_type{});
+    step(s + 1, c + 1, false, true, sw, std::false_type{});
+  }
+  if (s < s_end) step(s, c, true, true, scale_of(s >> 1), std::false_type{});   // a last block of 64 n or fewer
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // before the ring is used again
   store_tiles<S, T, A>(g, acc, ring, t0, f0, wt, wf, wave, lane, item.slot, parts);
 }
