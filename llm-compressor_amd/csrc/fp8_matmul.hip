@@ -478,6 +478,7 @@ void fp8_forward_kernel(ProductArgs g, TileOrder order, int steps_per_split, flo
   auto take_scales = [&]() __attribute__((always_inline)) {
 #pragma unroll
     for (int b = 0; b < T; ++b) {
+      asm volatile("" : "+v"(sx_load[b]));   // (not converted where it is loaded, which would wait for it there)
       sc_next[b] = (E8M0 ? e8m0_to_f32(sx_load[b]) : __uint_as_float(sx_load[b])) * sw_load;
       asm volatile("" : "+v"(sc_next[b]));
     }
