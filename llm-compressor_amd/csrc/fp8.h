@@ -14,10 +14,11 @@ constexpr int kGroup = 128;
 
 inline int64_t group_count(int64_t n) { return (n + kGroup - 1) / kGroup; }
 
-// fp32 value of an e8m0 byte (0 is 2^-127, a subnormal)
+// fp32 value of an e8m0 byte (0 is 2^-127, a subnormal; 255 NaN): the code of 1
+// times the scale as the conversions read it, by its exponent bits, in two
+// instructions without the special cases
 __device__ __forceinline__ float e8m0_to_f32(uint32_t b) {
-  const uint32_t u = b == 0 ? 0x00400000u : b == 255 ? 0x7fc00000u : b << 23;
-  return __uint_as_float(u);
+  return __builtin_amdgcn_cvt_scalef32_f32_fp8(0x38, __uint_as_float((b << 23) | 0x00400000u), 0);
 }
 
 __device__ __forceinline__ float load_scale(const void* s, int type, int64_t i) {

@@ -648,3 +648,19 @@ def test_scales_of_a_wide_pitch(dev):
     dy = heavy(g, rows, 128).to(torch.bfloat16).to(dev)
     check_sum(o.fp8_block_grad_weight(dy, c, far, torch.float32).cpu(), dy.cpu().double().T @ values(c, s),
               dy.cpu().double().abs().T @ values(c, s).abs(), torch.float32)
+
+
+@pytest.mark.parametrize("rows", [16, 256])
+def test_every_e8m0_scale(dev, rows):
+    """Every byte as a row's scale, in the few-token kernel and in tiles: 2^(b - 127) exactly, 255 NaN."""
+    o = ops()
+    for first in range(0, 256, rows):
+        b = torch.arange(first, first + rows, dtype=torch.uint8)
+        x = torch.ones(rows, 128).to(E4M3).to(dev)
+        w = torch.zeros(128, 128)
+        w[:, 5] = 1
+        ws = torch.ones(1, 1, device=dev)
+        y = o.fp8_block_matmul(x, b.view(E8M0)[:, None].to(dev), w.to(E4M3).to(dev), ws, out_dtype=torch.float32).cpu()
+        want = torch.exp2(b.double() - 127)
+        want[b == 255] = math.nan
+        assert torch.equal(y.double().nan_to_num(-1.0), want[:, None].expand(-1, 128).nan_to_num(-1.0))
