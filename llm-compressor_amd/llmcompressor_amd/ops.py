@@ -656,75 +656,86 @@ def quantize_int8_per_token(x: torch.Tensor):
 FP8_GROUP = 128     # columns per activation scale, rows and columns per weight scale
 _FP8_DT = {torch.bfloat16: L.BF16, torch.float16: L.F16, torch.float32: L.F32}
 _FP8_SCALES = {torch.float32: L.SCALE_F32, torch.float8_e8m0fnu: L.SCALE_E8M0}
-
-
-def _fp8_groups(n: int) -> int:
-    return -(-n // FP8_GROUP)
+_FP8_F32, _FP8_E8M0 = (torch.float32,), (torch.float8_e8m0fnu,)
 
 
 # These calls take a few microseconds on the device at serving sizes, so the
-# checks are written to cost little: one pass over each operand's attributes, and
-# the workspace sizes, which depend on the shape alone, looked up.
-def _rows_2d(t: torch.Tensor) -> torch.Tensor:
-    """t with contiguous rows that do not overlap.  (``contiguous()`` would
-    return a single row as it is, whatever its pitch.)"""
+# checks are written to cost little: each attribute of an operand is read once (a
+# tensor's shape or strides cost 0.1 us a look), and the workspace sizes, which
+# depend on the shape alone, are looked up.
+def _rows_2d(t: torch.Tensor, cols: int):
+    """t with contiguous rows that do not overlap, and their pitch.
+    (``contiguous()`` would return a single row as it is, whatever its
+    pitch.)"""
     pitch, step = t.stride()
-    return t if step == 1 and pitch >= t.shape[1] else t.clone(memory_format=torch.contiguous_format)
+    if step == 1 and pitch >= cols:
+        return t, pitch
+    return t.clone(memory_format=torch.contiguous_format), cols
 
 
-def _rows_16(t: torch.Tensor, width: int) -> torch.Tensor:
+def _rows_16(t: torch.Tensor, cols: int, width: int):
     """``_rows_2d``, and copied if its rows are a multiple of ``width``
     elements (16 bytes) but do not lie on 16-byte boundaries: the product
     kernels load such rows in whole chunks."""
     pitch, step = t.stride()
-    cols = t.shape[1]
     if step == 1 and pitch >= cols and (cols % width or (pitch % width == 0 and t.data_ptr() % 16 == 0)):
-        return t
-    return t.clone(memory_format=torch.contiguous_format)
+        return t, pitch
+    return t.clone(memory_format=torch.contiguous_format), cols
 
 
-def _fp8_source(x: torch.Tensor, what: str) -> torch.Tensor:
-    """x as a 2-D matrix with contiguous rows of bf16, fp16 or fp32."""
+def _fp8_source(x: torch.Tensor, what: str):
+    """x as a 2-D matrix with contiguous rows of bf16, fp16 or fp32: (x, its
+    rows, columns and pitch, its type's number)."""
     if not x.is_cuda:
         L.require_gpu(x)
-    if x.dtype not in _FP8_DT:
+    kind = _FP8_DT.get(x.dtype)
+    if kind is None:
         raise TypeError(f"{what} must be bf16, fp16 or fp32, got {x.dtype}")
-    if x.dim() != 2 or x.shape[1] == 0:
-        raise ValueError(f"{what} must be a 2-D matrix with columns, got {tuple(x.shape)}")
-    return _rows_2d(x)
+    shape = x.shape
+    if len(shape) != 2 or shape[1] == 0:
+        raise ValueError(f"{what} must be a 2-D matrix with columns, got {tuple(shape)}")
+    rows, cols = shape
+    x, pitch = _rows_2d(x, cols)
+    return x, rows, cols, pitch, kind
 
 
 def _fp8_matrix(codes: torch.Tensor, scales: torch.Tensor, what: str, blocks: bool, scale_dtypes):
-    """A checked fp8 matrix: e4m3 codes [rows, cols] and its scales."""
+    """A checked fp8 matrix, e4m3 codes and scales: (codes, their rows,
+    columns and pitch, scales, their pitch)."""
     if not (codes.is_cuda and scales.is_cuda):
         L.require_gpu(codes, scales)
-    if codes.dtype != torch.float8_e4m3fn or codes.dim() != 2 or codes.shape[1] == 0:
-        raise TypeError(f"{what} must be a 2-D float8_e4m3fn matrix with columns, got {tuple(codes.shape)} "
-                        f"{codes.dtype}")
-    rows, cols = codes.shape
-    want = (_fp8_groups(rows) if blocks else rows, _fp8_groups(cols))
+    shape = codes.shape
+    if codes.dtype != torch.float8_e4m3fn or len(shape) != 2 or shape[1] == 0:
+        raise TypeError(f"{what} must be a 2-D float8_e4m3fn matrix with columns, got {tuple(shape)} {codes.dtype}")
+    rows, cols = shape
+    groups = -(-cols // FP8_GROUP)
+    want = (-(-rows // FP8_GROUP) if blocks else rows, groups)
     if scales.dtype not in scale_dtypes:
         raise TypeError(f"{what} scales must be {' or '.join(str(d) for d in scale_dtypes)}, got {scales.dtype}")
     if scales.shape != want:
         raise ValueError(f"{what} of {(rows, cols)} takes scales of {want}, got {tuple(scales.shape)}")
-    return _rows_16(codes, 16), _rows_2d(scales)
+    codes, pitch = _rows_16(codes, cols, 16)
+    scales, scale_pitch = _rows_2d(scales, groups)
+    return codes, rows, cols, pitch, scales, scale_pitch
 
 
-def _fp8_gradient(dy: torch.Tensor, cols: int) -> torch.Tensor:
+def _fp8_gradient(dy: torch.Tensor, rows: int | None, cols: int | None):
+    """A checked output gradient of these sizes (None: any): (dy, its rows,
+    columns and pitch)."""
     if not dy.is_cuda:
         L.require_gpu(dy)
     if dy.dtype != torch.bfloat16:
         raise TypeError(f"the output gradient must be bf16, got {dy.dtype}")
-    if dy.dim() != 2 or dy.shape[1] != cols:
-        raise ValueError(f"the output gradient must be [rows, {cols}], got {tuple(dy.shape)}")
-    return _rows_16(dy, 8)
+    shape = dy.shape
+    if len(shape) != 2 or (rows is not None and shape[0] != rows) or (shape[1] != cols if cols else shape[1] == 0):
+        raise ValueError(f"the output gradient must be [{'rows' if rows is None else rows}, {cols or 'out'}], got "
+                         f"{tuple(shape)}")
+    dy, pitch = _rows_16(dy, shape[1], 8)
+    return dy, shape[0], shape[1], pitch
 
 
-def _one_device(first: torch.Tensor, *others) -> None:
-    here = first.get_device()
-    for t in others:
-        if t is not None and t.get_device() != here:
-            raise ValueError(f"operands on several devices: {first.device} and {t.device}")
+def _several_devices(*operands) -> ValueError:
+    return ValueError("operands on several devices: " + " and ".join(str(t.device) for t in operands if t is not None))
 
 
 @functools.lru_cache(maxsize=4096)
@@ -737,7 +748,7 @@ def _fp8_scratch(query: str, rows: int, out: int, cols: int, like: torch.Tensor)
     n = _fp8_workspace(query, rows, out, cols)
     if n == 0:
         return None, None, 0
-    ws = torch.empty(n, dtype=torch.uint8, device=like.device)
+    ws = like.new_empty(n, dtype=torch.uint8)
     return ws, ws.data_ptr(), n
 
 
@@ -749,15 +760,15 @@ def fp8_quantize_groups(x: torch.Tensor, scale_dtype: torch.dtype = torch.float3
     of two not below it, with which the codes are also the 8-bit checkpoint
     that ``fp8_block_grad_weight`` reads.  A group holding an infinity or a
     NaN becomes NaN as a whole."""
-    x = _fp8_source(x, "x")
-    if scale_dtype not in _FP8_SCALES:
+    x, rows, cols, pitch, kind = _fp8_source(x, "x")
+    scale_kind = _FP8_SCALES.get(scale_dtype)
+    if scale_kind is None:
         raise TypeError(f"scale_dtype must be float32 or float8_e8m0fnu, got {scale_dtype}")
-    rows, cols = x.shape
-    groups = _fp8_groups(cols)
+    groups = -(-cols // FP8_GROUP)
     codes = x.new_empty((rows, cols), dtype=torch.float8_e4m3fn)
     scales = x.new_empty((rows, groups), dtype=scale_dtype)
-    rc = L.lib().mi355q_fp8_quantize_groups(x.data_ptr(), _FP8_DT[x.dtype], rows, cols, x.stride(0), codes.data_ptr(),
-                                            cols, scales.data_ptr(), _FP8_SCALES[scale_dtype], groups, L.stream_of(x))
+    rc = L.lib().mi355q_fp8_quantize_groups(x.data_ptr(), kind, rows, cols, pitch, codes.data_ptr(), cols,
+                                            scales.data_ptr(), scale_kind, groups, L.stream_of(x))
     if rc:
         L.check(rc)
     return codes, scales
@@ -768,12 +779,14 @@ def fp8_quantize_blocks(w: torch.Tensor):
     448) per 128 x 128 block: (codes [rows, cols], scales [ceil(rows / 128),
     ceil(cols / 128)]).  A block holding an infinity or a NaN becomes NaN as a
     whole."""
-    w = _fp8_source(w, "w")
-    rows, cols = w.shape
-    codes = torch.empty((rows, cols), dtype=torch.float8_e4m3fn, device=w.device)
-    scales = torch.empty((_fp8_groups(rows), _fp8_groups(cols)), dtype=torch.float32, device=w.device)
-    L.call("mi355q_fp8_quantize_blocks", w.data_ptr(), _FP8_DT[w.dtype], rows, cols, w.stride(0), codes.data_ptr(),
-           cols, scales.data_ptr(), scales.shape[1], L.stream_of(w))
+    w, rows, cols, pitch, kind = _fp8_source(w, "w")
+    groups = -(-cols // FP8_GROUP)
+    codes = w.new_empty((rows, cols), dtype=torch.float8_e4m3fn)
+    scales = w.new_empty((-(-rows // FP8_GROUP), groups), dtype=torch.float32)
+    rc = L.lib().mi355q_fp8_quantize_blocks(w.data_ptr(), kind, rows, cols, pitch, codes.data_ptr(), cols,
+                                            scales.data_ptr(), groups, L.stream_of(w))
+    if rc:
+        L.check(rc)
     return codes, scales
 
 
@@ -785,30 +798,35 @@ def fp8_block_matmul(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w
     block (``fp8_quantize_blocks``, or an FP8_BLOCK checkpoint's
     ``weight_scale`` in fp32).  Sums in fp32, rounded once to ``out_dtype``
     (bf16, fp16 or fp32).  ``bias`` [out] is bf16, fp16 or fp32."""
-    x, x_scales = _fp8_matrix(x, x_scales, "x", False, _FP8_SCALES)
-    w, w_scales = _fp8_matrix(w, w_scales, "w", True, (torch.float32,))
-    rows, cols = x.shape
-    out = w.shape[0]
-    if w.shape[1] != cols or out == 0:
+    x, rows, cols, x_pitch, x_scales, xs_pitch = _fp8_matrix(x, x_scales, "x", False, _FP8_SCALES)
+    w, out, w_cols, w_pitch, w_scales, ws_pitch = _fp8_matrix(w, w_scales, "w", True, _FP8_F32)
+    if w_cols != cols or out == 0:
         raise ValueError(f"x [{rows}, {cols}] does not multiply w {tuple(w.shape)}")
-    if out_dtype not in _FP8_DT:
+    kind = _FP8_DT.get(out_dtype)
+    if kind is None:
         raise TypeError(f"out_dtype must be bf16, fp16 or fp32, got {out_dtype}")
+    here = x.get_device()
+    bias_ptr, bias_kind = None, 0
     if bias is not None:
         if not bias.is_cuda:
             L.require_gpu(bias)
-        if bias.dtype not in _FP8_DT:
+        bias_kind = _FP8_DT.get(bias.dtype)
+        if bias_kind is None:
             raise TypeError(f"bias must be bf16, fp16 or fp32, got {bias.dtype}")
         if bias.shape != (out,):
             raise ValueError(f"bias must be [{out}], got {tuple(bias.shape)}")
         bias = bias.contiguous()
-    _one_device(x, x_scales, w, w_scales, bias)
+        bias_ptr = bias.data_ptr()
+        if bias.get_device() != here:
+            raise _several_devices(x, bias)
+    if w.get_device() != here or x_scales.get_device() != here or w_scales.get_device() != here:
+        raise _several_devices(x, x_scales, w, w_scales)
     y = x.new_empty((rows, out), dtype=out_dtype)
     ws, ws_ptr, ws_bytes = _fp8_scratch("mi355q_fp8_block_matmul_workspace_size", rows, out, cols, x)
     rc = L.lib().mi355q_fp8_block_matmul(
-        x.data_ptr(), x.stride(0), x_scales.data_ptr(), _FP8_SCALES[x_scales.dtype], x_scales.stride(0), w.data_ptr(),
-        w.stride(0), w_scales.data_ptr(), w_scales.stride(0), None if bias is None else bias.data_ptr(),
-        0 if bias is None else _FP8_DT[bias.dtype], y.data_ptr(), _FP8_DT[out_dtype], out, rows, out, cols, ws_ptr,
-        ws_bytes, L.stream_of(x))
+        x.data_ptr(), x_pitch, x_scales.data_ptr(), _FP8_SCALES[x_scales.dtype], xs_pitch, w.data_ptr(), w_pitch,
+        w_scales.data_ptr(), ws_pitch, bias_ptr, bias_kind, y.data_ptr(), kind, out, rows, out, cols, ws_ptr, ws_bytes,
+        L.stream_of(x))
     if rc:
         L.check(rc)
     return y
@@ -818,18 +836,18 @@ def fp8_block_grad_input(dy: torch.Tensor, w: torch.Tensor, w_scales: torch.Tens
     """dX = dY W [rows, cols] in bf16: the input gradient of
     ``fp8_block_matmul`` (dy bf16 [rows, out], w as in the forward product;
     the weight's values enter exactly, sums in fp32)."""
-    w, w_scales = _fp8_matrix(w, w_scales, "w", True, (torch.float32,))
-    out, cols = w.shape
-    dy = _fp8_gradient(dy, out)
+    w, out, cols, w_pitch, w_scales, ws_pitch = _fp8_matrix(w, w_scales, "w", True, _FP8_F32)
     if out == 0:
         raise ValueError("w has no rows")
-    _one_device(dy, w, w_scales)
-    rows = dy.shape[0]
+    dy, rows, _, pitch = _fp8_gradient(dy, None, out)
+    here = dy.get_device()
+    if w.get_device() != here or w_scales.get_device() != here:
+        raise _several_devices(dy, w, w_scales)
     dx = dy.new_empty((rows, cols))
     ws, ws_ptr, ws_bytes = _fp8_scratch("mi355q_fp8_block_grad_input_workspace_size", rows, out, cols, dy)
-    rc = L.lib().mi355q_fp8_block_grad_input(dy.data_ptr(), dy.stride(0), w.data_ptr(), w.stride(0),
-                                             w_scales.data_ptr(), w_scales.stride(0), dx.data_ptr(), cols, rows, out,
-                                             cols, ws_ptr, ws_bytes, L.stream_of(dy))
+    rc = L.lib().mi355q_fp8_block_grad_input(dy.data_ptr(), pitch, w.data_ptr(), w_pitch, w_scales.data_ptr(),
+                                             ws_pitch, dx.data_ptr(), cols, rows, out, cols, ws_ptr, ws_bytes,
+                                             L.stream_of(dy))
     if rc:
         L.check(rc)
     return dx
@@ -842,20 +860,18 @@ def fp8_block_grad_weight(dy: torch.Tensor, x: torch.Tensor, x_scales: torch.Ten
     ``scale_dtype=torch.float8_e8m0fnu``; the checkpoint's values enter
     exactly).  dy bf16 [rows, out]; sums in fp32, rounded once to
     ``out_dtype`` (bf16, fp16 or fp32).  Zeros when there are no rows."""
-    x, x_scales = _fp8_matrix(x, x_scales, "x", False, (torch.float8_e8m0fnu,))
-    rows, cols = x.shape
-    if dy.dim() != 2 or dy.shape[0] != rows or dy.shape[1] == 0:
-        raise ValueError(f"the output gradient must be [{rows}, out], got {tuple(dy.shape)}")
-    out = dy.shape[1]
-    dy = _fp8_gradient(dy, out)
-    if out_dtype not in _FP8_DT:
+    x, rows, cols, x_pitch, x_scales, xs_pitch = _fp8_matrix(x, x_scales, "x", False, _FP8_E8M0)
+    dy, _, out, pitch = _fp8_gradient(dy, rows, None)
+    kind = _FP8_DT.get(out_dtype)
+    if kind is None:
         raise TypeError(f"out_dtype must be bf16, fp16 or fp32, got {out_dtype}")
-    _one_device(dy, x, x_scales)
+    here = dy.get_device()
+    if x.get_device() != here or x_scales.get_device() != here:
+        raise _several_devices(dy, x, x_scales)
     dw = dy.new_empty((out, cols), dtype=out_dtype)
     ws, ws_ptr, ws_bytes = _fp8_scratch("mi355q_fp8_block_grad_weight_workspace_size", rows, out, cols, dy)
-    rc = L.lib().mi355q_fp8_block_grad_weight(dy.data_ptr(), dy.stride(0), x.data_ptr(), x.stride(0),
-                                              x_scales.data_ptr(), x_scales.stride(0), dw.data_ptr(),
-                                              _FP8_DT[out_dtype], cols, rows, out, cols, ws_ptr, ws_bytes,
+    rc = L.lib().mi355q_fp8_block_grad_weight(dy.data_ptr(), pitch, x.data_ptr(), x_pitch, x_scales.data_ptr(),
+                                              xs_pitch, dw.data_ptr(), kind, cols, rows, out, cols, ws_ptr, ws_bytes,
                                               L.stream_of(dy))
     if rc:
         L.check(rc)
@@ -868,17 +884,17 @@ def fp8_silu_mul(gate_up: torch.Tensor, save: bool = True):
     [rows, ceil(n / 128)]).  With ``save`` also gate and up in 8 bits for the
     backward pass: (..., saved codes [rows, 2 n], saved scales [rows, 2
     ceil(n / 128)]), gate's groups before up's."""
-    x = _fp8_source(gate_up, "gate_up")
-    rows, cols = x.shape[0], x.shape[1] // 2
-    if x.shape[1] % 2:
-        raise ValueError(f"gate_up must hold gate and up side by side, got {x.shape[1]} columns")
-    groups = _fp8_groups(cols)
+    x, rows, both, pitch, kind = _fp8_source(gate_up, "gate_up")
+    if both % 2:
+        raise ValueError(f"gate_up must hold gate and up side by side, got {both} columns")
+    cols = both // 2
+    groups = -(-cols // FP8_GROUP)
     h = x.new_empty((rows, cols), dtype=torch.float8_e4m3fn)
     hs = x.new_empty((rows, groups), dtype=torch.float8_e8m0fnu)
     kept = x.new_empty((rows, 2 * cols), dtype=torch.float8_e4m3fn) if save else None
     ks = x.new_empty((rows, 2 * groups), dtype=torch.float8_e8m0fnu) if save else None
-    rc = L.lib().mi355q_fp8_silu_mul(x.data_ptr(), _FP8_DT[x.dtype], rows, cols, x.stride(0), h.data_ptr(), cols,
-                                     hs.data_ptr(), kept.data_ptr() if save else None, 2 * cols,
+    rc = L.lib().mi355q_fp8_silu_mul(x.data_ptr(), kind, rows, cols, pitch, h.data_ptr(), cols, hs.data_ptr(),
+                                     kept.data_ptr() if save else None, 2 * cols,
                                      ks.data_ptr() if save else None, L.stream_of(x))
     if rc:
         L.check(rc)
@@ -888,23 +904,25 @@ def fp8_silu_mul(gate_up: torch.Tensor, save: bool = True):
 def fp8_silu_mul_backward(dh: torch.Tensor, saved: torch.Tensor, saved_scales: torch.Tensor) -> torch.Tensor:
     """The gradient [rows, 2 n] of ``fp8_silu_mul``'s input, in dh's type,
     from dh [rows, n] (bf16, fp16 or fp32) and what the forward pass saved."""
-    dh = _fp8_source(dh, "dh")
+    dh, rows, cols, pitch, kind = _fp8_source(dh, "dh")
     if not (saved.is_cuda and saved_scales.is_cuda):
         L.require_gpu(saved, saved_scales)
-    rows, cols = dh.shape
-    groups = _fp8_groups(cols)
+    groups = -(-cols // FP8_GROUP)
     if saved.dtype != torch.float8_e4m3fn or saved_scales.dtype != torch.float8_e8m0fnu:
         raise TypeError(f"saved codes and scales must be float8_e4m3fn and float8_e8m0fnu, got {saved.dtype} and "
                         f"{saved_scales.dtype}")
     if saved.shape != (rows, 2 * cols) or saved_scales.shape != (rows, 2 * groups):
         raise ValueError(f"dh of {(rows, cols)} takes saved codes of {(rows, 2 * cols)} and scales of "
                          f"{(rows, 2 * groups)}, got {tuple(saved.shape)} and {tuple(saved_scales.shape)}")
-    _one_device(dh, saved, saved_scales)
-    saved, saved_scales = _rows_2d(saved), _rows_2d(saved_scales)
+    here = dh.get_device()
+    if saved.get_device() != here or saved_scales.get_device() != here:
+        raise _several_devices(dh, saved, saved_scales)
+    saved, saved_pitch = _rows_2d(saved, 2 * cols)
+    saved_scales, ss_pitch = _rows_2d(saved_scales, 2 * groups)
     dx = dh.new_empty((rows, 2 * cols))
-    rc = L.lib().mi355q_fp8_silu_mul_backward(dh.data_ptr(), _FP8_DT[dh.dtype], rows, cols, dh.stride(0),
-                                              saved.data_ptr(), saved.stride(0), saved_scales.data_ptr(),
-                                              saved_scales.stride(0), dx.data_ptr(), 2 * cols, L.stream_of(dh))
+    rc = L.lib().mi355q_fp8_silu_mul_backward(dh.data_ptr(), kind, rows, cols, pitch, saved.data_ptr(), saved_pitch,
+                                              saved_scales.data_ptr(), ss_pitch, dx.data_ptr(), 2 * cols,
+                                              L.stream_of(dh))
     if rc:
         L.check(rc)
     return dx
