@@ -1361,8 +1361,9 @@ struct ShapeCost {
 };
 // The cheapest cut by these costs: every shape, whole tiles for as many rounds of
 // the 256 CUs as come out even (or none, for fewer), and 1 .. 16 parts of at least
-// `least` steps for the rest.  Parts cost a second launch (4 us) and their partial
-// sums' way to it (written and read, mostly in the caches: 8 TB/s).
+// `least` steps for the rest.  Parts cost a second launch and a workspace (4 us on
+// the device, 5 on the host, which is what small calls wait for) and their partial
+// sums' way to it (written and read: 5 TB/s).
 static Plan make_plan(const ShapeCost* shapes, int n, int64_t rows, int64_t cols, int64_t steps, int64_t least) {
   Plan best{};
   double best_cost = 0;
@@ -1377,15 +1378,24 @@ static Plan make_plan(const ShapeCost* shapes, int n, int64_t rows, int64_t cols
         if (want > 1 && (rest == 0 || steps / want < least)) break;
         const int64_t per = (steps + want - 1) / want, k = (steps + per - 1) / per;
         const int64_t wgs = rest * k, whole = full / 256, parts = (wgs + 255) / 256;
-        // rounds run in pairs where two workgroups fit a CU; an odd last one runs alone
-        double t;
+        double t = (whole + parts) * c.ends;
         if (c.two > 0) {
-          t = (whole * steps + parts * per) * c.two / 2 + ((whole + parts + 1) / 2) * c.ends;
-          if ((whole + parts) % 2) t += (parts ? per : steps) * (c.one - c.two / 2);
+          // rounds run in pairs; a whole one left over shares its CU with the
+          // parts while they last, a part left over has it to itself
+          t -= (whole + parts) / 2 * c.ends;
+          t += whole / 2 * steps * c.two;
+          int64_t left = parts * per, alone = parts % 2 * per;
+          if (whole % 2) {
+            const int64_t both = left < steps ? left : steps;
+            t += both * c.two + (steps - both) * c.one;
+            left -= both;
+            alone = 0;
+          }
+          t += (left - alone) * c.two / 2 + alone * c.one;
         } else {
-          t = (whole * steps + parts * per) * c.one + (whole + parts) * c.ends;
+          t += (whole * steps + parts * per) * c.one;
         }
-        if (k > 1) t += 4 + (double)wgs * c.tile_rows * c.tile_cols * 8 / 8e6;
+        if (k > 1) t += 7 + (double)wgs * c.tile_rows * c.tile_cols * 8 / 5e6;
         if (best.tile_rows == 0 || t < best_cost) {
           best_cost = t;
           best = Plan{i, (uint32_t)c.tile_rows, (uint32_t)c.tile_cols, (uint32_t)tr, (uint32_t)tc,
@@ -1402,20 +1412,20 @@ static Plan make_plan(const ShapeCost* shapes, int n, int64_t rows, int64_t cols
 // these in 2 / 4 / 8 parts 19 / 16 / 19; 333 x 4096 x 14336 in 96 tiles of 128 x 128 110 us,
 // in 2 / 5 / 8 parts 73 / 58 / 61, in 192 of 64 x 128 in 1 / 4 parts 92 / 64.
 static Plan plan_forward(int64_t rows, int64_t cols, int64_t sum) {
-  static const ShapeCost shapes[] = {{64, 128, 0.69, 1.0, 4}, {128, 128, 0.93, 1.75, 4}};
+  static const ShapeCost shapes[] = {{64, 128, 0.75, 1.1, 4}, {128, 128, 1.0, 1.75, 4}};
   return make_plan(shapes, 2, rows, cols, group_count(sum), 4);
 }
 // Input gradient: 1024 x 4096 x 4096 48 us in 256 tiles of 128 x 128, 46 in 512 of 64 x 128;
 // 16 x 4096 x 4096 44 us and 35, these in 2 / 4 / 8 / 16 parts 22 / 14 / 11 / 12.
 static Plan plan_grad_input(int64_t rows, int64_t cols, int64_t sum) {
-  static const ShapeCost shapes[] = {{64, 128, 0.95, 1.2, 4}, {128, 128, 1.2, 2.1, 4}};
+  static const ShapeCost shapes[] = {{64, 128, 1.0, 1.25, 4}, {128, 128, 1.3, 2.0, 4}};
   return make_plan(shapes, 2, rows, cols, group_count(sum), 2);
 }
 // Weight gradient, in stages of 32 tokens: 8192 x 1024 x 4096 in 256 tiles of 128 x 128 106 us, in
 // 64 of 256 x 256 in 1 / 2 / 4 / 8 parts 216 / 127 / 89 / 108; 517 x 768 x 2048 in 96 of 128 x 128
 // 12 us, in 24 of 256 x 256 22; 1024 x 4096 x 4096 in 256 of 256 x 256 39 us, 1024 of 128 x 128 60.
 static Plan plan_weight(int64_t rows, int64_t out, int64_t cols) {
-  static const ShapeCost shapes[] = {{128, 128, 0.39, 0.7, 4}, {256, 256, 0.9, 0, 8}};
+  static const ShapeCost shapes[] = {{128, 128, 0.37, 0.65, 5}, {256, 256, 0.88, 0, 8}};
   return make_plan(shapes, 2, out, cols, (rows + 31) / 32, 4);
 }
 static size_t plan_bytes(const Plan& p) {
