@@ -1521,13 +1521,21 @@ static int launch_grad_weight(const ProductArgs& g, const Plan& p, float* parts,
 // The tile kernels take operands in 16-byte chunks.  Rows whose width is no whole
 // number of them are first copied to rows that are, ending in zeros: a read and a
 // write of both operands, of which the product reads each many times.
-__global__ __launch_bounds__(256) void pad_rows_kernel(const uint8_t* src, int64_t pitch, int64_t row_bytes,
-                                                       uint8_t* dst, uint32_t chunks, FastDiv per_row) {
-  const uint32_t i = blockIdx.x * 256 + threadIdx.x;
-  if (i >= chunks) return;
-  const uint32_t r = div(i, per_row);
-  const int64_t at = (int64_t)(i - r * per_row.d) * 16, left = row_bytes - at;
-  const uint8_t* p = src + r * pitch + at;
+// One launch for both operands: the first `blocks` workgroups take the first.
+struct PadJob {
+  const uint8_t* src;
+  int64_t pitch, row_bytes;
+  uint8_t* dst;
+  uint32_t chunks;
+  FastDiv per_row;
+};
+__global__ __launch_bounds__(256) void pad_rows_kernel(PadJob first, PadJob second, uint32_t blocks) {
+  const PadJob& job = blockIdx.x < blocks ? first : second;
+  const uint32_t i = (blockIdx.x < blocks ? blockIdx.x : blockIdx.x - blocks) * 256 + threadIdx.x;
+  if (i >= job.chunks) return;
+  const uint32_t r = div(i, job.per_row);
+  const int64_t at = (int64_t)(i - r * job.per_row.d) * 16, left = job.row_bytes - at;
+  const uint8_t* p = job.src + r * job.pitch + at;
   u32x4_t v;
   if (left >= 16) {
     __builtin_memcpy(&v, p, 16);
@@ -1537,21 +1545,38 @@ __global__ __launch_bounds__(256) void pad_rows_kernel(const uint8_t* src, int64
     for (int e = 0; e < 16; ++e) b[e] = e < left ? p[e] : 0;
     __builtin_memcpy(&v, b, 16);
   }
-  *reinterpret_cast<u32x4_t*>(dst + (int64_t)i * 16) = v;
+  *reinterpret_cast<u32x4_t*>(job.dst + (int64_t)i * 16) = v;
 }
 static int64_t padded(int64_t row_bytes) { return (row_bytes + 15) / 16 * 16; }
 static size_t padded_bytes(int64_t rows, int64_t row_bytes) { return (size_t)rows * padded(row_bytes); }
-static int pad_rows(const void* src, int64_t pitch, int64_t rows, int64_t row_bytes, void* dst, hipStream_t st) {
-  const int64_t per = padded(row_bytes) / 16, most = ((int64_t(1) << 31) - 256) / per;
-  for (int64_t r = 0; r < rows; r += most) {
-    const int64_t n = rows - r < most ? rows - r : most;
-    hipLaunchKernelGGL(pad_rows_kernel, dim3((unsigned)((n * per + 255) / 256)), dim3(256), 0, st,
-                       static_cast<const uint8_t*>(src) + r * pitch, pitch, row_bytes,
-                       static_cast<uint8_t*>(dst) + r * per * 16, (uint32_t)(n * per), fast_div((uint32_t)per));
+
+// Copies to be made before a product: two of them, of 2^30 chunks at the most, in one launch.
+struct Padding {
+  PadJob jobs[2] = {};
+  int n = 0;
+  const hipStream_t st;
+  explicit Padding(hipStream_t stream) : st(stream) {}
+  static uint32_t blocks(const PadJob& j) { return (j.chunks + 255) / 256; }
+  int flush() {
+    if (n == 0) return MI355Q_OK;
+    hipLaunchKernelGGL(pad_rows_kernel, dim3(blocks(jobs[0]) + (n > 1 ? blocks(jobs[1]) : 0)), dim3(256), 0, st, jobs[0],
+                       jobs[1], blocks(jobs[0]));
+    n = 0;
     MQ_LAUNCH_CHECK();
+    return MI355Q_OK;
   }
-  return MI355Q_OK;
-}
+  int add(const void* src, int64_t pitch, int64_t rows, int64_t row_bytes, void* dst) {
+    const int64_t per = padded(row_bytes) / 16, most = (int64_t(1) << 30) / per;
+    for (int64_t r = 0; r < rows; r += most) {
+      if (n == 2)
+        if (const int rc = flush()) return rc;
+      const int64_t m = rows - r < most ? rows - r : most;
+      jobs[n++] = PadJob{static_cast<const uint8_t*>(src) + r * pitch, pitch, row_bytes,
+                         static_cast<uint8_t*>(dst) + r * per * 16, (uint32_t)(m * per), fast_div((uint32_t)per)};
+    }
+    return MI355Q_OK;
+  }
+};
 
 // Odd widths and a sum of one step: the element loads of one launch cost less than
 // copies of both operands (2102 x 80 x 69 9 us against 18; 100 rows into 300 x 301 13 against
@@ -1623,8 +1648,10 @@ extern "C" int mi355q_fp8_block_matmul(const uint8_t* x_dev, int64_t ldx, const 
       return launch_any<kForward>(g, y_dtype, st, "fp8_block_matmul");
     char* const xc = static_cast<char*>(workspace_dev) + base;
     char* const wc = xc + padded_bytes(rows, cols);
-    if (const int rc = pad_rows(x_dev, ldx, rows, cols, xc, st)) return rc;
-    if (const int rc = pad_rows(w_dev, ldw, out, cols, wc, st)) return rc;
+    Padding pad(st);
+    if (const int rc = pad.add(x_dev, ldx, rows, cols, xc)) return rc;
+    if (const int rc = pad.add(w_dev, ldw, out, cols, wc)) return rc;
+    if (const int rc = pad.flush()) return rc;
     g.a = xc;
     g.b = reinterpret_cast<const uint8_t*>(wc);
     g.lda = g.ldb = g.R = padded(cols);
@@ -1672,16 +1699,18 @@ extern "C" int mi355q_fp8_block_grad_input(const uint16_t* dy_dev, int64_t lddy,
         !small_pitch(out) || short_sum(rows, cols, out))
       return launch_any<kGradInput>(g, MI355Q_BF16, st, "fp8_block_grad_input");
     char* const yc = static_cast<char*>(workspace_dev) + base;
+    Padding pad(st);
     if (!y_ok) {
-      if (const int rc = pad_rows(dy_dev, 2 * lddy, rows, 2 * out, yc, st)) return rc;
+      if (const int rc = pad.add(dy_dev, 2 * lddy, rows, 2 * out, yc)) return rc;
       g.a = yc;
       g.lda = padded(2 * out) / 2;
     }
     if (!w_ok) {
-      if (const int rc = pad_rows(w_dev, ldw, out, cols, yc + y_bytes, st)) return rc;
+      if (const int rc = pad.add(w_dev, ldw, out, cols, yc + y_bytes)) return rc;
       g.b = reinterpret_cast<const uint8_t*>(yc + y_bytes);
       g.ldb = padded(cols);
     }
+    if (const int rc = pad.flush()) return rc;
   }
   return p.shape ? launch_grad_input<2, 2>(g, p, parts, st) : launch_grad_input<1, 2>(g, p, parts, st);
 }
@@ -1728,16 +1757,18 @@ extern "C" int mi355q_fp8_block_grad_weight(const uint16_t* dy_dev, int64_t lddy
         !small_pitch(out) || short_sum(out, cols, rows))
       return launch_any<kGradWeight>(g, dw_dtype, st, "fp8_block_grad_weight");
     char* const yc = static_cast<char*>(workspace_dev) + base;
+    Padding pad(st);
     if (!y_ok) {
-      if (const int rc = pad_rows(dy_dev, 2 * lddy, rows, 2 * out, yc, st)) return rc;
+      if (const int rc = pad.add(dy_dev, 2 * lddy, rows, 2 * out, yc)) return rc;
       g.a = yc;
       g.lda = padded(2 * out) / 2;
     }
     if (!x_ok) {
-      if (const int rc = pad_rows(x_dev, ldx, rows, cols, yc + y_bytes, st)) return rc;
+      if (const int rc = pad.add(x_dev, ldx, rows, cols, yc + y_bytes)) return rc;
       g.b = reinterpret_cast<const uint8_t*>(yc + y_bytes);
       g.ldb = padded(cols);
     }
+    if (const int rc = pad.flush()) return rc;
   }
   return p.shape ? launch_grad_weight<4, 2, 2, 4>(g, p, parts, st) : launch_grad_weight<2, 2, 2, 2>(g, p, parts, st);
 }
