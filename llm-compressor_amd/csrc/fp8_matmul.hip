@@ -167,12 +167,12 @@ __global__ __launch_bounds__(256) void product_any_kernel(ProductArgs g) {
 //
 // Four waves with 2 x 2 tiles each, two workgroups on a CU: one's scaling and
 // conversions run beside the other's MFMAs (one workgroup of eight waves with
-// 256 x 128 tiles 2.06 ms against 1.77).  8192 x 28672 x 4096 1.77 ms, 1.09 PFLOP/s.  Per
-// MFMA it issues 7 vector instructions (4 conversions, 2 scaling FMAs); MFMAs and
-// vector instructions are busy 0.57 and 0.60 of the cycles at 1.75 GHz, down from
-// 2.4: what bounds it is power, which the conversions and the traffic from LDS
-// share with the MFMAs.  HBM reads are 2.8 GB of 150 MB (the operands once a row of
-// tiles and XCD), 1.6 TB/s.
+// 256 x 128 tiles 2.06 ms against 1.81, where this kernel now takes 1.71).
+// 8192 x 28672 x 4096 1.71 ms, 1.13 PFLOP/s.  Per MFMA it issues 6.3 vector
+// instructions (4 conversions, 2 scaling FMAs); MFMAs and vector instructions are
+// busy 0.62 and 0.61 of the cycles at 1.64 GHz, down from 2.4: what bounds it is
+// power, which the conversions and the traffic from LDS share with the MFMAs.
+// (The same loads from one tile's addresses, always in L2: 3 % less.)
 typedef __attribute__((address_space(3))) void lds_void_t;
 
 __device__ __forceinline__ uint32_t lds_u32(const void* p) {
@@ -631,9 +631,11 @@ void fp8_forward_kernel(ProductArgs g, TileOrder order, int steps_per_split, flo
 // run over the two steps of a 128 x 128 block before they take its scale.
 //
 // 128 x 128 tiles on four waves, two workgroups on a CU (256 x 128 on eight waves
-// 1.03 .. 1.05 ms against 1.00 .. 1.02).  8192 x 4096 x 14336 0.97 ms, 0.99 PFLOP/s: MFMAs busy
-// 0.51 of the cycles, vector instructions 0.38, at 1.71 GHz: power again, and the
-// LDS, which carries dY in 16 bits.
+// 1.03 .. 1.05 ms against 1.00 .. 1.02, before the steps lost their conditions).
+// 8192 x 4096 x 14336 0.91 ms, 1.06 PFLOP/s: MFMAs busy 0.60 of the cycles, vector
+// instructions 0.42, at 1.56 GHz: power again, and the LDS, which carries dY in
+// 16 bits.  Few tiles are bound by a wave's instructions, not by what they wait
+// for: rings of five and seven steps took as long as this one of three.
 template <int T, int WT>
 struct GradInputShape {
   static constexpr int A = 2, WF = 2;                        // 128 columns: one block scale per workgroup
@@ -858,10 +860,10 @@ void fp8_grad_input_kernel(ProductArgs g, TileOrder order, int blocks_per_split,
 // to be in the operand: each wave's DMA brings codes and scale bytes of its own
 // rows, and the wave writes them to LDS as bf16, scaled by the conversion (exact).
 // The MFMAs then add straight into the accumulators: vector instructions are few
-// (busy 0.18 of the cycles), so a large tile on eight waves, 256 x 256, saves
-// LDS reads (one wave's operands serve 4 x 2 tiles).  8192 x 4096 x 14336 0.865 ms,
-// 1.11 PFLOP/s, 16 us of it the sum of the split tiles; MFMAs busy 0.57 of the cycles
-// at 1.92 GHz.  Bound by the LDS, which a stage's rows pass twice, and by power.
+// (busy 0.15 of the cycles), so a large tile on eight waves, 256 x 256, saves
+// LDS reads (one wave's operands serve 4 x 2 tiles).  8192 x 4096 x 14336 0.80 ms,
+// 1.21 PFLOP/s, 17 us of it the sum of the split tiles; MFMAs busy 0.65 of the cycles
+// at 1.74 GHz.  Bound by power, and by the LDS, which a stage's rows pass twice.
 template <int MB, int NB2, int WK, int WN>
 struct GradWeightShape {
   static constexpr int W = WK * WN, NTH = 64 * W;
@@ -1230,8 +1232,8 @@ __global__ __launch_bounds__(256) void sum_splits_kernel(ProductArgs g, TileOrde
 // tokens come from L2, and the W waves of a workgroup take every W-th step of 16 AF
 // features; their sums are joined in LDS.  Bound by the weight's bytes, so what
 // counts is loads in flight: U steps are requested before the first is used.
-// 1 x 14336 x 4096 16.3 us (58.7 MB, 3.6 TB/s: a launch this short ends before HBM is
-// at its full rate).
+// 1 x 14336 x 4096 16 us (58.7 MB, 3.7 TB/s: a launch this short ends before HBM is
+// at its full rate; eight waves, eight steps or nontemporal loads 16 .. 19).
 typedef int i32x4_t __attribute__((ext_vector_type(4)));
 typedef int i32x8_t __attribute__((ext_vector_type(8)));
 
@@ -1407,23 +1409,24 @@ static Plan make_plan(const ShapeCost* shapes, int n, int64_t rows, int64_t cols
   return best;
 }
 // Forward and input gradient: `rows` tokens by `cols` columns, `sum` terms in
-// blocks of 128.  Measured, forward: 1024 x 4096 x 4096 in 256 tiles of 128 x 128 40 us,
-// in 512 of 64 x 128 41; 100 x 4096 x 4096 in 32 tiles of 128 x 128 36 us, 64 of 64 x 128 28,
-// these in 2 / 4 / 8 parts 19 / 16 / 19; 333 x 4096 x 14336 in 96 tiles of 128 x 128 110 us,
-// in 2 / 5 / 8 parts 73 / 58 / 61, in 192 of 64 x 128 in 1 / 4 parts 92 / 64.
+// blocks of 128.  Measured, forward: 1024 x 4096 x 4096 in 256 tiles of 128 x 128 39 us,
+// in 512 of 64 x 128 41; 100 x 4096 x 4096 in 32 tiles of 128 x 128 34 us, 64 of 64 x 128 27,
+// these in 2 / 4 / 8 parts 19 / 20 / 20; 333 x 4096 x 14336 in 96 tiles of 128 x 128 116 us,
+// in 2 / 5 / 8 parts 69 / 58 / 63, in 192 of 64 x 128 in 1 / 4 parts 101 / 71.
 static Plan plan_forward(int64_t rows, int64_t cols, int64_t sum) {
   static const ShapeCost shapes[] = {{64, 128, 0.75, 1.1, 4}, {128, 128, 1.0, 1.75, 4}};
   return make_plan(shapes, 2, rows, cols, group_count(sum), 4);
 }
-// Input gradient: 1024 x 4096 x 4096 48 us in 256 tiles of 128 x 128, 46 in 512 of 64 x 128;
-// 16 x 4096 x 4096 44 us and 35, these in 2 / 4 / 8 / 16 parts 22 / 14 / 11 / 12.
+// Input gradient: 1024 x 4096 x 4096 45 us in 256 tiles of 128 x 128, 41 in 512 of 64 x 128;
+// 16 x 4096 x 4096 39 us and 31, these in 2 / 4 / 8 / 16 parts 20 / 14 / 14 / 14;
+// 450 x 12544 x 7936 139 us in 248 tiles of 128 x 128, 114 in two parts each.
 static Plan plan_grad_input(int64_t rows, int64_t cols, int64_t sum) {
   static const ShapeCost shapes[] = {{64, 128, 1.0, 1.25, 4}, {128, 128, 1.3, 2.0, 4}};
   return make_plan(shapes, 2, rows, cols, group_count(sum), 2);
 }
-// Weight gradient, in stages of 32 tokens: 8192 x 1024 x 4096 in 256 tiles of 128 x 128 106 us, in
-// 64 of 256 x 256 in 1 / 2 / 4 / 8 parts 216 / 127 / 89 / 108; 517 x 768 x 2048 in 96 of 128 x 128
-// 12 us, in 24 of 256 x 256 22; 1024 x 4096 x 4096 in 256 of 256 x 256 39 us, 1024 of 128 x 128 60.
+// Weight gradient, in stages of 32 tokens: 8192 x 1024 x 4096 in 256 tiles of 128 x 128 98 us, in
+// 64 of 256 x 256 in 1 / 2 / 4 / 8 parts 162 / 98 / 77 / 98; 517 x 768 x 2048 in 96 of 128 x 128
+// 12 us, in 24 of 256 x 256 20; 1024 x 4096 x 4096 in 256 of 256 x 256 37 us, 1024 of 128 x 128 49.
 static Plan plan_weight(int64_t rows, int64_t out, int64_t cols) {
   static const ShapeCost shapes[] = {{128, 128, 0.37, 0.65, 5}, {256, 256, 0.88, 0, 8}};
   return make_plan(shapes, 2, out, cols, (rows + 31) / 32, 4);
@@ -1455,8 +1458,8 @@ static int launch_any(ProductArgs g, mi355q_dtype out, hipStream_t st, const cha
   return MI355Q_OK;
 }
 
-// Up to here the weight's bytes decide (24 x 4096 x 4096 12 us against 18 in tiles, 24 x 14336 x 4096 23
-// against 25); beyond, 48 tokens took 15 .. 17 us against 18, but 35 .. 47 against 28.
+// Up to here the weight's bytes decide (24 x 4096 x 4096 12 us against 13 in split tiles, which are two launches,
+// 24 x 14336 x 4096 23 against 21); beyond, 48 tokens took 15 .. 17 us against 14, and 35 .. 47 against 23.
 constexpr int64_t kFewTokens = 32;
 
 template <int TF, int AF, int W, int U>
@@ -1579,8 +1582,8 @@ struct Padding {
 };
 
 // Odd widths and a sum of one step: the element loads of one launch cost less than
-// copies of both operands (2102 x 80 x 69 9 us against 18; 100 rows into 300 x 301 13 against
-// 14; with three steps 300 x 513 x 515 44 against 17), unless the output is large.
+// copies of both operands (2102 x 80 x 69 9 us against 16; with three steps 300 x 513 x 515
+// 44 against 14), unless the output is large.
 static bool short_sum(int64_t rows, int64_t cols, int64_t sum) {
   return sum <= kGroup && ((rows + GT - 1) / GT) * ((cols + GT - 1) / GT) <= 1024;
 }
