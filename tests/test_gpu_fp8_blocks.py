@@ -666,3 +666,51 @@ def test_every_e8m0_scale(dev, rows):
         want = torch.exp2(b.double() - 127)
         want[b == 255] = math.nan
         assert torch.equal(y.double().nan_to_num(-1.0), want[:, None].expand(-1, 128).nan_to_num(-1.0))
+
+
+def test_offsets_past_32_bits(dev):
+    """Operands and outputs of more than 2^32 elements' bytes: rows that repeat every 1024 give results that do, and a
+    weight gradient of rows that are zero but for the last 1024 is theirs (small integers: every sum is exact)."""
+    o = ops()
+    g = gen(73)
+    period, times, wide = 1024, 512, 8320          # 2^19 rows of 8320: 4.4e9 codes, 8.7e9 bytes of bf16
+    rows = period * times
+
+    def base(cols):
+        return heavy(g, period, cols).to(torch.bfloat16).to(dev)
+
+    def repeats(t, unit):
+        t = t.view(torch.uint8).view(-1, unit * t.shape[-1] * t.element_size())
+        return all(torch.equal(t[i], t[0]) for i in (1, t.shape[0] // 2, t.shape[0] - 2, t.shape[0] - 1))
+
+    x = base(wide).repeat(times, 1)
+    assert x.numel() * 2 > 2 ** 33
+    codes, scales = o.fp8_quantize_groups(x, E8M0)
+    assert repeats(codes, period) and repeats(scales, period)
+    assert all(repeats(t, r) for t, r in zip(o.fp8_quantize_blocks(x), (period, period // G)))
+    h, hs, kept, ks = o.fp8_silu_mul(x)
+    assert all(repeats(t, period) for t in (h, hs, kept, ks))
+    del h, hs
+    dh = base(wide // 2).repeat(times, 1)
+    assert repeats(o.fp8_silu_mul_backward(dh, kept, ks), period)
+    del dh, kept, ks
+    narrow, tall = base(128).repeat(times, 1), heavy(g, wide, 128).to(torch.bfloat16).to(dev)
+    w, ws = o.fp8_quantize_blocks(tall.t().contiguous())            # [128, wide]
+    v, vs = o.fp8_quantize_blocks(tall)                             # [wide, 128]
+    assert repeats(o.fp8_block_matmul(codes, scales, w, ws), period)
+    assert repeats(o.fp8_block_matmul(*o.fp8_quantize_groups(narrow), v, vs), period)
+    assert repeats(o.fp8_block_grad_input(x, v, vs), period)
+    assert repeats(o.fp8_block_grad_input(narrow, w, ws), period)
+    del x, codes, scales
+    one = torch.full((rows, wide // G), 127, dtype=torch.uint8, device=dev).view(E8M0)
+    for out, cols in ((128, wide), (wide, 128)):
+        dy = torch.zeros(rows, out, dtype=torch.bfloat16, device=dev)
+        dy[-period:] = torch.randint(-8, 9, (period, out), generator=g).to(torch.bfloat16).to(dev)
+        c = torch.randint(-8, 9, (period, cols), generator=g).to(torch.float32).to(E4M3).to(dev)
+        c = c.view(torch.uint8).repeat(times, 1).view(E4M3)
+        e = one[:, :cols // G]
+        got = o.fp8_block_grad_weight(dy, c, e, torch.float32)
+        assert torch.equal(got, o.fp8_block_grad_weight(dy[-period:], c[-period:], e[-period:], torch.float32))
+        del dy, c
+    del one, narrow, e, got
+    torch.cuda.empty_cache()
