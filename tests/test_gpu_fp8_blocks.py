@@ -714,3 +714,105 @@ def test_offsets_past_32_bits(dev):
         del dy, c
     del one, narrow, e, got
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("rows,out,cols", [(1, 136, 256), (20, 300, 400), (33, 128, 128), (100, 264, 1040), (200, 24, 2064),
+                                           (517, 384, 48), (70, 131, 133)])
+@pytest.mark.parametrize("off", [16, 3])
+def test_only_the_views_are_touched(dev, off, rows, out, cols):
+    """Operands and outputs are views into larger buffers: NaN all around the operands reaches no result, and what is
+    around the outputs stays as it was."""
+    from llmcompressor_amd import _lib as L
+    o, lib, g = ops(), L.lib(), gen(79, rows, out, cols, off)
+    x, xs, w, ws = fp8_pair(g, rows, out, cols, E8M0)
+    dy = heavy(g, rows, out).to(torch.bfloat16).to(dev)
+
+    def inside(shape, dtype, fill):
+        pitch = (shape[1] + off + 47) // 16 * 16 + (off % 16)
+        buf = torch.full((shape[0] + 4, pitch), fill, dtype=torch.float32, device=dev).to(dtype)
+        return buf, buf[2:2 + shape[0], off:off + shape[1]]
+
+    def poisoned(t):
+        buf, v = inside(t.shape, t.dtype, float("nan"))
+        v.copy_(t)
+        return v
+
+    def unchanged(buf, v):
+        v.fill_(7)
+        return bool((buf.float() == 7).all())
+    px, pxs, pw, pws, pdy = (poisoned(t) for t in (x, xs, w, ws, dy))
+    a, b, d = values(x, xs), values(w, ws), dy.cpu().double()
+    st = L.stream_of(x)
+    for dtype, code in ((torch.float32, L.F32), (torch.bfloat16, L.BF16), (torch.float16, L.F16)):
+        for query, shape, want, mags, call in (
+                ("mi355q_fp8_block_matmul", (rows, out), a @ b.T, a.abs() @ b.abs().T,
+                 lambda v, p, n: (px.data_ptr(), px.stride(0), pxs.data_ptr(), L.SCALE_E8M0, pxs.stride(0), pw.data_ptr(),
+                                  pw.stride(0), pws.data_ptr(), pws.stride(0), None, 0, v.data_ptr(), code, v.stride(0),
+                                  rows, out, cols, p, n, st)),
+                ("mi355q_fp8_block_grad_input", (rows, cols), d @ b, d.abs() @ b.abs(),
+                 lambda v, p, n: (pdy.data_ptr(), pdy.stride(0), pw.data_ptr(), pw.stride(0), pws.data_ptr(),
+                                  pws.stride(0), v.data_ptr(), v.stride(0), rows, out, cols, p, n, st)),
+                ("mi355q_fp8_block_grad_weight", (out, cols), d.T @ a, d.abs().T @ a.abs(),
+                 lambda v, p, n: (pdy.data_ptr(), pdy.stride(0), px.data_ptr(), px.stride(0), pxs.data_ptr(),
+                                  pxs.stride(0), v.data_ptr(), code, v.stride(0), rows, out, cols, p, n, st))):
+            if query.endswith("grad_input") and dtype != torch.bfloat16:
+                continue
+            for room in (0, getattr(lib, query + "_workspace_size")(rows, out, cols)):
+                scratch = torch.full((room + 256,), 255, dtype=torch.uint8, device=dev)
+                buf, v = inside(shape, dtype, 7)
+                L.check(getattr(lib, query)(*call(v, scratch.data_ptr() if room else None, room)))
+                check_sum(v.contiguous(), want, mags, dtype)
+                assert unchanged(buf, v), query
+                assert bool((scratch[room:] == 255).all())
+
+
+@pytest.mark.parametrize("rows,cols", [(1, 128), (3, 300), (130, 392), (17, 16), (5, 7)])
+@pytest.mark.parametrize("off", [16, 3])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_quantizers_touch_only_their_views(dev, rows, cols, off, dtype):
+    """The same of the quantizers and the gated activation: NaN around the inputs, a byte pattern around the outputs."""
+    from llmcompressor_amd import _lib as L
+    o, lib, g = ops(), L.lib(), gen(83, rows, cols, off)
+    code, st, groups = L.BF16 if dtype == torch.bfloat16 else L.F32, L.stream_of(torch.zeros(1, device=dev)), -(-cols // G)
+
+    def poisoned(t):
+        buf = torch.full((t.shape[0] + 4, t.shape[1] + 2 * off), float("nan"), device=dev).to(t.dtype)
+        v = buf[2:-2, off:off + t.shape[1]]
+        v.copy_(t)
+        return v
+
+    def guarded(r, c, size):
+        buf = torch.full((r + 4, (c + 2 * off) * size), 0xA5, dtype=torch.uint8, device=dev)
+        return buf, buf[2:-2, off * size:(off + c) * size]
+
+    def check(outs, want):
+        for (buf, v), w in zip(outs, want):
+            assert torch.equal(v.contiguous(), w.contiguous().view(torch.uint8).reshape(v.shape))
+            v.fill_(0xA5)
+            assert bool((buf == 0xA5).all())
+    x = heavy(g, rows, 2 * cols).to(dtype).to(dev)
+    p, half = poisoned(x), x[:, :cols].contiguous()
+    q = poisoned(half)
+    for kind, num, size in ((torch.float32, L.SCALE_F32, 4), (E8M0, L.SCALE_E8M0, 1)):
+        (cb, c), (sb, s) = outs = guarded(rows, cols, 1), guarded(rows, groups, size)
+        L.check(lib.mi355q_fp8_quantize_groups(q.data_ptr(), code, rows, cols, q.stride(0), c.data_ptr(), c.stride(0),
+                                               s.data_ptr(), num, s.stride(0) // size, st))
+        check(outs, o.fp8_quantize_groups(half, kind))
+    (cb, c), (sb, s) = outs = guarded(rows, cols, 1), guarded(-(-rows // G), groups, 4)
+    L.check(lib.mi355q_fp8_quantize_blocks(q.data_ptr(), code, rows, cols, q.stride(0), c.data_ptr(), c.stride(0),
+                                           s.data_ptr(), s.stride(0) // 4, st))
+    check(outs, o.fp8_quantize_blocks(half))
+    want = o.fp8_silu_mul(x)
+    flat = [torch.full((2 + rows * n, 1), 0xA5, dtype=torch.uint8, device=dev) for n in (groups, 2 * groups)]
+    outs = guarded(rows, cols, 1), (flat[0], flat[0][1:-1]), guarded(rows, 2 * cols, 1), (flat[1], flat[1][1:-1])
+    h, hs, kept, ks = (v for _, v in outs)
+    L.check(lib.mi355q_fp8_silu_mul(p.data_ptr(), code, rows, cols, p.stride(0), h.data_ptr(), h.stride(0), hs.data_ptr(),
+                                    kept.data_ptr(), kept.stride(0), ks.data_ptr(), st))
+    check(outs, want)
+    dh = heavy(g, rows, cols).to(dtype).to(dev)
+    pd, pk, ps = poisoned(dh), poisoned(want[2]), poisoned(want[3])
+    size = dh.element_size()
+    (db, d), = outs = guarded(rows, 2 * cols, size),
+    L.check(lib.mi355q_fp8_silu_mul_backward(pd.data_ptr(), code, rows, cols, pd.stride(0), pk.data_ptr(), pk.stride(0),
+                                             ps.data_ptr(), ps.stride(0), d.data_ptr(), d.stride(0) // size, st))
+    check(outs, (o.fp8_silu_mul_backward(dh, want[2], want[3]),))
