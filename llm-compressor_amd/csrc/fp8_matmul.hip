@@ -299,38 +299,45 @@ __device__ __forceinline__ void store_tiles(const ProductArgs& g, f32x16_t (&acc
     biases[i] = g.bias && f0 + i < g.Q ? load_typed(g.bias, g.bias_type, f0 + i) : 0.f;
   __syncthreads();
   const float* const bw = biases + wf * A * 32 + 4 * (lane >> 5);
-  if (g.c_type == MI355Q_F32) {
+  // Outputs go through LDS (the wave's own part of it), so that a token's features
+  // leave as 16-byte stores of whole lines; straight from the tiles they are pieces of
+  // 16 or 32 bytes.
+  char* const stage = ring + wave * 32 * T * S::PITCH;
+  if (g.c_type == MI355Q_F32) {   // one column of tiles at a time
+    static_assert(S::PITCH >= 144, "32 fp32 columns and a shift of the banks");
     float* const out = static_cast<float*>(g.c);
-    const int64_t ld = g.ldc;
-    const bool wide = ld % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+    const bool wide = g.ldc % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
 #pragma unroll
-    for (int a = 0; a < A; ++a)
+    for (int a = 0; a < A; ++a) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int64_t f = fw + 32 * a + 8 * j + 4 * (lane >> 5);
         const f32x4_t bias = *reinterpret_cast<const f32x4_t*>(bw + 32 * a + 8 * j);
 #pragma unroll
-        for (int b = 0; b < T; ++b) {
-          const int64_t t = tw + 32 * b + (lane & 31);
-          const f32x4_t v = f32x4_t{acc[a][b][4 * j], acc[a][b][4 * j + 1], acc[a][b][4 * j + 2],
-                                    acc[a][b][4 * j + 3]} + bias;
-          if (t < g.P) {
-            float* o = out + t * ld + f;
-            if (wide && f + 4 <= g.Q) {
-              *reinterpret_cast<f32x4_t*>(o) = v;
-            } else {
+        for (int b = 0; b < T; ++b)
+          *reinterpret_cast<f32x4_t*>(stage + (32 * b + (lane & 31)) * S::PITCH + 32 * j + 16 * (lane >> 5)) =
+              f32x4_t{acc[a][b][4 * j], acc[a][b][4 * j + 1], acc[a][b][4 * j + 2], acc[a][b][4 * j + 3]} + bias;
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      const int64_t f = fw + 32 * a + 4 * (lane & 7);
 #pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if (f + e < g.Q) o[e] = v[e];
-            }
+      for (int i = 0; i < 4 * T; ++i) {
+        const int r = 8 * i + (lane >> 3);
+        const f32x4_t v = *reinterpret_cast<const f32x4_t*>(stage + r * S::PITCH + 16 * (lane & 7));
+        if (tw + r < g.P) {
+          float* o = out + (tw + r) * g.ldc + f;
+          if (wide && f + 4 <= g.Q) {
+            *reinterpret_cast<f32x4_t*>(o) = v;
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (f + e < g.Q) o[e] = v[e];
           }
         }
       }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
     return;
   }
-  // 16-bit outputs through LDS, so that a token's features leave as 16-byte
-  // stores of whole lines (straight from the tiles they are 16-byte pieces)
-  char* const stage = ring + wave * 32 * T * S::PITCH;
   const bool bf = g.c_type == MI355Q_BF16;
 #pragma unroll
   for (int a = 0; a < A; ++a)
