@@ -117,6 +117,22 @@ class _Weight(torch.nn.Module):
             self.register_buffer("weight", codes)
             self.register_buffer("weight_scale", scales)
 
+    @classmethod
+    def from_codes(cls, codes: torch.Tensor, scales: torch.Tensor) -> "_Weight":
+        if codes.dim() != 2 or codes.dtype != torch.float8_e4m3fn:
+            raise ValueError(f"codes must be a float8_e4m3fn matrix, got {tuple(codes.shape)} {codes.dtype}")
+        want = tuple(-(-n // ops.FP8_GROUP) for n in codes.shape)
+        if tuple(scales.shape) != want or scales.dtype not in _TYPES:
+            raise ValueError(f"codes of {tuple(codes.shape)} take bf16, fp16 or fp32 scales of {want}, got "
+                             f"{tuple(scales.shape)} {scales.dtype}")
+        self = cls.__new__(cls)
+        torch.nn.Module.__init__(self)
+        self.shape = tuple(codes.shape)
+        self.register_parameter("master", None)
+        self.register_buffer("weight", codes.detach().clone(memory_format=torch.contiguous_format))
+        self.register_buffer("weight_scale", scales.detach().to(torch.float32, copy=True))
+        return self
+
     def _apply(self, fn, *args, **kwargs):
         # module.to(dtype) would turn codes into numbers of that type: the format
         # keeps its types and moves only between devices
@@ -143,8 +159,11 @@ class Fp8BlockLinear(torch.nn.Module):
 
     def __init__(self, weight: torch.Tensor, bias: torch.Tensor | None = None, trainable: bool = False):
         super().__init__()
-        self.linear = _Weight(weight, trainable)
-        self.out_features, self.in_features = self.linear.shape
+        self._build(_Weight(weight, trainable), bias, trainable)
+
+    def _build(self, linear: _Weight, bias: torch.Tensor | None, trainable: bool) -> None:
+        self.linear = linear
+        self.out_features, self.in_features = linear.shape
         if bias is not None and tuple(bias.shape) != (self.out_features,):
             raise ValueError(f"bias must be [{self.out_features}], got {tuple(bias.shape)}")
         self.bias = None if bias is None else torch.nn.Parameter(bias.detach().clone(), requires_grad=trainable)
@@ -152,6 +171,16 @@ class Fp8BlockLinear(torch.nn.Module):
     @classmethod
     def from_linear(cls, linear: torch.nn.Linear, trainable: bool = False) -> "Fp8BlockLinear":
         return cls(linear.weight, linear.bias, trainable)
+
+    @classmethod
+    def from_compressed(cls, weight: torch.Tensor, weight_scale: torch.Tensor,
+                        bias: torch.Tensor | None = None) -> "Fp8BlockLinear":
+        """From a checkpoint's codes [out, in] and scales (one per 128 x 128
+        block; bf16 and fp16 ones are widened, which is exact), frozen."""
+        self = cls.__new__(cls)
+        torch.nn.Module.__init__(self)
+        self._build(_Weight.from_codes(weight, weight_scale), bias, False)
+        return self
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         rows = _rows(x, self.in_features, "input")

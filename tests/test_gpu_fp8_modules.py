@@ -205,3 +205,29 @@ def test_what_is_kept_follows_the_gradients_asked_for(dev, frozen):
     want = dict(none=(hidden + 3 * inter, hidden), input=(hidden + 3 * inter, hidden), weights=(2 * inter, 0),
                 gate_up=(3 * inter, 0), down=(hidden + 2 * inter, hidden))[frozen]
     assert tuple(sizes) == want
+
+
+@pytest.mark.parametrize("scale_dtype", [torch.float32, torch.bfloat16])
+def test_from_compressed(dev, scale_dtype):
+    """A checkpoint's codes and scales as a layer: its own weight's results, frozen, and it moves and saves as others do."""
+    m, ops = amd(), amd().fp8_block.ops
+    w, b = randn(dev, 1, 200, 333).to(torch.bfloat16), randn(dev, 2, 200).to(torch.bfloat16)
+    codes, scales = ops.fp8_quantize_blocks(w)
+    scales = scales.to(scale_dtype)
+    layer = m.Fp8BlockLinear.from_compressed(codes, scales, b)
+    x = randn(dev, 3, 5, 333).to(torch.bfloat16).requires_grad_()
+    y = layer(x)
+    xc, xs = ops.fp8_quantize_groups(x.detach(), E8M0)
+    same(y.detach(), ops.fp8_block_matmul(xc, xs, codes, scales.float(), b))
+    y.backward(torch.ones_like(y))
+    same(x.grad, ops.fp8_block_grad_input(torch.ones_like(y), codes, scales.float()))
+    assert not any(p.requires_grad for p in layer.parameters())
+    other = m.Fp8BlockLinear(torch.zeros_like(w), torch.zeros_like(b))
+    other.load_state_dict(layer.state_dict())
+    with torch.no_grad():
+        same(layer(x), other(x))
+    assert layer.to(torch.float16).linear.weight_scale.dtype == torch.float32
+    with pytest.raises(ValueError, match="float8_e4m3fn"):
+        m.Fp8BlockLinear.from_compressed(w, scales)
+    with pytest.raises(ValueError, match=r"\(2, 3\)"):
+        m.Fp8BlockLinear.from_compressed(codes, scales[:1])
