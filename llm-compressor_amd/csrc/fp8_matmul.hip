@@ -306,7 +306,6 @@ __device__ __forceinline__ void store_tiles(const ProductArgs& g, f32x16_t (&acc
   if (g.c_type == MI355Q_F32) {   // one column of tiles at a time
     static_assert(S::PITCH >= 144, "32 fp32 columns and a shift of the banks");
     float* const out = static_cast<float*>(g.c);
-    const bool wide = g.ldc % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
 #pragma unroll
     for (int a = 0; a < A; ++a) {
 #pragma unroll
@@ -325,8 +324,8 @@ __device__ __forceinline__ void store_tiles(const ProductArgs& g, f32x16_t (&acc
         const f32x4_t v = *reinterpret_cast<const f32x4_t*>(stage + r * S::PITCH + 16 * (lane & 7));
         if (tw + r < g.P) {
           float* o = out + (tw + r) * g.ldc + f;
-          if (wide && f + 4 <= g.Q) {
-            *reinterpret_cast<f32x4_t*>(o) = v;
+          if (f + 4 <= g.Q) {
+            __builtin_memcpy(o, &v, 16);   // (unaligned in rows of odd widths)
           } else {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
@@ -366,7 +365,6 @@ __device__ __forceinline__ void store_tiles(const ProductArgs& g, f32x16_t (&acc
   __syncthreads();
   constexpr int LPR = 4 * A, RPI = 64 / LPR;   // lanes per row, rows per pass
   uint16_t* const out = static_cast<uint16_t*>(g.c);
-  const bool wide = g.ldc % 8 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
   const int64_t f = fw + 8 * (lane % LPR);
 #pragma unroll
   for (int i = 0; i < 32 * T / RPI; ++i) {
@@ -374,8 +372,8 @@ __device__ __forceinline__ void store_tiles(const ProductArgs& g, f32x16_t (&acc
     const u32x4_t v = *reinterpret_cast<const u32x4_t*>(stage + r * S::PITCH + 16 * (lane % LPR));
     if (tw + r < g.P) {
       uint16_t* o = out + (tw + r) * g.ldc + f;
-      if (wide && f + 8 <= g.Q) {
-        *reinterpret_cast<u32x4_t*>(o) = v;
+      if (f + 8 <= g.Q) {
+        __builtin_memcpy(o, &v, 16);
       } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
@@ -1120,7 +1118,6 @@ void fp8_grad_weight_kernel(ProductArgs g, TileOrder order, int stages_per_split
   char* const stage_out = ring + wave * 32 * S::PITCH;
   const int es = f32 ? 4 : 2;
   char* const out = static_cast<char*>(g.c);
-  const bool wide = (g.ldc * es) % 16 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
 #pragma unroll
   for (int y = 0; y < NB2; ++y) {
 #pragma unroll
@@ -1146,8 +1143,8 @@ void fp8_grad_weight_kernel(ProductArgs g, TileOrder order, int stages_per_split
       const u32x4_t v = *reinterpret_cast<const u32x4_t*>(stage_out + r * S::PITCH + 16 * (lane % lpr));
       if (nw + r >= g.P) break;
       char* o = out + ((nw + r) * g.ldc + k) * es;
-      if (wide && k + per <= g.Q) {
-        *reinterpret_cast<u32x4_t*>(o) = v;
+      if (k + per <= g.Q) {
+        __builtin_memcpy(o, &v, 16);   // (unaligned in rows of odd widths)
       } else if (f32) {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
@@ -1210,8 +1207,8 @@ __global__ __launch_bounds__(256) void sum_splits_kernel(ProductArgs g, TileOrde
   const int64_t c = r * g.ldc + q;
   if (g.c_type == MI355Q_F32) {
     float* d = static_cast<float*>(g.c) + c;
-    if (whole && g.ldc % 4 == 0 && (reinterpret_cast<uintptr_t>(g.c) & 15) == 0) {
-      *reinterpret_cast<f32x4_t*>(d) = v;
+    if (whole) {
+      __builtin_memcpy(d, &v, 16);
     } else {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
@@ -1223,8 +1220,8 @@ __global__ __launch_bounds__(256) void sum_splits_kernel(ProductArgs g, TileOrde
 #pragma unroll
   for (int e = 0; e < 4; ++e) h[e] = g.c_type == MI355Q_BF16 ? Bf16::store(v[e]) : F16::store(v[e]);
   uint16_t* d = static_cast<uint16_t*>(g.c) + c;
-  if (whole && g.ldc % 4 == 0 && (reinterpret_cast<uintptr_t>(g.c) & 7) == 0) {
-    *reinterpret_cast<i32x2_t*>(d) = i32x2_t{(int)(h[0] | (uint32_t)h[1] << 16), (int)(h[2] | (uint32_t)h[3] << 16)};
+  if (whole) {
+    __builtin_memcpy(d, h, 8);
   } else {
 #pragma unroll
     for (int e = 0; e < 4; ++e)
