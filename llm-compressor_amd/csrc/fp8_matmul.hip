@@ -1585,11 +1585,12 @@ struct Padding {
   }
 };
 
-// Odd widths and a sum of one step: the element loads of one launch cost less than
-// copies of both operands (2102 x 80 x 69 9 us against 16; with three steps 300 x 513 x 515
-// 44 against 14), unless the output is large.
+// Odd widths and a sum of one step: the element loads of one launch cost less than a
+// launch for copies of both operands while every workgroup has a CU to itself
+// (2102 x 80 x 69 9 us against 12, 1000 x 1000 x 69 in 256 workgroups 9 against 12; input
+// gradient of 2000 x 99 x 1000 in 512 16 against 10; with three steps 300 x 513 x 515 44 against 14).
 static bool short_sum(int64_t rows, int64_t cols, int64_t sum) {
-  return sum <= kGroup && ((rows + GT - 1) / GT) * ((cols + GT - 1) / GT) <= 1024;
+  return sum <= kGroup && ((rows + GT - 1) / GT) * ((cols + GT - 1) / GT) <= 256;
 }
 // row offsets within a tile and a stage in 32 bits
 static bool small_pitch(int64_t ld) { return ld < (int64_t(1) << 22); }
