@@ -276,6 +276,38 @@ __device__ __forceinline__ void store_part(float* slot, int tile, const f32x16_t
   for (int j = 0; j < 4; ++j) out[64 * j] = f32x4_t{v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]};
 }
 
+// Four neighbouring columns of a row to LDS in the output's type, and 16 bytes of a
+// row from there to the output, `left` columns before the row's end (unaligned in
+// rows of odd widths).
+template <class O>
+__device__ __forceinline__ void stage_columns(char* o, const f32x4_t& v) {
+  typedef __bf16 bf16x4_t __attribute__((ext_vector_type(4)));
+  typedef _Float16 f16x4_t __attribute__((ext_vector_type(4)));
+  if constexpr (O::code == MI355Q_F32) *reinterpret_cast<f32x4_t*>(o) = v;
+  else if constexpr (O::code == MI355Q_BF16) *reinterpret_cast<bf16x4_t*>(o) = __builtin_convertvector(v, bf16x4_t);
+  else *reinterpret_cast<f16x4_t*>(o) = __builtin_convertvector(v, f16x4_t);
+}
+template <class O>
+__device__ __forceinline__ void store_piece(char* o, const u32x4_t& v, int64_t left) {
+  constexpr int PER = 16 / sizeof(typename O::raw);
+  if (left >= PER) {
+    __builtin_memcpy(o, &v, 16);
+  } else {
+    typename O::raw e[PER];
+    __builtin_memcpy(e, &v, 16);
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (i < left) reinterpret_cast<typename O::raw*>(o)[i] = e[i];
+  }
+}
+// f(Bf16{} / F16{} / F32{}): the type is told apart once, not at every column
+template <class Fn>
+__device__ __forceinline__ void by_output_type(int type, Fn&& f) {
+  if (type == MI355Q_BF16) f(Bf16{});
+  else if (type == MI355Q_F16) f(F16{});
+  else f(F32{});
+}
+
 // Stores a workgroup's tiles acc[A][T] of C [P][Q] (P on the lanes), laid out as
 // above.
 template <class S, int T, int A>
@@ -301,86 +333,42 @@ __device__ __forceinline__ void store_tiles(const ProductArgs& g, f32x16_t (&acc
   const float* const bw = biases + wf * A * 32 + 4 * (lane >> 5);
   // Outputs go through LDS (the wave's own part of it), so that a token's features
   // leave as 16-byte stores of whole lines; straight from the tiles they are pieces of
-  // 16 or 32 bytes.
+  // 16 or 32 bytes.  A pass of 128 bytes a row: 16-bit types two columns of tiles,
+  // fp32 one.  With the type told apart here 128 x 128 tiles take @@ us to store, with
+  // a choice at each column 2.4.
   char* const stage = ring + wave * 32 * T * S::PITCH;
-  if (g.c_type == MI355Q_F32) {   // one column of tiles at a time
-    static_assert(S::PITCH >= 144, "32 fp32 columns and a shift of the banks");
-    float* const out = static_cast<float*>(g.c);
+  by_output_type(g.c_type, [&](auto type) __attribute__((always_inline)) {
+    using O = decltype(type);
+    constexpr int ES = sizeof(typename O::raw), GROUP = ES == 4 ? 1 : A, PER = 16 / ES;
+    constexpr int LPR = 32 * GROUP / PER, RPI = 64 / LPR, N = 32 * T / RPI;   // lanes per row, rows per pass, passes
+    static_assert(A % GROUP == 0 && S::PITCH >= 32 * GROUP * ES + 16, "rows and a shift of the banks");
 #pragma unroll
-    for (int a = 0; a < A; ++a) {
+    for (int a0 = 0; a0 < A; a0 += GROUP) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const f32x4_t bias = *reinterpret_cast<const f32x4_t*>(bw + 32 * a + 8 * j);
+      for (int a = a0; a < a0 + GROUP; ++a)
 #pragma unroll
-        for (int b = 0; b < T; ++b)
-          *reinterpret_cast<f32x4_t*>(stage + (32 * b + (lane & 31)) * S::PITCH + 32 * j + 16 * (lane >> 5)) =
-              f32x4_t{acc[a][b][4 * j], acc[a][b][4 * j + 1], acc[a][b][4 * j + 2], acc[a][b][4 * j + 3]} + bias;
+        for (int j = 0; j < 4; ++j) {
+          const f32x4_t bias = *reinterpret_cast<const f32x4_t*>(bw + 32 * a + 8 * j);
+#pragma unroll
+          for (int b = 0; b < T; ++b)
+            stage_columns<O>(stage + (32 * b + (lane & 31)) * S::PITCH + (32 * (a - a0) + 8 * j + 4 * (lane >> 5)) * ES,
+                             f32x4_t{acc[a][b][4 * j], acc[a][b][4 * j + 1], acc[a][b][4 * j + 2],
+                                     acc[a][b][4 * j + 3]} + bias);
+        }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      u32x4_t v[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        v[i] = *reinterpret_cast<const u32x4_t*>(stage + (i * RPI + lane / LPR) * S::PITCH + 16 * (lane % LPR));
+      const int64_t f = fw + 32 * a0 + PER * (lane % LPR);
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int64_t t = tw + i * RPI + lane / LPR;
+        if (t < g.P) store_piece<O>(static_cast<char*>(g.c) + (t * g.ldc + f) * ES, v[i], g.Q - f);
       }
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      const int64_t f = fw + 32 * a + 4 * (lane & 7);
-#pragma unroll
-      for (int i = 0; i < 4 * T; ++i) {
-        const int r = 8 * i + (lane >> 3);
-        const f32x4_t v = *reinterpret_cast<const f32x4_t*>(stage + r * S::PITCH + 16 * (lane & 7));
-        if (tw + r < g.P) {
-          float* o = out + (tw + r) * g.ldc + f;
-          if (f + 4 <= g.Q) {
-            __builtin_memcpy(o, &v, 16);   // (unaligned in rows of odd widths)
-          } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (f + e < g.Q) o[e] = v[e];
-          }
-        }
-      }
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
-    return;
-  }
-  const bool bf = g.c_type == MI355Q_BF16;
-#pragma unroll
-  for (int a = 0; a < A; ++a)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const f32x4_t bias = *reinterpret_cast<const f32x4_t*>(bw + 32 * a + 8 * j);
-#pragma unroll
-      for (int b = 0; b < T; ++b) {
-        float v[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = acc[a][b][4 * j + e] + bias[e];
-        uint32_t lo, hi;
-        if (bf) {
-          lo = Bf16::store(v[0]) | (uint32_t)Bf16::store(v[1]) << 16;
-          hi = Bf16::store(v[2]) | (uint32_t)Bf16::store(v[3]) << 16;
-        } else {
-          lo = F16::store(v[0]) | (uint32_t)F16::store(v[1]) << 16;
-          hi = F16::store(v[2]) | (uint32_t)F16::store(v[3]) << 16;
-        }
-        uint32_t* o = reinterpret_cast<uint32_t*>(stage + (32 * b + (lane & 31)) * S::PITCH + 64 * a + 16 * j +
-                                                  8 * (lane >> 5));
-        o[0] = lo;
-        o[1] = hi;
-      }
-    }
-  __syncthreads();
-  constexpr int LPR = 4 * A, RPI = 64 / LPR;   // lanes per row, rows per pass
-  uint16_t* const out = static_cast<uint16_t*>(g.c);
-  const int64_t f = fw + 8 * (lane % LPR);
-#pragma unroll
-  for (int i = 0; i < 32 * T / RPI; ++i) {
-    const int r = i * RPI + lane / LPR;
-    const u32x4_t v = *reinterpret_cast<const u32x4_t*>(stage + r * S::PITCH + 16 * (lane % LPR));
-    if (tw + r < g.P) {
-      uint16_t* o = out + (tw + r) * g.ldc + f;
-      if (f + 8 <= g.Q) {
-        __builtin_memcpy(o, &v, 16);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (f + e < g.Q) o[e] = (uint16_t)(v[e >> 1] >> (16 * (e & 1)));
-      }
-    }
-  }
+  });
 }
 
 template <int T, int A, int WT, int WF, bool E8M0>
@@ -883,6 +871,36 @@ struct GradWeightShape {
   static_assert(SM * FK == NTH * 16, "one 16-byte chunk of codes per thread and stage");
 };
 
+// A wave's tiles through LDS, one row of them at a time: lane l holds column n l & 31
+// and four consecutive k a register quad; rows of 32 MB k leave as whole lines.
+template <class O, int MB, int NB2, int PITCH>
+__device__ __forceinline__ void store_weight_rows(const ProductArgs& g, f32x16_t (&acc)[MB][NB2], char* stage, int64_t nw,
+                                                  int64_t kw, int lane) {
+  constexpr int ES = sizeof(typename O::raw), PER = 16 / ES;
+  constexpr int LPR = 32 * MB / PER, RPI = 64 / LPR, N = 32 / RPI;   // lanes per row, rows per pass, passes
+  const int64_t k = kw + PER * (lane % LPR);
+#pragma unroll
+  for (int y = 0; y < NB2; ++y) {
+#pragma unroll
+    for (int x = 0; x < MB; ++x)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        stage_columns<O>(stage + (lane & 31) * PITCH + (32 * x + 8 * j + 4 * (lane >> 5)) * ES,
+                         f32x4_t{acc[x][y][4 * j], acc[x][y][4 * j + 1], acc[x][y][4 * j + 2], acc[x][y][4 * j + 3]});
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the wave's own region
+    u32x4_t v[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      v[i] = *reinterpret_cast<const u32x4_t*>(stage + (i * RPI + lane / LPR) * PITCH + 16 * (lane % LPR));
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int64_t n = nw + y * 32 + i * RPI + lane / LPR;
+      if (n < g.P) store_piece<O>(static_cast<char*>(g.c) + (n * g.ldc + k) * ES, v[i], g.Q - k);
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  }
+}
+
 template <int MB, int NB2, int WK, int WN>
 __global__ __launch_bounds__(64 * WK * WN) __attribute__((amdgpu_waves_per_eu(2)))
 void fp8_grad_weight_kernel(ProductArgs g, TileOrder order, int stages_per_split, float* parts) {
@@ -1111,52 +1129,12 @@ void fp8_grad_weight_kernel(ProductArgs g, TileOrder order, int stages_per_split
       }
     return;
   }
-  // One row of tiles at a time through LDS: lane l holds column n l & 31 and four
-  // consecutive k a register quad; rows of 32 MB k leave as whole lines.
   __syncthreads();
-  const bool f32 = g.c_type == MI355Q_F32;
   char* const stage_out = ring + wave * 32 * S::PITCH;
-  const int es = f32 ? 4 : 2;
-  char* const out = static_cast<char*>(g.c);
-#pragma unroll
-  for (int y = 0; y < NB2; ++y) {
-#pragma unroll
-    for (int x = 0; x < MB; ++x)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const f32x4_t v = {acc[x][y][4 * j], acc[x][y][4 * j + 1], acc[x][y][4 * j + 2], acc[x][y][4 * j + 3]};
-        char* o = stage_out + (lane & 31) * S::PITCH + (32 * x + 8 * j + 4 * (lane >> 5)) * es;
-        if (f32) {
-          *reinterpret_cast<f32x4_t*>(o) = v;
-        } else if (g.c_type == MI355Q_BF16) {
-          reinterpret_cast<uint32_t*>(o)[0] = Bf16::store(v[0]) | (uint32_t)Bf16::store(v[1]) << 16;
-          reinterpret_cast<uint32_t*>(o)[1] = Bf16::store(v[2]) | (uint32_t)Bf16::store(v[3]) << 16;
-        } else {
-          reinterpret_cast<uint32_t*>(o)[0] = F16::store(v[0]) | (uint32_t)F16::store(v[1]) << 16;
-          reinterpret_cast<uint32_t*>(o)[1] = F16::store(v[2]) | (uint32_t)F16::store(v[3]) << 16;
-        }
-      }
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the wave's own region
-    const int per = 16 / es, lpr = 32 * MB / per, rpi = 64 / lpr;   // elements per lane, lanes per row, rows per pass
-    const int64_t k = kw + per * (lane % lpr), nw = n0 + (wn * NB2 + y) * 32;
-    for (int r = lane / lpr; r < 32; r += rpi) {
-      const u32x4_t v = *reinterpret_cast<const u32x4_t*>(stage_out + r * S::PITCH + 16 * (lane % lpr));
-      if (nw + r >= g.P) break;
-      char* o = out + ((nw + r) * g.ldc + k) * es;
-      if (k + per <= g.Q) {
-        __builtin_memcpy(o, &v, 16);   // (unaligned in rows of odd widths)
-      } else if (f32) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (k + e < g.Q) reinterpret_cast<uint32_t*>(o)[e] = v[e];
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (k + e < g.Q) reinterpret_cast<uint16_t*>(o)[e] = (uint16_t)(v[e >> 1] >> (16 * (e & 1)));
-      }
-    }
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-  }
+  const int64_t nw = n0 + wn * NB2 * 32;
+  if (g.c_type == MI355Q_F32) store_weight_rows<F32, MB, NB2, S::PITCH>(g, acc, stage_out, nw, kw, lane);
+  else if (g.c_type == MI355Q_BF16) store_weight_rows<Bf16, MB, NB2, S::PITCH>(g, acc, stage_out, nw, kw, lane);
+  else store_weight_rows<F16, MB, NB2, S::PITCH>(g, acc, stage_out, nw, kw, lane);
 }
 
 // Sums the partial slots of the split tiles in the splits' order, adds the bias and
