@@ -276,8 +276,8 @@ __device__ __forceinline__ void store_part(float* slot, int tile, const f32x16_t
   for (int j = 0; j < 4; ++j) out[64 * j] = f32x4_t{v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]};
 }
 
-// Four neighbouring columns of a row to LDS in the output's type, and 16 bytes of a
-// row from there to the output, `left` columns before the row's end (unaligned in
+// Four neighbouring columns of a row to LDS in the output's type, and 16-byte pieces of
+// rows from there to the output, `left` columns before the rows' ends (unaligned in
 // rows of odd widths).
 template <class O>
 __device__ __forceinline__ void stage_columns(char* o, const f32x4_t& v) {
@@ -287,17 +287,28 @@ __device__ __forceinline__ void stage_columns(char* o, const f32x4_t& v) {
   else if constexpr (O::code == MI355Q_BF16) *reinterpret_cast<bf16x4_t*>(o) = __builtin_convertvector(v, bf16x4_t);
   else *reinterpret_cast<f16x4_t*>(o) = __builtin_convertvector(v, f16x4_t);
 }
-template <class O>
-__device__ __forceinline__ void store_piece(char* o, const u32x4_t& v, int64_t left) {
+// N pieces of rows `step` bytes apart, the first of row `row`.
+template <class O, int RPI, int N>
+__device__ __forceinline__ void store_pieces(char* o, int64_t step, const u32x4_t (&v)[N], int64_t row, int64_t rows,
+                                             int64_t left, bool whole) {
   constexpr int PER = 16 / sizeof(typename O::raw);
-  if (left >= PER) {
-    __builtin_memcpy(o, &v, 16);
-  } else {
-    typename O::raw e[PER];
-    __builtin_memcpy(e, &v, 16);
+  if (whole) {
 #pragma unroll
-    for (int i = 0; i < PER; ++i)
-      if (i < left) reinterpret_cast<typename O::raw*>(o)[i] = e[i];
+    for (int i = 0; i < N; ++i) __builtin_memcpy(o + i * step, &v[i], 16);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if (row + i * RPI >= rows) break;
+    if (left >= PER) {
+      __builtin_memcpy(o + i * step, &v[i], 16);
+    } else {
+      typename O::raw e[PER];
+      __builtin_memcpy(e, &v[i], 16);
+#pragma unroll
+      for (int k = 0; k < PER; ++k)
+        if (k < left) reinterpret_cast<typename O::raw*>(o + i * step)[k] = e[k];
+    }
   }
 }
 // f(Bf16{} / F16{} / F32{}): the type is told apart once, not at every column
@@ -334,8 +345,9 @@ __device__ __forceinline__ void store_tiles(const ProductArgs& g, f32x16_t (&acc
   // Outputs go through LDS (the wave's own part of it), so that a token's features
   // leave as 16-byte stores of whole lines; straight from the tiles they are pieces of
   // 16 or 32 bytes.  A pass of 128 bytes a row: 16-bit types two columns of tiles,
-  // fp32 one.  With the type told apart here 128 x 128 tiles take @@ us to store, with
-  // a choice at each column 2.4.
+  // fp32 one.  With the type told apart here, rows read before they are stored and whole
+  // tiles stored without conditions a 128 x 128 tile takes 1.5 us, with a choice at each
+  // column and row 2.4.
   char* const stage = ring + wave * 32 * T * S::PITCH;
   by_output_type(g.c_type, [&](auto type) __attribute__((always_inline)) {
     using O = decltype(type);
@@ -360,12 +372,9 @@ __device__ __forceinline__ void store_tiles(const ProductArgs& g, f32x16_t (&acc
 #pragma unroll
       for (int i = 0; i < N; ++i)
         v[i] = *reinterpret_cast<const u32x4_t*>(stage + (i * RPI + lane / LPR) * S::PITCH + 16 * (lane % LPR));
-      const int64_t f = fw + 32 * a0 + PER * (lane % LPR);
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const int64_t t = tw + i * RPI + lane / LPR;
-        if (t < g.P) store_piece<O>(static_cast<char*>(g.c) + (t * g.ldc + f) * ES, v[i], g.Q - f);
-      }
+      const int64_t f = fw + 32 * a0 + PER * (lane % LPR), t = tw + lane / LPR;
+      store_pieces<O, RPI>(static_cast<char*>(g.c) + (t * g.ldc + f) * ES, RPI * ES * g.ldc, v, t, g.P, g.Q - f,
+                           tw + 32 * T <= g.P && fw + 32 * A <= g.Q);
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
   });
@@ -892,11 +901,9 @@ __device__ __forceinline__ void store_weight_rows(const ProductArgs& g, f32x16_t
 #pragma unroll
     for (int i = 0; i < N; ++i)
       v[i] = *reinterpret_cast<const u32x4_t*>(stage + (i * RPI + lane / LPR) * PITCH + 16 * (lane % LPR));
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int64_t n = nw + y * 32 + i * RPI + lane / LPR;
-      if (n < g.P) store_piece<O>(static_cast<char*>(g.c) + (n * g.ldc + k) * ES, v[i], g.Q - k);
-    }
+    const int64_t n = nw + y * 32 + lane / LPR;
+    store_pieces<O, RPI>(static_cast<char*>(g.c) + (n * g.ldc + k) * ES, RPI * ES * g.ldc, v, n, g.P, g.Q - k,
+                         nw + 32 * NB2 <= g.P && kw + 32 * MB <= g.Q);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   }
 }
