@@ -167,10 +167,10 @@ __global__ __launch_bounds__(256) void product_any_kernel(ProductArgs g) {
 //
 // Four waves with 2 x 2 tiles each, two workgroups on a CU: one's scaling and
 // conversions run beside the other's MFMAs (one workgroup of eight waves with
-// 256 x 128 tiles 2.06 ms against 1.81, where this kernel now takes 1.71).
-// 8192 x 28672 x 4096 1.71 ms, 1.13 PFLOP/s.  Per MFMA it issues 6.3 vector
+// 256 x 128 tiles 2.06 ms against 1.81, where this kernel now takes 1.64).
+// 8192 x 28672 x 4096 1.64 ms, 1.17 PFLOP/s.  Per MFMA it issues 6.3 vector
 // instructions (4 conversions, 2 scaling FMAs); MFMAs and vector instructions are
-// busy 0.62 and 0.61 of the cycles at 1.64 GHz, down from 2.4: what bounds it is
+// busy 0.63 and 0.61 of the cycles at 1.68 GHz, down from 2.4: what bounds it is
 // power, which the conversions and the traffic from LDS share with the MFMAs.
 // (The same loads from one tile's addresses, always in L2: 3 % less.)
 typedef __attribute__((address_space(3))) void lds_void_t;
@@ -634,8 +634,8 @@ void fp8_forward_kernel(ProductArgs g, TileOrder order, int steps_per_split, flo
 //
 // 128 x 128 tiles on four waves, two workgroups on a CU (256 x 128 on eight waves
 // 1.03 .. 1.05 ms against 1.00 .. 1.02, before the steps lost their conditions).
-// 8192 x 4096 x 14336 0.91 ms, 1.06 PFLOP/s: MFMAs busy 0.60 of the cycles, vector
-// instructions 0.42, at 1.56 GHz: power again, and the LDS, which carries dY in
+// 8192 x 4096 x 14336 0.89 ms, 1.08 PFLOP/s: MFMAs busy 0.60 of the cycles, vector
+// instructions 0.40, at 1.62 GHz: power again, and the LDS, which carries dY in
 // 16 bits.  Few tiles are bound by a wave's instructions, not by what they wait
 // for: rings of five and seven steps took as long as this one of three.
 template <int T, int WT>
@@ -862,10 +862,10 @@ void fp8_grad_input_kernel(ProductArgs g, TileOrder order, int blocks_per_split,
 // to be in the operand: each wave's DMA brings codes and scale bytes of its own
 // rows, and the wave writes them to LDS as bf16, scaled by the conversion (exact).
 // The MFMAs then add straight into the accumulators: vector instructions are few
-// (busy 0.15 of the cycles), so a large tile on eight waves, 256 x 256, saves
-// LDS reads (one wave's operands serve 4 x 2 tiles).  8192 x 4096 x 14336 0.80 ms,
-// 1.21 PFLOP/s, 17 us of it the sum of the split tiles; MFMAs busy 0.65 of the cycles
-// at 1.74 GHz.  Bound by power, and by the LDS, which a stage's rows pass twice.
+// (busy 0.14 of the cycles), so a large tile on eight waves, 256 x 256, saves
+// LDS reads (one wave's operands serve 4 x 2 tiles).  8192 x 4096 x 14336 0.78 ms,
+// 1.24 PFLOP/s, 17 us of it the sum of the split tiles; MFMAs busy 0.65 of the cycles
+// at 1.76 GHz.  Bound by power, and by the LDS, which a stage's rows pass twice.
 template <int MB, int NB2, int WK, int WN>
 struct GradWeightShape {
   static constexpr int W = WK * WN, NTH = 64 * W;
@@ -1221,7 +1221,7 @@ __global__ __launch_bounds__(256) void sum_splits_kernel(ProductArgs g, TileOrde
 // tokens come from L2, and the W waves of a workgroup take every W-th step of 16 AF
 // features; their sums are joined in LDS.  Bound by the weight's bytes, so what
 // counts is loads in flight: U steps are requested before the first is used.
-// 1 x 14336 x 4096 16 us (58.7 MB, 3.7 TB/s: a launch this short ends before HBM is
+// 1 x 14336 x 4096 16 us (58.7 MB, 3.6 TB/s: a launch this short ends before HBM is
 // at its full rate; eight waves, eight steps or nontemporal loads 16 .. 19).
 typedef int i32x4_t __attribute__((ext_vector_type(4)));
 typedef int i32x8_t __attribute__((ext_vector_type(8)));
