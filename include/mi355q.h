@@ -527,8 +527,10 @@ int mi355q_quantize_int8_per_token(const void* x_dev, int64_t rows, int64_t cols
  * mi355q_fp8_quantize_groups: per row and 128 columns, a = max |x|; scale =
  * a / 448 (fp32, correctly rounded; 2^-23 where a is 0) or the least power of
  * two not below it as an e8m0 byte (1 where a is 0, 2^-126 at the least);
- * codes = e4m3fn(x / scale), round to nearest even.  A group holding an
- * infinity or a NaN becomes NaN as a whole (scale NaN / byte 255, NaN codes).
+ * codes = e4m3fn(x / scale), round to nearest even, clamped to +-448 (which only
+ * fp32 scales of a few 2^-149 need: they are rounded down by up to a third).  A group
+ * holding an infinity or a NaN becomes NaN as a whole (scale NaN / byte 255, NaN
+ * codes), no other does.
  * codes [rows, cols] (ld_codes), scales [rows, ceil(cols / 128)] (ld_scales,
  * in scales).  rows may be 0.  fp32 scales are those of the FP8_BLOCK
  * scheme's dynamic group-128 activations; with e8m0 scales from 2^-117 up

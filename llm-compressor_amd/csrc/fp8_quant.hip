@@ -4,8 +4,9 @@
 //   a = max |x| over a group (1 x 128 of an activation, 128 x 128 of a weight)
 //   s = a / 448 (fp32, correctly rounded; a = 0: fp32 epsilon), or
 //       2^ceil(log2(a / 448)) as an e8m0 byte (a = 0: 1; never below 2^-126)
-//   c = e4m3(x / s), round to nearest even; 448 is e4m3's largest value, so
-//       nothing saturates
+//   c = e4m3(x / s), round to nearest even, clamped to +-448, e4m3's largest value.
+//       Quotients pass it only where an fp32 scale is a few of fp32's smallest steps
+//       (a below 9e-42: a / 448 is rounded to whole steps there)
 // A group that holds an infinity or a NaN becomes NaN as a whole, scale and
 // codes: its largest magnitude is no number to scale by, and a silent zero
 // would hide the overflow.
@@ -116,7 +117,8 @@ __device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d) {
 // from the correctly rounded reciprocal r and one residual step (q0 = x r,
 // q = q0 + (x - q0 s) r, both steps fused), a third of a division's
 // instructions.  Scales outside [2^-100, 2^100] could lose the residual to
-// underflow and take the division.
+// underflow and take the division, and a clamp that only subnormal scales need: past
+// 464 the conversion would give NaN (NaN quotients of non-finite groups pass it).
 __device__ __forceinline__ void codes_f32(const float x[kChunk], float s, float r, uint32_t w[2]) {
   float q[kChunk];
   if (s >= 0x1p-100f && s <= 0x1p100f) {
@@ -127,7 +129,10 @@ __device__ __forceinline__ void codes_f32(const float x[kChunk], float s, float 
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < kChunk; ++i) q[i] = x[i] / s;
+    for (int i = 0; i < kChunk; ++i) {
+      const float t = x[i] / s;
+      q[i] = t > 448.f ? 448.f : t < -448.f ? -448.f : t;
+    }
   }
   w[0] = pack4(q[0], q[1], q[2], q[3]);
   w[1] = pack4(q[4], q[5], q[6], q[7]);
