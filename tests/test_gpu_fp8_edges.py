@@ -40,3 +40,43 @@ def test_blocks_whose_scale_is_a_few_smallest_steps(dev, cols):
     codes, scales = ops().fp8_quantize_blocks(x.to(dev))
     assert bool(torch.isfinite(codes.float()).all()) and bool(torch.isfinite(scales).all())
     check_codes(codes, scales, x, G, torch.float32)
+
+
+# ---------------------------------------------------------------- gated activation
+def test_silu_mul_backward_in_fp32_over_the_whole_range(dev):
+    """Every gate code under scales 2^-12 .. 2^-2 up to |gate| = 87, where the sigmoid is still a normal number.
+
+    In units of 2^-24: e^-g is within 2 (exp2's unit in the last place; what rounding its argument costs is added
+    back), 1 + e^-g and its reciprocal add 1 and 2, the correction 1: the sigmoid is within 6 of itself, and so is the
+    product dh gate s within 8 after its two roundings (2^-21).  In s (1 + gate (1 - s)) the sigmoid enters twice, gate
+    (1 - s) with an error of 6 s + 1 of |gate| at the most, and four roundings follow: 16 of s + |gate| s (2^-20)."""
+    codes = torch.arange(256, dtype=torch.uint8).view(E4M3)
+    codes = codes[torch.isfinite(codes.float())].repeat(11, 1)
+    shift = torch.arange(-12, -1)
+    gate = codes.double() * torch.exp2(shift.double())[:, None]
+    codes = torch.where(gate.abs() <= 87, codes.float(), torch.zeros(())).to(E4M3)
+    rows, cols = codes.shape
+    gate = codes.double() * torch.exp2(shift.double())[:, None]
+    groups = -(-cols // G)
+    kept = torch.cat([codes.float(), torch.ones(rows, cols)], 1).to(E4M3)
+    ks = torch.cat([(shift + 127)[:, None].repeat(1, groups), torch.full((rows, groups), 127)], 1).to(torch.uint8).view(E8M0)
+    dh = 1 + torch.rand(rows, cols, generator=gen(91))
+    got = ops().fp8_silu_mul_backward(dh.to(dev), kept.to(dev), ks.to(dev)).cpu().double()
+    d, s, rest = dh.double(), torch.sigmoid(gate), torch.sigmoid(-gate)
+    want = torch.cat([d * s * (1 + gate * rest), d * gate * s], 1)
+    tol = torch.cat([2.0 ** -20 * d * s * (1 + gate.abs()), 2.0 ** -21 * d * gate.abs() * s], 1)
+    worst = ((got - want).abs() / tol.clamp_min(1e-300)).max()
+    assert bool(((got - want).abs() <= tol).all()), f"{float(worst):.3g} of the bound"
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_silu_mul_backward_past_the_sigmoids_range(dev, dtype):
+    """Gates far past the exponent's range: the gradients of silu's ends, 0 and the identity."""
+    g = torch.tensor([-448.0, -104.0, 104.0, 448.0])
+    kept = torch.cat([g, torch.full((4,), 3.0)])[None].to(E4M3)
+    for e in (127, 127 + 100):
+        ks = torch.tensor([[e, 127]], dtype=torch.uint8).view(E8M0)
+        got = ops().fp8_silu_mul_backward(torch.ones(1, 4, dtype=dtype).to(dev), kept.to(dev), ks.to(dev)).cpu()
+        big = kept[0, :4].float() * 2.0 ** (e - 127)
+        want = torch.cat([torch.tensor([0.0, 0.0, 3.0, 3.0]), torch.where(big < 0, 0.0, big)])[None]
+        assert torch.equal(got.float(), want.to(dtype).float())
