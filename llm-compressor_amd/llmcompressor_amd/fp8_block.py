@@ -20,6 +20,7 @@ relative, beside 2^-4 of the codes it is multiplied with).
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import ops
@@ -35,6 +36,12 @@ def _rows(x: torch.Tensor, width: int, what: str) -> torch.Tensor:
     if x.dim() == 0 or x.shape[-1] != width:
         raise ValueError(f"{what} must be [..., {width}], got {tuple(x.shape)}")
     return x.reshape(-1, width)
+
+
+def _no_tangents(*tensors) -> None:
+    """Refuses operands of forward-mode differentiation: the kernels would return their results without tangents."""
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError("block-scaled fp8 layers have no forward-mode derivatives")
 
 
 def _grad_rows(dy: torch.Tensor, width: int) -> torch.Tensor:
@@ -184,8 +191,9 @@ class Fp8BlockLinear(torch.nn.Module):
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         rows = _rows(x, self.in_features, "input")
-        codes, scales = self.linear.codes()
         master, bias = self.linear.master, self.bias
+        _no_tangents(x, master, bias)
+        codes, scales = self.linear.codes()
         if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, master, bias)):
             y = _Linear.apply(rows, master, codes, scales, bias)
         else:
@@ -225,8 +233,9 @@ class Fp8GatedMLP(torch.nn.Module):
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         rows = _rows(x, self.hidden_size, "input")
-        gu, d = self.gate_up.codes(), self.down.codes()
         masters = self.gate_up.master, self.down.master
+        _no_tangents(x, *masters)
+        gu, d = self.gate_up.codes(), self.down.codes()
         if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, *masters)):
             y = _GatedMLP.apply(rows, *masters, *gu, *d)
         else:
