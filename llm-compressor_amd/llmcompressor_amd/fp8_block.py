@@ -205,6 +205,13 @@ class Fp8GatedMLP(torch.nn.Module):
     """A gated MLP ``down(silu(gate x) * (up x))`` in block-scaled fp8, gate
     and up stacked into one weight [2 intermediate, hidden].
 
+    The stacked weight is what is cut into 128 x 128 blocks.  Where the intermediate size is a
+    multiple of 128 these are the blocks of gate and of up; elsewhere one row of blocks
+    holds gate's last rows and up's first under shared scales and up's later blocks
+    are shifted, so the codes are not those of the two projections quantized apart, and
+    up to 127 rows of a projection much smaller than the other lose precision (two
+    ``Fp8BlockLinear`` keep them apart).  There is no construction from a checkpoint's codes.
+
     The activation goes from the first product to the second in fp8 without a
     pass of its own; with gradients, 8-bit codes are what the backward pass gets
     (hidden + 3 intermediate bytes per token and their scales, where bf16

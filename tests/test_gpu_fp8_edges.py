@@ -80,3 +80,21 @@ def test_silu_mul_backward_past_the_sigmoids_range(dev, dtype):
         big = kept[0, :4].float() * 2.0 ** (e - 127)
         want = torch.cat([torch.tensor([0.0, 0.0, 3.0, 3.0]), torch.where(big < 0, 0.0, big)])[None]
         assert torch.equal(got.float(), want.to(dtype).float())
+
+
+@pytest.mark.parametrize("inter", [128, 384, 200])
+def test_gated_mlp_blocks(dev, inter):
+    """Gate and up are one stacked weight.  Where the intermediate size is a multiple of 128 its blocks are those of the
+    two projections quantized apart; elsewhere one row of blocks holds rows of both under a shared scale, which a small
+    gate beside a large up pays for."""
+    from llmcompressor_amd import Fp8GatedMLP
+    o, g = ops(), gen(97, inter)
+    gate, up, down = (torch.randn(*s, generator=g).to(dev) for s in ((inter, 256), (inter, 256), (256, inter)))
+    gate = gate * 1e-3
+    codes, scales = Fp8GatedMLP(gate, up, down).gate_up.codes()
+    apart = [torch.cat(t) for t in zip(*((c.view(torch.uint8), s) for c, s in map(o.fp8_quantize_blocks, (gate, up))))]
+    check_codes(codes, scales, torch.cat([gate, up]).cpu(), G, torch.float32)
+    same = codes.shape == apart[0].shape and torch.equal(codes.view(torch.uint8), apart[0])
+    assert same == (inter % G == 0)
+    if same:
+        assert torch.equal(scales, apart[1])
