@@ -98,3 +98,25 @@ def test_gated_mlp_blocks(dev, inter):
     assert same == (inter % G == 0)
     if same:
         assert torch.equal(scales, apart[1])
+
+
+# ---------------------------------------------------------------- products
+@pytest.mark.parametrize("rows,out,cols", [(40, 8264, 256), (300, 16520, 144)])
+def test_input_gradients_over_more_than_64_blocks(dev, rows, out, cols):
+    """A wave holds the weight's scales 64 blocks at a time: sums of 65 and of 130 blocks in one item (no workspace,
+    so no split), each block's scale its own, from 2^-6 to 2^6; and as the plan splits them."""
+    from llmcompressor_amd import _lib as L
+    o, g = ops(), gen(rows, out, cols, 93)
+    w = (torch.randn(out, cols, generator=g) * 64).to(E4M3).to(dev)
+    ws = torch.exp2(12 * torch.rand(-(-out // G), -(-cols // G), generator=g) - 6).to(dev)
+    dy = heavy(g, rows, out).to(torch.bfloat16).to(dev)
+    b, d = values(w, ws), dy.cpu().double()
+    want, mags = d @ b, d.abs() @ b.abs()
+    dx = torch.full((rows, cols), math.nan, dtype=torch.bfloat16, device=dev)
+    L.check(L.lib().mi355q_fp8_block_grad_input(dy.data_ptr(), out, w.data_ptr(), cols, ws.data_ptr(), ws.shape[1],
+                                                dx.data_ptr(), cols, rows, out, cols, None, 0, L.stream_of(dy)))
+    # a block chains 8 matrix instructions of two roundings each, the blocks one each: 130 of them pass the 64
+    # roundings of the bound of check_sum, and the magnitudes are widened for that
+    wider = max(1.0, (out // G + 16) / 64)
+    check_sum(dx, want, mags * wider, torch.bfloat16)
+    check_sum(o.fp8_block_grad_input(dy, w, ws), want, mags * wider, torch.bfloat16)
