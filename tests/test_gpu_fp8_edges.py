@@ -120,3 +120,25 @@ def test_input_gradients_over_more_than_64_blocks(dev, rows, out, cols):
     wider = max(1.0, (out // G + 16) / 64)
     check_sum(dx, want, mags * wider, torch.bfloat16)
     check_sum(o.fp8_block_grad_input(dy, w, ws), want, mags * wider, torch.bfloat16)
+
+
+@pytest.mark.parametrize("rows,out,cols", [(2100, 136, 272), (8200, 264, 144), (16384, 128, 128)])
+@pytest.mark.parametrize("split", [False, True])
+def test_weight_gradients_of_many_tokens(dev, rows, out, cols, split):
+    """The sum over tokens is one chain of matrix instructions of 16 tokens each (within a part, if the plan splits
+    it): each rounds its products' sum and the accumulator's, and the parts are added one after the other, so that
+    (2 ceil(rows / 16) + 16) 2^-24 of the terms' magnitudes bounds the error."""
+    from llmcompressor_amd import _lib as L
+    o, g = ops(), torch.Generator(device=dev).manual_seed(rows)
+    x, xs = o.fp8_quantize_groups((torch.randn(rows, cols, generator=g, device=dev) * 3).to(torch.bfloat16), E8M0)
+    dy = (torch.randn(rows, out, generator=g, device=dev) + 1).to(torch.bfloat16)      # sums that grow along the chain
+    if split:
+        dw = o.fp8_block_grad_weight(dy, x, xs, torch.float32)
+    else:
+        dw = torch.full((out, cols), math.nan, device=dev)
+        L.check(L.lib().mi355q_fp8_block_grad_weight(dy.data_ptr(), out, x.data_ptr(), cols, xs.data_ptr(), xs.shape[1],
+                                                     dw.data_ptr(), L.F32, cols, rows, out, cols, None, 0,
+                                                     L.stream_of(dy)))
+    a, d = values(x, xs), dy.cpu().double()
+    tol = (2 * -(-rows // 16) + 16) * 2.0 ** -24 * (d.abs().T @ a.abs())
+    assert bool(((dw.cpu().double() - d.T @ a).abs() <= tol).all())
