@@ -1439,10 +1439,14 @@ static int launch_any(ProductArgs g, mi355q_dtype out, hipStream_t st, const cha
   MQ_CHECK_ARG(tp * tq < (int64_t(1) << 31), "%s: output too large", who);
   g.q_tiles = (uint32_t)tq;
   const dim3 grid((unsigned)(tp * tq));
-  with_dtype(out, [&](auto t) {
-    using T = decltype(t);
-    hipLaunchKernelGGL((product_any_kernel<KIND, T>), grid, dim3(256), 0, st, g);
-  });
+  if constexpr (KIND == kGradInput) {   // (bf16 outputs only)
+    hipLaunchKernelGGL((product_any_kernel<KIND, Bf16>), grid, dim3(256), 0, st, g);
+  } else {
+    with_dtype(out, [&](auto t) {
+      using T = decltype(t);
+      hipLaunchKernelGGL((product_any_kernel<KIND, T>), grid, dim3(256), 0, st, g);
+    });
+  }
   MQ_LAUNCH_CHECK();
   return MI355Q_OK;
 }

@@ -139,9 +139,9 @@ __device__ __forceinline__ void codes_f32(const float x[kChunk], float s, float 
 }
 
 // ... over a power of two: the product with 2^(127 - byte) is exact (down to
-// the fp32 subnormals, far below e4m3's smallest value)
+// the fp32 subnormals, far below e4m3's smallest value); bytes are e8m0_of's, 1 .. 247 or 255
 __device__ __forceinline__ void codes_e8m0(const float x[kChunk], uint32_t byte, uint32_t w[2]) {
-  const float r = byte == 254 ? 0x1p-127f : __uint_as_float(byte == 255 ? 0x7fc00000u : (254u - byte) << 23);
+  const float r = __uint_as_float(byte == 255 ? 0x7fc00000u : (254u - byte) << 23);
   w[0] = pack4(x[0] * r, x[1] * r, x[2] * r, x[3] * r);
   w[1] = pack4(x[4] * r, x[5] * r, x[6] * r, x[7] * r);
 }
