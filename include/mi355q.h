@@ -535,7 +535,9 @@ int mi355q_quantize_int8_per_token(const void* x_dev, int64_t rows, int64_t cols
  * in scales).  rows may be 0.  fp32 scales are those of the FP8_BLOCK
  * scheme's dynamic group-128 activations; with e8m0 scales from 2^-117 up
  * code * scale is exact in bf16, which the weight gradient relies on (values
- * below bf16's normal range may lose bits). */
+ * below bf16's normal range may lose bits; magnitudes from 248 * 2^120 up, which
+ * only groups beside fp32's and bf16's largest numbers hold, round to 2^128 and so
+ * to infinity there). */
 int mi355q_fp8_quantize_groups(const void* x_dev, mi355q_dtype dtype, int64_t rows, int64_t cols,
                                int64_t ldx, uint8_t* codes_dev, int64_t ld_codes, void* scales_dev,
                                mi355q_scale_type scale_type, int64_t ld_scales, void* stream);
@@ -555,7 +557,10 @@ int mi355q_fp8_quantize_blocks(const void* w_dev, mi355q_dtype dtype, int64_t ro
  * not split over workgroups, and operands that are not 16-byte aligned with rows
  * of whole 16-byte chunks take a slow kernel instead of a padded copy (the query
  * counts the copies where cols is no multiple of 16; operands that lie badly
- * although it is are not copied). */
+ * although it is are not copied).  Operands or activation scales whose rows lie 2^22
+ * or more elements apart take the slow kernel too (about 30 times slower on large
+ * products), above 32 rows and in the gradients; of the operands, only those of odd
+ * widths are copied. */
 size_t mi355q_fp8_block_matmul_workspace_size(int64_t rows, int64_t out, int64_t cols);
 int mi355q_fp8_block_matmul(const uint8_t* x_dev, int64_t ldx, const void* x_scales_dev,
                             mi355q_scale_type x_scale_type, int64_t ld_x_scales, const uint8_t* w_dev,

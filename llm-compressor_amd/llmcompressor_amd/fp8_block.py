@@ -4,18 +4,28 @@ training with 8-bit activation checkpoints.
 A weight is e4m3 codes with one fp32 scale per 128 x 128 block, activations are
 e4m3 codes with one scale per row and 128 columns: the FP8_BLOCK format
 (compressed-tensors' preset of that name: float 8-bit weights of strategy
-block [128, 128], dynamic group-128 activations).  Without gradients activations take fp32 scales, as the scheme
-has them.  With gradients they take powers of two (e8m0), and the same codes
-that enter the product are all that is kept of the activation for the backward
-pass: one byte per element and one per 128, where the bf16 tensor takes two.
+block [128, 128], dynamic group-128 activations).  Weights come from plain ones, which are quantized here
+(``ops.fp8_quantize_blocks``), or from a checkpoint that another tool wrote: this package's
+schemes, modifiers and save path do not write the format.
+
+Without gradients a layer's input takes fp32 scales, as the scheme has them; the
+gated MLP's inner activation has e8m0 scales in both cases.  With gradients all take
+powers of two (e8m0), and the same codes that enter the product are all that is
+kept of the activation for the backward pass: one byte per element and one per 128,
+where the bf16 tensor takes two.  (A first pass without gradients that is run again
+with them, as reentrant checkpointing does, therefore differs from the second by
+the input's quantization.)
 
 Backward formulas, for y = x W^T + b with X, W the values that the codes stand
 for (quantization itself counts as the identity):
 
     dX = dY W,  dW = dY^T X,  db = sum of dY's rows
 
-dY is read in bf16; gradients of other types are rounded to it first (2^-9
-relative, beside 2^-4 of the codes it is multiplied with).
+Gradients of activations are bf16 inside, whatever the layer's type: dY of another
+type is rounded to it first, the input gradient (and in the MLP the gradients of the inner
+activation and of gate and up) is a bf16 result, and dX is then converted to the input's type.
+Each rounding is up to 2^-8 relative, beside 2^-4 of the codes it is multiplied
+with.  Weight gradients are rounded once, to the master's type.
 """
 from __future__ import annotations
 

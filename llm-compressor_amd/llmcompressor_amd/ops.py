@@ -797,7 +797,11 @@ def fp8_block_matmul(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w
     ``fp8_quantize_groups``), w [out, cols] with float32 scales per 128 x 128
     block (``fp8_quantize_blocks``, or an FP8_BLOCK checkpoint's
     ``weight_scale`` in fp32).  Sums in fp32, rounded once to ``out_dtype``
-    (bf16, fp16 or fp32).  ``bias`` [out] is bf16, fp16 or fp32."""
+    (bf16, fp16 or fp32).  ``bias`` [out] is bf16, fp16 or fp32.
+
+    Views whose rows lie 2^22 or more elements apart, codes or x_scales, are right but
+    slow above 32 rows, and in the gradients: about 30 times on large products.  Make them
+    contiguous first."""
     x, rows, cols, x_pitch, x_scales, xs_pitch = _fp8_matrix(x, x_scales, "x", False, _FP8_SCALES)
     w, out, w_cols, w_pitch, w_scales, ws_pitch = _fp8_matrix(w, w_scales, "w", True, _FP8_F32)
     if w_cols != cols or out == 0:
