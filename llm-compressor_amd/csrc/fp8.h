@@ -57,7 +57,8 @@ inline bool known_dtype(int dt) { return dt == MI355Q_BF16 || dt == MI355Q_F16 |
 inline int dtype_size(int dt) { return dt == MI355Q_F32 ? 4 : 2; }
 inline bool aligned_to(const void* p, unsigned n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
-// n / d for n < 2^31 without a division: (mulhi(n, mul) + n) >> shift
+// n / d for n < 2^31 without a division: (mulhi(n, mul) + n) >> shift, the division by
+// an invariant divisor of Granlund and Montgomery (1994)
 struct FastDiv {
   uint32_t d, mul, shift;
 };

@@ -48,7 +48,7 @@ __device__ __forceinline__ float load_typed(const void* p, int type, int64_t i) 
 // alignment.  It runs where the tile kernels cannot (operands off 16 bytes without
 // a workspace for their copies, pitches past 32-bit offsets), where odd widths
 // have a sum of one step, and for a weight gradient of no tokens.  Bound by its
-// element loads: input gradient of 8192 x 4096 x 14336 29 ms against the tiles' 0.97.
+// element loads: input gradient of 8192 x 4096 x 14336 29 ms against the tiles' 0.9.
 constexpr int GT = 64, GPITCH = kGroup + 8;
 
 template <int KIND, class T>
@@ -155,9 +155,10 @@ __global__ __launch_bounds__(256) void product_any_kernel(ProductArgs g) {
 // 256-byte line of them), which is what a 16-byte read takes at a time.
 //
 // The fp8 matrix instructions would take the codes as they are at twice the
-// rate, but they add with few bits: on heavy-tailed codes up to 2.6e-4 of the
-// terms' magnitudes (16x16x128 and 16x16x32 alike) where the bf16 instructions
-// are within 3.2e-7.  So the codes are converted to bf16 in registers (exact,
+// rate, but they add with few bits: on heavy-tailed codes 2.9e-4 of the terms'
+// magnitudes at the most over 128 terms (16x16x128, 32x32x64, 16x16x32 and 32x32x16
+// alike), 2e-5 on normal ones, where the bf16 instructions are within 3.2e-7 and 5e-8
+// (512 random tiles each).  So the codes are converted to bf16 in registers (exact,
 // two an instruction) and the sums are fp32 sums of exact products.
 //
 // A step is, per 32 x 32 tile, eight 32x32x16 MFMAs from zero and
@@ -167,8 +168,8 @@ __global__ __launch_bounds__(256) void product_any_kernel(ProductArgs g) {
 //
 // Four waves with 2 x 2 tiles each, two workgroups on a CU: one's scaling and
 // conversions run beside the other's MFMAs (one workgroup of eight waves with
-// 256 x 128 tiles 2.06 ms against 1.81, where this kernel now takes 1.64).
-// 8192 x 28672 x 4096 1.64 ms, 1.17 PFLOP/s.  Per MFMA it issues 6.3 vector
+// 256 x 128 tiles 2.06 ms against 1.81, where this kernel now takes 1.64 on the same card).
+// 8192 x 28672 x 4096 1.64 .. 1.71 ms by the card, 1.13 .. 1.17 PFLOP/s.  Per MFMA it issues 6.3 vector
 // instructions (4 conversions, 2 scaling FMAs); MFMAs and vector instructions are
 // busy 0.63 and 0.61 of the cycles at 1.68 GHz, down from 2.4: what bounds it is
 // power, which the conversions and the traffic from LDS share with the MFMAs.
@@ -634,7 +635,7 @@ void fp8_forward_kernel(ProductArgs g, TileOrder order, int steps_per_split, flo
 //
 // 128 x 128 tiles on four waves, two workgroups on a CU (256 x 128 on eight waves
 // 1.03 .. 1.05 ms against 1.00 .. 1.02, before the steps lost their conditions).
-// 8192 x 4096 x 14336 0.89 ms, 1.08 PFLOP/s: MFMAs busy 0.60 of the cycles, vector
+// 8192 x 4096 x 14336 0.89 .. 0.91 ms by the card, 1.05 .. 1.08 PFLOP/s: MFMAs busy 0.60 of the cycles, vector
 // instructions 0.40, at 1.62 GHz: power again, and the LDS, which carries dY in
 // 16 bits.  Few tiles are bound by a wave's instructions, not by what they wait
 // for: rings of five and seven steps took as long as this one of three.
@@ -863,8 +864,8 @@ void fp8_grad_input_kernel(ProductArgs g, TileOrder order, int blocks_per_split,
 // rows, and the wave writes them to LDS as bf16, scaled by the conversion (exact).
 // The MFMAs then add straight into the accumulators: vector instructions are few
 // (busy 0.14 of the cycles), so a large tile on eight waves, 256 x 256, saves
-// LDS reads (one wave's operands serve 4 x 2 tiles).  8192 x 4096 x 14336 0.78 ms,
-// 1.24 PFLOP/s, 17 us of it the sum of the split tiles; MFMAs busy 0.65 of the cycles
+// LDS reads (one wave's operands serve 4 x 2 tiles).  8192 x 4096 x 14336 0.78 .. 0.81 ms
+// by the card, 1.19 .. 1.24 PFLOP/s, 17 us of it the sum of the split tiles; MFMAs busy 0.65 of the cycles
 // at 1.76 GHz.  Bound by power, and by the LDS, which a stage's rows pass twice.
 template <int MB, int NB2, int WK, int WN>
 struct GradWeightShape {
@@ -1219,10 +1220,11 @@ __global__ __launch_bounds__(256) void sum_splits_kernel(ProductArgs g, TileOrde
 // registers (lane l: row l & 15, 16 bytes each at 16 (l / 16) of
 // both halves of the step's 128, so that a load takes 64 bytes of 16 rows), the
 // tokens come from L2, and the W waves of a workgroup take every W-th step of 16 AF
-// features; their sums are joined in LDS.  Bound by the weight's bytes, so what
-// counts is loads in flight: U steps are requested before the first is used.
-// 1 x 14336 x 4096 16 us (58.7 MB, 3.6 TB/s: a launch this short ends before HBM is
-// at its full rate; eight waves, eight steps or nontemporal loads 16 .. 19).
+// features; their sums are joined in LDS.  What it has to move is the weight, so what
+// counts is loads in flight: U steps are requested before the first is used.  It is not
+// at HBM's rate: 1 x 14336 x 4096 takes 18 us (58.7 MB, 3.2 of 6.6 TB/s; 16 where the last-level
+// cache holds the weight).  A wave requests as many chunks of the tokens as of the
+// weight, and none while a batch of U steps is used.  (Eight steps or nontemporal loads: no faster.)
 typedef int i32x4_t __attribute__((ext_vector_type(4)));
 typedef int i32x8_t __attribute__((ext_vector_type(8)));
 
@@ -1467,7 +1469,9 @@ static void launch_few_shape(const ProductArgs& g, bool e8, bool aligned, hipStr
   }
 }
 static void launch_few(const ProductArgs& g, bool e8, bool aligned, hipStream_t st) {
-  // (one token: 4096 x 14336 16 us on eight waves, 18 on four; 14336 x 4096 18 on either)
+  // Four waves / eight, weights from HBM: one token, 4096 x 14336 16.8 / 14.0 us, 4096 x 8192 12.6 / 9.6, 14336 x 4096
+  // 18.2 / 16.1; 16 tokens 21.0 / 20.8, 14.4 / 13.9, 23.5 / 23.5, 28672 x 4096 38.2 / 42.9.  (One token would gain from
+  // eight on narrower rows too.)
   if (g.P <= 16 && g.R > 8192) launch_few_shape<1, 1, 8, 4>(g, e8, aligned, st);
   else if (g.P <= 16) launch_few_shape<1, 1, 4, 4>(g, e8, aligned, st);
   else launch_few_shape<2, 2, 8, 1>(g, e8, aligned, st);

@@ -13,11 +13,12 @@
 //
 // All kernels pass over the data once (a group never leaves the registers
 // between its maximum and its codes) and are bound by HBM.  What is read is read
-// once, so the loads are nontemporal; the stores are where a call moves more than the
+// once, so the 16-byte loads of elements are nontemporal (those of kept codes and of
+// unaligned chunks are plain); the stores are where a call moves more than the
 // last-level cache holds, and its results could not stay there for their reader
 // anyway.  Against plain accesses: gated activation of 8192 x 14336 142 -> 138 us with
 // the loads, 131 with the stores too (6.3 TB/s), its backward pass 164 -> 157 -> 149 us
-// (6.3 TB/s); 14336 x 4096 in blocks 37 -> 33 us (31 with the blocks ordered by XCD,
+// (146 by itself, 6.4 TB/s); 14336 x 4096 in blocks 37 -> 33 us (31 with the blocks ordered by XCD,
 // 5.7 TB/s); 16384 x 4096 in groups 37 -> 36 us (5.6 TB/s).
 // Rows of odd widths are moved in whole chunks too, unaligned, and by elements only
 // at their ends: 8192 x 4099 in groups 48 -> 21 us, 7392 x 10364 in blocks 135 -> 57.
