@@ -64,6 +64,9 @@ typedef enum {
 /* Scales of block-scaled fp8 activations: fp32, or e8m0 bytes 2^(b - 127). */
 typedef enum { MI355Q_SCALE_F32 = 0, MI355Q_SCALE_E8M0 = 1 } mi355q_scale_type;
 
+/* 4-bit weights as checkpoints hold them */
+typedef enum { MI355Q_W4_INT4 = 0, MI355Q_W4_MXFP4 = 1 } mi355q_w4_format;
+
 /* MXFP4 shared-exponent rule (see mi355q_mxfp4_quantize_pack). */
 typedef enum { MI355Q_MX_RULE_CT = 0, MI355Q_MX_RULE_OCP = 1 } mi355q_mx_rule;
 
@@ -606,6 +609,71 @@ int mi355q_fp8_silu_mul_backward(const void* dh_dev, mi355q_dtype dtype, int64_t
                                  int64_t ld_dh, const uint8_t* kept_codes_dev, int64_t ld_kept,
                                  const uint8_t* kept_scales_dev, int64_t ld_scales, void* dx_dev,
                                  int64_t ld_dx, void* stream);
+
+/* ------------------------------------------------------------------ tokens by expert
+ * A pair (t, k) is token t's k-th choice; ids [tokens, top] (ld_ids) are int32 or
+ * int64 (id_bits).  The plan orders the pairs by expert, then position k, then
+ * token; pairs whose id is outside [0, experts) come last:
+ *   slots [tokens, top]   the place of every pair
+ *   rows  [tokens * top]  the token at every place
+ *   offsets [experts + 1] the first place of every expert; offsets[experts] is
+ *                         where the pairs of no expert begin
+ * This is the order in which LinearExperts2D meets the tokens
+ * (modeling/moe/linear_experts.py:244-277).  At most 2040 experts
+ * (MI355Q_UNSUPPORTED beyond), fewer than 2^31 pairs.  workspace: the queried size,
+ * 4-byte aligned. */
+size_t mi355q_moe_plan_workspace_size(int64_t tokens, int64_t top, int64_t experts);
+int mi355q_moe_plan(const void* ids_dev, int id_bits, int64_t tokens, int64_t top, int64_t ld_ids, int64_t experts,
+                    int32_t* rows_dev, int32_t* slots_dev, int64_t* offsets_dev, void* workspace_dev,
+                    size_t workspace_bytes, void* stream);
+
+/* y[slots[t][k]] = x[t], zeros for places from *end_dev (offsets + experts) on.
+ * x [tokens, cols], y [tokens * top, cols] in one dtype; slots contiguous.  Places
+ * outside [0, tokens * top) are skipped, here and below. */
+int mi355q_moe_sort(const void* x_dev, mi355q_dtype dtype, int64_t tokens, int64_t top, int64_t cols, int64_t ldx,
+                    const int32_t* slots_dev, const int64_t* end_dev, void* y_dev, int64_t ldy, void* stream);
+
+/* y[t] = sum over k of weights[t][k] * x[slots[t][k]], places from *end_dev on left
+ * out; fp32 sums in the order of k, rounded once.  weights [tokens, top] contiguous,
+ * or NULL: ones (the gradient of mi355q_moe_sort). */
+int mi355q_moe_combine(const void* x_dev, mi355q_dtype dtype, int64_t tokens, int64_t top, int64_t cols, int64_t ldx,
+                       const void* weights_dev, mi355q_dtype weights_dtype, const int32_t* slots_dev,
+                       const int64_t* end_dev, void* y_dev, int64_t ldy, void* stream);
+
+/* The gradients of mi355q_moe_combine: dx[slots[t][k]] = weights[t][k] * dy[t] (zeros
+ * from *end_dev on), dweights[t][k] = the dot product of x[slots[t][k]] and dy[t] in
+ * fp32 (0 there), in weights_dtype.  dx or dweights may be NULL (x then too). */
+int mi355q_moe_combine_backward(const void* dy_dev, mi355q_dtype dtype, int64_t tokens, int64_t top, int64_t cols,
+                                int64_t lddy, const void* x_dev, int64_t ldx, const void* weights_dev,
+                                mi355q_dtype weights_dtype, const int32_t* slots_dev, const int64_t* end_dev,
+                                void* dx_dev, int64_t lddx, void* dweights_dev, void* stream);
+
+/* ------------------------------------------------------------------ 4-bit weights
+ * Products of 16-bit activations with weights as compressed checkpoints hold them.
+ * y[m][n] = bias[n] + sum over groups g of scales[n][g] *
+ *           sum_{k in g} x[m][k] * (q[n][k] - z[n][g])
+ * x [n_x, cols] and y [rows, out] row-major, x bf16 or fp16; sums in fp32, rounded
+ * once to y_dtype.  gated: the weight's rows are gate and then up (out even), and
+ * y [rows, out / 2] = silu(gate) * up, both with their bias, in fp32 before the
+ * rounding.
+ * MI355Q_W4_INT4 (pack-quantized): q = nibble k % 8 of 32-bit word k / 8 of a row, z = 8 or
+ *   nibble n % 8 of word zeros[n / 8][g]; scales [out, ceil(cols / group_size)] in
+ *   scales_dtype; group_size 32, 64, a multiple of 128, or at least cols.
+ * MI355Q_W4_MXFP4 (mxfp4-pack-quantized): e2m1 codes, even column in the low nibble,
+ *   scales are bytes e, 2^(e - 127), group_size 32, cols % 32 == 0.
+ * cols >= 8.  ldw and stride_w in bytes (multiples of 4), others in elements.
+ * offsets_dev NULL: one weight for all rows; else expert e has rows
+ * [offsets[e], offsets[e + 1]) of y and the weight at e times the strides, and rows from
+ * offsets[experts] on are written as zeros.  rows_dev: row of x behind each row of y
+ * (NULL: the same row); one that x does not have counts as zeros.
+ * A row of x that holds an infinity or a NaN may come out as NaN throughout. */
+int mi355q_w4a16_matmul(const void* x_dev, mi355q_dtype x_dtype, int64_t n_x, int64_t ldx, const int32_t* rows_dev,
+                        const int64_t* offsets_dev, int64_t experts, const void* w_dev, mi355q_w4_format format,
+                        int64_t ldw, int64_t stride_w, const void* scales_dev, mi355q_dtype scales_dtype,
+                        int64_t ld_scales, int64_t stride_scales, const uint32_t* zeros_dev, int64_t ld_zeros,
+                        int64_t stride_zeros, int64_t group_size, const void* bias_dev, mi355q_dtype bias_dtype,
+                        int gated, void* y_dev, mi355q_dtype y_dtype, int64_t ldy, int64_t rows, int64_t out,
+                        int64_t cols, void* stream);
 
 #ifdef __cplusplus
 }

@@ -17,6 +17,7 @@ BF16, F32, F16 = 0, 1, 2
 TENSOR, CHANNEL, GROUP, BLOCK, TOKEN = 0, 1, 2, 3, 4
 MX_RULE_CT, MX_RULE_OCP = 0, 1
 SCALE_F32, SCALE_E8M0 = 0, 1
+W4_INT4, W4_MXFP4 = 0, 1
 QTYPE_INT, QTYPE_FP8_E4M3, QTYPE_FP4_E2M1, QTYPE_MXFP4_CT, QTYPE_MXFP4_OCP = 0, 1, 2, 3, 4
 
 _vp, _i64, _i32, _f32, _f64, _sz = C.c_void_p, C.c_int64, C.c_int, C.c_float, C.c_double, C.c_size_t
@@ -100,6 +101,14 @@ SIGNATURES = {
                                             _sz, _vp]),
     "mi355q_fp8_silu_mul": (_i32, [_vp, _i32, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _vp]),
     "mi355q_fp8_silu_mul_backward": (_i32, [_vp, _i32, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp]),
+    "mi355q_moe_plan_workspace_size": (_sz, [_i64, _i64, _i64]),
+    "mi355q_moe_plan": (_i32, [_vp, _i32, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "mi355q_moe_sort": (_i32, [_vp, _i32, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _vp]),
+    "mi355q_moe_combine": (_i32, [_vp, _i32, _i64, _i64, _i64, _i64, _vp, _i32, _vp, _vp, _vp, _i64, _vp]),
+    "mi355q_moe_combine_backward": (_i32, [_vp, _i32, _i64, _i64, _i64, _i64, _vp, _i64, _vp, _i32, _vp, _vp, _vp, _i64,
+                                           _vp, _vp]),
+    "mi355q_w4a16_matmul": (_i32, [_vp, _i32, _i64, _i64, _vp, _vp, _i64, _vp, _i32, _i64, _i64, _vp, _i32, _i64, _i64,
+                                   _vp, _i64, _i64, _i64, _vp, _i32, _i32, _vp, _i32, _i64, _i64, _i64, _i64, _vp]),
 }
 
 _lock = threading.Lock()

@@ -15,8 +15,10 @@ from __future__ import annotations
 
 import contextlib
 import re
+from typing import NamedTuple
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import ops
 from .staging import hold, held
@@ -64,6 +66,67 @@ def route_tokens(top_k_index: torch.Tensor, num_experts: int, num_tokens: int | 
     counts = torch.bincount(top_k_index.reshape(-1).long(), minlength=num_experts)
     offsets = [0] + torch.cumsum(counts, 0).tolist()
     return sorted_tok.to(torch.int32), offsets, pos.reshape(-1)[order]
+
+
+class TokenPlan(NamedTuple):
+    """Where the (token, choice) pairs of a router's ids go when they are
+    ordered by expert, then choice, then token (``ops.moe_plan``): ``slots`` [tokens,
+    top] the place of each pair, ``rows`` [tokens * top] the token at each place,
+    ``offsets`` [experts + 1] the first place of each expert.  Pairs of no expert
+    (ids outside [0, experts): padding) are behind ``offsets[-1]``."""
+    rows: torch.Tensor
+    slots: torch.Tensor
+    offsets: torch.Tensor
+
+
+def plan_tokens(top_k_index: torch.Tensor, num_experts: int) -> TokenPlan:
+    """The plan of ``top_k_index`` [tokens, top]; on the device, nothing is waited for."""
+    return TokenPlan(*ops.moe_plan(top_k_index, num_experts))
+
+
+class _Sort(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, slots, offsets):
+        ctx.save_for_backward(slots, offsets)
+        return ops.moe_sort(x, slots, offsets)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        return ops.moe_combine(dy, None, *ctx.saved_tensors), None, None
+
+
+class _Combine(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weights, slots, offsets):
+        ctx.save_for_backward(x if ctx.needs_input_grad[1] else None, weights, slots, offsets)
+        return ops.moe_combine(x, weights, slots, offsets)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, weights, slots, offsets = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        return *ops.moe_combine_backward(dy, x, weights, slots, offsets, need[0], need[1]), None, None
+
+
+def sort_tokens(hidden_states: torch.Tensor, top_k_index: torch.Tensor, num_experts: int):
+    """Tokens [tokens, hidden] in the order of the experts that they are routed
+    to: (rows [tokens * top, hidden], the ``TokenPlan``).  Expert e owns rows
+    plan.offsets[e] .. plan.offsets[e + 1]; rows of padding (ids outside [0,
+    num_experts)) come last, as zeros.  Differentiable in ``hidden_states``: a
+    token's gradient is the sum of its rows', in fp32, rounded once."""
+    plan = plan_tokens(top_k_index, num_experts)
+    return _Sort.apply(hidden_states, plan.slots, plan.offsets), plan
+
+
+def combine_tokens(expert_out: torch.Tensor, top_k_weights: torch.Tensor, plan: TokenPlan) -> torch.Tensor:
+    """The experts' rows [tokens * top, hidden] (ordered as ``sort_tokens``
+    leaves them) back at their tokens: out[t] = sum over k of
+    top_k_weights[t, k] * expert_out[plan.slots[t, k]], fp32 sums in the order of k,
+    rounded once to expert_out's type; padding takes no part.  Differentiable in
+    both."""
+    return _Combine.apply(expert_out, top_k_weights, plan.slots, plan.offsets)
 
 
 def accumulate_expert_hessians(x: torch.Tensor, rows: torch.Tensor | None, offsets, H: torch.Tensor,

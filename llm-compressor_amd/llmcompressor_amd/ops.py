@@ -932,6 +932,278 @@ def fp8_silu_mul_backward(dh: torch.Tensor, saved: torch.Tensor, saved_scales: t
     return dx
 
 
+# ---------------------------------------------------------------- tokens by expert
+_MOE_DT = _FP8_DT
+
+
+def moe_plan(top_k_index: torch.Tensor, num_experts: int):
+    """The order of tokens by expert of ``top_k_index`` [tokens, top] (int32 or
+    int64): (rows int32 [tokens * top], slots int32 [tokens, top], offsets int64
+    [num_experts + 1]).
+
+    Pairs (token, choice) are ordered by expert, then choice, then token;
+    ``slots`` is the place of each, ``rows`` the token at each place and
+    ``offsets`` the first place of each expert.  Pairs whose id is outside [0,
+    num_experts) - padding - come last, from ``offsets[-1]`` on."""
+    L.require_gpu(top_k_index)
+    bits = {torch.int32: 32, torch.int64: 64}.get(top_k_index.dtype)
+    if bits is None:
+        raise TypeError(f"top_k_index must be int32 or int64, got {top_k_index.dtype}")
+    if top_k_index.dim() != 2 or top_k_index.shape[1] == 0:
+        raise ValueError(f"top_k_index must be [tokens, top], got {tuple(top_k_index.shape)}")
+    tokens, top = top_k_index.shape
+    ids, pitch = _rows_2d(top_k_index, top)
+    rows = ids.new_empty(tokens * top, dtype=torch.int32)
+    slots = ids.new_empty((tokens, top), dtype=torch.int32)
+    offsets = ids.new_empty(num_experts + 1 if num_experts > 0 else 1, dtype=torch.int64)
+    lib = L.lib()
+    need = lib.mi355q_moe_plan_workspace_size(tokens, top, num_experts)
+    ws = _ws(need, ids.device)
+    L.check(lib.mi355q_moe_plan(ids.data_ptr(), bits, tokens, top, pitch, num_experts, rows.data_ptr(),
+                                slots.data_ptr(), offsets.data_ptr(), L.ptr(ws), need, L.stream_of(ids)))
+    return rows, slots, offsets
+
+
+def _moe_places(slots: torch.Tensor, offsets: torch.Tensor, like: torch.Tensor):
+    """Checked slots and offsets: (slots, tokens, top, the address of offsets'
+    last entry)."""
+    if not (slots.is_cuda and offsets.is_cuda):
+        L.require_gpu(slots, offsets)
+    if slots.dtype != torch.int32 or slots.dim() != 2 or slots.shape[1] == 0:
+        raise TypeError(f"slots must be int32 [tokens, top], got {tuple(slots.shape)} {slots.dtype}")
+    if offsets.dtype != torch.int64 or offsets.dim() != 1 or offsets.shape[0] < 2:
+        raise TypeError(f"offsets must be int64 [experts + 1], got {tuple(offsets.shape)} {offsets.dtype}")
+    if slots.device != like.device or offsets.device != like.device:
+        raise _several_devices(like, slots, offsets)
+    return slots.contiguous(), *slots.shape, offsets.data_ptr() + 8 * (offsets.shape[0] - 1) * offsets.stride(0)
+
+
+def _moe_weights(weights: torch.Tensor, slots: torch.Tensor):
+    if not weights.is_cuda:
+        L.require_gpu(weights)
+    if weights.dtype not in _MOE_DT:
+        raise TypeError(f"weights must be bf16, fp16 or fp32, got {weights.dtype}")
+    if weights.shape != slots.shape:
+        raise ValueError(f"slots of {tuple(slots.shape)} take weights of the same shape, got {tuple(weights.shape)}")
+    if weights.device != slots.device:
+        raise _several_devices(slots, weights)
+    return weights.contiguous(), _MOE_DT[weights.dtype]
+
+
+def moe_sort(x: torch.Tensor, slots: torch.Tensor, offsets: torch.Tensor) -> torch.Tensor:
+    """x [tokens, cols] (bf16, fp16 or fp32) in the order of the experts:
+    out[slots[t, k]] = x[t], [tokens * top, cols]; zeros from ``offsets[-1]``
+    on."""
+    x, rows, cols, pitch, kind = _fp8_source(x, "x")
+    slots, tokens, top, end = _moe_places(slots, offsets, x)
+    if rows != tokens:
+        raise ValueError(f"slots of {tuple(slots.shape)} take x of {tokens} rows, got {rows}")
+    y = x.new_empty((tokens * top, cols))
+    L.check(L.lib().mi355q_moe_sort(x.data_ptr(), kind, tokens, top, cols, pitch, slots.data_ptr(), end, y.data_ptr(),
+                                    cols, L.stream_of(x)))
+    return y
+
+
+def moe_combine(x: torch.Tensor, weights: torch.Tensor | None, slots: torch.Tensor,
+                offsets: torch.Tensor) -> torch.Tensor:
+    """The experts' rows x [tokens * top, cols] back at their tokens: out[t] =
+    sum over k of weights[t, k] * x[slots[t, k]] (``weights`` None: ones), fp32
+    sums in the order of k, rounded once to x's type.  Places from
+    ``offsets[-1]`` on take no part, whatever x holds there."""
+    x, rows, cols, pitch, kind = _fp8_source(x, "x")
+    slots, tokens, top, end = _moe_places(slots, offsets, x)
+    if rows != tokens * top:
+        raise ValueError(f"slots of {tuple(slots.shape)} take x of {tokens * top} rows, got {rows}")
+    w_ptr, w_kind = None, 0
+    if weights is not None:
+        weights, w_kind = _moe_weights(weights, slots)
+        w_ptr = weights.data_ptr()
+    y = x.new_empty((tokens, cols))
+    L.check(L.lib().mi355q_moe_combine(x.data_ptr(), kind, tokens, top, cols, pitch, w_ptr, w_kind, slots.data_ptr(),
+                                       end, y.data_ptr(), cols, L.stream_of(x)))
+    return y
+
+
+def moe_combine_backward(dy: torch.Tensor, x: torch.Tensor | None, weights: torch.Tensor, slots: torch.Tensor,
+                         offsets: torch.Tensor, need_x: bool = True, need_weights: bool = True):
+    """The gradients of ``moe_combine`` for dy [tokens, cols]: (dx [tokens *
+    top, cols] in dy's type or None, dweights [tokens, top] in the weights'
+    type or None).  ``x`` is read for dweights only.  Zeros at places from
+    ``offsets[-1]`` on."""
+    dy, rows, cols, pitch, kind = _fp8_source(dy, "dy")
+    slots, tokens, top, end = _moe_places(slots, offsets, dy)
+    if rows != tokens:
+        raise ValueError(f"slots of {tuple(slots.shape)} take dy of {tokens} rows, got {rows}")
+    weights, w_kind = _moe_weights(weights, slots)
+    x_ptr, x_pitch = None, 0
+    if need_weights:
+        if x is None:
+            raise ValueError("the weights' gradient takes x")
+        x, n, x_cols, x_pitch, x_kind = _fp8_source(x, "x")
+        if (n, x_cols, x_kind) != (tokens * top, cols, kind):
+            raise ValueError(f"dy of {tuple(dy.shape)} {dy.dtype} takes x of {(tokens * top, cols)} in its type, got "
+                             f"{tuple(x.shape)} {x.dtype}")
+        if x.device != dy.device:
+            raise _several_devices(dy, x)
+        x_ptr = x.data_ptr()
+    dx = dy.new_empty((tokens * top, cols)) if need_x else None
+    dw = torch.empty_like(weights) if need_weights else None
+    L.check(L.lib().mi355q_moe_combine_backward(dy.data_ptr(), kind, tokens, top, cols, pitch, x_ptr, x_pitch,
+                                                weights.data_ptr(), w_kind, slots.data_ptr(), end, L.ptr(dx), cols,
+                                                L.ptr(dw), L.stream_of(dy)))
+    return dx, dw
+
+
+# ---------------------------------------------------------------- 4-bit weights
+_W4_DT = {torch.bfloat16: L.BF16, torch.float16: L.F16}
+
+
+def _w4_operand(t: torch.Tensor, shape, dtypes, what: str, lead: int):
+    """A checked part of a 4-bit weight with contiguous rows: (t, its pitch, the
+    stride of its experts); ``lead`` 1: [experts, ...]."""
+    if not t.is_cuda:
+        L.require_gpu(t)
+    if t.dtype not in dtypes:
+        raise TypeError(f"{what} must be {' or '.join(str(d) for d in dtypes)}, got {t.dtype}")
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{what} must be {tuple(shape)}, got {tuple(t.shape)}")
+    rows, cols = shape[-2], shape[-1]
+    strides = t.stride()
+    if strides[-1] != 1 and cols > 1 or strides[-2] < cols and rows > 1:
+        t = t.clone(memory_format=torch.contiguous_format)
+        strides = t.stride()
+    return t, strides[-2] if rows > 1 else cols, strides[0] if lead else 0
+
+
+def _w4_matmul(x, index, offsets, experts, n_rows, weight_packed, weight_scale, weight_zero_point, group_size, bias,
+               gated, out_dtype):
+    if not x.is_cuda:
+        L.require_gpu(x)
+    kind = _W4_DT.get(x.dtype)
+    if kind is None:
+        raise TypeError(f"x must be bf16 or fp16, got {x.dtype}")
+    if x.dim() != 2 or x.shape[1] == 0:
+        raise ValueError(f"x must be a 2-D matrix with columns, got {tuple(x.shape)}")
+    n_x, cols = x.shape
+    if cols < 8:                  # the kernels read x in chunks of 8: zeros behind it
+        if group_size is None or group_size >= cols:
+            group_size = 32       # one group
+        x, cols = torch.nn.functional.pad(x, (0, 8 - cols)), 8
+    x, pitch = _rows_2d(x, cols)
+    lead = 0 if experts is None else 1
+    if weight_packed.dim() != 2 + lead:
+        raise ValueError(f"weight_packed must be {'[experts, out, ...]' if lead else '[out, ...]'}, got "
+                         f"{tuple(weight_packed.shape)}")
+    out = weight_packed.shape[-2]
+    first = (experts,) if lead else ()
+    mx = weight_packed.dtype == torch.uint8
+    if out == 0:
+        raise ValueError("weight_packed has no rows")
+    if gated and out % 2:
+        raise ValueError(f"a gated weight holds gate and up, got {out} rows")
+    if mx:
+        if cols % 32:
+            raise ValueError(f"MXFP4 weights take whole groups of 32 columns, got {cols}")
+        if weight_zero_point is not None:
+            raise ValueError("MXFP4 weights have no zero points")
+        group, groups = 32, cols // 32
+        w, ldw, stride_w = _w4_operand(weight_packed, (*first, out, cols // 2), (torch.uint8,), "weight_packed", lead)
+        if ldw % 4 or stride_w % 4 or w.data_ptr() % 4:
+            w = w.clone(memory_format=torch.contiguous_format)
+            ldw, stride_w = cols // 2, out * (cols // 2)
+        s, lds, stride_s = _w4_operand(weight_scale, (*first, out, groups), (torch.uint8, torch.float8_e8m0fnu),
+                                       "weight_scale", lead)
+        s_kind = L.BF16
+    else:
+        group = cols if group_size is None else group_size
+        if group <= 0 or not (group in (32, 64) or group % 128 == 0 or group >= cols):
+            raise ValueError(f"group_size must be 32, 64, a multiple of 128 or all columns (None), got {group_size}")
+        groups = -(-cols // group)
+        w, ldw, stride_w = _w4_operand(weight_packed, (*first, out, -(-cols // 8)), (torch.int32,), "weight_packed",
+                                       lead)
+        ldw, stride_w = 4 * ldw, 4 * stride_w
+        s, lds, stride_s = _w4_operand(weight_scale, (*first, out, groups), tuple(_FP8_DT), "weight_scale", lead)
+        s_kind = _FP8_DT[s.dtype]
+    here, z_ptr, ldz, stride_z, b_ptr, b_kind = x.get_device(), None, 0, 0, None, 0
+    z = b = None
+    if weight_zero_point is not None:
+        z, ldz, stride_z = _w4_operand(weight_zero_point, (*first, -(-out // 8), groups), (torch.int32,),
+                                       "weight_zero_point", lead)
+        z_ptr = z.data_ptr()
+    if bias is not None:
+        if not bias.is_cuda:
+            L.require_gpu(bias)
+        b_kind = _FP8_DT.get(bias.dtype)
+        if b_kind is None:
+            raise TypeError(f"bias must be bf16, fp16 or fp32, got {bias.dtype}")
+        if bias.shape != (out,):
+            raise ValueError(f"bias must be [{out}], got {tuple(bias.shape)}")
+        b = bias.contiguous()
+        b_ptr = b.data_ptr()
+    if any(t is not None and t.get_device() != here for t in (w, s, z, b, index, offsets)):
+        raise _several_devices(x, w, s, z, b, index, offsets)
+    out_dtype = x.dtype if out_dtype is None else out_dtype
+    y_kind = _FP8_DT.get(out_dtype)
+    if y_kind is None:
+        raise TypeError(f"out_dtype must be bf16, fp16 or fp32, got {out_dtype}")
+    width = out // 2 if gated else out
+    y = x.new_empty((n_rows, width), dtype=out_dtype)
+    rc = L.lib().mi355q_w4a16_matmul(
+        x.data_ptr(), kind, n_x, pitch, None if index is None else index.data_ptr(),
+        None if offsets is None else offsets.data_ptr(), experts or 1, w.data_ptr(), L.W4_MXFP4 if mx else L.W4_INT4,
+        ldw, stride_w, s.data_ptr(), s_kind, lds, stride_s, z_ptr, ldz, stride_z, group, b_ptr, b_kind, int(gated),
+        y.data_ptr(), y_kind, width, n_rows, out, cols, L.stream_of(x))
+    if rc:
+        L.check(rc)
+    return y
+
+
+def w4a16_matmul(x: torch.Tensor, weight_packed: torch.Tensor, weight_scale: torch.Tensor,
+                 weight_zero_point: torch.Tensor | None = None, group_size: int | None = 128,
+                 bias: torch.Tensor | None = None, gated: bool = False,
+                 out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """y = x W^T (+ bias) [rows, out] of 16-bit activations x [rows, cols] (bf16
+    or fp16) and a 4-bit weight as a compressed checkpoint holds it:
+
+    * ``pack-quantized``: ``weight_packed`` int32 [out, ceil(cols / 8)],
+      ``weight_scale`` [out, ceil(cols / group_size)] in bf16, fp16 or fp32,
+      ``weight_zero_point`` int32 [ceil(out / 8), groups] or None (symmetric);
+      ``group_size`` 32, 64, a multiple of 128, or None (channel);
+    * ``mxfp4-pack-quantized``: ``weight_packed`` uint8 [out, cols / 2],
+      ``weight_scale`` uint8 (or float8_e8m0fnu) [out, cols / 32]; cols % 32 == 0.
+
+    ``gated``: the weight holds gate's rows and then up's, and y [rows, out /
+    2] = silu(gate) * up.  Sums in fp32, rounded once to ``out_dtype`` (x's
+    type, or bf16, fp16, fp32).  No gradients.  A row of x that holds an infinity may
+    come out as NaN throughout, as one with a NaN does."""
+    return _w4_matmul(x, None, None, None, x.shape[0], weight_packed, weight_scale, weight_zero_point, group_size,
+                      bias, gated, out_dtype)
+
+
+def w4a16_experts_matmul(x: torch.Tensor, rows: torch.Tensor | None, offsets: torch.Tensor,
+                         weight_packed: torch.Tensor, weight_scale: torch.Tensor,
+                         weight_zero_point: torch.Tensor | None = None, group_size: int | None = 128,
+                         gated: bool = False, out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """``w4a16_matmul`` for rows grouped by expert, with the experts' weights
+    stacked ([experts, ...] each): row i of y, offsets[e] <= i < offsets[e +
+    1], is x[rows[i]] times expert e's weight (``rows`` int32, as ``moe_plan``
+    gives them, or None: x[i]).  ``offsets`` int64 [experts + 1] stays on the
+    device: the call waits for nothing.  Rows from offsets[-1] on are zeros."""
+    if not offsets.is_cuda:
+        L.require_gpu(offsets)
+    if offsets.dtype != torch.int64 or offsets.dim() != 1 or offsets.shape[0] < 2:
+        raise TypeError(f"offsets must be int64 [experts + 1], got {tuple(offsets.shape)} {offsets.dtype}")
+    if rows is not None:
+        if not rows.is_cuda:
+            L.require_gpu(rows)
+        if rows.dtype != torch.int32 or rows.dim() != 1:
+            raise TypeError(f"rows must be int32 and 1-D, got {tuple(rows.shape)} {rows.dtype}")
+        rows = rows.contiguous()
+    return _w4_matmul(x, rows, offsets.contiguous(), offsets.shape[0] - 1,
+                      x.shape[0] if rows is None else rows.shape[0], weight_packed, weight_scale, weight_zero_point,
+                      group_size, None, gated, out_dtype)
+
+
 # ---------------------------------------------------------------- SparseGPT
 def sparsegpt_base_mask(w_work: torch.Tensor):
     """(mask uint8 [rows, cols] = w_work == 0, count int32 [1] on the device)."""
