@@ -48,4 +48,108 @@ struct W4Args {
   int gated;               // y = silu(first half) * second half
 };
 
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+
+constexpr int kStep = 128;      // columns per step
+
+__device__ __forceinline__ float load_any(const void* p, int type, int64_t i) {
+  if (type == MI355Q_F32) return static_cast<const float*>(p)[i];
+  const uint16_t v = static_cast<const uint16_t*>(p)[i];
+  return type == MI355Q_BF16 ? Bf16::load(v) : F16::load(v);
+}
+
+// ---------------------------------------------------------------- operands
+// eight nibbles of a word, lowest first, as 0 .. 15
+template <class T>
+__device__ __forceinline__ u32x4_t nibbles(uint32_t w) {
+  const uint32_t even = w & 0x0f0f0f0fu, odd = (w >> 4) & 0x0f0f0f0fu;
+  const uint32_t lo = __builtin_amdgcn_perm(odd, even, 0x05010400u), hi = __builtin_amdgcn_perm(odd, even, 0x07030602u);
+  if constexpr (T::code == MI355Q_BF16)
+    return u32x4_t{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 512.f, false)),
+                   __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 512.f, true)),
+                   __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 512.f, false)),
+                   __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 512.f, true))};
+  else
+    return u32x4_t{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 512.f, false)),
+                   __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 512.f, true)),
+                   __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 512.f, false)),
+                   __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 512.f, true))};
+}
+// eight e2m1 codes of a word, lowest first, times a power of two
+template <class T>
+__device__ __forceinline__ u32x4_t e2m1s(uint32_t w, float e) {
+  if constexpr (T::code == MI355Q_BF16)
+    return u32x4_t{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, e, 0)),
+                   __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, e, 1)),
+                   __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, e, 2)),
+                   __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, e, 3))};
+  else
+    return u32x4_t{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, e, 0)),
+                   __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, e, 1)),
+                   __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, e, 2)),
+                   __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, e, 3))};
+}
+// ---------------------------------------------------------------- tiles of rows
+// The rows [first, first + count) of y that a tile of ROWS rows holds, and their
+// expert (-1: rows behind the last expert's, which are written as zeros).
+struct RowTile {
+  int64_t first;
+  int count, expert;
+};
+// Tile `id` in the order of experts, each expert's last one shorter; a wave finds it with its lanes taking
+// E / 64 neighbouring experts each.  count = 0: there is no such tile.
+template <int ROWS>
+__device__ __forceinline__ RowTile find_row_tile(const W4Args& g, uint32_t id) {
+  if (!g.offsets) {
+    const int64_t first = (int64_t)id * ROWS, left = g.n_rows - first;
+    return {first, (int)(left < ROWS ? left : ROWS), 0};
+  }
+  const int lane = threadIdx.x & 63, per = (g.experts + 64) / 64;      // experts and the rows behind them
+  const int e0 = lane * per;
+  // (whatever the offsets hold, a tile lies within y)
+  auto begin = [&](int e) __attribute__((always_inline)) {
+    const int64_t o = e <= g.experts ? g.offsets[e] : g.n_rows;
+    return o < 0 ? 0 : o < g.n_rows ? o : g.n_rows;
+  };
+  auto size = [&](int e, int64_t& first) __attribute__((always_inline)) {
+    first = begin(e);
+    const int64_t n = begin(e + 1) - first;
+    return n > 0 ? n : 0;
+  };
+  int64_t tiles = 0, first;
+  for (int e = e0; e < e0 + per; ++e) tiles += (size(e, first) + ROWS - 1) / ROWS;
+  int64_t sum = tiles;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int64_t o = __shfl_up(sum, d);
+    if (lane >= d) sum += o;
+  }
+  const uint64_t past = __ballot(sum > (int64_t)id);
+  if (!past) return {0, 0, 0};
+  const int src = __ffsll((unsigned long long)past) - 1;
+  int64_t in = (int64_t)id - __shfl(sum - tiles, src);
+  for (int e = src * per;; ++e) {                       // sum > id: it ends inside src's experts
+    const int64_t n = size(e, first), t = (n + ROWS - 1) / ROWS;
+    if (in < t) {
+      const int64_t left = n - in * ROWS;
+      return {first + in * ROWS, (int)(left < ROWS ? left : ROWS), e < g.experts ? e : -1};
+    }
+    in -= t;
+  }
+}
+// the same in scalar registers
+template <int ROWS>
+__device__ __forceinline__ RowTile row_tile(const W4Args& g, uint32_t id) {
+  const RowTile t = find_row_tile<ROWS>(g, id);
+  const int64_t first = (int64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)t.first) |
+                        (int64_t)__builtin_amdgcn_readfirstlane((int)(t.first >> 32)) << 32;
+  return {first, __builtin_amdgcn_readfirstlane(t.count), __builtin_amdgcn_readfirstlane(t.expert)};
+}
+
+// The tile kernels (w4a16_tiles.hip): whether they take a call, the workspace that they
+// ask for, and the launch.
+bool w4_tiles_fit(const W4Args& g);
+size_t w4_tiles_workspace(int64_t n_x, int64_t cols, uint32_t groups, bool zero_points_enter);
+int launch_w4_tiles(const W4Args& g, mi355q_dtype x_dtype, int kind, void* workspace, hipStream_t st);
+
 }  // namespace mi355q

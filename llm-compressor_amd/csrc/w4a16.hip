@@ -1,22 +1,8 @@
 // Products of 16-bit activations with 4-bit weights (w4a16.h).
-#include <type_traits>
-
 #include "w4a16.h"
 
 namespace mi355q {
 
-typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
-typedef uint32_t u32x2v_t __attribute__((ext_vector_type(2)));
-
-constexpr int kStep = 128;      // columns per step
-
-__device__ __forceinline__ float load_any(const void* p, int type, int64_t i) {
-  if (type == MI355Q_F32) return static_cast<const float*>(p)[i];
-  const uint16_t v = static_cast<const uint16_t*>(p)[i];
-  return type == MI355Q_BF16 ? Bf16::load(v) : F16::load(v);
-}
-
-// ---------------------------------------------------------------- operands
 template <class T>
 __device__ __forceinline__ f32x4_t mfma(const u32x4_t& a, const u32x4_t& b, const f32x4_t& c) {
   if constexpr (T::code == MI355Q_BF16)
@@ -25,36 +11,6 @@ __device__ __forceinline__ f32x4_t mfma(const u32x4_t& a, const u32x4_t& b, cons
   else
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0,
                                                   0, 0);
-}
-// eight nibbles of a word, lowest first, as 0 .. 15
-template <class T>
-__device__ __forceinline__ u32x4_t nibbles(uint32_t w) {
-  const uint32_t even = w & 0x0f0f0f0fu, odd = (w >> 4) & 0x0f0f0f0fu;
-  const uint32_t lo = __builtin_amdgcn_perm(odd, even, 0x05010400u), hi = __builtin_amdgcn_perm(odd, even, 0x07030602u);
-  if constexpr (T::code == MI355Q_BF16)
-    return u32x4_t{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 512.f, false)),
-                   __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 512.f, true)),
-                   __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 512.f, false)),
-                   __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 512.f, true))};
-  else
-    return u32x4_t{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 512.f, false)),
-                   __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 512.f, true)),
-                   __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 512.f, false)),
-                   __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 512.f, true))};
-}
-// eight e2m1 codes of a word, lowest first, times a power of two
-template <class T>
-__device__ __forceinline__ u32x4_t e2m1s(uint32_t w, float e) {
-  if constexpr (T::code == MI355Q_BF16)
-    return u32x4_t{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, e, 0)),
-                   __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, e, 1)),
-                   __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, e, 2)),
-                   __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, e, 3))};
-  else
-    return u32x4_t{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, e, 0)),
-                   __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, e, 1)),
-                   __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, e, 2)),
-                   __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, e, 3))};
 }
 // A lane holds 16 bytes of a weight's row, the 32 columns from 32 (lane / 16) on;
 // an instruction wants 32 neighbouring columns over the four lanes of a row.  So the
@@ -80,55 +36,6 @@ __device__ __forceinline__ u32x4_t last_chunk(const uint16_t* p, int64_t left) {
   v[0] = (v[0] >> bits) | (v[1] << 1 << (63 - bits));
   v[1] >>= bits;
   return u32x4_t{(uint32_t)v[0], (uint32_t)(v[0] >> 32), (uint32_t)v[1], (uint32_t)(v[1] >> 32)};
-}
-
-// ---------------------------------------------------------------- tiles of rows
-// The rows [first, first + count) of y that a tile of ROWS rows holds, and their
-// expert (-1: rows behind the last expert's, which are written as zeros).
-struct RowTile {
-  int64_t first;
-  int count, expert;
-};
-// Tile `id` in the order of experts, each expert's last one shorter; a wave finds it with its lanes taking
-// E / 64 neighbouring experts each.  count = 0: there is no such tile.
-template <int ROWS>
-__device__ __forceinline__ RowTile row_tile(const W4Args& g, uint32_t id) {
-  if (!g.offsets) {
-    const int64_t first = (int64_t)id * ROWS, left = g.n_rows - first;
-    return {first, (int)(left < ROWS ? left : ROWS), 0};
-  }
-  const int lane = threadIdx.x & 63, per = (g.experts + 64) / 64;      // experts and the rows behind them
-  const int e0 = lane * per;
-  // (whatever the offsets hold, a tile lies within y)
-  auto begin = [&](int e) __attribute__((always_inline)) {
-    const int64_t o = e <= g.experts ? g.offsets[e] : g.n_rows;
-    return o < 0 ? 0 : o < g.n_rows ? o : g.n_rows;
-  };
-  auto size = [&](int e, int64_t& first) __attribute__((always_inline)) {
-    first = begin(e);
-    const int64_t n = begin(e + 1) - first;
-    return n > 0 ? n : 0;
-  };
-  int64_t tiles = 0, first;
-  for (int e = e0; e < e0 + per; ++e) tiles += (size(e, first) + ROWS - 1) / ROWS;
-  int64_t sum = tiles;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int64_t o = __shfl_up(sum, d);
-    if (lane >= d) sum += o;
-  }
-  const uint64_t past = __ballot(sum > (int64_t)id);
-  if (!past) return {0, 0, 0};
-  const int src = __ffsll((unsigned long long)past) - 1;
-  int64_t in = (int64_t)id - __shfl(sum - tiles, src);
-  for (int e = src * per;; ++e) {                       // sum > id: it ends inside src's experts
-    const int64_t n = size(e, first), t = (n + ROWS - 1) / ROWS;
-    if (in < t) {
-      const int64_t left = n - in * ROWS;
-      return {first + in * ROWS, (int)(left < ROWS ? left : ROWS), e < g.experts ? e : -1};
-    }
-    in -= t;
-  }
 }
 
 // ---------------------------------------------------------------- few rows
@@ -333,6 +240,9 @@ static int launch_few(const W4Args& g, hipStream_t st) {
   return MI355Q_OK;
 }
 
+// Up to this many rows (per expert, in the mean) the weight's bytes decide.
+static bool few_rows(int64_t rows, int64_t experts) { return rows <= 64 * experts; }
+
 template <class T, int KIND, int GPS>
 static int launch_kind(const W4Args& g, hipStream_t st) {
   const int64_t rows = g.offsets ? (g.n_rows + g.experts - 1) / g.experts : g.n_rows;     // per expert, in the mean
@@ -358,6 +268,13 @@ static int launch_type(const W4Args& g, int kind, hipStream_t st) {
 
 using namespace mi355q;
 
+extern "C" size_t mi355q_w4a16_matmul_workspace_size(int64_t n_x, int64_t rows, int64_t experts, int64_t out,
+                                                     int64_t cols, mi355q_w4_format format, int64_t group_size) {
+  if (n_x <= 0 || rows <= 0 || experts <= 0 || out <= 0 || cols <= 0 || group_size <= 0 || few_rows(rows, experts))
+    return 0;
+  return w4_tiles_workspace(n_x, cols, (uint32_t)((cols + group_size - 1) / group_size), format == MI355Q_W4_INT4);
+}
+
 extern "C" int mi355q_w4a16_matmul(const void* x_dev, mi355q_dtype x_dtype, int64_t n_x, int64_t ldx,
                                    const int32_t* rows_dev, const int64_t* offsets_dev, int64_t experts,
                                    const void* w_dev, mi355q_w4_format format, int64_t ldw, int64_t stride_w,
@@ -365,7 +282,8 @@ extern "C" int mi355q_w4a16_matmul(const void* x_dev, mi355q_dtype x_dtype, int6
                                    int64_t stride_scales, const uint32_t* zeros_dev, int64_t ld_zeros,
                                    int64_t stride_zeros, int64_t group_size, const void* bias_dev,
                                    mi355q_dtype bias_dtype, int gated, void* y_dev, mi355q_dtype y_dtype, int64_t ldy,
-                                   int64_t rows, int64_t out, int64_t cols, void* stream) {
+                                   int64_t rows, int64_t out, int64_t cols, void* workspace_dev,
+                                   size_t workspace_bytes, void* stream) {
   const bool mx = format == MI355Q_W4_MXFP4;
   MQ_CHECK_ARG(mx || format == MI355Q_W4_INT4, "w4a16_matmul: unknown weight format %d", (int)format);
   MQ_CHECK_ARG(x_dtype == MI355Q_BF16 || x_dtype == MI355Q_F16, "w4a16_matmul: x must be bf16 or fp16");
@@ -398,5 +316,8 @@ extern "C" int mi355q_w4a16_matmul(const void* x_dev, mi355q_dtype x_dtype, int6
               fast_div((uint32_t)(group_size < cols ? (group_size + 127) / 128 : (cols + 127) / 128)), gated != 0};
   const int kind = mx ? kMxfp4 : zeros_dev ? kInt4Zero : kInt4;
   hipStream_t st = static_cast<hipStream_t>(stream);
+  if (!few_rows(rows, experts) && w4_tiles_fit(g) && workspace_dev && aligned16(workspace_dev) &&
+      workspace_bytes >= w4_tiles_workspace(n_x, cols, g.groups, !mx))
+    return launch_w4_tiles(g, x_dtype, kind, workspace_dev, st);
   return x_dtype == MI355Q_BF16 ? launch_type<Bf16>(g, kind, st) : launch_type<F16>(g, kind, st);
 }

@@ -1,0 +1,457 @@
+// Products of 16-bit activations with 4-bit weights (w4a16.h) for many rows: tiles on
+// the matrix instructions.
+//
+// A workgroup of four waves makes 32 MTW rows by 128 NTW columns of y, each wave all of
+// the rows and 32 NTW of the columns, in steps of 128 of the sum.  A step's rows of x go
+// global -> LDS by the LDS-DMA load, in 16-byte chunks placed so that an operand read
+// takes 16 different bank groups, and are read by all four waves; a weight's codes belong to one
+// wave, so they go straight into its registers and are converted there once per step.
+//
+// Per 32 x 32 tile and group the MFMAs start from zero and acc += s * tile follows in fp32.
+// The conversions give codes 0 .. 15 (a signed one would cost more than it saves), and
+// the zero points' part of the sum,
+//   - sum_g s[n][g] z[n][g] sum_{k in g} x[m][k],
+// is a product of its own with one column per group: a first pass over x (prepare_kernel)
+// leaves the groups' sums as three bf16 numbers each (24 bits), the factors -s z are split
+// the same way, and the accumulators begin with the six products that count down to
+// 2^-24.  With 128 columns per group that is 1/43 of the MFMAs, 1/21 where s z has more bits
+// than bf16 holds.
+#include "w4a16.h"
+
+namespace mi355q {
+
+constexpr int kSlices = kStep / 16;   // MFMAs per step and tile
+constexpr int kWaves = 4;
+
+typedef __attribute__((address_space(3))) void lds_void_t;
+__device__ __forceinline__ uint32_t lds_u32(const void* p) {
+  return (uint32_t) reinterpret_cast<uintptr_t>((lds_void_t*)p);
+}
+// 64 lanes x 16 bytes to LDS at m0, from a scalar base and lane offsets; waited for explicitly (vmcnt)
+__device__ __forceinline__ void dma16(uint32_t off, const void* base, uint32_t m0) {
+  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(m0) : "memory", "m0");
+}
+
+template <class T>
+__device__ __forceinline__ f32x16_t mfma32(const u32x4_t& a, const u32x4_t& b, const f32x16_t& c) {
+  if constexpr (T::code == MI355Q_BF16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c,
+                                                   0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0,
+                                                  0, 0);
+}
+
+// v as three bf16 numbers: v - (p0 + p1 + p2) is below 2^-26 of it
+__device__ __forceinline__ void split3(float v, uint16_t (&p)[3]) {
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {
+    p[i] = f32_to_bf16_bits(v);
+    v -= bf16_bits_to_f32(p[i]);
+  }
+}
+
+// ---------------------------------------------------------------- sums of x
+// sums[m][piece][g]: the sum of x[m] over group g as three bf16 numbers, zeros behind
+// the last group; copy: x with rows of whole steps, zeros behind the last column.
+// 2^lanes lanes share a group, and a wave holds 64 >> lanes of them.
+template <class T>
+__global__ __launch_bounds__(256) void w4_prepare_kernel(const uint16_t* x, int64_t ldx, int64_t n_x, int64_t cols,
+                                                         int group, uint32_t groups, uint32_t padded, int lanes,
+                                                         uint16_t* sums, uint16_t* copy, int64_t ld_copy) {
+  const int lane = threadIdx.x & 63, sub = lane & ((1 << lanes) - 1);
+  const uint32_t per = 64u >> lanes, parts = (padded + per - 1) / per;
+  const uint64_t item = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int64_t m = (int64_t)(item / parts);
+  if (m >= n_x) return;
+  const uint32_t gi = (uint32_t)(item % parts) * per + (lane >> lanes);
+  const uint16_t* const row = x + m * ldx;
+  const int64_t k0 = (int64_t)gi * group, k1 = gi < groups ? (k0 + group < cols ? k0 + group : cols) : k0;
+  float sum = 0.f;
+  for (int64_t k = k0 + 8 * sub; k < k1; k += 8 << lanes) {
+    uint16_t v[8];
+    const int64_t left = cols - k;
+    if (left >= 8) {
+      __builtin_memcpy(v, row + k, 16);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = e < left ? row[k + e] : 0;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (k + e < k1) sum += T::load(v[e]);
+    if (copy) __builtin_memcpy(copy + m * ld_copy + k, v, 16);       // groups are whole chunks but for the last
+  }
+  for (int d = 1; d < 1 << lanes; d <<= 1) sum += __shfl_xor(sum, d);
+  if (sums && sub == 0 && gi < padded) {
+    uint16_t p[3];
+    split3(sum, p);
+#pragma unroll
+    for (int i = 0; i < 3; ++i) sums[((size_t)m * 3 + i) * padded + gi] = p[i];
+  }
+  if (copy && gi == groups - 1)
+    for (int64_t k = (cols + 7) / 8 * 8 + 8 * sub; k < ld_copy; k += 8 << lanes)
+      *reinterpret_cast<u32x4_t*>(copy + m * ld_copy + k) = u32x4_t{0u, 0u, 0u, 0u};
+}
+
+// ---------------------------------------------------------------- tiles
+struct W4Tiles {
+  const uint16_t* sums;      // [n_x][3][padded], or null: no zero points (MXFP4)
+  uint32_t padded;           // groups, a multiple of 16
+  int pieces;                // of the factors s z: 1 or 3
+  uint32_t row_tiles, col_tiles;
+};
+
+template <int MTW>
+struct TileShape {
+  static constexpr int R = 32 * MTW;                 // rows of x
+  static constexpr int SLOT = R * kStep * 2;         // bytes of a step
+  static constexpr int NI = R / 16;                  // DMA instructions per wave and step
+};
+
+template <class T, int KIND, int GPS, int MTW, int NTW>
+__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2)))
+void w4_tiles_kernel(W4Args g, W4Tiles o) {
+  using S = TileShape<MTW>;
+  constexpr int R = S::R;
+  constexpr bool FOLD = KIND == kMxfp4 && T::code == MI355Q_BF16;
+  constexpr int PER = kSlices / GPS;                 // MFMAs per group
+  __shared__ __attribute__((aligned(16))) char ring[2 * S::SLOT];
+  __shared__ int64_t x_row[R];                       // -1: a row that is not there
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int ln = lane & 31, h = lane >> 5;
+
+  // neighbouring workgroups of an XCD share rows of x, and in bands of 8 row tiles the weight
+  const uint32_t t = xcd_order(blockIdx.x, o.row_tiles * o.col_tiles);
+  const uint32_t band = t / (8 * o.col_tiles), left = o.row_tiles - 8 * band, in = t - band * 8 * o.col_tiles;
+  const uint32_t high = left < 8 ? left : 8, tc = in / high, tr = 8 * band + in - tc * high;
+  const RowTile tile = row_tile<R>(g, tr);
+  if (tile.count <= 0) return;
+  const int64_t half = g.gated ? g.out / 2 : 0, width = g.gated ? half : g.out;
+  const int per_wave = g.gated ? 16 * NTW : 32 * NTW;                 // columns of y
+  const int64_t n0 = ((int64_t)tc * kWaves + wave) * per_wave;
+  // first column of tile a of the wave
+  auto column = [&](int a) __attribute__((always_inline)) {
+    return g.gated ? (a >= NTW / 2 ? half : 0) + n0 + 32 * (a % (NTW / 2 ? NTW / 2 : 1)) : n0 + 32 * a;
+  };
+  auto store = [&](int64_t row, int64_t n, float v) __attribute__((always_inline)) {
+    const int64_t at = row * g.ldy + n;
+    if (g.y_type == MI355Q_F32) static_cast<float*>(g.y)[at] = v;
+    else static_cast<uint16_t*>(g.y)[at] = g.y_type == MI355Q_BF16 ? Bf16::store(v) : F16::store(v);
+  };
+  if (tile.expert < 0) {                                              // rows of no expert
+    for (int r = 0; r < tile.count; ++r)
+      for (int c = lane; c < per_wave; c += 64)
+        if (n0 + c < width) store(tile.first + r, n0 + c, 0.f);
+    return;
+  }
+  for (int r = threadIdx.x; r < R; r += 64 * kWaves) {
+    int64_t row = tile.first + r;
+    if (g.rows && r < tile.count) row = g.rows[row];
+    x_row[r] = r < tile.count && row >= 0 && row < g.n_x ? row : -1;
+  }
+  __syncthreads();
+
+  // DMA: instruction q of a step fills 16 rows' 64 bytes; lane l the place l & 3 of row l / 4, with the
+  // row's chunk (l & 3) ^ (row / 4 & 3).  Rows that are not there read another row (their results are
+  // not stored).
+  const int steps = (int)((g.cols + kStep - 1) / kStep);
+  const int64_t x0 = g.rows ? 0 : tile.first;
+  constexpr int NR = S::NI > 4 ? S::NI / 4 : 1;       // rows per lane
+  uint32_t xo[NR];
+  const int chunk = (lane & 3) ^ ((lane >> 4) & 3);
+#pragma unroll
+  for (int i = 0; i < NR; ++i) {
+    const int64_t row = x_row[((wave * S::NI + 4 * i) >> 2) * 16 + (lane >> 2)];
+    xo[i] = (uint32_t)((row < 0 ? x0 : row) - x0) * (uint32_t)(2 * g.ldx) + 16 * chunk;
+  }
+  const char* const xb = reinterpret_cast<const char*>(g.x + x0 * g.ldx);
+  const uint32_t l0 = lds_u32(ring);
+  const int whole = (int)(g.cols / kStep);            // steps of 128 columns
+  const int tail = (int)(g.cols % kStep + 7) / 8;     // chunks of a shorter last one (rows that end inside one are copies)
+  auto dma = [&](int s, int slot) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < S::NI; ++i) {
+      const int q = wave * S::NI + i, hi = q & 3;
+      const char* const base = xb + (int64_t)s * (2 * kStep);
+      const uint32_t m0 = l0 + slot * S::SLOT + hi * (R * 64) + (q >> 2) * 1024;
+      if (s < whole) {
+        dma16(xo[i / 4], base + 64 * hi, m0);
+      } else {
+        // chunks past the last column: the row's first one of the step, which meets zeros (offsets are
+        // unsigned: the 64 hi columns are added to them, so that taking the chunk off stays above the base)
+        dma16(xo[i / 4] + (4 * hi + chunk < tail ? 64 * hi : -16 * chunk), base, m0);
+      }
+    }
+  };
+  // operand reads: lane l has row l & 31, columns 16 j + 8 (l / 32) and on of slice j
+  const int ra[2] = {ln * 64 + 16 * (h ^ ((ln >> 2) & 3)), ln * 64 + 16 * ((2 + h) ^ ((ln >> 2) & 3))};
+  auto read_x = [&](int slot, int b, int j) __attribute__((always_inline)) {
+    return *reinterpret_cast<const u32x4_t*>(ring + slot * S::SLOT + (j >> 1) * (R * 64) + b * 2048 + ra[j & 1]);
+  };
+
+  // weights: lane l has column l & 31 of every tile, 16 bytes each at 16 (l / 32) of both halves of the step
+  uint32_t wo[NTW];
+  uint32_t so[NTW];
+#pragma unroll
+  for (int a = 0; a < NTW; ++a) {
+    const int64_t limit = g.gated && column(a) < half ? half : g.out, n = column(a) + ln;
+    const int64_t c = n < limit ? n : limit - 1;
+    wo[a] = (uint32_t)(c * g.ldw) + 16 * h;
+    so[a] = (uint32_t)(c * g.lds);
+  }
+  const uint8_t* const wb = g.w + tile.expert * g.stride_w;
+  const int64_t s_base = tile.expert * g.stride_s;
+  const int words = KIND == kMxfp4 ? (int)(g.cols / 8) : (int)((g.cols + 7) / 8);
+  struct Raw {
+    u32x4_t w[NTW][2];
+    uint32_t s[NTW][GPS];
+  };
+  auto load_w = [&](Raw& r, int s) __attribute__((always_inline)) {
+#pragma unroll
+    for (int a = 0; a < NTW; ++a) {
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        const uint8_t* const p = wb + (int64_t)s * (kStep / 2) + 32 * b + wo[a];
+        if (s < whole) {
+          __builtin_memcpy(&r.w[a][b], p, 16);
+        } else {
+          const int last = words - s * (kStep / 8) - 8 * b - 4 * h;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) r.w[a][b][i] = i < last ? reinterpret_cast<const uint32_t*>(p)[i] : 0u;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < GPS; ++i) {
+        const uint32_t gs = GPS == 1 ? div((uint32_t)s, g.per) : (uint32_t)s * GPS + i;
+        const int64_t at = s_base + so[a] + (gs < g.groups ? gs : g.groups - 1);
+        if constexpr (KIND == kMxfp4) r.s[a][i] = static_cast<const uint8_t*>(g.s)[at];
+        else if (g.s_type == MI355Q_F32) r.s[a][i] = static_cast<const uint32_t*>(g.s)[at];
+        else r.s[a][i] = static_cast<const uint16_t*>(g.s)[at];
+      }
+    }
+  };
+  auto scale_of = [&](uint32_t v) __attribute__((always_inline)) {
+    if constexpr (FOLD) return __uint_as_float((v << 23) | 0x00400000u);
+    else if constexpr (KIND == kMxfp4) return e8m0_to_f32(v);
+    else return g.s_type == MI355Q_F32 ? __uint_as_float(v)
+                : g.s_type == MI355Q_BF16 ? __uint_as_float(v << 16) : F16::load((uint16_t)v);
+  };
+
+  f32x16_t acc[MTW][NTW];
+#pragma unroll
+  for (int b = 0; b < MTW; ++b)
+#pragma unroll
+    for (int a = 0; a < NTW; ++a)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[b][a][e] = 0.f;
+
+  Raw raw;
+  dma(0, 0);
+  load_w(raw, 0);
+  if constexpr (KIND != kMxfp4) {
+    // the zero points' part: sums of x [m][g] times -s z [n][g], 16 groups at a time
+    for (uint32_t g0 = 0; g0 < o.padded; g0 += 16) {
+      u32x4_t f[NTW][3];
+#pragma unroll
+      for (int a = 0; a < NTW; ++a) {
+        uint16_t p[3][8];
+        const int64_t limit = g.gated && column(a) < half ? half : g.out, n = column(a) + ln;
+        const int64_t c = n < limit ? n : limit - 1;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const uint32_t gi = g0 + 8 * h + e;
+          float v = 0.f;
+          if (gi < g.groups) {
+            float z = 8.f;
+            if constexpr (KIND == kInt4Zero)
+              z = (float)((g.z[tile.expert * g.stride_z + c / 8 * g.ldz + gi] >> (4 * (int)(c % 8))) & 15u);
+            v = -z * load_any(g.s, g.s_type, s_base + so[a] + gi);
+          }
+          uint16_t q[3];
+          split3(v, q);
+#pragma unroll
+          for (int i = 0; i < 3; ++i) p[i][e] = q[i];
+        }
+#pragma unroll
+        for (int i = 0; i < 3; ++i) __builtin_memcpy(&f[a][i], p[i], 16);
+      }
+#pragma unroll
+      for (int b = 0; b < MTW; ++b) {
+        const int64_t row = x_row[32 * b + ln];
+        const uint16_t* const sp = o.sums + (row < 0 ? 0 : row) * 3 * o.padded + g0 + 8 * h;
+        u32x4_t v[3];
+#pragma unroll
+        for (int i = 0; i < 3; ++i) v[i] = *reinterpret_cast<const u32x4_t*>(sp + (size_t)i * o.padded);
+#pragma unroll
+        for (int a = 0; a < NTW; ++a) {
+#pragma unroll
+          for (int i = 0; i < 3; ++i) acc[b][a] = mfma32<Bf16>(v[i], f[a][0], acc[b][a]);
+          if (o.pieces > 1) {
+            acc[b][a] = mfma32<Bf16>(v[0], f[a][1], acc[b][a]);
+            acc[b][a] = mfma32<Bf16>(v[1], f[a][1], acc[b][a]);
+            acc[b][a] = mfma32<Bf16>(v[0], f[a][2], acc[b][a]);
+          }
+        }
+      }
+    }
+  }
+  for (int s = 0; s < steps; ++s) {
+    const int slot = s & 1;
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");   // the step is here, the other slot read
+    if (s + 1 < steps) dma(s + 1, slot ^ 1);
+    u32x4_t q[NTW][kSlices];
+    float sc[NTW][GPS];
+#pragma unroll
+    for (int a = 0; a < NTW; ++a) {
+#pragma unroll
+      for (int i = 0; i < GPS; ++i) sc[a][i] = scale_of(raw.s[a][i]);
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        // words 0 and 1 of both halves of the wave are slices 0 and 2, words 2 and 3 slices 1 and 3
+        const auto u = __builtin_amdgcn_permlane32_swap(raw.w[a][b][0], raw.w[a][b][1], false, false);
+        const auto v = __builtin_amdgcn_permlane32_swap(raw.w[a][b][2], raw.w[a][b][3], false, false);
+        const uint32_t w[4] = {(uint32_t)u[0], (uint32_t)v[0], (uint32_t)u[1], (uint32_t)v[1]};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int j = 4 * b + i;
+          if constexpr (KIND == kMxfp4) q[a][j] = e2m1s<T>(w[i], FOLD ? sc[a][j * GPS / kSlices] : 1.f);
+          else q[a][j] = nibbles<T>(w[i]);
+        }
+      }
+    }
+    if (s + 1 < steps) load_w(raw, s + 1);
+#pragma unroll
+    for (int b = 0; b < MTW; ++b) {
+      u32x4_t v[kSlices];
+#pragma unroll
+      for (int j = 0; j < kSlices; ++j) v[j] = read_x(slot, b, j);
+#pragma unroll
+      for (int i = 0; i < GPS; ++i)
+#pragma unroll
+        for (int a = 0; a < NTW; ++a) {
+          if constexpr (FOLD) {
+#pragma unroll
+            for (int j = 0; j < PER; ++j) acc[b][a] = mfma32<T>(v[i * PER + j], q[a][i * PER + j], acc[b][a]);
+          } else {
+            f32x16_t p = {};
+#pragma unroll
+            for (int j = 0; j < PER; ++j) p = mfma32<T>(v[i * PER + j], q[a][i * PER + j], p);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[b][a][e] = fmaf(p[e], sc[a][i], acc[b][a][e]);
+          }
+        }
+    }
+  }
+  // a lane has column l & 31 and rows 8 (e / 4) + 4 (l / 32) + e % 4
+#pragma unroll
+  for (int a = 0; a < NTW; ++a) {
+    if (g.bias) {
+      const int64_t n = column(a) + ln;
+      const float bias = n < g.out ? load_any(g.bias, g.bias_type, n) : 0.f;
+#pragma unroll
+      for (int b = 0; b < MTW; ++b)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[b][a][e] += bias;
+    }
+  }
+#pragma unroll
+  for (int b = 0; b < MTW; ++b)
+#pragma unroll
+    for (int a = 0; a < NTW; ++a) {
+      if (g.gated && (NTW == 1 || a >= NTW / 2)) continue;
+      const int64_t n = n0 + 32 * a + ln;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int r = 32 * b + 8 * (e >> 2) + 4 * h + (e & 3);
+        float v = acc[b][a][e];
+        if constexpr (NTW > 1)
+          if (g.gated) v = v / (1.f + expf(-v)) * acc[b][a + NTW / 2 < NTW ? a + NTW / 2 : 0][e];
+        if (r < tile.count && n < width) store(tile.first + r, n, x_row[r] < 0 ? 0.f : v);
+      }
+    }
+}
+
+// ---------------------------------------------------------------- launches
+bool w4_tiles_fit(const W4Args& g) {
+  // 32-bit offsets: of a tile's rows (all of x's where they are gathered), of a weight's rows and scales
+  const int64_t span = g.rows ? g.n_x : 128;
+  const int64_t limit = (int64_t)1 << 32;
+  const int64_t steps = (g.cols + kStep - 1) / kStep * kStep;
+  const int64_t pitch = g.ldx > steps ? g.ldx : steps;
+  return span < limit / (2 * pitch) && g.out < limit / g.ldw && g.out < limit / (g.lds > 0 ? g.lds : 1);
+}
+
+static bool in_place(const W4Args& g) { return aligned16(g.x) && g.ldx % 8 == 0 && g.cols % 8 == 0; }
+
+static size_t sums_bytes(int64_t n_x, uint32_t groups) {
+  return ((size_t)n_x * 3 * ((groups + 15) / 16 * 16) * sizeof(uint16_t) + 255) / 256 * 256;
+}
+
+size_t w4_tiles_workspace(int64_t n_x, int64_t cols, uint32_t groups, bool zero_points_enter) {
+  // an x that the DMA cannot read (rows off 16 bytes or of no whole chunks) is copied
+  return (zero_points_enter ? sums_bytes(n_x, groups) : 0) +
+         (size_t)n_x * ((cols + kStep - 1) / kStep * kStep) * sizeof(uint16_t);
+}
+
+template <class T, int KIND, int GPS, int MTW, int NTW>
+static int launch_shape(const W4Args& g, W4Tiles o, hipStream_t st) {
+  constexpr int R = TileShape<MTW>::R;
+  const int64_t width = g.gated ? g.out / 2 : g.out, per = kWaves * (g.gated ? 16 * NTW : 32 * NTW);
+  const int64_t ct = (width + per - 1) / per;
+  int64_t rt = (g.n_rows + R - 1) / R;
+  if (g.offsets) rt = g.n_rows / R + g.experts + 1 < g.n_rows ? g.n_rows / R + g.experts + 1 : g.n_rows;
+  MQ_CHECK_ARG(ct * rt <= (int64_t)(UINT32_MAX / 256), "w4a16_matmul: %lld rows by %lld columns are too many",
+               (long long)g.n_rows, (long long)width);
+  o.row_tiles = (uint32_t)rt;
+  o.col_tiles = (uint32_t)ct;
+  hipLaunchKernelGGL((w4_tiles_kernel<T, KIND, GPS, MTW, NTW>), dim3((unsigned)(ct * rt)), dim3(64 * kWaves), 0, st, g,
+                     o);
+  MQ_LAUNCH_CHECK();
+  return MI355Q_OK;
+}
+
+template <class T, int KIND, int GPS>
+static int launch_kind(const W4Args& g, const W4Tiles& o, hipStream_t st) {
+  return launch_shape<T, KIND, GPS, 4, 2>(g, o, st);
+}
+
+template <class T>
+static int launch_type(W4Args g, int kind, void* workspace, hipStream_t st) {
+  const bool copy = !in_place(g), sums = kind != kMxfp4;
+  const uint32_t padded = (g.groups + 15) / 16 * 16;
+  W4Tiles o = {sums ? static_cast<const uint16_t*>(workspace) : nullptr, padded,
+               kind == kInt4 && g.s_type == MI355Q_BF16 ? 1 : 3, 0, 0};
+  const int64_t ld_copy = (g.cols + kStep - 1) / kStep * kStep;
+  uint16_t* const to = copy ? reinterpret_cast<uint16_t*>(static_cast<char*>(workspace) +
+                                                          (sums ? sums_bytes(g.n_x, g.groups) : 0)) : nullptr;
+  if (copy || sums) {
+    int lanes = 0;
+    while (lanes < 6 && (8 << lanes) < g.group) ++lanes;
+    const uint64_t parts = (padded + (64u >> lanes) - 1) / (64u >> lanes), items = parts * (uint64_t)g.n_x;
+    MQ_CHECK_ARG((items + 3) / 4 <= UINT32_MAX / 256, "w4a16_matmul: %lld rows of x are too many", (long long)g.n_x);
+    hipLaunchKernelGGL((w4_prepare_kernel<T>), dim3((unsigned)((items + 3) / 4)), dim3(256), 0, st, g.x, g.ldx, g.n_x,
+                       g.cols, g.group, g.groups, padded, lanes, sums ? static_cast<uint16_t*>(workspace) : nullptr, to,
+                       ld_copy);
+    MQ_LAUNCH_CHECK();
+  }
+  if (copy) {
+    g.x = to;
+    g.ldx = ld_copy;
+  }
+  if (kind == kMxfp4) return launch_kind<T, kMxfp4, 4>(g, o, st);
+  const int gps = g.groups > 1 && g.group == 32 ? 4 : g.groups > 1 && g.group == 64 ? 2 : 1;
+  // zero points enter before the sum: both kinds take one kernel but for that
+  if (kind == kInt4)
+    return gps == 4 ? launch_kind<T, kInt4, 4>(g, o, st)
+           : gps == 2 ? launch_kind<T, kInt4, 2>(g, o, st) : launch_kind<T, kInt4, 1>(g, o, st);
+  return gps == 4 ? launch_kind<T, kInt4Zero, 4>(g, o, st)
+         : gps == 2 ? launch_kind<T, kInt4Zero, 2>(g, o, st) : launch_kind<T, kInt4Zero, 1>(g, o, st);
+}
+
+int launch_w4_tiles(const W4Args& g, mi355q_dtype x_dtype, int kind, void* workspace, hipStream_t st) {
+  return x_dtype == MI355Q_BF16 ? launch_type<Bf16>(g, kind, workspace, st)
+                                : launch_type<F16>(g, kind, workspace, st);
+}
+
+}  // namespace mi355q

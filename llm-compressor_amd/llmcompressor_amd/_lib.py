@@ -108,7 +108,9 @@ SIGNATURES = {
     "mi355q_moe_combine_backward": (_i32, [_vp, _i32, _i64, _i64, _i64, _i64, _vp, _i64, _vp, _i32, _vp, _vp, _vp, _i64,
                                            _vp, _vp]),
     "mi355q_w4a16_matmul": (_i32, [_vp, _i32, _i64, _i64, _vp, _vp, _i64, _vp, _i32, _i64, _i64, _vp, _i32, _i64, _i64,
-                                   _vp, _i64, _i64, _i64, _vp, _i32, _i32, _vp, _i32, _i64, _i64, _i64, _i64, _vp]),
+                                   _vp, _i64, _i64, _i64, _vp, _i32, _i32, _vp, _i32, _i64, _i64, _i64, _i64, _vp, _sz,
+                                   _vp]),
+    "mi355q_w4a16_matmul_workspace_size": (_sz, [_i64, _i64, _i64, _i64, _i64, _i32, _i64]),
 }
 
 _lock = threading.Lock()

@@ -1075,6 +1075,11 @@ def _w4_operand(t: torch.Tensor, shape, dtypes, what: str, lead: int):
     return t, strides[-2] if rows > 1 else cols, strides[0] if lead else 0
 
 
+@functools.lru_cache(maxsize=4096)
+def _w4_workspace(n_x: int, rows: int, experts: int, out: int, cols: int, fmt: int, group: int) -> int:
+    return L.lib().mi355q_w4a16_matmul_workspace_size(n_x, rows, experts, out, cols, fmt, group)
+
+
 def _w4_matmul(x, index, offsets, experts, n_rows, weight_packed, weight_scale, weight_zero_point, group_size, bias,
                gated, out_dtype):
     if not x.is_cuda:
@@ -1148,11 +1153,15 @@ def _w4_matmul(x, index, offsets, experts, n_rows, weight_packed, weight_scale, 
         raise TypeError(f"out_dtype must be bf16, fp16 or fp32, got {out_dtype}")
     width = out // 2 if gated else out
     y = x.new_empty((n_rows, width), dtype=out_dtype)
+    fmt = L.W4_MXFP4 if mx else L.W4_INT4
+    ws_bytes = _w4_workspace(n_x, n_rows, experts or 1, out, cols, fmt, group)
+    ws = x.new_empty(ws_bytes, dtype=torch.uint8) if ws_bytes else None
+    ws_ptr = None if ws is None else ws.data_ptr()
     rc = L.lib().mi355q_w4a16_matmul(
         x.data_ptr(), kind, n_x, pitch, None if index is None else index.data_ptr(),
-        None if offsets is None else offsets.data_ptr(), experts or 1, w.data_ptr(), L.W4_MXFP4 if mx else L.W4_INT4,
-        ldw, stride_w, s.data_ptr(), s_kind, lds, stride_s, z_ptr, ldz, stride_z, group, b_ptr, b_kind, int(gated),
-        y.data_ptr(), y_kind, width, n_rows, out, cols, L.stream_of(x))
+        None if offsets is None else offsets.data_ptr(), experts or 1, w.data_ptr(), fmt, ldw,
+        stride_w, s.data_ptr(), s_kind, lds, stride_s, z_ptr, ldz, stride_z, group, b_ptr, b_kind, int(gated),
+        y.data_ptr(), y_kind, width, n_rows, out, cols, ws_ptr, ws_bytes, L.stream_of(x))
     if rc:
         L.check(rc)
     return y
