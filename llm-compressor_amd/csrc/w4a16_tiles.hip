@@ -16,6 +16,8 @@
 // the same way, and the accumulators begin with the six products that count down to
 // 2^-24.  With 128 columns per group that is 1/43 of the MFMAs, 1/21 where s z has more bits
 // than bf16 holds.
+#include <type_traits>
+
 #include "w4a16.h"
 
 namespace mi355q {
@@ -56,17 +58,17 @@ __device__ __forceinline__ void split3(float v, uint16_t (&p)[3]) {
 // the last group; copy: x with rows of whole steps, zeros behind the last column.
 // 2^lanes lanes share a group, and a wave holds 64 >> lanes of them.
 template <class T>
-__global__ __launch_bounds__(256) void w4_prepare_kernel(const uint16_t* x, int64_t ldx, int64_t n_x, int64_t cols,
-                                                         int group, uint32_t groups, uint32_t padded, int lanes,
-                                                         uint16_t* sums, uint16_t* copy, int64_t ld_copy) {
+__device__ __forceinline__ void w4_sums(const W4Args& g, uint32_t padded, int lanes, uint32_t block, uint16_t* sums,
+                                        uint16_t* copy, int64_t ld_copy) {
+  const int64_t cols = g.cols;
   const int lane = threadIdx.x & 63, sub = lane & ((1 << lanes) - 1);
   const uint32_t per = 64u >> lanes, parts = (padded + per - 1) / per;
-  const uint64_t item = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const uint64_t item = (uint64_t)block * 4 + (threadIdx.x >> 6);
   const int64_t m = (int64_t)(item / parts);
-  if (m >= n_x) return;
+  if (m >= g.n_x) return;
   const uint32_t gi = (uint32_t)(item % parts) * per + (lane >> lanes);
-  const uint16_t* const row = x + m * ldx;
-  const int64_t k0 = (int64_t)gi * group, k1 = gi < groups ? (k0 + group < cols ? k0 + group : cols) : k0;
+  const uint16_t* const row = g.x + m * g.ldx;
+  const int64_t k0 = (int64_t)gi * g.group, k1 = gi < g.groups ? (k0 + g.group < cols ? k0 + g.group : cols) : k0;
   float sum = 0.f;
   for (int64_t k = k0 + 8 * sub; k < k1; k += 8 << lanes) {
     uint16_t v[8];
@@ -89,14 +91,66 @@ __global__ __launch_bounds__(256) void w4_prepare_kernel(const uint16_t* x, int6
 #pragma unroll
     for (int i = 0; i < 3; ++i) sums[((size_t)m * 3 + i) * padded + gi] = p[i];
   }
-  if (copy && gi == groups - 1)
+  if (copy && gi == g.groups - 1)
     for (int64_t k = (cols + 7) / 8 * 8 + 8 * sub; k < ld_copy; k += 8 << lanes)
       *reinterpret_cast<u32x4_t*>(copy + m * ld_copy + k) = u32x4_t{0u, 0u, 0u, 0u};
 }
 
+// Of every expert's column n: factors[n][piece][g], -s z over group g as three bf16
+// numbers, zeros behind the last group; and scales[expert][g][column], what the tiles
+// multiply with (the operand of the conversion where the scale goes there), so that neighbouring
+// lanes read neighbouring scales.  A thread takes one, 32 neighbouring columns to 8 groups.
+template <int KIND, bool FOLD>
+__device__ __forceinline__ void w4_factors(const W4Args& g, uint32_t padded, uint32_t block, uint16_t* factors,
+                                           uint32_t* scales) {
+  const uint32_t cols = (uint32_t)((g.out + 31) / 32), in = block % (cols * (padded / 8));
+  const int64_t e = block / (cols * (padded / 8));
+  const int64_t c = (int64_t)(in % cols) * 32 + (threadIdx.x >> 3);
+  const uint32_t gi = in / cols * 8 + (threadIdx.x & 7);
+  __shared__ uint32_t turn[8][33];
+  if (c < g.out) {
+    float s = 0.f, v = 0.f;
+    if (gi < g.groups) {
+      if constexpr (KIND == kMxfp4) {
+        const uint32_t b = static_cast<const uint8_t*>(g.s)[e * g.stride_s + c * g.lds + gi];
+        s = FOLD ? __uint_as_float((b << 23) | 0x00400000u) : e8m0_to_f32(b);
+      } else {
+        s = load_any(g.s, g.s_type, e * g.stride_s + c * g.lds + gi);
+        float z = 8.f;
+        if constexpr (KIND == kInt4Zero)
+          z = (float)((g.z[e * g.stride_z + c / 8 * g.ldz + gi] >> (4 * (int)(c % 8))) & 15u);
+        v = -z * s;
+      }
+    }
+    turn[threadIdx.x & 7][threadIdx.x >> 3] = __float_as_uint(s);
+    if constexpr (KIND != kMxfp4) {
+      uint16_t p[3];
+      split3(v, p);
+#pragma unroll
+      for (int k = 0; k < 3; ++k) factors[((e * g.out + c) * 3 + k) * padded + gi] = p[k];
+    }
+  }
+  __syncthreads();
+  const int64_t n = (int64_t)(in % cols) * 32 + (threadIdx.x & 31);
+  if (n < g.out)
+    scales[(e * padded + in / cols * 8 + (threadIdx.x >> 5)) * g.out + n] = turn[threadIdx.x >> 5][threadIdx.x & 31];
+}
+
+// What the tiles read beside x and the weight, in one launch: the first `x_blocks` workgroups
+// take x, the others the weight's factors.
+template <class T, int KIND>
+__global__ __launch_bounds__(256) void w4_prepare_kernel(W4Args g, uint32_t padded, int lanes, uint32_t x_blocks,
+                                                         uint16_t* sums, uint16_t* factors, uint32_t* scales,
+                                                         uint16_t* copy, int64_t ld_copy) {
+  if (blockIdx.x < x_blocks) w4_sums<T>(g, padded, lanes, blockIdx.x, sums, copy, ld_copy);
+  else w4_factors<KIND, KIND == kMxfp4 && T::code == MI355Q_BF16>(g, padded, blockIdx.x - x_blocks, factors, scales);
+}
+
 // ---------------------------------------------------------------- tiles
 struct W4Tiles {
-  const uint16_t* sums;      // [n_x][3][padded], or null: no zero points (MXFP4)
+  const uint16_t* sums;      // [n_x][3][padded]; MXFP4: unused
+  const uint16_t* factors;   // [experts][out][3][padded]
+  const float* scales;       // [experts][padded][out]
   uint32_t padded;           // groups, a multiple of 16
   int pieces;                // of the factors s z: 1 or 3
   uint32_t row_tiles, col_tiles;
@@ -169,76 +223,82 @@ void w4_tiles_kernel(W4Args g, W4Tiles o) {
   const uint32_t l0 = lds_u32(ring);
   const int whole = (int)(g.cols / kStep);            // steps of 128 columns
   const int tail = (int)(g.cols % kStep + 7) / 8;     // chunks of a shorter last one (rows that end inside one are copies)
-  auto dma = [&](int s, int slot) __attribute__((always_inline)) {
+  auto dma = [&](int s, int slot, auto full) __attribute__((always_inline)) {
+    const char* const base = xb + (int64_t)s * (2 * kStep);
+    const uint32_t m0 = l0 + slot * S::SLOT;
+    auto place = [&](int i) __attribute__((always_inline)) {
+      const int q = wave * S::NI + i;
+      return m0 + (q & 3) * (R * 64) + (q >> 2) * 1024;
+    };
+    if (decltype(full)::value || s < whole) {
 #pragma unroll
-    for (int i = 0; i < S::NI; ++i) {
-      const int q = wave * S::NI + i, hi = q & 3;
-      const char* const base = xb + (int64_t)s * (2 * kStep);
-      const uint32_t m0 = l0 + slot * S::SLOT + hi * (R * 64) + (q >> 2) * 1024;
-      if (s < whole) {
-        dma16(xo[i / 4], base + 64 * hi, m0);
-      } else {
-        // chunks past the last column: the row's first one of the step, which meets zeros (offsets are
-        // unsigned: the 64 hi columns are added to them, so that taking the chunk off stays above the base)
-        dma16(xo[i / 4] + (4 * hi + chunk < tail ? 64 * hi : -16 * chunk), base, m0);
+      for (int i = 0; i < S::NI; ++i) dma16(xo[i / 4], base + 64 * ((wave * S::NI + i) & 3), place(i));
+    } else {
+      // chunks past the last column: the row's first one of the step, which meets zeros (offsets are
+      // unsigned: the 64 columns of a chunk's quarter are added to them, so that taking the chunk off stays
+      // above the base)
+#pragma unroll
+      for (int i = 0; i < S::NI; ++i) {
+        const int hi = (wave * S::NI + i) & 3;
+        dma16(xo[i / 4] + (4 * hi + chunk < tail ? 64 * hi : -16 * chunk), base, place(i));
       }
     }
   };
   // operand reads: lane l has row l & 31, columns 16 j + 8 (l / 32) and on of slice j
-  const int ra[2] = {ln * 64 + 16 * (h ^ ((ln >> 2) & 3)), ln * 64 + 16 * ((2 + h) ^ ((ln >> 2) & 3))};
-  auto read_x = [&](int slot, int b, int j) __attribute__((always_inline)) {
-    return *reinterpret_cast<const u32x4_t*>(ring + slot * S::SLOT + (j >> 1) * (R * 64) + b * 2048 + ra[j & 1]);
+  int ra[2] = {ln * 64 + 16 * (h ^ ((ln >> 2) & 3)), ln * 64 + 16 * ((2 + h) ^ ((ln >> 2) & 3))};
+  static_assert((S::SLOT & (S::SLOT - 1)) == 0 && S::SLOT >= 2048, "the slots differ in one bit of the address");
+  auto read_x = [&](int b, int j) __attribute__((always_inline)) {
+    return *reinterpret_cast<const u32x4_t*>(ring + (j >> 1) * (R * 64) + b * 2048 + ra[j & 1]);
   };
 
   // weights: lane l has column l & 31 of every tile, 16 bytes each at 16 (l / 32) of both halves of the step
-  uint32_t wo[NTW];
-  uint32_t so[NTW];
+  uint32_t wo[NTW], wn[NTW];
 #pragma unroll
   for (int a = 0; a < NTW; ++a) {
     const int64_t limit = g.gated && column(a) < half ? half : g.out, n = column(a) + ln;
     const int64_t c = n < limit ? n : limit - 1;
+    wn[a] = (uint32_t)c;
     wo[a] = (uint32_t)(c * g.ldw) + 16 * h;
-    so[a] = (uint32_t)(c * g.lds);
   }
+  // (buffer loads: a 32-bit offset per lane)
   const uint8_t* const wb = g.w + tile.expert * g.stride_w;
-  const int64_t s_base = tile.expert * g.stride_s;
+  const auto w_rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(wb), 0, 0xffffffffu, 0x00020000);
+  const auto s_rsrc = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<float*>(o.scales) + (size_t)tile.expert * o.padded * g.out, 0, 0xffffffffu, 0x00020000);
   const int words = KIND == kMxfp4 ? (int)(g.cols / 8) : (int)((g.cols + 7) / 8);
   struct Raw {
     u32x4_t w[NTW][2];
-    uint32_t s[NTW][GPS];
+    float s[NTW][GPS];
   };
-  auto load_w = [&](Raw& r, int s) __attribute__((always_inline)) {
+  auto load_w = [&](Raw& r, int s, auto full) __attribute__((always_inline)) {
 #pragma unroll
-    for (int a = 0; a < NTW; ++a) {
+    for (int a = 0; a < NTW; ++a)
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
-        const uint8_t* const p = wb + (int64_t)s * (kStep / 2) + 32 * b + wo[a];
-        if (s < whole) {
-          __builtin_memcpy(&r.w[a][b], p, 16);
+        if (decltype(full)::value || s < whole) {
+          r.w[a][b] = __builtin_bit_cast(
+              u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(w_rsrc, wo[a], s * (kStep / 2) + 32 * b, 0));
         } else {
           const int last = words - s * (kStep / 8) - 8 * b - 4 * h;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) r.w[a][b][i] = i < last ? reinterpret_cast<const uint32_t*>(p)[i] : 0u;
+          for (int i = 0; i < 4; ++i)
+            r.w[a][b][i] = i < last ? *reinterpret_cast<const uint32_t*>(wb + (int64_t)s * (kStep / 2) + 32 * b + wo[a] +
+                                                                         4 * i) : 0u;
         }
       }
 #pragma unroll
-      for (int i = 0; i < GPS; ++i) {
-        const uint32_t gs = GPS == 1 ? div((uint32_t)s, g.per) : (uint32_t)s * GPS + i;
-        const int64_t at = s_base + so[a] + (gs < g.groups ? gs : g.groups - 1);
-        if constexpr (KIND == kMxfp4) r.s[a][i] = static_cast<const uint8_t*>(g.s)[at];
-        else if (g.s_type == MI355Q_F32) r.s[a][i] = static_cast<const uint32_t*>(g.s)[at];
-        else r.s[a][i] = static_cast<const uint16_t*>(g.s)[at];
-      }
-    }
+    for (int i = 0; i < GPS; ++i)
+#pragma unroll
+      for (int a = 0; a < NTW; ++a)
+        r.s[a][i] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(
+            s_rsrc, 4 * wn[a], (GPS == 1 ? div((uint32_t)s, g.per) : (uint32_t)s * GPS + i) * (uint32_t)(4 * g.out), 0));
   };
-  auto scale_of = [&](uint32_t v) __attribute__((always_inline)) {
-    if constexpr (FOLD) return __uint_as_float((v << 23) | 0x00400000u);
-    else if constexpr (KIND == kMxfp4) return e8m0_to_f32(v);
-    else return g.s_type == MI355Q_F32 ? __uint_as_float(v)
-                : g.s_type == MI355Q_BF16 ? __uint_as_float(v << 16) : F16::load((uint16_t)v);
+  // (floats, not the MFMAs' tuples of 16, unless an MFMA adds to them)
+  struct Floats {
+    float v[16];
+    __device__ float& operator[](int i) { return v[i]; }
   };
-
-  f32x16_t acc[MTW][NTW];
+  typename std::conditional<FOLD, f32x16_t, Floats>::type acc[MTW][NTW];
 #pragma unroll
   for (int b = 0; b < MTW; ++b)
 #pragma unroll
@@ -246,103 +306,119 @@ void w4_tiles_kernel(W4Args g, W4Tiles o) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[b][a][e] = 0.f;
 
-  Raw raw;
-  dma(0, 0);
-  load_w(raw, 0);
+  dma(0, 0, std::false_type{});
   if constexpr (KIND != kMxfp4) {
     // the zero points' part: sums of x [m][g] times -s z [n][g], 16 groups at a time
+    const uint16_t* fp[NTW];
+    const uint16_t* sp[MTW];
+#pragma unroll
+    for (int a = 0; a < NTW; ++a)
+      fp[a] = o.factors + ((size_t)tile.expert * g.out + wn[a]) * 3 * o.padded + 8 * h;
+#pragma unroll
+    for (int b = 0; b < MTW; ++b) {
+      const int64_t row = x_row[32 * b + ln];
+      sp[b] = o.sums + (size_t)(row < 0 ? 0 : row) * 3 * o.padded + 8 * h;
+    }
     for (uint32_t g0 = 0; g0 < o.padded; g0 += 16) {
       u32x4_t f[NTW][3];
 #pragma unroll
-      for (int a = 0; a < NTW; ++a) {
-        uint16_t p[3][8];
-        const int64_t limit = g.gated && column(a) < half ? half : g.out, n = column(a) + ln;
-        const int64_t c = n < limit ? n : limit - 1;
+      for (int a = 0; a < NTW; ++a)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const uint32_t gi = g0 + 8 * h + e;
-          float v = 0.f;
-          if (gi < g.groups) {
-            float z = 8.f;
-            if constexpr (KIND == kInt4Zero)
-              z = (float)((g.z[tile.expert * g.stride_z + c / 8 * g.ldz + gi] >> (4 * (int)(c % 8))) & 15u);
-            v = -z * load_any(g.s, g.s_type, s_base + so[a] + gi);
-          }
-          uint16_t q[3];
-          split3(v, q);
-#pragma unroll
-          for (int i = 0; i < 3; ++i) p[i][e] = q[i];
-        }
-#pragma unroll
-        for (int i = 0; i < 3; ++i) __builtin_memcpy(&f[a][i], p[i], 16);
-      }
+        for (int i = 0; i < 3; ++i) f[a][i] = *reinterpret_cast<const u32x4_t*>(fp[a] + g0 + (size_t)i * o.padded);
 #pragma unroll
       for (int b = 0; b < MTW; ++b) {
-        const int64_t row = x_row[32 * b + ln];
-        const uint16_t* const sp = o.sums + (row < 0 ? 0 : row) * 3 * o.padded + g0 + 8 * h;
         u32x4_t v[3];
 #pragma unroll
-        for (int i = 0; i < 3; ++i) v[i] = *reinterpret_cast<const u32x4_t*>(sp + (size_t)i * o.padded);
+        for (int i = 0; i < 3; ++i) v[i] = *reinterpret_cast<const u32x4_t*>(sp[b] + g0 + (size_t)i * o.padded);
 #pragma unroll
         for (int a = 0; a < NTW; ++a) {
+          f32x16_t p = {};
 #pragma unroll
-          for (int i = 0; i < 3; ++i) acc[b][a] = mfma32<Bf16>(v[i], f[a][0], acc[b][a]);
+          for (int i = 0; i < 3; ++i) p = mfma32<Bf16>(v[i], f[a][0], p);
           if (o.pieces > 1) {
-            acc[b][a] = mfma32<Bf16>(v[0], f[a][1], acc[b][a]);
-            acc[b][a] = mfma32<Bf16>(v[1], f[a][1], acc[b][a]);
-            acc[b][a] = mfma32<Bf16>(v[0], f[a][2], acc[b][a]);
+            p = mfma32<Bf16>(v[0], f[a][1], p);
+            p = mfma32<Bf16>(v[1], f[a][1], p);
+            p = mfma32<Bf16>(v[0], f[a][2], p);
           }
+#pragma unroll
+          for (int e = 0; e < 16; ++e) acc[b][a][e] += p[e];
         }
       }
     }
   }
-  for (int s = 0; s < steps; ++s) {
+  Raw raw;
+  load_w(raw, 0, std::false_type{});
+  // Step s; `full`: the next one is a whole step (no branches then: the order of the loop's
+  // instructions is kept).
+  auto step = [&](int s, auto full) __attribute__((always_inline)) {
+    constexpr bool FULL = decltype(full)::value;
     const int slot = s & 1;
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");   // the step is here, the other slot read
-    if (s + 1 < steps) dma(s + 1, slot ^ 1);
-    u32x4_t q[NTW][kSlices];
+    // what was loaded is used, and so waited for by the compiler's count, before the DMA that it does not count
+    uint32_t w[NTW][kSlices];
     float sc[NTW][GPS];
 #pragma unroll
     for (int a = 0; a < NTW; ++a) {
-#pragma unroll
-      for (int i = 0; i < GPS; ++i) sc[a][i] = scale_of(raw.s[a][i]);
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
         // words 0 and 1 of both halves of the wave are slices 0 and 2, words 2 and 3 slices 1 and 3
         const auto u = __builtin_amdgcn_permlane32_swap(raw.w[a][b][0], raw.w[a][b][1], false, false);
         const auto v = __builtin_amdgcn_permlane32_swap(raw.w[a][b][2], raw.w[a][b][3], false, false);
-        const uint32_t w[4] = {(uint32_t)u[0], (uint32_t)v[0], (uint32_t)u[1], (uint32_t)v[1]};
+        w[a][4 * b] = u[0], w[a][4 * b + 1] = v[0], w[a][4 * b + 2] = u[1], w[a][4 * b + 3] = v[1];
+      }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int j = 4 * b + i;
-          if constexpr (KIND == kMxfp4) q[a][j] = e2m1s<T>(w[i], FOLD ? sc[a][j * GPS / kSlices] : 1.f);
-          else q[a][j] = nibbles<T>(w[i]);
-        }
+      for (int i = 0; i < GPS; ++i) {
+        sc[a][i] = raw.s[a][i];
+        asm volatile("" : "+v"(sc[a][i]));
       }
     }
-    if (s + 1 < steps) load_w(raw, s + 1);
+    __builtin_amdgcn_sched_barrier(0);
+    if (FULL || s + 1 < steps) dma(s + 1, slot ^ 1, full);
+    u32x4_t q[NTW][kSlices];
+#pragma unroll
+    for (int a = 0; a < NTW; ++a)
+#pragma unroll
+      for (int j = 0; j < kSlices; ++j) {
+        if constexpr (KIND == kMxfp4) q[a][j] = e2m1s<T>(w[a][j], FOLD ? sc[a][j * GPS / kSlices] : 1.f);
+        else q[a][j] = nibbles<T>(w[a][j]);
+      }
 #pragma unroll
     for (int b = 0; b < MTW; ++b) {
-      u32x4_t v[kSlices];
+      __builtin_amdgcn_sched_barrier(0);
+      f32x16_t p[NTW];
 #pragma unroll
-      for (int j = 0; j < kSlices; ++j) v[j] = read_x(slot, b, j);
-#pragma unroll
-      for (int i = 0; i < GPS; ++i)
+      for (int j = 0; j < kSlices; ++j) {
+        const u32x4_t v = read_x(b, j);
 #pragma unroll
         for (int a = 0; a < NTW; ++a) {
           if constexpr (FOLD) {
-#pragma unroll
-            for (int j = 0; j < PER; ++j) acc[b][a] = mfma32<T>(v[i * PER + j], q[a][i * PER + j], acc[b][a]);
+            acc[b][a] = mfma32<T>(v, q[a][j], acc[b][a]);
           } else {
-            f32x16_t p = {};
+            p[a] = mfma32<T>(v, q[a][j], j % PER ? p[a] : f32x16_t{});
+            if (j % PER == PER - 1) {
 #pragma unroll
-            for (int j = 0; j < PER; ++j) p = mfma32<T>(v[i * PER + j], q[a][i * PER + j], p);
-#pragma unroll
-            for (int e = 0; e < 16; ++e) acc[b][a][e] = fmaf(p[e], sc[a][i], acc[b][a][e]);
+              for (int e = 0; e < 16; ++e) acc[b][a][e] = fmaf(p[a][e], sc[a][j / PER], acc[b][a][e]);
+            }
           }
         }
+      }
+      // two operand reads ahead of their MFMAs
+      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+#pragma unroll
+      for (int j = 0; j < kSlices - 2; ++j) {
+        __builtin_amdgcn_sched_group_barrier(0x008, NTW, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      }
     }
-  }
+    __builtin_amdgcn_sched_barrier(0);
+    // the next step's weights, when this one's are out of the registers
+    if (FULL || s + 1 < steps) load_w(raw, s + 1, full);
+    ra[0] ^= S::SLOT;
+    ra[1] ^= S::SLOT;
+  };
+  int s = 0;
+  for (; s + 1 < whole; ++s) step(s, std::true_type{});
+  for (; s < steps; ++s) step(s, std::false_type{});
   // a lane has column l & 31 and rows 8 (e / 4) + 4 (l / 32) + e % 4
 #pragma unroll
   for (int a = 0; a < NTW; ++a) {
@@ -379,7 +455,8 @@ bool w4_tiles_fit(const W4Args& g) {
   const int64_t limit = (int64_t)1 << 32;
   const int64_t steps = (g.cols + kStep - 1) / kStep * kStep;
   const int64_t pitch = g.ldx > steps ? g.ldx : steps;
-  return span < limit / (2 * pitch) && g.out < limit / g.ldw && g.out < limit / (g.lds > 0 ? g.lds : 1);
+  return span < limit / (2 * pitch) && g.out < limit / g.ldw &&
+         g.out < limit / (4 * (int64_t)((g.groups + 15) / 16 * 16));
 }
 
 static bool in_place(const W4Args& g) { return aligned16(g.x) && g.ldx % 8 == 0 && g.cols % 8 == 0; }
@@ -388,9 +465,13 @@ static size_t sums_bytes(int64_t n_x, uint32_t groups) {
   return ((size_t)n_x * 3 * ((groups + 15) / 16 * 16) * sizeof(uint16_t) + 255) / 256 * 256;
 }
 
-size_t w4_tiles_workspace(int64_t n_x, int64_t cols, uint32_t groups, bool zero_points_enter) {
+static size_t scales_bytes(int64_t rows_w, uint32_t groups) {
+  return ((size_t)rows_w * ((groups + 15) / 16 * 16) * sizeof(float) + 255) / 256 * 256;
+}
+
+size_t w4_tiles_workspace(int64_t n_x, int64_t rows_w, int64_t cols, uint32_t groups, bool zero_points_enter) {
   // an x that the DMA cannot read (rows off 16 bytes or of no whole chunks) is copied
-  return (zero_points_enter ? sums_bytes(n_x, groups) : 0) +
+  return (zero_points_enter ? sums_bytes(n_x, groups) + sums_bytes(rows_w, groups) : 0) + scales_bytes(rows_w, groups) +
          (size_t)n_x * ((cols + kStep - 1) / kStep * kStep) * sizeof(uint16_t);
 }
 
@@ -420,33 +501,47 @@ template <class T>
 static int launch_type(W4Args g, int kind, void* workspace, hipStream_t st) {
   const bool copy = !in_place(g), sums = kind != kMxfp4;
   const uint32_t padded = (g.groups + 15) / 16 * 16;
-  W4Tiles o = {sums ? static_cast<const uint16_t*>(workspace) : nullptr, padded,
-               kind == kInt4 && g.s_type == MI355Q_BF16 ? 1 : 3, 0, 0};
-  const int64_t ld_copy = (g.cols + kStep - 1) / kStep * kStep;
-  uint16_t* const to = copy ? reinterpret_cast<uint16_t*>(static_cast<char*>(workspace) +
-                                                          (sums ? sums_bytes(g.n_x, g.groups) : 0)) : nullptr;
-  if (copy || sums) {
-    int lanes = 0;
-    while (lanes < 6 && (8 << lanes) < g.group) ++lanes;
-    const uint64_t parts = (padded + (64u >> lanes) - 1) / (64u >> lanes), items = parts * (uint64_t)g.n_x;
-    MQ_CHECK_ARG((items + 3) / 4 <= UINT32_MAX / 256, "w4a16_matmul: %lld rows of x are too many", (long long)g.n_x);
-    hipLaunchKernelGGL((w4_prepare_kernel<T>), dim3((unsigned)((items + 3) / 4)), dim3(256), 0, st, g.x, g.ldx, g.n_x,
-                       g.cols, g.group, g.groups, padded, lanes, sums ? static_cast<uint16_t*>(workspace) : nullptr, to,
-                       ld_copy);
-    MQ_LAUNCH_CHECK();
+  char* at = static_cast<char*>(workspace);
+  uint16_t *to_sums = nullptr, *to_factors = nullptr, *to = nullptr;
+  if (sums) {
+    to_sums = reinterpret_cast<uint16_t*>(at);
+    at += sums_bytes(g.n_x, g.groups);
+    to_factors = reinterpret_cast<uint16_t*>(at);
+    at += sums_bytes(g.experts * g.out, g.groups);
   }
+  float* const to_scales = reinterpret_cast<float*>(at);
+  at += scales_bytes(g.experts * g.out, g.groups);
+  const int64_t ld_copy = (g.cols + kStep - 1) / kStep * kStep;
+  if (copy) to = reinterpret_cast<uint16_t*>(at);
+  const W4Tiles o = {to_sums, to_factors, to_scales, padded, kind == kInt4 && g.s_type == MI355Q_BF16 ? 1 : 3, 0, 0};
+  int lanes = 0;
+  while (lanes < 6 && (8 << lanes) < g.group) ++lanes;
+  const uint64_t parts = (padded + (64u >> lanes) - 1) / (64u >> lanes);
+  const uint64_t x_blocks = copy || sums ? (parts * (uint64_t)g.n_x + 3) / 4 : 0;
+  const uint64_t w_blocks = (uint64_t)g.experts * ((g.out + 31) / 32) * (padded / 8);
+  MQ_CHECK_ARG(x_blocks + w_blocks <= UINT32_MAX / 256, "w4a16_matmul: %lld rows of x and %lld of weights are too many",
+               (long long)g.n_x, (long long)(g.experts * g.out));
+  const dim3 grid((unsigned)(x_blocks + w_blocks)), block(256);
+  auto* const s_out = reinterpret_cast<uint32_t*>(to_scales);
+  if (kind == kInt4Zero)
+    hipLaunchKernelGGL((w4_prepare_kernel<T, kInt4Zero>), grid, block, 0, st, g, padded, lanes, (uint32_t)x_blocks,
+                       to_sums, to_factors, s_out, to, ld_copy);
+  else if (kind == kInt4)
+    hipLaunchKernelGGL((w4_prepare_kernel<T, kInt4>), grid, block, 0, st, g, padded, lanes, (uint32_t)x_blocks, to_sums,
+                       to_factors, s_out, to, ld_copy);
+  else
+    hipLaunchKernelGGL((w4_prepare_kernel<T, kMxfp4>), grid, block, 0, st, g, padded, lanes, (uint32_t)x_blocks,
+                       to_sums, to_factors, s_out, to, ld_copy);
+  MQ_LAUNCH_CHECK();
   if (copy) {
     g.x = to;
     g.ldx = ld_copy;
   }
   if (kind == kMxfp4) return launch_kind<T, kMxfp4, 4>(g, o, st);
   const int gps = g.groups > 1 && g.group == 32 ? 4 : g.groups > 1 && g.group == 64 ? 2 : 1;
-  // zero points enter before the sum: both kinds take one kernel but for that
-  if (kind == kInt4)
-    return gps == 4 ? launch_kind<T, kInt4, 4>(g, o, st)
-           : gps == 2 ? launch_kind<T, kInt4, 2>(g, o, st) : launch_kind<T, kInt4, 1>(g, o, st);
-  return gps == 4 ? launch_kind<T, kInt4Zero, 4>(g, o, st)
-         : gps == 2 ? launch_kind<T, kInt4Zero, 2>(g, o, st) : launch_kind<T, kInt4Zero, 1>(g, o, st);
+  if (gps == 4) return launch_kind<T, kInt4, 4>(g, o, st);
+  if (gps == 2) return launch_kind<T, kInt4, 2>(g, o, st);
+  return launch_kind<T, kInt4, 1>(g, o, st);
 }
 
 int launch_w4_tiles(const W4Args& g, mi355q_dtype x_dtype, int kind, void* workspace, hipStream_t st) {
