@@ -272,7 +272,7 @@ extern "C" size_t mi355q_w4a16_matmul_workspace_size(int64_t n_x, int64_t rows, 
                                                      int64_t cols, mi355q_w4_format format, int64_t group_size) {
   if (n_x <= 0 || rows <= 0 || experts <= 0 || out <= 0 || cols <= 0 || group_size <= 0 || few_rows(rows, experts))
     return 0;
-  return w4_tiles_workspace(n_x, experts * out, cols, (uint32_t)((cols + group_size - 1) / group_size), format == MI355Q_W4_INT4);
+  return w4_tiles_workspace(n_x, experts * out, cols, (uint32_t)((cols + group_size - 1) / group_size), format == MI355Q_W4_MXFP4);
 }
 
 extern "C" int mi355q_w4a16_matmul(const void* x_dev, mi355q_dtype x_dtype, int64_t n_x, int64_t ldx,
@@ -316,8 +316,8 @@ extern "C" int mi355q_w4a16_matmul(const void* x_dev, mi355q_dtype x_dtype, int6
               fast_div((uint32_t)(group_size < cols ? (group_size + 127) / 128 : (cols + 127) / 128)), gated != 0};
   const int kind = mx ? kMxfp4 : zeros_dev ? kInt4Zero : kInt4;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (!few_rows(rows, experts) && w4_tiles_fit(g) && workspace_dev && aligned16(workspace_dev) &&
-      workspace_bytes >= w4_tiles_workspace(n_x, experts * out, cols, g.groups, !mx))
+  if (!few_rows(rows, experts) && w4_tiles_fit(g, kind) && workspace_dev && aligned16(workspace_dev) &&
+      workspace_bytes >= w4_tiles_workspace(n_x, experts * out, cols, g.groups, mx))
     return launch_w4_tiles(g, x_dtype, kind, workspace_dev, st);
   return x_dtype == MI355Q_BF16 ? launch_type<Bf16>(g, kind, st) : launch_type<F16>(g, kind, st);
 }

@@ -136,14 +136,39 @@ __device__ __forceinline__ void w4_factors(const W4Args& g, uint32_t padded, uin
     scales[(e * padded + in / cols * 8 + (threadIdx.x >> 5)) * g.out + n] = turn[threadIdx.x >> 5][threadIdx.x & 31];
 }
 
-// What the tiles read beside x and the weight, in one launch: the first `x_blocks` workgroups
-// take x, the others the weight's factors.
+// The weight with rows of whole 16-byte chunks, which the DMA can read.  A thread takes one.
+__device__ __forceinline__ void w4_copy(const W4Args& g, uint64_t i, int64_t bytes, uint8_t* copy) {
+  const uint64_t chunks = (uint64_t)(bytes + 15) / 16, n = i / chunks;
+  const int64_t at = (int64_t)(i - n * chunks) * 16, e = (int64_t)(n / (uint64_t)g.out);
+  if (e >= g.experts) return;
+  const uint8_t* const p = g.w + e * g.stride_w + (int64_t)(n % (uint64_t)g.out) * g.ldw + at;
+  u32x4_t v;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) v[k] = at + 4 * k < bytes ? reinterpret_cast<const uint32_t*>(p)[k] : 0u;
+  *reinterpret_cast<u32x4_t*>(copy + i * 16) = v;
+}
+
+// What the tiles read beside x and the weight, in one launch: the first workgroups take x,
+// the next the weight's factors, the others (if there are) its codes.
+struct W4Prepare {
+  uint32_t padded;         // groups, a multiple of 16
+  int lanes;               // log2 of the lanes per group of x
+  uint32_t x_blocks, f_blocks;
+  uint16_t *sums, *factors;
+  uint32_t* scales;
+  uint16_t* x_copy;        // or null
+  int64_t ld_copy;
+  uint8_t* w_copy;
+  int64_t w_bytes;         // of a row
+};
 template <class T, int KIND>
-__global__ __launch_bounds__(256) void w4_prepare_kernel(W4Args g, uint32_t padded, int lanes, uint32_t x_blocks,
-                                                         uint16_t* sums, uint16_t* factors, uint32_t* scales,
-                                                         uint16_t* copy, int64_t ld_copy) {
-  if (blockIdx.x < x_blocks) w4_sums<T>(g, padded, lanes, blockIdx.x, sums, copy, ld_copy);
-  else w4_factors<KIND, KIND == kMxfp4 && T::code == MI355Q_BF16>(g, padded, blockIdx.x - x_blocks, factors, scales);
+__global__ __launch_bounds__(256) void w4_prepare_kernel(W4Args g, W4Prepare p) {
+  if (blockIdx.x < p.x_blocks)
+    w4_sums<T>(g, p.padded, p.lanes, blockIdx.x, p.sums, p.x_copy, p.ld_copy);
+  else if (blockIdx.x - p.x_blocks < p.f_blocks)
+    w4_factors<KIND, KIND == kMxfp4 && T::code == MI355Q_BF16>(g, p.padded, blockIdx.x - p.x_blocks, p.factors, p.scales);
+  else
+    w4_copy(g, (uint64_t)(blockIdx.x - p.x_blocks - p.f_blocks) * 256 + threadIdx.x, p.w_bytes, p.w_copy);
 }
 
 // ---------------------------------------------------------------- tiles
@@ -161,7 +186,14 @@ struct TileShape {
   static constexpr int R = 32 * MTW;                 // rows of x
   static constexpr int SLOT = R * kStep * 2;         // bytes of a step
   static constexpr int NI = R / 16;                  // DMA instructions per wave and step
+  static constexpr int W = 2 * SLOT;                 // where the waves' codes begin
 };
+__device__ __forceinline__ float silu(float v) {
+  // e^-v = 2^(-v log2 e), with what the product's rounding leaves put back
+  const float k = -1.44269504f, t = v * k, r = fmaf(v, k, -t) + v * -1.92596299e-8f;
+  const float e = __builtin_amdgcn_exp2f(t);
+  return v * __builtin_amdgcn_rcpf(1.f + fmaf(e, r * 0.693147181f, e));
+}
 
 template <class T, int KIND, int GPS, int MTW, int NTW>
 __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2)))
@@ -170,8 +202,8 @@ void w4_tiles_kernel(W4Args g, W4Tiles o) {
   constexpr int R = S::R;
   constexpr bool FOLD = KIND == kMxfp4 && T::code == MI355Q_BF16;
   constexpr int PER = kSlices / GPS;                 // MFMAs per group
-  __shared__ __attribute__((aligned(16))) char ring[2 * S::SLOT];
-  __shared__ int64_t x_row[R];                       // -1: a row that is not there
+  constexpr int WSTEP = NTW * 2048;                  // bytes of a wave's codes of a step
+  __shared__ __attribute__((aligned(16))) char ring[S::W + kWaves * WSTEP];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int ln = lane & 31, h = lane >> 5;
 
@@ -199,12 +231,12 @@ void w4_tiles_kernel(W4Args g, W4Tiles o) {
         if (n0 + c < width) store(tile.first + r, n0 + c, 0.f);
     return;
   }
-  for (int r = threadIdx.x; r < R; r += 64 * kWaves) {
+  // row of x behind row r of the tile, -1: a row that is not there
+  auto x_row = [&](int r) __attribute__((always_inline)) {
     int64_t row = tile.first + r;
     if (g.rows && r < tile.count) row = g.rows[row];
-    x_row[r] = r < tile.count && row >= 0 && row < g.n_x ? row : -1;
-  }
-  __syncthreads();
+    return r < tile.count && row >= 0 && row < g.n_x ? row : (int64_t)-1;
+  };
 
   // DMA: instruction q of a step fills 16 rows' 64 bytes; lane l the place l & 3 of row l / 4, with the
   // row's chunk (l & 3) ^ (row / 4 & 3).  Rows that are not there read another row (their results are
@@ -216,7 +248,7 @@ void w4_tiles_kernel(W4Args g, W4Tiles o) {
   const int chunk = (lane & 3) ^ ((lane >> 4) & 3);
 #pragma unroll
   for (int i = 0; i < NR; ++i) {
-    const int64_t row = x_row[((wave * S::NI + 4 * i) >> 2) * 16 + (lane >> 2)];
+    const int64_t row = x_row(((wave * S::NI + 4 * i) >> 2) * 16 + (lane >> 2));
     xo[i] = (uint32_t)((row < 0 ? x0 : row) - x0) * (uint32_t)(2 * g.ldx) + 16 * chunk;
   }
   const char* const xb = reinterpret_cast<const char*>(g.x + x0 * g.ldx);
@@ -251,48 +283,51 @@ void w4_tiles_kernel(W4Args g, W4Tiles o) {
     return *reinterpret_cast<const u32x4_t*>(ring + (j >> 1) * (R * 64) + b * 2048 + ra[j & 1]);
   };
 
-  // weights: lane l has column l & 31 of every tile, 16 bytes each at 16 (l / 32) of both halves of the step
-  uint32_t wo[NTW], wn[NTW];
+  // weights: each wave's 32 NTW columns, 64 bytes a step, go through its own part of LDS the same way: an
+  // instruction fills 16 columns, and a lane reads its column's 16 bytes at 16 (l / 32) of both halves of the
+  // step.  (32-bit offsets everywhere: 64-bit addresses would not fit into the registers.)
+  const uint8_t* const wb = g.w + tile.expert * g.stride_w;
+  const uint32_t lw = l0 + S::W + wave * WSTEP;
+  const char* const w_slot = ring + S::W + wave * WSTEP;
+  auto clamped = [&](int64_t n, int a) __attribute__((always_inline)) {
+    const int64_t limit = g.gated && column(a) < half ? half : g.out;
+    return (uint32_t)(n < limit ? n : limit - 1);                     // columns past the end are not stored
+  };
+  uint32_t wo[NTW][2], wn[NTW];
 #pragma unroll
   for (int a = 0; a < NTW; ++a) {
-    const int64_t limit = g.gated && column(a) < half ? half : g.out, n = column(a) + ln;
-    const int64_t c = n < limit ? n : limit - 1;
-    wn[a] = (uint32_t)c;
-    wo[a] = (uint32_t)(c * g.ldw) + 16 * h;
+    wn[a] = clamped(column(a) + ln, a);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      wo[a][i] = clamped(column(a) + 16 * i + (lane >> 2), a) * (uint32_t)g.ldw + 16 * chunk;
   }
-  // (buffer loads: a 32-bit offset per lane)
-  const uint8_t* const wb = g.w + tile.expert * g.stride_w;
-  const auto w_rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(wb), 0, 0xffffffffu, 0x00020000);
-  const auto s_rsrc = __builtin_amdgcn_make_buffer_rsrc(
-      const_cast<float*>(o.scales) + (size_t)tile.expert * o.padded * g.out, 0, 0xffffffffu, 0x00020000);
-  const int words = KIND == kMxfp4 ? (int)(g.cols / 8) : (int)((g.cols + 7) / 8);
-  struct Raw {
-    u32x4_t w[NTW][2];
-    float s[NTW][GPS];
-  };
-  auto load_w = [&](Raw& r, int s, auto full) __attribute__((always_inline)) {
+  auto dma_w = [&](int s) __attribute__((always_inline)) {
 #pragma unroll
     for (int a = 0; a < NTW; ++a)
 #pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        if (decltype(full)::value || s < whole) {
-          r.w[a][b] = __builtin_bit_cast(
-              u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(w_rsrc, wo[a], s * (kStep / 2) + 32 * b, 0));
-        } else {
-          const int last = words - s * (kStep / 8) - 8 * b - 4 * h;
+      for (int i = 0; i < 2; ++i) dma16(wo[a][i], wb + (int64_t)s * (kStep / 2), lw + a * 2048 + i * 1024);
+  };
+  const auto s_rsrc = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<float*>(o.scales) + (size_t)tile.expert * o.padded * g.out, 0, 0xffffffffu, 0x00020000);
+  const int words = KIND == kMxfp4 ? (int)(g.cols / 8) : (int)((g.cols + 7) / 8);
+  // the codes of a step that is shorter than the others, zeros past the last column
+  auto last_w = [&](int s, int a, int b) __attribute__((always_inline)) {
+    u32x4_t v;
+    const uint8_t* const p = wb + (size_t)wn[a] * g.ldw + (int64_t)s * (kStep / 2) + 32 * b + 16 * h;
+    const int last = words - s * (kStep / 8) - 8 * b - 4 * h;
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            r.w[a][b][i] = i < last ? *reinterpret_cast<const uint32_t*>(wb + (int64_t)s * (kStep / 2) + 32 * b + wo[a] +
-                                                                         4 * i) : 0u;
-        }
-      }
+    for (int i = 0; i < 4; ++i) v[i] = i < last ? reinterpret_cast<const uint32_t*>(p)[i] : 0u;
+    return v;
+  };
+  auto load_s = [&](float (&v)[NTW][GPS], int s) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < GPS; ++i)
 #pragma unroll
       for (int a = 0; a < NTW; ++a)
-        r.s[a][i] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(
+        v[a][i] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(
             s_rsrc, 4 * wn[a], (GPS == 1 ? div((uint32_t)s, g.per) : (uint32_t)s * GPS + i) * (uint32_t)(4 * g.out), 0));
   };
+
   // (floats, not the MFMAs' tuples of 16, unless an MFMA adds to them)
   struct Floats {
     float v[16];
@@ -307,73 +342,86 @@ void w4_tiles_kernel(W4Args g, W4Tiles o) {
       for (int e = 0; e < 16; ++e) acc[b][a][e] = 0.f;
 
   dma(0, 0, std::false_type{});
+  if (whole) dma_w(0);
   if constexpr (KIND != kMxfp4) {
     // the zero points' part: sums of x [m][g] times -s z [n][g], 16 groups at a time
-    const uint16_t* fp[NTW];
-    const uint16_t* sp[MTW];
-#pragma unroll
-    for (int a = 0; a < NTW; ++a)
-      fp[a] = o.factors + ((size_t)tile.expert * g.out + wn[a]) * 3 * o.padded + 8 * h;
 #pragma unroll
     for (int b = 0; b < MTW; ++b) {
-      const int64_t row = x_row[32 * b + ln];
-      sp[b] = o.sums + (size_t)(row < 0 ? 0 : row) * 3 * o.padded + 8 * h;
-    }
-    for (uint32_t g0 = 0; g0 < o.padded; g0 += 16) {
-      u32x4_t f[NTW][3];
+      const int64_t row = x_row(32 * b + ln);
+      const uint16_t* const sp = o.sums + (size_t)(row < 0 ? 0 : row) * 3 * o.padded + 8 * h;
+      f32x16_t p[NTW];
 #pragma unroll
       for (int a = 0; a < NTW; ++a)
 #pragma unroll
-        for (int i = 0; i < 3; ++i) f[a][i] = *reinterpret_cast<const u32x4_t*>(fp[a] + g0 + (size_t)i * o.padded);
+        for (int e = 0; e < 16; ++e) p[a][e] = 0.f;
+      for (uint32_t g0 = 0; g0 < o.padded; g0 += 16) {
+        u32x4_t f[NTW][3], v[3];
 #pragma unroll
-      for (int b = 0; b < MTW; ++b) {
-        u32x4_t v[3];
-#pragma unroll
-        for (int i = 0; i < 3; ++i) v[i] = *reinterpret_cast<const u32x4_t*>(sp[b] + g0 + (size_t)i * o.padded);
+        for (int i = 0; i < 3; ++i) v[i] = *reinterpret_cast<const u32x4_t*>(sp + g0 + (size_t)i * o.padded);
 #pragma unroll
         for (int a = 0; a < NTW; ++a) {
-          f32x16_t p = {};
+          const uint16_t* const fp = o.factors + ((size_t)tile.expert * g.out + wn[a]) * 3 * o.padded + 8 * h + g0;
 #pragma unroll
-          for (int i = 0; i < 3; ++i) p = mfma32<Bf16>(v[i], f[a][0], p);
-          if (o.pieces > 1) {
-            p = mfma32<Bf16>(v[0], f[a][1], p);
-            p = mfma32<Bf16>(v[1], f[a][1], p);
-            p = mfma32<Bf16>(v[0], f[a][2], p);
+          for (int i = 0; i < 3; ++i) f[a][i] = *reinterpret_cast<const u32x4_t*>(fp + (size_t)i * o.padded);
+        }
+#pragma unroll
+        for (int i = 0; i < 3; ++i)
+#pragma unroll
+          for (int a = 0; a < NTW; ++a) p[a] = mfma32<Bf16>(v[i], f[a][0], p[a]);
+        if (o.pieces > 1) {
+#pragma unroll
+          for (int a = 0; a < NTW; ++a) {
+            p[a] = mfma32<Bf16>(v[0], f[a][1], p[a]);
+            p[a] = mfma32<Bf16>(v[1], f[a][1], p[a]);
+            p[a] = mfma32<Bf16>(v[0], f[a][2], p[a]);
           }
-#pragma unroll
-          for (int e = 0; e < 16; ++e) acc[b][a][e] += p[e];
         }
       }
+#pragma unroll
+      for (int a = 0; a < NTW; ++a)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[b][a][e] = p[a][e];
     }
   }
-  Raw raw;
-  load_w(raw, 0, std::false_type{});
+  float next[NTW][GPS];
+  load_s(next, 0);
   // Step s; `full`: the next one is a whole step (no branches then: the order of the loop's
   // instructions is kept).
   auto step = [&](int s, auto full) __attribute__((always_inline)) {
     constexpr bool FULL = decltype(full)::value;
     const int slot = s & 1;
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");   // the step is here, the other slot read
-    // what was loaded is used, and so waited for by the compiler's count, before the DMA that it does not count
-    uint32_t w[NTW][kSlices];
     float sc[NTW][GPS];
+    u32x4_t raw[NTW][2];
 #pragma unroll
     for (int a = 0; a < NTW; ++a) {
 #pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        // words 0 and 1 of both halves of the wave are slices 0 and 2, words 2 and 3 slices 1 and 3
-        const auto u = __builtin_amdgcn_permlane32_swap(raw.w[a][b][0], raw.w[a][b][1], false, false);
-        const auto v = __builtin_amdgcn_permlane32_swap(raw.w[a][b][2], raw.w[a][b][3], false, false);
-        w[a][4 * b] = u[0], w[a][4 * b + 1] = v[0], w[a][4 * b + 2] = u[1], w[a][4 * b + 3] = v[1];
-      }
+      for (int b = 0; b < 2; ++b)
+        raw[a][b] = FULL || s < whole ? *reinterpret_cast<const u32x4_t*>(w_slot + a * 2048 + (ra[b] & (S::SLOT - 1)))
+                                      : last_w(s, a, b);
 #pragma unroll
       for (int i = 0; i < GPS; ++i) {
-        sc[a][i] = raw.s[a][i];
-        asm volatile("" : "+v"(sc[a][i]));
+        sc[a][i] = next[a][i];
+        asm volatile("" : "+v"(sc[a][i]));   // waited for before the DMA, which the compiler does not count
       }
     }
+    uint32_t w[NTW][kSlices];
+#pragma unroll
+    for (int a = 0; a < NTW; ++a)
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        // words 0 and 1 of both halves of the wave are slices 0 and 2, words 2 and 3 slices 1 and 3
+        const auto u = __builtin_amdgcn_permlane32_swap(raw[a][b][0], raw[a][b][1], false, false);
+        const auto v = __builtin_amdgcn_permlane32_swap(raw[a][b][2], raw[a][b][3], false, false);
+        w[a][4 * b] = u[0], w[a][4 * b + 1] = v[0], w[a][4 * b + 2] = u[1], w[a][4 * b + 3] = v[1];
+      }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");                      // the codes are read
     __builtin_amdgcn_sched_barrier(0);
-    if (FULL || s + 1 < steps) dma(s + 1, slot ^ 1, full);
+    if (FULL || s + 1 < steps) {
+      dma(s + 1, slot ^ 1, full);
+      if (FULL || s + 1 < whole) dma_w(s + 1);
+      load_s(next, s + 1);
+    }
     u32x4_t q[NTW][kSlices];
 #pragma unroll
     for (int a = 0; a < NTW; ++a)
@@ -411,8 +459,6 @@ void w4_tiles_kernel(W4Args g, W4Tiles o) {
       }
     }
     __builtin_amdgcn_sched_barrier(0);
-    // the next step's weights, when this one's are out of the registers
-    if (FULL || s + 1 < steps) load_w(raw, s + 1, full);
     ra[0] ^= S::SLOT;
     ra[1] ^= S::SLOT;
   };
@@ -420,9 +466,9 @@ void w4_tiles_kernel(W4Args g, W4Tiles o) {
   for (; s + 1 < whole; ++s) step(s, std::true_type{});
   for (; s < steps; ++s) step(s, std::false_type{});
   // a lane has column l & 31 and rows 8 (e / 4) + 4 (l / 32) + e % 4
+  if (g.bias) {
 #pragma unroll
-  for (int a = 0; a < NTW; ++a) {
-    if (g.bias) {
+    for (int a = 0; a < NTW; ++a) {
       const int64_t n = column(a) + ln;
       const float bias = n < g.out ? load_any(g.bias, g.bias_type, n) : 0.f;
 #pragma unroll
@@ -431,31 +477,73 @@ void w4_tiles_kernel(W4Args g, W4Tiles o) {
         for (int e = 0; e < 16; ++e) acc[b][a][e] += bias;
     }
   }
+  constexpr int UP = NTW / 2;
+  if constexpr (UP > 0) {
+    if (g.gated) {
 #pragma unroll
-  for (int b = 0; b < MTW; ++b)
+      for (int b = 0; b < MTW; ++b)
 #pragma unroll
-    for (int a = 0; a < NTW; ++a) {
-      if (g.gated && (NTW == 1 || a >= NTW / 2)) continue;
-      const int64_t n = n0 + 32 * a + ln;
+        for (int a = 0; a < UP; ++a)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int r = 32 * b + 8 * (e >> 2) + 4 * h + (e & 3);
-        float v = acc[b][a][e];
-        if constexpr (NTW > 1)
-          if (g.gated) v = v / (1.f + expf(-v)) * acc[b][a + NTW / 2 < NTW ? a + NTW / 2 : 0][e];
-        if (r < tile.count && n < width) store(tile.first + r, n, x_row[r] < 0 ? 0.f : v);
+          for (int e = 0; e < 16; ++e) acc[b][a][e] = silu(acc[b][a][e]) * acc[b][a + UP][e];
+    }
+  }
+  const int tiles = g.gated ? UP : NTW;
+  bool dead = false;                                  // a row that x does not have
+  if (g.rows)
+    for (int r = lane; r < tile.count; r += 64) dead |= x_row(r) < 0;
+  const bool inside = tile.count == R && !__any(dead) && n0 + 32 * tiles <= width;     // all of the wave's part is stored
+  auto store_tiles = [&](auto type) __attribute__((always_inline)) {
+    using O = decltype(type);
+    using raw_t = typename O::raw;
+    raw_t* const y = static_cast<raw_t*>(g.y) + tile.first * g.ldy + n0;
+#pragma unroll
+    for (int b = 0; b < MTW; ++b) {
+      if (inside && sizeof(raw_t) == 2) {
+        // pairs of columns: the even lanes take the even rows of both, the odd lanes the odd ones
+        const bool odd = lane & 1;
+        char* const at = reinterpret_cast<char*>(y + (32 * b + 4 * h + (lane & 1)) * g.ldy + (ln & ~1));
+#pragma unroll
+        for (int a = 0; a < NTW; ++a) {
+          if (a >= tiles) continue;
+#pragma unroll
+          for (int e = 0; e < 16; e += 2) {
+            const float mine = acc[b][a][e], below = acc[b][a][e + 1];
+            const float got = __uint_as_float((uint32_t)__builtin_amdgcn_mov_dpp(
+                (int)__float_as_uint(odd ? mine : below), 0xb1, 0xf, 0xf, true));   // the neighbour's
+            const uint32_t lo = O::store(odd ? got : mine), hi = O::store(odd ? below : got);
+            const uint32_t v = lo | hi << 16;
+            __builtin_memcpy(at + ((8 * (e >> 2) + (e & 3)) * g.ldy + 32 * a) * 2, &v, 4);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int a = 0; a < NTW; ++a) {
+          if (a >= tiles || n0 + 32 * a + ln >= width) continue;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int r = 32 * b + 8 * (e >> 2) + 4 * h + (e & 3);
+            if (r < tile.count) y[(int64_t)r * g.ldy + 32 * a + ln] = x_row(r) < 0 ? raw_t(0) : O::store(acc[b][a][e]);
+          }
+        }
       }
     }
+  };
+  if (g.y_type == MI355Q_BF16) store_tiles(Bf16{});
+  else if (g.y_type == MI355Q_F16) store_tiles(F16{});
+  else store_tiles(F32{});
 }
 
 // ---------------------------------------------------------------- launches
-bool w4_tiles_fit(const W4Args& g) {
+static bool w_in_place(const W4Args& g) { return aligned16(g.w) && g.ldw % 16 == 0 && g.stride_w % 16 == 0; }
+bool w4_tiles_fit(const W4Args& g, int kind) {
+  const int64_t row_bytes = kind == kMxfp4 ? g.cols / 2 : (g.cols + 7) / 8 * 4;
   // 32-bit offsets: of a tile's rows (all of x's where they are gathered), of a weight's rows and scales
   const int64_t span = g.rows ? g.n_x : 128;
   const int64_t limit = (int64_t)1 << 32;
   const int64_t steps = (g.cols + kStep - 1) / kStep * kStep;
   const int64_t pitch = g.ldx > steps ? g.ldx : steps;
-  return span < limit / (2 * pitch) && g.out < limit / g.ldw &&
+  return span < limit / (2 * pitch) && g.out < limit / (g.ldw + 16) && (w_in_place(g) || row_bytes % 16) &&
          g.out < limit / (4 * (int64_t)((g.groups + 15) / 16 * 16));
 }
 
@@ -469,10 +557,15 @@ static size_t scales_bytes(int64_t rows_w, uint32_t groups) {
   return ((size_t)rows_w * ((groups + 15) / 16 * 16) * sizeof(float) + 255) / 256 * 256;
 }
 
-size_t w4_tiles_workspace(int64_t n_x, int64_t rows_w, int64_t cols, uint32_t groups, bool zero_points_enter) {
-  // an x that the DMA cannot read (rows off 16 bytes or of no whole chunks) is copied
-  return (zero_points_enter ? sums_bytes(n_x, groups) + sums_bytes(rows_w, groups) : 0) + scales_bytes(rows_w, groups) +
-         (size_t)n_x * ((cols + kStep - 1) / kStep * kStep) * sizeof(uint16_t);
+static size_t x_copy_bytes(int64_t n_x, int64_t cols) {
+  return (size_t)n_x * ((cols + kStep - 1) / kStep * kStep) * sizeof(uint16_t);
+}
+
+size_t w4_tiles_workspace(int64_t n_x, int64_t rows_w, int64_t cols, uint32_t groups, bool mx) {
+  // operands that the DMA cannot read (rows off 16 bytes or not of whole chunks) are copied
+  const int64_t w_bytes = mx ? cols / 2 : (cols + 7) / 8 * 4;
+  return (mx ? 0 : sums_bytes(n_x, groups) + sums_bytes(rows_w, groups)) + scales_bytes(rows_w, groups) +
+         x_copy_bytes(n_x, cols) + (w_bytes % 16 ? (size_t)rows_w * ((w_bytes + 15) / 16 * 16) : 0);
 }
 
 template <class T, int KIND, int GPS, int MTW, int NTW>
@@ -513,26 +606,34 @@ static int launch_type(W4Args g, int kind, void* workspace, hipStream_t st) {
   at += scales_bytes(g.experts * g.out, g.groups);
   const int64_t ld_copy = (g.cols + kStep - 1) / kStep * kStep;
   if (copy) to = reinterpret_cast<uint16_t*>(at);
+  uint8_t* to_w = nullptr;
+  const int64_t w_bytes = kind == kMxfp4 ? g.cols / 2 : (g.cols + 7) / 8 * 4, w_pitch = (w_bytes + 15) / 16 * 16;
+  if (w_bytes % 16) {
+    if (copy) at += x_copy_bytes(g.n_x, g.cols);
+    to_w = reinterpret_cast<uint8_t*>(at);
+  }
   const W4Tiles o = {to_sums, to_factors, to_scales, padded, kind == kInt4 && g.s_type == MI355Q_BF16 ? 1 : 3, 0, 0};
   int lanes = 0;
   while (lanes < 6 && (8 << lanes) < g.group) ++lanes;
   const uint64_t parts = (padded + (64u >> lanes) - 1) / (64u >> lanes);
   const uint64_t x_blocks = copy || sums ? (parts * (uint64_t)g.n_x + 3) / 4 : 0;
-  const uint64_t w_blocks = (uint64_t)g.experts * ((g.out + 31) / 32) * (padded / 8);
-  MQ_CHECK_ARG(x_blocks + w_blocks <= UINT32_MAX / 256, "w4a16_matmul: %lld rows of x and %lld of weights are too many",
-               (long long)g.n_x, (long long)(g.experts * g.out));
-  const dim3 grid((unsigned)(x_blocks + w_blocks)), block(256);
-  auto* const s_out = reinterpret_cast<uint32_t*>(to_scales);
-  if (kind == kInt4Zero)
-    hipLaunchKernelGGL((w4_prepare_kernel<T, kInt4Zero>), grid, block, 0, st, g, padded, lanes, (uint32_t)x_blocks,
-                       to_sums, to_factors, s_out, to, ld_copy);
-  else if (kind == kInt4)
-    hipLaunchKernelGGL((w4_prepare_kernel<T, kInt4>), grid, block, 0, st, g, padded, lanes, (uint32_t)x_blocks, to_sums,
-                       to_factors, s_out, to, ld_copy);
-  else
-    hipLaunchKernelGGL((w4_prepare_kernel<T, kMxfp4>), grid, block, 0, st, g, padded, lanes, (uint32_t)x_blocks,
-                       to_sums, to_factors, s_out, to, ld_copy);
+  const uint64_t f_blocks = (uint64_t)g.experts * ((g.out + 31) / 32) * (padded / 8);
+  const uint64_t c_blocks = to_w ? ((uint64_t)g.experts * g.out * (w_pitch / 16) + 255) / 256 : 0;
+  MQ_CHECK_ARG(x_blocks + f_blocks + c_blocks <= UINT32_MAX / 256,
+               "w4a16_matmul: %lld rows of x and %lld of weights are too many", (long long)g.n_x,
+               (long long)(g.experts * g.out));
+  const W4Prepare p = {padded, lanes, (uint32_t)x_blocks, (uint32_t)f_blocks, to_sums, to_factors,
+                       reinterpret_cast<uint32_t*>(to_scales), to, ld_copy, to_w, w_bytes};
+  const dim3 grid((unsigned)(x_blocks + f_blocks + c_blocks)), block(256);
+  if (kind == kInt4Zero) hipLaunchKernelGGL((w4_prepare_kernel<T, kInt4Zero>), grid, block, 0, st, g, p);
+  else if (kind == kInt4) hipLaunchKernelGGL((w4_prepare_kernel<T, kInt4>), grid, block, 0, st, g, p);
+  else hipLaunchKernelGGL((w4_prepare_kernel<T, kMxfp4>), grid, block, 0, st, g, p);
   MQ_LAUNCH_CHECK();
+  if (to_w) {
+    g.w = to_w;
+    g.ldw = w_pitch;
+    g.stride_w = g.out * w_pitch;
+  }
   if (copy) {
     g.x = to;
     g.ldx = ld_copy;

@@ -1113,9 +1113,6 @@ def _w4_matmul(x, index, offsets, experts, n_rows, weight_packed, weight_scale, 
             raise ValueError("MXFP4 weights have no zero points")
         group, groups = 32, cols // 32
         w, ldw, stride_w = _w4_operand(weight_packed, (*first, out, cols // 2), (torch.uint8,), "weight_packed", lead)
-        if ldw % 4 or stride_w % 4 or w.data_ptr() % 4:
-            w = w.clone(memory_format=torch.contiguous_format)
-            ldw, stride_w = cols // 2, out * (cols // 2)
         s, lds, stride_s = _w4_operand(weight_scale, (*first, out, groups), (torch.uint8, torch.float8_e8m0fnu),
                                        "weight_scale", lead)
         s_kind = L.BF16
@@ -1129,6 +1126,11 @@ def _w4_matmul(x, index, offsets, experts, n_rows, weight_packed, weight_scale, 
         ldw, stride_w = 4 * ldw, 4 * stride_w
         s, lds, stride_s = _w4_operand(weight_scale, (*first, out, groups), tuple(_FP8_DT), "weight_scale", lead)
         s_kind = _FP8_DT[s.dtype]
+    wide = (cols // 2 if mx else -(-cols // 8) * 4)
+    if (ldw % 16 or stride_w % 16 or w.data_ptr() % 16) and (wide % 16 == 0 or w.data_ptr() % 4 or ldw % 4):
+        # rows of whole 16-byte chunks that do not lie on 16-byte boundaries
+        w = w.clone(memory_format=torch.contiguous_format)
+        ldw, stride_w = wide, out * wide
     here, z_ptr, ldz, stride_z, b_ptr, b_kind = x.get_device(), None, 0, 0, None, 0
     z = b = None
     if weight_zero_point is not None:
