@@ -667,8 +667,8 @@ int mi355q_moe_combine_backward(const void* dy_dev, mi355q_dtype dtype, int64_t 
  * offsets[experts] on are written as zeros.  rows_dev: row of x behind each row of y
  * (NULL: the same row); one that x does not have counts as zeros.
  * A row of x that holds an infinity or a NaN may come out as NaN throughout.
- * workspace (16-byte aligned): the queried size; with less, calls of many rows take a
- * kernel that is made for few. */
+ * workspace (16-byte aligned): the queried size; with less, sums are not split over
+ * workgroups and calls of many rows take a kernel that is made for few. */
 size_t mi355q_w4a16_matmul_workspace_size(int64_t n_x, int64_t rows, int64_t experts, int64_t out, int64_t cols,
                                           mi355q_w4_format format, int64_t group_size);
 int mi355q_w4a16_matmul(const void* x_dev, mi355q_dtype x_dtype, int64_t n_x, int64_t ldx, const int32_t* rows_dev,

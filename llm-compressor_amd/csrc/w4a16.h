@@ -89,6 +89,13 @@ __device__ __forceinline__ u32x4_t e2m1s(uint32_t w, float e) {
                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, e, 2)),
                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, e, 3))};
 }
+__device__ __forceinline__ float silu(float v) {
+  // e^-v = 2^(-v log2 e), with what the product's rounding leaves put back
+  const float k = -1.44269504f, t = v * k, r = fmaf(v, k, -t) + v * -1.92596299e-8f;
+  const float e = __builtin_amdgcn_exp2f(t);
+  return v * __builtin_amdgcn_rcpf(1.f + fmaf(e, r * 0.693147181f, e));
+}
+
 // ---------------------------------------------------------------- tiles of rows
 // The rows [first, first + count) of y that a tile of ROWS rows holds, and their
 // expert (-1: rows behind the last expert's, which are written as zeros).
@@ -96,46 +103,43 @@ struct RowTile {
   int64_t first;
   int count, expert;
 };
-// Tile `id` in the order of experts, each expert's last one shorter; a wave finds it with its lanes taking
-// E / 64 neighbouring experts each.  count = 0: there is no such tile.
+// Tile `id` in the order of experts, each expert's last one shorter; count = 0: there is no such
+// tile.  A wave looks at 64 experts at a time, a lane at one: its tiles, their prefix sums, and the lane
+// whose range holds the tile.  (Whatever the offsets hold, a tile lies within y.)
 template <int ROWS>
 __device__ __forceinline__ RowTile find_row_tile(const W4Args& g, uint32_t id) {
   if (!g.offsets) {
     const int64_t first = (int64_t)id * ROWS, left = g.n_rows - first;
     return {first, (int)(left < ROWS ? left : ROWS), 0};
   }
-  const int lane = threadIdx.x & 63, per = (g.experts + 64) / 64;      // experts and the rows behind them
-  const int e0 = lane * per;
-  // (whatever the offsets hold, a tile lies within y)
+  const int lane = threadIdx.x & 63, n_rows = (int)g.n_rows;
   auto begin = [&](int e) __attribute__((always_inline)) {
-    const int64_t o = e <= g.experts ? g.offsets[e] : g.n_rows;
-    return o < 0 ? 0 : o < g.n_rows ? o : g.n_rows;
+    const int64_t o = e <= g.experts ? g.offsets[e] : (int64_t)n_rows;
+    return o < 0 ? 0 : o < n_rows ? (int)o : n_rows;
   };
-  auto size = [&](int e, int64_t& first) __attribute__((always_inline)) {
-    first = begin(e);
-    const int64_t n = begin(e + 1) - first;
-    return n > 0 ? n : 0;
-  };
-  int64_t tiles = 0, first;
-  for (int e = e0; e < e0 + per; ++e) tiles += (size(e, first) + ROWS - 1) / ROWS;
-  int64_t sum = tiles;
+  uint32_t left = id;
+  int a = begin(lane), b = begin(lane + 1);
+  for (int e0 = 0; e0 <= g.experts; e0 += 64) {          // (the rows behind the experts count as one)
+    const int na = begin(e0 + 64 + lane), nb = begin(e0 + 65 + lane);
+    const uint32_t tiles = b > a ? (uint32_t)(b - a + ROWS - 1) / ROWS : 0u;
+    uint32_t sum = tiles;
 #pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int64_t o = __shfl_up(sum, d);
-    if (lane >= d) sum += o;
-  }
-  const uint64_t past = __ballot(sum > (int64_t)id);
-  if (!past) return {0, 0, 0};
-  const int src = __ffsll((unsigned long long)past) - 1;
-  int64_t in = (int64_t)id - __shfl(sum - tiles, src);
-  for (int e = src * per;; ++e) {                       // sum > id: it ends inside src's experts
-    const int64_t n = size(e, first), t = (n + ROWS - 1) / ROWS;
-    if (in < t) {
-      const int64_t left = n - in * ROWS;
-      return {first + in * ROWS, (int)(left < ROWS ? left : ROWS), e < g.experts ? e : -1};
+    for (int d = 1; d < 64; d <<= 1) {
+      const uint32_t o = __shfl_up(sum, d);
+      if (lane >= d) sum += o;
     }
-    in -= t;
+    const uint64_t past = __ballot(sum > left);
+    if (past) {
+      const int src = __builtin_ctzll(past);
+      const int first = __shfl(a, src), end = __shfl(b, src);
+      const int in = (int)(left - __shfl(sum - tiles, src)) * ROWS, rest = end - first - in;
+      return {first + in, rest < ROWS ? rest : ROWS, e0 + src < g.experts ? e0 + src : -1};
+    }
+    left -= __shfl(sum, 63);
+    a = na;
+    b = nb;
   }
+  return {0, 0, 0};
 }
 // the same in scalar registers
 template <int ROWS>
@@ -145,6 +149,19 @@ __device__ __forceinline__ RowTile row_tile(const W4Args& g, uint32_t id) {
                         (int64_t)__builtin_amdgcn_readfirstlane((int)(t.first >> 32)) << 32;
   return {first, __builtin_amdgcn_readfirstlane(t.count), __builtin_amdgcn_readfirstlane(t.expert)};
 }
+
+// How a call of few rows is cut (w4a16_few.h): rows per tile (16 mt, or 4), column tiles and waves per
+// workgroup, and workgroups that share a sum.
+struct FewPlan {
+  int mt, nt, w;
+  uint32_t splits;
+};
+int launch_w4_few_bf16(const W4Args& g, int kind, const FewPlan& p, float* parts, hipStream_t st);
+int launch_w4_few_f16(const W4Args& g, int kind, const FewPlan& p, float* parts, hipStream_t st);
+int launch_w4_few_zero_bf16(const W4Args& g, const FewPlan& p, float* parts, hipStream_t st);
+int launch_w4_few_zero_f16(const W4Args& g, const FewPlan& p, float* parts, hipStream_t st);
+// y from the parts of the sums
+int join_parts(const W4Args& g, uint32_t splits, const float* parts, hipStream_t st);
 
 // The tile kernels (w4a16_tiles.hip): whether they take a call, the workspace that they
 // ask for, and the launch.

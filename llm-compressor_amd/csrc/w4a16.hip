@@ -1,241 +1,32 @@
-// Products of 16-bit activations with 4-bit weights (w4a16.h).
+// Products of 16-bit activations with 4-bit weights (w4a16.h): which kernel a call takes.
 #include "w4a16.h"
 
 namespace mi355q {
 
-template <class T>
-__device__ __forceinline__ f32x4_t mfma(const u32x4_t& a, const u32x4_t& b, const f32x4_t& c) {
-  if constexpr (T::code == MI355Q_BF16)
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c,
-                                                   0, 0, 0);
-  else
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0,
-                                                  0, 0);
-}
-// A lane holds 16 bytes of a weight's row, the 32 columns from 32 (lane / 16) on;
-// an instruction wants 32 neighbouring columns over the four lanes of a row.  So the
-// words are transposed over registers and quarters of the wave: word i then holds
-// columns 32 i + 8 (lane / 16) and on.
-__device__ __forceinline__ u32x4_t transpose_words(u32x4_t w) {
-  auto a = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false);
-  auto b = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
-  auto c = __builtin_amdgcn_permlane16_swap(a[0], b[0], false, false);
-  auto d = __builtin_amdgcn_permlane16_swap(a[1], b[1], false, false);
-  return u32x4_t{(uint32_t)c[0], (uint32_t)c[1], (uint32_t)d[0], (uint32_t)d[1]};
-}
-
-// The eight elements at p of which `left` are inside a row of eight or more, zeros
-// for the others: the row's last eight, shifted down.
-__device__ __forceinline__ u32x4_t last_chunk(const uint16_t* p, int64_t left) {
-  uint64_t v[2] = {0, 0};
-  if (left <= 0) return u32x4_t{0u, 0u, 0u, 0u};
-  const int n = left < 8 ? 8 - (int)left : 0;
-  __builtin_memcpy(v, p - n, 16);
-  if (n >= 4) v[0] = v[1], v[1] = 0;
-  const int bits = 16 * (n & 3);
-  v[0] = (v[0] >> bits) | (v[1] << 1 << (63 - bits));
-  v[1] >>= bits;
-  return u32x4_t{(uint32_t)v[0], (uint32_t)(v[0] >> 32), (uint32_t)v[1], (uint32_t)(v[1] >> 32)};
+// y from the parts of the sums, added in the order of the splits.  A thread takes a column of a row.
+__global__ __launch_bounds__(256) void w4_join_kernel(W4Args g, uint32_t splits, const float* parts) {
+  const int64_t half = g.out / 2, width = g.gated ? half : g.out;
+  const uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t row = (int64_t)(i / (uint64_t)width), n = (int64_t)(i % (uint64_t)width);
+  if (row >= g.n_rows) return;
+  auto total = [&](int64_t c) __attribute__((always_inline)) {
+    const float* p = parts + row * g.out + c;
+    float v = 0.f;
+#pragma unroll 4
+    for (uint32_t s = 0; s < splits; ++s) v += p[(size_t)s * g.n_rows * g.out];
+    return g.bias ? v + load_any(g.bias, g.bias_type, c) : v;
+  };
+  float v = total(n);
+  if (g.gated) v = silu(v) * total(half + n);
+  const int64_t at = row * g.ldy + n;
+  if (g.y_type == MI355Q_F32) static_cast<float*>(g.y)[at] = v;
+  else static_cast<uint16_t*>(g.y)[at] = g.y_type == MI355Q_BF16 ? Bf16::store(v) : F16::store(v);
 }
 
-// ---------------------------------------------------------------- few rows
-// 16 MT rows of y times 16 NT columns per workgroup; its W waves take every W-th
-// step of 128 columns, straight from memory into the MFMAs' registers (x: rows,
-// w: columns; a lane's sums are one column's), and join their sums in LDS.
-template <class T, int KIND, int GPS, int MT, int NT, int W, int D>
-__global__ __launch_bounds__(64 * W) void w4_few_kernel(W4Args g, uint32_t nt) {
-  constexpr bool FOLD = KIND == kMxfp4 && T::code == MI355Q_BF16;     // the scale is in the operand
-  __shared__ f32x4_t sums[W][NT][MT][64];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int col = lane & 15, quarter = lane >> 4;
-  const RowTile tile = row_tile<16 * MT>(g, blockIdx.x / nt);
-  if (tile.count <= 0) return;
-  const int64_t half = g.gated ? g.out / 2 : 0, width = g.gated ? half : g.out;   // of y
-  const int64_t n0 = (int64_t)(blockIdx.x % nt) * 16 * (g.gated ? NT / 2 : NT);
-  // column of tile a on this lane: the second half of a gated weight's tiles holds its second half
-  auto column = [&](int a) __attribute__((always_inline)) {
-    return g.gated && a >= NT / 2 ? half + n0 + 16 * (a - NT / 2) : n0 + 16 * a;
-  };
-  const int steps = tile.expert < 0 ? 0 : (int)((g.cols + kStep - 1) / kStep);
-  const uint8_t* wp[NT];
-  int64_t sp[NT], zp[NT];
-  int zs[NT];
-#pragma unroll
-  for (int a = 0; a < NT; ++a) {
-    const int64_t limit = g.gated && a < NT / 2 ? half : g.out;
-    int64_t n = column(a) + col;
-    n = n < limit ? n : limit - 1;                                   // the columns past the end are not stored
-    const int64_t e = tile.expert < 0 ? 0 : tile.expert;
-    wp[a] = g.w + e * g.stride_w + n * g.ldw + 16 * quarter;
-    sp[a] = e * g.stride_s + n * g.lds;
-    zp[a] = e * g.stride_z + n / 8 * g.ldz;
-    zs[a] = 4 * (int)(n % 8);
-  }
-  const uint16_t* xp[MT];
-  bool live[MT];
-#pragma unroll
-  for (int b = 0; b < MT; ++b) {
-    const int r = 16 * b + col;
-    int64_t row = tile.first + (r < tile.count ? r : 0);
-    if (g.rows) row = g.rows[row];
-    live[b] = r < tile.count && row >= 0 && row < g.n_x;             // a row that x does not have counts as zeros
-    xp[b] = g.x + (live[b] ? row : 0) * g.ldx + 8 * quarter;
-  }
-  f32x4_t acc[NT][MT];
-#pragma unroll
-  for (int a = 0; a < NT; ++a)
-#pragma unroll
-    for (int b = 0; b < MT; ++b) acc[a][b] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-
-  struct Step {
-    u32x4_t w[NT], x[MT][4];
-    float s[NT][GPS];
-    uint32_t z[NT][GPS];
-  };
-  const int64_t bytes = (g.cols + 1) / 2, words = KIND == kMxfp4 ? bytes / 4 : (g.cols + 7) / 8;
-  auto load = [&](Step& o, int s) __attribute__((always_inline)) {
-    const int64_t k0 = (int64_t)s * kStep;
-    const bool whole = k0 + kStep <= g.cols;
-#pragma unroll
-    for (int a = 0; a < NT; ++a) {
-      if (whole) {
-        __builtin_memcpy(&o.w[a], wp[a] + k0 / 2, 16);
-      } else {
-        const int64_t left = words - k0 / 8 - 4 * quarter;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          o.w[a][i] = i < left ? *reinterpret_cast<const uint32_t*>(wp[a] + k0 / 2 + 4 * i) : 0u;
-      }
-#pragma unroll
-      for (int i = 0; i < GPS; ++i) {
-        const uint32_t gs = GPS == 1 ? div((uint32_t)s, g.per) : (uint32_t)s * GPS + i;
-        const uint32_t gi = gs < g.groups ? gs : g.groups - 1;        // (groups behind the last column)
-        if constexpr (KIND == kMxfp4) {
-          const uint32_t e = static_cast<const uint8_t*>(g.s)[sp[a] + gi];
-          o.s[a][i] = FOLD ? __uint_as_float((e << 23) | 0x00400000u) : e8m0_to_f32(e);
-        } else {
-          o.s[a][i] = load_any(g.s, g.s_type, sp[a] + gi);
-        }
-        if constexpr (KIND == kInt4Zero) o.z[a][i] = g.z[zp[a] + gi];
-      }
-    }
-#pragma unroll
-    for (int b = 0; b < MT; ++b)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int64_t k = k0 + 32 * i;
-        if (whole) {
-          o.x[b][i] = u32x4_t{0u, 0u, 0u, 0u};
-          if (live[b]) __builtin_memcpy(&o.x[b][i], xp[b] + k, 16);
-        } else {
-          o.x[b][i] = last_chunk(xp[b] + k, live[b] ? g.cols - k - 8 * quarter : 0);
-        }
-      }
-  };
-  constexpr uint32_t one = T::code == MI355Q_BF16 ? 0x3f803f80u : 0x3c003c00u;
-  constexpr uint32_t minus8 = T::code == MI355Q_BF16 ? 0xc100c100u : 0xc800c800u;
-  constexpr uint32_t unit = KIND == kInt4 ? minus8 : one;
-  const u32x4_t units = {unit, unit, unit, unit};
-  auto use = [&](const Step& o) __attribute__((always_inline)) {
-    constexpr int PER = 4 / GPS;                                   // instructions per group
-    u32x4_t q[NT][4];
-#pragma unroll
-    for (int a = 0; a < NT; ++a) {
-      const u32x4_t w = transpose_words(o.w[a]);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if constexpr (KIND == kMxfp4) q[a][i] = e2m1s<T>(w[i], FOLD ? o.s[a][i * GPS / 4] : 1.f);
-        else q[a][i] = nibbles<T>(w[i]);
-      }
-    }
-#pragma unroll
-    for (int b = 0; b < MT; ++b)
-#pragma unroll
-      for (int i = 0; i < GPS; ++i) {
-        f32x4_t base = {0.f, 0.f, 0.f, 0.f};
-        if constexpr (KIND != kMxfp4) {
-#pragma unroll
-          for (int j = 0; j < PER; ++j) base = mfma<T>(o.x[b][i * PER + j], units, base);
-        }
-#pragma unroll
-        for (int a = 0; a < NT; ++a) {
-          if constexpr (FOLD) {
-#pragma unroll
-            for (int j = 0; j < PER; ++j) acc[a][b] = mfma<T>(o.x[b][i * PER + j], q[a][i * PER + j], acc[a][b]);
-          } else {
-            f32x4_t t = base;
-            if constexpr (KIND == kInt4Zero) {
-              const float z = -(float)((o.z[a][i] >> zs[a]) & 15u);
-#pragma unroll
-              for (int r = 0; r < 4; ++r) t[r] = base[r] * z;
-            }
-#pragma unroll
-            for (int j = 0; j < PER; ++j) t = mfma<T>(o.x[b][i * PER + j], q[a][i * PER + j], t);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) acc[a][b][r] = fmaf(t[r], o.s[a][i], acc[a][b][r]);
-          }
-        }
-      }
-  };
-  for (int s0 = wave; s0 < steps; s0 += W * D) {
-    Step o[D];
-#pragma unroll
-    for (int d = 0; d < D; ++d)
-      if (s0 + d * W < steps) load(o[d], s0 + d * W);
-#pragma unroll
-    for (int d = 0; d < D; ++d)
-      if (s0 + d * W < steps) use(o[d]);
-  }
-#pragma unroll
-  for (int a = 0; a < NT; ++a)
-#pragma unroll
-    for (int b = 0; b < MT; ++b) sums[wave][a][b][lane] = acc[a][b];
-  __syncthreads();
-  auto total = [&](int a, int b) __attribute__((always_inline)) {
-    f32x4_t v = sums[0][a][b][lane];
-#pragma unroll
-    for (int w = 1; w < W; ++w) v += sums[w][a][b][lane];
-    const int64_t n = column(a) + col;
-    if (g.bias && n < g.out) {
-      const float bias = load_any(g.bias, g.bias_type, n);
-#pragma unroll
-      for (int r = 0; r < 4; ++r) v[r] += bias;
-    }
-    return v;
-  };
-  for (int i = wave; i < (g.gated ? NT / 2 : NT) * MT; i += W) {
-    const int a = i / MT, b = i % MT;
-    f32x4_t v = total(a, b);
-    if (g.gated) {
-      const f32x4_t up = total(a + NT / 2, b);
-#pragma unroll
-      for (int r = 0; r < 4; ++r) v[r] = v[r] / (1.f + expf(-v[r])) * up[r];
-    }
-    const int64_t n = n0 + 16 * a + col;
-    if (n >= width) continue;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int row = 16 * b + 4 * quarter + r;
-      if (row >= tile.count) continue;
-      const int64_t at = (tile.first + row) * g.ldy + n;
-      if (g.y_type == MI355Q_F32) static_cast<float*>(g.y)[at] = v[r];
-      else static_cast<uint16_t*>(g.y)[at] = g.y_type == MI355Q_BF16 ? Bf16::store(v[r]) : F16::store(v[r]);
-    }
-  }
-}
-
-template <class T, int KIND, int GPS, int MT, int NT, int W, int D>
-static int launch_few(const W4Args& g, hipStream_t st) {
-  const int64_t width = g.gated ? g.out / 2 : g.out, per = 16 * (g.gated ? NT / 2 : NT);
-  const int64_t nt = (width + per - 1) / per;
-  // an expert's last tile may be short: no more tiles than rows, and at most one short one per expert
-  // (and one behind them)
-  int64_t mt = (g.n_rows + 16 * MT - 1) / (16 * MT);
-  if (g.offsets) mt = g.n_rows / (16 * MT) + g.experts + 1 < g.n_rows ? g.n_rows / (16 * MT) + g.experts + 1 : g.n_rows;
-  MQ_CHECK_ARG(nt * mt <= (int64_t)(UINT32_MAX / (64 * W)), "w4a16: %lld rows by %lld columns are too many",
-               (long long)g.n_rows, (long long)width);
-  hipLaunchKernelGGL((w4_few_kernel<T, KIND, GPS, MT, NT, W, D>), dim3((unsigned)(nt * mt)), dim3(64 * W), 0, st, g,
-                     (uint32_t)nt);
+int join_parts(const W4Args& g, uint32_t splits, const float* parts, hipStream_t st) {
+  const int64_t width = g.gated ? g.out / 2 : g.out;
+  hipLaunchKernelGGL(w4_join_kernel, dim3((unsigned)((g.n_rows * width + 255) / 256)), dim3(256), 0, st, g, splits,
+                     parts);
   MQ_LAUNCH_CHECK();
   return MI355Q_OK;
 }
@@ -243,35 +34,50 @@ static int launch_few(const W4Args& g, hipStream_t st) {
 // Up to this many rows (per expert, in the mean) the weight's bytes decide.
 static bool few_rows(int64_t rows, int64_t experts) { return rows <= 64 * experts; }
 
-template <class T, int KIND, int GPS>
-static int launch_kind(const W4Args& g, hipStream_t st) {
-  const int64_t rows = g.offsets ? (g.n_rows + g.experts - 1) / g.experts : g.n_rows;     // per expert, in the mean
-  if (rows <= 16) return launch_few<T, KIND, GPS, 1, 2, 8, 2>(g, st);
-  if (rows <= 32) return launch_few<T, KIND, GPS, 2, 2, 4, 2>(g, st);
-  return launch_few<T, KIND, GPS, 4, 2, 4, 1>(g, st);
-}
-
-template <class T>
-static int launch_type(const W4Args& g, int kind, hipStream_t st) {
-  if (kind == kMxfp4) return launch_kind<T, kMxfp4, 4>(g, st);
-  if (kind == kInt4) {
-    if (g.groups > 1 && g.group == 32) return launch_kind<T, kInt4, 4>(g, st);
-    if (g.groups > 1 && g.group == 64) return launch_kind<T, kInt4, 2>(g, st);
-    return launch_kind<T, kInt4, 1>(g, st);
+// Rows per tile (4 or 16 mt), columns, waves and splits of a call of few rows.
+//
+// A wave's loads are x's and the weight's, and it takes some 2048 waves to keep the memory busy.  Up
+// to 4 rows: one column tile a wave, and as many waves on one tile's sum as make 2048 (14336 x
+// 4096 9.3 us with two, 10.4 with eight; 4096 x 4096 6.2 and 5.1; gated ones have two column tiles, experts_token's
+// 8 x 1536 x 2048 7.8 us).  More rows: x is what is loaded most, so a wave takes up to four column tiles (16 x
+// 14336 x 4096 14.7 us, with two 16.9, with one 22.5), and where that leaves CUs idle the sum is split over
+// workgroups (23 x 4096 x 14336 34 us whole, 21 in four).  Tiles of experts are many: one or two waves each
+// (61 tokens to 8 of 128 experts of 1536 x 2048 54 us, with four waves 85).
+static FewPlan few_plan(int64_t rows, int64_t experts, int64_t out, int64_t cols, bool gated) {
+  const int64_t mean = (rows + experts - 1) / experts, steps = (cols + kStep - 1) / kStep;
+  FewPlan p = {mean <= (experts > 1 ? 1 : 4) ? 0 : mean <= 16 ? 1 : mean <= 32 ? 2 : 4, 1, 8, 1};
+  const int64_t row_tiles = experts > 1 ? (rows < experts ? rows : experts) : (rows + 63) / 64;
+  if (p.mt == 0) {
+    p.nt = gated ? 2 : 1;
+    const int64_t tiles = row_tiles * ((out + 16 * p.nt - 1) / (16 * p.nt));
+    p.w = tiles >= 1024 ? 2 : tiles >= 384 ? 4 : 8;
+  } else if (p.mt == 1) {
+    const int64_t tiles = row_tiles * ((out + 15) / 16);
+    p.nt = tiles >= 768 ? 4 : tiles >= 512 || gated ? 2 : 1;
+    p.w = experts > 1 ? (tiles >= 4096 ? 1 : 4) : p.nt == 1 ? 8 : 4;
+    if (p.w == 1) p.nt = 2;
+  } else {
+    p.nt = 4;
+    const int64_t tiles = row_tiles * ((out + 63) / 64);
+    while (tiles * p.splits < 192 && steps >= 16 * (int64_t)p.splits && p.splits < 16) p.splits *= 2;
   }
-  if (g.groups > 1 && g.group == 32) return launch_kind<T, kInt4Zero, 4>(g, st);
-  if (g.groups > 1 && g.group == 64) return launch_kind<T, kInt4Zero, 2>(g, st);
-  return launch_kind<T, kInt4Zero, 1>(g, st);
+  return p;
 }
 
 }  // namespace mi355q
 
 using namespace mi355q;
 
+// The parts of split sums (`gated` does not split them otherwise).
+static size_t few_bytes(int64_t rows, int64_t experts, int64_t out, int64_t cols) {
+  const uint32_t splits = few_plan(rows, experts, out, cols, false).splits;
+  return splits > 1 ? (size_t)splits * rows * out * sizeof(float) : 0;
+}
+
 extern "C" size_t mi355q_w4a16_matmul_workspace_size(int64_t n_x, int64_t rows, int64_t experts, int64_t out,
                                                      int64_t cols, mi355q_w4_format format, int64_t group_size) {
-  if (n_x <= 0 || rows <= 0 || experts <= 0 || out <= 0 || cols <= 0 || group_size <= 0 || few_rows(rows, experts))
-    return 0;
+  if (n_x <= 0 || rows <= 0 || experts <= 0 || out <= 0 || cols <= 0 || group_size <= 0) return 0;
+  if (few_rows(rows, experts)) return few_bytes(rows, experts, out, cols);
   return w4_tiles_workspace(n_x, experts * out, cols, (uint32_t)((cols + group_size - 1) / group_size), format == MI355Q_W4_MXFP4);
 }
 
@@ -295,6 +101,8 @@ extern "C" int mi355q_w4a16_matmul(const void* x_dev, mi355q_dtype x_dtype, int6
   MQ_CHECK_ARG(cols >= 8, "w4a16_matmul: x must have 8 columns at the least, got %lld", (long long)cols);
   MQ_CHECK_ARG(!gated || out % 2 == 0, "w4a16_matmul: a gated weight has two halves, got %lld rows", (long long)out);
   MQ_CHECK_ARG(offsets_dev || experts == 1, "w4a16_matmul: several experts take offsets");
+  MQ_CHECK_ARG(!offsets_dev || (rows < INT32_MAX && experts < INT32_MAX - 128),
+               "w4a16_matmul: %lld rows of %lld experts are too many", (long long)rows, (long long)experts);
   MQ_CHECK_ARG(rows_dev || n_x >= rows, "w4a16_matmul: x has fewer rows than y (%lld of %lld)", (long long)n_x,
                (long long)rows);
   MQ_CHECK_ARG(!mx || (cols % 32 == 0 && group_size == 32 && !zeros_dev),
@@ -319,5 +127,12 @@ extern "C" int mi355q_w4a16_matmul(const void* x_dev, mi355q_dtype x_dtype, int6
   if (!few_rows(rows, experts) && w4_tiles_fit(g, kind) && workspace_dev && aligned16(workspace_dev) &&
       workspace_bytes >= w4_tiles_workspace(n_x, experts * out, cols, g.groups, mx))
     return launch_w4_tiles(g, x_dtype, kind, workspace_dev, st);
-  return x_dtype == MI355Q_BF16 ? launch_type<Bf16>(g, kind, st) : launch_type<F16>(g, kind, st);
+  FewPlan p = few_plan(rows, experts, out, cols, gated);
+  if (!few_rows(rows, experts) || !workspace_dev || !aligned16(workspace_dev) ||
+      workspace_bytes < few_bytes(rows, experts, out, cols))
+    p.splits = 1;
+  float* const parts = static_cast<float*>(workspace_dev);
+  if (kind == kInt4Zero)
+    return x_dtype == MI355Q_BF16 ? launch_w4_few_zero_bf16(g, p, parts, st) : launch_w4_few_zero_f16(g, p, parts, st);
+  return x_dtype == MI355Q_BF16 ? launch_w4_few_bf16(g, kind, p, parts, st) : launch_w4_few_f16(g, kind, p, parts, st);
 }

@@ -188,12 +188,6 @@ struct TileShape {
   static constexpr int NI = R / 16;                  // DMA instructions per wave and step
   static constexpr int W = 2 * SLOT;                 // where the waves' codes begin
 };
-__device__ __forceinline__ float silu(float v) {
-  // e^-v = 2^(-v log2 e), with what the product's rounding leaves put back
-  const float k = -1.44269504f, t = v * k, r = fmaf(v, k, -t) + v * -1.92596299e-8f;
-  const float e = __builtin_amdgcn_exp2f(t);
-  return v * __builtin_amdgcn_rcpf(1.f + fmaf(e, r * 0.693147181f, e));
-}
 
 template <class T, int KIND, int GPS, int MTW, int NTW>
 __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2)))
