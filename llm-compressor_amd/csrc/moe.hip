@@ -16,6 +16,8 @@
 // Sums are fp32, in the order of k, rounded once; rows from offsets[E] on take no part
 // (their gradients are zeros).  Nothing is added with atomics that are not integer
 // counts, so results do not change from run to run.
+#include <type_traits>
+
 #include "fp8.h"
 
 namespace mi355q {
@@ -183,117 +185,218 @@ template <class T> struct Piece {
   static constexpr int N = 16 / sizeof(typename T::raw);
   typename T::raw v[N];
 };
-// 16 bytes of a row with `left` elements from p on, zeros past its end
-template <class T>
+// 16 bytes of a row with `left` elements from p on, zeros past its end.  FULL: there are 16 (a branch around loads
+// has them waited for one by one, so the kernels tell rows' ends apart around all of a thread's).
+typedef uint32_t __attribute__((ext_vector_type(4), aligned(2))) chunk_t;
+template <class T, bool FULL, bool NT>
 __device__ __forceinline__ Piece<T> load_piece(const typename T::raw* p, int64_t left) {
   Piece<T> c;
-  if (left >= Piece<T>::N) {
-    __builtin_memcpy(&c, p, 16);
+  if constexpr (FULL) {
+    const chunk_t* const q = reinterpret_cast<const chunk_t*>(p);
+    const chunk_t v = NT ? __builtin_nontemporal_load(q) : *q;
+    __builtin_memcpy(&c, &v, 16);
   } else {
 #pragma unroll
     for (int e = 0; e < Piece<T>::N; ++e) c.v[e] = e < left ? p[e] : typename T::raw(0);
   }
   return c;
 }
-template <class T>
+template <class T, bool FULL, bool NT>
 __device__ __forceinline__ void store_piece(typename T::raw* p, const Piece<T>& c, int64_t left) {
-  if (left >= Piece<T>::N) {
-    __builtin_memcpy(p, &c, 16);
+  if constexpr (FULL) {
+    chunk_t v;
+    __builtin_memcpy(&v, &c, 16);
+    if constexpr (NT) __builtin_nontemporal_store(v, reinterpret_cast<chunk_t*>(p));
+    else *reinterpret_cast<chunk_t*>(p) = v;
   } else {
 #pragma unroll
     for (int e = 0; e < Piece<T>::N; ++e)
       if (e < left) p[e] = c.v[e];
   }
 }
-__device__ __forceinline__ float weight_of(const RowsArgs& g, int64_t i) {
-  if (!g.w) return 1.f;
-  if (g.w_type == MI355Q_F32) return static_cast<const float*>(g.w)[i];
-  const uint16_t v = static_cast<const uint16_t*>(g.w)[i];
-  return g.w_type == MI355Q_BF16 ? Bf16::load(v) : F16::load(v);
+
+// the weights of K pairs from pair i on, of which `n` are there
+template <int K>
+__device__ __forceinline__ void load_weights(const RowsArgs& g, int64_t i, uint32_t n, float (&w)[K]) {
+  if (!g.w) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) w[k] = 1.f;
+  } else if (g.w_type == MI355Q_F32) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) w[k] = static_cast<const float*>(g.w)[i + (k < (int)n ? k : 0)];
+  } else {
+    uint16_t v[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] = static_cast<const uint16_t*>(g.w)[i + (k < (int)n ? k : 0)];
+#pragma unroll
+    for (int k = 0; k < K; ++k) w[k] = g.w_type == MI355Q_BF16 ? Bf16::load(v[k]) : F16::load(v[k]);
+  }
+}
+// the places of K pairs from pair i on, -1 for those that are not there
+template <int K>
+__device__ __forceinline__ void load_places(const RowsArgs& g, int64_t i, uint32_t n, int64_t (&s)[K]) {
+#pragma unroll
+  for (int k = 0; k < K; ++k) s[k] = g.slots[i + (k < (int)n ? k : 0)];
+#pragma unroll
+  for (int k = 0; k < K; ++k) s[k] = k < (int)n && (uint64_t)s[k] < (uint64_t)g.pairs ? s[k] : -1;
+}
+// f(std::true_type) where 16 bytes are left, else f(std::false_type)
+template <class Fn>
+__device__ __forceinline__ void by_fullness(bool full, Fn&& f) {
+  if (full) f(std::true_type{});
+  else f(std::false_type{});
 }
 
+// The kernels below take K of a token's pairs at a time, whose rows are in flight together.
+//
 // A thread takes 16 bytes of one token: loaded once, stored `top` times.
-template <class T>
+// NT: what moves once bypasses the caches.
+template <class T, int K, bool NT>
 __global__ __launch_bounds__(256) void moe_sort_kernel(RowsArgs g) {
   using raw = typename T::raw;
-  const uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x;
-  const uint64_t t = i / g.chunks.d;
+  const uint32_t i = blockIdx.x * 256u + threadIdx.x, t = div(i, g.chunks);
   if (t >= g.tokens) return;
   const int64_t c = (int64_t)(i - t * g.chunks.d) * Piece<T>::N, left = g.cols - c;
   const int64_t end = *g.end;
-  const Piece<T> v = load_piece<T>(static_cast<const raw*>(g.x) + t * g.ldx + c, left);
-  for (uint32_t k = 0; k < g.top; ++k) {
-    const int64_t s = g.slots[t * g.top + k];
-    if ((uint64_t)s >= (uint64_t)g.pairs) continue;
-    store_piece<T>(static_cast<raw*>(g.y) + s * g.ldy + c, s < end ? v : Piece<T>{}, left);
-  }
+  by_fullness(left >= Piece<T>::N, [&](auto full) __attribute__((always_inline)) {
+    constexpr bool FULL = decltype(full)::value;
+    const Piece<T> v = load_piece<T, FULL, NT>(static_cast<const raw*>(g.x) + t * g.ldx + c, left);
+    for (uint32_t k0 = 0; k0 < g.top; k0 += K) {
+      int64_t s[K];
+      load_places(g, (int64_t)t * g.top + k0, g.top - k0, s);
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+        if (s[k] >= 0)
+          store_piece<T, FULL, NT>(static_cast<raw*>(g.y) + s[k] * g.ldy + c, s[k] < end ? v : Piece<T>{}, left);
+    }
+  });
 }
 
 // A thread takes 16 bytes of one token's sum.
-template <class T>
+template <class T, int K, bool NT>
 __global__ __launch_bounds__(256) void moe_combine_kernel(RowsArgs g) {
   using raw = typename T::raw;
   constexpr int N = Piece<T>::N;
-  const uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x;
-  const uint64_t t = i / g.chunks.d;
+  const uint32_t i = blockIdx.x * 256u + threadIdx.x, t = div(i, g.chunks);
   if (t >= g.tokens) return;
   const int64_t c = (int64_t)(i - t * g.chunks.d) * N, left = g.cols - c;
   const int64_t end = *g.end;
-  float acc[N] = {};
-  for (uint32_t k = 0; k < g.top; ++k) {
-    const int64_t s = g.slots[t * g.top + k];
-    if (s >= end || (uint64_t)s >= (uint64_t)g.pairs) continue;
-    const float w = weight_of(g, t * g.top + k);
-    const Piece<T> v = load_piece<T>(static_cast<const raw*>(g.x) + s * g.ldx + c, left);
+  by_fullness(left >= N, [&](auto full) __attribute__((always_inline)) {
+    constexpr bool FULL = decltype(full)::value;
+    float acc[N] = {};
+    for (uint32_t k0 = 0; k0 < g.top; k0 += K) {
+      int64_t s[K];
+      float w[K];
+      Piece<T> v[K];
+      load_places(g, (int64_t)t * g.top + k0, g.top - k0, s);
+      load_weights(g, (int64_t)t * g.top + k0, g.top - k0, w);
+      // rows that take no part: the first one is read, and counts as zeros
 #pragma unroll
-    for (int e = 0; e < N; ++e) acc[e] = fmaf(w, T::load(v.v[e]), acc[e]);
-  }
-  Piece<T> o;
-#pragma unroll
-  for (int e = 0; e < N; ++e) o.v[e] = T::store(acc[e]);
-  store_piece<T>(static_cast<raw*>(g.y) + t * g.ldy + c, o, left);
-}
-
-// A workgroup takes one token.
-template <class T>
-__global__ __launch_bounds__(256) void moe_combine_backward_kernel(RowsArgs g) {
-  using raw = typename T::raw;
-  constexpr int N = Piece<T>::N;
-  __shared__ float sums[4];
-  const int64_t t = blockIdx.x;
-  const int64_t end = *g.end;
-  for (uint32_t k = 0; k < g.top; ++k) {
-    const int64_t s = g.slots[t * g.top + k];
-    const bool in = (uint64_t)s < (uint64_t)g.pairs, kept = in && s < end;
-    const float w = kept ? weight_of(g, t * g.top + k) : 0.f;
-    float dot = 0.f;
-    for (int64_t c = threadIdx.x * N; c < g.cols; c += 256 * N) {
-      const int64_t left = g.cols - c;
-      const Piece<T> d = load_piece<T>(static_cast<const raw*>(g.dy) + t * g.lddy + c, left);
-      if (g.dw && kept) {
-        const Piece<T> v = load_piece<T>(static_cast<const raw*>(g.x) + s * g.ldx + c, left);
-#pragma unroll
-        for (int e = 0; e < N; ++e) dot = fmaf(T::load(v.v[e]), T::load(d.v[e]), dot);
+      for (int k = 0; k < K; ++k) {
+        s[k] = s[k] < end ? s[k] : -1;
+        v[k] = load_piece<T, FULL, NT>(static_cast<const raw*>(g.x) + (s[k] < 0 ? 0 : s[k]) * g.ldx + c, left);
       }
-      if (g.y && in) {
-        Piece<T> o;
 #pragma unroll
-        for (int e = 0; e < N; ++e) o.v[e] = kept ? T::store(w * T::load(d.v[e])) : typename T::raw(0);
-        store_piece<T>(static_cast<raw*>(g.y) + s * g.ldy + c, o, left);
+      for (int k = 0; k < K; ++k) {
+        const float f = s[k] < 0 ? 0.f : w[k];
+#pragma unroll
+        for (int e = 0; e < N; ++e) acc[e] = fmaf(f, s[k] < 0 ? 0.f : T::load(v[k].v[e]), acc[e]);
       }
     }
-    if (g.dw) {
+    Piece<T> o;
 #pragma unroll
-      for (int m = 32; m; m >>= 1) dot += __shfl_xor(dot, m);
-      if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = dot;
-      __syncthreads();
-      if (threadIdx.x == 0) {
-        const float v = (sums[0] + sums[1]) + (sums[2] + sums[3]);
-        const int64_t o = t * g.top + k;
-        if (g.w_type == MI355Q_F32) static_cast<float*>(g.dw)[o] = v;
-        else static_cast<uint16_t*>(g.dw)[o] = g.w_type == MI355Q_BF16 ? Bf16::store(v) : F16::store(v);
+    for (int e = 0; e < N; ++e) o.v[e] = T::store(acc[e]);
+    store_piece<T, FULL, false>(static_cast<raw*>(g.y) + t * g.ldy + c, o, left);
+  });
+}
+
+// Sums of K (2, 4 or 8) values over the wave, value k in the lanes with l % K = k: at each of log2 K steps a lane
+// hands half of its values to its partner and adds the partner's other half; the last steps add what is left.
+template <int K>
+__device__ __forceinline__ float sum_values(float (&v)[K], int lane) {
+#pragma unroll
+  for (int n = K / 2, d = 1; n; n >>= 1, d <<= 1) {
+    const bool up = lane & d;
+#pragma unroll
+    for (int k = 0; k < n; ++k) {
+      // value bits go to lane bits from the lowest on: of the pair (2 k, 2 k + 1) the lane keeps the one of its bit
+      const float keep = up ? v[2 * k + 1] : v[2 * k], give = up ? v[2 * k] : v[2 * k + 1];
+      v[k] = keep + __shfl_xor(give, d);
+    }
+  }
+  float s = v[0];
+#pragma unroll
+  for (int d = K; d < 64; d <<= 1) s += __shfl_xor(s, d);
+  return s;
+}
+
+// W waves take one token: they read its gradient and its experts' rows, write the rows' gradients and add up the
+// weights' over the row.
+template <class T, int K, int W, bool NT>
+__global__ __launch_bounds__(256) void moe_combine_backward_kernel(RowsArgs g) {
+  using raw = typename T::raw;
+  constexpr int N = Piece<T>::N, PER = 4 / W;            // tokens per workgroup
+  __shared__ float sums[4][K];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t t = (int64_t)blockIdx.x * PER + wave / W;
+  const bool in = t < g.tokens;
+  const int64_t end = *g.end;
+  for (uint32_t k0 = 0; k0 < g.top; k0 += K) {
+    int64_t s[K], from[K];
+    float w[K], dot[K] = {};
+    load_places(g, (in ? t : 0) * g.top + k0, g.top - k0, s);
+    load_weights(g, (in ? t : 0) * g.top + k0, g.top - k0, w);
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      from[k] = s[k] < end ? s[k] : -1;
+      w[k] = from[k] < 0 ? 0.f : w[k];
+    }
+    if (in)
+      for (int64_t c = ((wave % W) * 64 + lane) * N; c < g.cols; c += 64 * W * N) {
+        const int64_t left = g.cols - c;
+        by_fullness(left >= N, [&](auto full) __attribute__((always_inline)) {
+          constexpr bool FULL = decltype(full)::value;
+          const Piece<T> d = load_piece<T, FULL, false>(static_cast<const raw*>(g.dy) + t * g.lddy + c, left);
+          Piece<T> v[K];
+          if (g.dw) {                                     // rows that take no part: the first one, as zeros
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+              v[k] = load_piece<T, FULL, NT>(static_cast<const raw*>(g.x) + (from[k] < 0 ? 0 : from[k]) * g.ldx + c, left);
+          }
+          if (g.y) {
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+              if (s[k] < 0) continue;
+              Piece<T> o;
+#pragma unroll
+              for (int e = 0; e < N; ++e) o.v[e] = from[k] < 0 ? typename T::raw(0) : T::store(w[k] * T::load(d.v[e]));
+              store_piece<T, FULL, NT>(static_cast<raw*>(g.y) + s[k] * g.ldy + c, o, left);
+            }
+          }
+          if (g.dw) {
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+#pragma unroll
+              for (int e = 0; e < N; ++e)
+                dot[k] = fmaf(from[k] < 0 ? 0.f : T::load(v[k].v[e]), from[k] < 0 ? 0.f : T::load(d.v[e]), dot[k]);
+          }
+        });
       }
+    if (!g.dw) continue;
+    float v = sum_values<K>(dot, lane);
+    if constexpr (W > 1) {
+      if (lane < K) sums[wave][lane] = v;
       __syncthreads();
+      v = sums[0][lane & (K - 1)];
+#pragma unroll
+      for (int i = 1; i < W; ++i) v += sums[i][lane & (K - 1)];
+      __syncthreads();
+      if (wave) continue;
+    }
+    if (in && lane < K && k0 + lane < g.top) {
+      const int64_t o = t * g.top + k0 + lane;
+      if (g.w_type == MI355Q_F32) static_cast<float*>(g.dw)[o] = v;
+      else static_cast<uint16_t*>(g.dw)[o] = g.w_type == MI355Q_BF16 ? Bf16::store(v) : F16::store(v);
     }
   }
 }
@@ -315,16 +418,37 @@ static int check_rows(const RowsArgs& g, int64_t tokens, int64_t top, int64_t co
   return MI355Q_OK;
 }
 
-// launches `kernel`, a thread per 16 bytes of a token's row
+// f(std::integral_constant) of the pairs that are taken at a time
 template <class Fn>
-static int launch_rows(RowsArgs& g, int64_t tokens, int64_t cols, mi355q_dtype dt, Fn&& kernel) {
-  const int64_t chunks = (cols * dtype_size(dt) + 15) / 16;
-  MQ_CHECK_ARG(chunks <= INT32_MAX, "moe: rows of %lld columns are too wide", (long long)cols);
-  const int64_t blocks = (tokens * chunks + 255) / 256;
-  MQ_CHECK_ARG(blocks <= INT32_MAX, "moe: %lld rows of %lld columns are too many", (long long)tokens, (long long)cols);
-  g.chunks = {(uint32_t)chunks, 0, 0};
-  with_dtype(dt, [&](auto type) { kernel(type, dim3((unsigned)blocks)); });
-  MQ_LAUNCH_CHECK();
+static void by_top(int64_t top, Fn&& f) {
+  if (top <= 2) f(std::integral_constant<int, 2>{});
+  else if (top <= 4) f(std::integral_constant<int, 4>{});
+  else f(std::integral_constant<int, 8>{});
+}
+
+// Experts' rows of more bytes than this, half of the last-level cache, go around the caches: 8192 tokens to 8 experts
+// of 2048 bf16 (256 MB) combine 60 -> 54 us, their gradients 120 -> 113, sort 59 -> 54.
+constexpr int64_t kCached = 128ll << 20;
+
+// launches `kernel(type, grid, g)`, a thread per 16 bytes of a token's row, over as many tokens at a time as
+// the kernels' 31 bits count
+template <class Fn>
+static int launch_rows(RowsArgs g, int64_t tokens, int64_t cols, mi355q_dtype dt, int64_t row_x, int64_t row_y,
+                       Fn&& kernel) {
+  const int64_t chunks = (cols * dtype_size(dt) + 15) / 16, most = INT32_MAX / 2;
+  MQ_CHECK_ARG(chunks <= most, "moe: rows of %lld columns are too wide", (long long)cols);
+  g.chunks = fast_div((uint32_t)chunks);
+  const int64_t step = most / chunks;
+  for (int64_t t = 0; t < tokens; t += step) {
+    RowsArgs part = g;
+    part.tokens = (uint32_t)(tokens - t < step ? tokens - t : step);
+    part.x = static_cast<const char*>(g.x) + t * row_x * dtype_size(dt);
+    part.y = static_cast<char*>(g.y) + t * row_y * dtype_size(dt);
+    part.slots = g.slots + t * g.top;
+    if (g.w) part.w = static_cast<const char*>(g.w) + t * g.top * dtype_size((mi355q_dtype)g.w_type);
+    with_dtype(dt, [&](auto type) { kernel(type, dim3((unsigned)((part.tokens * chunks + 255) / 256)), part); });
+    MQ_LAUNCH_CHECK();
+  }
   return MI355Q_OK;
 }
 
@@ -383,8 +507,15 @@ int mi355q_moe_sort(const void* x_dev, mi355q_dtype dtype, int64_t tokens, int64
   if (rc != MI355Q_OK || tokens == 0) return rc;
   MQ_CHECK_ARG(x_dev && y_dev, "moe_sort: a null operand");
   MQ_CHECK_ARG((tokens <= 1 || ldx >= 0) && (tokens * top <= 1 || ldy >= cols), "moe_sort: rows overlap");
-  return launch_rows(g, tokens, cols, dtype, [&](auto type, dim3 grid) {
-    hipLaunchKernelGGL((moe_sort_kernel<decltype(type)>), grid, dim3(256), 0, static_cast<hipStream_t>(stream), g);
+  const bool past = tokens * top * cols * dtype_size(dtype) > kCached;
+  return launch_rows(g, tokens, cols, dtype, ldx, 0, [&](auto type, dim3 grid, const RowsArgs& part) {
+    using T = decltype(type);
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    by_top(top, [&](auto k) {
+      constexpr int K = decltype(k)::value;
+      if (past) hipLaunchKernelGGL((moe_sort_kernel<T, K, true>), grid, dim3(256), 0, st, part);
+      else hipLaunchKernelGGL((moe_sort_kernel<T, K, false>), grid, dim3(256), 0, st, part);
+    });
   });
 }
 
@@ -397,8 +528,15 @@ int mi355q_moe_combine(const void* x_dev, mi355q_dtype dtype, int64_t tokens, in
   if (rc != MI355Q_OK || tokens == 0) return rc;
   MQ_CHECK_ARG(x_dev && y_dev, "moe_combine: a null operand");
   MQ_CHECK_ARG(ldx >= 0 && (tokens <= 1 || ldy >= cols), "moe_combine: rows overlap");
-  return launch_rows(g, tokens, cols, dtype, [&](auto type, dim3 grid) {
-    hipLaunchKernelGGL((moe_combine_kernel<decltype(type)>), grid, dim3(256), 0, static_cast<hipStream_t>(stream), g);
+  const bool past = tokens * top * cols * dtype_size(dtype) > kCached;
+  return launch_rows(g, tokens, cols, dtype, 0, ldy, [&](auto type, dim3 grid, const RowsArgs& part) {
+    by_top(top, [&](auto k) {
+      using T = decltype(type);
+      constexpr int K = decltype(k)::value;
+      hipStream_t st = static_cast<hipStream_t>(stream);
+      if (past) hipLaunchKernelGGL((moe_combine_kernel<T, K, true>), grid, dim3(256), 0, st, part);
+      else hipLaunchKernelGGL((moe_combine_kernel<T, K, false>), grid, dim3(256), 0, st, part);
+    });
   });
 }
 
@@ -414,9 +552,18 @@ int mi355q_moe_combine_backward(const void* dy_dev, mi355q_dtype dtype, int64_t 
   MQ_CHECK_ARG(ldx >= 0 && lddy >= 0 && (!dx_dev || tokens * top <= 1 || lddx >= cols),
                "moe_combine_backward: rows overlap");
   if (!dx_dev && !dw_dev) return MI355Q_OK;
+  const bool past = dx_dev && tokens * top * cols * dtype_size(dtype) > kCached;
+  const bool wide = cols * dtype_size(dtype) > 64 * 16;
   with_dtype(dtype, [&](auto type) {
-    hipLaunchKernelGGL((moe_combine_backward_kernel<decltype(type)>), dim3((unsigned)tokens), dim3(256), 0,
-                       static_cast<hipStream_t>(stream), g);
+    using T = decltype(type);
+    const dim3 grid((unsigned)(wide ? tokens : (tokens + 3) / 4)), block(256);
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    by_top(top, [&](auto k) {
+      constexpr int K = decltype(k)::value;
+      if (wide && past) hipLaunchKernelGGL((moe_combine_backward_kernel<T, K, 4, true>), grid, block, 0, st, g);
+      else if (wide) hipLaunchKernelGGL((moe_combine_backward_kernel<T, K, 4, false>), grid, block, 0, st, g);
+      else hipLaunchKernelGGL((moe_combine_backward_kernel<T, K, 1, false>), grid, block, 0, st, g);
+    });
   });
   MQ_LAUNCH_CHECK();
   return MI355Q_OK;
