@@ -1,5 +1,8 @@
 """MoE expert routing and grouped per-expert Hessians.
 
+``sort_tokens`` and ``combine_tokens`` move the tokens themselves, with gradients:
+two launches instead of a gather and a scatter per expert.
+
 Token routing follows ``modeling/moe/linear_experts.py:244-277``: for expert
 e the tokens are ``torch.where(one_hot(top_k_index)[..., e].T)`` - ordered by
 top-k position, then token index.  Outside ``moe_calibration_context`` an
@@ -57,6 +60,13 @@ def route_tokens(top_k_index: torch.Tensor, num_experts: int, num_tokens: int | 
         rows = torch.arange(nt, device=dev, dtype=torch.int32).repeat(num_experts)
         offsets = [e * nt for e in range(num_experts + 1)]
         return rows, offsets, None
+    if top_k_index.is_cuda and tokens and 0 < num_experts <= ops.MOE_MAX_EXPERTS and \
+            top_k_index.dtype in (torch.int32, torch.int64):
+        sorted_tok, slots, ends = ops.moe_plan(top_k_index, num_experts)
+        offsets = ends.tolist()
+        if offsets[-1] == tokens * k:               # every id is an expert's
+            pos = torch.arange(k, device=dev).expand(tokens, k).reshape(-1)
+            return sorted_tok, offsets, torch.empty_like(pos).scatter_(0, slots.reshape(-1).long(), pos)
     # key = expert * (k * T) + pos * T + token  ->  sort = reference order
     pos = torch.arange(k, device=dev).unsqueeze(0).expand(tokens, k)
     tok = torch.arange(tokens, device=dev).unsqueeze(1).expand(tokens, k)
@@ -186,13 +196,21 @@ class LinearExperts(torch.nn.ModuleList):
     ``torch.where(one_hot(top_k_index)[..., e].T)`` (all tokens under
     ``moe_calibration_context``, the outputs then taken at the routed rows),
     weighted by their top-k weights and summed into the output with
-    ``index_add_``."""
+    ``index_add_``.
+
+    ``sorted_tokens`` (an attribute, too; on the GPU, outside
+    ``moe_calibration_context``): the tokens are sorted by expert once
+    (``sort_tokens``), each expert gets a slice of them - the same rows in the
+    same order - and ``combine_tokens`` weights and adds the results in fp32 with
+    one rounding, where the loop adds in the output's type.  Also differentiable; ids
+    outside [0, num_experts) take no part."""
 
     def __init__(self, num_experts: int, hidden: int, intermediate: int, bias: bool = False,
-                 act=torch.nn.functional.silu, dtype=None, device=None):
+                 act=torch.nn.functional.silu, dtype=None, device=None, sorted_tokens: bool = False):
         super().__init__([ExpertMLP(hidden, intermediate, bias, act, dtype, device) for _ in range(num_experts)])
         self.num_experts = num_experts
         self.intermediate_size = intermediate
+        self.sorted_tokens = sorted_tokens
 
     @classmethod
     @torch.no_grad()
@@ -209,6 +227,14 @@ class LinearExperts(torch.nn.ModuleList):
 
     def forward(self, hidden_states: torch.Tensor, top_k_index: torch.Tensor,
                 top_k_weights: torch.Tensor) -> torch.Tensor:
+        if self.sorted_tokens and hidden_states.is_cuda and not get_calibrate_all_experts_flag():
+            rows, plan = sort_tokens(hidden_states, top_k_index, self.num_experts)
+            # the last part: rows of no expert
+            offsets = plan.offsets.tolist()
+            sizes = [b - a for a, b in zip(offsets, [*offsets[1:], rows.shape[0]])]
+            parts = rows.split(sizes)
+            out = [expert(part) for expert, part in zip(self, parts)] + [parts[-1]]
+            return combine_tokens(torch.cat(out), top_k_weights, plan)
         final = torch.zeros_like(hidden_states)
         with torch.no_grad():
             mask = torch.nn.functional.one_hot(top_k_index, self.num_experts).permute(2, 1, 0)

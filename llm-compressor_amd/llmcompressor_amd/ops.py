@@ -934,6 +934,12 @@ def fp8_silu_mul_backward(dh: torch.Tensor, saved: torch.Tensor, saved_scales: t
 
 # ---------------------------------------------------------------- tokens by expert
 _MOE_DT = _FP8_DT
+MOE_MAX_EXPERTS = 2040      # of a plan
+
+
+@functools.lru_cache(maxsize=4096)
+def _moe_workspace(tokens: int, top: int, num_experts: int) -> int:
+    return L.lib().mi355q_moe_plan_workspace_size(tokens, top, num_experts)
 
 
 def moe_plan(top_k_index: torch.Tensor, num_experts: int):
@@ -949,18 +955,22 @@ def moe_plan(top_k_index: torch.Tensor, num_experts: int):
     bits = {torch.int32: 32, torch.int64: 64}.get(top_k_index.dtype)
     if bits is None:
         raise TypeError(f"top_k_index must be int32 or int64, got {top_k_index.dtype}")
+    if num_experts <= 0:
+        raise ValueError(f"num_experts must be positive, got {num_experts}")
     if top_k_index.dim() != 2 or top_k_index.shape[1] == 0:
         raise ValueError(f"top_k_index must be [tokens, top], got {tuple(top_k_index.shape)}")
     tokens, top = top_k_index.shape
     ids, pitch = _rows_2d(top_k_index, top)
     rows = ids.new_empty(tokens * top, dtype=torch.int32)
     slots = ids.new_empty((tokens, top), dtype=torch.int32)
-    offsets = ids.new_empty(num_experts + 1 if num_experts > 0 else 1, dtype=torch.int64)
+    offsets = ids.new_empty(num_experts + 1, dtype=torch.int64)
     lib = L.lib()
-    need = lib.mi355q_moe_plan_workspace_size(tokens, top, num_experts)
-    ws = _ws(need, ids.device)
-    L.check(lib.mi355q_moe_plan(ids.data_ptr(), bits, tokens, top, pitch, num_experts, rows.data_ptr(),
-                                slots.data_ptr(), offsets.data_ptr(), L.ptr(ws), need, L.stream_of(ids)))
+    need = _moe_workspace(tokens, top, num_experts)
+    ws = ids.new_empty(need, dtype=torch.uint8) if need else None
+    rc = lib.mi355q_moe_plan(ids.data_ptr(), bits, tokens, top, pitch, num_experts, rows.data_ptr(), slots.data_ptr(),
+                             offsets.data_ptr(), None if ws is None else ws.data_ptr(), need, L.stream_of(ids))
+    if rc:
+        L.check(rc)
     return rows, slots, offsets
 
 
