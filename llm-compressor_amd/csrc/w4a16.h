@@ -90,10 +90,12 @@ __device__ __forceinline__ u32x4_t e2m1s(uint32_t w, float e) {
                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, e, 3))};
 }
 __device__ __forceinline__ float silu(float v) {
-  // e^-v = 2^(-v log2 e), with what the product's rounding leaves put back
+  // e^-v = 2^(-v log2 e), with what the product's rounding leaves put back; beyond 2^+-126 it is infinite or 0
+  // for the sum with 1 (v is then rounded to 0 or itself, and an infinite v has no rounding to put back)
   const float k = -1.44269504f, t = v * k, r = fmaf(v, k, -t) + v * -1.92596299e-8f;
-  const float e = __builtin_amdgcn_exp2f(t);
-  return v * __builtin_amdgcn_rcpf(1.f + fmaf(e, r * 0.693147181f, e));
+  float e = __builtin_amdgcn_exp2f(t);
+  e = fabsf(t) > 126.f ? (t > 0.f ? INFINITY : 0.f) : fmaf(e, r * 0.693147181f, e);
+  return v * __builtin_amdgcn_rcpf(1.f + e);
 }
 
 // ---------------------------------------------------------------- tiles of rows

@@ -139,6 +139,19 @@ def test_gated(rows, kind, group, out, bias):
     check(rows, out, 512, kind, group, BF16, bias, True)
 
 
+@pytest.mark.parametrize("rows", [1, 9, 40, 130])
+@pytest.mark.parametrize("size", [30.0, 300.0, 3e4])
+def test_gated_far_from_zero(rows, size):
+    """Gates of -88 and below, where e^-gate passes fp32's range, and far above."""
+    g = gen("far", rows, size)
+    x = (torch.randn(rows, 256, generator=g) * size).to(BF16)
+    w = Weight(g, 192, 256, "int4", 128)
+    want, tol = expected(x, w.values, w.sizes, None, True)
+    y = ops().w4a16_matmul(x.cuda(), *w.cuda(), gated=True, out_dtype=F32)
+    assert bool((x.double() @ w.values.T)[:, :96].min() < -100) or size < 100
+    close(y, want, tol)
+
+
 @pytest.mark.parametrize("out_dtype", [BF16, F16, F32])
 @pytest.mark.parametrize("scale_dtype", [BF16, F16, F32])
 @pytest.mark.parametrize("rows", [3, 200])
