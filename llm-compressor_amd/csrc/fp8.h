@@ -54,7 +54,7 @@ inline void with_dtype(mi355q_dtype dt, Fn&& f) {
 }
 
 inline bool known_dtype(int dt) { return dt == MI355Q_BF16 || dt == MI355Q_F16 || dt == MI355Q_F32; }
-inline int dtype_size(int dt) { return dt == MI355Q_F32 ? 4 : 2; }
+__host__ __device__ inline int dtype_size(int dt) { return dt == MI355Q_F32 ? 4 : 2; }
 inline bool aligned_to(const void* p, unsigned n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
 // n / d for n < 2^31 without a division: (mulhi(n, mul) + n) >> shift, the division by

@@ -168,7 +168,10 @@ int join_parts(const W4Args& g, uint32_t splits, const float* parts, hipStream_t
 // The tile kernels (w4a16_tiles.hip): whether they take a call, the workspace that they
 // ask for, and the launch.
 bool w4_tiles_fit(const W4Args& g, int kind);
-size_t w4_tiles_workspace(int64_t n_x, int64_t rows_w, int64_t cols, uint32_t groups, bool mx);
+size_t w4_tiles_workspace(int64_t n_x, int64_t rows, int64_t experts, int64_t rows_w, int64_t cols, uint32_t groups,
+                          bool mx);
 int launch_w4_tiles(const W4Args& g, mi355q_dtype x_dtype, int kind, void* workspace, hipStream_t st);
+int launch_w4_tiles_bf16(const W4Args& g, int kind, void* workspace, hipStream_t st);
+int launch_w4_tiles_f16(const W4Args& g, int kind, void* workspace, hipStream_t st);
 
 }  // namespace mi355q

@@ -31,8 +31,12 @@ int join_parts(const W4Args& g, uint32_t splits, const float* parts, hipStream_t
   return MI355Q_OK;
 }
 
-// Up to this many rows (per expert, in the mean) the weight's bytes decide.
-static bool few_rows(int64_t rows, int64_t experts) { return rows <= 64 * experts; }
+// Up to this many rows (per expert, in the mean) the weight's bytes decide.  4096 x 4096: 64 rows 22 us here, 24 in
+// tiles; 128 experts of 1536 x 2048: 8 rows each 72 and 83, 16 rows 109 and 88 (groups of 32, whose scales the tiles
+// have laid out first: 137 and 180).
+static bool few_rows(int64_t rows, int64_t experts, int64_t group) {
+  return rows <= (experts == 1 ? 64 : group < 128 ? 20 : 10) * experts;
+}
 
 // Rows per tile (4 or 16 mt), columns, waves and splits of a call of few rows.
 //
@@ -77,8 +81,8 @@ static size_t few_bytes(int64_t rows, int64_t experts, int64_t out, int64_t cols
 extern "C" size_t mi355q_w4a16_matmul_workspace_size(int64_t n_x, int64_t rows, int64_t experts, int64_t out,
                                                      int64_t cols, mi355q_w4_format format, int64_t group_size) {
   if (n_x <= 0 || rows <= 0 || experts <= 0 || out <= 0 || cols <= 0 || group_size <= 0) return 0;
-  if (few_rows(rows, experts)) return few_bytes(rows, experts, out, cols);
-  return w4_tiles_workspace(n_x, experts * out, cols, (uint32_t)((cols + group_size - 1) / group_size), format == MI355Q_W4_MXFP4);
+  if (few_rows(rows, experts, group_size)) return few_bytes(rows, experts, out, cols);
+  return w4_tiles_workspace(n_x, rows, experts, experts * out, cols, (uint32_t)((cols + group_size - 1) / group_size), format == MI355Q_W4_MXFP4);
 }
 
 extern "C" int mi355q_w4a16_matmul(const void* x_dev, mi355q_dtype x_dtype, int64_t n_x, int64_t ldx,
@@ -124,11 +128,11 @@ extern "C" int mi355q_w4a16_matmul(const void* x_dev, mi355q_dtype x_dtype, int6
               fast_div((uint32_t)(group_size < cols ? (group_size + 127) / 128 : (cols + 127) / 128)), gated != 0};
   const int kind = mx ? kMxfp4 : zeros_dev ? kInt4Zero : kInt4;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (!few_rows(rows, experts) && w4_tiles_fit(g, kind) && workspace_dev && aligned16(workspace_dev) &&
-      workspace_bytes >= w4_tiles_workspace(n_x, experts * out, cols, g.groups, mx))
+  if (!few_rows(rows, experts, group_size) && w4_tiles_fit(g, kind) && workspace_dev && aligned16(workspace_dev) &&
+      workspace_bytes >= w4_tiles_workspace(n_x, rows, experts, experts * out, cols, g.groups, mx))
     return launch_w4_tiles(g, x_dtype, kind, workspace_dev, st);
   FewPlan p = few_plan(rows, experts, out, cols, gated);
-  if (!few_rows(rows, experts) || !workspace_dev || !aligned16(workspace_dev) ||
+  if (!few_rows(rows, experts, group_size) || !workspace_dev || !aligned16(workspace_dev) ||
       workspace_bytes < few_bytes(rows, experts, out, cols))
     p.splits = 1;
   float* const parts = static_cast<float*>(workspace_dev);

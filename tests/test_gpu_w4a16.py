@@ -159,6 +159,45 @@ def test_types(rows, out_dtype, scale_dtype):
     check(rows, 130, 384, "int4z", 64, BF16, True, False, out_dtype, scale_dtype)
 
 
+@pytest.mark.parametrize("rows,out", [(700, 3000), (1300, 5000), (2700, 5300)], ids=["64x128", "64x256", "128x256"])
+@pytest.mark.parametrize("cols,kind,group,dtype", [(256, "int4", 128, BF16), (168, "int4z", 32, F16),
+                                                   (300, "int4z", 64, BF16), (160, "mxfp4", 32, BF16),
+                                                   (352, "mxfp4", 32, F16), (261, "int4", None, F16)])
+def test_larger_tiles(rows, out, cols, kind, group, dtype):
+    check(rows, out, cols, kind, group, dtype, bias=True)
+
+
+@pytest.mark.parametrize("rows,out", [(70, 600), (700, 6000), (1300, 10000), (2700, 10600)])
+@pytest.mark.parametrize("cols,kind,group", [(256, "int4", 128), (168, "int4z", 32), (160, "mxfp4", 32)])
+def test_larger_gated_tiles(rows, out, cols, kind, group):
+    check(rows, out, cols, kind, group, BF16, rows % 2 == 0, True)
+
+
+@pytest.mark.parametrize("rows,cols", [(80, 6144), (130, 9000), (70, 2304)])
+@pytest.mark.parametrize("gated", [False, True])
+def test_split_sums_of_many_columns(rows, cols, gated):
+    check(rows, 256, cols, "int4z", 128, BF16, True, gated)
+    check(rows // 3, 256, cols, "int4", 128, BF16, True, gated)
+
+
+@pytest.mark.parametrize("rows", [90, 20])
+def test_without_a_workspace(rows):
+    """The C entry takes calls without one, by the kernel for few rows and without splitting sums."""
+    import ctypes as C
+
+    from llmcompressor_amd import _lib as L
+    g = gen("ws", rows)
+    x = torch.randn(rows, 4096, generator=g).to(BF16)
+    w = Weight(g, 64, 4096, "int4", 128)
+    p, s, _ = w.cuda()
+    xc, y = x.cuda(), torch.empty(rows, 64, dtype=BF16, device="cuda")
+    assert L.lib().mi355q_w4a16_matmul_workspace_size(rows, rows, 1, 64, 4096, L.W4_INT4, 128) > 0
+    L.check(L.lib().mi355q_w4a16_matmul(xc.data_ptr(), L.BF16, rows, 4096, None, None, 1, p.data_ptr(), L.W4_INT4, 2048, 0,
+                                        s.data_ptr(), L.BF16, 32, 0, None, 0, 0, 128, None, 0, 0, y.data_ptr(), L.BF16, 64,
+                                        rows, 64, 4096, None, C.c_size_t(0), L.stream_of(xc)))
+    close(y, *expected(x, w.values, w.sizes))
+
+
 def test_no_rows():
     w = Weight(gen(1), 24, 64, "int4", 32)
     assert ops().w4a16_matmul(torch.empty(0, 64, dtype=BF16, device="cuda"), *w.cuda(), group_size=32).shape == (0, 24)
@@ -236,6 +275,13 @@ def test_experts(tokens, top, experts, gated):
 @pytest.mark.parametrize("tokens", [3, 90, 400])
 def test_experts_formats(tokens, kind, group, dtype):
     check_experts(tokens, 3, 6, 72, 416, kind, group, dtype, spread=2.0)
+
+
+@pytest.mark.parametrize("tokens,top,experts", [(200, 2, 2), (700, 3, 3), (100, 3, 3)])
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("kind,group", [("int4", 128), ("int4z", 32)])
+def test_experts_of_many_rows(tokens, top, experts, gated, kind, group):
+    check_experts(tokens, top, experts, 300, 264, kind, group, gated=gated, gather=not gated, dropped=0.1)
 
 
 @pytest.mark.parametrize("gather", [False, True])
