@@ -90,12 +90,11 @@ __device__ __forceinline__ u32x4_t e2m1s(uint32_t w, float e) {
                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, e, 3))};
 }
 __device__ __forceinline__ float silu(float v) {
-  // e^-v = 2^(-v log2 e), with what the product's rounding leaves put back; beyond 2^+-126 it is infinite or 0
-  // for the sum with 1 (v is then rounded to 0 or itself, and an infinite v has no rounding to put back)
+  // e^-v = 2^(-v log2 e), with what the product's rounding leaves put back; held within 2^+-126, where the sum with
+  // 1 has long lost the smaller one (without a branch: the compiler makes one of a choice of results)
   const float k = -1.44269504f, t = v * k, r = fmaf(v, k, -t) + v * -1.92596299e-8f;
-  float e = __builtin_amdgcn_exp2f(t);
-  e = fabsf(t) > 126.f ? (t > 0.f ? INFINITY : 0.f) : fmaf(e, r * 0.693147181f, e);
-  return v * __builtin_amdgcn_rcpf(1.f + e);
+  const float e = __builtin_amdgcn_exp2f(__builtin_amdgcn_fmed3f(t, -126.f, 126.f));
+  return v * __builtin_amdgcn_rcpf(1.f + fmaf(e, r * 0.693147181f, e));
 }
 
 // ---------------------------------------------------------------- tiles of rows

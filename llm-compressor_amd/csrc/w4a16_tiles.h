@@ -208,10 +208,13 @@ void w4_tiles_kernel(W4Args g, W4Tiles o) {
   const int ln = lane & 31, h = lane >> 5;
 
   // neighbouring workgroups of an XCD share rows of x, and in bands of 8 row tiles the weight
-  const uint32_t id = xcd_order(blockIdx.x, gridDim.x), split = id / (o.row_tiles * o.col_tiles);
+  // (divisions run on the vector unit: what follows from them is brought back to scalar registers by hand)
+  const uint32_t id = xcd_order(blockIdx.x, gridDim.x);
+  const uint32_t split = __builtin_amdgcn_readfirstlane((int)(id / (o.row_tiles * o.col_tiles)));
   const uint32_t t = id - split * (o.row_tiles * o.col_tiles);
-  const uint32_t band = t / (8 * o.col_tiles), left = o.row_tiles - 8 * band, in = t - band * 8 * o.col_tiles;
-  const uint32_t high = left < 8 ? left : 8, tc = in / high, tr = 8 * band + in - tc * high;
+  const uint32_t band = __builtin_amdgcn_readfirstlane((int)(t / (8 * o.col_tiles)));
+  const uint32_t left = o.row_tiles - 8 * band, in = t - band * 8 * o.col_tiles, high = left < 8 ? left : 8;
+  const uint32_t tc = __builtin_amdgcn_readfirstlane((int)(in / high)), tr = 8 * band + in - tc * high;
   const RowTile tile = row_tile<R>(g, tr);
   if (tile.count <= 0) return;
   const int64_t half = g.gated ? g.out / 2 : 0, width = g.gated ? half : g.out;
@@ -244,7 +247,8 @@ void w4_tiles_kernel(W4Args g, W4Tiles o) {
   // row's chunk (l & 3) ^ (row / 4 & 3).  Rows that are not there read another row (their results are
   // not stored).
   const uint32_t all = (uint32_t)((g.cols + kStep - 1) / kStep);
-  const int s_begin = (int)(all * split / o.splits), steps = (int)(all * (split + 1) / o.splits);
+  const int s_begin = __builtin_amdgcn_readfirstlane((int)(all * split / o.splits));
+  const int steps = __builtin_amdgcn_readfirstlane((int)(all * (split + 1) / o.splits));
   const int64_t x0 = g.rows ? 0 : tile.first;
   constexpr int NR = S::NI > 4 ? S::NI / 4 : 1;       // rows per lane
   uint32_t xo[NR];
@@ -350,45 +354,59 @@ void w4_tiles_kernel(W4Args g, W4Tiles o) {
   if (s_begin < whole) dma_w(s_begin);
   if (KIND != kMxfp4 && split == 0) {
     // the zero points' part: sums of x [m][g] times -s z [n][g], 16 groups at a time
+    const uint16_t *fp[NTW], *sp[MTW];
+#pragma unroll
+    for (int a = 0; a < NTW; ++a)
+      fp[a] = o.factors + ((size_t)tile.expert * g.out + wn[a]) * o.pieces * o.padded + 8 * h;
 #pragma unroll
     for (int b = 0; b < MTW; ++b) {
       const int64_t row = x_row(32 * b + ln);
-      const uint16_t* const sp = o.sums + (size_t)(row < 0 ? 0 : row) * 3 * o.padded + 8 * h;
-      f32x16_t p[NTW];
+      sp[b] = o.sums + (size_t)(row < 0 ? 0 : row) * 3 * o.padded + 8 * h;
+    }
+    f32x16_t p[MTW][NTW];
+#pragma unroll
+    for (int b = 0; b < MTW; ++b)
 #pragma unroll
       for (int a = 0; a < NTW; ++a)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) p[a][e] = 0.f;
-      for (uint32_t g0 = 0; g0 < o.padded; g0 += 16) {
-        u32x4_t f[NTW][3], v[3];
+        for (int e = 0; e < 16; ++e) p[b][a][e] = 0.f;
+    for (uint32_t g0 = 0; g0 < o.padded; g0 += 16) {
+      u32x4_t f[NTW][3], v[MTW][3];
 #pragma unroll
-        for (int i = 0; i < 3; ++i) v[i] = *reinterpret_cast<const u32x4_t*>(sp + g0 + (size_t)i * o.padded);
+      for (int b = 0; b < MTW; ++b)
+#pragma unroll
+        for (int i = 0; i < 3; ++i) v[b][i] = *reinterpret_cast<const u32x4_t*>(sp[b] + g0 + (size_t)i * o.padded);
+#pragma unroll
+      for (int a = 0; a < NTW; ++a) f[a][0] = *reinterpret_cast<const u32x4_t*>(fp[a] + g0);
+      if (o.pieces > 1) {
 #pragma unroll
         for (int a = 0; a < NTW; ++a) {
-          const uint16_t* const fp = o.factors + ((size_t)tile.expert * g.out + wn[a]) * o.pieces * o.padded + 8 * h + g0;
-          f[a][0] = *reinterpret_cast<const u32x4_t*>(fp);
-          f[a][1] = f[a][2] = u32x4_t{0u, 0u, 0u, 0u};
-          if (o.pieces > 1) f[a][1] = *reinterpret_cast<const u32x4_t*>(fp + o.padded);
-          if (o.pieces > 2) f[a][2] = *reinterpret_cast<const u32x4_t*>(fp + 2 * (size_t)o.padded);
+          f[a][1] = *reinterpret_cast<const u32x4_t*>(fp[a] + g0 + o.padded);
+          f[a][2] = o.pieces > 2 ? *reinterpret_cast<const u32x4_t*>(fp[a] + g0 + 2 * (size_t)o.padded)
+                                 : u32x4_t{0u, 0u, 0u, 0u};
         }
 #pragma unroll
-        for (int i = 0; i < 3; ++i)
-#pragma unroll
-          for (int a = 0; a < NTW; ++a) p[a] = mfma32<Bf16>(v[i], f[a][0], p[a]);
-        if (o.pieces > 1) {
+        for (int b = 0; b < MTW; ++b)
 #pragma unroll
           for (int a = 0; a < NTW; ++a) {
-            p[a] = mfma32<Bf16>(v[0], f[a][1], p[a]);
-            p[a] = mfma32<Bf16>(v[1], f[a][1], p[a]);
-            p[a] = mfma32<Bf16>(v[0], f[a][2], p[a]);
+            p[b][a] = mfma32<Bf16>(v[b][0], f[a][1], p[b][a]);
+            p[b][a] = mfma32<Bf16>(v[b][1], f[a][1], p[b][a]);
+            p[b][a] = mfma32<Bf16>(v[b][0], f[a][2], p[b][a]);
           }
-        }
       }
+#pragma unroll
+      for (int b = 0; b < MTW; ++b)
+#pragma unroll
+        for (int a = 0; a < NTW; ++a)
+#pragma unroll
+          for (int i = 0; i < 3; ++i) p[b][a] = mfma32<Bf16>(v[b][i], f[a][0], p[b][a]);
+    }
+#pragma unroll
+    for (int b = 0; b < MTW; ++b)
 #pragma unroll
       for (int a = 0; a < NTW; ++a)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) acc[b][a][e] = p[a][e];
-    }
+        for (int e = 0; e < 16; ++e) acc[b][a][e] = p[b][a][e];
   }
   float next[NTW][GPS];
   if (s_begin < steps) load_s(next, s_begin);
@@ -472,12 +490,21 @@ void w4_tiles_kernel(W4Args g, W4Tiles o) {
   int s = s_begin;
   for (; s + 1 < whole; ++s) step(s, std::true_type{});
   for (; s < steps; ++s) step(s, std::false_type{});
+  // The arguments are read anew: kept over the loop they would not fit into the scalar registers.
+  typedef const __attribute__((address_space(4))) W4Args* args_t;
+  args_t again = (args_t)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(again));
+  const auto& z = *again;
+  auto missing = [&](int r) __attribute__((always_inline)) {
+    const int64_t row = z.rows[tile.first + r];
+    return row < 0 || row >= z.n_x;
+  };
   // a lane has column l & 31 and rows 8 (e / 4) + 4 (l / 32) + e % 4
-  if (g.bias) {
+  if (z.bias) {
 #pragma unroll
     for (int a = 0; a < NTW; ++a) {
       const int64_t n = column(a) + ln;
-      const float bias = n < g.out ? load_any(g.bias, g.bias_type, n) : 0.f;
+      const float bias = n < z.out ? load_any(z.bias, z.bias_type, n) : 0.f;
 #pragma unroll
       for (int b = 0; b < MTW; ++b)
 #pragma unroll
@@ -486,7 +513,7 @@ void w4_tiles_kernel(W4Args g, W4Tiles o) {
   }
   constexpr int UP = NTW / 2;
   if constexpr (UP > 0) {
-    if (g.gated) {
+    if (z.gated) {
 #pragma unroll
       for (int b = 0; b < MTW; ++b)
 #pragma unroll
@@ -495,50 +522,69 @@ void w4_tiles_kernel(W4Args g, W4Tiles o) {
           for (int e = 0; e < 16; ++e) acc[b][a][e] = silu(acc[b][a][e]) * acc[b][a + UP][e];
     }
   }
-  const int tiles = g.gated ? UP : NTW;
-  bool dead = false;                                  // a row that x does not have
-  if (g.rows)
-    for (int r = lane; r < tile.count; r += 64) dead |= x_row(r) < 0;
-  const bool inside = tile.count == R && !__any(dead) && n0 + 32 * tiles <= width;     // all of the wave's part is stored
-  auto store_tiles = [&](auto type) __attribute__((always_inline)) {
-    using O = decltype(type);
-    using raw_t = typename O::raw;
-    raw_t* const y = static_cast<raw_t*>(y_dev) + tile.first * g.ldy + n0;
+  const int tiles = z.gated ? UP : NTW;
+  // rows that x does not have (bit r of the tile's rows) are written as zeros
+  uint64_t dead[2] = {0, 0};
+  if (z.rows) {
+    dead[0] = __ballot(lane < tile.count && missing(lane));
+    if constexpr (R > 64) dead[1] = __ballot(64 + lane < tile.count && missing(64 + lane));
+  }
+  char* const y0 = static_cast<char*>(y_dev) + (tile.first * z.ldy + n0) * dtype_size((mi355q_dtype)z.y_type);
+  if (n0 + 32 * tiles <= width && !(dead[0] | dead[1]) && z.ldy < (1 << 27)) {
+    // all of the wave's columns are stored
+    auto store_tiles = [&](auto type) __attribute__((always_inline)) {
+      using O = decltype(type);
+      constexpr int ES = sizeof(typename O::raw);
+      const uint32_t pitch = (uint32_t)z.ldy * ES;
+      // 16-bit types in pairs of columns: the even lanes take the even rows of both, the odd lanes the odd ones
+      constexpr int STEP = ES == 2 ? 2 : 1;
+      const bool odd = ES == 2 && (lane & 1);
+      const int above = 4 * h + odd;
+      const uint32_t off = (uint32_t)above * pitch + (uint32_t)(ln & -STEP) * ES;
 #pragma unroll
-    for (int b = 0; b < MTW; ++b) {
-      if (inside && sizeof(raw_t) == 2) {
-        // pairs of columns: the even lanes take the even rows of both, the odd lanes the odd ones
-        const bool odd = lane & 1;
-        char* const at = reinterpret_cast<char*>(y + (32 * b + 4 * h + (lane & 1)) * g.ldy + (ln & ~1));
+      for (int b = 0; b < MTW; ++b)
 #pragma unroll
-        for (int a = 0; a < NTW; ++a) {
-          if (a >= tiles) continue;
+        for (int e = 0; e < 16; e += STEP) {
+          const int r = 32 * b + 8 * (e >> 2) + (e & 3);
+          uint32_t v[NTW];
 #pragma unroll
-          for (int e = 0; e < 16; e += 2) {
-            const float mine = acc[b][a][e], below = acc[b][a][e + 1];
-            const float got = __uint_as_float((uint32_t)__builtin_amdgcn_mov_dpp(
-                (int)__float_as_uint(odd ? mine : below), 0xb1, 0xf, 0xf, true));   // the neighbour's
-            const uint32_t lo = O::store(odd ? got : mine), hi = O::store(odd ? below : got);
-            const uint32_t v = lo | hi << 16;
-            __builtin_memcpy(at + ((8 * (e >> 2) + (e & 3)) * g.ldy + 32 * a) * 2, &v, 4);
+          for (int a = 0; a < NTW; ++a) {
+            if constexpr (ES == 4) {
+              v[a] = __float_as_uint(acc[b][a][e]);
+            } else {
+              const float mine = acc[b][a][e], below = acc[b][a][e + 1];
+              const float got = __uint_as_float((uint32_t)__builtin_amdgcn_mov_dpp(
+                  (int)__float_as_uint(odd ? mine : below), 0xb1, 0xf, 0xf, true));   // the neighbour's
+              v[a] = O::store(odd ? got : mine) | (uint32_t)O::store(odd ? below : got) << 16;
+            }
+          }
+          if (r + above < tile.count) {
+#pragma unroll
+            for (int a = 0; a < NTW; ++a)
+              if (a < tiles) __builtin_memcpy(y0 + (int64_t)r * pitch + 32 * a * ES + off, &v[a], 4);
           }
         }
-      } else {
+    };
+    if (z.y_type == MI355Q_BF16) store_tiles(Bf16{});
+    else if (z.y_type == MI355Q_F16) store_tiles(F16{});
+    else store_tiles(F32{});
+    return;
+  }
 #pragma unroll
-        for (int a = 0; a < NTW; ++a) {
-          if (a >= tiles || n0 + 32 * a + ln >= width) continue;
+  for (int b = 0; b < MTW; ++b)
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const int r = 32 * b + 8 * (e >> 2) + 4 * h + (e & 3);
-            if (r < tile.count) y[(int64_t)r * g.ldy + 32 * a + ln] = x_row(r) < 0 ? raw_t(0) : O::store(acc[b][a][e]);
-          }
-        }
+    for (int a = 0; a < NTW; ++a) {
+      if (a >= tiles || n0 + 32 * a + ln >= width) continue;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int r = 32 * b + 8 * (e >> 2) + 4 * h + (e & 3);
+        if (r >= tile.count) continue;
+        const float v = dead[b / 2] >> (r & 63) & 1 ? 0.f : acc[b][a][e];
+        const int64_t at = (int64_t)r * z.ldy + 32 * a + ln;
+        if (z.y_type == MI355Q_F32) reinterpret_cast<float*>(y0)[at] = v;
+        else reinterpret_cast<uint16_t*>(y0)[at] = z.y_type == MI355Q_BF16 ? Bf16::store(v) : F16::store(v);
       }
     }
-  };
-  if (g.y_type == MI355Q_BF16) store_tiles(Bf16{});
-  else if (g.y_type == MI355Q_F16) store_tiles(F16{});
-  else store_tiles(F32{});
 }
 
 // ---------------------------------------------------------------- launches
