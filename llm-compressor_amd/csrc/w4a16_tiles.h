@@ -184,6 +184,7 @@ struct W4Tiles {
   uint32_t padded;           // groups, a multiple of 16
   int pieces;                // of the factors s z that are not zero: 1, 2 or 3
   uint32_t row_tiles, col_tiles, splits;
+  uint32_t band;             // row tiles, of experts
   float* parts;              // with splits: [splits][rows][out], the sums of each range of steps
 };
 
@@ -207,14 +208,25 @@ void w4_tiles_kernel(W4Args g, W4Tiles o) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int ln = lane & 31, h = lane >> 5;
 
-  // neighbouring workgroups of an XCD share rows of x, and in bands of 8 row tiles the weight
+  // Workgroups of an XCD (every eighth) that follow each other share rows of x, and in bands of row tiles the
+  // weight.  One weight: an XCD takes a run of tiles, in bands of 8.  Experts: the bands go round the XCDs, as the
+  // last ones may be empty (how many row tiles there are is known on the device alone).
   // (divisions run on the vector unit: what follows from them is brought back to scalar registers by hand)
-  const uint32_t id = xcd_order(blockIdx.x, gridDim.x);
-  const uint32_t split = __builtin_amdgcn_readfirstlane((int)(id / (o.row_tiles * o.col_tiles)));
-  const uint32_t t = id - split * (o.row_tiles * o.col_tiles);
-  const uint32_t band = __builtin_amdgcn_readfirstlane((int)(t / (8 * o.col_tiles)));
-  const uint32_t left = o.row_tiles - 8 * band, in = t - band * 8 * o.col_tiles, high = left < 8 ? left : 8;
-  const uint32_t tc = __builtin_amdgcn_readfirstlane((int)(in / high)), tr = 8 * band + in - tc * high;
+  uint32_t split = 0, tc, tr;
+  if (g.offsets) {
+    const uint32_t xcd = blockIdx.x % 8, l = blockIdx.x / 8, size = o.band * o.col_tiles;
+    const uint32_t turn = __builtin_amdgcn_readfirstlane((int)(l / size)), in = l - turn * size;
+    tc = __builtin_amdgcn_readfirstlane((int)(in / o.band));
+    tr = (turn * 8 + xcd) * o.band + in - tc * o.band;
+  } else {
+    const uint32_t id = xcd_order(blockIdx.x, gridDim.x);
+    split = __builtin_amdgcn_readfirstlane((int)(id / (o.row_tiles * o.col_tiles)));
+    const uint32_t t = id - split * (o.row_tiles * o.col_tiles);
+    const uint32_t band = __builtin_amdgcn_readfirstlane((int)(t / (8 * o.col_tiles)));
+    const uint32_t left = o.row_tiles - 8 * band, in = t - band * 8 * o.col_tiles, high = left < 8 ? left : 8;
+    tc = __builtin_amdgcn_readfirstlane((int)(in / high));
+    tr = 8 * band + in - tc * high;
+  }
   const RowTile tile = row_tile<R>(g, tr);
   if (tile.count <= 0) return;
   const int64_t half = g.gated ? g.out / 2 : 0, width = g.gated ? half : g.out;
@@ -448,13 +460,57 @@ void w4_tiles_kernel(W4Args g, W4Tiles o) {
       load_s(next, s + 1);
     }
     u32x4_t q[NTW][kSlices];
+    auto convert = [&](int a, int j) __attribute__((always_inline)) {
+      if constexpr (KIND == kMxfp4) q[a][j] = e2m1s<T>(w[a][j], FOLD ? sc[a][j * GPS / kSlices] : 1.f);
+      else q[a][j] = nibbles<T>(w[a][j]);
+    };
+    if constexpr (!FOLD && MTW < 4) {
+      // Units of PER MFMAs, one tile's group each, take turns with two sets of sums: while one is made the other is
+      // scaled and added, and during the first the other tiles' codes are converted.
 #pragma unroll
-    for (int a = 0; a < NTW; ++a)
+      for (int j = 0; j < kSlices; ++j) convert(0, j);
+      u32x4_t v[kSlices];
 #pragma unroll
-      for (int j = 0; j < kSlices; ++j) {
-        if constexpr (KIND == kMxfp4) q[a][j] = e2m1s<T>(w[a][j], FOLD ? sc[a][j * GPS / kSlices] : 1.f);
-        else q[a][j] = nibbles<T>(w[a][j]);
+      for (int j = 0; j < kSlices; ++j) v[j] = read_x(0, j);
+      f32x16_t p[2];
+      constexpr int UNITS = MTW * NTW * GPS;
+      auto finish = [&](int u) __attribute__((always_inline)) {
+        const int b = u / (NTW * GPS), a = u / GPS % NTW, i = u % GPS;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[b][a][e] = fmaf(p[u & 1][e], sc[a][i], acc[b][a][e]);
+      };
+#pragma unroll
+      for (int u = 0; u < UNITS; ++u) {
+        const int b = u / (NTW * GPS), a = u / GPS % NTW, i = u % GPS;
+        const bool ahead = a == NTW - 1 && b + 1 < MTW, first = b == 0 && a == 0 && NTW > 1;
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
+          const int j = i * PER + k;
+          p[u & 1] = mfma32<T>(v[j], q[a][j], k ? p[u & 1] : f32x16_t{});
+          if (ahead) v[j] = read_x(b + 1, j);
+          if (first) {
+#pragma unroll
+            for (int c = 1; c < NTW; ++c) convert(c, j);
+          }
+        }
+        if (u) finish(u - 1);
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+          if (ahead) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+          // (the other unit's last sums are not there at once)
+          if (first) __builtin_amdgcn_sched_group_barrier(0x002, 9, 0);
+          else if (k >= PER / 4) __builtin_amdgcn_sched_group_barrier(0x002, PER == 8 ? 3 : PER == 4 ? 6 : 8, 0);
+        }
       }
+      __builtin_amdgcn_sched_barrier(0);
+      finish(UNITS - 1);
+    } else {
+#pragma unroll
+      for (int a = 0; a < NTW; ++a)
+#pragma unroll
+        for (int j = 0; j < kSlices; ++j) convert(a, j);
 #pragma unroll
     for (int b = 0; b < MTW; ++b) {
       __builtin_amdgcn_sched_barrier(0);
@@ -482,6 +538,7 @@ void w4_tiles_kernel(W4Args g, W4Tiles o) {
         __builtin_amdgcn_sched_group_barrier(0x008, NTW, 0);
         __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
       }
+    }
     }
     __builtin_amdgcn_sched_barrier(0);
     ra[0] ^= S::SLOT;
@@ -624,12 +681,18 @@ static int launch_shape(W4Args g, W4Tiles o, hipStream_t st) {
   const int64_t ct = (width + per - 1) / per;
   int64_t rt = (g.n_rows + R - 1) / R;
   if (g.offsets) rt = g.n_rows / R + g.experts + 1 < g.n_rows ? g.n_rows / R + g.experts + 1 : g.n_rows;
-  MQ_CHECK_ARG(ct * rt * o.splits <= (int64_t)(UINT32_MAX / 256), "w4a16_matmul: %lld rows by %lld columns are too many",
-               (long long)g.n_rows, (long long)width);
+  int64_t rounded = rt;
+  if (g.offsets) {                 // whole rounds of bands, a band for each XCD
+    o.splits = 1;
+    o.band = (uint32_t)(rt >= 512 ? 8 : rt >= 64 ? rt / 64 : 1);
+    rounded = (rt + 8 * o.band - 1) / (8 * o.band) * (8 * o.band);
+  }
+  MQ_CHECK_ARG(ct * rounded * o.splits <= (int64_t)(UINT32_MAX / 256),
+               "w4a16_matmul: %lld rows by %lld columns are too many", (long long)g.n_rows, (long long)width);
   o.row_tiles = (uint32_t)rt;
   o.col_tiles = (uint32_t)ct;
-  hipLaunchKernelGGL((w4_tiles_kernel<T, KIND, GPS, MTW, NTW>), dim3((unsigned)(ct * rt * o.splits)), dim3(64 * kWaves),
-                     0, st, g, o);
+  hipLaunchKernelGGL((w4_tiles_kernel<T, KIND, GPS, MTW, NTW>), dim3((unsigned)(ct * rounded * o.splits)),
+                     dim3(64 * kWaves), 0, st, g, o);
   MQ_LAUNCH_CHECK();
   return o.splits > 1 ? join_parts(whole, o.splits, o.parts, st) : MI355Q_OK;
 }
@@ -671,7 +734,7 @@ static int launch_type(W4Args g, int kind, void* workspace, hipStream_t st) {
     if (copy) at += x_copy_bytes(g.n_x, g.cols);
     to_w = reinterpret_cast<uint8_t*>(at);
   }
-  const W4Tiles o = {to_sums, to_factors, to_scales, padded, pieces, 0, 0, 1, parts};
+  const W4Tiles o = {to_sums, to_factors, to_scales, padded, pieces, 0, 0, 1, 1, parts};
   int lanes = 0;
   while (lanes < 6 && (8 << lanes) < g.group) ++lanes;
   const uint64_t waves = (padded + (64u >> lanes) - 1) / (64u >> lanes);
