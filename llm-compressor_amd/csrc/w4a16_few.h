@@ -174,18 +174,37 @@ __global__ __launch_bounds__(64 * W) void w4_few_kernel(W4Args g, uint32_t nt, u
                                   g.cols - (int64_t)s * kStep - 32 * (MT ? i : col & 3) - 8 * quarter);
   };
   const bool bf16_scales = g.s_type == MI355Q_BF16;
-  // scale i of step d of a batch
-  auto scale = [&](const auto& o, int a, int d, int i) __attribute__((always_inline)) {
+  // the scales of step d of a batch
+  auto scales = [&](const auto& o, int d, float (&sc)[NT][G1]) __attribute__((always_inline)) {
     if constexpr (KIND == kMxfp4) {
-      const uint32_t e = (o.s[a][d] >> 8 * i) & 255u;
-      return FOLD ? __uint_as_float((e << 23) | 0x00400000u) : e8m0_to_f32(e);
+#pragma unroll
+      for (int a = 0; a < NT; ++a)
+#pragma unroll
+        for (int i = 0; i < G1; ++i) {
+          const uint32_t e = (o.s[a][d] >> 8 * i) & 255u;
+          sc[a][i] = FOLD ? __uint_as_float((e << 23) | 0x00400000u) : e8m0_to_f32(e);
+        }
     } else if constexpr (ES == 4) {
-      return __uint_as_float(o.s[a][d * G1 + i]);
+#pragma unroll
+      for (int a = 0; a < NT; ++a)
+#pragma unroll
+        for (int i = 0; i < G1; ++i) sc[a][i] = __uint_as_float(o.s[a][d * G1 + i]);
     } else {
-      const int at = GPS ? d * GPS + i : 2 * d;
-      const uint32_t v = (o.s[a][at / 2] >> 16 * (at & 1)) & 0xffffu;
-      const float x = __uint_as_float(v << 16), y = F16::load((uint16_t)v);
-      return bf16_scales ? x : y;
+      auto half = [&](int a, int i) __attribute__((always_inline)) {
+        const int at = GPS ? d * GPS + i : 2 * d;
+        return at & 1 ? o.s[a][at / 2] >> 16 : o.s[a][at / 2] & 0xffffu;
+      };
+      if (bf16_scales) {
+#pragma unroll
+        for (int a = 0; a < NT; ++a)
+#pragma unroll
+          for (int i = 0; i < G1; ++i) sc[a][i] = __uint_as_float(half(a, i) << 16);
+      } else {
+#pragma unroll
+        for (int a = 0; a < NT; ++a)
+#pragma unroll
+          for (int i = 0; i < G1; ++i) sc[a][i] = F16::load((uint16_t)half(a, i));
+      }
     }
   };
   constexpr uint32_t one = T::code == MI355Q_BF16 ? 0x3f803f80u : 0x3c003c00u;
@@ -196,11 +215,11 @@ __global__ __launch_bounds__(64 * W) void w4_few_kernel(W4Args g, uint32_t nt, u
     constexpr int PER = 4 / G1;                                    // instructions per group
     u32x4_t q[NT][4];
     float sc[NT][G1], z[NT][G1];
+    scales(o, d, sc);
 #pragma unroll
     for (int a = 0; a < NT; ++a) {
 #pragma unroll
       for (int i = 0; i < G1; ++i) {
-        sc[a][i] = scale(o, a, d, i);
         if constexpr (KIND == kInt4Zero) z[a][i] = -(float)((o.z[a][d * G1 + i] >> zs[a]) & 15u);
       }
       const u32x4_t w = transpose_words(o.w[d][a]);
