@@ -82,7 +82,8 @@ extern "C" size_t mi355q_w4a16_matmul_workspace_size(int64_t n_x, int64_t rows, 
                                                      int64_t cols, mi355q_w4_format format, int64_t group_size) {
   if (n_x <= 0 || rows <= 0 || experts <= 0 || out <= 0 || cols <= 0 || group_size <= 0) return 0;
   if (few_rows(rows, experts, group_size)) return few_bytes(rows, experts, out, cols);
-  return w4_tiles_workspace(n_x, rows, experts, experts * out, cols, (uint32_t)((cols + group_size - 1) / group_size), format == MI355Q_W4_MXFP4);
+  return w4_tiles_workspace(n_x, rows, experts, experts * out, cols,
+                            (uint32_t)((cols + group_size - 1) / group_size), format == MI355Q_W4_MXFP4);
 }
 
 extern "C" int mi355q_w4a16_matmul(const void* x_dev, mi355q_dtype x_dtype, int64_t n_x, int64_t ldx,
@@ -132,7 +133,8 @@ extern "C" int mi355q_w4a16_matmul(const void* x_dev, mi355q_dtype x_dtype, int6
       workspace_bytes >= w4_tiles_workspace(n_x, rows, experts, experts * out, cols, g.groups, mx))
     return launch_w4_tiles(g, x_dtype, kind, workspace_dev, st);
   FewPlan p = few_plan(rows, experts, out, cols, gated);
-  if (!few_rows(rows, experts, group_size) || !workspace_dev || !aligned16(workspace_dev) ||
+  // (rows behind the last expert's and rows that x does not have become zeros where the sum is whole)
+  if (rows_dev || offsets_dev || !few_rows(rows, experts, group_size) || !workspace_dev || !aligned16(workspace_dev) ||
       workspace_bytes < few_bytes(rows, experts, out, cols))
     p.splits = 1;
   float* const parts = static_cast<float*>(workspace_dev);

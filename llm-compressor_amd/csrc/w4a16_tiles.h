@@ -650,7 +650,7 @@ struct TilePlan {
   int mt, nt;
   uint32_t splits;
 };
-TilePlan tile_plan(int64_t rows, int64_t experts, int64_t out, int64_t cols, bool gated);
+TilePlan tile_plan(int64_t rows, int64_t experts, int64_t out, int64_t cols, bool gated, bool listed);
 
 inline bool w_in_place(const W4Args& g) { return aligned16(g.w) && g.ldw % 16 == 0 && g.stride_w % 16 == 0; }
 inline bool in_place(const W4Args& g) { return aligned16(g.x) && g.ldx % 8 == 0 && g.cols % 8 == 0; }
@@ -683,7 +683,6 @@ static int launch_shape(W4Args g, W4Tiles o, hipStream_t st) {
   if (g.offsets) rt = g.n_rows / R + g.experts + 1 < g.n_rows ? g.n_rows / R + g.experts + 1 : g.n_rows;
   int64_t rounded = rt;
   if (g.offsets) {                 // whole rounds of bands, a band for each XCD
-    o.splits = 1;
     o.band = (uint32_t)(rt >= 512 ? 8 : rt >= 64 ? rt / 64 : 1);
     rounded = (rt + 8 * o.band - 1) / (8 * o.band) * (8 * o.band);
   }
@@ -709,7 +708,7 @@ static int launch_kind(const W4Args& g, W4Tiles o, const TilePlan& p, hipStream_
 
 template <class T>
 static int launch_type(W4Args g, int kind, void* workspace, hipStream_t st) {
-  const TilePlan plan = tile_plan(g.n_rows, g.experts, g.out, g.cols, g.gated);
+  const TilePlan plan = tile_plan(g.n_rows, g.experts, g.out, g.cols, g.gated, g.offsets || g.rows);
   const bool copy = !in_place(g), sums = kind != kMxfp4;
   const uint32_t padded = (g.groups + 15) / 16 * 16;
   char* at = static_cast<char*>(workspace);

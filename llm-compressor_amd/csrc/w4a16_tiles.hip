@@ -14,19 +14,15 @@ bool w4_tiles_fit(const W4Args& g, int kind) {
          g.out < limit / (4 * (int64_t)((g.groups + 15) / 16 * 16));
 }
 
-
-
-
-
 // Small tiles while there are few of them, then larger ones, which convert a weight's codes for more rows; and a sum
 // over several workgroups where even the smallest leave CUs idle.  4096 x 4096, tiles as rows x columns: 128 rows 25 us
 // (32 x 128 in two parts; 27 whole), 512 rows 35 (32 x 128; 64 x 256 58), 1024 rows 51 (64 x 128; 56 in 32 x 128), 2048
 // rows 80 (64 x 256; 84 in 64 x 128, 100 in 128 x 256); 1024 x 14336 x 4096 133 (128 x 256; 139 in 64 x 128).  128 x
 // 4096 x 14336 40 us in four parts, 45 in two.  128 experts of 1536 x 2048: 16 to 64 rows each 88 to 145 us in 32 x 256
 // (98 to 167 in 64 x 256), 256 rows 366 (379).
-TilePlan tile_plan(int64_t rows, int64_t experts, int64_t out, int64_t cols, bool gated) {
+TilePlan tile_plan(int64_t rows, int64_t experts, int64_t out, int64_t cols, bool gated, bool listed) {
   const int64_t steps = (cols + kStep - 1) / kStep, mean = rows / experts;
-  if (experts > 1) {
+  if (experts > 1 || listed) {
     const int mt = mean < 128 ? 1 : mean < 512 ? 2 : 4;
     return {mt, gated || mean >= 48 ? 2 : 1, 1};
   }
@@ -45,7 +41,7 @@ size_t w4_tiles_workspace(int64_t n_x, int64_t rows, int64_t experts, int64_t ro
   // operands that the DMA cannot read (rows off 16 bytes or not of whole chunks) are copied
   const int64_t w_bytes = mx ? cols / 2 : (cols + 7) / 8 * 4;
   return (mx ? 0 : sums_bytes(n_x, groups) + sums_bytes(rows_w, groups)) + scales_bytes(rows_w, groups) +
-         parts_bytes(tile_plan(rows, experts, rows_w / experts, cols, false), rows, rows_w / experts) +
+         parts_bytes(tile_plan(rows, experts, rows_w / experts, cols, false, false), rows, rows_w / experts) +
          x_copy_bytes(n_x, cols) + (w_bytes % 16 ? (size_t)rows_w * ((w_bytes + 15) / 16 * 16) : 0);
 }
 

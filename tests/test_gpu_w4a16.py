@@ -284,6 +284,32 @@ def test_experts_of_many_rows(tokens, top, experts, gated, kind, group):
     check_experts(tokens, top, experts, 300, 264, kind, group, gated=gated, gather=not gated, dropped=0.1)
 
 
+# One expert: as many rows as a dense product, whose sums are split over workgroups at these widths.
+@pytest.mark.parametrize("tokens", [1, 24, 60, 100, 700])
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("kind,group", [("int4z", 128), ("mxfp4", 32)])
+def test_one_expert(tokens, gated, kind, group):
+    check_experts(tokens, 1, 1, 96, 2304, kind, group, gated=gated, gather=gated, dropped=0.2)
+
+
+# Rows that x does not have are zeros, of one expert too.
+@pytest.mark.parametrize("tokens", [24, 100])
+@pytest.mark.parametrize("gated", [False, True])
+def test_one_expert_rows_not_there(tokens, gated):
+    g = gen(tokens, gated)
+    x = torch.randn(tokens, 2304, generator=g).to(BF16)
+    w = Weight(g, 96, 2304, "int4", 128, experts=1)
+    rows = torch.arange(tokens, dtype=torch.int32)
+    rows[::3] = -1
+    rows[1::6] = tokens
+    rows[4] = 2**31 - 1
+    there = (rows >= 0) & (rows < tokens)
+    y = ops().w4a16_experts_matmul(x.cuda(), rows.cuda(), torch.tensor([0, tokens]).cuda(), *w.cuda(), group_size=128,
+                                   gated=gated).cpu()
+    close(y[there], *expected(x[there], w.values[0], w.sizes[0], None, gated))
+    assert not y[~there].any()
+
+
 @pytest.mark.parametrize("gather", [False, True])
 @pytest.mark.parametrize("dropped", [0.3, 1.0])
 @pytest.mark.parametrize("tokens", [5, 150])
