@@ -81,6 +81,7 @@ static size_t few_bytes(int64_t rows, int64_t experts, int64_t out, int64_t cols
 extern "C" size_t mi355q_w4a16_matmul_workspace_size(int64_t n_x, int64_t rows, int64_t experts, int64_t out,
                                                      int64_t cols, mi355q_w4_format format, int64_t group_size) {
   if (n_x <= 0 || rows <= 0 || experts <= 0 || out <= 0 || cols <= 0 || group_size <= 0) return 0;
+  if (group_size > cols) group_size = cols;
   if (few_rows(rows, experts, group_size)) return few_bytes(rows, experts, out, cols);
   return w4_tiles_workspace(n_x, rows, experts, experts * out, cols,
                             (uint32_t)((cols + group_size - 1) / group_size), format == MI355Q_W4_MXFP4);
@@ -115,6 +116,8 @@ extern "C" int mi355q_w4a16_matmul(const void* x_dev, mi355q_dtype x_dtype, int6
   MQ_CHECK_ARG(group_size == 32 || group_size == 64 || (group_size > 0 && group_size % 128 == 0) || group_size >= cols,
                "w4a16_matmul: groups must have 32, 64, a multiple of 128 or all columns, got %lld",
                (long long)group_size);
+  if (group_size > cols) group_size = cols;
+  MQ_CHECK_ARG(ldx >= 0, "w4a16_matmul: x has a pitch of %lld", (long long)ldx);
   if (rows == 0) return MI355Q_OK;
   MQ_CHECK_ARG(x_dev && w_dev && scales_dev && y_dev, "w4a16_matmul: a null operand");
   const int64_t row_bytes = mx ? cols / 2 : (cols + 7) / 8 * 4;
@@ -125,8 +128,8 @@ extern "C" int mi355q_w4a16_matmul(const void* x_dev, mi355q_dtype x_dtype, int6
   W4Args g = {static_cast<const uint16_t*>(x_dev), ldx, n_x, rows_dev, offsets_dev, (int)experts, rows,
               static_cast<const uint8_t*>(w_dev), ldw, stride_w, scales_dev, (int)scales_dtype, ld_scales,
               stride_scales, zeros_dev, ld_zeros, stride_zeros, bias_dev, (int)bias_dtype, y_dev, (int)y_dtype, ldy,
-              out, cols, (int)(group_size < cols ? group_size : cols), (uint32_t)((cols + group_size - 1) / group_size),
-              fast_div((uint32_t)(group_size < cols ? (group_size + 127) / 128 : (cols + 127) / 128)), gated != 0};
+              out, cols, (int)group_size, (uint32_t)((cols + group_size - 1) / group_size),
+              fast_div((uint32_t)((group_size + kStep - 1) / kStep)), gated != 0};
   const int kind = mx ? kMxfp4 : zeros_dev ? kInt4Zero : kInt4;
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (!few_rows(rows, experts, group_size) && w4_tiles_fit(g, kind) && workspace_dev && aligned16(workspace_dev) &&

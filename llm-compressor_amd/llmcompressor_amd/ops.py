@@ -1137,7 +1137,7 @@ def _w4_matmul(x, index, offsets, experts, n_rows, weight_packed, weight_scale, 
         s, lds, stride_s = _w4_operand(weight_scale, (*first, out, groups), tuple(_FP8_DT), "weight_scale", lead)
         s_kind = _FP8_DT[s.dtype]
     wide = (cols // 2 if mx else -(-cols // 8) * 4)
-    if (ldw % 16 or stride_w % 16 or w.data_ptr() % 16) and (wide % 16 == 0 or w.data_ptr() % 4 or ldw % 4):
+    if wide % 16 == 0 and (ldw % 16 or stride_w % 16 or w.data_ptr() % 16):
         # rows of whole 16-byte chunks that do not lie on 16-byte boundaries
         w = w.clone(memory_format=torch.contiguous_format)
         ldw, stride_w = wide, out * wide

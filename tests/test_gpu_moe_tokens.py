@@ -235,3 +235,23 @@ def test_replayed_graph_follows_new_ids():
         torch.cuda.synchronize()
         again, other = step()
         assert torch.equal(y, again) and all(torch.equal(a, b) for a, b in zip(plan, other)), i
+
+
+def test_rows_past_four_gigabytes():
+    """Experts' rows of more than 2^32 bytes, and more than 2^31 elements."""
+    tokens, cols = 300_000, 4096
+    ids = torch.stack([torch.arange(tokens) % 3, 3 + torch.arange(tokens) % 2], 1).cuda()
+    x = (torch.arange(tokens, device="cuda") % 251).to(BF16)[:, None] + (torch.arange(cols, device="cuda") % 2).to(BF16)
+    x = x.requires_grad_()
+    m = moe()
+    y, plan = m.sort_tokens(x, ids, 5)
+    for a in range(0, 2 * tokens, 50_000):
+        assert torch.equal(y[a:a + 50_000], x[plan.rows[a:a + 50_000].long()]), a
+    w = torch.full((tokens, 2), 0.5, device="cuda", requires_grad=True)
+    out = m.combine_tokens(y, w, plan)
+    assert torch.equal(out, x)
+    (out[:, :2].float() * 2).sum().backward()
+    want = torch.zeros_like(out)
+    want[:, :2] = 2
+    assert torch.equal(x.grad, want)
+    assert torch.equal(w.grad, (2 * x[:, :2].float().sum(1, keepdim=True)).expand(-1, 2))

@@ -363,3 +363,60 @@ def test_results_do_not_change_from_run_to_run_and_under_graphs():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(y, step()), i
+
+
+def test_rows_past_four_gigabytes():
+    """x of more than 2^32 bytes, in order and gathered."""
+    g = gen("far")
+    rows, cols = 300_000, 8192
+    x = torch.zeros(rows, cols, dtype=BF16, device="cuda")
+    some = torch.tensor([0, 1, 255_999, 262_143, 262_144, 299_904, 299_999])
+    x[some.cuda()] = torch.randn(len(some), cols, generator=g).to(BF16).cuda()
+    w = Weight(g, 32, cols, "int4", 128)
+    want = expected(x[some.cuda()].cpu(), w.values, w.sizes)
+    y = ops().w4a16_matmul(x, *w.cuda())
+    close(y[some.cuda()], *want)
+    assert not y[2:255_999].any() and not y[262_145:299_904].any()
+    several = [p.expand(3, *p.shape) if p is not None else None for p in w.cuda()]         # the same weight thrice
+    for n in (1, 40):
+        y = ops().w4a16_experts_matmul(x, some.int().cuda().repeat(n), torch.tensor([0, 2 * n, 2 * n, 7 * n]).cuda(),
+                                       *several)
+        close(y, want[0].repeat(n, 1), want[1].repeat(n, 1))
+
+
+def test_bytes_off_every_boundary():
+    """MXFP4 codes whose rows and experts lie at odd bytes."""
+    g = gen("odd")
+    w = Weight(g, 24, 96, "mxfp4", 32, experts=3)
+    x = torch.randn(60, 96, generator=g).to(BF16)
+    offsets = torch.tensor([0, 20, 20, 60])
+    p, s, _ = w.cuda()
+    for lead, pitch, gap in ((1, 48, 0), (0, 53, 0), (0, 52, 1), (4, 52, 2)):
+        flat = torch.zeros(lead + 3 * (24 * pitch + gap), dtype=torch.uint8, device="cuda")
+        view = flat.as_strided((3, 24, 48), (24 * pitch + gap, pitch, 1), lead)
+        view.copy_(p)
+        y = ops().w4a16_experts_matmul(x.cuda(), None, offsets.cuda(), view, s).cpu()
+        for e in (0, 2):
+            a, b = int(offsets[e]), int(offsets[e + 1])
+            close(y[a:b], *expected(x[a:b], w.values[e], w.sizes[e]))
+
+
+def test_two_calls_at_once():
+    """Calls on two streams, whose workspaces are their own."""
+    g = gen("streams")
+    w = Weight(g, 256, 1024, "int4z", 32)
+    parts = w.cuda()
+    xs = [torch.randn(r, 1024, generator=g).to(BF16) for r in (200, 333)]
+    gs = [x.cuda() for x in xs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in xs]
+    ys = [[], []]
+    for _ in range(4):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                ys[i].append(ops().w4a16_matmul(gs[i], *parts, group_size=32))
+    torch.cuda.synchronize()
+    for x, got in zip(xs, ys):
+        want = expected(x, w.values, w.sizes)
+        for y in got:
+            close(y, *want)

@@ -23,6 +23,7 @@ def w4(lib, **k):
     (dict(fmt=_lib.W4_MXFP4, group=128), "MXFP4"), (dict(fmt=_lib.W4_MXFP4, group=32, z=P), "MXFP4"),
     (dict(fmt=_lib.W4_MXFP4, group=32, cols=264), "MXFP4"), (dict(x=None), "null"), (dict(w=None), "null"),
     (dict(ldw=64), "overlap"), (dict(ldw=130), "4-byte"), (dict(w=C.c_void_p(18)), "4-byte"), (dict(ldy=15), "overlap"),
+    (dict(ldx=-256), "pitch"), (dict(group=2 ** 63 - 1, x=None), "null"),
     (dict(offsets=P, rows=2 ** 31, n_x=2 ** 31), "too many"),
 ])
 def test_product_arguments(args, needle):
@@ -41,6 +42,7 @@ def test_workspaces():
     assert f(1, 1, 1, 4096, 4096, _lib.W4_INT4, 128) == 0
     assert f(0, 0, 1, 4096, 4096, _lib.W4_INT4, 128) == 0
     assert f(-1, 4, 1, 16, 64, _lib.W4_INT4, 0) == 0
+    assert f(256, 256, 1, 512, 1024, _lib.W4_INT4, 2 ** 63 - 1) == f(256, 256, 1, 512, 1024, _lib.W4_INT4, 1024)
     # many rows: sums of x and factors (three 16-bit pieces a group), scales in fp32, a copy of x
     assert f(256, 256, 1, 512, 1024, _lib.W4_INT4, 128) >= (256 + 512) * 3 * 16 * 2 + 512 * 16 * 4 + 256 * 1024 * 2
     g = lib.mi355q_moe_plan_workspace_size
