@@ -31,25 +31,31 @@ int join_parts(const W4Args& g, uint32_t splits, const float* parts, hipStream_t
   return MI355Q_OK;
 }
 
-// Up to this many rows (per expert, in the mean) the weight's bytes decide.  4096 x 4096: 64 rows 22 us here, 24 in
-// tiles; 128 experts of 1536 x 2048: 8 rows each 72 and 83, 16 rows 109 and 88 (groups of 32, whose scales the tiles
-// have laid out first: 137 and 180).
-static bool few_rows(int64_t rows, int64_t experts, int64_t group) {
-  return rows <= (experts == 1 ? 64 : group < 128 ? 20 : 10) * experts;
+// Up to this many rows the weight's bytes decide, and the kernel for few rows is the faster one.  One weight: 64 rows of
+// 4096 x 4096 20 us, in tiles 23 (14336 x 4096 30 and 27); 128 rows 23 and 24 (56 and 33).  The tiles have the scales
+// laid out first, which costs some 10 us and what the scales weigh: 128 experts of 1536 x 2048 in groups of 128, 2 rows
+// each 34 and 44 us, 3 rows 43 and 43, 4 rows 51 and 45; 8 experts of 8192 x 4096 6 rows each 40 and 48, 8 rows 50 and
+// 48.  The 128 experts in groups of 64: 8 rows 68 and 72, 10 rows 77 and 73; of 32: 12 rows 114 and 135, 16 rows 134 and
+// 149, 24 rows 241 and 155; MXFP4 8 rows 65 and 82, 12 rows 86 and 86, 16 rows 103 and 97.
+static bool few_rows(int64_t rows, int64_t experts, int64_t group, bool mx) {
+  if (experts == 1) return rows <= 64;
+  return rows <= 40 + experts * (group >= 128 ? 3 : group >= 64 ? 9 : mx ? 12 : 16);
 }
 
 // Rows per tile (4 or 16 mt), columns, waves and splits of a call of few rows.
 //
 // A wave's loads are x's and the weight's, and it takes some 2048 waves to keep the memory busy.  Up
-// to 4 rows: one column tile a wave, and as many waves on one tile's sum as make 2048 (14336 x
-// 4096 9.3 us with two, 10.4 with eight; 4096 x 4096 6.2 and 5.1; gated ones have two column tiles, experts_token's
-// 8 x 1536 x 2048 7.8 us).  More rows: x is what is loaded most, so a wave takes up to four column tiles (16 x
+// to 4 rows (of experts: where a quarter of them have a row, as more rows of one would read its weight again: 128
+// experts of 1536 x 2048, 32 rows 20 us in both, 64 rows 29 in tiles of 4 and 20 in tiles of 16): one column tile a
+// wave, and as many waves on one tile's sum as make 2048 (14336 x
+// 4096 9.3 us with two, 10.4 with eight; 4096 x 4096 6.2 and 5.1; gated ones have two column tiles, 8 experts of
+// 1536 x 2048 7.8 us).  More rows: x is what is loaded most, so a wave takes up to four column tiles (16 x
 // 14336 x 4096 14.7 us, with two 16.9, with one 22.5), and where that leaves CUs idle the sum is split over
 // workgroups (23 x 4096 x 14336 34 us whole, 21 in four).  Tiles of experts are many: one or two waves each
 // (61 tokens to 8 of 128 experts of 1536 x 2048 54 us, with four waves 85).
 static FewPlan few_plan(int64_t rows, int64_t experts, int64_t out, int64_t cols, bool gated) {
   const int64_t mean = (rows + experts - 1) / experts, steps = (cols + kStep - 1) / kStep;
-  FewPlan p = {mean <= (experts > 1 ? 1 : 4) ? 0 : mean <= 16 ? 1 : mean <= 32 ? 2 : 4, 1, 8, 1};
+  FewPlan p = {(experts > 1 ? 4 * rows <= experts : rows <= 4) ? 0 : mean <= 16 ? 1 : mean <= 32 ? 2 : 4, 1, 8, 1};
   const int64_t row_tiles = experts > 1 ? (rows < experts ? rows : experts) : (rows + 63) / 64;
   if (p.mt == 0) {
     p.nt = gated ? 2 : 1;
@@ -81,10 +87,11 @@ static size_t few_bytes(int64_t rows, int64_t experts, int64_t out, int64_t cols
 extern "C" size_t mi355q_w4a16_matmul_workspace_size(int64_t n_x, int64_t rows, int64_t experts, int64_t out,
                                                      int64_t cols, mi355q_w4_format format, int64_t group_size) {
   if (n_x <= 0 || rows <= 0 || experts <= 0 || out <= 0 || cols <= 0 || group_size <= 0) return 0;
+  const bool mx = format == MI355Q_W4_MXFP4;
   if (group_size > cols) group_size = cols;
-  if (few_rows(rows, experts, group_size)) return few_bytes(rows, experts, out, cols);
+  if (few_rows(rows, experts, group_size, mx)) return few_bytes(rows, experts, out, cols);
   return w4_tiles_workspace(n_x, rows, experts, experts * out, cols,
-                            (uint32_t)((cols + group_size - 1) / group_size), format == MI355Q_W4_MXFP4);
+                            (uint32_t)((cols + group_size - 1) / group_size), mx);
 }
 
 extern "C" int mi355q_w4a16_matmul(const void* x_dev, mi355q_dtype x_dtype, int64_t n_x, int64_t ldx,
@@ -132,12 +139,12 @@ extern "C" int mi355q_w4a16_matmul(const void* x_dev, mi355q_dtype x_dtype, int6
               fast_div((uint32_t)((group_size + kStep - 1) / kStep)), gated != 0};
   const int kind = mx ? kMxfp4 : zeros_dev ? kInt4Zero : kInt4;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (!few_rows(rows, experts, group_size) && w4_tiles_fit(g, kind) && workspace_dev && aligned16(workspace_dev) &&
+  if (!few_rows(rows, experts, group_size, mx) && w4_tiles_fit(g, kind) && workspace_dev && aligned16(workspace_dev) &&
       workspace_bytes >= w4_tiles_workspace(n_x, rows, experts, experts * out, cols, g.groups, mx))
     return launch_w4_tiles(g, x_dtype, kind, workspace_dev, st);
   FewPlan p = few_plan(rows, experts, out, cols, gated);
   // (rows behind the last expert's and rows that x does not have become zeros where the sum is whole)
-  if (rows_dev || offsets_dev || !few_rows(rows, experts, group_size) || !workspace_dev || !aligned16(workspace_dev) ||
+  if (rows_dev || offsets_dev || !few_rows(rows, experts, group_size, mx) || !workspace_dev || !aligned16(workspace_dev) ||
       workspace_bytes < few_bytes(rows, experts, out, cols))
     p.splits = 1;
   float* const parts = static_cast<float*>(workspace_dev);
