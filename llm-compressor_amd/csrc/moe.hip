@@ -25,7 +25,8 @@ namespace mi355q {
 // ---------------------------------------------------------------- plan
 // Workgroups of 8 waves take `chunk` consecutive pairs each, a wave an eighth of
 // them.  With one workgroup the plan is one launch; else a first launch leaves each
-// chunk's counts per expert, and the second adds up those before its own.
+// chunk's counts per expert, and the second adds up those before its own.  Latency bounds it: one token's 8 pairs
+// 3.2 us, 8192 tokens to 8 of 128 experts (32 chunks) 2.5 and 8.9 us.
 constexpr int kPlanWaves = 8, kPlanThreads = 64 * kPlanWaves;
 constexpr int kMaxExperts = 2040;                   // 8 waves' counts of E + 1 ids in 64 KB of LDS
 constexpr int kPlanChunk = 2048;                    // pairs per workgroup, at the least
@@ -250,7 +251,7 @@ __device__ __forceinline__ void by_fullness(bool full, Fn&& f) {
 // The kernels below take K of a token's pairs at a time, whose rows are in flight together.
 //
 // A thread takes 16 bytes of one token: loaded once, stored `top` times.
-// NT: what moves once bypasses the caches.
+// NT: what moves once bypasses the caches.  8192 tokens of 2048 bf16 to 8 experts, 302 MB: 54 to 60 us, 5.0 to 5.6 TB/s.
 template <class T, int K, bool NT>
 __global__ __launch_bounds__(256) void moe_sort_kernel(RowsArgs g) {
   using raw = typename T::raw;
@@ -272,7 +273,9 @@ __global__ __launch_bounds__(256) void moe_sort_kernel(RowsArgs g) {
   });
 }
 
-// A thread takes 16 bytes of one token's sum.
+// A thread takes 16 bytes of one token's sum; the K rows' loads are what keeps the memory busy.  8192 tokens of 2048
+// bf16 from 8 experts: 52 to 54 us, 5.6 to 5.8 TB/s.  (Row after row and without going around the caches sort and
+// combine took 179 and 292 us there with their gradients, now 124 and 160.)
 template <class T, int K, bool NT>
 __global__ __launch_bounds__(256) void moe_combine_kernel(RowsArgs g) {
   using raw = typename T::raw;
@@ -331,7 +334,8 @@ __device__ __forceinline__ float sum_values(float (&v)[K], int lane) {
 }
 
 // W waves take one token: they read its gradient and its experts' rows, write the rows' gradients and add up the
-// weights' over the row.
+// weights' over the row.  8192 tokens of 2048 bf16, 8 experts, 570 MB: 106 to 113 us, 5.0 to 5.4 TB/s.  Rows of up to
+// 1 KB have a wave per token, longer ones a workgroup, so that few tokens fill the CUs too.
 template <class T, int K, int W, bool NT>
 __global__ __launch_bounds__(256) void moe_combine_backward_kernel(RowsArgs g) {
   using raw = typename T::raw;
@@ -501,8 +505,8 @@ int mi355q_moe_plan(const void* ids_dev, int id_bits, int64_t tokens, int64_t to
 
 int mi355q_moe_sort(const void* x_dev, mi355q_dtype dtype, int64_t tokens, int64_t top, int64_t cols, int64_t ldx,
                     const int32_t* slots_dev, const int64_t* end_dev, void* y_dev, int64_t ldy, void* stream) {
-  RowsArgs g = {x_dev, ldx, nullptr, 0, nullptr, 0, slots_dev, end_dev, tokens * top, y_dev, ldy, nullptr, (uint32_t)tokens,
-                (uint32_t)top, cols, {}};
+  RowsArgs g = {x_dev, ldx, nullptr, 0, nullptr, 0, slots_dev, end_dev, tokens * top, y_dev, ldy, nullptr,
+                (uint32_t)tokens, (uint32_t)top, cols, {}};
   const int rc = check_rows(g, tokens, top, cols, dtype);
   if (rc != MI355Q_OK || tokens == 0) return rc;
   MQ_CHECK_ARG(x_dev && y_dev, "moe_sort: a null operand");

@@ -1,21 +1,26 @@
 // Products of 16-bit activations with 4-bit weights (w4a16.h) for many rows: tiles on
 // the matrix instructions.
 //
-// A workgroup of four waves makes 32 MTW rows by 128 NTW columns of y, each wave all of
+// A workgroup of four waves makes 32 MTW rows by 128 NTW columns of w, each wave all of
 // the rows and 32 NTW of the columns, in steps of 128 of the sum.  A step's rows of x go
 // global -> LDS by the LDS-DMA load, in 16-byte chunks placed so that an operand read
 // takes 16 different bank groups, and are read by all four waves; a weight's codes belong to one
-// wave, so they go straight into its registers and are converted there once per step.
+// wave, go through its part of LDS the same way (a load into registers would have the compiler wait for the DMA
+// requested before it), and are converted once per step.  Both are requested a step ahead.
 //
-// Per 32 x 32 tile and group the MFMAs start from zero and acc += s * tile follows in fp32.
-// The conversions give codes 0 .. 15 (a signed one would cost more than it saves), and
-// the zero points' part of the sum,
+// Per 32 x 32 tile and group the MFMAs start from zero and acc += s * tile follows in fp32; in tiles of up to 64
+// rows two sets of sums take turns, one scaled while the other is made.  The conversions give codes 0 .. 15 (a
+// signed one would cost more than it saves), and the zero points' part of the sum,
 //   - sum_g s[n][g] z[n][g] sum_{k in g} x[m][k],
-// is a product of its own with one column per group: a first pass over x (prepare_kernel)
-// leaves the groups' sums as three bf16 numbers each (24 bits), the factors -s z are split
-// the same way, and the accumulators begin with the six products that count down to
-// 2^-24.  With 128 columns per group that is 1/43 of the MFMAs, 1/21 where s z has more bits
-// than bf16 holds.
+// is a product of its own with one column per group: a first pass (w4_prepare_kernel)
+// leaves the groups' sums of x as three bf16 numbers each (24 bits) and the factors -s z as one, two or three, as many
+// as s z has bits for, and the accumulators begin with the products that count down to 2^-24: three of 1/128
+// of the sum's length where one piece holds a factor.  The same pass lays the scales out in fp32 by group, so that
+// a tile's 32 are neighbours, and costs 10 to 20 us.
+//
+// What bounds it (bf16, groups of 128): 8192 x 28672 x 4096, gated, takes 1.70 ms, 1.13 PFLOP/s, the MFMAs 56 % and the
+// vector unit 45 % busy at 1.9 GHz: power.  4096 tokens to 8 of 128 experts of 1536 x 2048 take 0.28 to 0.32 ms: the tiles
+// are 64 rows, so codes are converted twice as often (MFMAs 40 % busy), and an eighth of their rows is empty.
 #pragma once
 
 #include <type_traits>
@@ -129,7 +134,7 @@ __device__ __forceinline__ void w4_factors(const W4Args& g, uint32_t padded, int
       uint16_t p[3];
       split3(v, p);
 #pragma unroll
-        for (int k = 0; k < 3; ++k)
+      for (int k = 0; k < 3; ++k)
         if (k < pieces) factors[((e * g.out + c) * pieces + k) * padded + gi] = p[k];
     }
   }
@@ -507,38 +512,39 @@ void w4_tiles_kernel(W4Args g, W4Tiles o) {
       __builtin_amdgcn_sched_barrier(0);
       finish(UNITS - 1);
     } else {
+      // (256 columns by 128 rows: the registers hold no second set of sums)
 #pragma unroll
       for (int a = 0; a < NTW; ++a)
 #pragma unroll
         for (int j = 0; j < kSlices; ++j) convert(a, j);
 #pragma unroll
-    for (int b = 0; b < MTW; ++b) {
-      __builtin_amdgcn_sched_barrier(0);
-      f32x16_t p[NTW];
+      for (int b = 0; b < MTW; ++b) {
+        __builtin_amdgcn_sched_barrier(0);
+        f32x16_t p[NTW];
 #pragma unroll
-      for (int j = 0; j < kSlices; ++j) {
-        const u32x4_t v = read_x(b, j);
+        for (int j = 0; j < kSlices; ++j) {
+          const u32x4_t v = read_x(b, j);
 #pragma unroll
-        for (int a = 0; a < NTW; ++a) {
-          if constexpr (FOLD) {
-            acc[b][a] = mfma32<T>(v, q[a][j], acc[b][a]);
-          } else {
-            p[a] = mfma32<T>(v, q[a][j], j % PER ? p[a] : f32x16_t{});
-            if (j % PER == PER - 1) {
+          for (int a = 0; a < NTW; ++a) {
+            if constexpr (FOLD) {
+              acc[b][a] = mfma32<T>(v, q[a][j], acc[b][a]);
+            } else {
+              p[a] = mfma32<T>(v, q[a][j], j % PER ? p[a] : f32x16_t{});
+              if (j % PER == PER - 1) {
 #pragma unroll
-              for (int e = 0; e < 16; ++e) acc[b][a][e] = fmaf(p[a][e], sc[a][j / PER], acc[b][a][e]);
+                for (int e = 0; e < 16; ++e) acc[b][a][e] = fmaf(p[a][e], sc[a][j / PER], acc[b][a][e]);
+              }
             }
           }
         }
-      }
-      // two operand reads ahead of their MFMAs
-      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+        // two operand reads ahead of their MFMAs
+        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
 #pragma unroll
-      for (int j = 0; j < kSlices - 2; ++j) {
-        __builtin_amdgcn_sched_group_barrier(0x008, NTW, 0);
-        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        for (int j = 0; j < kSlices - 2; ++j) {
+          __builtin_amdgcn_sched_group_barrier(0x008, NTW, 0);
+          __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        }
       }
-    }
     }
     __builtin_amdgcn_sched_barrier(0);
     ra[0] ^= S::SLOT;

@@ -18,8 +18,9 @@ bool w4_tiles_fit(const W4Args& g, int kind) {
 // over several workgroups where even the smallest leave CUs idle.  4096 x 4096, tiles as rows x columns: 128 rows 25 us
 // (32 x 128 in two parts; 27 whole), 512 rows 35 (32 x 128; 64 x 256 58), 1024 rows 51 (64 x 128; 56 in 32 x 128), 2048
 // rows 80 (64 x 256; 84 in 64 x 128, 100 in 128 x 256); 1024 x 14336 x 4096 133 (128 x 256; 139 in 64 x 128).  128 x
-// 4096 x 14336 40 us in four parts, 45 in two.  128 experts of 1536 x 2048: 16 to 64 rows each 88 to 145 us in 32 x 256
-// (98 to 167 in 64 x 256), 256 rows 366 (379).
+// 4096 x 14336 40 us in four parts, 45 in two.  128 experts of 1536 x 2048, 32, 64 and 128 x 256: 64 rows each 127, 140
+// and 165 us, 128 rows 209, 200 and 238, 256 rows 372, 341 and 343; 8 experts of 8192 x 4096, 250 rows each 242, 201 and
+// 220, 750 rows 575, 513 and 486.  Rows told apart by experts or an index (`listed`) keep their sums whole.
 TilePlan tile_plan(int64_t rows, int64_t experts, int64_t out, int64_t cols, bool gated, bool listed) {
   const int64_t steps = (cols + kStep - 1) / kStep, mean = rows / experts;
   if (experts > 1 || listed) {

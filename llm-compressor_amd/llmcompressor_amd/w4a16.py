@@ -132,7 +132,8 @@ class W4A16Linear(torch.nn.Module):
 class W4A16Experts(torch.nn.Module):
     """The experts of an MoE layer on stacked 4-bit weights: down(silu(gate x)
     * (up x)) of every token's experts, weighted and summed.  Three launches behind
-    the plan's, whatever the number of experts, and none waits for the host."""
+    the plan's (one more before a product of many rows), whatever the number of
+    experts, and none waits for the host."""
 
     def __init__(self, gate_up, down, num_experts: int, intermediate_size: int):
         """``gate_up`` [experts, 2 intermediate, hidden] (gate's rows first) and
