@@ -71,9 +71,9 @@ struct W4Batch {
 // neither is stored.  GPS: scales per step, 0: one for several steps.
 //
 // One token, 14336 x 4096 in groups of 128: 9.3 us, 3.2 TB/s (reading the same 30 MB alone 6.0, a launch of nothing 1.8).
-// 23 rows, 4096 x 14336 MXFP4: 19.7 us with the join; the MFMAs are 6 % busy, a wave's 3 or 4 steps wait for
-// their loads one after the other.  61 tokens to 8 of 128 experts, 1536 x 2048 in groups of 32 with zero points: 56 us,
-// 4.1 TB/s.
+// 23 rows, 4096 x 14336 MXFP4: 19.7 us with the join; the MFMAs are 6 % busy, and it is x's loads that count, which every
+// 64 columns read anew (two column tiles a wave 25 us; two steps in flight instead of one 21).  61 tokens to 8
+// of 128 experts, 1536 x 2048 in groups of 32 with zero points: 56 us, 4.1 TB/s.
 template <class T, int KIND, int GPS, int ES, int MT, int NT, int W, int D>
 __global__ __launch_bounds__(64 * W) void w4_few_kernel(W4Args g, uint32_t nt, uint32_t splits, float* parts) {
   constexpr bool FOLD = KIND == kMxfp4 && T::code == MI355Q_BF16;     // the scale is in the operand
