@@ -105,7 +105,7 @@ __global__ __launch_bounds__(kPlanThreads) void moe_place_kernel(PlanArgs g) {
     atomicAdd(&mine[id_of(g, f, t, k)], 1u);
   }
   __syncthreads();
-  uint32_t run = 0;                                            // pairs of the ids before this round's
+  uint32_t run = 0;                                            // pairs of the ids before these
   for (uint32_t e0 = 0; e0 < ids; e0 += kPlanThreads) {
     const uint32_t e = e0 + threadIdx.x;
     uint32_t all = 0, before = 0;

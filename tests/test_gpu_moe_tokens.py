@@ -255,3 +255,33 @@ def test_rows_past_four_gigabytes():
     want[:, :2] = 2
     assert torch.equal(x.grad, want)
     assert torch.equal(w.grad, (2 * x[:, :2].float().sum(1, keepdim=True)).expand(-1, 2))
+
+
+def test_replayed_gradients_follow_their_inputs():
+    """Forward and backward in one graph, no eager graph of the leaves alive while it is captured."""
+    g = torch.Generator().manual_seed(17)
+    ids = torch.randint(0, 6, (70, 3), generator=g).cuda()
+    x = torch.randn(70, 96, generator=g).to(BF16).cuda().requires_grad_()
+    w = torch.rand(70, 3, generator=g).cuda().requires_grad_()
+    d = torch.randn(70, 96, generator=g).to(BF16).cuda()
+    m = moe()
+
+    def step():
+        rows, plan = m.sort_tokens(x, ids, 6)
+        return torch.autograd.grad(m.combine_tokens(rows, w, plan), (x, w), d)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    for i in range(3):
+        ids.add_(1).remainder_(7)                               # 6: of no expert
+        with torch.no_grad():
+            x.mul_(-0.5)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(captured, step())), i
