@@ -43,6 +43,13 @@ __device__ __forceinline__ u32x4_t last_chunk(const uint16_t* p, int64_t left) {
   return u32x4_t{(uint32_t)v[0], (uint32_t)(v[0] >> 32), (uint32_t)v[1], (uint32_t)(v[1] >> 32)};
 }
 
+// The scales' type is a parameter of the kernel (Bf16, F16, F32, and this for MXFP4's bytes).  Told apart by a branch
+// between a step's matrix instructions and its sums, the compiler counted the wait for their results along the longer of
+// the branch's two paths alone, and the other one read the last registers before they were written.
+struct E8m0 {
+  typedef uint8_t raw;
+};
+
 // ---------------------------------------------------------------- few rows
 // The operands, scales and zero points of steps_ neighbouring steps as loaded.
 template <int steps_, int NT, int MB, int XL, int GPS, int ES>
@@ -74,8 +81,9 @@ struct W4Batch {
 // 23 rows, 4096 x 14336 MXFP4: 19.7 us with the join; the MFMAs are 6 % busy, and it is x's loads that count, which every
 // 64 columns read anew (two column tiles a wave 25 us; two steps in flight instead of one 21).  61 tokens to 8
 // of 128 experts, 1536 x 2048 in groups of 32 with zero points: 56 us, 4.1 TB/s.
-template <class T, int KIND, int GPS, int ES, int MT, int NT, int W, int D>
+template <class T, int KIND, int GPS, class S, int MT, int NT, int W, int D>
 __global__ __launch_bounds__(64 * W) void w4_few_kernel(W4Args g, uint32_t nt, uint32_t splits, float* parts) {
+  constexpr int ES = sizeof(typename S::raw);
   constexpr bool FOLD = KIND == kMxfp4 && T::code == MI355Q_BF16;     // the scale is in the operand
   using Sum = typename std::conditional<MT == 0, float, f32x4_t>::type;
   constexpr int MB = MT ? MT : 1;
@@ -180,7 +188,6 @@ __global__ __launch_bounds__(64 * W) void w4_few_kernel(W4Args g, uint32_t nt, u
         o.x[0][b][i] = last_chunk(xp[b] + (int64_t)s * kStep + 32 * i,
                                   g.cols - (int64_t)s * kStep - 32 * (MT ? i : col & 3) - 8 * quarter);
   };
-  const bool bf16_scales = g.s_type == MI355Q_BF16;
   // the scales of step d of a batch
   auto scales = [&](const auto& o, int d, float (&sc)[NT][G1]) __attribute__((always_inline)) {
     if constexpr (KIND == kMxfp4) {
@@ -201,17 +208,10 @@ __global__ __launch_bounds__(64 * W) void w4_few_kernel(W4Args g, uint32_t nt, u
         const int at = GPS ? d * GPS + i : 2 * d;
         return at & 1 ? o.s[a][at / 2] >> 16 : o.s[a][at / 2] & 0xffffu;
       };
-      if (bf16_scales) {
 #pragma unroll
-        for (int a = 0; a < NT; ++a)
+      for (int a = 0; a < NT; ++a)
 #pragma unroll
-          for (int i = 0; i < G1; ++i) sc[a][i] = __uint_as_float(half(a, i) << 16);
-      } else {
-#pragma unroll
-        for (int a = 0; a < NT; ++a)
-#pragma unroll
-          for (int i = 0; i < G1; ++i) sc[a][i] = F16::load((uint16_t)half(a, i));
-      }
+        for (int i = 0; i < G1; ++i) sc[a][i] = S::load((uint16_t)half(a, i));
     }
   };
   constexpr uint32_t one = T::code == MI355Q_BF16 ? 0x3f803f80u : 0x3c003c00u;
@@ -384,7 +384,7 @@ __global__ __launch_bounds__(64 * W) void w4_few_kernel(W4Args g, uint32_t nt, u
   }
 }
 
-template <class T, int KIND, int GPS, int ES, int MT, int NT, int W, int D>
+template <class T, int KIND, int GPS, class S, int MT, int NT, int W, int D>
 static int launch_few(const W4Args& g, uint32_t splits, float* parts, hipStream_t st) {
   const int64_t width = g.gated ? g.out / 2 : g.out, per = 16 * (g.gated ? NT / 2 : NT);
   const int64_t nt = (width + per - 1) / per;
@@ -395,39 +395,46 @@ static int launch_few(const W4Args& g, uint32_t splits, float* parts, hipStream_
   if (g.offsets) mt = g.n_rows / ROWS + g.experts + 1 < g.n_rows ? g.n_rows / ROWS + g.experts + 1 : g.n_rows;
   MQ_CHECK_ARG(nt * mt * splits <= (int64_t)(UINT32_MAX / (64 * W)),
                "w4a16_matmul: %lld rows by %lld columns are too many", (long long)g.n_rows, (long long)width);
-  hipLaunchKernelGGL((w4_few_kernel<T, KIND, GPS, ES, MT, NT, W, D>), dim3((unsigned)(nt * mt * splits)), dim3(64 * W), 0,
+  hipLaunchKernelGGL((w4_few_kernel<T, KIND, GPS, S, MT, NT, W, D>), dim3((unsigned)(nt * mt * splits)), dim3(64 * W), 0,
                      st, g, (uint32_t)nt, splits, parts);
   MQ_LAUNCH_CHECK();
   return splits > 1 ? join_parts(g, splits, parts, st) : MI355Q_OK;
 }
 
-template <class T, int KIND, int GPS, int ES>
+template <class T, int KIND, int GPS, class S>
 static int launch_kind(const W4Args& g, const FewPlan& p, float* parts, hipStream_t st) {
   const uint32_t splits = p.splits;
-  if (p.mt == 4) return launch_few<T, KIND, GPS, ES, 4, 4, 8, 1>(g, splits, parts, st);
-  if (p.mt == 2) return launch_few<T, KIND, GPS, ES, 2, 4, 8, 1>(g, splits, parts, st);
+  if (p.mt == 4) return launch_few<T, KIND, GPS, S, 4, 4, 8, 1>(g, splits, parts, st);
+  if (p.mt == 2) return launch_few<T, KIND, GPS, S, 2, 4, 8, 1>(g, splits, parts, st);
   if (p.mt == 1) {
-    if (p.w == 1) return launch_few<T, KIND, GPS, ES, 1, 2, 1, 2>(g, 1, parts, st);
-    if (p.nt == 4) return launch_few<T, KIND, GPS, ES, 1, 4, 4, 2>(g, 1, parts, st);
-    if (p.nt == 2) return launch_few<T, KIND, GPS, ES, 1, 2, 4, 2>(g, 1, parts, st);
-    return launch_few<T, KIND, GPS, ES, 1, 1, 8, 2>(g, 1, parts, st);
+    if (p.w == 1) return launch_few<T, KIND, GPS, S, 1, 2, 1, 2>(g, 1, parts, st);
+    if (p.nt == 4) return launch_few<T, KIND, GPS, S, 1, 4, 4, 2>(g, 1, parts, st);
+    if (p.nt == 2) return launch_few<T, KIND, GPS, S, 1, 2, 4, 2>(g, 1, parts, st);
+    return launch_few<T, KIND, GPS, S, 1, 1, 8, 2>(g, 1, parts, st);
   }
   if (p.nt == 2) {
-    if (p.w == 2) return launch_few<T, KIND, GPS, ES, 0, 2, 2, 4>(g, 1, parts, st);
-    if (p.w == 4) return launch_few<T, KIND, GPS, ES, 0, 2, 4, 2>(g, 1, parts, st);
-    return launch_few<T, KIND, GPS, ES, 0, 2, 8, 2>(g, 1, parts, st);
+    if (p.w == 2) return launch_few<T, KIND, GPS, S, 0, 2, 2, 4>(g, 1, parts, st);
+    if (p.w == 4) return launch_few<T, KIND, GPS, S, 0, 2, 4, 2>(g, 1, parts, st);
+    return launch_few<T, KIND, GPS, S, 0, 2, 8, 2>(g, 1, parts, st);
   }
-  if (p.w == 2) return launch_few<T, KIND, GPS, ES, 0, 1, 2, 4>(g, 1, parts, st);
-  if (p.w == 4) return launch_few<T, KIND, GPS, ES, 0, 1, 4, 4>(g, 1, parts, st);
-  return launch_few<T, KIND, GPS, ES, 0, 1, 8, 2>(g, 1, parts, st);
+  if (p.w == 2) return launch_few<T, KIND, GPS, S, 0, 1, 2, 4>(g, 1, parts, st);
+  if (p.w == 4) return launch_few<T, KIND, GPS, S, 0, 1, 4, 4>(g, 1, parts, st);
+  return launch_few<T, KIND, GPS, S, 0, 1, 8, 2>(g, 1, parts, st);
 }
 
-template <class T, int KIND, int ES>
+template <class T, int KIND, class S>
+static int launch_scales(const W4Args& g, const FewPlan& p, float* parts, hipStream_t st) {
+  if (g.groups > 1 && g.group == 32) return launch_kind<T, KIND, 4, S>(g, p, parts, st);
+  if (g.groups > 1 && g.group == 64) return launch_kind<T, KIND, 2, S>(g, p, parts, st);
+  if (g.per.d == 1) return launch_kind<T, KIND, 1, S>(g, p, parts, st);
+  return launch_kind<T, KIND, 0, S>(g, p, parts, st);
+}
+
+template <class T, int KIND>
 static int launch_groups(const W4Args& g, const FewPlan& p, float* parts, hipStream_t st) {
-  if (g.groups > 1 && g.group == 32) return launch_kind<T, KIND, 4, ES>(g, p, parts, st);
-  if (g.groups > 1 && g.group == 64) return launch_kind<T, KIND, 2, ES>(g, p, parts, st);
-  if (g.per.d == 1) return launch_kind<T, KIND, 1, ES>(g, p, parts, st);
-  return launch_kind<T, KIND, 0, ES>(g, p, parts, st);
+  if (g.s_type == MI355Q_F32) return launch_scales<T, KIND, F32>(g, p, parts, st);
+  if (g.s_type == MI355Q_BF16) return launch_scales<T, KIND, Bf16>(g, p, parts, st);
+  return launch_scales<T, KIND, F16>(g, p, parts, st);
 }
 
 }  // namespace mi355q

@@ -4,9 +4,8 @@
 namespace mi355q {
 
 int launch_w4_few_bf16(const W4Args& g, int kind, const FewPlan& p, float* parts, hipStream_t st) {
-  if (kind == kMxfp4) return launch_kind<Bf16, kMxfp4, 4, 1>(g, p, parts, st);
-  return g.s_type == MI355Q_F32 ? launch_groups<Bf16, kInt4, 4>(g, p, parts, st)
-                                : launch_groups<Bf16, kInt4, 2>(g, p, parts, st);
+  if (kind == kMxfp4) return launch_kind<Bf16, kMxfp4, 4, E8m0>(g, p, parts, st);
+  return launch_groups<Bf16, kInt4>(g, p, parts, st);
 }
 
 }  // namespace mi355q

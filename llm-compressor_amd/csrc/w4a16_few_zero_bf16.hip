@@ -4,8 +4,7 @@
 namespace mi355q {
 
 int launch_w4_few_zero_bf16(const W4Args& g, const FewPlan& p, float* parts, hipStream_t st) {
-  return g.s_type == MI355Q_F32 ? launch_groups<Bf16, kInt4Zero, 4>(g, p, parts, st)
-                                : launch_groups<Bf16, kInt4Zero, 2>(g, p, parts, st);
+  return launch_groups<Bf16, kInt4Zero>(g, p, parts, st);
 }
 
 }  // namespace mi355q
