@@ -338,7 +338,7 @@ __global__ __launch_bounds__(64 * W) void w4_few_kernel(W4Args g, uint32_t nt, u
     for (int w = 1; w < W; ++w) t += sums[w][a][b][lane];
     __builtin_memcpy(v, &t, sizeof(t));
     const int64_t n = column(a) + col;
-    if (g.bias && n < g.out && splits == 1) {
+    if (g.bias && n < g.out && splits == 1 && tile.expert >= 0) {      // (rows of no expert are zeros)
       const float bias = load_any(g.bias, g.bias_type, n);
 #pragma unroll
       for (int r = 0; r < REGS; ++r) v[r] += bias;

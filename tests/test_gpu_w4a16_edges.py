@@ -1,0 +1,51 @@
+"""4-bit products where the definition says what is easily got wrong: rows of no expert beside a bias, rows before the
+first expert's, gates at the ends of fp32's range, every byte that MXFP4's scales can have."""
+import ctypes as C
+
+import pytest
+import torch
+
+from test_gpu_w4a16 import BF16, E2M1, F16, F32, Weight, close, expected, gen, ops
+
+pytestmark = pytest.mark.gpu
+
+
+def entry(x, w, fmt, offsets, experts, group, out, gated, y, bias=None, rows_index=None, n_x=None, workspace=True):
+    """The C entry, for what the Python functions do not pass."""
+    from llmcompressor_amd import _lib as L
+    dt = {BF16: L.BF16, F16: L.F16, F32: L.F32}
+    p, s, z = w
+    cols, rows = x.shape[1], y.shape[0]
+    n_x = x.shape[0] if n_x is None else n_x
+    need = L.lib().mi355q_w4a16_matmul_workspace_size(n_x, rows, experts, out, cols, fmt, group) if workspace else 0
+    ws = torch.empty(need, dtype=torch.uint8, device="cuda") if need else None
+    per = lambda t: 0 if t is None or t.dim() < 3 else t.stride(0)     # noqa: E731
+    L.check(L.lib().mi355q_w4a16_matmul(
+        x.data_ptr(), dt[x.dtype], n_x, x.stride(0), L.ptr(rows_index), L.ptr(offsets), experts, p.data_ptr(), fmt,
+        p.stride(-2) * p.element_size(), per(p) * p.element_size(), s.data_ptr(), dt.get(s.dtype, L.BF16), s.stride(-2),
+        per(s), L.ptr(z), 0 if z is None else z.stride(-2), per(z), group, L.ptr(bias),
+        dt[bias.dtype] if bias is not None else 0, int(gated), y.data_ptr(), dt[y.dtype], y.stride(0), rows, out, cols,
+        L.ptr(ws), C.c_size_t(need), L.stream_of(x)))
+    torch.cuda.synchronize()
+    return y
+
+
+# ---------------------------------------------------------------- rows of no expert
+# 9, 40: tiles of few rows; 200, 400: of many; 200 without a workspace: few again
+@pytest.mark.parametrize("rows,workspace", [(3, True), (9, True), (40, True), (200, True), (200, False), (400, True)])
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("kind", ["int4", "int4z", "mxfp4"])
+def test_rows_of_no_expert_have_no_bias(rows, workspace, gated, kind):
+    from llmcompressor_amd import _lib as L
+    g = gen("bias", rows, gated)
+    out, cols = 96, 256
+    x = torch.randn(rows, cols, generator=g).to(BF16)
+    w = Weight(g, out, cols, kind, 32, experts=2)
+    b = torch.randn(out, generator=g).to(BF16)
+    ends = [0, rows // 3, rows - rows // 3]
+    y = torch.full((rows, out // 2 if gated else out), float("nan"), dtype=BF16, device="cuda")
+    entry(x.cuda(), w.cuda(), L.W4_MXFP4 if kind == "mxfp4" else L.W4_INT4, torch.tensor(ends).cuda(), 2, 32, out, gated,
+          y, b.cuda(), workspace=workspace)
+    for e in range(2):
+        close(y[ends[e]:ends[e + 1]], *expected(x[ends[e]:ends[e + 1]], w.values[e], w.sizes[e], b, gated))
+    assert not y[ends[-1]:].any()
