@@ -99,7 +99,7 @@ __device__ __forceinline__ float silu(float v) {
 
 // ---------------------------------------------------------------- tiles of rows
 // The rows [first, first + count) of y that a tile of ROWS rows holds, and their
-// expert (-1: rows behind the last expert's, which are written as zeros).
+// expert (-1: rows before the first expert's and behind the last one's, which are written as zeros).
 struct RowTile {
   int64_t first;
   int count, expert;
@@ -114,13 +114,14 @@ __device__ __forceinline__ RowTile find_row_tile(const W4Args& g, uint32_t id) {
     return {first, (int)(left < ROWS ? left : ROWS), 0};
   }
   const int lane = threadIdx.x & 63, n_rows = (int)g.n_rows;
+  // (the rows before the experts count as one, number -1, and so do those behind them)
   auto begin = [&](int e) __attribute__((always_inline)) {
-    const int64_t o = e <= g.experts ? g.offsets[e] : (int64_t)n_rows;
+    const int64_t o = e < 0 ? 0 : e <= g.experts ? g.offsets[e] : (int64_t)n_rows;
     return o < 0 ? 0 : o < n_rows ? (int)o : n_rows;
   };
   uint32_t left = id;
-  int a = begin(lane), b = begin(lane + 1);
-  for (int e0 = 0; e0 <= g.experts; e0 += 64) {          // (the rows behind the experts count as one)
+  int a = begin(lane - 1), b = begin(lane);
+  for (int e0 = -1; e0 <= g.experts; e0 += 64) {
     const int na = begin(e0 + 64 + lane), nb = begin(e0 + 65 + lane);
     const uint32_t tiles = b > a ? (uint32_t)(b - a + ROWS - 1) / ROWS : 0u;
     uint32_t sum = tiles;
@@ -134,7 +135,7 @@ __device__ __forceinline__ RowTile find_row_tile(const W4Args& g, uint32_t id) {
       const int src = __builtin_ctzll(past);
       const int first = __shfl(a, src), end = __shfl(b, src);
       const int in = (int)(left - __shfl(sum - tiles, src)) * ROWS, rest = end - first - in;
-      return {first + in, rest < ROWS ? rest : ROWS, e0 + src < g.experts ? e0 + src : -1};
+      return {first + in, rest < ROWS ? rest : ROWS, e0 + src < g.experts ? e0 + src : -1};    // (e0 + src: -1 and up)
     }
     left -= __shfl(sum, 63);
     a = na;
@@ -149,6 +150,13 @@ __device__ __forceinline__ RowTile row_tile(const W4Args& g, uint32_t id) {
   const int64_t first = (int64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)t.first) |
                         (int64_t)__builtin_amdgcn_readfirstlane((int)(t.first >> 32)) << 32;
   return {first, __builtin_amdgcn_readfirstlane(t.count), __builtin_amdgcn_readfirstlane(t.expert)};
+}
+
+// How many tiles a call with offsets may have, whatever they hold: no more than rows, and at most one short one per
+// expert, before them and behind them.
+inline int64_t most_row_tiles(const W4Args& g, int64_t tile_rows) {
+  const int64_t n = g.n_rows / tile_rows + g.experts + 2;
+  return n < g.n_rows ? n : g.n_rows;
 }
 
 // How a call of few rows is cut (w4a16_few.h): rows per tile (16 mt, or 4), column tiles and waves per

@@ -388,11 +388,8 @@ template <class T, int KIND, int GPS, class S, int MT, int NT, int W, int D>
 static int launch_few(const W4Args& g, uint32_t splits, float* parts, hipStream_t st) {
   const int64_t width = g.gated ? g.out / 2 : g.out, per = 16 * (g.gated ? NT / 2 : NT);
   const int64_t nt = (width + per - 1) / per;
-  // an expert's last tile may be short: no more tiles than rows, and at most one short one per expert
-  // (and one behind them)
   constexpr int ROWS = MT ? 16 * MT : 4;
-  int64_t mt = (g.n_rows + ROWS - 1) / ROWS;
-  if (g.offsets) mt = g.n_rows / ROWS + g.experts + 1 < g.n_rows ? g.n_rows / ROWS + g.experts + 1 : g.n_rows;
+  const int64_t mt = g.offsets ? most_row_tiles(g, ROWS) : (g.n_rows + ROWS - 1) / ROWS;
   MQ_CHECK_ARG(nt * mt * splits <= (int64_t)(UINT32_MAX / (64 * W)),
                "w4a16_matmul: %lld rows by %lld columns are too many", (long long)g.n_rows, (long long)width);
   hipLaunchKernelGGL((w4_few_kernel<T, KIND, GPS, S, MT, NT, W, D>), dim3((unsigned)(nt * mt * splits)), dim3(64 * W), 0,

@@ -685,8 +685,7 @@ static int launch_shape(W4Args g, W4Tiles o, hipStream_t st) {
   }
   const int64_t width = g.gated ? g.out / 2 : g.out, per = kWaves * (g.gated ? 16 * NTW : 32 * NTW);
   const int64_t ct = (width + per - 1) / per;
-  int64_t rt = (g.n_rows + R - 1) / R;
-  if (g.offsets) rt = g.n_rows / R + g.experts + 1 < g.n_rows ? g.n_rows / R + g.experts + 1 : g.n_rows;
+  const int64_t rt = g.offsets ? most_row_tiles(g, R) : (g.n_rows + R - 1) / R;
   int64_t rounded = rt;
   if (g.offsets) {                 // whole rounds of bands, a band for each XCD
     o.band = (uint32_t)(rt >= 512 ? 8 : rt >= 64 ? rt / 64 : 1);

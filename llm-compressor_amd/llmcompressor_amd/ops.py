@@ -1208,8 +1208,9 @@ def w4a16_experts_matmul(x: torch.Tensor, rows: torch.Tensor | None, offsets: to
     """``w4a16_matmul`` for rows grouped by expert, with the experts' weights
     stacked ([experts, ...] each): row i of y, offsets[e] <= i < offsets[e +
     1], is x[rows[i]] times expert e's weight (``rows`` int32, as ``moe_plan``
-    gives them, or None: x[i]).  ``offsets`` int64 [experts + 1] stays on the
-    device: the call waits for nothing.  Rows from offsets[-1] on are zeros."""
+    gives them, or None: x[i]).  ``offsets`` int64 [experts + 1], ascending, stays on
+    the device: the call waits for nothing.  Rows before offsets[0] (of experts
+    that others hold) and from offsets[-1] on are zeros."""
     if not offsets.is_cuda:
         L.require_gpu(offsets)
     if offsets.dtype != torch.int64 or offsets.dim() != 1 or offsets.shape[0] < 2:

@@ -49,3 +49,28 @@ def test_rows_of_no_expert_have_no_bias(rows, workspace, gated, kind):
     for e in range(2):
         close(y[ends[e]:ends[e + 1]], *expected(x[ends[e]:ends[e + 1]], w.values[e], w.sizes[e], b, gated))
     assert not y[ends[-1]:].any()
+
+
+@pytest.mark.parametrize("rows", [3, 40, 200, 400])
+@pytest.mark.parametrize("experts", [1, 3, 70])
+@pytest.mark.parametrize("gated", [False, True])
+def test_rows_before_the_first_expert_are_zeros(rows, experts, gated):
+    """Offsets of a part of the experts: others own the rows before them, and the rows behind."""
+    from llmcompressor_amd import _lib as L
+    g = gen("before", rows, experts)
+    out, cols = 64, 256
+    x = torch.randn(rows, cols, generator=g).to(BF16)
+    w = Weight(g, out, cols, "int4", 128, experts=experts)
+    first, last = rows // 2, rows - rows // 4
+    ends = sorted(torch.randint(first, last + 1, (experts - 1,), generator=g).tolist())
+    ends = [first, *ends, last]
+    for n in (1, experts):
+        part = torch.tensor(ends[:n] + [last])
+        y = torch.full((rows, out // 2 if gated else out), float("nan"), dtype=BF16, device="cuda")
+        p = [None if t is None else t[:n] for t in w.cuda()]
+        entry(x.cuda(), p, L.W4_INT4, part.cuda(), n, 128, out, gated, y)
+        for e in range(n):
+            a, b = int(part[e]), int(part[e + 1])
+            if a < b:
+                close(y[a:b], *expected(x[a:b], w.values[e], w.sizes[e], None, gated))
+        assert not y[:first].any() and not y[last:].any(), n
