@@ -89,12 +89,13 @@ __device__ __forceinline__ u32x4_t e2m1s(uint32_t w, float e) {
                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, e, 2)),
                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, e, 3))};
 }
+// v / (1 + e^-v) for every v: v itself far above zero, 0 far below, NaN for NaN and -infinity.
 __device__ __forceinline__ float silu(float v) {
-  // e^-v = 2^(-v log2 e), with what the product's rounding leaves put back; held within 2^+-126, where the sum with
-  // 1 has long lost the smaller one (without a branch: the compiler makes one of a choice of results)
+  // e^-v = 2^(-v log2 e), with what the product's rounding leaves put back as a factor: below 2^-16 where the
+  // exponential is neither 0 nor infinite, and held there where v log2 e passes fp32, so that it cannot become one
   const float k = -1.44269504f, t = v * k, r = fmaf(v, k, -t) + v * -1.92596299e-8f;
-  const float e = __builtin_amdgcn_exp2f(__builtin_amdgcn_fmed3f(t, -126.f, 126.f));
-  return v * __builtin_amdgcn_rcpf(1.f + fmaf(e, r * 0.693147181f, e));
+  const float e = __builtin_amdgcn_exp2f(t);
+  return v * __builtin_amdgcn_rcpf(1.f + e * fmaf(__builtin_amdgcn_fmed3f(r, -0x1p-10f, 0x1p-10f), 0.693147181f, 1.f));
 }
 
 // ---------------------------------------------------------------- tiles of rows

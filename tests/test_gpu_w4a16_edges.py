@@ -74,3 +74,44 @@ def test_rows_before_the_first_expert_are_zeros(rows, experts, gated):
             if a < b:
                 close(y[a:b], *expected(x[a:b], w.values[e], w.sizes[e], None, gated))
         assert not y[:first].any() and not y[last:].any(), n
+
+
+# ---------------------------------------------------------------- the ends of the range
+def one_gate(dtype, gate, rows):
+    """(x, packed, scales): MXFP4, of 32 columns of gate and 32 of up, whose gates are `gate` in every row and whose
+    ups are 1."""
+    exponent = 0 if dtype == BF16 else 112                       # fp16 activations end at 65504
+    x = torch.zeros(rows, 64, dtype=dtype)
+    x[:, 0], x[:, 32] = gate * 2.0 ** -exponent, 1
+    codes = torch.zeros(2, 64, dtype=torch.uint8)
+    codes[0, 0] = codes[1, 32] = 2                               # the code of 1
+    s = torch.tensor([[127 + exponent, 127], [127, 127]], dtype=torch.uint8)
+    return x, codes[:, 0::2] | (codes[:, 1::2] << 4), s
+
+
+@pytest.mark.parametrize("rows", [2, 9, 40, 130])
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("gate", [3.3e38, 2.4e38, 2.3e38, 1e30, 1e5])
+def test_gates_at_the_ends_of_the_range(rows, dtype, gate):
+    """silu(gate) is the gate far above zero and 0 far below, up to fp32's largest numbers; the quotient's and the
+    product's roundings are within 2^-20 of the value."""
+    x, p, s = one_gate(dtype, gate, rows)
+    want = x[0, 0].double() * (1.0 if dtype == BF16 else 2.0 ** 112)
+    for out_dtype in (F32, BF16):
+        y = ops().w4a16_matmul(x.cuda(), p.cuda(), s.cuda(), gated=True, out_dtype=out_dtype).cpu().double()
+        bound = 2.0 ** -20 + torch.finfo(out_dtype).eps / 2
+        assert bool(((y - want).abs() <= bound * want).all()), y.flatten()[:3]
+        y = ops().w4a16_matmul((-x * (torch.arange(64) < 32) + x * (torch.arange(64) >= 32)).cuda(), p.cuda(), s.cuda(),
+                               gated=True, out_dtype=out_dtype).cpu()
+        assert not y.any(), y.flatten()[:3]
+
+
+def test_gates_of_infinity():
+    """An infinite gate (bf16: the sum passes fp32) stays one; a gate of -infinity is NaN or 0, never something else."""
+    x, p, s = one_gate(BF16, 3.3e38, 4)
+    s[0, 0] = 129                                                # times 4
+    y = ops().w4a16_matmul(x.cuda(), p.cuda(), s.cuda(), gated=True, out_dtype=F32).cpu()
+    assert bool((y == float("inf")).all())
+    x[:, 0] *= -1
+    y = ops().w4a16_matmul(x.cuda(), p.cuda(), s.cuda(), gated=True, out_dtype=F32).cpu()
+    assert bool(((y == 0) | y.isnan()).all())
