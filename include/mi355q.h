@@ -660,7 +660,9 @@ int mi355q_moe_combine_backward(const void* dy_dev, mi355q_dtype dtype, int64_t 
  *   nibble n % 8 of word zeros[n / 8][g]; scales [out, ceil(cols / group_size)] in
  *   scales_dtype; group_size 32, 64, a multiple of 128, or at least cols.
  * MI355Q_W4_MXFP4 (mxfp4-pack-quantized): e2m1 codes, even column in the low nibble,
- *   scales are bytes e, 2^(e - 127), group_size 32, cols % 32 == 0.
+ *   scales are bytes e, 2^(e - 127) (255: NaN), group_size 32, cols % 32 == 0.  With
+ *   bf16 x the weights are bf16 numbers: those of 2^128 and more (e 253 and 254) are
+ *   infinite.
  * cols >= 8.  ldw and stride_w in bytes (multiples of 4), others in elements.
  * offsets_dev NULL: one weight for all rows; else expert e has rows
  * [offsets[e], offsets[e + 1]) of y and the weight at e times the strides (offsets ascend), and

@@ -12,8 +12,9 @@
 // zero point enters as the first addend of a group's sum, -z sum_k x[m][k], which one
 // more product per group forms (with a constant operand).  Group sums are scaled and
 // added in fp32, and the result is rounded once.  MXFP4 with bf16 activations has its
-// scale in the conversion, exact from 2^-117 up, so it needs no group sums; fp16's
-// range would not hold it.
+// scale in the conversion, exact down to byte 0 and up to 252, so it needs no group sums;
+// of bytes 253 and 254 the weights of 2^128 and more are infinite there, as in bf16.
+// fp16's range would not hold the weights, and its groups have their sums scaled.
 #pragma once
 
 #include "fp8.h"

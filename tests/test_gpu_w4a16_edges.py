@@ -115,3 +115,39 @@ def test_gates_of_infinity():
     x[:, 0] *= -1
     y = ops().w4a16_matmul(x.cuda(), p.cuda(), s.cuda(), gated=True, out_dtype=F32).cpu()
     assert bool(((y == 0) | y.isnan()).all())
+
+
+@pytest.mark.parametrize("rows", [1, 8, 40, 130])
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=["bf16", "fp16"])
+def test_every_scale_of_mxfp4(rows, dtype):
+    """Every byte e as 2^(e - 127), a row of w each, with all codes; activations that bring the results back into the
+    range (a power of two, by bytes in turn).  With bf16 activations a weight is a bf16 number, so those of 2^128 and
+    more (bytes 253 and 254) are infinite there.  255 is NaN."""
+    g = gen("bytes", rows)
+    codes = torch.stack([torch.randperm(16, generator=g).repeat(2) for _ in range(255)])
+    codes[:, 1] = 7                                              # a code of 6
+    e = torch.arange(255)
+    packed = (codes[:, 0::2] | (codes[:, 1::2] << 4)).to(torch.uint8)
+    values = E2M1[codes] * torch.exp2(e.double() - 127)[:, None]
+    nan = ops().w4a16_matmul(torch.ones(rows, 32, dtype=dtype).cuda(), packed[:9].cuda(),
+                             torch.full((9, 1), 255, dtype=torch.uint8).cuda())
+    assert bool(nan.isnan().all())
+    mantissas = torch.randint(-127, 128, (rows, 32), generator=g).double()
+    top = 15 if dtype == F16 else 127
+    for lo in range(0, 255, 16):
+        # |sums| between 2^-126 (normal numbers) and 2^127 for bytes lo .. lo + 15, as far as x's type goes
+        power = max(-14 if dtype == F16 else -100, min(top - 8, 127 - lo - 8))
+        x = (mantissas * 2.0 ** power).to(dtype)
+        part = slice(lo, min(lo + 16, 255))
+        y = ops().w4a16_matmul(x.cuda(), packed[part].cuda(), e[part, None].to(torch.uint8).cuda(), out_dtype=F32).cpu()
+        want = x.double() @ values[part].T
+        # 33 roundings at most, and half a step of subnormal numbers at each
+        tol = 33 * (2.0 ** -24 * (x.double().abs() @ values[part].abs().T) + 2.0 ** -150)
+        over = (E2M1[codes[part]].abs().double() * torch.exp2(e[part].double() - 127)[:, None] >= 2.0 ** 128).any(1)
+        if dtype == BF16 and over.any():
+            assert e[part][over].tolist() == [253, 254] and not torch.isfinite(y[:, over]).any()
+            y, want, tol = y[:, ~over], want[:, ~over], tol[:, ~over]
+        fits = (want.abs() + tol < 3.4e38)
+        bad = ((y.double() - want).abs() > tol) & fits
+        assert not bad.any(), (lo, e[part][bad.any(0)[:16].nonzero().view(-1)].tolist()
+                               if bad.shape[1] == 16 else int(bad.sum()))
