@@ -189,6 +189,9 @@ class W4A16Experts(torch.nn.Module):
         """hidden_states [tokens, hidden] (bf16 or fp16), top_k_index and
         top_k_weights [tokens, top]; ids outside [0, num_experts) take no
         part."""
+        if hidden_states.dim() != 2 or top_k_index.dim() != 2 or top_k_index.shape[0] != hidden_states.shape[0]:
+            raise ValueError(f"hidden_states [tokens, hidden] take ids of the same tokens, got "
+                             f"{tuple(hidden_states.shape)} and {tuple(top_k_index.shape)}")
         _no_derivatives(hidden_states, top_k_weights)
         plan = moe.plan_tokens(top_k_index, self.num_experts)
         h = ops.w4a16_experts_matmul(hidden_states, plan.rows, plan.offsets, *self.gate_up.parts(), gated=True)
