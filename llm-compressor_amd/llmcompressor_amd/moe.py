@@ -60,7 +60,7 @@ def route_tokens(top_k_index: torch.Tensor, num_experts: int, num_tokens: int | 
         rows = torch.arange(nt, device=dev, dtype=torch.int32).repeat(num_experts)
         offsets = [e * nt for e in range(num_experts + 1)]
         return rows, offsets, None
-    if top_k_index.is_cuda and tokens and 0 < num_experts <= ops.MOE_MAX_EXPERTS and \
+    if top_k_index.is_cuda and 0 < tokens * k < 2 ** 31 and 0 < num_experts <= ops.MOE_MAX_EXPERTS and \
             top_k_index.dtype in (torch.int32, torch.int64):
         sorted_tok, slots, ends = ops.moe_plan(top_k_index, num_experts)
         offsets = ends.tolist()
