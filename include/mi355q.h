@@ -666,8 +666,9 @@ int mi355q_moe_combine_backward(const void* dy_dev, mi355q_dtype dtype, int64_t 
  * cols >= 8.  ldw and stride_w in bytes (multiples of 4), others in elements.
  * offsets_dev NULL: one weight for all rows; else expert e has rows
  * [offsets[e], offsets[e + 1]) of y and the weight at e times the strides (offsets ascend), and
- * rows before offsets[0] and from offsets[experts] on are written as zeros.  rows_dev: row of x behind each row of y
- * (NULL: the same row); one that x does not have counts as zeros.
+ * rows before offsets[0] and from offsets[experts] on are written as zeros.  rows_dev: row
+ * of x behind each row of y (NULL: the same row); where x does not have it (n_x may be
+ * 0), the row of y is zeros, without the bias.
  * A row of x that holds an infinity or a NaN may come out as NaN throughout.
  * workspace (16-byte aligned): the queried size; with less, sums are not split over
  * workgroups and calls of many rows take a kernel that is made for few. */

@@ -23,6 +23,16 @@ __global__ __launch_bounds__(256) void w4_join_kernel(W4Args g, uint32_t splits,
   else static_cast<uint16_t*>(g.y)[at] = g.y_type == MI355Q_BF16 ? Bf16::store(v) : F16::store(v);
 }
 
+// y of an x without rows: zeros.
+__global__ __launch_bounds__(256) void w4_zero_kernel(W4Args g) {
+  const int64_t width = g.gated ? g.out / 2 : g.out, n = g.n_rows * width;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    const int64_t at = i / width * g.ldy + i % width;
+    if (g.y_type == MI355Q_F32) static_cast<float*>(g.y)[at] = 0.f;
+    else static_cast<uint16_t*>(g.y)[at] = 0;
+  }
+}
+
 int join_parts(const W4Args& g, uint32_t splits, const float* parts, hipStream_t st) {
   const int64_t width = g.gated ? g.out / 2 : g.out;
   hipLaunchKernelGGL(w4_join_kernel, dim3((unsigned)((g.n_rows * width + 255) / 256)), dim3(256), 0, st, g, splits,
@@ -126,7 +136,7 @@ extern "C" int mi355q_w4a16_matmul(const void* x_dev, mi355q_dtype x_dtype, int6
   if (group_size > cols) group_size = cols;
   MQ_CHECK_ARG(ldx >= 0, "w4a16_matmul: x has a pitch of %lld", (long long)ldx);
   if (rows == 0) return MI355Q_OK;
-  MQ_CHECK_ARG(x_dev && w_dev && scales_dev && y_dev, "w4a16_matmul: a null operand");
+  MQ_CHECK_ARG((x_dev || n_x == 0) && w_dev && scales_dev && y_dev, "w4a16_matmul: a null operand");
   const int64_t row_bytes = mx ? cols / 2 : (cols + 7) / 8 * 4;
   MQ_CHECK_ARG(ldw >= row_bytes && ldw % 4 == 0 && stride_w % 4 == 0 && aligned_to(w_dev, 4),
                "w4a16_matmul: the weight's rows must not overlap and lie on 4-byte boundaries");
@@ -139,6 +149,12 @@ extern "C" int mi355q_w4a16_matmul(const void* x_dev, mi355q_dtype x_dtype, int6
               fast_div((uint32_t)((group_size + kStep - 1) / kStep)), gated != 0};
   const int kind = mx ? kMxfp4 : zeros_dev ? kInt4Zero : kInt4;
   hipStream_t st = static_cast<hipStream_t>(stream);
+  if (n_x == 0) {                  // (the kernels read row 0 of x in the place of rows that are not there)
+    const int64_t blocks = (rows * (gated ? out / 2 : out) + 255) / 256;
+    hipLaunchKernelGGL(w4_zero_kernel, dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, st, g);
+    MQ_LAUNCH_CHECK();
+    return MI355Q_OK;
+  }
   if (!few_rows(rows, experts, group_size, mx) && w4_tiles_fit(g, kind) && workspace_dev && aligned16(workspace_dev) &&
       workspace_bytes >= w4_tiles_workspace(n_x, rows, experts, experts * out, cols, g.groups, mx))
     return launch_w4_tiles(g, x_dtype, kind, workspace_dev, st);

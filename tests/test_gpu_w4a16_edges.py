@@ -76,6 +76,24 @@ def test_rows_before_the_first_expert_are_zeros(rows, experts, gated):
         assert not y[:first].any() and not y[last:].any(), n
 
 
+@pytest.mark.parametrize("rows", [1, 20, 700])
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("out_dtype", [BF16, F32])
+def test_x_without_rows(rows, gated, out_dtype):
+    """No row of x is there: every row of y is zeros, whatever the index says, and x is not read."""
+    from llmcompressor_amd import _lib as L
+    w = Weight(gen("none"), 40, 128, "int4", 128, experts=3)
+    x = torch.empty(0, 128, dtype=BF16, device="cuda")
+    index = torch.arange(rows, dtype=torch.int32, device="cuda")
+    offsets = torch.tensor([0, rows // 2, rows // 2, rows], device="cuda")
+    y = ops().w4a16_experts_matmul(x, index, offsets, *w.cuda(), gated=gated, out_dtype=out_dtype)
+    assert y.shape == (rows, 20 if gated else 40) and not y.any()
+    wide = torch.full((rows, 50), float("nan"), dtype=out_dtype, device="cuda")      # a pitch, and a bias
+    b = torch.ones(40, dtype=BF16, device="cuda")
+    entry(x, w.cuda(), L.W4_INT4, offsets, 3, 128, 40, gated, wide[:, :y.shape[1]], b, index)
+    assert not wide[:, :y.shape[1]].any() and bool(wide[:, y.shape[1]:].isnan().all())
+
+
 # ---------------------------------------------------------------- the ends of the range
 def one_gate(dtype, gate, rows):
     """(x, packed, scales): MXFP4, of 32 columns of gate and 32 of up, whose gates are `gate` in every row and whose
