@@ -558,18 +558,28 @@ int mi355q_moe_combine_backward(const void* dy_dev, mi355q_dtype dtype, int64_t 
   if (!dx_dev && !dw_dev) return MI355Q_OK;
   const bool past = dx_dev && tokens * top * cols * dtype_size(dtype) > kCached;
   const bool wide = cols * dtype_size(dtype) > 64 * 16;
-  with_dtype(dtype, [&](auto type) {
-    using T = decltype(type);
-    const dim3 grid((unsigned)(wide ? tokens : (tokens + 3) / 4)), block(256);
-    hipStream_t st = static_cast<hipStream_t>(stream);
-    by_top(top, [&](auto k) {
-      constexpr int K = decltype(k)::value;
-      if (wide && past) hipLaunchKernelGGL((moe_combine_backward_kernel<T, K, 4, true>), grid, block, 0, st, g);
-      else if (wide) hipLaunchKernelGGL((moe_combine_backward_kernel<T, K, 4, false>), grid, block, 0, st, g);
-      else hipLaunchKernelGGL((moe_combine_backward_kernel<T, K, 1, false>), grid, block, 0, st, g);
+  // a launch has fewer than 2^32 threads: 2^22 tokens, a workgroup of 256 each where rows are wide
+  constexpr int64_t step = 1 << 22;
+  for (int64_t t = 0; t < tokens; t += step) {
+    RowsArgs part = g;
+    part.tokens = (uint32_t)(tokens - t < step ? tokens - t : step);
+    part.dy = static_cast<const char*>(dy_dev) + t * lddy * dtype_size(dtype);
+    part.w = static_cast<const char*>(weights_dev) + t * top * dtype_size(weights_dtype);
+    part.slots = slots_dev + t * top;
+    if (dw_dev) part.dw = static_cast<char*>(dw_dev) + t * top * dtype_size(weights_dtype);
+    const dim3 grid(wide ? part.tokens : (part.tokens + 3) / 4), block(256);
+    with_dtype(dtype, [&](auto type) {
+      using T = decltype(type);
+      hipStream_t st = static_cast<hipStream_t>(stream);
+      by_top(top, [&](auto k) {
+        constexpr int K = decltype(k)::value;
+        if (wide && past) hipLaunchKernelGGL((moe_combine_backward_kernel<T, K, 4, true>), grid, block, 0, st, part);
+        else if (wide) hipLaunchKernelGGL((moe_combine_backward_kernel<T, K, 4, false>), grid, block, 0, st, part);
+        else hipLaunchKernelGGL((moe_combine_backward_kernel<T, K, 1, false>), grid, block, 0, st, part);
+      });
     });
-  });
-  MQ_LAUNCH_CHECK();
+    MQ_LAUNCH_CHECK();
+  }
   return MI355Q_OK;
 }
 
