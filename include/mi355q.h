@@ -671,9 +671,13 @@ int mi355q_moe_combine_backward(const void* dy_dev, mi355q_dtype dtype, int64_t 
  * 0), the row of y is zeros, without the bias.
  * A row of x that holds an infinity or a NaN may come out as NaN throughout.
  * workspace (16-byte aligned): the queried size; with less, sums are not split over
- * workgroups and calls of many rows take a kernel that is made for few. */
+ * workgroups and calls of many rows take a kernel that is made for few.  The size has
+ * room for a copy of x; size_in_place is without, for an x that lies on 16 bytes with
+ * rows of a multiple of 8 elements (ldx), which is read where it is. */
 size_t mi355q_w4a16_matmul_workspace_size(int64_t n_x, int64_t rows, int64_t experts, int64_t out, int64_t cols,
                                           mi355q_w4_format format, int64_t group_size);
+size_t mi355q_w4a16_matmul_workspace_size_in_place(int64_t n_x, int64_t rows, int64_t experts, int64_t out,
+                                                   int64_t cols, mi355q_w4_format format, int64_t group_size);
 int mi355q_w4a16_matmul(const void* x_dev, mi355q_dtype x_dtype, int64_t n_x, int64_t ldx, const int32_t* rows_dev,
                         const int64_t* offsets_dev, int64_t experts, const void* w_dev, mi355q_w4_format format,
                         int64_t ldw, int64_t stride_w, const void* scales_dev, mi355q_dtype scales_dtype,

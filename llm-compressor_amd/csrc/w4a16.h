@@ -174,11 +174,12 @@ int launch_w4_few_zero_f16(const W4Args& g, const FewPlan& p, float* parts, hipS
 // y from the parts of the sums
 int join_parts(const W4Args& g, uint32_t splits, const float* parts, hipStream_t st);
 
-// The tile kernels (w4a16_tiles.hip): whether they take a call, the workspace that they
-// ask for, and the launch.
+// The tile kernels (w4a16_tiles.hip): whether they take a call, whether they read x where
+// it is, the workspace that they ask for, and the launch.
 bool w4_tiles_fit(const W4Args& g, int kind);
+inline bool in_place(const W4Args& g) { return aligned16(g.x) && g.ldx % 8 == 0 && g.cols % 8 == 0; }
 size_t w4_tiles_workspace(int64_t n_x, int64_t rows, int64_t experts, int64_t rows_w, int64_t cols, uint32_t groups,
-                          bool mx);
+                          bool mx, bool x_copy);
 int launch_w4_tiles(const W4Args& g, mi355q_dtype x_dtype, int kind, void* workspace, hipStream_t st);
 int launch_w4_tiles_bf16(const W4Args& g, int kind, void* workspace, hipStream_t st);
 int launch_w4_tiles_f16(const W4Args& g, int kind, void* workspace, hipStream_t st);

@@ -94,14 +94,25 @@ static size_t few_bytes(int64_t rows, int64_t experts, int64_t out, int64_t cols
   return splits > 1 ? (size_t)splits * rows * out * sizeof(float) : 0;
 }
 
-extern "C" size_t mi355q_w4a16_matmul_workspace_size(int64_t n_x, int64_t rows, int64_t experts, int64_t out,
-                                                     int64_t cols, mi355q_w4_format format, int64_t group_size) {
+static size_t workspace_size(int64_t n_x, int64_t rows, int64_t experts, int64_t out, int64_t cols,
+                             mi355q_w4_format format, int64_t group_size, bool x_copy) {
   if (n_x <= 0 || rows <= 0 || experts <= 0 || out <= 0 || cols <= 0 || group_size <= 0) return 0;
   const bool mx = format == MI355Q_W4_MXFP4;
   if (group_size > cols) group_size = cols;
   if (few_rows(rows, experts, group_size, mx)) return few_bytes(rows, experts, out, cols);
   return w4_tiles_workspace(n_x, rows, experts, experts * out, cols,
-                            (uint32_t)((cols + group_size - 1) / group_size), mx);
+                            (uint32_t)((cols + group_size - 1) / group_size), mx, x_copy);
+}
+
+extern "C" size_t mi355q_w4a16_matmul_workspace_size(int64_t n_x, int64_t rows, int64_t experts, int64_t out,
+                                                     int64_t cols, mi355q_w4_format format, int64_t group_size) {
+  return workspace_size(n_x, rows, experts, out, cols, format, group_size, true);
+}
+
+extern "C" size_t mi355q_w4a16_matmul_workspace_size_in_place(int64_t n_x, int64_t rows, int64_t experts, int64_t out,
+                                                              int64_t cols, mi355q_w4_format format,
+                                                              int64_t group_size) {
+  return workspace_size(n_x, rows, experts, out, cols, format, group_size, cols % 8 != 0);
 }
 
 extern "C" int mi355q_w4a16_matmul(const void* x_dev, mi355q_dtype x_dtype, int64_t n_x, int64_t ldx,
@@ -156,7 +167,7 @@ extern "C" int mi355q_w4a16_matmul(const void* x_dev, mi355q_dtype x_dtype, int6
     return MI355Q_OK;
   }
   if (!few_rows(rows, experts, group_size, mx) && w4_tiles_fit(g, kind) && workspace_dev && aligned16(workspace_dev) &&
-      workspace_bytes >= w4_tiles_workspace(n_x, rows, experts, experts * out, cols, g.groups, mx))
+      workspace_bytes >= w4_tiles_workspace(n_x, rows, experts, experts * out, cols, g.groups, mx, !in_place(g)))
     return launch_w4_tiles(g, x_dtype, kind, workspace_dev, st);
   FewPlan p = few_plan(rows, experts, out, cols, gated);
   // (rows behind the last expert's and rows that x does not have become zeros where the sum is whole)

@@ -659,7 +659,6 @@ struct TilePlan {
 TilePlan tile_plan(int64_t rows, int64_t experts, int64_t out, int64_t cols, bool gated, bool listed);
 
 inline bool w_in_place(const W4Args& g) { return aligned16(g.w) && g.ldw % 16 == 0 && g.stride_w % 16 == 0; }
-inline bool in_place(const W4Args& g) { return aligned16(g.x) && g.ldx % 8 == 0 && g.cols % 8 == 0; }
 inline size_t sums_bytes(int64_t n_x, uint32_t groups) {
   return ((size_t)n_x * 3 * ((groups + 15) / 16 * 16) * sizeof(uint16_t) + 255) / 256 * 256;
 }

@@ -38,12 +38,12 @@ TilePlan tile_plan(int64_t rows, int64_t experts, int64_t out, int64_t cols, boo
 }
 
 size_t w4_tiles_workspace(int64_t n_x, int64_t rows, int64_t experts, int64_t rows_w, int64_t cols, uint32_t groups,
-                          bool mx) {
+                          bool mx, bool x_copy) {
   // operands that the DMA cannot read (rows off 16 bytes or not of whole chunks) are copied
   const int64_t w_bytes = mx ? cols / 2 : (cols + 7) / 8 * 4;
   return (mx ? 0 : sums_bytes(n_x, groups) + sums_bytes(rows_w, groups)) + scales_bytes(rows_w, groups) +
          parts_bytes(tile_plan(rows, experts, rows_w / experts, cols, false, false), rows, rows_w / experts) +
-         x_copy_bytes(n_x, cols) + (w_bytes % 16 ? (size_t)rows_w * ((w_bytes + 15) / 16 * 16) : 0);
+         (x_copy ? x_copy_bytes(n_x, cols) : 0) + (w_bytes % 16 ? (size_t)rows_w * ((w_bytes + 15) / 16 * 16) : 0);
 }
 
 int launch_w4_tiles(const W4Args& g, mi355q_dtype x_dtype, int kind, void* workspace, hipStream_t st) {

@@ -111,6 +111,7 @@ SIGNATURES = {
                                    _vp, _i64, _i64, _i64, _vp, _i32, _i32, _vp, _i32, _i64, _i64, _i64, _i64, _vp, _sz,
                                    _vp]),
     "mi355q_w4a16_matmul_workspace_size": (_sz, [_i64, _i64, _i64, _i64, _i64, _i32, _i64]),
+    "mi355q_w4a16_matmul_workspace_size_in_place": (_sz, [_i64, _i64, _i64, _i64, _i64, _i32, _i64]),
 }
 
 _lock = threading.Lock()

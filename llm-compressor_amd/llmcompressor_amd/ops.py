@@ -1086,8 +1086,10 @@ def _w4_operand(t: torch.Tensor, shape, dtypes, what: str, lead: int):
 
 
 @functools.lru_cache(maxsize=4096)
-def _w4_workspace(n_x: int, rows: int, experts: int, out: int, cols: int, fmt: int, group: int) -> int:
-    return L.lib().mi355q_w4a16_matmul_workspace_size(n_x, rows, experts, out, cols, fmt, group)
+def _w4_workspace(in_place: bool, n_x: int, rows: int, experts: int, out: int, cols: int, fmt: int, group: int) -> int:
+    lib = L.lib()
+    query = lib.mi355q_w4a16_matmul_workspace_size_in_place if in_place else lib.mi355q_w4a16_matmul_workspace_size
+    return query(n_x, rows, experts, out, cols, fmt, group)
 
 
 def _w4_matmul(x, index, offsets, experts, n_rows, weight_packed, weight_scale, weight_zero_point, group_size, bias,
@@ -1166,7 +1168,8 @@ def _w4_matmul(x, index, offsets, experts, n_rows, weight_packed, weight_scale, 
     width = out // 2 if gated else out
     y = x.new_empty((n_rows, width), dtype=out_dtype)
     fmt = L.W4_MXFP4 if mx else L.W4_INT4
-    ws_bytes = _w4_workspace(n_x, n_rows, experts or 1, out, cols, fmt, group)
+    in_place = pitch % 8 == 0 and x.data_ptr() % 16 == 0
+    ws_bytes = _w4_workspace(in_place, n_x, n_rows, experts or 1, out, cols, fmt, group)
     ws = x.new_empty(ws_bytes, dtype=torch.uint8) if ws_bytes else None
     ws_ptr = None if ws is None else ws.data_ptr()
     rc = L.lib().mi355q_w4a16_matmul(

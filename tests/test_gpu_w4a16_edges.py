@@ -94,6 +94,47 @@ def test_x_without_rows(rows, gated, out_dtype):
     assert not wide[:, :y.shape[1]].any() and bool(wide[:, y.shape[1]:].isnan().all())
 
 
+# ---------------------------------------------------------------- workspaces
+@pytest.mark.parametrize("cols,kind", [(512, "int4"), (520, "int4z"), (544, "mxfp4")])
+@pytest.mark.parametrize("rows", [130, 700])
+def test_workspace_without_a_copy_of_x(rows, cols, kind):
+    """Aligned operands: the smaller size is enough, nothing is written behind it, and the result is that of the larger."""
+    from llmcompressor_amd import _lib as L
+    g = gen("in place", rows, cols)
+    x = torch.randn(rows, cols, generator=g).to(BF16)
+    w = Weight(g, 300, cols, kind, 32)
+    fmt = L.W4_MXFP4 if kind == "mxfp4" else L.W4_INT4
+    need = L.lib().mi355q_w4a16_matmul_workspace_size_in_place(rows, rows, 1, 300, cols, fmt, 32)
+    xc, (p, s, z) = x.cuda(), w.cuda()
+
+    def run(size, ws):
+        y = torch.empty(rows, 300, dtype=BF16, device="cuda")
+        L.check(L.lib().mi355q_w4a16_matmul(
+            xc.data_ptr(), L.BF16, rows, cols, None, None, 1, p.data_ptr(), fmt, p.stride(0) * p.element_size(), 0,
+            s.data_ptr(), L.BF16, s.stride(0), 0, L.ptr(z), 0 if z is None else z.stride(0), 0, 32, None, 0, 0, y.data_ptr(),
+            L.BF16, 300, rows, 300, cols, ws.data_ptr(), C.c_size_t(size), L.stream_of(xc)))
+        return y
+
+    ws = torch.full((need + 4096,), 77, dtype=torch.uint8, device="cuda")
+    y = run(need, ws)
+    close(y, *expected(x, w.values, w.sizes))
+    assert bool((ws[need:] == 77).all()) and not bool((ws[:need] == 77).all())
+    full = L.lib().mi355q_w4a16_matmul_workspace_size(rows, rows, 1, 300, cols, fmt, 32)
+    assert torch.equal(y, run(full, torch.empty(full, dtype=torch.uint8, device="cuda")))
+
+
+def test_ordinary_calls_do_not_take_the_memory_of_a_copy_of_x():
+    g = gen("memory")
+    x = torch.randn(20000, 4096, device="cuda").to(BF16)
+    parts = Weight(g, 64, 4096, "int4", 128).cuda()
+    ops().w4a16_matmul(x, *parts)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    ops().w4a16_matmul(x, *parts)
+    assert torch.cuda.max_memory_allocated() - before < x.numel()      # half of x's bytes
+
+
 # ---------------------------------------------------------------- the ends of the range
 def one_gate(dtype, gate, rows):
     """(x, packed, scales): MXFP4, of 32 columns of gate and 32 of up, whose gates are `gate` in every row and whose

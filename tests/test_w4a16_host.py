@@ -88,3 +88,15 @@ def test_host_tensors_are_refused():
     with pytest.raises(RuntimeError, match="GPU only"):
         ops.w4a16_matmul(torch.zeros(2, 64, dtype=torch.bfloat16), torch.zeros(4, 8, dtype=torch.int32),
                          torch.zeros(4, 1, dtype=torch.bfloat16))
+
+
+@pytest.mark.parametrize("cols,fmt,group", [(1024, _lib.W4_INT4, 128), (1032, _lib.W4_INT4, 32), (1024, _lib.W4_MXFP4, 32),
+                                            (1023, _lib.W4_INT4, 128)])
+def test_workspace_without_a_copy_of_x(cols, fmt, group):
+    """Less by x with rows of whole steps of 128 columns; rows of an odd number of columns are copied all the same."""
+    lib = _lib.load_library()
+    for n_x, rows, experts in ((256, 256, 1), (1000, 4000, 4)):
+        args = n_x, rows, experts, 512, cols, fmt, group
+        copy = n_x * -(-cols // 128) * 128 * 2 if cols % 8 == 0 else 0
+        assert lib.mi355q_w4a16_matmul_workspace_size(*args) - lib.mi355q_w4a16_matmul_workspace_size_in_place(*args) == copy
+    assert lib.mi355q_w4a16_matmul_workspace_size_in_place(1, 1, 1, 4096, 4096, _lib.W4_INT4, 128) == 0
