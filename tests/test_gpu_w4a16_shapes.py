@@ -173,3 +173,39 @@ def test_cuts_of_few_rows_of_experts(pairs, experts, out, steps, gated, kind, gr
                                                     ("mxfp4", 32, BF16, False), ("mxfp4", 32, F16, True)])
 def test_bands_of_experts_tiles(pairs, experts, out, kind, group, dtype, gated):
     check_experts(pairs, experts, out, 288, kind, group, dtype, BF16, gated, not gated)
+
+
+# Tiles of many rows: rows, out, gated; the tile's rows and columns
+TILES = [
+    (200, 1000, False),     # 32 x 128
+    (200, 1000, True),      # 32 x 256
+    (700, 3000, False),     # 64 x 128
+    (1290, 5100, False),    # 64 x 256
+    (1290, 5100, True),
+    (2050, 6700, False),    # 128 x 256
+    (2050, 6700, True),
+]
+
+
+@pytest.mark.parametrize("rows,out,gated", TILES)
+@pytest.mark.parametrize("kind,group,dtype,scale_dtype", FORMATS + [("int4", 64, BF16, F32), ("int4z", 32, F16, F16)],
+                         ids=NAMES + ["int4-64-bf16-f32", "int4z-32-f16-f16"])
+def test_tiles_of_several_steps(rows, out, gated, kind, group, dtype, scale_dtype):
+    """Five whole steps and a shorter one: eight instructions a step, of eight roundings, stay below the bound."""
+    cols = 640 + (32 if kind == "mxfp4" else 41)
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    x = (torch.randn(rows, cols, generator=g, device="cuda")
+         * torch.randn(cols, generator=g, device="cuda").exp()).to(dtype)
+    w = Weight(out + rows, (), out, cols, kind, group, scale_dtype)
+    b = torch.randn(out, generator=g, device="cuda").to(dtype)
+    y = ops().w4a16_matmul(x, *w.parts, group_size=group, bias=b, gated=gated, out_dtype=F32)
+    close(y, x, *w.exact(), b, gated)
+
+
+@pytest.mark.parametrize("pairs,experts,out", [(180, 4, 400), (420, 5, 600), (1500, 7, 600), (3300, 5, 600)],
+                         ids=["32x128", "32x256", "64x256", "128x256"])
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("kind,group,dtype,scale_dtype", FORMATS, ids=NAMES)
+def test_tiles_of_experts_of_several_steps(pairs, experts, out, gated, kind, group, dtype, scale_dtype):
+    check_experts(pairs, experts, out, 640 + (32 if kind == "mxfp4" else 41), kind, group, dtype, scale_dtype, gated,
+                  not gated)
