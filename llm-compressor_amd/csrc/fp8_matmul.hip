@@ -180,14 +180,15 @@ __device__ __forceinline__ uint32_t lds_u32(const void* p) {
   return (uint32_t) reinterpret_cast<uintptr_t>((lds_void_t*)p);
 }
 // 64 lanes x 16 bytes to LDS at m0, from a scalar base and lane offsets.
-// Completion is waited for explicitly (vmcnt).
+// Completion is waited for explicitly (vmcnt).  The load reads m0 one state after
+// it is written, at the earliest.
 __device__ __forceinline__ void dma_s(uint32_t off, const void* base, uint32_t m0) {
-  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(m0) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(m0) : "memory", "m0");
 }
 
 // 64 lanes x 1 byte, each as a dword
 __device__ __forceinline__ void dma_bytes(uint32_t off, const void* base, uint32_t m0) {
-  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_ubyte %0, %1" ::"v"(off), "s"(base), "s"(m0) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_ubyte %0, %1" ::"v"(off), "s"(base), "s"(m0) : "memory", "m0");
 }
 
 typedef int i32x2_t __attribute__((ext_vector_type(2)));

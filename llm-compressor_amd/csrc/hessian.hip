@@ -517,12 +517,13 @@ __device__ __forceinline__ void stream_item(const SyrkParams& p, char* ring, int
                           lds_u32(a3) + wave_lds};
   const uint32_t sb[4] = {lds_u32(b0) + wave_lds, lds_u32(b1) + wave_lds, lds_u32(b2) + wave_lds,
                           lds_u32(b3) + wave_lds};
+  // (the loads read m0 one state after it is written, at the earliest)
   auto dma_s = [&](uint32_t off, const char* base, uint32_t m0) __attribute__((always_inline)) {
-    asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(m0)
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(m0)
                  : "memory", "m0");
   };
   auto dma_v = [&](const void* gaddr, uint32_t m0) __attribute__((always_inline)) {
-    asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(gaddr), "s"(m0) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(gaddr), "s"(m0) : "memory", "m0");
   };
   const char* xbase = reinterpret_cast<const char*>(p.x + (mat.row_begin + st_begin * SK) * p.ldx);
   const int64_t sbytes = (int64_t)SK * p.ldx * 2;  // bytes per stage

@@ -590,8 +590,9 @@ constexpr int LKK = 32;          // K per stage
 typedef __attribute__((address_space(3))) void lds_void_t;
 __device__ __attribute__((aligned(16))) const float kZeroF4[4] = {0.f, 0.f, 0.f, 0.f};
 
+// (the load reads m0 one state after it is written, at the earliest)
 __device__ __forceinline__ void dma16(const void* gaddr, uint32_t lds_addr) {
-  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(gaddr), "s"(lds_addr) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(gaddr), "s"(lds_addr) : "memory", "m0");
 }
 
 template <int TM, int TN, int WGM, int WGN, bool BT, int NS>

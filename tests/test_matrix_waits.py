@@ -1,4 +1,5 @@
-"""The built library's code: no instruction touches a matrix instruction's result before it is there.
+"""The built library's code: no instruction touches a matrix instruction's result before it is there, and no load to
+LDS reads m0 before it is written.
 
 The processor does not wait by itself between a matrix instruction and a vector, memory or LDS instruction that
 touches the registers it writes; the compiler leaves room for it.  This walks every path behind every matrix
@@ -8,6 +9,10 @@ place that is too near reads what was in the registers before, now and then.
 Wait states after an instruction of n passes (gfx950): n + 4 until its result may be read or written, n + 2 for
 those that multiply fp32, n - 1 until registers that it only adds from may be overwritten.  (In the code between two
 branches the compiler keeps to these numbers everywhere.)
+
+A load from memory to LDS takes its place there from m0, one state after a scalar instruction wrote it at the
+earliest; and its address from scalar registers, five states after a vector instruction wrote them.  In assembly
+written by hand the compiler sees to neither.
 """
 import re
 import shutil
@@ -125,6 +130,47 @@ def too_near(code, at):
     return found
 
 
+SCALARS = re.compile(r"\bs(?:(\d+)\b|\[(\d+):(\d+)\])")
+
+
+def scalars(text: str) -> set:
+    return {i for one, first, last in SCALARS.findall(text)
+            for i in (range(int(one), int(one) + 1) if one else range(int(first), int(last) + 1))}
+
+
+def early_loads(listing):
+    """(function, what wrote m0 or a scalar of the address too near before, the load to LDS)"""
+    name, before = None, []
+    for line in listing:
+        head = re.match(r"^[0-9a-f]+ <(.*)>:", line)
+        if head:
+            name, before = head[1], []
+            continue
+        op, _, operands = line.partition("//")[0].strip().partition(" ")
+        if not op:
+            continue
+        if "load_lds" in op:
+            states, address = 0, scalars(operands)
+            for last, written, took in reversed(before):
+                if states < 1 and last.startswith("s_") and written.strip() == "m0":
+                    yield name, f"{last} {written}", op
+                if states < 5 and last.startswith("v_") and scalars(written) & address:
+                    yield name, f"{last} {written}", op
+                states += took
+        before = [*before[-5:], (op, operands.split(",")[0], int(operands, 0) + 1 if op == "s_nop" else 1)]
+
+
+def test_early_loads_are_found():
+    wait = "\ts_nop 0  // 1: 0"
+    load = "\tglobal_load_lds_dwordx4 v1, s[4:5]  // 1: 0"
+    head = "0000000000001000 <kernel>:"
+    m0, base = "\ts_mov_b32 m0, s7  // 1: 0", "\tv_readfirstlane_b32 s5, v3  // 1: 0"
+    assert [f[1] for f in early_loads([head, m0, load])] == ["s_mov_b32 m0"]
+    assert not list(early_loads([head, m0, wait, load]))
+    assert [f[1] for f in early_loads([head, base, m0, wait, wait, wait, load])] == ["v_readfirstlane_b32 s5"]
+    assert not list(early_loads([head, base, m0, *[wait] * 4, load]))
+
+
 def test_walk_finds_what_a_branch_hides():
     """Results read three states behind their instruction on one of two paths, eight on the other."""
     def listing(pad):
@@ -147,19 +193,21 @@ def test_walk_finds_what_a_branch_hides():
 
 
 @pytest.mark.skipif(OBJDUMP is None or not _lib.LIB_PATH.exists(), reason="needs llvm-objdump and the built library")
-def test_results_of_matrix_instructions_are_waited_for(tmp_path):
+def test_built_code_waits(tmp_path):
     objects = list(code_objects(_lib.LIB_PATH.read_bytes()))
     assert objects
-    seen, near = 0, []
+    seen, near, early = 0, [], []
     for n, o in enumerate(objects):
         path = tmp_path / f"{n}.co"
         path.write_bytes(o)
-        with subprocess.Popen([OBJDUMP, "-d", "--mcpu=gfx950", str(path)], stdout=subprocess.PIPE, text=True) as p:
-            for name, code, at in functions(p.stdout):
-                seen += 1
-                found = too_near(code, at)
-                if found:
-                    near.append((name, len(found), [(code[m].op, code[i].op, s, need) for m, i, s, need in found[:3]]))
-        assert p.returncode == 0
+        listing = subprocess.run([OBJDUMP, "-d", "--mcpu=gfx950", str(path)], stdout=subprocess.PIPE, text=True,
+                                 check=True).stdout.splitlines()
+        early += early_loads(listing)
+        for name, code, at in functions(listing):
+            seen += 1
+            found = too_near(code, at)
+            if found:
+                near.append((name, len(found), [(code[m].op, code[i].op, s, need) for m, i, s, need in found[:3]]))
     assert seen > 100
     assert not near, f"{len(near)} kernels touch results too early: {near[:5]}"
+    assert not early, f"{len(early)} loads to LDS come too early: {early[:5]}"
