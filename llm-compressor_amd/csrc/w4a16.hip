@@ -41,8 +41,9 @@ int join_parts(const W4Args& g, uint32_t splits, const float* parts, hipStream_t
   return MI355Q_OK;
 }
 
-// Up to this many rows the weight's bytes decide, and the kernel for few rows is the faster one.  One weight: 64 rows of
-// 4096 x 4096 20 us, in tiles 23 (14336 x 4096 30 and 27); 128 rows 23 and 24 (56 and 33).  The tiles have the scales
+// Up to this many rows the weight's bytes decide, and the kernel for few rows is the faster one.  One weight (twelve of
+// them in turn): 48 rows of 4096 x 4096 13.6 us, in tiles 14.9 (14336 x 4096 27 and 30, 4096 x 14336 28 and 28); 64 rows
+// 14.7 and 15.3 (30 and 29, 31 and 30); 96 rows 21 and 18 (51 and 32, 48 and 38).  The tiles have the scales
 // laid out first, which costs some 10 us and what the scales weigh: 128 experts of 1536 x 2048 in groups of 128, 2 rows
 // each 34 and 44 us, 3 rows 43 and 43, 4 rows 51 and 45; 8 experts of 8192 x 4096 6 rows each 40 and 48, 8 rows 50 and
 // 48.  The 128 experts in groups of 64: 8 rows 68 and 72, 10 rows 77 and 73; of 32: 12 rows 114 and 135, 16 rows 134 and
@@ -54,14 +55,15 @@ static bool few_rows(int64_t rows, int64_t experts, int64_t group, bool mx) {
 
 // Rows per tile (4 or 16 mt), columns, waves and splits of a call of few rows.
 //
-// A wave's loads are x's and the weight's, and it takes some 2048 waves to keep the memory busy.  Up
+// A wave's loads are x's and the weight's, and it takes many waves to keep the memory busy.  Up
 // to 4 rows (of experts: where a quarter of them have a row, as more rows of one would read its weight again: 128
 // experts of 1536 x 2048, 32 rows 20 us in both, 64 rows 29 in tiles of 4 and 20 in tiles of 16): one column tile a
-// wave, and as many waves on one tile's sum as make 2048 (14336 x
-// 4096 9.3 us with two, 10.4 with eight; 4096 x 4096 6.2 and 5.1; gated ones have two column tiles, 8 experts of
-// 1536 x 2048 7.8 us).  More rows: x is what is loaded most, so a wave takes up to four column tiles (16 x
-// 14336 x 4096 14.7 us, with two 16.9, with one 22.5), and where that leaves CUs idle the sum is split over
-// workgroups (23 x 4096 x 14336 34 us whole, 21 in four).  Tiles of experts are many: one or two waves each
+// wave, and fewer waves on one tile's sum the more tiles there are (one token with two, four and eight, twelve weights
+// in turn: 28672 x 4096, 1792 tiles, 17.8, 17.0 and 16.5 us; 14336 x 4096, 896, 10.0, 11.2 and 10.8; 4096 x 4096, 256,
+// 6.1, 5.3 and 4.9; 4096 x 14336 17.7, 11.7 and 10.3; so the choice is within 12 % of the best of the three.  Gated ones
+// have two column tiles, 8 experts of 1536 x 2048 7.8 us).  More rows: x is what is loaded most, so a wave takes up to four
+// column tiles (16 x 14336 x 4096 14.7 us, with two 16.9, with one 22.5), and where that leaves CUs idle the sum is split
+// over workgroups (23 x 4096 x 14336 34 us whole, 21 in four).  Tiles of experts are many: one or two waves each
 // (61 tokens to 8 of 128 experts of 1536 x 2048 54 us, with four waves 85).
 static FewPlan few_plan(int64_t rows, int64_t experts, int64_t out, int64_t cols, bool gated) {
   const int64_t mean = (rows + experts - 1) / experts, steps = (cols + kStep - 1) / kStep;

@@ -73,14 +73,19 @@ struct W4Batch {
 // What counts is loads, their number and how many are in flight: D steps of a wave are requested before
 // the first is used, the scales of all D in one load, the next ones as the registers come free, and
 // nothing in the loop over whole steps branches (a wait belongs to a branch, so one around a load
-// ends the overlap: one token's 14336 x 4096 took 13.2 us with branches on the scales' type and around dead rows).
+// ends the overlap: one token's 14336 x 4096 took 13.2 us with branches around dead rows).  A batch's scales are its
+// last request and the first thing that its use needs, so a wave waits for nearly the whole batch at its head, and
+// batches hardly overlap.
 // Rows past a tile's end read its first row, columns past w's end its last;
 // neither is stored.  GPS: scales per step, 0: one for several steps.
 //
-// One token, 14336 x 4096 in groups of 128: 9.3 us, 3.2 TB/s (reading the same 30 MB alone 6.0, a launch of nothing 1.8).
-// 23 rows, 4096 x 14336 MXFP4: 19.7 us with the join; the MFMAs are 6 % busy, and it is x's loads that count, which every
-// 64 columns read anew (two column tiles a wave 25 us; two steps in flight instead of one 21).  61 tokens to 8
-// of 128 experts, 1536 x 2048 in groups of 32 with zero points: 56 us, 4.1 TB/s.
+// One token, 14336 x 4096 in groups of 128: 10.4 us, 2.9 TB/s (9.0 to 9.3 with the same weight again and again, 11.2 with
+// twelve in turn; reading the same 30 MB alone 6.0, a launch of nothing 1.8).  23 rows, 4096 x 14336 MXFP4: 19.7 us
+// with the join; the MFMAs are 6 % busy: one step is in flight, and every 64 columns read x anew (two column
+// tiles a wave 25 us; two steps in flight instead of one 21).  61 tokens to 8 of 128 experts, 1536 x 2048 in groups of 32
+// with zero points: 56 us, 4.1 TB/s.  Tiles of 64 rows do not fit the registers for int4: 32 to 52 bytes a lane go to
+// scratch with 16-bit scales, up to 520 with zero points (48 rows of 4096 x 4096 in groups of 128 16.3 us, with zero
+// points in groups of 32 30).
 template <class T, int KIND, int GPS, class S, int MT, int NT, int W, int D>
 __global__ __launch_bounds__(64 * W) void w4_few_kernel(W4Args g, uint32_t nt, uint32_t splits, float* parts) {
   constexpr int ES = sizeof(typename S::raw);

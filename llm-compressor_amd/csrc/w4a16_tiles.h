@@ -18,9 +18,14 @@
 // of the sum's length where one piece holds a factor.  The same pass lays the scales out in fp32 by group, so that
 // a tile's 32 are neighbours, and costs 10 to 20 us.
 //
-// What bounds it (bf16, groups of 128): 8192 x 28672 x 4096, gated, takes 1.70 ms, 1.13 PFLOP/s, the MFMAs 56 % and the
-// vector unit 45 % busy at 1.9 GHz: power.  4096 tokens to 8 of 128 experts of 1536 x 2048 take 0.28 to 0.32 ms: the tiles
-// are 64 rows, so codes are converted twice as often (MFMAs 40 % busy), and an eighth of their rows is empty.
+// What bounds it (bf16, groups of 128): 8192 x 28672 x 4096, gated, takes 1.67 to 1.76 ms, 1.13 PFLOP/s, the MFMAs 56 %
+// and the vector unit 45 % busy at 1.9 GHz.  The two take turns more than they overlap: in the tiles of 128 rows most
+// operands of x are read right before their MFMAs, and nothing is multiplied while a tile's sums are scaled.  Those of
+// int4, and of MXFP4 with fp16, do not fit the registers either (7 of the 40 kernels, 40 to 108 bytes a lane in
+// scratch); in groups of 32 and for fp16 the loop reads offsets back between the requests of a step and waits for what
+// is under way: groups of 128, 64 and 32 take 1.75, 1.96 and 2.45 ms, MXFP4 1.55 with bf16 and 2.14 with fp16.  4096
+// tokens to 8 of 128 experts of 1536 x 2048 take 0.28 to 0.32 ms: the tiles are 64 rows, so codes are converted twice
+// as often (MFMAs 40 % busy), and an eighth of their rows is empty.
 #pragma once
 
 #include <type_traits>
@@ -538,7 +543,7 @@ void w4_tiles_kernel(W4Args g, W4Tiles o) {
             }
           }
         }
-        // two operand reads ahead of their MFMAs
+        // asks for two operand reads ahead of their MFMAs (the compiled loop waits for 18 of 32 right behind the read)
         __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
 #pragma unroll
         for (int j = 0; j < kSlices - 2; ++j) {
